@@ -230,6 +230,88 @@ int rnn_attn_backward_ex(rnn_ctx *ctx, const rnn_attn_desc *d, size_t n, const f
                          const float *kv, const float *tau, const float *p, const float *dout,
                          float *dq, float *dkv, float *dtau, float *drel, uint32_t flags);
 
+/* ------------------------------------------------------- rotary positions */
+/* Rotary positions with up to three axes (no counterpart in the reference,
+ * whose attention takes its positions from the relative bias): every row holds
+ * h heads of dh channels, and the R = p0 + p1 + p2 channel pairs of each head
+ * are turned by angles from the row's position.  Axis a owns p_a pairs (axis
+ * 0's first); its pair p turns by pos_a * base^(-p / p_a):
+ *   (u, v) -> (u cos - v sin, u sin + v cos).
+ * Pair j is channels (2j, 2j + 1) when interleaved, else (j, j + R); channels
+ * from 2R on are copied.  Angles are computed and reduced in 64 bits, so that
+ * far positions keep theirs, and rounded to 32 for the sine and cosine.
+ * Rows are read at x + r*xstride + xoff and written at y + r*ystride + yoff;
+ * only the h*dh channels of a row are written.  y may be x when strides and
+ * offsets agree (in place), else the two must not overlap. */
+typedef struct {
+    uint32_t h, dh;
+    size_t xstride, xoff, ystride, yoff;
+    uint32_t axes;       /* 1, 2 or 3 */
+    uint32_t p0, p1, p2; /* pairs of each axis (0 beyond axes) */
+    uint32_t g0, g1, g2; /* grid of an image's tokens, last axis fastest (1 beyond axes) */
+    int interleaved;
+    float base;
+} rnn_rotary_desc;
+/* Checks a description for n images of t tokens with (have_pos) or without
+ * explicit positions; host only.  RNN_OK or the code rnn_rotary returns. */
+int rnn_rotary_check(const rnn_rotary_desc *d, size_t n, size_t t, int have_pos);
+/* Turns the rows of n images of t tokens.  pos NULL: token i of an image sits
+ * at its grid coordinates (t = the product of the grid's axes); else pos
+ * [n*t][axes] holds every row's position, which may be fractional or negative.
+ * inverse: by the negated angles, which is the backward pass (x = dy, y = dx). */
+int rnn_rotary(rnn_ctx *ctx, const rnn_rotary_desc *d, size_t n, size_t t, const float *x,
+               const float *pos, float *y, int inverse);
+
+/* -------------------------------------------------- differential attention */
+/* Differential attention (no counterpart in the reference): the difference of
+ * two softmax maps, with a norm over each head's output.  Head j has two query
+ * maps of dh channels, at q + r*qstride + qoff + (2j + m)*dh (m = 0, 1); key
+ * head g = j / (h / hkv) has two key maps, at kv + r*kvstride + koff +
+ * (2g + m)*dh, and values of 2 dh channels at kv + r*kvstride + voff + 2g*dh.
+ *   P_m = softmax(scale Q_m K_m^T) over the keys that the query sees
+ *   lambda = exp(lq1 . lk1) - exp(lq2 . lk2) + lam_init
+ *   O = (P_1 - lambda P_2) V
+ *   y = (1 - lam_init) gain O / sqrt(mean(O^2) + eps)   (gain NULL: y = O)
+ * lam [lam_heads][4][dh] holds lq1, lk1, lq2, lk2, one set for all heads
+ * (lam_heads 1) or one for each (lam_heads h); gain [2 dh] serves every head.
+ * Image b has min(qlen[b], tq) queries and min(klen[b], tk) keys (device
+ * arrays; NULL: tq, tk): rows behind them are padding, which is never read and
+ * may hold anything.  causal: query i sees keys j <= i + (keys - queries), the
+ * two sequences aligned at their ends; mask_diag: not key j = i.  A query that
+ * sees no key, and a padding query, give y = 0.  The values that are read are
+ * finite. */
+typedef struct {
+    uint32_t h, hkv, dh, tq, tk;
+    size_t qstride, qoff, kvstride, koff, voff;
+    uint32_t lam_heads;
+    int mask_diag, causal;
+    float scale, lam_init, eps;
+} rnn_diff_attn_desc;
+/* Checks a description and gives the bytes of device workspace that the
+ * forward (backward = 0) or the backward needs for n images; host only.  The
+ * workspace is the caller's, 256-byte aligned, holds nothing between calls
+ * and is not shared by calls that may run at the same time.  dh <= 64
+ * (RNN_E_UNSUPPORTED above), scale > 0, 0 <= lam_init < 1. */
+int rnn_diff_attn_workspace(const rnn_diff_attn_desc *d, size_t n, int backward, size_t *bytes);
+/* y [n][tq][h][2 dh].  For a backward: o12 [n][tq][h][2][2 dh] receives each
+ * map's P_m V and stats [n][tq][h][4] each map's largest scaled score and the
+ * reciprocal of its softmax sum; both NULL: not kept. */
+int rnn_diff_attn_forward(rnn_ctx *ctx, const rnn_diff_attn_desc *d, size_t n, const float *q,
+                          const float *kv, const float *lam, const float *gain,
+                          const uint32_t *qlen, const uint32_t *klen, void *ws, size_t ws_bytes,
+                          float *y, float *o12, float *stats);
+/* From dy [n][tq][h][2 dh] and the forward's o12 and stats: dq and dkv, laid
+ * out as q and kv, ACCUMULATE or are overwritten as flags say
+ * (RNN_ATTN_SET_DQ, RNN_ATTN_SET_DKV: the columns of queries, or of keys and
+ * values, padding rows included, which receive 0); dlam [lam_heads][4][dh] and
+ * dgain [2 dh] (NULL with gain) accumulate.  dq and dkv may be one buffer with
+ * disjoint columns.  Sums run in a fixed order. */
+int rnn_diff_attn_backward(rnn_ctx *ctx, const rnn_diff_attn_desc *d, size_t n, const float *q,
+                           const float *kv, const float *lam, const float *gain,
+                           const uint32_t *qlen, const uint32_t *klen, const float *o12,
+                           const float *stats, const float *dy, void *ws, size_t ws_bytes,
+                           float *dq, float *dkv, float *dlam, float *dgain, uint32_t flags);
+
 /* ---------------------------------------------------------- linear.rs */
 /* Linear::forward (linear.rs:44-63): y[rows x fout] = x W^T + b (b may be NULL). */
 int rnn_linear_forward(rnn_ctx *ctx, size_t rows, size_t fin, size_t fout, const float *x,
@@ -254,6 +336,30 @@ int rnn_linear_backward(rnn_ctx *ctx, size_t rows, size_t fin, size_t fout, cons
 int rnn_linear_backward_ex(rnn_ctx *ctx, size_t rows, size_t fin, size_t fout, const float *dy,
                            const float *x, const float *w, float *dw, float *db, float *dx,
                            uint32_t flags);
+
+/* The Linear product with an activation and a residual (no counterpart in the
+ * reference, whose MLP is SwiGLU): z = x W^T + b, y = act(z) + res (b, res may
+ * be NULL; res [rows x fout], may be y).  z [rows x fout] is kept for the
+ * backward (NULL: not kept; not needed for RNN_ACT_NONE).  act: RNN_ACT_NONE
+ * z, RNN_ACT_RELU max(z, 0), RNN_ACT_GELU z (1 + erf(z / sqrt 2)) / 2,
+ * RNN_ACT_GELU_TANH z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2,
+ * RNN_ACT_SILU z / (1 + exp(-z)). */
+#define RNN_ACT_NONE 0u
+#define RNN_ACT_RELU 1u
+#define RNN_ACT_GELU 2u
+#define RNN_ACT_GELU_TANH 3u
+#define RNN_ACT_SILU 4u
+int rnn_linear_act_forward(rnn_ctx *ctx, size_t rows, size_t fin, size_t fout, const float *x,
+                           const float *w, const float *b, uint32_t act, const float *res,
+                           float *z, float *y);
+/* Its backward: dz = dy act'(z) (0 for RELU at z = 0), then as
+ * rnn_linear_backward_ex: dw += dz^T x, db += colsum(dz) (db may be NULL), dx =
+ * dz W (added with RNN_LINEAR_ACC_DX).  dz [rows x fout] is the caller's
+ * scratch, may be z and is not read for RNN_ACT_NONE (z and dz may then be
+ * NULL).  The residual's gradient is dy itself. */
+int rnn_linear_act_backward(rnn_ctx *ctx, size_t rows, size_t fin, size_t fout, const float *dy,
+                            const float *x, const float *w, const float *z, uint32_t act,
+                            float *dz, float *dw, float *db, float *dx, uint32_t flags);
 
 /* ------------------------------------------ host-slice forms (Rust shim) */
 /* The same entry points over HOST memory, for the Rust shim, whose callers

@@ -12,6 +12,11 @@ pub const RNN_E_UNSUPPORTED: c_int = -5;
 pub const RNN_ATTN_SET_DQ: u32 = 1;
 pub const RNN_ATTN_SET_DKV: u32 = 2;
 pub const RNN_LINEAR_ACC_DX: u32 = 1;
+pub const RNN_ACT_NONE: u32 = 0;
+pub const RNN_ACT_RELU: u32 = 1;
+pub const RNN_ACT_GELU: u32 = 2;
+pub const RNN_ACT_GELU_TANH: u32 = 3;
+pub const RNN_ACT_SILU: u32 = 4;
 pub const RNN_DW3_ACC_DX: u32 = 1;
 
 #[repr(C)] pub struct rnn_ctx { _p: [u8; 0] }
@@ -46,6 +51,45 @@ pub struct rnn_attn_desc {
     pub nrel: u32,
     pub relidx: *const u32,
     pub mask_diag: c_int,
+}
+
+#[repr(C)] #[derive(Clone, Copy)]
+pub struct rnn_rotary_desc {
+    pub h: u32,
+    pub dh: u32,
+    pub xstride: usize,
+    pub xoff: usize,
+    pub ystride: usize,
+    pub yoff: usize,
+    pub axes: u32,
+    pub p0: u32,
+    pub p1: u32,
+    pub p2: u32,
+    pub g0: u32,
+    pub g1: u32,
+    pub g2: u32,
+    pub interleaved: c_int,
+    pub base: f32,
+}
+
+#[repr(C)] #[derive(Clone, Copy)]
+pub struct rnn_diff_attn_desc {
+    pub h: u32,
+    pub hkv: u32,
+    pub dh: u32,
+    pub tq: u32,
+    pub tk: u32,
+    pub qstride: usize,
+    pub qoff: usize,
+    pub kvstride: usize,
+    pub koff: usize,
+    pub voff: usize,
+    pub lam_heads: u32,
+    pub mask_diag: c_int,
+    pub causal: c_int,
+    pub scale: f32,
+    pub lam_init: f32,
+    pub eps: f32,
 }
 
 #[repr(C)] #[derive(Clone, Copy)]
@@ -126,10 +170,17 @@ extern "C" {
     pub fn rnn_attn_forward(ctx: *mut rnn_ctx, d: *const rnn_attn_desc, n: usize, q: *const f32, kv: *const f32, tau: *const f32, rel: *const f32, p: *mut f32, o: *mut f32) -> c_int;
     pub fn rnn_attn_backward(ctx: *mut rnn_ctx, d: *const rnn_attn_desc, n: usize, q: *const f32, kv: *const f32, tau: *const f32, p: *const f32, dout: *const f32, dq: *mut f32, dkv: *mut f32, dtau: *mut f32, drel: *mut f32) -> c_int;
     pub fn rnn_attn_backward_ex(ctx: *mut rnn_ctx, d: *const rnn_attn_desc, n: usize, q: *const f32, kv: *const f32, tau: *const f32, p: *const f32, dout: *const f32, dq: *mut f32, dkv: *mut f32, dtau: *mut f32, drel: *mut f32, flags: u32) -> c_int;
+    pub fn rnn_rotary_check(d: *const rnn_rotary_desc, n: usize, t: usize, have_pos: c_int) -> c_int;
+    pub fn rnn_rotary(ctx: *mut rnn_ctx, d: *const rnn_rotary_desc, n: usize, t: usize, x: *const f32, pos: *const f32, y: *mut f32, inverse: c_int) -> c_int;
+    pub fn rnn_diff_attn_workspace(d: *const rnn_diff_attn_desc, n: usize, backward: c_int, bytes: *mut usize) -> c_int;
+    pub fn rnn_diff_attn_forward(ctx: *mut rnn_ctx, d: *const rnn_diff_attn_desc, n: usize, q: *const f32, kv: *const f32, lam: *const f32, gain: *const f32, qlen: *const u32, klen: *const u32, ws: *mut c_void, ws_bytes: usize, y: *mut f32, o12: *mut f32, stats: *mut f32) -> c_int;
+    pub fn rnn_diff_attn_backward(ctx: *mut rnn_ctx, d: *const rnn_diff_attn_desc, n: usize, q: *const f32, kv: *const f32, lam: *const f32, gain: *const f32, qlen: *const u32, klen: *const u32, o12: *const f32, stats: *const f32, dy: *const f32, ws: *mut c_void, ws_bytes: usize, dq: *mut f32, dkv: *mut f32, dlam: *mut f32, dgain: *mut f32, flags: u32) -> c_int;
     pub fn rnn_linear_forward(ctx: *mut rnn_ctx, rows: usize, fin: usize, fout: usize, x: *const f32, w: *const f32, b: *const f32, y: *mut f32) -> c_int;
     pub fn rnn_linear_forward_residual(ctx: *mut rnn_ctx, rows: usize, fin: usize, fout: usize, x: *const f32, w: *const f32, b: *const f32, y: *mut f32, l: *const f32, mask: *const f32, rpi: usize, out: *mut f32) -> c_int;
     pub fn rnn_linear_backward(ctx: *mut rnn_ctx, rows: usize, fin: usize, fout: usize, dy: *const f32, x: *const f32, w: *const f32, dw: *mut f32, db: *mut f32, dx: *mut f32) -> c_int;
     pub fn rnn_linear_backward_ex(ctx: *mut rnn_ctx, rows: usize, fin: usize, fout: usize, dy: *const f32, x: *const f32, w: *const f32, dw: *mut f32, db: *mut f32, dx: *mut f32, flags: u32) -> c_int;
+    pub fn rnn_linear_act_forward(ctx: *mut rnn_ctx, rows: usize, fin: usize, fout: usize, x: *const f32, w: *const f32, b: *const f32, act: u32, res: *const f32, z: *mut f32, y: *mut f32) -> c_int;
+    pub fn rnn_linear_act_backward(ctx: *mut rnn_ctx, rows: usize, fin: usize, fout: usize, dy: *const f32, x: *const f32, w: *const f32, z: *const f32, act: u32, dz: *mut f32, dw: *mut f32, db: *mut f32, dx: *mut f32, flags: u32) -> c_int;
     pub fn rnn_matmul_host(ctx: *mut rnn_ctx, m: usize, n: usize, k: usize, a: *const f32, at: c_int, b: *const f32, bt: c_int, c: *mut f32, acc: c_int) -> c_int;
     pub fn rnn_gemm_small_batched_host(ctx: *mut rnn_ctx, count: usize, m: usize, n: usize, k: usize, a: *const f32, stride_a: usize, at: c_int, b: *const f32, stride_b: usize, bt: c_int, c: *mut f32, stride_c: usize, acc: c_int) -> c_int;
     pub fn rnn_matmul_dw_host(ctx: *mut rnn_ctx, m: usize, n: usize, k: usize, a: *const f32, b: *const f32, c: *mut f32) -> c_int;

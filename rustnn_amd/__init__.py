@@ -8,6 +8,9 @@ reference's host interface for the hot path:
 * ``Conv2d`` (forward / backward_w / backward)          -- nn.rs:115-250
 * ``Linear`` (forward / backward)                       -- linear.rs:14-104
 * ``Core`` (forward / backward), ``rel_index``          -- attn.rs:21-343
+* ``Rotary``, ``DiffCore``, ``linear_act_forward`` / ``linear_act_backward``:
+  rotary positions, differential attention and the Linear product with an
+  activation and a residual (no counterpart in the reference)
 * ``rustnn_amd.nn``: BatchNorm2d, the classifier Linear, gap, softmax_ce,
   Param::step                                           -- nn.rs:37-637
 * ``rustnn_amd.model.ResNet``: the device-resident train step -- model.rs
@@ -33,6 +36,8 @@ HEADER = os.path.join(HERE, "..", "include", "rnn.h")
 RNN_OK, RNN_E_INVALID, RNN_E_NULL, RNN_E_HIP, RNN_E_NOMEM, RNN_E_UNSUPPORTED = 0, -1, -2, -3, -4, -5
 RNN_LINEAR_ACC_DX = 1  # rnn_linear_backward_ex
 RNN_DW3_ACC_DX = 1  # rnn_dwconv3_backward_ex
+RNN_ATTN_SET_DQ, RNN_ATTN_SET_DKV = 1, 2  # rnn_attn_backward_ex, rnn_diff_attn_backward
+ACTS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}  # RNN_ACT_*
 
 _sz = C.c_size_t
 _vp = C.c_void_p
@@ -87,6 +92,21 @@ class AttnDesc(C.Structure):
                 ("voff", _sz), ("nrel", _u32), ("relidx", C.POINTER(_u32)), ("mask_diag", _i)]
 
 
+class RotaryDesc(C.Structure):
+    """rnn_rotary_desc."""
+    _fields_ = [("h", _u32), ("dh", _u32), ("xstride", _sz), ("xoff", _sz), ("ystride", _sz),
+                ("yoff", _sz)] + [(k, _u32) for k in ("axes", "p0", "p1", "p2", "g0", "g1", "g2")
+                                  ] + [("interleaved", _i), ("base", C.c_float)]
+
+
+class DiffAttnDesc(C.Structure):
+    """rnn_diff_attn_desc."""
+    _fields_ = [(k, _u32) for k in ("h", "hkv", "dh", "tq", "tk")] + [
+        (k, _sz) for k in ("qstride", "qoff", "kvstride", "koff", "voff")] + [
+        ("lam_heads", _u32), ("mask_diag", _i), ("causal", _i)] + [
+        (k, C.c_float) for k in ("scale", "lam_init", "eps")]
+
+
 _lib = None
 _lib_lock = threading.Lock()
 
@@ -136,6 +156,17 @@ def lib():
                                        _vp, _vp]),
             "rnn_attn_backward_ex": (_i, [_vp, P(AttnDesc), _sz, _vp, _vp, _vp, _vp, _vp, _vp,
                                           _vp, _vp, _vp, _u32]),
+            "rnn_rotary_check": (_i, [P(RotaryDesc), _sz, _sz, _i]),
+            "rnn_rotary": (_i, [_vp, P(RotaryDesc), _sz, _sz, _vp, _vp, _vp, _i]),
+            "rnn_diff_attn_workspace": (_i, [P(DiffAttnDesc), _sz, _i, P(_sz)]),
+            "rnn_diff_attn_forward": (_i, [_vp, P(DiffAttnDesc), _sz] + [_vp] * 7 +
+                                      [_sz, _vp, _vp, _vp]),
+            "rnn_diff_attn_backward": (_i, [_vp, P(DiffAttnDesc), _sz] + [_vp] * 10 +
+                                       [_sz, _vp, _vp, _vp, _vp, _u32]),
+            "rnn_linear_act_forward": (_i, [_vp, _sz, _sz, _sz, _vp, _vp, _vp, _u32, _vp, _vp,
+                                            _vp]),
+            "rnn_linear_act_backward": (_i, [_vp, _sz, _sz, _sz, _vp, _vp, _vp, _vp, _u32, _vp,
+                                             _vp, _vp, _vp, _u32]),
             "rnn_linear_forward": (_i, [_vp, _sz, _sz, _sz, _vp, _vp, _vp, _vp]),
             "rnn_linear_forward_residual": (_i, [_vp, _sz, _sz, _sz, _vp, _vp, _vp, _vp, _vp,
                                                  _vp, _sz, _vp]),
@@ -377,6 +408,37 @@ def _new(n, like=None, device=0):
     import torch
     dev = like.device if like is not None else torch.device("cuda", device)
     return torch.empty(n, dtype=torch.float32, device=dev)
+
+
+def _arg(ctx, t, need, name, dtype="float32"):
+    """Device pointer of a contiguous tensor of ``dtype`` ("float32", or
+    "u32": uint32 / int32) on the context's device with >= need elements."""
+    if t is None:
+        return None
+    import torch
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError(f"{name} must be a CUDA tensor")
+    want = (torch.float32,) if dtype == "float32" else (torch.uint32, torch.int32)
+    if t.dtype not in want:
+        raise TypeError(f"{name} must be {'/'.join(str(w)[6:] for w in want)} (got {t.dtype})")
+    if t.device.index != ctx.device:
+        raise ValueError(f"{name} is on cuda:{t.device.index}, the context on cuda:{ctx.device}")
+    return _ptr(t, need, name)
+
+
+def _on_ctx_stream(ctx, *ts):
+    """Tells torch's allocator of tensors that the context's stream uses, where
+    that is not the current one, so that their memory is not handed out again
+    before its work is done."""
+    import torch
+    sp = ctx.stream_ptr()
+    if torch.cuda.current_stream(ctx.device).cuda_stream == sp:
+        return
+    st = torch.cuda.ExternalStream(sp, device=ctx.device) if sp else \
+        torch.cuda.default_stream(ctx.device)
+    for t in ts:
+        if t is not None:
+            t.record_stream(st)
 
 
 # ------------------------------------------------------------------ gemm.rs
@@ -679,6 +741,169 @@ class Core:
             _ptr(drel, self.h * self.nrel, "drel"), flags))
 
 
+# ------------------------------------------------- rotary, differential attention
+class Rotary:
+    """Rotary positions with one to three axes on heads of dh channels
+    (rnn_rotary).  grid: the sides of an image's token grid, last fastest
+    (a time axis first: frames, rows, columns); pairs: the channel pairs that
+    each axis turns (default: an even share of dh // 2, what is left over to
+    the first axes); interleaved: pair j is channels (2j, 2j + 1), else
+    (j, j + R), R the sum of pairs.  A number for ``grid`` is one axis."""
+
+    def __init__(self, heads, dh, grid, base=10000.0, pairs=None, interleaved=False, ctx=None):
+        self.grid = tuple(int(v) for v in (grid if hasattr(grid, "__len__") else (grid,)))
+        self.heads, self.dh, self.base = int(heads), int(dh), float(base)
+        axes = len(self.grid)
+        if not 1 <= axes <= 3:
+            raise ValueError(f"Rotary: {axes} axes (1 to 3)")
+        if pairs is None:
+            r = self.dh // 2
+            pairs = [r // axes + (i < r % axes) for i in range(axes)]
+        self.pairs = tuple(int(v) for v in pairs)
+        if len(self.pairs) != axes:
+            raise ValueError(f"Rotary: {len(self.pairs)} shares of pairs for {axes} axes")
+        if min(self.pairs + self.grid + (self.heads, self.dh)) < 0:
+            raise ValueError("Rotary: a negative size")
+        self.interleaved, self.ctx = bool(interleaved), ctx
+        self.t = math.prod(self.grid)
+        w = self.heads * self.dh
+        rc = lib().rnn_rotary_check(C.byref(self._desc(w, 0, w, 0)), 1, self.t, 0)
+        if rc:
+            raise ValueError(f"Rotary: {lib().rnn_status_string(rc).decode()} (heads={heads} "
+                             f"dh={dh} grid={self.grid} pairs={self.pairs} base={base})")
+
+    def _desc(self, xstride, xoff, ystride, yoff):
+        p = self.pairs + (0,) * (3 - len(self.pairs))
+        g = self.grid + (1,) * (3 - len(self.grid))
+        return RotaryDesc(self.heads, self.dh, xstride, xoff, ystride, yoff, len(self.grid), *p,
+                          *g, int(self.interleaved), self.base)
+
+    def _turn(self, n, x, xstride, xoff, pos, y, ystride, yoff, t, inverse):
+        import torch
+        ctx, w = self.ctx or default_ctx(x.device.index or 0), self.heads * self.dh
+        t = self.t if t is None else int(t)
+        if y is None:
+            ystride, yoff = w, 0
+            y = torch.empty(n, t, w, dtype=torch.float32, device=x.device)
+        elif ystride is None:
+            ystride, yoff = xstride, xoff
+        d = self._desc(xstride, xoff, ystride, yoff)
+        rows = n * t
+        need = lambda stride, off: (rows - 1) * stride + off + w if rows else 0
+        ctx.check(lib().rnn_rotary(
+            ctx.h, C.byref(d), n, t, _arg(ctx, x, need(xstride, xoff), "x"),
+            _arg(ctx, pos, rows * len(self.grid), "pos"),
+            _arg(ctx, y, need(ystride, yoff), "y"), int(inverse)))
+        _on_ctx_stream(ctx, x, y, pos)
+        return y
+
+    def forward(self, n, x, xstride, xoff=0, pos=None, y=None, ystride=None, yoff=0, t=None):
+        """Turns the heads at x[r * xstride + xoff ...] of n images; writes
+        y (x: in place; None: a new [n, t, heads * dh]), at the same layout
+        unless ystride is given.  pos [n * t, axes]: each row's position
+        instead of its grid coordinates; then t may be any length."""
+        return self._turn(n, x, xstride, xoff, pos, y, ystride, yoff, t, False)
+
+    def backward(self, n, dy, xstride, xoff=0, pos=None, y=None, ystride=None, yoff=0, t=None):
+        """dx from dy, in the layouts of forward (the inverse turn)."""
+        return self._turn(n, dy, xstride, xoff, pos, y, ystride, yoff, t, True)
+
+
+class DiffCore:
+    """Differential attention (rnn_diff_attn_*): per (image, head)
+    y = (1 - lam_init) gain norm((P1 - lambda P2) V) over two query and key
+    maps of dh channels and values of 2 dh, h query heads on hkv key heads.
+    forward / backward take q and kv as Core's: a buffer with its row stride
+    and the first channel of the queries, and of the keys and values.  scale:
+    default 1 / sqrt(dh); lam_heads: 1 (one lambda for all heads) or h."""
+
+    def __init__(self, h, dh, tq, tk, hkv=None, mask_diag=False, causal=False, lam_heads=1,
+                 scale=None, lam_init=0.8, eps=1e-5, ctx=None):
+        self.h, self.dh, self.tq, self.tk = int(h), int(dh), int(tq), int(tk)
+        self.hkv = self.h if hkv is None else int(hkv)
+        self.mask_diag, self.causal, self.lam_heads = bool(mask_diag), bool(causal), int(lam_heads)
+        if min(self.h, self.dh, self.tq, self.tk, self.hkv, self.lam_heads) < 0:
+            raise ValueError("DiffCore: a negative size")
+        self.scale = 1.0 / math.sqrt(max(self.dh, 1)) if scale is None else float(scale)
+        self.lam_init, self.eps, self.ctx = float(lam_init), float(eps), ctx
+        self.c = 2 * self.h * self.dh
+        kw = 2 * self.hkv * self.dh
+        d = self.desc(self.c, 0, 2 * kw, 0, kw)
+        self._bytes(d, 1, 0)
+
+    def desc(self, qstride, qoff, kvstride, koff, voff):
+        return DiffAttnDesc(self.h, self.hkv, self.dh, self.tq, self.tk, qstride, qoff, kvstride,
+                            koff, voff, self.lam_heads, int(self.mask_diag), int(self.causal),
+                            self.scale, self.lam_init, self.eps)
+
+    def _bytes(self, d, n, backward):
+        nb = _sz()
+        rc = lib().rnn_diff_attn_workspace(C.byref(d), n, backward, C.byref(nb))
+        if rc:
+            raise ValueError(f"DiffCore: {lib().rnn_status_string(rc).decode()} (h={self.h} "
+                             f"hkv={self.hkv} dh={self.dh} tq={self.tq} tk={self.tk} n={n} "
+                             f"lam_heads={self.lam_heads} scale={self.scale} "
+                             f"lam_init={self.lam_init} eps={self.eps})")
+        return nb.value
+
+    def _inputs(self, ctx, d, n, q, kv, lam, gain, qlen, klen):
+        kw = 2 * self.hkv * self.dh
+        nq = (n * self.tq - 1) * d.qstride + d.qoff + self.c if n * self.tq else 0
+        nkv = (n * self.tk - 1) * d.kvstride + max(d.koff, d.voff) + kw if n * self.tk else 0
+        return nq, nkv, (_arg(ctx, q, nq, "q"), _arg(ctx, kv, nkv, "kv"),
+                         _arg(ctx, lam, self.lam_heads * 4 * self.dh, "lam"),
+                         _arg(ctx, gain, 2 * self.dh, "gain"), _arg(ctx, qlen, n, "qlen", "u32"),
+                         _arg(ctx, klen, n, "klen", "u32"))
+
+    def forward(self, n, q, qstride, qoff, kv, kvstride, koff, voff, lam, gain=None, qlen=None,
+                klen=None, train=True, y=None):
+        """(y [n, tq, 2 h dh], what backward needs: None unless train).  qlen,
+        klen (int32 / uint32 [n]): the images' lengths where they are padded."""
+        import torch
+        ctx = self.ctx or default_ctx(q.device.index or 0)
+        d = self.desc(qstride, qoff, kvstride, koff, voff)
+        nb = self._bytes(d, n, 0)
+        _, _, ins = self._inputs(ctx, d, n, q, kv, lam, gain, qlen, klen)
+        rows = n * self.tq
+        if y is None:
+            y = torch.empty(n, self.tq, self.c, dtype=torch.float32, device=q.device)
+        saved = None
+        if train:
+            saved = (torch.empty(rows * 2 * self.c, dtype=torch.float32, device=q.device),
+                     torch.empty(rows * self.h * 4, dtype=torch.float32, device=q.device))
+        ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None
+        o12, stats = saved or (None, None)
+        ctx.check(lib().rnn_diff_attn_forward(
+            ctx.h, C.byref(d), n, *ins, ws.data_ptr() if nb else None, nb,
+            _arg(ctx, y, rows * self.c, "y"), _arg(ctx, o12, 0, "o12"),
+            _arg(ctx, stats, 0, "stats")))
+        _on_ctx_stream(ctx, q, kv, lam, gain, qlen, klen, ws, y, o12, stats)
+        return y, saved
+
+    def backward(self, n, q, qstride, qoff, kv, kvstride, koff, voff, lam, gain, saved, dy, dq,
+                 dkv, dlam, dgain=None, qlen=None, klen=None, set_dq=False, set_dkv=False):
+        """Accumulates into dq, dkv (laid out as q, kv), dlam and dgain; set_dq
+        / set_dkv overwrite dq / dkv instead."""
+        import torch
+        if saved is None:
+            raise ValueError("DiffCore.backward: the forward did not keep its maps (train=False)")
+        ctx = self.ctx or default_ctx(dy.device.index or 0)
+        d = self.desc(qstride, qoff, kvstride, koff, voff)
+        nb = self._bytes(d, n, 1)
+        nq, nkv, ins = self._inputs(ctx, d, n, q, kv, lam, gain, qlen, klen)
+        rows = n * self.tq
+        o12, stats = saved
+        ws = torch.empty(nb, dtype=torch.uint8, device=dy.device) if nb else None
+        flags = (RNN_ATTN_SET_DQ if set_dq else 0) | (RNN_ATTN_SET_DKV if set_dkv else 0)
+        ctx.check(lib().rnn_diff_attn_backward(
+            ctx.h, C.byref(d), n, *ins, _arg(ctx, o12, rows * 2 * self.c, "o12"),
+            _arg(ctx, stats, rows * self.h * 4, "stats"), _arg(ctx, dy, rows * self.c, "dy"),
+            ws.data_ptr() if nb else None, nb, _arg(ctx, dq, nq, "dq"),
+            _arg(ctx, dkv, nkv, "dkv"), _arg(ctx, dlam, self.lam_heads * 4 * self.dh, "dlam"),
+            _arg(ctx, dgain, 2 * self.dh, "dgain"), flags))
+        _on_ctx_stream(ctx, q, kv, lam, gain, qlen, klen, ws, dy, o12, stats, dq, dkv, dlam, dgain)
+
+
 # ------------------------------------------------------------------ linear.rs
 def linear_forward(rows, fin, fout, x, w, b=None, y=None, ctx=None):
     ctx = ctx or default_ctx()
@@ -713,6 +938,54 @@ def linear_backward(rows, fin, fout, dy, x, w, dw, db=None, dx=None, ctx=None, a
                                            _ptr(dw, fout * fin, "dw"), _ptr(db, fout, "db"),
                                            _ptr(dx, rows * fin, "dx"),
                                            RNN_LINEAR_ACC_DX if acc_dx else 0))
+    return dx
+
+
+def _act_code(act):
+    if act not in ACTS:
+        raise ValueError(f"activation {act!r} (one of {', '.join(ACTS)})")
+    return ACTS[act]
+
+
+def linear_act_forward(rows, fin, fout, x, w, b=None, act="none", res=None, y=None, train=True,
+                       ctx=None):
+    """(y, z): z = x W^T + b, y = act(z) + res, act one of ACTS; z is kept for
+    linear_act_backward when train and act is not "none", else None."""
+    import torch
+    code = _act_code(act)
+    ctx = ctx or default_ctx(x.device.index or 0)
+    new = lambda: torch.empty(rows, fout, dtype=torch.float32, device=x.device)
+    y = new() if y is None else y
+    z = new() if train and code else None
+    ctx.check(lib().rnn_linear_act_forward(
+        ctx.h, rows, fin, fout, _arg(ctx, x, rows * fin, "x"), _arg(ctx, w, fout * fin, "w"),
+        _arg(ctx, b, fout, "b"), code, _arg(ctx, res, rows * fout, "res"),
+        _arg(ctx, z, rows * fout, "z"), _arg(ctx, y, rows * fout, "y")))
+    _on_ctx_stream(ctx, x, w, b, res, z, y)
+    return y, z
+
+
+def linear_act_backward(rows, fin, fout, dy, x, w, z, act, dw, db=None, dx=None, acc_dx=False,
+                        ctx=None):
+    """dx (returned; acc_dx: added to the given dx); dw and db accumulate.
+    z, as linear_act_forward kept it, is left unchanged.  The residual's
+    gradient is dy."""
+    import torch
+    code = _act_code(act)
+    if acc_dx and dx is None:
+        raise ValueError("linear_act_backward: acc_dx needs dx")
+    if code and z is None:
+        raise ValueError("linear_act_backward: the forward did not keep z (train=False)")
+    ctx = ctx or default_ctx(dy.device.index or 0)
+    dx = torch.empty(rows, fin, dtype=torch.float32, device=dy.device) if dx is None else dx
+    dz = torch.empty(rows, fout, dtype=torch.float32, device=dy.device) if code else None
+    ctx.check(lib().rnn_linear_act_backward(
+        ctx.h, rows, fin, fout, _arg(ctx, dy, rows * fout, "dy"), _arg(ctx, x, rows * fin, "x"),
+        _arg(ctx, w, fout * fin, "w"), _arg(ctx, z, rows * fout, "z"), code,
+        _arg(ctx, dz, rows * fout, "dz"), _arg(ctx, dw, fout * fin, "dw"),
+        _arg(ctx, db, fout, "db"), _arg(ctx, dx, rows * fin, "dx"),
+        RNN_LINEAR_ACC_DX if acc_dx else 0))
+    _on_ctx_stream(ctx, dy, x, w, z, dz, dw, db, dx)
     return dx
 
 

@@ -288,6 +288,26 @@ int rnn_fail(rnn_ctx *ctx, int code, const char *fmt, ...);
                             hipGetErrorString(e_), __FILE__, __LINE__);                 \
     } while (0)
 
+// Makes a context's device the current one for a call, and the caller's
+// current again after it.
+struct RnnDeviceGuard {
+    int prev = -1;
+    bool ok = false;
+    explicit RnnDeviceGuard(int device) {
+        int cur = -1;
+        if (hipGetDevice(&cur) != hipSuccess) return;
+        ok = cur == device || hipSetDevice(device) == hipSuccess;
+        if (cur != device) prev = cur;
+    }
+    ~RnnDeviceGuard() {
+        if (prev >= 0) (void)hipSetDevice(prev);
+    }
+    RnnDeviceGuard(const RnnDeviceGuard &) = delete;
+};
+#define RNN_ON_DEVICE(ctx)                   \
+    RnnDeviceGuard dev_guard_((ctx)->device); \
+    if (!dev_guard_.ok) return rnn_fail((ctx), RNN_E_HIP, "hipSetDevice(%d) failed", (ctx)->device)
+
 // Returns a device workspace of at least `bytes` (256-byte aligned), or
 // nullptr after recording RNN_E_NOMEM / RNN_E_HIP in ctx.
 void *rnn_workspace(rnn_ctx *ctx, size_t bytes);
