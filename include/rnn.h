@@ -291,11 +291,13 @@ typedef struct {
  * forward (backward = 0) or the backward needs for n images; host only.  The
  * workspace is the caller's, 256-byte aligned, holds nothing between calls
  * and is not shared by calls that may run at the same time.  dh <= 64
- * (RNN_E_UNSUPPORTED above), scale > 0, 0 <= lam_init < 1. */
+ * and row strides <= 2^22 (RNN_E_UNSUPPORTED above), scale > 0, 0 <= lam_init
+ * < 1. */
 int rnn_diff_attn_workspace(const rnn_diff_attn_desc *d, size_t n, int backward, size_t *bytes);
 /* y [n][tq][h][2 dh].  For a backward: o12 [n][tq][h][2][2 dh] receives each
- * map's P_m V and stats [n][tq][h][4] each map's largest scaled score and the
- * reciprocal of its softmax sum; both NULL: not kept. */
+ * map's P_m V and stats [n][tq][h][4] (16-byte aligned) each map's largest score
+ * and the reciprocal of its softmax sum, as the backward takes them; both NULL:
+ * not kept. */
 int rnn_diff_attn_forward(rnn_ctx *ctx, const rnn_diff_attn_desc *d, size_t n, const float *q,
                           const float *kv, const float *lam, const float *gain,
                           const uint32_t *qlen, const uint32_t *klen, void *ws, size_t ws_bytes,

@@ -270,10 +270,10 @@ def test_captured_and_replayed(rnn, name):
 
 
 def test_rows_past_32_bit_offsets(rnn):
-    """A key and value buffer whose rows lie further apart than 2^31 floats."""
-    n, h, dh, tq, tk = 1, 2, 32, 5, 70
+    """A key and value buffer of more than 2^31 floats, rows 16 MiB apart."""
+    n, h, dh, tq, tk = 1, 2, 32, 5, 530
     kw = 2 * h * dh
-    stride = (2 ** 31 + 2 ** 20) // (tk - 1) + 1
+    stride = 2 ** 22
     cs = DiffCase(n, h, h, dh, tq, tk, True, gap=0, seed=8)
     buf = torch.empty((tk - 1) * stride + 2 * kw, device="cuda")
     view = buf.as_strided((tk, 2 * kw), (stride, 1))
@@ -318,6 +318,8 @@ def test_refusals(rnn):
         core.forward(2, q, cs.qw - 1, 0, *geo[3:], lam, gain)  # heads do not fit
     with pytest.raises(ValueError):
         core.forward(2, *geo[:5], 0, cs.kw - 1, lam, gain)  # keys over values
+    with pytest.raises(ValueError):
+        core.forward(2, q, cs.qstride, 0, kv, 2 ** 22 + 1, 0, cs.kw, lam, gain)  # rows too far apart
     y, saved = core.forward(2, *geo, lam, gain, train=False)
     assert saved is None
     with pytest.raises(ValueError):
