@@ -26,7 +26,7 @@ struct DiffArgs {
     float *y, *o12, *stats;
     float *dq, *dkv;
     float *dout;  // dO, [n][tq][h][2 dh]
-    float *dd;    // D_1, D_2, [n][tq][h][2]
+    float *rec;   // [n][tq][h][8]: the forward's stats, D_1, D_2, |dO|, lambda
     float *part32, *pstat;  // splits: outputs [n][tq][h][splits][2][2 dh], (max, sum) beside them
     double *part; // partials of dgain and dlambda, [blocks][2 dh + h]
     long long qstride, kvstride;
@@ -201,7 +201,8 @@ template <int ROWS, int W, int NT>
 struct StagePlan {
     static constexpr int C8 = W / 8;
     static constexpr int fit = NT / C8;
-    static constexpr int RPP = fit >= 64 ? 64 : fit >= 32 ? 32 : fit >= 16 ? 16 : 8;
+    static constexpr int most = fit >= 64 ? 64 : fit >= 32 ? 32 : fit >= 16 ? 16 : fit >= 8 ? 8 : 4;
+    static constexpr int RPP = most < ROWS ? most : ROWS;
     static constexpr int PASSES = ROWS / RPP;
     static constexpr bool ALL = RPP * C8 == NT;
     static_assert(RPP * C8 <= NT && PASSES * RPP == ROWS, "whole passes");
@@ -234,6 +235,100 @@ __device__ __forceinline__ float lane_lambda(const DiffArgs &g, int head) {
     return (float)(exp(a) - exp(b) + (double)g.lam_init);
 }
 
+// Tiles of TK keys and values on their way to LDS: a thread's share in registers
+// from its loads on.
+template <int DHP, int TK, int NT, bool VEC>
+struct KvStage {
+    static constexpr int W = 2 * DHP;
+    using Tile = HalfTile<TK, W>;
+    using Stage = StagePlan<TK, W, NT>;
+    static constexpr int CH = Stage::PASSES;
+    float xk[CH][8], xv[CH][8];
+    const float *kp, *vp;
+    long long stride;
+    uint32_t koff, voff, step;
+    int kend, klim, vlim, sc, sr;
+    // The thread's channels [sc, sc + 8) of rows sr, sr + RPP, ...; keys: two
+    // runs of dh padded to DHP, values: one of 2 dh.
+    __device__ __forceinline__ KvStage(const DiffArgs &g, int b, int kh, int kend_) : kend(kend_) {
+        const float *kv = g.kv + (long long)b * g.tk * g.kvstride;
+        kp = kv + g.koff + 2 * kh * g.dh;
+        vp = kv + g.voff + 2 * kh * g.dh;
+        stride = g.kvstride;
+        sc = (int)threadIdx.x % Stage::C8 * 8;
+        sr = (int)threadIdx.x / Stage::C8;
+        const int run = sc >= DHP ? 1 : 0;
+        klim = stager() ? g.dh - (sc - run * DHP) : 0;
+        vlim = stager() ? 2 * g.dh - sc : 0;
+        koff = sr * (uint32_t)stride + sc - run * (DHP - g.dh);
+        voff = sr * (uint32_t)stride + sc;
+        step = Stage::RPP * (uint32_t)stride;
+    }
+    __device__ __forceinline__ bool stager() const { return Stage::ALL || sr < Stage::RPP; }
+    __device__ __forceinline__ void load(int k0) {
+        // rows from kend on are past the resource's end
+        const uint32_t bytes = (uint32_t)min(kend - k0, TK) * (uint32_t)stride * 4;
+        const auto rk = make_rsrc(kp + k0 * stride, bytes), rv = make_rsrc(vp + k0 * stride, bytes);
+#pragma unroll
+        for (int i = 0; i < CH; i++) {
+            load8<VEC>(rk, koff + i * step, klim, xk[i]);
+            load8<VEC>(rv, voff + i * step, vlim, xv[i]);
+        }
+    }
+    __device__ __forceinline__ void maxima(float *mk, float *mv) const {
+        float a = 0.f, b = 0.f;
+#pragma unroll
+        for (int i = 0; i < CH; i++) {
+            a = absmax8(xk[i], a);
+            b = absmax8(xv[i], b);
+        }
+        a = wave_max(a);
+        b = wave_max(b);
+        if ((threadIdx.x & 63) == 0) {
+            mk[wave_index()] = a;
+            mv[wave_index()] = b;
+        }
+    }
+    // K's tile at lds, V's behind it.
+    __device__ __forceinline__ void store(_Float16 *lds, float kup, float vup) const {
+        if (!stager()) return;
+#pragma unroll
+        for (int i = 0; i < CH; i++) {
+            _Float16 *d = lds + (sr + i * Stage::RPP) * Tile::STRIDE + sc;
+            const Half2 hk = half_split(xk[i], kup), hv = half_split(xv[i], vup);
+            *(h8 *)d = hk.hi;
+            *(h8 *)(d + Tile::PART) = hk.lo;
+            *(h8 *)(d + Tile::HALVES) = hv.hi;
+            *(h8 *)(d + Tile::HALVES + Tile::PART) = hv.lo;
+        }
+    }
+};
+
+// Channels c0 + {0..3} + 4 lh + 8 j of a row (an accumulator of 32 channels, lane
+// = row), below lim, times f (live) or 0, stored or added.
+template <bool VEC>
+__device__ __forceinline__ void put_channels(float *dst, int lim, int c0, const f32x16 &a, float f,
+                                             bool live, int add) {
+    const int lh = (threadIdx.x >> 5) & 1;
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+        const int ch = c0 + 2 * r + 4 * lh;
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = live ? a[r + e] * f : 0.f;
+        if (VEC) {
+            if (ch >= lim) continue;
+            float4 *d = (float4 *)(dst + ch);
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (add) o = *d;
+            *d = make_float4(o.x + v[0], o.y + v[1], o.z + v[2], o.w + v[3]);
+        } else {
+            for (int e = 0; e < 4; e++)
+                if (ch + e < lim) dst[ch + e] = add ? dst[ch + e] + v[e] : v[e];
+        }
+    }
+}
+
 // Forward.  One workgroup of 2 QG waves per (image, key head, 32 QG rows); a
 // row is a query of one of the head group's heads, so that heads that share
 // keys share their tiles.  Wave 2 i + m owns rows [32 i, 32 i + 32) and map m:
@@ -250,8 +345,6 @@ __attribute__((amdgpu_waves_per_eu(QG == 4 || DHP <= 32 ? 2 : 1))) void
 diff_fwd_kernel(DiffArgs g) {
     constexpr int W = 2 * DHP, TK = 64, NT = 128 * QG, KS = DHP / 16, CT = DHP / 16;
     using Tile = HalfTile<TK, W>;
-    using Stage = StagePlan<TK, W, NT>;
-    constexpr int CH = Stage::PASSES;
     static_assert((int)sizeof(_Float16) * 2 * Tile::HALVES >= QG * CT * 16 * 64 * 4, "exchange");
     __shared__ __align__(16) _Float16 lds[2 * Tile::HALVES];
     __shared__ float tmax[2][2][2 * QG];
@@ -273,44 +366,8 @@ diff_fwd_kernel(DiffArgs g) {
     if (SPLIT) kend = min(kend, kbeg + g.split_keys);
     const int ntile = kend > kbeg ? (kend - kbeg + TK - 1) / TK : 0;
 
-    const float *kv = g.kv + (long long)b * g.tk * g.kvstride;
-    const float *kp = kv + g.koff + 2 * kh * g.dh, *vp = kv + g.voff + 2 * kh * g.dh;
-    float xk[CH][8], xv[CH][8];
-    // the thread's channels [sc, sc + 8) of rows sr, sr + RPP, ...; keys: two
-    // runs of dh padded to DHP, values: one of 2 dh
-    const int sc = (int)threadIdx.x % Stage::C8 * 8, sr = (int)threadIdx.x / Stage::C8;
-    const bool stager = Stage::ALL || sr < Stage::RPP;
-    const int run = sc >= DHP ? 1 : 0;
-    const int klim = stager ? g.dh - (sc - run * DHP) : 0, vlim = stager ? 2 * g.dh - sc : 0;
-    const uint32_t koff = sr * (uint32_t)g.kvstride + sc - run * (DHP - g.dh);
-    const uint32_t voff = sr * (uint32_t)g.kvstride + sc;
-    auto load = [&](int k0) {
-        // rows from kend on are past the resource's end
-        const uint32_t bytes = (uint32_t)min(kend - k0, TK) * (uint32_t)g.kvstride * 4;
-        const long long at = k0 * g.kvstride;
-        const auto rk = make_rsrc(kp + at, bytes), rv = make_rsrc(vp + at, bytes);
-#pragma unroll
-        for (int i = 0; i < CH; i++) {
-            const uint32_t step = i * Stage::RPP * (uint32_t)g.kvstride;
-            load8<VEC>(rk, koff + step, klim, xk[i]);
-            load8<VEC>(rv, voff + step, vlim, xv[i]);
-        }
-    };
-    auto maxima = [&](int slot) {
-        float mk = 0.f, mv = 0.f;
-#pragma unroll
-        for (int i = 0; i < CH; i++) {
-            mk = absmax8(xk[i], mk);
-            mv = absmax8(xv[i], mv);
-        }
-        mk = wave_max(mk);
-        mv = wave_max(mv);
-        if (lane == 0) {
-            tmax[slot][0][wave] = mk;
-            tmax[slot][1][wave] = mv;
-        }
-    };
-    if (ntile) load(kbeg);
+    KvStage<DHP, TK, NT, VEC> st(g, b, kh, kend);
+    if (ntile) st.load(kbeg);
 
     // the row's query of this map, times its own power of two
     Half2 q[KS];
@@ -340,8 +397,8 @@ diff_fwd_kernel(DiffArgs g) {
     // rows of the wave's queries, for tiles that every one of them sees whole
     const int w_first = (rb * 32 * QG + qg * 32) / g.group;
     const int w_last = min(nq - 1, (rb * 32 * QG + qg * 32 + 31) / g.group);
-    if (ntile) maxima(0);
-    _Float16 *const kt = lds, *const vt = lds + Tile::HALVES;
+    if (ntile) st.maxima(tmax[0][0], tmax[0][1]);
+    const _Float16 *const kt = lds, *const vt = lds + Tile::HALVES;
     for (int t = 0; t < ntile; t++) {
         const int k0 = kbeg + t * TK;
         __syncthreads();
@@ -357,18 +414,8 @@ diff_fwd_kernel(DiffArgs g) {
         float vup = up_of(mv);
         if (t) vup = fminf(vup, down_of(vdown) * 0x1p60f);
         vdown = down_of(vup);
-        if (stager) {
-#pragma unroll
-            for (int i = 0; i < CH; i++) {
-                _Float16 *d = kt + (sr + i * Stage::RPP) * Tile::STRIDE + sc;
-                const Half2 hk = half_split(xk[i], kup), hv = half_split(xv[i], vup);
-                *(h8 *)d = hk.hi;
-                *(h8 *)(d + Tile::PART) = hk.lo;
-                *(h8 *)(d + Tile::HALVES) = hv.hi;
-                *(h8 *)(d + Tile::HALVES + Tile::PART) = hv.lo;
-            }
-        }
-        if (t + 1 < ntile) load(k0 + TK);
+        st.store(lds, kup, vup);
+        if (t + 1 < ntile) st.load(k0 + TK);
         __syncthreads();
         const bool any = g.causal ? k0 <= w_last + shift : true;
         if (any && w_first < nq) {
@@ -443,7 +490,7 @@ diff_fwd_kernel(DiffArgs g) {
                 for (int r = 0; r < 16; r++) o[c][r] = __builtin_fmaf(o[c][r], keep, a[r]);
             }
         }
-        if (t + 1 < ntile) maxima((t + 1) & 1);
+        if (t + 1 < ntile) st.maxima(tmax[(t + 1) & 1][0], tmax[(t + 1) & 1][1]);
     }
     l += __shfl_xor(l, 32, 64);
     const bool some = live && l > 0.f;
@@ -583,13 +630,20 @@ __global__ __launch_bounds__(256) void diff_join_kernel(DiffArgs g, int splits) 
     if (g.stats && lane == 0) *(float4 *)(g.stats + w * 4) = make_float4(st[0], st[1], st[2], st[3]);
 }
 
-// dO and D_1, D_2 of the rows [blk rpb, (blk + 1) rpb) of tokens, and the
-// block's partials of dgain and dlambda.
+// Backward's first pass: dO, D_1 and D_2 of the rows [blk rpb, (blk + 1) rpb) of
+// tokens, and the block's partials of dgain and dlambda.  One wave per (row,
+// head), lane c on channels c and c + 64.  The dots are 64-bit sums: dO is
+// perpendicular to O, so that D_2, whose sum dlambda is, is small beside its
+// terms.
 __global__ __launch_bounds__(256) void diff_bwd_pre_kernel(DiffArgs g) {
     extern __shared__ double sh[];  // [4][2 dh + h]
     const int lane = threadIdx.x & 63, wv = wave_index(), dv = 2 * g.dh, cols = dv + g.h;
     double dg[2] = {0.0, 0.0};
     const int rows = g.n * g.tq, r0 = (int)blockIdx.x * g.rpb, r1 = min(rows, r0 + g.rpb);
+    float gain[2] = {0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+        if (g.gain && lane + 64 * u < dv) gain[u] = g.gain[lane + 64 * u] * (1.0f - g.lam_init);
     for (int hd = 0; hd < g.h; hd++) {
         double e1, e2;
         lambda_terms(g.lam, g.lam_heads, g.dh, hd, &e1, &e2);
@@ -599,7 +653,8 @@ __global__ __launch_bounds__(256) void diff_bwd_pre_kernel(DiffArgs g) {
             const long long w = (long long)row * g.h + hd;
             const int b = row / g.tq, i = row % g.tq;
             const bool live = i < len_of(g.qlen, b, g.tq);
-            float o1[2], o2[2], o[2], dy[2], t[2], ss = 0.f;
+            float o1[2], o2[2], o[2], dy[2], d[2], ss = 0.f;
+#pragma unroll
             for (int u = 0; u < 2; u++) {
                 const int c = lane + 64 * u;
                 const bool in = live && c < dv;
@@ -608,40 +663,46 @@ __global__ __launch_bounds__(256) void diff_bwd_pre_kernel(DiffArgs g) {
                 dy[u] = in ? g.dy[w * dv + c] : 0.f;
                 o[u] = o1[u] - lam * o2[u];
                 ss += o[u] * o[u];
+                d[u] = dy[u];
             }
-            float d[2];
             if (g.gain) {
                 const float r = 1.0f / sqrtf(wave_sum(ss) / (float)dv + g.eps);
                 float s = 0.f;
+#pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    const int c = lane + 64 * u;
                     o[u] *= r;
-                    t[u] = c < dv ? dy[u] * (g.gain[c] * (1.0f - g.lam_init)) : 0.f;
-                    s += t[u] * o[u];
+                    s += dy[u] * gain[u] * o[u];
                     dg[u] += (double)(dy[u] * o[u]);
                 }
                 s = wave_sum(s) / (float)dv;
-                for (int u = 0; u < 2; u++) d[u] = r * (t[u] - o[u] * s);
-            } else {
-                for (int u = 0; u < 2; u++) d[u] = dy[u];
+#pragma unroll
+                for (int u = 0; u < 2; u++) d[u] = r * (dy[u] * gain[u] - o[u] * s);
             }
-            float d1 = 0.f, d2 = 0.f;
+            double d1 = 0.0, d2 = 0.0;
+            float nd = 0.f;
+#pragma unroll
             for (int u = 0; u < 2; u++) {
                 const int c = lane + 64 * u;
                 if (c < dv) g.dout[w * dv + c] = d[u];
-                d1 += d[u] * o1[u];
-                d2 += d[u] * o2[u];
+                d1 += (double)d[u] * (double)o1[u];
+                d2 += (double)d[u] * (double)o2[u];
+                nd += d[u] * d[u];
             }
-            d1 = wave_sum(d1);
-            d2 = wave_sum(d2);
+            d1 = rnn_wave_sum_d(d1);
+            d2 = rnn_wave_sum_d(d2);
+            nd = sqrtf(wave_sum(nd));
             if (lane == 0) {
-                g.dd[w * 2] = d1;
-                g.dd[w * 2 + 1] = d2;
+                const float4 st = live ? *(const float4 *)(g.statsc + w * 4)
+                                       : make_float4(0.f, 0.f, 0.f, 0.f);
+                float4 *rec = (float4 *)(g.rec + w * 8);
+                rec[0] = st;
+                rec[1] = make_float4((float)d1, (float)d2, nd, lam);
             }
-            dl += (double)d2;
+            dl += d2;
         }
         if (lane == 0) sh[wv * cols + dv + hd] = -dl;
     }
+#pragma unroll
     for (int u = 0; u < 2; u++)
         if (lane + 64 * u < dv)
             sh[wv * cols + lane + 64 * u] = dg[u] * (double)(1.0f - g.lam_init);
@@ -716,122 +777,508 @@ __global__ __launch_bounds__(256) void diff_bwd_params_kernel(const double *__re
     }
 }
 
-// dQ of one (image, query, head) a wave.
-__global__ __launch_bounds__(256) void diff_dq_row_kernel(DiffArgs g) {
-    const int lane = threadIdx.x & 63;
-    const long long w = (long long)blockIdx.x * 4 + wave_index();
-    if (w >= (long long)g.n * g.tq * g.h) return;
-    const int hd = (int)(w % g.h);
-    const long long row = w / g.h;
-    const int i = (int)(row % g.tq), b = (int)(row / g.tq);
-    const Seen see(g, b);
-    const float *q = g.q + row * g.qstride + 2 * hd * g.dh;
-    const float *kv = g.kv + (long long)b * g.tk * g.kvstride;
-    const int kh = hd / g.group, dv = 2 * g.dh;
-    const float *k0 = kv + g.koff + 2 * kh * g.dh, *v0 = kv + g.voff + kh * dv;
-    const float4 st = *(const float4 *)(g.statsc + w * 4);
-    double e1, e2;
-    lambda_terms(g.lam, g.lam_heads, g.dh, hd, &e1, &e2);
-    const float lam = (float)(e1 - e2 + (double)g.lam_init);
-    const float d1 = g.dd[w * 2], d2 = g.dd[w * 2 + 1];
-    const float *dout = g.dout + w * dv;
-    float acc[2][1] = {{0.f}, {0.f}};
-    const int last = i < see.nq ? (g.causal ? min(see.nk, i + see.shift + 1) : see.nk) : 0;
-    for (int j0 = 0; j0 < last; j0 += 64) {
-        const int j = j0 + lane;
-        const bool in = see(i, j);
-        const long long off = (long long)min(j, see.nk - 1) * g.kvstride;
-        float s1 = 0.f, s2 = 0.f, da = 0.f;
-        for (int c = 0; c < g.dh; c++) {
-            s1 = __builtin_fmaf(q[c], k0[off + c], s1);
-            s2 = __builtin_fmaf(q[g.dh + c], k0[off + g.dh + c], s2);
-        }
-        for (int c = 0; c < dv; c++) da = __builtin_fmaf(dout[c], v0[off + c], da);
-        const float p1 = in ? exp2f(s1 * (g.scale * LOG2E) - st.x) * st.y : 0.f;
-        const float p2 = in ? exp2f(s2 * (g.scale * LOG2E) - st.z) * st.w : 0.f;
-        const float ds1 = in ? p1 * (da - d1) * g.scale : 0.f;
-        const float ds2 = in ? -lam * p2 * (da - d2) * g.scale : 0.f;
-        const int cnt = min(64, last - j0);
-        for (int t = 0; t < cnt; t++) {
-            const float a = __shfl(ds1, t, 64), c2 = __shfl(ds2, t, 64);
-            const float *kr = k0 + (long long)(j0 + t) * g.kvstride;
-            if (lane < g.dh && see(i, j0 + t)) {
-                acc[0][0] = __builtin_fmaf(a, kr[lane], acc[0][0]);
-                acc[1][0] = __builtin_fmaf(c2, kr[g.dh + lane], acc[1][0]);
-            }
-        }
-    }
-    float *dq = g.dq + row * g.qstride + 2 * hd * g.dh;
-    if (lane < g.dh)
-        for (int m = 0; m < 2; m++) {
-            float *p = dq + m * g.dh + lane;
-            *p = g.acc_q ? *p + acc[m][0] : acc[m][0];
-        }
+// A bound for 2 |dA| of rows with |dO| <= nd and values of magnitude <= vmax, and
+// the power of two that keeps dS below 2^15 under it.
+template <int W>
+__device__ __forceinline__ float ds_up(float nd, float vmax) {
+    constexpr float root = W == 32 ? 5.6568543f : W == 64 ? 8.0f : W == 96 ? 9.7979590f : 11.313709f;
+    return up_of(nd * (2.0f * root * vmax));
 }
 
-// dK and dV of one (image, key, key head) a wave.
-__global__ __launch_bounds__(256) void diff_dkv_row_kernel(DiffArgs g) {
-    const int lane = threadIdx.x & 63;
-    const long long w = (long long)blockIdx.x * 4 + wave_index();
-    if (w >= (long long)g.n * g.tk * g.hkv) return;
-    const int kh = (int)(w % g.hkv);
-    const long long row = w / g.hkv;
-    const int j = (int)(row % g.tk), b = (int)(row / g.tk);
-    const Seen see(g, b);
-    const int dv = 2 * g.dh;
-    const float *k = g.kv + row * g.kvstride + g.koff + 2 * kh * g.dh;
-    const float *v = g.kv + row * g.kvstride + g.voff + kh * dv;
-    float dk[2] = {0.f, 0.f}, dvv[2] = {0.f, 0.f};
-    const int from = g.causal ? max(0, j - see.shift) : 0, last = j < see.nk ? see.nq : 0;
-    for (int hd = kh * g.group; hd < (kh + 1) * g.group; hd++) {
-        double e1, e2;
-        lambda_terms(g.lam, g.lam_heads, g.dh, hd, &e1, &e2);
-        const float lam = (float)(e1 - e2 + (double)g.lam_init);
-        for (int i0 = from; i0 < last; i0 += 64) {
-            const int i = i0 + lane, ic = min(i, see.nq - 1);
-            const bool in = see(i, j);
-            const long long qr = (long long)b * g.tq + ic, wr = qr * g.h + hd;
-            const float *q = g.q + qr * g.qstride + 2 * hd * g.dh;
-            const float4 st = *(const float4 *)(g.statsc + wr * 4);
-            const float *dout = g.dout + wr * dv;
-            float s1 = 0.f, s2 = 0.f, da = 0.f;
-            for (int c = 0; c < g.dh; c++) {
-                s1 = __builtin_fmaf(q[c], k[c], s1);
-                s2 = __builtin_fmaf(q[g.dh + c], k[g.dh + c], s2);
+// dQ.  Rows and tiles as in the forward, a wave on both maps of its 32 rows:
+// S_m^T = K_m Q_m^T and dA^T = V dO^T (lane = row), dS_m in registers is the
+// operand of dQ_m^T = K_m^T dS_m^T.  Each tile's products are summed apart and
+// added to the gradient in fp32, which carries the tile's powers of two and
+// rounds to nearest (the matrix core's own sum cuts off).
+template <int DHP, bool VEC, int NW>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DHP <= 32 ? 2 : 1))) void
+diff_dq_kernel(DiffArgs g) {
+    constexpr int W = 2 * DHP, TK = 32, NT = 64 * NW, KS = DHP / 16, VS = W / 16;
+    constexpr int CT = (DHP + 31) / 32;
+    using Tile = HalfTile<TK, W>;
+    // (a map's last 32-channel tile may run past the row: into the padding)
+    __shared__ __align__(16) _Float16 lds[2 * Tile::HALVES + 32];
+    __shared__ float tmax[2][2][NW];
+    const int lane = threadIdx.x & 63, wave = wave_index(), lr = lane & 31, lh = lane >> 5;
+    const int R = g.tq * g.group, nrb = (R + 32 * NW - 1) / (32 * NW);
+    const long long id = xcd_order(blockIdx.x, gridDim.x);
+    const int prob = (int)(id / nrb), rb = nrb - 1 - (int)(id % nrb);
+    const int b = prob / g.hkv, kh = prob % g.hkv;
+    const int nq = len_of(g.qlen, b, g.tq), nk = len_of(g.klen, b, g.tk), shift = nk - nq;
+    const int row = rb * 32 * NW + wave * 32 + lr;
+    const int qi = row / g.group, head = kh * g.group + row % g.group;
+    const bool live = qi < nq;
+    const int last_q = min(nq - 1, (rb * 32 * NW + 32 * NW - 1) / g.group);
+    int kend = g.causal ? min(nk, last_q + shift + 1) : nk;
+    if (rb * 32 * NW / g.group >= nq) kend = 0;
+    const int ntile = kend > 0 ? (kend + TK - 1) / TK : 0;
+    KvStage<DHP, TK, NT, VEC> st(g, b, kh, kend);
+    if (ntile) st.load(0);
+
+    // the row's queries, its dO and what the first pass left of it
+    Half2 q[2][KS], d[VS];
+    float qdown[2], ddown, nd;
+    const long long qr = (long long)b * g.tq + min(qi, g.tq - 1);
+    const long long at = qr * g.h + head;
+    {
+        const float *qp = g.q + qr * g.qstride + 2 * head * g.dh;
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+            float v[KS][8], mx = 0.f;
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                const int c = 16 * s + 8 * lh;
+                load8g<VEC>(qp + m * g.dh + c, live ? g.dh - c : 0, v[s]);
+                mx = absmax8(v[s], mx);
             }
-            for (int c = 0; c < dv; c++) da = __builtin_fmaf(dout[c], v[c], da);
-            const float p1 = in ? exp2f(s1 * (g.scale * LOG2E) - st.x) * st.y : 0.f;
-            const float p2 = in ? exp2f(s2 * (g.scale * LOG2E) - st.z) * st.w : 0.f;
-            const float a = p1 - lam * p2;
-            const float ds1 = in ? p1 * (da - g.dd[wr * 2]) * g.scale : 0.f;
-            const float ds2 = in ? -lam * p2 * (da - g.dd[wr * 2 + 1]) * g.scale : 0.f;
-            const int cnt = min(64, last - i0);
-            for (int t = 0; t < cnt; t++) {
-                const float at = __shfl(a, t, 64), x1 = __shfl(ds1, t, 64), x2 = __shfl(ds2, t, 64);
-                const long long qt = (long long)b * g.tq + i0 + t;
-                const float *qq = g.q + qt * g.qstride + 2 * hd * g.dh;
-                const float *dd = g.dout + (qt * g.h + hd) * dv;
-                if (lane < g.dh) {
-                    dk[0] = __builtin_fmaf(x1, qq[lane], dk[0]);
-                    dk[1] = __builtin_fmaf(x2, qq[g.dh + lane], dk[1]);
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            const float up = up_of(mx);
+            qdown[m] = down_of(up) * (g.scale * LOG2E);
+#pragma unroll
+            for (int s = 0; s < KS; s++) q[m][s] = half_split(v[s], up);
+        }
+        float v[VS][8], mx = 0.f;
+#pragma unroll
+        for (int s = 0; s < VS; s++) {
+            const int c = 16 * s + 8 * lh;
+            load8g<VEC>(g.dout + at * 2 * g.dh + c, live ? 2 * g.dh - c : 0, v[s]);
+            mx = absmax8(v[s], mx);
+        }
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float up = up_of(mx);
+        ddown = down_of(up);
+#pragma unroll
+        for (int s = 0; s < VS; s++) d[s] = half_split(v[s], up);
+    }
+    float4 sm4 = make_float4(0.f, 0.f, 0.f, 0.f), dd4 = sm4;
+    if (live) {
+        sm4 = *(const float4 *)(g.rec + at * 8);
+        dd4 = *(const float4 *)(g.rec + at * 8 + 4);
+    }
+    nd = dd4.z;
+    f32x16 acc[2][CT];
+#pragma unroll
+    for (int m = 0; m < 2; m++)
+#pragma unroll
+        for (int c = 0; c < CT; c++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) acc[m][c][r] = 0.f;
+    const int w_first = (rb * 32 * NW + wave * 32) / g.group;
+    const int w_last = min(nq - 1, (rb * 32 * NW + wave * 32 + 31) / g.group);
+    if (ntile) st.maxima(tmax[0][0], tmax[0][1]);
+    const _Float16 *const kt = lds, *const vt = lds + Tile::HALVES;
+    for (int t = 0; t < ntile; t++) {
+        const int k0 = t * TK;
+        __syncthreads();
+        float mk = 0.f, mv = 0.f;
+#pragma unroll
+        for (int i = 0; i < NW; i++) {
+            mk = fmaxf(mk, tmax[t & 1][0][i]);
+            mv = fmaxf(mv, tmax[t & 1][1][i]);
+        }
+        const float kup = up_of(mk), vup = up_of(mv);
+        st.store(lds, kup, vup);
+        if (t + 1 < ntile) st.load(k0 + TK);
+        __syncthreads();
+        if (w_first < nq && !(g.causal && k0 > w_last + shift)) {
+            const bool whole = k0 + TK <= nk && !(g.causal && k0 + TK - 1 > w_first + shift) &&
+                               !(g.diag && k0 <= w_last && w_first < k0 + TK);
+            const float kdown = down_of(kup);
+            const float dup = ds_up<W>(nd, mv), fd = down_of(vup) * ddown * dup;
+            f32x16 da;
+            {
+                f32x16 hh, sm;
+#pragma unroll
+                for (int r = 0; r < 16; r++) hh[r] = sm[r] = 0.f;
+#pragma unroll
+                for (int s = 0; s < VS; s++) {
+                    const h8 hi = Tile::along(vt, lr, 16 * s + 8 * lh);
+                    const h8 lo = Tile::along(vt + Tile::PART, lr, 16 * s + 8 * lh);
+                    sm = mm(hi, d[s].lo, sm);
+                    hh = mm(hi, d[s].hi, hh);
+                    sm = mm(lo, d[s].hi, sm);
                 }
-                for (int u = 0; u < 2; u++)
-                    if (lane + 64 * u < dv) dvv[u] = __builtin_fmaf(at, dd[lane + 64 * u], dvv[u]);
+#pragma unroll
+                for (int r = 0; r < 16; r++) da[r] = (hh[r] + sm[r]) * fd;
+            }
+#pragma unroll
+            for (int m = 0; m < 2; m++) {
+                f32x16 hh, sm;
+#pragma unroll
+                for (int r = 0; r < 16; r++) hh[r] = sm[r] = 0.f;
+#pragma unroll
+                for (int s = 0; s < KS; s++) {
+                    const int c = m * DHP + 16 * s + 8 * lh;
+                    const h8 hi = Tile::along(kt, lr, c);
+                    const h8 lo = Tile::along(kt + Tile::PART, lr, c);
+                    sm = mm(hi, q[m][s].lo, sm);
+                    hh = mm(hi, q[m][s].hi, hh);
+                    sm = mm(lo, q[m][s].hi, sm);
+                }
+                const float f = kdown * qdown[m], mx = m ? sm4.z : sm4.x, il = m ? sm4.w : sm4.y;
+                const float D = (m ? dd4.y : dd4.x) * dup;
+                Half2 ds[2];
+#pragma unroll
+                for (int s = 0; s < 2; s++) {
+                    float e[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int r = 8 * s + i;
+                        float p = __builtin_amdgcn_exp2f((hh[r] + sm[r]) * f - mx) * il;
+                        if (!whole) {
+                            const int j = k0 + 8 * (r >> 2) + 4 * lh + (r & 3);
+                            const bool in = j < nk && !(g.causal && j > qi + shift) &&
+                                            !(g.diag && j == qi);
+                            p = in ? p : 0.f;
+                        }
+                        e[i] = p * (da[r] - D);
+                    }
+                    ds[s] = half_split(e, 1.0f);
+                }
+                const float back = kdown * down_of(dup);
+#pragma unroll
+                for (int c = 0; c < CT; c++) {
+                    f32x16 a;
+#pragma unroll
+                    for (int r = 0; r < 16; r++) a[r] = 0.f;
+#pragma unroll
+                    for (int s = 0; s < 2; s++) {
+                        const h8 hi = Tile::across(kt, 16 * s, m * DHP + 32 * c);
+                        const h8 lo = Tile::across(kt + Tile::PART, 16 * s, m * DHP + 32 * c);
+                        a = mm(lo, ds[s].hi, a);
+                        a = mm(hi, ds[s].lo, a);
+                        a = mm(hi, ds[s].hi, a);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 16; r++)
+                        acc[m][c][r] = __builtin_fmaf(a[r], back, acc[m][c][r]);
+                }
             }
         }
+        if (t + 1 < ntile) st.maxima(tmax[(t + 1) & 1][0], tmax[(t + 1) & 1][1]);
     }
-    float *dkp = g.dkv + row * g.kvstride + g.koff + 2 * kh * g.dh;
-    float *dvp = g.dkv + row * g.kvstride + g.voff + kh * dv;
-    for (int u = 0; u < 2; u++) {
-        if (lane < g.dh) {
-            float *p = dkp + u * g.dh + lane;
-            *p = g.acc_kv ? *p + dk[u] : dk[u];
-        }
-        if (lane + 64 * u < dv) {
-            float *p = dvp + lane + 64 * u;
-            *p = g.acc_kv ? *p + dvv[u] : dvv[u];
-        }
+    if (row >= R) return;
+    float *dst = g.dq + qr * g.qstride + 2 * head * g.dh;
+#pragma unroll
+    for (int m = 0; m < 2; m++) {
+        const float f = m ? -dd4.w * g.scale : g.scale;
+#pragma unroll
+        for (int c = 0; c < CT; c++)
+            put_channels<VEC>(dst + m * g.dh, g.dh, 32 * c, acc[m][c], f, live, g.acc_q);
     }
+}
+
+// dK and dV.  One workgroup of NW waves per (image, key head, 32 NW keys), wave
+// w on 32 of them: its keys' and values' parts stay in registers.  Tiles of 32
+// rows (queries of the head group) are split into LDS with their records:
+// S_m = Q_m K_m^T and dA = dO V^T (lane = key), and P and dS in registers are
+// the operands of dV^T = dO^T (P_1 - lambda P_2) and dK_m^T = Q_m^T dS_m.
+template <int DHP, bool VEC, int NW>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DHP <= 16 ? 2 : 1))) void
+diff_dkv_kernel(DiffArgs g) {
+    constexpr int W = 2 * DHP, TR = 32, NT = 64 * NW, KS = DHP / 16, VS = W / 16;
+    constexpr int CT = (DHP + 31) / 32, VT = DHP / 16;
+    using Tile = HalfTile<TR, W>;
+    using Stage = StagePlan<TR, W, NT>;
+    constexpr int CH = Stage::PASSES;
+    __shared__ __align__(16) _Float16 lds[2 * Tile::HALVES + 32];
+    __shared__ __align__(16) float rec[7][TR];  // m1, il1, m2, il2, D1, D2, lambda
+    __shared__ float tmax[2][4][NW];  // largest |q|, |dO|, |dO|_2, |lambda|
+    const int lane = threadIdx.x & 63, wave = wave_index(), lr = lane & 31, lh = lane >> 5;
+    const int nkb = (g.tk + 32 * NW - 1) / (32 * NW);
+    const long long id = xcd_order(blockIdx.x, gridDim.x);
+    const int prob = (int)(id / nkb), kb = (int)(id % nkb);
+    const int b = prob / g.hkv, kh = prob % g.hkv;
+    const int nq = len_of(g.qlen, b, g.tq), nk = len_of(g.klen, b, g.tk), shift = nk - nq;
+    const int w_first = kb * 32 * NW + wave * 32, key = w_first + lr;
+    const bool live = key < nk;
+    // rows that see some key of the block
+    const int first_q = g.causal ? max(0, kb * 32 * NW - shift) : 0;
+    const int row_end = kb * 32 * NW < nk ? nq * g.group : 0;
+    const int row_beg = min(first_q, nq) * g.group;
+    const int ntile = row_end > row_beg ? (row_end - row_beg + TR - 1) / TR : 0;
+    const float ginv = 1.0f / (float)g.group;
+
+    float xq[CH][8], xd[CH][8];
+    float4 r0 = make_float4(0.f, 0.f, 0.f, 0.f), r1 = r0;
+    const int sc = (int)threadIdx.x % Stage::C8 * 8, sr = (int)threadIdx.x / Stage::C8;
+    const bool stager = Stage::ALL || sr < Stage::RPP;
+    const int run = sc >= DHP ? 1 : 0;
+    const float *qimg = g.q + (long long)b * g.tq * g.qstride + 2 * kh * g.group * g.dh;
+    const float *dimg = g.dout + ((long long)b * g.tq * g.h + kh * g.group) * 2 * g.dh;
+    auto load = [&](int row0) {
+        // rows of a tile lie in queries [q0, q0 + 32]; row x of the tile is
+        // query q0 + (x0 + x) / group (x0 + x < 32 + group, exact in floats)
+        const int q0 = row0 / g.group, x0 = row0 - q0 * g.group;
+        const float *qb = qimg + q0 * g.qstride;
+        const float *db = dimg + (long long)q0 * g.h * 2 * g.dh;
+#pragma unroll
+        for (int i = 0; i < CH; i++) {
+            const int x = sr + i * Stage::RPP;
+            const int dq = (int)(((float)(x0 + x) + 0.5f) * ginv), hd = x0 + x - dq * g.group;
+            const bool in = stager && row0 + x < row_end;
+            load8g<VEC>(qb + dq * g.qstride + (2 * hd + run) * g.dh + sc - run * DHP,
+                        in ? g.dh - (sc - run * DHP) : 0, xq[i]);
+            load8g<VEC>(db + ((long long)dq * g.h + hd) * 2 * g.dh + sc, in ? 2 * g.dh - sc : 0,
+                        xd[i]);
+        }
+        if (threadIdx.x < TR) {
+            const int x = (int)threadIdx.x;
+            const int dq = (int)(((float)(x0 + x) + 0.5f) * ginv), hd = x0 + x - dq * g.group;
+            r0 = r1 = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (row0 + x < row_end) {
+                const float *rp = g.rec + (((long long)b * g.tq + q0 + dq) * g.h + kh * g.group + hd) * 8;
+                r0 = *(const float4 *)rp;
+                r1 = *(const float4 *)(rp + 4);
+            }
+        }
+    };
+    auto maxima = [&](int slot) {
+        float mq = 0.f, md = 0.f;
+#pragma unroll
+        for (int i = 0; i < CH; i++) {
+            mq = absmax8(xq[i], mq);
+            md = absmax8(xd[i], md);
+        }
+        mq = wave_max(mq);
+        md = wave_max(md);
+        const float mn = wave_max(r1.z), ml = wave_max(fabsf(r1.w));
+        if (lane == 0) {
+            tmax[slot][0][wave] = mq;
+            tmax[slot][1][wave] = md;
+            tmax[slot][2][wave] = mn;
+            tmax[slot][3][wave] = ml;
+        }
+    };
+    if (ntile) load(row_beg);
+
+    // the lane's key and value
+    Half2 k[2][KS], v[VS];
+    float kdown[2], vdown, vmax;
+    const long long krow = (long long)b * g.tk + min(key, g.tk - 1);
+    {
+        const float *kp = g.kv + krow * g.kvstride + g.koff + 2 * kh * g.dh;
+        const float *vp = g.kv + krow * g.kvstride + g.voff + 2 * kh * g.dh;
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+            float x[KS][8], mx = 0.f;
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                const int c = 16 * s + 8 * lh;
+                load8g<VEC>(kp + m * g.dh + c, live ? g.dh - c : 0, x[s]);
+                mx = absmax8(x[s], mx);
+            }
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            const float up = up_of(mx);
+            kdown[m] = down_of(up) * (g.scale * LOG2E);
+#pragma unroll
+            for (int s = 0; s < KS; s++) k[m][s] = half_split(x[s], up);
+        }
+        float x[VS][8];
+        vmax = 0.f;
+#pragma unroll
+        for (int s = 0; s < VS; s++) {
+            const int c = 16 * s + 8 * lh;
+            load8g<VEC>(vp + c, live ? 2 * g.dh - c : 0, x[s]);
+            vmax = absmax8(x[s], vmax);
+        }
+        vmax = fmaxf(vmax, __shfl_xor(vmax, 32, 64));
+        const float up = up_of(vmax);
+        vdown = down_of(up);
+#pragma unroll
+        for (int s = 0; s < VS; s++) v[s] = half_split(x[s], up);
+    }
+    f32x16 dk[2][CT], dv[VT];
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+#pragma unroll
+            for (int c = 0; c < CT; c++) dk[m][c][r] = 0.f;
+#pragma unroll
+        for (int c = 0; c < VT; c++) dv[c][r] = 0.f;
+    }
+    if (ntile) maxima(0);
+    const _Float16 *const qt = lds, *const dt = lds + Tile::HALVES;
+    for (int t = 0; t < ntile; t++) {
+        const int row0 = row_beg + t * TR;
+        __syncthreads();
+        float mq = 0.f, md = 0.f, mn = 0.f, ml = 0.f;
+#pragma unroll
+        for (int i = 0; i < NW; i++) {
+            mq = fmaxf(mq, tmax[t & 1][0][i]);
+            md = fmaxf(md, tmax[t & 1][1][i]);
+            mn = fmaxf(mn, tmax[t & 1][2][i]);
+            ml = fmaxf(ml, tmax[t & 1][3][i]);
+        }
+        const float qup = up_of(mq), dup = up_of(md);
+        if (stager) {
+#pragma unroll
+            for (int i = 0; i < CH; i++) {
+                _Float16 *p = lds + (sr + i * Stage::RPP) * Tile::STRIDE + sc;
+                const Half2 hq = half_split(xq[i], qup), hd = half_split(xd[i], dup);
+                *(h8 *)p = hq.hi;
+                *(h8 *)(p + Tile::PART) = hq.lo;
+                *(h8 *)(p + Tile::HALVES) = hd.hi;
+                *(h8 *)(p + Tile::HALVES + Tile::PART) = hd.lo;
+            }
+        }
+        if (threadIdx.x < TR) {
+            rec[0][threadIdx.x] = r0.x;
+            rec[1][threadIdx.x] = r0.y;
+            rec[2][threadIdx.x] = r0.z;
+            rec[3][threadIdx.x] = r0.w;
+            rec[4][threadIdx.x] = r1.x;
+            rec[5][threadIdx.x] = r1.y;
+            rec[6][threadIdx.x] = r1.w;
+        }
+        if (t + 1 < ntile) load(row0 + TR);
+        __syncthreads();
+        const int tq0 = row0 / g.group, tq1 = min(nq - 1, (row0 + TR - 1) / g.group);
+        if (w_first < nk && !(g.causal && w_first > tq1 + shift)) {
+            // rows past the last carry il = 0, keys past the last are not stored
+            const bool whole = !(g.causal && w_first + 31 > tq0 + shift) &&
+                               !(g.diag && w_first <= tq1 && tq0 <= w_first + 31);
+            const int x0 = row0 - tq0 * g.group;
+            const float qd = down_of(qup), dd = down_of(dup);
+            const float up = ds_up<W>(mn, vmax), fd = vdown * dd * up;
+            const float lup = up_of(ml) * 0x1p-15f;  // takes lambda below 1
+            float p1[16], p2[16], da[16];
+            {
+                f32x16 hh, sm;
+#pragma unroll
+                for (int r = 0; r < 16; r++) hh[r] = sm[r] = 0.f;
+#pragma unroll
+                for (int s = 0; s < VS; s++) {
+                    const h8 hi = Tile::along(dt, lr, 16 * s + 8 * lh);
+                    const h8 lo = Tile::along(dt + Tile::PART, lr, 16 * s + 8 * lh);
+                    sm = mm(hi, v[s].lo, sm);
+                    hh = mm(hi, v[s].hi, hh);
+                    sm = mm(lo, v[s].hi, sm);
+                }
+#pragma unroll
+                for (int r = 0; r < 16; r++) da[r] = (hh[r] + sm[r]) * fd;
+            }
+#pragma unroll
+            for (int m = 0; m < 2; m++) {
+                f32x16 hh, sm;
+#pragma unroll
+                for (int r = 0; r < 16; r++) hh[r] = sm[r] = 0.f;
+#pragma unroll
+                for (int s = 0; s < KS; s++) {
+                    const int c = m * DHP + 16 * s + 8 * lh;
+                    const h8 hi = Tile::along(qt, lr, c);
+                    const h8 lo = Tile::along(qt + Tile::PART, lr, c);
+                    sm = mm(hi, k[m][s].lo, sm);
+                    hh = mm(hi, k[m][s].hi, hh);
+                    sm = mm(lo, k[m][s].hi, sm);
+                }
+                const float f = qd * kdown[m];
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    const float4 mx = *(const float4 *)&rec[2 * m][2 * r + 4 * lh];
+                    const float4 il = *(const float4 *)&rec[2 * m + 1][2 * r + 4 * lh];
+                    const float mxv[4] = {mx.x, mx.y, mx.z, mx.w}, ilv[4] = {il.x, il.y, il.z, il.w};
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        float p = __builtin_amdgcn_exp2f((hh[r + e] + sm[r + e]) * f - mxv[e]) * ilv[e];
+                        if (!whole) {
+                            const int i = tq0 + (int)(((float)(x0 + 2 * r + 4 * lh + e) + 0.5f) * ginv);
+                            const bool in = !(g.causal && key > i + shift) && !(g.diag && key == i);
+                            p = in ? p : 0.f;
+                        }
+                        (m ? p2 : p1)[r + e] = p;
+                    }
+                }
+            }
+            // dV: (P_1 - lambda P_2) times a power of two that no lambda passes
+            const float aup = up_of(1.0f + ml), adown = down_of(aup) * dd;
+            {
+                Half2 a[2];
+#pragma unroll
+                for (int s = 0; s < 2; s++) {
+                    float e[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i += 4) {
+                        const float4 lv = *(const float4 *)&rec[6][2 * (8 * s + i) + 4 * lh];
+                        const float l4[4] = {lv.x, lv.y, lv.z, lv.w};
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            e[i + j] = p1[8 * s + i + j] - l4[j] * p2[8 * s + i + j];
+                    }
+                    a[s] = half_split(e, aup);
+                }
+#pragma unroll
+                for (int c = 0; c < VT; c++) {
+                    f32x16 x;
+#pragma unroll
+                    for (int r = 0; r < 16; r++) x[r] = 0.f;
+#pragma unroll
+                    for (int s = 0; s < 2; s++) {
+                        const h8 hi = Tile::across(dt, 16 * s, 32 * c);
+                        const h8 lo = Tile::across(dt + Tile::PART, 16 * s, 32 * c);
+                        x = mm(lo, a[s].hi, x);
+                        x = mm(hi, a[s].lo, x);
+                        x = mm(hi, a[s].hi, x);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 16; r++) dv[c][r] = __builtin_fmaf(x[r], adown, dv[c][r]);
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < 2; m++) {
+                Half2 ds[2];
+#pragma unroll
+                for (int s = 0; s < 2; s++) {
+                    float e[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i += 4) {
+                        const float4 Dv = *(const float4 *)&rec[4 + m][2 * (8 * s + i) + 4 * lh];
+                        const float4 lv = *(const float4 *)&rec[6][2 * (8 * s + i) + 4 * lh];
+                        const float D4[4] = {Dv.x, Dv.y, Dv.z, Dv.w}, l4[4] = {lv.x, lv.y, lv.z, lv.w};
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const int r = 8 * s + i + j;
+                            const float x = (m ? p2 : p1)[r] * (da[r] - D4[j] * up);
+                            e[i + j] = m ? x * l4[j] : x;
+                        }
+                    }
+                    ds[s] = half_split(e, m ? lup : 1.0f);
+                }
+                const float back = (m ? down_of(lup) : 1.0f) * qd * down_of(up);
+#pragma unroll
+                for (int c = 0; c < CT; c++) {
+                    f32x16 a;
+#pragma unroll
+                    for (int r = 0; r < 16; r++) a[r] = 0.f;
+#pragma unroll
+                    for (int s = 0; s < 2; s++) {
+                        const h8 hi = Tile::across(qt, 16 * s, m * DHP + 32 * c);
+                        const h8 lo = Tile::across(qt + Tile::PART, 16 * s, m * DHP + 32 * c);
+                        a = mm(lo, ds[s].hi, a);
+                        a = mm(hi, ds[s].lo, a);
+                        a = mm(hi, ds[s].hi, a);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 16; r++)
+                        dk[m][c][r] = __builtin_fmaf(a[r], back, dk[m][c][r]);
+                }
+            }
+        }
+        if (t + 1 < ntile) maxima((t + 1) & 1);
+    }
+    if (key >= g.tk) return;
+    float *kd = g.dkv + krow * g.kvstride + g.koff + 2 * kh * g.dh;
+    float *vd = g.dkv + krow * g.kvstride + g.voff + 2 * kh * g.dh;
+#pragma unroll
+    for (int m = 0; m < 2; m++)
+#pragma unroll
+        for (int c = 0; c < CT; c++)
+            put_channels<VEC>(kd + m * g.dh, g.dh, 32 * c, dk[m][c], m ? -g.scale : g.scale, live,
+                              g.acc_kv);
+#pragma unroll
+    for (int c = 0; c < VT; c++)
+        put_channels<VEC>(vd, 2 * g.dh, 32 * c, dv[c], 1.0f, live, g.acc_kv);
 }
 
 // Token rows of a block of the backward's first pass, and its blocks: at most
@@ -859,7 +1306,7 @@ FwdPlan plan_fwd(const rnn_diff_attn_desc *d, size_t n, bool vec) {
 }
 
 struct DiffWs {
-    size_t part32 = 0, pstat = 0, dout = 0, dd = 0, part = 0, bytes = 0;
+    size_t part32 = 0, pstat = 0, dout = 0, rec = 0, part = 0, bytes = 0;
 };
 
 DiffWs plan_ws(const rnn_diff_attn_desc *d, size_t n, bool backward) {
@@ -868,7 +1315,7 @@ DiffWs plan_ws(const rnn_diff_attn_desc *d, size_t n, bool backward) {
     const size_t rows = n * d->tq, heads = rows * d->h;
     if (backward) {
         w.dout = cv.take(heads * 2 * d->dh * sizeof(float));
-        w.dd = cv.take(heads * 2 * sizeof(float));
+        w.rec = cv.take(heads * 8 * sizeof(float));
         const size_t nblk = rows ? rnn_div_up(rows, (size_t)pre_rows(rows)) : 0;
         w.part = cv.take(nblk * (2 * d->dh + d->h) * sizeof(double));
     } else {
@@ -968,6 +1415,46 @@ void launch_fwd(rnn_ctx *ctx, const DiffArgs &g, const FwdPlan &p, bool vec) {
         launch_fwd_qg<DHP, true, 4>(ctx, g, p);
 }
 
+// Waves of a workgroup by the rows (or keys) that there are: 32 each, up to four.
+int waves_of(size_t rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : 4; }
+
+template <int DHP, bool VEC, int NW>
+void launch_dq(rnn_ctx *ctx, const DiffArgs &g) {
+    const size_t R = (size_t)g.tq * g.group;
+    const unsigned grid = (unsigned)((size_t)g.n * g.hkv * rnn_div_up(R, 32 * NW));
+    diff_dq_kernel<DHP, VEC, NW><<<grid, 64 * NW, 0, ctx->stream>>>(g);
+}
+template <int DHP, bool VEC, int NW>
+void launch_dkv(rnn_ctx *ctx, const DiffArgs &g) {
+    const unsigned grid = (unsigned)((size_t)g.n * g.hkv * rnn_div_up((size_t)g.tk, 32 * NW));
+    diff_dkv_kernel<DHP, VEC, NW><<<grid, 64 * NW, 0, ctx->stream>>>(g);
+}
+template <int DHP>
+void launch_bwd(rnn_ctx *ctx, const DiffArgs &g, bool vec) {
+    if (g.tq) {
+        const int nw = waves_of((size_t)g.tq * g.group);
+        if (!vec)
+            launch_dq<DHP, false, 4>(ctx, g);
+        else if (nw == 1)
+            launch_dq<DHP, true, 1>(ctx, g);
+        else if (nw == 2)
+            launch_dq<DHP, true, 2>(ctx, g);
+        else
+            launch_dq<DHP, true, 4>(ctx, g);
+    }
+    if (g.tk) {
+        const int nw = waves_of((size_t)g.tk);
+        if (!vec)
+            launch_dkv<DHP, false, 4>(ctx, g);
+        else if (nw == 1)
+            launch_dkv<DHP, true, 1>(ctx, g);
+        else if (nw == 2)
+            launch_dkv<DHP, true, 2>(ctx, g);
+        else
+            launch_dkv<DHP, true, 4>(ctx, g);
+    }
+}
+
 int check_ws(rnn_ctx *ctx, const DiffWs &w, const void *ws, size_t ws_bytes) {
     if (!w.bytes) return RNN_OK;
     if (!ws) return rnn_fail(ctx, RNN_E_NULL, "diff_attn: workspace is null");
@@ -1064,7 +1551,7 @@ int rnn_diff_attn_backward(rnn_ctx *ctx, const rnn_diff_attn_desc *d, size_t n, 
     g.dq = dq ? dq + d->qoff : nullptr;
     g.dkv = dkv;
     g.dout = (float *)((char *)ws + w.dout);
-    g.dd = (float *)((char *)ws + w.dd);
+    g.rec = (float *)((char *)ws + w.rec);
     g.part = (double *)((char *)ws + w.part);
     g.acc_q = (flags & RNN_ATTN_SET_DQ) ? 0 : 1;
     g.acc_kv = (flags & RNN_ATTN_SET_DKV) ? 0 : 1;
@@ -1079,13 +1566,15 @@ int rnn_diff_attn_backward(rnn_ctx *ctx, const rnn_diff_attn_desc *d, size_t n, 
                                  ctx->stream>>>(g.part, (int)nblk, lam, g.lam_heads, g.dh, g.h,
                                                 dlam, dgain);
         RNN_LAUNCHED(ctx);
-        diff_dq_row_kernel<<<(unsigned)rnn_div_up(rows * d->h, 4), 256, 0, ctx->stream>>>(g);
-        RNN_LAUNCHED(ctx);
     }
-    if (d->tk) {
-        diff_dkv_row_kernel<<<(unsigned)rnn_div_up(n * d->tk * d->hkv, 4), 256, 0, ctx->stream>>>(g);
-        RNN_LAUNCHED(ctx);
+    const bool vec = rows_vec(g);
+    switch ((g.dh + 15) / 16) {
+        case 1: launch_bwd<16>(ctx, g, vec); break;
+        case 2: launch_bwd<32>(ctx, g, vec); break;
+        case 3: launch_bwd<48>(ctx, g, vec); break;
+        default: launch_bwd<64>(ctx, g, vec); break;
     }
+    RNN_LAUNCHED(ctx);
     return RNN_OK;
 }
 
