@@ -59,7 +59,11 @@ def rustvit_config_hash(cfg, nclass, ncoarse, use_exits, parent):
     parent = [int(p) for p in parent]
     fields.append(len(parent))
     fields += parent
-    return config_hash(b"rustvit", fields)
+    kind = b"rustvit"
+    # blocks that the reference does not have: a configuration of its own
+    if (cfg.get("attn", "lsa"), cfg.get("mlp", "swiglu")) != ("lsa", "swiglu"):
+        kind += f":{cfg.get('attn', 'lsa')}:{cfg.get('mlp', 'swiglu')}".encode()
+    return config_hash(kind, fields)
 
 
 def save(path, tensors, chash):

@@ -1,4 +1,4 @@
-"""norm.rs on the device: LayerNorm, LayerScale, SwiGlu, DwConv3, SeqPool.
+"""norm.rs on the device: LayerNorm, LayerScale, SwiGlu, DwConv3, SeqPool; Mlp.
 
 Mirrors the reference's layer interface (norm.rs:17-586) over token tensors:
 float32 CUDA tensors of shape [n, t, c] (tok.rs ``Tok``, channel fastest).
@@ -9,7 +9,8 @@ librnn.so; there is no CPU fallback.
 """
 from __future__ import annotations
 
-from . import RNN_DW3_ACC_DX, Linear, _ptr, default_ctx, lib
+from . import (RNN_DW3_ACC_DX, Linear, _act_code, _ptr, default_ctx, lib, linear_act_backward,
+               linear_act_forward)
 from .optim import Param
 
 
@@ -185,6 +186,45 @@ class SwiGlu:
                                                  _ptr(self.ab, rows * 2 * h, "ab"),
                                                  _ptr(dab, rows * 2 * h, "dab")))
         return self.wg.backward(dab).view(dy.shape)
+
+    def for_each_param(self, f):
+        for p in self._params:
+            f(p)
+
+
+class Mlp:
+    """Linear(c, h) with an activation -> Linear(h, c): the plain MLP beside
+    SwiGlu, in its interface (no counterpart in the reference).  act: one of
+    ``rustnn_amd.ACTS``; w1 / w2 take the given weights (or 0.02 normals)."""
+
+    def __init__(self, c, h, act="gelu", w1=None, b1=None, w2=None, b2=None, device=0, ctx=None):
+        _act_code(act)
+        self.c, self.h, self.act = c, h, act
+        self.ctx = ctx or default_ctx(device)
+        self.up = Linear(c, h, True, w1, b1, device, self.ctx)
+        self.down = Linear(h, c, True, w2, b2, device, self.ctx)
+        self._params = _linear_param(self.up) + _linear_param(self.down)
+        self.x = self.z = None
+        self.rows = 0
+
+    def forward(self, x, train, residual=None):
+        """residual = (out, l, mask, rows per image): the second product also
+        adds out += (y l) mask[image] (Linear.forward)."""
+        rows, c = _rows_c(x)
+        if c != self.c:
+            raise ValueError(f"Mlp: {c} channels, the layer has {self.c}")
+        up = self.up
+        u, z = linear_act_forward(rows, c, self.h, x, up.w, up.b, self.act, train=train,
+                                  ctx=self.ctx)
+        if train:
+            self.x, self.z, self.rows = x, z, rows
+        return self.down.forward(u.view(-1), rows, train, residual).view(x.shape)
+
+    def backward(self, dy):
+        up = self.up
+        du = self.down.backward(dy.reshape(-1))
+        return linear_act_backward(self.rows, self.c, self.h, du, self.x, up.w, self.z, self.act,
+                                   up.gw, up.gb, ctx=self.ctx).view(dy.shape)
 
     def for_each_param(self, f):
         for p in self._params:

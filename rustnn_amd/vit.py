@@ -1,5 +1,5 @@
 """vit.rs / attn.rs call sites on the device: SelfAttn, CrossAttn, DropPath,
-the pre-LN Block, token merge, TaxoHead and Exit.
+DiffSelfAttn (differential attention with rotary positions), the pre-LN Block, token merge, TaxoHead and Exit.
 
 Mirrors the reference's layer interface (attn.rs:346-560, vit.rs:25-353)
 over token tensors [n, t, c] (float32 CUDA, channel fastest):
@@ -17,9 +17,10 @@ from __future__ import annotations
 
 import numpy as np
 
-from . import Core, Linear, _ptr, default_ctx, lib, linear_backward, linear_forward, rel_index
+from . import (Core, DiffCore, Linear, Rotary, _ptr, default_ctx, lib, linear_backward,
+               linear_forward, rel_index)
 from .data import Rng
-from .norm import DwConv3, LayerNorm, LayerScale, SeqPool, SwiGlu, _linear_param
+from .norm import DwConv3, LayerNorm, LayerScale, Mlp, SeqPool, SwiGlu, _linear_param
 from .optim import Param
 
 
@@ -108,6 +109,69 @@ class SelfAttn:
             f(p)
         f(self.tau)
         f(self.rel)
+
+
+class DiffSelfAttn:
+    """Differential self-attention in SelfAttn's interface (no counterpart in
+    the reference): fused qkv Linear(c, 3c) -> rotary positions on the token
+    grid, in place on the queries and keys -> DiffCore of h heads with two maps
+    of c / 2h channels each -> proj Linear::scaled.  grid: the token grid's
+    sides, one to three of them (a time axis first); lambda's start is
+    0.8 - 0.6 exp(-0.3 (idx - 1)), idx the block's number from 1."""
+
+    def __init__(self, c, h, grid, depth, idx=1, rng=None, device=0, ctx=None, causal=False,
+                 base=100.0):
+        import torch
+        dev = f"cuda:{device}"
+        self.ctx = ctx or default_ctx(device)
+        rng = _rng(rng, 0)
+        if c % (4 * h):
+            raise ValueError(f"DiffSelfAttn: {c} channels are not {h} heads of two even maps")
+        self.c, self.h, self.dh = c, h, c // (2 * h)
+        self.rot = Rotary(4 * h, self.dh, grid, base, ctx=self.ctx)
+        self.t = self.rot.t
+        lam0 = 0.8 - 0.6 * float(np.exp(-0.3 * (int(idx) - 1)))
+        self.core = DiffCore(h, self.dh, self.t, self.t, causal=causal, lam_init=lam0,
+                             ctx=self.ctx)
+        self.qkv = _linear(c, 3 * c, True, 0.02, rng, dev, self.ctx)
+        self.proj = _linear(c, c, True, _scaled_std(depth), rng, dev, self.ctx)
+        self.lam = Param(_trunc_normal(4 * self.dh, 0.1, rng, dev), False)
+        self.gain = Param(torch.ones(2 * self.dh, device=dev), False)
+        self._lin = _linear_param(self.qkv) + _linear_param(self.proj)
+        self.ab = self.saved = None
+        self.n = 0
+
+    def _geo(self, ab):
+        c = self.c
+        return ab, 3 * c, 0, ab, 3 * c, c, 2 * c
+
+    def forward(self, x, train):
+        n, t, c = x.shape
+        ab = self.qkv.forward(x.reshape(-1), n * t, train)
+        self.rot.forward(n, ab, 3 * c, 0, y=ab)
+        o, saved = self.core.forward(n, *self._geo(ab), self.lam.v, self.gain.v, train=train)
+        y = self.proj.forward(o.view(-1), n * t, train)
+        if train:
+            self.ab, self.saved, self.n = ab, saved, n
+        return y.view(n, t, c)
+
+    def backward(self, dy, acc_dx=None):
+        """dx, or acc_dx += dx (returned) when given."""
+        import torch
+        n, t, c = self.n, self.t, self.c
+        do = self.proj.backward(dy.reshape(-1))
+        dab = torch.empty(n * t * 3 * c, device=dy.device)
+        self.core.backward(n, *self._geo(self.ab), self.lam.v, self.gain.v, self.saved, do, dab,
+                           dab, self.lam.g, self.gain.g, set_dq=True, set_dkv=True)
+        self.rot.backward(n, dab, 3 * c, 0, y=dab)
+        acc = acc_dx.reshape(-1) if acc_dx is not None else None
+        return self.qkv.backward(dab, acc_dx=acc).view(n, t, c)
+
+    def for_each_param(self, f):
+        for p in self._lin:
+            f(p)
+        f(self.lam)
+        f(self.gain)
 
 
 class CrossAttn:
@@ -259,12 +323,15 @@ def draw_masks(layers, n, device, ctx):
 class Block:
     """Block (vit.rs:76-250), pre-LN with three branches from one norm:
     h = LN(x); x += ls1 * dp1(SelfAttn(h) + gamma * DwConv3(h));
-    x += lsm * dp2(CrossAttn(h, mem)) (reader blocks); x += ls2 * dp3(SwiGlu(LN(x)))."""
+    x += lsm * dp2(CrossAttn(h, mem)) (reader blocks); x += ls2 * dp3(SwiGlu(LN(x))).
+    attn="diff": DiffSelfAttn in SelfAttn's place; mlp: "swiglu", or an
+    activation (one of rustnn_amd.ACTS) for an Mlp of 4c hidden channels."""
 
     def __init__(self, c, h, th, tw, mem, depth, drop, idx, ls_init, rng=None, device=0,
-                 ctx=None):
+                 ctx=None, attn="lsa", mlp="swiglu"):
         """Block::new (vit.rs:117-143): draws, in order, SelfAttn (qkv, proj),
-        DwConv3, CrossAttn (wq, proj) for a reader block, SwiGlu (wg, wd)."""
+        DwConv3, CrossAttn (wq, proj) for a reader block, SwiGlu (wg, wd).
+        DiffSelfAttn draws its lambda vectors after proj."""
         import torch
         dev = f"cuda:{device}"
         self.ctx = ctx or default_ctx(device)
@@ -272,7 +339,10 @@ class Block:
         self.c, self.idx = c, int(idx)
         hidden = -(-(4 * c // 3) // 16) * 16
         self.n1 = LayerNorm(c, device, self.ctx)
-        self.attn = SelfAttn(c, h, th, tw, depth, rng, device, self.ctx)
+        if attn not in ("lsa", "diff"):
+            raise ValueError(f"Block: attn {attn!r} (lsa or diff)")
+        self.attn = (SelfAttn(c, h, th, tw, depth, rng, device, self.ctx) if attn == "lsa" else
+                     DiffSelfAttn(c, h, (th, tw), depth, idx, rng, device, self.ctx))
         self.dw = DwConv3(c, th, tw, _trunc_normal(9 * c, 0.1, rng, dev), None, device, self.ctx)
         self.gamma = Param(torch.full((c,), 0.5, device=dev), False)
         self.ls1 = LayerScale(c, ls_init, device, self.ctx)
@@ -280,9 +350,11 @@ class Block:
                       if mem else None)
         self.lsm = LayerScale(c, ls_init, device, self.ctx) if mem else None
         self.n2 = LayerNorm(c, device, self.ctx)
-        wg = _trunc_normal(2 * hidden * c, 0.02, rng, dev)
-        wd = _trunc_normal(hidden * c, _scaled_std(depth), rng, dev)
-        self.mlp = SwiGlu(c, hidden, wg, None, wd, None, device, self.ctx)
+        wide = hidden if mlp == "swiglu" else 2 * c
+        wg = _trunc_normal(2 * wide * c, 0.02, rng, dev)
+        wd = _trunc_normal((wide if mlp == "swiglu" else 4 * c) * c, _scaled_std(depth), rng, dev)
+        self.mlp = (SwiGlu(c, hidden, wg, None, wd, None, device, self.ctx) if mlp == "swiglu" else
+                    Mlp(c, 4 * c, mlp, wg, None, wd, None, device, self.ctx))
         self.ls2 = LayerScale(c, ls_init, device, self.ctx)
         self.dp1, self.dp2, self.dp3 = (DropPath(drop, self.ctx), DropPath(drop, self.ctx),
                                         DropPath(drop, self.ctx))
@@ -586,7 +658,7 @@ class BasicBlock:
 
 
 VIT_DEFAULT = dict(width=32, cmid=96, dim=256, heads=4, depth3=5, dim4=384, heads4=6, depth4=2,
-                   mem_at=(1, 3), droppath=0.1, img=32)
+                   mem_at=(1, 3), droppath=0.1, img=32, attn="lsa", mlp="swiglu")
 
 
 class RustViT:
@@ -594,8 +666,9 @@ class RustViT:
     a 16x16 memory of 2*dim channels (1x1 conv + LayerNorm), 8x8 tokens
     (3x3/s2 conv + BN), depth3 Blocks (cross-attention readers at mem_at), a
     2x2 token merge to dim4, depth4 Blocks, LayerNorm + SeqPool + TaxoHead,
-    and two exits (GAP of the trunk; SeqPool of the stage-3 tokens).  parent:
-    the superclass of each fine class (CUDA int32); seed seeds the weights."""
+    and two exits (GAP of the trunk; SeqPool of the stage-3 tokens).  cfg's attn
+    and mlp are the Blocks' (the reference's: "lsa", "swiglu").  parent: the
+    superclass of each fine class (CUDA int32); seed seeds the weights."""
 
     def __init__(self, cfg=None, parent=None, ncoarse=20, seed=0, device=0, ctx=None):
         """RustViT::new (vit.rs:432-507): one Rng::new(seed) drawn in the
@@ -619,12 +692,12 @@ class RustViT:
         rate = lambda i: float(np.float32(cfg["droppath"]) * np.float32(i) / div)
         self.blocks3 = [Block(d, cfg["heads"], self.th, self.th,
                               (self.mh, self.mh) if i in cfg["mem_at"] else None, depth,
-                              rate(i), i + 1, 1e-4, rng, device, ctx)
+                              rate(i), i + 1, 1e-4, rng, device, ctx, cfg["attn"], cfg["mlp"])
                         for i in range(cfg["depth3"])]
         th4 = self.th // 2
         self.blocks4 = [Block(d4, cfg["heads4"], th4, th4, None, depth,
                               rate(cfg["depth3"] + i), cfg["depth3"] + i + 1, 1e-4, rng, device,
-                              ctx)
+                              ctx, cfg["attn"], cfg["mlp"])
                         for i in range(cfg["depth4"])]
         self.stem = _ConvBN(3, w, 3, 1, 1, rng, dev, device, ctx, relu=True)
         self.c1 = BasicBlock(w, w, 1, rng, dev, device, ctx)
