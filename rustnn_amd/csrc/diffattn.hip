@@ -51,24 +51,51 @@ __device__ __forceinline__ void lambda_terms(const float *lam, int lam_heads, in
     *e2 = exp(rnn_wave_sum_d(b));
 }
 
-__device__ __forceinline__ float wave_max(float v) {
-    for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    return v;
+// Maxima in one instruction each (fmaxf takes a second one to quiet NaNs).
+__device__ __forceinline__ float max2(float a, float b) {
+    float d;
+    asm("v_max_f32 %0, %1, %2" : "=v"(d) : "v"(a), "v"(b));
+    return d;
 }
-__device__ __forceinline__ float wave_sum(float v) {
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+    return d;
 }
-
-struct Seen {  // the keys that a query sees, and the queries that see a key
-    int nq, nk, shift, diag, causal;
-    __device__ Seen(const DiffArgs &g, int b)
-        : nq(len_of(g.qlen, b, g.tq)), nk(len_of(g.klen, b, g.tk)), shift(nk - nq), diag(g.diag),
-          causal(g.causal) {}
-    __device__ bool operator()(int i, int j) const {
-        return i < nq && j < nk && !(causal && j > i + shift) && !(diag && i == j);
-    }
-};
+__device__ __forceinline__ float max3abs(float a, float b, float c) {
+    float d;
+    asm("v_max3_f32 %0, %1, |%2|, |%3|" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+    return d;
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp_f(float v) {
+    return __uint_as_float(__builtin_amdgcn_mov_dpp((int)__float_as_uint(v), CTRL, 0xf, 0xf, false));
+}
+// Both lanes of each pair (l, l xor 32), or (l, l xor 16): f of the two values.
+template <typename F>
+__device__ __forceinline__ float pair32(float v, F f) {
+    const uint32_t u = __float_as_uint(v);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+template <typename F>
+__device__ __forceinline__ float pair16(float v, F f) {
+    const uint32_t u = __float_as_uint(v);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float add2(float a, float b) { return a + b; }
+// f over the 64 lanes, every lane receiving it, in a fixed tree.
+template <typename F>
+__device__ __forceinline__ float wave_all(float v, F f) {
+    v = f(v, dpp_f<0xB1>(v));
+    v = f(v, dpp_f<0x4E>(v));
+    v = f(v, dpp_f<0x141>(v));
+    v = f(v, dpp_f<0x140>(v));
+    return pair32(pair16(v, f), f);
+}
+__device__ __forceinline__ float wave_max(float v) { return wave_all(v, max2); }
+__device__ __forceinline__ float wave_sum(float v) { return wave_all(v, add2); }
 
 // ---------------------------------------------------------------------------
 // fp32 products on the fp16 matrix cores.
@@ -95,21 +122,51 @@ struct Half2 {
     h8 hi, lo;
 };
 
+// x - (the lower / upper half of h): the rest of a rounding, exact.
+__device__ __forceinline__ float rest_lo(uint32_t h, float x) {
+    float d;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(d) : "v"(h), "v"(x));
+    return d;
+}
+__device__ __forceinline__ float rest_hi(uint32_t h, float x) {
+    float d;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(d) : "v"(h), "v"(x));
+    return d;
+}
+// Two floats' parts, each pair in a register.
+__device__ __forceinline__ void half_pair(float a, float b, uint32_t &hi, uint32_t &lo) {
+    const f2 v = {a, b};
+    hi = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, h2));
+    const f2 d = {rest_lo(hi, a), rest_hi(hi, b)};
+    lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(d, h2));
+}
+
 // The two parts of 8 floats times up (a power of two).
 __device__ __forceinline__ Half2 half_split(const float (&x)[8], float up) {
-    Half2 r;
+    u32x4 hi, lo;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        const f2 v = {x[2 * j] * up, x[2 * j + 1] * up};
-        const h2 h = __builtin_convertvector(v, h2);
-        const f2 d = {v[0] - (float)h[0], v[1] - (float)h[1]};
-        const h2 l = __builtin_convertvector(d, h2);
-        r.hi[2 * j] = h[0];
-        r.hi[2 * j + 1] = h[1];
-        r.lo[2 * j] = l[0];
-        r.lo[2 * j + 1] = l[1];
+        uint32_t a, b;
+        half_pair(x[2 * j] * up, x[2 * j + 1] * up, a, b);
+        hi[j] = a;
+        lo[j] = b;
     }
-    return r;
+    return Half2{__builtin_bit_cast(h8, hi), __builtin_bit_cast(h8, lo)};
+}
+// The parts of an accumulator's registers 0..7 and 8..15, as they are.
+__device__ __forceinline__ void split16(const f32x16 &x, Half2 (&d)[2]) {
+#pragma unroll
+    for (int s = 0; s < 2; s++) {
+        u32x4 hi, lo;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            uint32_t a, b;
+            half_pair(x[8 * s + 2 * j], x[8 * s + 2 * j + 1], a, b);
+            hi[j] = a;
+            lo[j] = b;
+        }
+        d[s] = Half2{__builtin_bit_cast(h8, hi), __builtin_bit_cast(h8, lo)};
+    }
 }
 
 // The power of two that takes a largest magnitude m to [2^14, 2^15) (m of 0,
@@ -158,6 +215,48 @@ struct HalfTile {
     }
 };
 
+// acc += the rows of a tile times a register operand over channels c0 ..
+// c0 + 16 N - 1: accumulator rows are the tile's, columns the operand's lanes.
+template <class Tile, int N>
+__device__ __forceinline__ void dot_along(const _Float16 *t, int c0, const Half2 (&x)[N], f32x16 &acc) {
+    const int l = threadIdx.x & 63;
+#pragma unroll
+    for (int s = 0; s < N; s++) {
+        const h8 hi = Tile::along(t, l & 31, c0 + 16 * s + 8 * (l >> 5));
+        const h8 lo = Tile::along(t + Tile::PART, l & 31, c0 + 16 * s + 8 * (l >> 5));
+        acc = mm(lo, x[s].hi, acc);
+        acc = mm(hi, x[s].lo, acc);
+        acc = mm(hi, x[s].hi, acc);
+    }
+}
+// acc += channels c0 .. c0 + 31 of a tile (accumulator rows) times a register
+// operand over the tile's first 16 N rows.
+template <class Tile, int N>
+__device__ __forceinline__ void dot_across(const _Float16 *t, int c0, const Half2 (&x)[N], f32x16 &acc) {
+#pragma unroll
+    for (int s = 0; s < N; s++) {
+        const h8 hi = Tile::across(t, 16 * s, c0), lo = Tile::across(t + Tile::PART, 16 * s, c0);
+        acc = mm(lo, x[s].hi, acc);
+        acc = mm(hi, x[s].lo, acc);
+        acc = mm(hi, x[s].hi, acc);
+    }
+}
+
+// Tells the scheduler to keep LDS reads AHEAD steps before the products that
+// take them, in a block of STEPS steps of READS reads and three products each:
+// with one or two waves a SIMD nothing else hides their latency.
+template <int STEPS, int READS, int AHEAD>
+__device__ __forceinline__ void read_ahead() {
+    constexpr int A = AHEAD < STEPS ? AHEAD : STEPS;
+    __builtin_amdgcn_sched_group_barrier(0x100, READS * A, 0);
+#pragma unroll
+    for (int i = 0; i < STEPS - A; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 3, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x8, 3 * A, 0);
+}
+
 // 8 consecutive channels, `off` floats into a buffer resource, zero from `lim`
 // channels on and past the resource's end.
 template <bool VEC>
@@ -179,21 +278,6 @@ __device__ __forceinline__ void load8(__amdgpu_buffer_rsrc_t rs, uint32_t off, i
     }
 }
 
-// The same from a row's address.
-template <bool VEC>
-__device__ __forceinline__ void load8g(const float *p, int lim, float (&x)[8]) {
-    if constexpr (VEC) {
-        const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-        const float4 a = lim > 0 ? *(const float4 *)p : z;
-        const float4 b = lim > 4 ? *(const float4 *)(p + 4) : z;
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
-        x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = e < lim ? p[e] : 0.f;
-    }
-}
-
 // How NT threads stage a tile of ROWS rows of W channels: RPP rows a pass, 8
 // channels a thread, so that a thread keeps its channels from pass to pass
 // (W = 96: the last quarter of the threads idle).
@@ -210,8 +294,34 @@ struct StagePlan {
 
 __device__ __forceinline__ float absmax8(const float (&x)[8], float m) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) m = fmaxf(m, fabsf(x[e]));
+    for (int e = 0; e < 8; e += 2) m = max3abs(m, x[e], x[e + 1]);
     return m;
+}
+
+// A lane's row of 16 N channels (of `lim` channels, zeros past them) as an operand:
+// times the power of two that its largest magnitude calls for, whose reciprocal
+// and the magnitude are returned.  The lanes l and l + 32 hold a row together.
+template <bool VEC, int N>
+__device__ __forceinline__ float load_row(__amdgpu_buffer_rsrc_t rs, uint32_t off, int lim,
+                                          Half2 (&x)[N], float *mx = nullptr) {
+    const int lh = (threadIdx.x >> 5) & 1;
+    float v[N][8], m = 0.f;
+#pragma unroll
+    for (int s = 0; s < N; s++) load8<VEC>(rs, off + 16 * s + 8 * lh, lim - (16 * s + 8 * lh), v[s]);
+#pragma unroll
+    for (int s = 0; s < N; s++) m = absmax8(v[s], m);
+    m = pair32(m, max2);
+    const float up = up_of(m);
+#pragma unroll
+    for (int s = 0; s < N; s++) x[s] = half_split(v[s], up);
+    if (mx) *mx = m;
+    return down_of(up);
+}
+// A resource over `rows` rows (at most 64) of `stride` floats from p on, the last
+// of them `width` floats long.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const float *p, int rows, long long stride,
+                                                            int width) {
+    return make_rsrc(p, rows > 0 ? ((uint32_t)(rows - 1) * (uint32_t)stride + width) * 4u : 0u);
 }
 
 constexpr float P_UP = 16384.0f, P_EXP = 14.0f;  // softmax values enter the products times 2^14
@@ -224,15 +334,23 @@ __device__ __forceinline__ long long xcd_order(long long id, long long total) {
     return x < rem ? x * (per + 1) + loc : rem * (per + 1) + (x - rem) * per + loc;
 }
 
-// The four lambda vectors' terms of a lane's own head.
+// Lambda of a lane's own head: the wave's one head together, else each lane its
+// own.
 __device__ __forceinline__ float lane_lambda(const DiffArgs &g, int head) {
-    const float *l = g.lam + (g.lam_heads > 1 ? (long long)head * 4 * g.dh : 0);
-    double a = 0.0, b = 0.0;
-    for (int c = 0; c < g.dh; c++) {
-        a = fma((double)l[c], (double)l[g.dh + c], a);
-        b = fma((double)l[2 * g.dh + c], (double)l[3 * g.dh + c], b);
+    double e1, e2;
+    if (g.lam_heads == 1 || g.group == 1) {
+        lambda_terms(g.lam, g.lam_heads, g.dh, __builtin_amdgcn_readfirstlane(head), &e1, &e2);
+    } else {
+        const float *l = g.lam + (long long)head * 4 * g.dh;
+        double a = 0.0, b = 0.0;
+        for (int c = 0; c < g.dh; c++) {
+            a = fma((double)l[c], (double)l[g.dh + c], a);
+            b = fma((double)l[2 * g.dh + c], (double)l[3 * g.dh + c], b);
+        }
+        e1 = exp(a);
+        e2 = exp(b);
     }
-    return (float)(exp(a) - exp(b) + (double)g.lam_init);
+    return (float)(e1 - e2 + (double)g.lam_init);
 }
 
 // Tiles of TK keys and values on their way to LDS: a thread's share in registers
@@ -247,7 +365,7 @@ struct KvStage {
     const float *kp, *vp;
     long long stride;
     uint32_t koff, voff, step;
-    int kend, klim, vlim, sc, sr;
+    int kend, klim, vlim, sc, sr, width;
     // The thread's channels [sc, sc + 8) of rows sr, sr + RPP, ...; keys: two
     // runs of dh padded to DHP, values: one of 2 dh.
     __device__ __forceinline__ KvStage(const DiffArgs &g, int b, int kh, int kend_) : kend(kend_) {
@@ -255,6 +373,7 @@ struct KvStage {
         kp = kv + g.koff + 2 * kh * g.dh;
         vp = kv + g.voff + 2 * kh * g.dh;
         stride = g.kvstride;
+        width = 2 * g.dh;
         sc = (int)threadIdx.x % Stage::C8 * 8;
         sr = (int)threadIdx.x / Stage::C8;
         const int run = sc >= DHP ? 1 : 0;
@@ -267,8 +386,9 @@ struct KvStage {
     __device__ __forceinline__ bool stager() const { return Stage::ALL || sr < Stage::RPP; }
     __device__ __forceinline__ void load(int k0) {
         // rows from kend on are past the resource's end
-        const uint32_t bytes = (uint32_t)min(kend - k0, TK) * (uint32_t)stride * 4;
-        const auto rk = make_rsrc(kp + k0 * stride, bytes), rv = make_rsrc(vp + k0 * stride, bytes);
+        const int rows = min(kend - k0, TK);
+        const auto rk = rows_rsrc(kp + k0 * stride, rows, stride, width);
+        const auto rv = rows_rsrc(vp + k0 * stride, rows, stride, width);
 #pragma unroll
         for (int i = 0; i < CH; i++) {
             load8<VEC>(rk, koff + i * step, klim, xk[i]);
@@ -305,17 +425,17 @@ struct KvStage {
 };
 
 // Channels c0 + {0..3} + 4 lh + 8 j of a row (an accumulator of 32 channels, lane
-// = row), below lim, times f (live) or 0, stored or added.
+// = row), below lim, times f f2 (live) or 0, stored or added.
 template <bool VEC>
 __device__ __forceinline__ void put_channels(float *dst, int lim, int c0, const f32x16 &a, float f,
-                                             bool live, int add) {
+                                             float f2, bool live, int add) {
     const int lh = (threadIdx.x >> 5) & 1;
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
         const int ch = c0 + 2 * r + 4 * lh;
         float v[4];
 #pragma unroll
-        for (int e = 0; e < 4; e++) v[e] = live ? a[r + e] * f : 0.f;
+        for (int e = 0; e < 4; e++) v[e] = live ? a[r + e] * f * f2 : 0.f;
         if (VEC) {
             if (ch >= lim) continue;
             float4 *d = (float4 *)(dst + ch);
@@ -335,8 +455,8 @@ __device__ __forceinline__ void put_channels(float *dst, int lim, int c0, const 
 // its scores are S^T = K Q^T (lane = row), so that a row's maximum and sum stay
 // in two lanes, and the exponentials are, register by register, the operand of
 // O^T = V^T P^T.  Tiles of 64 keys and values are split into LDS once for all
-// waves; the next tile's loads are in flight meanwhile, and its largest
-// magnitudes are taken while they are in registers.
+// waves, in two buffers: while one is read the next is written, and the loads of
+// the one after it are in flight.
 // SPLIT: the keys [z TS, (z + 1) TS) alone (z = blockIdx.y), each map's own
 // normalised output, maximum and sum left for diff_join_kernel.
 template <int DHP, bool VEC, int QG, bool SPLIT>
@@ -346,7 +466,7 @@ diff_fwd_kernel(DiffArgs g) {
     constexpr int W = 2 * DHP, TK = 64, NT = 128 * QG, KS = DHP / 16, CT = DHP / 16;
     using Tile = HalfTile<TK, W>;
     static_assert((int)sizeof(_Float16) * 2 * Tile::HALVES >= QG * CT * 16 * 64 * 4, "exchange");
-    __shared__ __align__(16) _Float16 lds[2 * Tile::HALVES];
+    __shared__ __align__(16) _Float16 lds[2][2 * Tile::HALVES];
     __shared__ float tmax[2][2][2 * QG];
     const int lane = threadIdx.x & 63, wave = wave_index(), lr = lane & 31, lh = lane >> 5;
     const int map = wave & 1, qg = wave >> 1;
@@ -355,7 +475,7 @@ diff_fwd_kernel(DiffArgs g) {
     const int prob = (int)(id / nrb), rb = nrb - 1 - (int)(id % nrb);  // causal: longest first
     const int b = prob / g.hkv, kh = prob % g.hkv;
     const int nq = len_of(g.qlen, b, g.tq), nk = len_of(g.klen, b, g.tk), shift = nk - nq;
-    const int row = rb * 32 * QG + qg * 32 + lr;
+    const int row0 = rb * 32 * QG + qg * 32, row = row0 + lr;
     const int qi = row / g.group, head = kh * g.group + row % g.group;
     const bool live = qi < nq;
     // keys that some row of the block sees
@@ -368,133 +488,111 @@ diff_fwd_kernel(DiffArgs g) {
 
     KvStage<DHP, TK, NT, VEC> st(g, b, kh, kend);
     if (ntile) st.load(kbeg);
-
-    // the row's query of this map, times its own power of two
+    // the row's query of this map; the wave's queries
+    const int w_first = row0 / g.group, w_last = min(nq - 1, (row0 + 31) / g.group);
     Half2 q[KS];
-    float qdown;
-    {
-        const float *qp = g.q + ((long long)b * g.tq + min(qi, g.tq - 1)) * g.qstride +
-                          (2 * head + map) * g.dh;
-        float v[KS][8], mx = 0.f;
-#pragma unroll
-        for (int s = 0; s < KS; s++) {
-            const int c = 16 * s + 8 * lh;
-            load8g<VEC>(qp + c, live ? g.dh - c : 0, v[s]);
-            mx = absmax8(v[s], mx);
-        }
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float up = up_of(mx);
-        qdown = down_of(up) * (g.scale * LOG2E);
-#pragma unroll
-        for (int s = 0; s < KS; s++) q[s] = half_split(v[s], up);
-    }
+    const int q0 = min(w_first, g.tq - 1);
+    float qdown = load_row<VEC>(rows_rsrc(g.q + ((long long)b * g.tq + q0) * g.qstride,
+                                          min(g.tq - q0, 32), g.qstride, 2 * g.h * g.dh),
+                                (uint32_t)(qi - q0) * (uint32_t)g.qstride + (2 * head + map) * g.dh,
+                                live ? g.dh : 0, q);
+    qdown *= g.scale * LOG2E;
+    float lam = 0.f;
+    if (!SPLIT && map == 0) lam = lane_lambda(g, min(head, g.h - 1));
     f32x16 o[CT];
 #pragma unroll
     for (int c = 0; c < CT; c++)
 #pragma unroll
         for (int r = 0; r < 16; r++) o[c][r] = 0.f;
-    float m = NO_MAX, l = 0.f, vdown = 0.f, odown = 0.f;
-    // rows of the wave's queries, for tiles that every one of them sees whole
-    const int w_first = (rb * 32 * QG + qg * 32) / g.group;
-    const int w_last = min(nq - 1, (rb * 32 * QG + qg * 32 + 31) / g.group);
-    if (ntile) st.maxima(tmax[0][0], tmax[0][1]);
-    const _Float16 *const kt = lds, *const vt = lds + Tile::HALVES;
-    for (int t = 0; t < ntile; t++) {
-        const int k0 = kbeg + t * TK;
-        __syncthreads();
+    float m = NO_MAX, l = 0.f;
+    // powers of two: of the tile that is staged (.1), and the output's unit
+    float kup1 = 1.f, vup1 = 0.f, vdown = 0.f;
+    auto stage = [&](int t) {
         float mk = 0.f, mv = 0.f;
 #pragma unroll
         for (int i = 0; i < 2 * QG; i++) {
-            mk = fmaxf(mk, tmax[t & 1][0][i]);
-            mv = fmaxf(mv, tmax[t & 1][1][i]);
+            mk = max2(mk, tmax[t & 1][0][i]);
+            mv = max2(mv, tmax[t & 1][1][i]);
         }
-        const float kup = up_of(mk);
+        kup1 = up_of(mk);
         // the output's unit follows the tile's; at most 2^60 down at once, so
         // that what is there does not overflow
-        float vup = up_of(mv);
-        if (t) vup = fminf(vup, down_of(vdown) * 0x1p60f);
-        vdown = down_of(vup);
-        st.store(lds, kup, vup);
-        if (t + 1 < ntile) st.load(k0 + TK);
+        const float up = up_of(mv);
+        vup1 = t ? fminf(up, vup1 * 0x1p60f) : up;
+        st.store(lds[t & 1], kup1, vup1);
+    };
+    if (ntile) {
+        st.maxima(tmax[0][0], tmax[0][1]);
         __syncthreads();
-        const bool any = g.causal ? k0 <= w_last + shift : true;
-        if (any && w_first < nq) {
-            const float f = down_of(kup) * qdown;
-            float u[2][16];
-#pragma unroll
-            for (int s2 = 0; s2 < 2; s2++) {
-                f32x16 hh, sm;
-#pragma unroll
-                for (int r = 0; r < 16; r++) hh[r] = sm[r] = 0.f;
-#pragma unroll
-                for (int s = 0; s < KS; s++) {
-                    const int c = map * DHP + 16 * s + 8 * lh;
-                    const h8 hi = Tile::along(kt, 32 * s2 + lr, c);
-                    const h8 lo = Tile::along(kt + Tile::PART, 32 * s2 + lr, c);
-                    sm = mm(hi, q[s].lo, sm);
-                    hh = mm(hi, q[s].hi, hh);
-                    sm = mm(lo, q[s].hi, sm);
-                }
-#pragma unroll
-                for (int r = 0; r < 16; r++) u[s2][r] = (hh[r] + sm[r]) * f;
-            }
-            const bool whole = k0 + TK <= nk && !(g.causal && k0 + TK - 1 > w_first + shift) &&
-                               !(g.diag && k0 <= w_last && w_first < k0 + TK);
-            if (!whole) {
-#pragma unroll
-                for (int s2 = 0; s2 < 2; s2++)
-#pragma unroll
-                    for (int r = 0; r < 16; r++) {
-                        const int j = k0 + 32 * s2 + 8 * (r >> 2) + 4 * lh + (r & 3);
-                        const bool in = j < nk && !(g.causal && j > qi + shift) &&
-                                        !(g.diag && j == qi);
-                        u[s2][r] = in ? u[s2][r] : -INFINITY;
-                    }
-            }
-            float mn = m;
-#pragma unroll
-            for (int r = 0; r < 16; r++) mn = fmaxf(mn, fmaxf(u[0][r], u[1][r]));
-            mn = fmaxf(mn, __shfl_xor(mn, 32, 64));
-            const float al = __builtin_amdgcn_exp2f(m - mn), base = mn - P_EXP;
-            m = mn;
-            l *= al;
-            Half2 p[4];
-            float ps = 0.f;
-#pragma unroll
-            for (int s = 0; s < 4; s++) {
-                float e[8];
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    e[i] = __builtin_amdgcn_exp2f(u[s >> 1][8 * (s & 1) + i] - base);
-                    ps += e[i];
-                }
-                p[s] = half_split(e, 1.0f);
-            }
-            l += ps;
-            const float keep = al * (odown * vup);
-            odown = vdown;
-#pragma unroll
-            for (int c = 0; c < CT; c++) {
-                f32x16 a;
-#pragma unroll
-                for (int r = 0; r < 16; r++) a[r] = 0.f;
-#pragma unroll
-                for (int s = 0; s < 4; s++) {
-                    const h8 hi = Tile::across(vt, 16 * s, 32 * c);
-                    const h8 lo = Tile::across(vt + Tile::PART, 16 * s, 32 * c);
-                    a = mm(lo, p[s].hi, a);
-                    a = mm(hi, p[s].lo, a);
-                    a = mm(hi, p[s].hi, a);
-                }
-#pragma unroll
-                for (int r = 0; r < 16; r++) o[c][r] = __builtin_fmaf(o[c][r], keep, a[r]);
-            }
-        }
-        if (t + 1 < ntile) st.maxima(tmax[(t + 1) & 1][0], tmax[(t + 1) & 1][1]);
+        stage(0);
+        st.load(kbeg + TK);
+        st.maxima(tmax[1][0], tmax[1][1]);
     }
-    l += __shfl_xor(l, 32, 64);
+    for (int t = 0; t < ntile; t++) {
+        const int k0 = kbeg + t * TK;
+        __syncthreads();
+        const _Float16 *const kt = lds[t & 1], *const vt = kt + Tile::HALVES;
+        const float f = down_of(kup1) * qdown, turn = vdown * vup1;
+        vdown = down_of(vup1);
+        // (past the last tile: zeros, into a buffer that nothing reads)
+        stage(t + 1);
+        st.load(k0 + 2 * TK);
+        f32x16 u[2];
+#pragma unroll
+        for (int s2 = 0; s2 < 2; s2++) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) u[s2][r] = 0.f;
+            dot_along<Tile>(kt + 32 * s2 * Tile::STRIDE, map * DHP, q, u[s2]);
+        }
+#pragma unroll
+        for (int s2 = 0; s2 < 2; s2++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) u[s2][r] *= f;
+        const bool whole = k0 + TK <= nk && !(g.causal && k0 + TK - 1 > w_first + shift) &&
+                           !(g.diag && k0 <= w_last && w_first < k0 + TK);
+        if (!whole) {
+#pragma unroll
+            for (int s2 = 0; s2 < 2; s2++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int j = k0 + 32 * s2 + 8 * (r >> 2) + 4 * lh + (r & 3);
+                    const bool in = j < nk && !(g.causal && j > qi + shift) && !(g.diag && j == qi);
+                    u[s2][r] = in ? u[s2][r] : -INFINITY;
+                }
+        }
+        float mn = m;
+#pragma unroll
+        for (int r = 0; r < 16; r++) mn = max3(mn, u[0][r], u[1][r]);
+        mn = pair32(mn, max2);
+        const float al = __builtin_amdgcn_exp2f(m - mn), base = mn - P_EXP;
+        m = mn;
+        Half2 p[4];
+        float ps[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                u[s][r] = __builtin_amdgcn_exp2f(u[s][r] - base);
+                ps[r & 3] += u[s][r];
+            }
+            split16(u[s], *(Half2(*)[2]) & p[2 * s]);
+        }
+        l = __builtin_fmaf(l, al, (ps[0] + ps[1]) + (ps[2] + ps[3]));
+        const float keep = al * turn;
+#pragma unroll
+        for (int c = 0; c < CT; c++) {
+            f32x16 a;
+#pragma unroll
+            for (int r = 0; r < 16; r++) a[r] = 0.f;
+            dot_across<Tile>(vt, 32 * c, p, a);
+#pragma unroll
+            for (int r = 0; r < 16; r++) o[c][r] = __builtin_fmaf(o[c][r], keep, a[r]);
+        }
+        st.maxima(tmax[t & 1][0], tmax[t & 1][1]);
+    }
+    l = pair32(l, add2);
     const bool some = live && l > 0.f;
-    const float il = some ? odown / l : 0.f;  // both carry 2^14
+    const float il = some ? vdown / l : 0.f;  // both carry 2^14
 #pragma unroll
     for (int c = 0; c < CT; c++)
 #pragma unroll
@@ -519,7 +617,7 @@ diff_fwd_kernel(DiffArgs g) {
     }
     // map 1's output to its partner wave
     __syncthreads();
-    float *ex = (float *)lds + qg * CT * 16 * 64;
+    float *ex = (float *)lds[0] + qg * CT * 16 * 64;
     if (map == 1) {
 #pragma unroll
         for (int c = 0; c < CT; c++)
@@ -528,8 +626,6 @@ diff_fwd_kernel(DiffArgs g) {
     }
     if (g.stats && row < R && lh == 0)
         *(f2 *)(g.stats + out * 4 + 2 * map) = f2{m, some ? P_UP / l : 0.f};
-    float lam = 0.f;
-    if (map == 0) lam = lane_lambda(g, min(head, g.h - 1));
     __syncthreads();
     const bool vst = VEC;  // whole float4s: dv % 4 == 0, aligned rows
     auto store = [&](float *dst, auto &&val) {
@@ -563,7 +659,7 @@ diff_fwd_kernel(DiffArgs g) {
         }
     float rn = 1.0f;
     if (g.gain) {
-        ss += __shfl_xor(ss, 32, 64);
+        ss = pair32(ss, add2);
         rn = (1.0f / sqrtf(ss / (float)dv + g.eps)) * (1.0f - g.lam_init);
         store(g.y + out * dv, [&](int c, int r, int ch) { return o[c][r] * rn * g.gain[ch]; });
     } else {
@@ -777,19 +873,29 @@ __global__ __launch_bounds__(256) void diff_bwd_params_kernel(const double *__re
     }
 }
 
-// A bound for 2 |dA| of rows with |dO| <= nd and values of magnitude <= vmax, and
-// the power of two that keeps dS below 2^15 under it.
+// The power of two that takes 2 |dA| of rows with |dO| <= nd and values of
+// magnitude <= vmax below 2: |dA| <= nd sqrt(W) vmax, and D is a mean of dA.
 template <int W>
 __device__ __forceinline__ float ds_up(float nd, float vmax) {
     constexpr float root = W == 32 ? 5.6568543f : W == 64 ? 8.0f : W == 96 ? 9.7979590f : 11.313709f;
-    return up_of(nd * (2.0f * root * vmax));
+    return up_of(nd * (2.0f * root * vmax)) * 0x1p-14f;
 }
+// The power of two that softmax values, and lambda times them, enter the
+// backward's products with: at most 2^14, so that P_1 - lambda P_2 and P (dA - D)
+// stay below 2^15.
+__device__ __forceinline__ float p_up(float lam) { return up_of(fmaxf(1.0f, lam)) * 0.5f; }
 
-// dQ.  Rows and tiles as in the forward, a wave on both maps of its 32 rows:
-// S_m^T = K_m Q_m^T and dA^T = V dO^T (lane = row), dS_m in registers is the
-// operand of dQ_m^T = K_m^T dS_m^T.  Each tile's products are summed apart and
-// added to the gradient in fp32, which carries the tile's powers of two and
-// rounds to nearest (the matrix core's own sum cuts off).
+// The matrix core's sum is cut off towards -inf, which leaves every element of
+// a long sum a little low.  Two thirds of the way (where a sum that grows with
+// the square root of its length has collected half of it) the accumulators
+// change sign, and the operand from registers with them.
+__device__ __forceinline__ int flip_at(int ntile) { return (2 * ntile + 2) / 3; }
+
+// dQ.  Rows as in the forward, a wave on both maps of its 32 rows, tiles of 32
+// keys in two LDS buffers: S_m^T = K_m Q_m^T and dA^T = V dO^T (lane = row), and
+// P (dA - D) in registers is the operand of dQ_m^T = K_m^T dS_m^T, which is
+// summed over all tiles in the accumulators.  Their unit is a power of two from
+// the largest magnitudes so far; where it changes they are rescaled.
 template <int DHP, bool VEC, int NW>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DHP <= 32 ? 2 : 1))) void
 diff_dq_kernel(DiffArgs g) {
@@ -797,7 +903,7 @@ diff_dq_kernel(DiffArgs g) {
     constexpr int CT = (DHP + 31) / 32;
     using Tile = HalfTile<TK, W>;
     // (a map's last 32-channel tile may run past the row: into the padding)
-    __shared__ __align__(16) _Float16 lds[2 * Tile::HALVES + 32];
+    __shared__ __align__(16) _Float16 lds[2][2 * Tile::HALVES + 32];
     __shared__ float tmax[2][2][NW];
     const int lane = threadIdx.x & 63, wave = wave_index(), lr = lane & 31, lh = lane >> 5;
     const int R = g.tq * g.group, nrb = (R + 32 * NW - 1) / (32 * NW);
@@ -816,46 +922,30 @@ diff_dq_kernel(DiffArgs g) {
     if (ntile) st.load(0);
 
     // the row's queries, its dO and what the first pass left of it
-    Half2 q[2][KS], d[VS];
-    float qdown[2], ddown, nd;
-    const long long qr = (long long)b * g.tq + min(qi, g.tq - 1);
-    const long long at = qr * g.h + head;
+    const int w_first = (rb * 32 * NW + wave * 32) / g.group;
+    const int w_last = min(nq - 1, (rb * 32 * NW + wave * 32 + 31) / g.group);
+    const int q0 = min(w_first, g.tq - 1), qx = qi - q0, dv = 2 * g.dh;
+    const long long img = (long long)b * g.tq + q0;
+    const int left = min(g.tq - q0, 32);
+    const auto rq = rows_rsrc(g.q + img * g.qstride, left, g.qstride, 2 * g.h * g.dh);
+    const auto rd = rows_rsrc(g.dout + img * g.h * dv, left, (long long)g.h * dv, g.h * dv);
+    const auto rr = rows_rsrc(g.rec + img * g.h * 8, left, (long long)g.h * 8, g.h * 8);
+    f32x4 sm, dd;
     {
-        const float *qp = g.q + qr * g.qstride + 2 * head * g.dh;
-#pragma unroll
-        for (int m = 0; m < 2; m++) {
-            float v[KS][8], mx = 0.f;
-#pragma unroll
-            for (int s = 0; s < KS; s++) {
-                const int c = 16 * s + 8 * lh;
-                load8g<VEC>(qp + m * g.dh + c, live ? g.dh - c : 0, v[s]);
-                mx = absmax8(v[s], mx);
-            }
-            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            const float up = up_of(mx);
-            qdown[m] = down_of(up) * (g.scale * LOG2E);
-#pragma unroll
-            for (int s = 0; s < KS; s++) q[m][s] = half_split(v[s], up);
-        }
-        float v[VS][8], mx = 0.f;
-#pragma unroll
-        for (int s = 0; s < VS; s++) {
-            const int c = 16 * s + 8 * lh;
-            load8g<VEC>(g.dout + at * 2 * g.dh + c, live ? 2 * g.dh - c : 0, v[s]);
-            mx = absmax8(v[s], mx);
-        }
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float up = up_of(mx);
-        ddown = down_of(up);
-#pragma unroll
-        for (int s = 0; s < VS; s++) d[s] = half_split(v[s], up);
+        const uint32_t at = live ? (uint32_t)(qx * g.h + head) * 32u : DMA_OOB;
+        sm = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rr, at, 0, 0));
+        dd = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rr, at + 16u, 0, 0));
     }
-    float4 sm4 = make_float4(0.f, 0.f, 0.f, 0.f), dd4 = sm4;
-    if (live) {
-        sm4 = *(const float4 *)(g.rec + at * 8);
-        dd4 = *(const float4 *)(g.rec + at * 8 + 4);
-    }
-    nd = dd4.z;
+    Half2 q[2][KS], d[VS];
+    float qdown[2];
+#pragma unroll
+    for (int m = 0; m < 2; m++)
+        qdown[m] = load_row<VEC>(rq, (uint32_t)qx * (uint32_t)g.qstride + (2 * head + m) * g.dh,
+                                 live ? g.dh : 0, q[m]) * (g.scale * LOG2E);
+    const float ddown = load_row<VEC>(rd, (uint32_t)(qx * g.h + head) * dv, live ? dv : 0, d);
+    const float pup = p_up(fabsf(dd[3]));
+    const float nm[2] = {-sm[0], -sm[2]};
+    float il[2] = {sm[1] * pup, sm[3] * dd[3] * pup};
     f32x16 acc[2][CT];
 #pragma unroll
     for (int m = 0; m < 2; m++)
@@ -863,127 +953,125 @@ diff_dq_kernel(DiffArgs g) {
         for (int c = 0; c < CT; c++)
 #pragma unroll
             for (int r = 0; r < 16; r++) acc[m][c][r] = 0.f;
-    const int w_first = (rb * 32 * NW + wave * 32) / g.group;
-    const int w_last = min(nq - 1, (rb * 32 * NW + wave * 32 + 31) / g.group);
-    if (ntile) st.maxima(tmax[0][0], tmax[0][1]);
-    const _Float16 *const kt = lds, *const vt = lds + Tile::HALVES;
+    // largest magnitudes so far, and the powers of two of the tile in each buffer
+    float mk = 0.f, mv = 0.f, kup1 = 1.f, vup1 = 1.f, kup = 1.f, dsup = 1.f, sgn = 1.f;
+    const int flip = flip_at(ntile);
+    auto stage = [&](int t) {  // tile t, whose maxima are there, into its buffer
+#pragma unroll
+        for (int i = 0; i < NW; i++) {
+            mk = max2(mk, tmax[t & 1][0][i]);
+            mv = max2(mv, tmax[t & 1][1][i]);
+        }
+        kup1 = up_of(mk);
+        vup1 = up_of(mv);
+        st.store(lds[t & 1], kup1, vup1);
+    };
+    if (ntile) {
+        st.maxima(tmax[0][0], tmax[0][1]);
+        __syncthreads();
+        stage(0);
+        st.load(TK);
+        st.maxima(tmax[1][0], tmax[1][1]);
+    }
     for (int t = 0; t < ntile; t++) {
         const int k0 = t * TK;
         __syncthreads();
-        float mk = 0.f, mv = 0.f;
-#pragma unroll
-        for (int i = 0; i < NW; i++) {
-            mk = fmaxf(mk, tmax[t & 1][0][i]);
-            mv = fmaxf(mv, tmax[t & 1][1][i]);
+        // dS's power of two, and the accumulators in the tile's unit
+        const float vup = vup1, dsup1 = ds_up<W>(dd[2], mv);
+        float ratio = down_of(kup) * kup1 * (down_of(dsup) * dsup1);
+        kup = kup1;
+        dsup = dsup1;
+        if (t == flip) {
+            sgn = -1.0f;
+            il[0] = -il[0];
+            il[1] = -il[1];
+            ratio = -ratio;
         }
-        const float kup = up_of(mk), vup = up_of(mv);
-        st.store(lds, kup, vup);
-        if (t + 1 < ntile) st.load(k0 + TK);
-        __syncthreads();
-        if (w_first < nq && !(g.causal && k0 > w_last + shift)) {
+        if (t && __any(ratio != 1.0f)) {
+#pragma unroll
+            for (int m = 0; m < 2; m++)
+#pragma unroll
+                for (int c = 0; c < CT; c++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) acc[m][c][r] *= ratio;
+        }
+        // (past the last tile: zeros, into a buffer that nothing reads)
+        stage(t + 1);
+        st.load(k0 + 2 * TK);
+        {
+            const _Float16 *const kt = lds[t & 1], *const vt = kt + Tile::HALVES;
+            const float kdown = down_of(kup);
+            f32x16 s1, s2, da;
+#pragma unroll
+            for (int r = 0; r < 16; r++) s1[r] = s2[r] = da[r] = 0.f;
+            dot_along<Tile>(kt, 0, q[0], s1);
+            dot_along<Tile>(kt, DHP, q[1], s2);
+            dot_along<Tile>(vt, 0, d, da);
+            read_ahead<2 * KS + VS, 2, 3>();
+            const float f1 = kdown * qdown[0], f2 = kdown * qdown[1];
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                s1[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s1[r], f1, nm[0])) * il[0];
+                s2[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s2[r], f2, nm[1])) * il[1];
+            }
             const bool whole = k0 + TK <= nk && !(g.causal && k0 + TK - 1 > w_first + shift) &&
                                !(g.diag && k0 <= w_last && w_first < k0 + TK);
-            const float kdown = down_of(kup);
-            const float dup = ds_up<W>(nd, mv), fd = down_of(vup) * ddown * dup;
-            f32x16 da;
-            {
-                f32x16 hh, sm;
+            if (!whole) {
 #pragma unroll
-                for (int r = 0; r < 16; r++) hh[r] = sm[r] = 0.f;
-#pragma unroll
-                for (int s = 0; s < VS; s++) {
-                    const h8 hi = Tile::along(vt, lr, 16 * s + 8 * lh);
-                    const h8 lo = Tile::along(vt + Tile::PART, lr, 16 * s + 8 * lh);
-                    sm = mm(hi, d[s].lo, sm);
-                    hh = mm(hi, d[s].hi, hh);
-                    sm = mm(lo, d[s].hi, sm);
+                for (int r = 0; r < 16; r++) {
+                    const int j = k0 + 8 * (r >> 2) + 4 * lh + (r & 3);
+                    const bool in = j < nk && !(g.causal && j > qi + shift) && !(g.diag && j == qi);
+                    s1[r] = in ? s1[r] : 0.f;
+                    s2[r] = in ? s2[r] : 0.f;
                 }
+            }
+            const float fd = down_of(vup) * ddown * dsup, D1 = -dd[0] * dsup, D2 = -dd[1] * dsup;
 #pragma unroll
-                for (int r = 0; r < 16; r++) da[r] = (hh[r] + sm[r]) * fd;
+            for (int r = 0; r < 16; r++) {
+                s1[r] *= __builtin_fmaf(da[r], fd, D1);
+                s2[r] *= __builtin_fmaf(da[r], fd, D2);
             }
 #pragma unroll
             for (int m = 0; m < 2; m++) {
-                f32x16 hh, sm;
-#pragma unroll
-                for (int r = 0; r < 16; r++) hh[r] = sm[r] = 0.f;
-#pragma unroll
-                for (int s = 0; s < KS; s++) {
-                    const int c = m * DHP + 16 * s + 8 * lh;
-                    const h8 hi = Tile::along(kt, lr, c);
-                    const h8 lo = Tile::along(kt + Tile::PART, lr, c);
-                    sm = mm(hi, q[m][s].lo, sm);
-                    hh = mm(hi, q[m][s].hi, hh);
-                    sm = mm(lo, q[m][s].hi, sm);
-                }
-                const float f = kdown * qdown[m], mx = m ? sm4.z : sm4.x, il = m ? sm4.w : sm4.y;
-                const float D = (m ? dd4.y : dd4.x) * dup;
                 Half2 ds[2];
+                split16(m ? s2 : s1, ds);
 #pragma unroll
-                for (int s = 0; s < 2; s++) {
-                    float e[8];
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const int r = 8 * s + i;
-                        float p = __builtin_amdgcn_exp2f((hh[r] + sm[r]) * f - mx) * il;
-                        if (!whole) {
-                            const int j = k0 + 8 * (r >> 2) + 4 * lh + (r & 3);
-                            const bool in = j < nk && !(g.causal && j > qi + shift) &&
-                                            !(g.diag && j == qi);
-                            p = in ? p : 0.f;
-                        }
-                        e[i] = p * (da[r] - D);
-                    }
-                    ds[s] = half_split(e, 1.0f);
-                }
-                const float back = kdown * down_of(dup);
-#pragma unroll
-                for (int c = 0; c < CT; c++) {
-                    f32x16 a;
-#pragma unroll
-                    for (int r = 0; r < 16; r++) a[r] = 0.f;
-#pragma unroll
-                    for (int s = 0; s < 2; s++) {
-                        const h8 hi = Tile::across(kt, 16 * s, m * DHP + 32 * c);
-                        const h8 lo = Tile::across(kt + Tile::PART, 16 * s, m * DHP + 32 * c);
-                        a = mm(lo, ds[s].hi, a);
-                        a = mm(hi, ds[s].lo, a);
-                        a = mm(hi, ds[s].hi, a);
-                    }
-#pragma unroll
-                    for (int r = 0; r < 16; r++)
-                        acc[m][c][r] = __builtin_fmaf(a[r], back, acc[m][c][r]);
-                }
+                for (int c = 0; c < CT; c++) dot_across<Tile>(kt, m * DHP + 32 * c, ds, acc[m][c]);
             }
+            read_ahead<4 * CT, 4, 3>();
         }
-        if (t + 1 < ntile) st.maxima(tmax[(t + 1) & 1][0], tmax[(t + 1) & 1][1]);
+        st.maxima(tmax[t & 1][0], tmax[t & 1][1]);
     }
     if (row >= R) return;
-    float *dst = g.dq + qr * g.qstride + 2 * head * g.dh;
+    float *dst = g.dq + ((long long)b * g.tq + qi) * g.qstride + 2 * head * g.dh;
+    const float f = down_of(kup) * (g.scale * sgn), f2 = down_of(dsup) * down_of(pup);
 #pragma unroll
-    for (int m = 0; m < 2; m++) {
-        const float f = m ? -dd4.w * g.scale : g.scale;
+    for (int m = 0; m < 2; m++)
 #pragma unroll
         for (int c = 0; c < CT; c++)
-            put_channels<VEC>(dst + m * g.dh, g.dh, 32 * c, acc[m][c], f, live, g.acc_q);
-    }
+            put_channels<VEC>(dst + m * g.dh, g.dh, 32 * c, acc[m][c], m ? -f : f, f2, live,
+                              g.acc_q);
 }
 
 // dK and dV.  One workgroup of NW waves per (image, key head, 32 NW keys), wave
 // w on 32 of them: its keys' and values' parts stay in registers.  Tiles of 32
-// rows (queries of the head group) are split into LDS with their records:
+// rows (queries of the head group) and their records in two LDS buffers:
 // S_m = Q_m K_m^T and dA = dO V^T (lane = key), and P and dS in registers are
-// the operands of dV^T = dO^T (P_1 - lambda P_2) and dK_m^T = Q_m^T dS_m.
+// the operands of dV^T = dO^T (P_1 - lambda P_2) and dK_m^T = Q_m^T dS_m, summed
+// over all tiles in the accumulators as in diff_dq_kernel.
 template <int DHP, bool VEC, int NW>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DHP <= 16 ? 2 : 1))) void
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(1))) void
 diff_dkv_kernel(DiffArgs g) {
     constexpr int W = 2 * DHP, TR = 32, NT = 64 * NW, KS = DHP / 16, VS = W / 16;
     constexpr int CT = (DHP + 31) / 32, VT = DHP / 16;
     using Tile = HalfTile<TR, W>;
     using Stage = StagePlan<TR, W, NT>;
     constexpr int CH = Stage::PASSES;
-    __shared__ __align__(16) _Float16 lds[2 * Tile::HALVES + 32];
-    __shared__ __align__(16) float rec[7][TR];  // m1, il1, m2, il2, D1, D2, lambda
-    __shared__ float tmax[2][4][NW];  // largest |q|, |dO|, |dO|_2, |lambda|
+    __shared__ __align__(16) _Float16 lds[2][2 * Tile::HALVES + 32];
+    // -m1, il1, -m2, lambda il2, -D1, -D2, with their powers of two
+    __shared__ __align__(16) float rec[2][6][TR];
+    __shared__ float tmax[2][4][NW];  // largest |q|, |dO|, |dO|_2, |lambda| of a tile
+    __shared__ float vmaxs[NW];
     const int lane = threadIdx.x & 63, wave = wave_index(), lr = lane & 31, lh = lane >> 5;
     const int nkb = (g.tk + 32 * NW - 1) / (32 * NW);
     const long long id = xcd_order(blockIdx.x, gridDim.x);
@@ -1000,37 +1088,38 @@ diff_dkv_kernel(DiffArgs g) {
     const float ginv = 1.0f / (float)g.group;
 
     float xq[CH][8], xd[CH][8];
-    float4 r0 = make_float4(0.f, 0.f, 0.f, 0.f), r1 = r0;
+    f32x4 r0 = {0.f, 0.f, 0.f, 0.f}, r1 = r0;
     const int sc = (int)threadIdx.x % Stage::C8 * 8, sr = (int)threadIdx.x / Stage::C8;
     const bool stager = Stage::ALL || sr < Stage::RPP;
-    const int run = sc >= DHP ? 1 : 0;
-    const float *qimg = g.q + (long long)b * g.tq * g.qstride + 2 * kh * g.group * g.dh;
-    const float *dimg = g.dout + ((long long)b * g.tq * g.h + kh * g.group) * 2 * g.dh;
+    const int run = sc >= DHP ? 1 : 0, dw = 2 * g.dh;
+    const int qlim = stager ? g.dh - (sc - run * DHP) : 0, dlim = stager ? dw - sc : 0;
+    const long long img = (long long)b * g.tq;
+    const int qc = run * g.dh + sc - run * DHP;
     auto load = [&](int row0) {
-        // rows of a tile lie in queries [q0, q0 + 32]; row x of the tile is
-        // query q0 + (x0 + x) / group (x0 + x < 32 + group, exact in floats)
-        const int q0 = row0 / g.group, x0 = row0 - q0 * g.group;
-        const float *qb = qimg + q0 * g.qstride;
-        const float *db = dimg + (long long)q0 * g.h * 2 * g.dh;
+        // row x of the tile is query q0 + (x0 + x) / group, head (x0 + x) % group of
+        // the group (x0 + x < 32 + group, exact in floats); rows from row_end on
+        // are left out
+        const int q0 = row0 / g.group, x0 = row0 - q0 * g.group, left = row_end - row0;
+        const int rows = left > 0 ? min(nq - q0, 33) : 0;
+        const auto rq = rows_rsrc(g.q + (img + q0) * g.qstride + 2 * kh * g.group * g.dh, rows,
+                                  g.qstride, 2 * g.group * g.dh);
+        const auto rd = rows_rsrc(g.dout + ((img + q0) * g.h + kh * g.group) * dw, rows,
+                                  (long long)g.h * dw, g.group * dw);
+        const auto rr = rows_rsrc(g.rec + ((img + q0) * g.h + kh * g.group) * 8, rows,
+                                  (long long)g.h * 8, g.group * 8);
 #pragma unroll
         for (int i = 0; i < CH; i++) {
             const int x = sr + i * Stage::RPP;
             const int dq = (int)(((float)(x0 + x) + 0.5f) * ginv), hd = x0 + x - dq * g.group;
-            const bool in = stager && row0 + x < row_end;
-            load8g<VEC>(qb + dq * g.qstride + (2 * hd + run) * g.dh + sc - run * DHP,
-                        in ? g.dh - (sc - run * DHP) : 0, xq[i]);
-            load8g<VEC>(db + ((long long)dq * g.h + hd) * 2 * g.dh + sc, in ? 2 * g.dh - sc : 0,
-                        xd[i]);
+            const bool in = x < left;
+            load8<VEC>(rq, (uint32_t)dq * (uint32_t)g.qstride + 2 * hd * g.dh + qc, in ? qlim : 0, xq[i]);
+            load8<VEC>(rd, (uint32_t)(dq * g.h + hd) * dw + sc, in ? dlim : 0, xd[i]);
         }
-        if (threadIdx.x < TR) {
-            const int x = (int)threadIdx.x;
-            const int dq = (int)(((float)(x0 + x) + 0.5f) * ginv), hd = x0 + x - dq * g.group;
-            r0 = r1 = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (row0 + x < row_end) {
-                const float *rp = g.rec + (((long long)b * g.tq + q0 + dq) * g.h + kh * g.group + hd) * 8;
-                r0 = *(const float4 *)rp;
-                r1 = *(const float4 *)(rp + 4);
-            }
+        if (wave == 0) {
+            const int dq = (int)(((float)(x0 + lr) + 0.5f) * ginv), hd = x0 + lr - dq * g.group;
+            const uint32_t at = lr < left ? (uint32_t)(dq * g.h + hd) * 32u : DMA_OOB;
+            r0 = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rr, at, 0, 0));
+            r1 = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rr, at + 16u, 0, 0));
         }
     };
     auto maxima = [&](int slot) {
@@ -1042,7 +1131,11 @@ diff_dkv_kernel(DiffArgs g) {
         }
         mq = wave_max(mq);
         md = wave_max(md);
-        const float mn = wave_max(r1.z), ml = wave_max(fabsf(r1.w));
+        float mn = 0.f, ml = 0.f;
+        if (wave == 0) {
+            mn = wave_max(r1[2]);
+            ml = wave_max(fabsf(r1[3]));
+        }
         if (lane == 0) {
             tmax[slot][0][wave] = mq;
             tmax[slot][1][wave] = md;
@@ -1054,39 +1147,21 @@ diff_dkv_kernel(DiffArgs g) {
 
     // the lane's key and value
     Half2 k[2][KS], v[VS];
-    float kdown[2], vdown, vmax;
+    float kdown[2], vdown;
     const long long krow = (long long)b * g.tk + min(key, g.tk - 1);
     {
-        const float *kp = g.kv + krow * g.kvstride + g.koff + 2 * kh * g.dh;
-        const float *vp = g.kv + krow * g.kvstride + g.voff + 2 * kh * g.dh;
+        const int k0 = min(w_first, g.tk - 1), rows = min(g.tk - k0, 32);
+        const float *kvp = g.kv + ((long long)b * g.tk + k0) * g.kvstride + 2 * kh * g.dh;
+        const auto rk = rows_rsrc(kvp + g.koff, rows, g.kvstride, dw);
+        const auto rv = rows_rsrc(kvp + g.voff, rows, g.kvstride, dw);
+        const uint32_t off = (uint32_t)(key - k0) * (uint32_t)g.kvstride;
 #pragma unroll
-        for (int m = 0; m < 2; m++) {
-            float x[KS][8], mx = 0.f;
-#pragma unroll
-            for (int s = 0; s < KS; s++) {
-                const int c = 16 * s + 8 * lh;
-                load8g<VEC>(kp + m * g.dh + c, live ? g.dh - c : 0, x[s]);
-                mx = absmax8(x[s], mx);
-            }
-            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            const float up = up_of(mx);
-            kdown[m] = down_of(up) * (g.scale * LOG2E);
-#pragma unroll
-            for (int s = 0; s < KS; s++) k[m][s] = half_split(x[s], up);
-        }
-        float x[VS][8];
-        vmax = 0.f;
-#pragma unroll
-        for (int s = 0; s < VS; s++) {
-            const int c = 16 * s + 8 * lh;
-            load8g<VEC>(vp + c, live ? 2 * g.dh - c : 0, x[s]);
-            vmax = absmax8(x[s], vmax);
-        }
-        vmax = fmaxf(vmax, __shfl_xor(vmax, 32, 64));
-        const float up = up_of(vmax);
-        vdown = down_of(up);
-#pragma unroll
-        for (int s = 0; s < VS; s++) v[s] = half_split(x[s], up);
+        for (int m = 0; m < 2; m++)
+            kdown[m] = load_row<VEC>(rk, off + m * g.dh, live ? g.dh : 0, k[m]) * (g.scale * LOG2E);
+        float mx;
+        vdown = load_row<VEC>(rv, off, live ? dw : 0, v, &mx);
+        mx = wave_max(mx);
+        if (lane == 0) vmaxs[wave] = mx;
     }
     f32x16 dk[2][CT], dv[VT];
 #pragma unroll
@@ -1098,25 +1173,28 @@ diff_dkv_kernel(DiffArgs g) {
 #pragma unroll
         for (int c = 0; c < VT; c++) dv[c][r] = 0.f;
     }
-    if (ntile) maxima(0);
-    const _Float16 *const qt = lds, *const dt = lds + Tile::HALVES;
-    for (int t = 0; t < ntile; t++) {
-        const int row0 = row_beg + t * TR;
-        __syncthreads();
-        float mq = 0.f, md = 0.f, mn = 0.f, ml = 0.f;
+    // largest magnitudes so far, the powers of two of the tile that is staged
+    // (.1) and of the one that is computed
+    float mq = 0.f, md = 0.f, mn = 0.f, ml = 0.f, vmax = 0.f;
+    float qup1 = 1.f, dup1 = 1.f, pup1 = 1.f, sup1 = 1.f, qup = 1.f, dup = 1.f, pup = 1.f, sup = 1.f;
+    const int flip = flip_at(ntile);
+    auto stage = [&](int t) {
 #pragma unroll
         for (int i = 0; i < NW; i++) {
-            mq = fmaxf(mq, tmax[t & 1][0][i]);
-            md = fmaxf(md, tmax[t & 1][1][i]);
-            mn = fmaxf(mn, tmax[t & 1][2][i]);
-            ml = fmaxf(ml, tmax[t & 1][3][i]);
+            mq = max2(mq, tmax[t & 1][0][i]);
+            md = max2(md, tmax[t & 1][1][i]);
         }
-        const float qup = up_of(mq), dup = up_of(md);
+        mn = max2(mn, tmax[t & 1][2][0]);
+        ml = max2(ml, tmax[t & 1][3][0]);
+        qup1 = up_of(mq);
+        dup1 = up_of(md);
+        pup1 = p_up(ml);
+        sup1 = ds_up<W>(mn, vmax);
         if (stager) {
 #pragma unroll
             for (int i = 0; i < CH; i++) {
-                _Float16 *p = lds + (sr + i * Stage::RPP) * Tile::STRIDE + sc;
-                const Half2 hq = half_split(xq[i], qup), hd = half_split(xd[i], dup);
+                _Float16 *p = lds[t & 1] + (sr + i * Stage::RPP) * Tile::STRIDE + sc;
+                const Half2 hq = half_split(xq[i], qup1), hd = half_split(xd[i], dup1);
                 *(h8 *)p = hq.hi;
                 *(h8 *)(p + Tile::PART) = hq.lo;
                 *(h8 *)(p + Tile::HALVES) = hd.hi;
@@ -1124,161 +1202,131 @@ diff_dkv_kernel(DiffArgs g) {
             }
         }
         if (threadIdx.x < TR) {
-            rec[0][threadIdx.x] = r0.x;
-            rec[1][threadIdx.x] = r0.y;
-            rec[2][threadIdx.x] = r0.z;
-            rec[3][threadIdx.x] = r0.w;
-            rec[4][threadIdx.x] = r1.x;
-            rec[5][threadIdx.x] = r1.y;
-            rec[6][threadIdx.x] = r1.w;
+            float(*rc)[TR] = rec[t & 1];
+            const float u = t >= flip ? -pup1 : pup1;
+            rc[0][threadIdx.x] = -r0[0];
+            rc[1][threadIdx.x] = r0[1] * u;
+            rc[2][threadIdx.x] = -r0[2];
+            rc[3][threadIdx.x] = r0[3] * r1[3] * u;
+            rc[4][threadIdx.x] = -r1[0] * sup1;
+            rc[5][threadIdx.x] = -r1[1] * sup1;
         }
-        if (t + 1 < ntile) load(row0 + TR);
+    };
+    if (ntile) {
+        maxima(0);
         __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NW; i++) vmax = max2(vmax, vmaxs[i]);
+        stage(0);
+        load(row_beg + TR);
+        maxima(1);
+    }
+    for (int t = 0; t < ntile; t++) {
+        const int row0 = row_beg + t * TR;
+        __syncthreads();
+        float rv = down_of(pup) * pup1 * (down_of(dup) * dup1);
+        float rk = down_of(pup) * pup1 * (down_of(qup) * qup1) * (down_of(sup) * sup1);
+        qup = qup1;
+        dup = dup1;
+        pup = pup1;
+        sup = sup1;
+        if (t == flip) {
+            rv = -rv;
+            rk = -rk;
+        }
+        if (t && (rv != 1.0f || rk != 1.0f)) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+#pragma unroll
+                for (int m = 0; m < 2; m++)
+#pragma unroll
+                    for (int c = 0; c < CT; c++) dk[m][c][r] *= rk;
+#pragma unroll
+                for (int c = 0; c < VT; c++) dv[c][r] *= rv;
+            }
+        }
+        // (past the last tile: zeros, into a buffer that nothing reads)
+        stage(t + 1);
+        load(row0 + 2 * TR);
         const int tq0 = row0 / g.group, tq1 = min(nq - 1, (row0 + TR - 1) / g.group);
-        if (w_first < nk && !(g.causal && w_first > tq1 + shift)) {
+        {
+            const _Float16 *const qt = lds[t & 1], *const dt = qt + Tile::HALVES;
+            const float(*rc)[TR] = rec[t & 1];
+            f32x16 s1, s2, da;
+#pragma unroll
+            for (int r = 0; r < 16; r++) s1[r] = s2[r] = da[r] = 0.f;
+            dot_along<Tile>(qt, 0, k[0], s1);
+            dot_along<Tile>(qt, DHP, k[1], s2);
+            dot_along<Tile>(dt, 0, v, da);
+            read_ahead<2 * KS + VS, 2, 3>();
+            const float qd = down_of(qup), f1 = qd * kdown[0], f2 = qd * kdown[1];
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const f32x4 m1 = *(const f32x4 *)&rc[0][2 * r + 4 * lh], l1 = *(const f32x4 *)&rc[1][2 * r + 4 * lh];
+                const f32x4 m2 = *(const f32x4 *)&rc[2][2 * r + 4 * lh], l2 = *(const f32x4 *)&rc[3][2 * r + 4 * lh];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    s1[r + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s1[r + e], f1, m1[e])) * l1[e];
+                    s2[r + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s2[r + e], f2, m2[e])) * l2[e];
+                }
+            }
             // rows past the last carry il = 0, keys past the last are not stored
             const bool whole = !(g.causal && w_first + 31 > tq0 + shift) &&
                                !(g.diag && w_first <= tq1 && tq0 <= w_first + 31);
-            const int x0 = row0 - tq0 * g.group;
-            const float qd = down_of(qup), dd = down_of(dup);
-            const float up = ds_up<W>(mn, vmax), fd = vdown * dd * up;
-            const float lup = up_of(ml) * 0x1p-15f;  // takes lambda below 1
-            float p1[16], p2[16], da[16];
-            {
-                f32x16 hh, sm;
+            if (!whole) {
+                const int x0 = row0 - tq0 * g.group;
 #pragma unroll
-                for (int r = 0; r < 16; r++) hh[r] = sm[r] = 0.f;
-#pragma unroll
-                for (int s = 0; s < VS; s++) {
-                    const h8 hi = Tile::along(dt, lr, 16 * s + 8 * lh);
-                    const h8 lo = Tile::along(dt + Tile::PART, lr, 16 * s + 8 * lh);
-                    sm = mm(hi, v[s].lo, sm);
-                    hh = mm(hi, v[s].hi, hh);
-                    sm = mm(lo, v[s].hi, sm);
-                }
-#pragma unroll
-                for (int r = 0; r < 16; r++) da[r] = (hh[r] + sm[r]) * fd;
-            }
-#pragma unroll
-            for (int m = 0; m < 2; m++) {
-                f32x16 hh, sm;
-#pragma unroll
-                for (int r = 0; r < 16; r++) hh[r] = sm[r] = 0.f;
-#pragma unroll
-                for (int s = 0; s < KS; s++) {
-                    const int c = m * DHP + 16 * s + 8 * lh;
-                    const h8 hi = Tile::along(qt, lr, c);
-                    const h8 lo = Tile::along(qt + Tile::PART, lr, c);
-                    sm = mm(hi, k[m][s].lo, sm);
-                    hh = mm(hi, k[m][s].hi, hh);
-                    sm = mm(lo, k[m][s].hi, sm);
-                }
-                const float f = qd * kdown[m];
-#pragma unroll
-                for (int r = 0; r < 16; r += 4) {
-                    const float4 mx = *(const float4 *)&rec[2 * m][2 * r + 4 * lh];
-                    const float4 il = *(const float4 *)&rec[2 * m + 1][2 * r + 4 * lh];
-                    const float mxv[4] = {mx.x, mx.y, mx.z, mx.w}, ilv[4] = {il.x, il.y, il.z, il.w};
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        float p = __builtin_amdgcn_exp2f((hh[r + e] + sm[r + e]) * f - mxv[e]) * ilv[e];
-                        if (!whole) {
-                            const int i = tq0 + (int)(((float)(x0 + 2 * r + 4 * lh + e) + 0.5f) * ginv);
-                            const bool in = !(g.causal && key > i + shift) && !(g.diag && key == i);
-                            p = in ? p : 0.f;
-                        }
-                        (m ? p2 : p1)[r + e] = p;
-                    }
+                for (int r = 0; r < 16; r++) {
+                    const int x = x0 + 8 * (r >> 2) + 4 * lh + (r & 3);
+                    const int i = tq0 + (int)(((float)x + 0.5f) * ginv);
+                    const bool in = !(g.causal && key > i + shift) && !(g.diag && key == i);
+                    s1[r] = in ? s1[r] : 0.f;
+                    s2[r] = in ? s2[r] : 0.f;
                 }
             }
-            // dV: (P_1 - lambda P_2) times a power of two that no lambda passes
-            const float aup = up_of(1.0f + ml), adown = down_of(aup) * dd;
             {
-                Half2 a[2];
+                f32x16 a;
 #pragma unroll
-                for (int s = 0; s < 2; s++) {
-                    float e[8];
+                for (int r = 0; r < 16; r++) a[r] = s1[r] - s2[r];
+                Half2 ah[2];
+                split16(a, ah);
 #pragma unroll
-                    for (int i = 0; i < 8; i += 4) {
-                        const float4 lv = *(const float4 *)&rec[6][2 * (8 * s + i) + 4 * lh];
-                        const float l4[4] = {lv.x, lv.y, lv.z, lv.w};
+                for (int c = 0; c < VT; c++) dot_across<Tile>(dt, 32 * c, ah, dv[c]);
+            }
+            const float fd = vdown * down_of(dup) * sup;
 #pragma unroll
-                        for (int j = 0; j < 4; j++)
-                            e[i + j] = p1[8 * s + i + j] - l4[j] * p2[8 * s + i + j];
-                    }
-                    a[s] = half_split(e, aup);
-                }
+            for (int r = 0; r < 16; r += 4) {
+                const f32x4 D1 = *(const f32x4 *)&rc[4][2 * r + 4 * lh], D2 = *(const f32x4 *)&rc[5][2 * r + 4 * lh];
 #pragma unroll
-                for (int c = 0; c < VT; c++) {
-                    f32x16 x;
-#pragma unroll
-                    for (int r = 0; r < 16; r++) x[r] = 0.f;
-#pragma unroll
-                    for (int s = 0; s < 2; s++) {
-                        const h8 hi = Tile::across(dt, 16 * s, 32 * c);
-                        const h8 lo = Tile::across(dt + Tile::PART, 16 * s, 32 * c);
-                        x = mm(lo, a[s].hi, x);
-                        x = mm(hi, a[s].lo, x);
-                        x = mm(hi, a[s].hi, x);
-                    }
-#pragma unroll
-                    for (int r = 0; r < 16; r++) dv[c][r] = __builtin_fmaf(x[r], adown, dv[c][r]);
+                for (int e = 0; e < 4; e++) {
+                    s1[r + e] *= __builtin_fmaf(da[r + e], fd, D1[e]);
+                    s2[r + e] *= __builtin_fmaf(da[r + e], fd, D2[e]);
                 }
             }
 #pragma unroll
             for (int m = 0; m < 2; m++) {
                 Half2 ds[2];
+                split16(m ? s2 : s1, ds);
 #pragma unroll
-                for (int s = 0; s < 2; s++) {
-                    float e[8];
-#pragma unroll
-                    for (int i = 0; i < 8; i += 4) {
-                        const float4 Dv = *(const float4 *)&rec[4 + m][2 * (8 * s + i) + 4 * lh];
-                        const float4 lv = *(const float4 *)&rec[6][2 * (8 * s + i) + 4 * lh];
-                        const float D4[4] = {Dv.x, Dv.y, Dv.z, Dv.w}, l4[4] = {lv.x, lv.y, lv.z, lv.w};
-#pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const int r = 8 * s + i + j;
-                            const float x = (m ? p2 : p1)[r] * (da[r] - D4[j] * up);
-                            e[i + j] = m ? x * l4[j] : x;
-                        }
-                    }
-                    ds[s] = half_split(e, m ? lup : 1.0f);
-                }
-                const float back = (m ? down_of(lup) : 1.0f) * qd * down_of(up);
-#pragma unroll
-                for (int c = 0; c < CT; c++) {
-                    f32x16 a;
-#pragma unroll
-                    for (int r = 0; r < 16; r++) a[r] = 0.f;
-#pragma unroll
-                    for (int s = 0; s < 2; s++) {
-                        const h8 hi = Tile::across(qt, 16 * s, m * DHP + 32 * c);
-                        const h8 lo = Tile::across(qt + Tile::PART, 16 * s, m * DHP + 32 * c);
-                        a = mm(lo, ds[s].hi, a);
-                        a = mm(hi, ds[s].lo, a);
-                        a = mm(hi, ds[s].hi, a);
-                    }
-#pragma unroll
-                    for (int r = 0; r < 16; r++)
-                        dk[m][c][r] = __builtin_fmaf(a[r], back, dk[m][c][r]);
-                }
+                for (int c = 0; c < CT; c++) dot_across<Tile>(qt, m * DHP + 32 * c, ds, dk[m][c]);
             }
+            read_ahead<2 * (VT + 2 * CT), 4, 3>();
         }
-        if (t + 1 < ntile) maxima((t + 1) & 1);
+        maxima(t & 1);
     }
     if (key >= g.tk) return;
     float *kd = g.dkv + krow * g.kvstride + g.koff + 2 * kh * g.dh;
     float *vd = g.dkv + krow * g.kvstride + g.voff + 2 * kh * g.dh;
+    const float sgn = ntile > flip ? -1.0f : 1.0f;
+    const float fk = down_of(qup) * (g.scale * sgn), fk2 = down_of(pup) * down_of(sup);
 #pragma unroll
     for (int m = 0; m < 2; m++)
 #pragma unroll
         for (int c = 0; c < CT; c++)
-            put_channels<VEC>(kd + m * g.dh, g.dh, 32 * c, dk[m][c], m ? -g.scale : g.scale, live,
-                              g.acc_kv);
+            put_channels<VEC>(kd + m * g.dh, g.dh, 32 * c, dk[m][c], m ? -fk : fk, fk2, live, g.acc_kv);
 #pragma unroll
     for (int c = 0; c < VT; c++)
-        put_channels<VEC>(vd, 2 * g.dh, 32 * c, dv[c], 1.0f, live, g.acc_kv);
+        put_channels<VEC>(vd, 2 * g.dh, 32 * c, dv[c], down_of(dup) * sgn, down_of(pup), live, g.acc_kv);
 }
 
 // Token rows of a block of the backward's first pass, and its blocks: at most

@@ -17,8 +17,9 @@ from diffref import D, act, diff_attn, rotary
 pytestmark = pytest.mark.gpu
 
 
-def block64(c, heads, th, x, mem, ps, lam0, kind):
-    """Block with DiffSelfAttn and Mlp from the parameters in their order."""
+def block64(c, heads, th, x, mem, ps, lam0, kind, parts):
+    """Block with DiffSelfAttn and Mlp from the parameters in their order; parts
+    receives the attention's O and P_2 V."""
     n, t, _ = x.shape
     F, it = torch.nn.functional, iter(ps)
     lin = lambda v, fout: v @ next(it).view(fout, -1).T + next(it)
@@ -39,7 +40,7 @@ def block64(c, heads, th, x, mem, ps, lam0, kind):
     q, k = (v.reshape(n, t, heads, 2, dh) for v in qk.split(c, -1))
     see = torch.ones(n, t, t, dtype=torch.bool)
     a = diff_attn(q, k, qkv[..., 2 * c:].reshape(n, t, heads, 2 * dh), lam.view(1, 4, dh), gain,
-                  see, 1 / math.sqrt(dh), lam0, 1e-5)
+                  see, 1 / math.sqrt(dh), lam0, 1e-5, parts)
     a = a @ wp.view(c, c).T + bp
     w9, b9 = next(it).view(9, c), next(it)
     img = F.pad(h.view(n, th, th, c), (0, 0, 1, 1, 1, 1))
@@ -66,8 +67,12 @@ def test_block(rnn, n, c, heads, th, kind):
     dz = torch.randn(n, th * th, c, generator=g)
     xl = x.to(D).requires_grad_(True)
     leaves = [p.v.cpu().to(D).requires_grad_(True) for p in ps]
-    want = block64(c, heads, th, xl, None, leaves, blk.attn.core.lam_init, kind)
-    grads = torch.autograd.grad(want, [xl] + leaves, dz.to(D))
+    parts = {}
+    want = block64(c, heads, th, xl, None, leaves, blk.attn.core.lam_init, kind, parts)
+    do, *grads = torch.autograd.grad(want, [parts["o"], xl] + leaves, dz.to(D))
+    lam = blk.attn.lam.v.cpu().to(D).view(4, -1)
+    lam_size = float((do.norm(dim=-1) * parts["o2"].norm(dim=-1)).norm().detach() * lam.norm()
+                     * torch.exp((lam[::2] * lam[1::2]).sum(-1)).max())
     y = blk.forward(x.cuda(), None, True, 0)
     assert rel_frob(y.cpu(), want.detach()) < TOL
     assert torch.equal(blk.forward(x.cuda(), None, False, 0), y)
@@ -75,8 +80,9 @@ def test_block(rnn, n, c, heads, th, kind):
     assert rel_frob(dx.cpu(), grads[0]) < TOL
     for i, (p, ref) in enumerate(zip(ps, grads[1:])):
         err = float((p.g.cpu().to(D) - ref).norm())
-        # lambda's vectors: a sum of cancelling terms (test_gpu_diffattn.py)
-        size = float(ref.norm()) if p is not blk.attn.lam else 1.0
+        # lambda's vectors: a sum of terms dO . (P_2 V) that the norm makes small
+        # beside |dO| |P_2 V|, which its error goes by (test_gpu_diffattn.py)
+        size = float(ref.norm()) if p is not blk.attn.lam else lam_size
         assert err < TOL * size, (i, err, size)
 
 
