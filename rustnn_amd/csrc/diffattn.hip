@@ -28,10 +28,10 @@ struct DiffArgs {
     float *dout;  // dO, [n][tq][h][2 dh]
     float *rec;   // [n][tq][h][8]: the forward's stats, D_1, D_2, |dO|, lambda
     float *part32, *pstat;  // splits: outputs [n][tq][h][splits][2][2 dh], (max, sum) beside them
-    double *part; // partials of dgain and dlambda, [blocks][2 dh + h]
+    double *part; // partials of dgain and dlambda, [blocks][2 dh + groups of a block]
     long long qstride, kvstride;
     int n, h, hkv, dh, tq, tk, koff, voff, lam_heads, diag, causal, group;
-    int acc_q, acc_kv, rpb, split_keys;
+    int acc_q, acc_kv, split_keys;
     float scale, lam_init, eps;
 };
 
@@ -117,6 +117,8 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef __fp16 g4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f2 __attribute__((ext_vector_type(2)));
+typedef float f2u __attribute__((ext_vector_type(2), aligned(4)));
+typedef float f4 __attribute__((ext_vector_type(4)));
 
 struct Half2 {
     h8 hi, lo;
@@ -324,7 +326,9 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const float *p, int 
     return make_rsrc(p, rows > 0 ? ((uint32_t)(rows - 1) * (uint32_t)stride + width) * 4u : 0u);
 }
 
-constexpr float P_UP = 16384.0f, P_EXP = 14.0f;  // softmax values enter the products times 2^14
+// Softmax values enter the products times 2^6, relative to a reference that a row's
+// largest score may pass by 2^8 before it moves: at most 2^14.
+constexpr float P_UP = 64.0f, P_EXP = 6.0f, SLACK = 8.0f;
 constexpr float NO_MAX = -1e30f;                 // a running maximum before any score
 
 // The block's number in an order in which each XCD (block id % 8) gets a
@@ -463,9 +467,10 @@ template <int DHP, bool VEC, int QG, bool SPLIT>
 __global__ __launch_bounds__(128 * QG)
 __attribute__((amdgpu_waves_per_eu(QG == 4 || DHP <= 32 ? 2 : 1))) void
 diff_fwd_kernel(DiffArgs g) {
-    constexpr int W = 2 * DHP, TK = 64, NT = 128 * QG, KS = DHP / 16, CT = DHP / 16;
+    constexpr int W = 2 * DHP, TK = QG < 4 && DHP > 32 ? 32 : 64, NT = 128 * QG, KS = DHP / 16;
+    constexpr int CT = DHP / 16, S2 = TK / 32;
     using Tile = HalfTile<TK, W>;
-    static_assert((int)sizeof(_Float16) * 2 * Tile::HALVES >= QG * CT * 16 * 64 * 4, "exchange");
+    static_assert((int)sizeof(_Float16) * 4 * Tile::HALVES >= QG * CT * 16 * 64 * 4, "exchange");
     __shared__ __align__(16) _Float16 lds[2][2 * Tile::HALVES];
     __shared__ float tmax[2][2][2 * QG];
     const int lane = threadIdx.x & 63, wave = wave_index(), lr = lane & 31, lh = lane >> 5;
@@ -505,20 +510,18 @@ diff_fwd_kernel(DiffArgs g) {
 #pragma unroll
         for (int r = 0; r < 16; r++) o[c][r] = 0.f;
     float m = NO_MAX, l = 0.f;
-    // powers of two: of the tile that is staged (.1), and the output's unit
-    float kup1 = 1.f, vup1 = 0.f, vdown = 0.f;
+    // powers of two of the tile that is staged, from the largest magnitudes (of
+    // the values: so far, so that the output's unit hardly changes)
+    float kup1 = 1.f, vup1 = 1.f, vup = 1.f, mv = 0.f;
     auto stage = [&](int t) {
-        float mk = 0.f, mv = 0.f;
+        float mk = 0.f;
 #pragma unroll
         for (int i = 0; i < 2 * QG; i++) {
             mk = max2(mk, tmax[t & 1][0][i]);
             mv = max2(mv, tmax[t & 1][1][i]);
         }
         kup1 = up_of(mk);
-        // the output's unit follows the tile's; at most 2^60 down at once, so
-        // that what is there does not overflow
-        const float up = up_of(mv);
-        vup1 = t ? fminf(up, vup1 * 0x1p60f) : up;
+        vup1 = up_of(mv);
         st.store(lds[t & 1], kup1, vup1);
     };
     if (ntile) {
@@ -532,27 +535,23 @@ diff_fwd_kernel(DiffArgs g) {
         const int k0 = kbeg + t * TK;
         __syncthreads();
         const _Float16 *const kt = lds[t & 1], *const vt = kt + Tile::HALVES;
-        const float f = down_of(kup1) * qdown, turn = vdown * vup1;
-        vdown = down_of(vup1);
+        const float f = down_of(kup1) * qdown, turn = down_of(vup) * vup1;
+        vup = vup1;
         // (past the last tile: zeros, into a buffer that nothing reads)
         stage(t + 1);
         st.load(k0 + 2 * TK);
-        f32x16 u[2];
+        f32x16 u[S2];
 #pragma unroll
-        for (int s2 = 0; s2 < 2; s2++) {
+        for (int s2 = 0; s2 < S2; s2++) {
 #pragma unroll
             for (int r = 0; r < 16; r++) u[s2][r] = 0.f;
             dot_along<Tile>(kt + 32 * s2 * Tile::STRIDE, map * DHP, q, u[s2]);
         }
-#pragma unroll
-        for (int s2 = 0; s2 < 2; s2++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) u[s2][r] *= f;
         const bool whole = k0 + TK <= nk && !(g.causal && k0 + TK - 1 > w_first + shift) &&
                            !(g.diag && k0 <= w_last && w_first < k0 + TK);
         if (!whole) {
 #pragma unroll
-            for (int s2 = 0; s2 < 2; s2++)
+            for (int s2 = 0; s2 < S2; s2++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
                     const int j = k0 + 32 * s2 + 8 * (r >> 2) + 4 * lh + (r & 3);
@@ -560,39 +559,45 @@ diff_fwd_kernel(DiffArgs g) {
                     u[s2][r] = in ? u[s2][r] : -INFINITY;
                 }
         }
-        float mn = m;
+        float top = u[0][0];
 #pragma unroll
-        for (int r = 0; r < 16; r++) mn = max3(mn, u[0][r], u[1][r]);
-        mn = pair32(mn, max2);
-        const float al = __builtin_amdgcn_exp2f(m - mn), base = mn - P_EXP;
-        m = mn;
-        Half2 p[4];
+        for (int s2 = 0; s2 < S2; s2++)
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) top = max3(top, u[s2][r], u[s2][r + 1]);
+        // (a score times f: f > 0 keeps the order)
+        top = pair32(top, max2) * f;
+        // the reference moves where a score passes it by the slack, the output's
+        // unit where the tile's does; both rarely after the first tile
+        const bool moves = top > m + SLACK;
+        if (__any(moves || turn != 1.0f)) {
+            const float mn = moves ? top : m, al = __builtin_amdgcn_exp2f(m - mn), keep = al * turn;
+            m = mn;
+            l *= al;
+#pragma unroll
+            for (int c = 0; c < CT; c++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) o[c][r] *= keep;
+        }
+        const float base = P_EXP - m;
+        Half2 p[2 * S2];
         float ps[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int s = 0; s < 2; s++) {
+        for (int s = 0; s < S2; s++) {
 #pragma unroll
             for (int r = 0; r < 16; r++) {
-                u[s][r] = __builtin_amdgcn_exp2f(u[s][r] - base);
+                u[s][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(u[s][r], f, base));
                 ps[r & 3] += u[s][r];
             }
             split16(u[s], *(Half2(*)[2]) & p[2 * s]);
         }
-        l = __builtin_fmaf(l, al, (ps[0] + ps[1]) + (ps[2] + ps[3]));
-        const float keep = al * turn;
+        l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
 #pragma unroll
-        for (int c = 0; c < CT; c++) {
-            f32x16 a;
-#pragma unroll
-            for (int r = 0; r < 16; r++) a[r] = 0.f;
-            dot_across<Tile>(vt, 32 * c, p, a);
-#pragma unroll
-            for (int r = 0; r < 16; r++) o[c][r] = __builtin_fmaf(o[c][r], keep, a[r]);
-        }
+        for (int c = 0; c < CT; c++) dot_across<Tile>(vt, 32 * c, p, o[c]);
         st.maxima(tmax[t & 1][0], tmax[t & 1][1]);
     }
     l = pair32(l, add2);
     const bool some = live && l > 0.f;
-    const float il = some ? vdown / l : 0.f;  // both carry 2^14
+    const float il = some ? down_of(vup) / l : 0.f;  // both carry 2^6
 #pragma unroll
     for (int c = 0; c < CT; c++)
 #pragma unroll
@@ -667,209 +672,279 @@ diff_fwd_kernel(DiffArgs g) {
     }
 }
 
-// The splits of diff_fwd_kernel joined: one wave per (image, query, head); lane
-// c holds channels c and c + 64.  Each map: M = max of the splits' maxima,
-// weights l_s 2^(m_s - M), in split order.
+// The splits of diff_fwd_kernel joined, WPR waves per (image, query, head): each
+// map's M = max of the splits' maxima, weights l_s 2^(m_s - M).  Lane s holds
+// split s's statistics (at most 64 splits); wave w adds the splits w, w + WPR, ...
+// in order, eight loads ahead, then the waves' sums are added in order.  Lane c
+// holds channels 2 c and 2 c + 1.
+template <int WPR>
 __global__ __launch_bounds__(256) void diff_join_kernel(DiffArgs g, int splits) {
-    const int lane = threadIdx.x & 63;
-    const long long w = (long long)blockIdx.x * 4 + wave_index();
-    if (w >= (long long)g.n * g.tq * g.h) return;
+    __shared__ f2 sums[4][2][64];
+    const int lane = threadIdx.x & 63, wave = wave_index(), part = wave % WPR;
+    const long long w = (long long)blockIdx.x * (4 / WPR) + wave / WPR;
+    const long long total = (long long)g.n * g.tq * g.h;
+    if (WPR == 1 && w >= total) return;
     const int hd = (int)(w % g.h), dv = 2 * g.dh;
-    float o[2][2], st[4];
+    const f4 st = lane < splits ? *(const f4 *)(g.pstat + (w * splits + lane) * 4)
+                                : f4{NO_MAX, 0.f, NO_MAX, 0.f};
+    const float M0 = wave_max(st[1] > 0.f ? st[0] : NO_MAX);
+    const float M1 = wave_max(st[3] > 0.f ? st[2] : NO_MAX);
+    const float w0 = st[1] > 0.f ? st[1] * __builtin_amdgcn_exp2f(st[0] - M0) : 0.f;
+    const float w1 = st[3] > 0.f ? st[3] * __builtin_amdgcn_exp2f(st[2] - M1) : 0.f;
+    const float t0 = wave_sum(w0), t1 = wave_sum(w1);
+    f2 o0 = {0.f, 0.f}, o1 = o0;
+    const int c = 2 * lane;
+    if (c < dv) {
+        const float *src = g.part32 + w * splits * 2 * dv + c;
+        for (int s0 = part; s0 < splits; s0 += 8 * WPR) {
+            f2 a[8], b[8];
 #pragma unroll
-    for (int mp = 0; mp < 2; mp++) {
-        float M = NO_MAX;
-        for (int s0 = 0; s0 < splits; s0 += 64) {
-            const int s = s0 + lane;
-            if (s < splits) {
-                const f2 v = *(const f2 *)(g.pstat + ((w * splits + s) * 2 + mp) * 2);
-                if (v[1] > 0.f) M = fmaxf(M, v[0]);
+            for (int i = 0; i < 8; i++) {
+                const long long at = (long long)min(s0 + i * WPR, splits - 1) * 2 * dv;
+                a[i] = *(const f2 *)(src + at);
+                b[i] = *(const f2 *)(src + at + dv);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int s = s0 + i * WPR;
+                if (s >= splits) break;
+                const float x = __shfl(w0, s, 64), y = __shfl(w1, s, 64);
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    o0[e] = __builtin_fmaf(x, a[i][e], o0[e]);
+                    o1[e] = __builtin_fmaf(y, b[i][e], o1[e]);
+                }
             }
         }
-        M = wave_max(M);
-        float tot = 0.f;
-        o[mp][0] = o[mp][1] = 0.f;
-        for (int s = 0; s < splits; s++) {
-            const long long at = (w * splits + s) * 2 + mp;
-            const f2 v = *(const f2 *)(g.pstat + at * 2);
-            const float wt = v[1] > 0.f ? v[1] * __builtin_amdgcn_exp2f(v[0] - M) : 0.f;
-            tot += wt;
-#pragma unroll
-            for (int u = 0; u < 2; u++)
-                if (lane + 64 * u < dv)
-                    o[mp][u] = __builtin_fmaf(wt, g.part32[at * dv + lane + 64 * u], o[mp][u]);
+    }
+    if constexpr (WPR > 1) {
+        sums[wave][0][lane] = o0;
+        sums[wave][1][lane] = o1;
+        __syncthreads();
+        if (part) return;
+        for (int i = 1; i < WPR; i++) {
+            o0 += sums[wave + i][0][lane];
+            o1 += sums[wave + i][1][lane];
         }
-        const float il = tot > 0.f ? 1.0f / tot : 0.f;
-        o[mp][0] *= il;
-        o[mp][1] *= il;
-        st[2 * mp] = tot > 0.f ? M : 0.f;
-        st[2 * mp + 1] = tot > 0.f ? P_UP / tot : 0.f;
     }
-    double e1, e2;
-    lambda_terms(g.lam, g.lam_heads, g.dh, hd, &e1, &e2);
-    const float lam = (float)(e1 - e2 + (double)g.lam_init);
-    float out[2], ss = 0.f;
-    for (int u = 0; u < 2; u++) {
-        out[u] = o[0][u] - lam * o[1][u];
-        if (lane + 64 * u < dv) ss += out[u] * out[u];
+    o0 *= t0 > 0.f ? 1.0f / t0 : 0.f;
+    o1 *= t1 > 0.f ? 1.0f / t1 : 0.f;
+    const float lam = lane_lambda(g, hd);
+    f2 out = o0 - lam * o1;
+    float rn = 1.0f;
+    f2 gn = {1.f, 1.f};
+    if (g.gain) {
+        const float ss = wave_sum(out[0] * out[0] + out[1] * out[1]);
+        rn = (1.0f / sqrtf(ss / (float)dv + g.eps)) * (1.0f - g.lam_init);
+        if (c < dv) gn = f2{g.gain[c], g.gain[c + 1]};
     }
-    const float rn = (1.0f / sqrtf(wave_sum(ss) / (float)dv + g.eps)) * (1.0f - g.lam_init);
-    for (int u = 0; u < 2; u++) {
-        const int c = lane + 64 * u;
-        if (c >= dv) continue;
-        g.y[w * dv + c] = g.gain ? out[u] * rn * g.gain[c] : out[u];
+    if (c < dv) {
+        out *= rn;
+        *(f2u *)(g.y + w * dv + c) = out * gn;
         if (g.o12) {
-            g.o12[(w * 2) * dv + c] = o[0][u];
-            g.o12[(w * 2 + 1) * dv + c] = o[1][u];
+            *(f2u *)(g.o12 + (w * 2) * dv + c) = o0;
+            *(f2u *)(g.o12 + (w * 2 + 1) * dv + c) = o1;
         }
     }
-    if (g.stats && lane == 0) *(float4 *)(g.stats + w * 4) = make_float4(st[0], st[1], st[2], st[3]);
+    if (g.stats && lane == 0)
+        *(f4 *)(g.stats + w * 4) = f4{t0 > 0.f ? M0 : 0.f, t0 > 0.f ? P_UP / t0 : 0.f,
+                                      t1 > 0.f ? M1 : 0.f, t1 > 0.f ? P_UP / t1 : 0.f};
 }
 
-// Backward's first pass: dO, D_1 and D_2 of the rows [blk rpb, (blk + 1) rpb) of
-// tokens, and the block's partials of dgain and dlambda.  One wave per (row,
-// head), lane c on channels c and c + 64.  The dots are 64-bit sums: dO is
+// Backward's first pass: dO, D_1 and D_2 of every (row, head), and the block's
+// partials of dgain and dlambda.  LPU lanes a unit, four channels each (VEC), or a
+// wave (LPU 64), two each; a group of lanes keeps one head, the groups in the
+// grid being a multiple of the heads.  The dots are 64-bit sums: dO is
 // perpendicular to O, so that D_2, whose sum dlambda is, is small beside its
 // terms.
+template <int LPU>
+__device__ __forceinline__ float group_sum(float v) {
+    v += dpp_f<0xB1>(v);
+    v += dpp_f<0x4E>(v);
+    v += dpp_f<0x141>(v);
+    if (LPU > 8) v += dpp_f<0x140>(v);
+    if (LPU > 16) v = pair16(v, add2);
+    if (LPU > 32) v = pair32(v, add2);
+    return v;
+}
+template <int LPU>
+__device__ __forceinline__ double group_sum(double v) {
+    v += rnn_dpp_d<0xB1>(v);
+    v += rnn_dpp_d<0x4E>(v);
+    v += rnn_dpp_d<0x141>(v);
+    if (LPU > 8) v += rnn_dpp_d<0x140>(v);
+    if (LPU > 16) v += __shfl_xor(v, 16, 64);
+    if (LPU > 32) v += __shfl_xor(v, 32, 64);
+    return v;
+}
+template <int LPU>
 __global__ __launch_bounds__(256) void diff_bwd_pre_kernel(DiffArgs g) {
-    extern __shared__ double sh[];  // [4][2 dh + h]
-    const int lane = threadIdx.x & 63, wv = wave_index(), dv = 2 * g.dh, cols = dv + g.h;
-    double dg[2] = {0.0, 0.0};
-    const int rows = g.n * g.tq, r0 = (int)blockIdx.x * g.rpb, r1 = min(rows, r0 + g.rpb);
-    float gain[2] = {0.f, 0.f};
+    constexpr bool VEC = LPU < 64;
+    constexpr int E = VEC ? 4 : 2, GPB = 256 / LPU;  // channels a lane, groups a block
+    __shared__ double sh[GPB][128];
+    const int c0 = ((int)threadIdx.x % LPU) * E, grp = (int)threadIdx.x / LPU, dv = 2 * g.dh;
+    const bool in = c0 < dv;
+    const int stride = (int)gridDim.x * GPB;  // a multiple of h
+    const int unit0 = (int)blockIdx.x * GPB + grp, hd = unit0 % g.h;
+    const float *lp = g.lam + (g.lam_heads > 1 ? (long long)hd * 4 * g.dh : 0);
+    double e1 = 0.0, e2 = 0.0;
+    for (int c = (int)threadIdx.x % LPU; c < g.dh; c += LPU) {
+        e1 += (double)lp[c] * (double)lp[g.dh + c];
+        e2 += (double)lp[2 * g.dh + c] * (double)lp[3 * g.dh + c];
+    }
+    e1 = exp(group_sum<LPU>(e1));
+    e2 = exp(group_sum<LPU>(e2));
+    const float lam = (float)(e1 - e2 + (double)g.lam_init);
+    float gain[E];
+    double dg[E], dl = 0.0;
 #pragma unroll
-    for (int u = 0; u < 2; u++)
-        if (g.gain && lane + 64 * u < dv) gain[u] = g.gain[lane + 64 * u] * (1.0f - g.lam_init);
-    for (int hd = 0; hd < g.h; hd++) {
-        double e1, e2;
-        lambda_terms(g.lam, g.lam_heads, g.dh, hd, &e1, &e2);
-        const float lam = (float)(e1 - e2 + (double)g.lam_init);
-        double dl = 0.0;
-        for (int row = r0 + wv; row < r1; row += 4) {
-            const long long w = (long long)row * g.h + hd;
-            const int b = row / g.tq, i = row % g.tq;
-            const bool live = i < len_of(g.qlen, b, g.tq);
-            float o1[2], o2[2], o[2], dy[2], d[2], ss = 0.f;
+    for (int e = 0; e < E; e++) {
+        gain[e] = g.gain && c0 + e < dv ? g.gain[c0 + e] * (1.0f - g.lam_init) : 0.f;
+        dg[e] = 0.0;
+    }
+    const int units = g.n * g.tq * g.h;
+    for (int u = unit0; u < units; u += stride) {
+        const int row = u / g.h, b = row / g.tq;
+        const bool live = row - b * g.tq < len_of(g.qlen, b, g.tq);
+        float o1[E], o2[E], o[E], dy[E], d[E], ss = 0.f;
+        const float *p1 = g.o12c + (long long)u * 2 * dv + c0, *py = g.dy + (long long)u * dv + c0;
+        if constexpr (VEC) {
+            const f4 z = {0.f, 0.f, 0.f, 0.f};
+            const f4 a = live && in ? *(const f4 *)p1 : z, c = live && in ? *(const f4 *)(p1 + dv) : z;
+            const f4 y = live && in ? *(const f4 *)py : z;
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const int c = lane + 64 * u;
-                const bool in = live && c < dv;
-                o1[u] = in ? g.o12c[(w * 2) * dv + c] : 0.f;
-                o2[u] = in ? g.o12c[(w * 2 + 1) * dv + c] : 0.f;
-                dy[u] = in ? g.dy[w * dv + c] : 0.f;
-                o[u] = o1[u] - lam * o2[u];
-                ss += o[u] * o[u];
-                d[u] = dy[u];
+            for (int e = 0; e < E; e++) o1[e] = a[e], o2[e] = c[e], dy[e] = y[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const bool ok = live && c0 + e < dv;
+                o1[e] = ok ? p1[e] : 0.f;
+                o2[e] = ok ? p1[dv + e] : 0.f;
+                dy[e] = ok ? py[e] : 0.f;
             }
-            if (g.gain) {
-                const float r = 1.0f / sqrtf(wave_sum(ss) / (float)dv + g.eps);
-                float s = 0.f;
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    o[u] *= r;
-                    s += dy[u] * gain[u] * o[u];
-                    dg[u] += (double)(dy[u] * o[u]);
-                }
-                s = wave_sum(s) / (float)dv;
-#pragma unroll
-                for (int u = 0; u < 2; u++) d[u] = r * (dy[u] * gain[u] - o[u] * s);
-            }
-            double d1 = 0.0, d2 = 0.0;
-            float nd = 0.f;
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const int c = lane + 64 * u;
-                if (c < dv) g.dout[w * dv + c] = d[u];
-                d1 += (double)d[u] * (double)o1[u];
-                d2 += (double)d[u] * (double)o2[u];
-                nd += d[u] * d[u];
-            }
-            d1 = rnn_wave_sum_d(d1);
-            d2 = rnn_wave_sum_d(d2);
-            nd = sqrtf(wave_sum(nd));
-            if (lane == 0) {
-                const float4 st = live ? *(const float4 *)(g.statsc + w * 4)
-                                       : make_float4(0.f, 0.f, 0.f, 0.f);
-                float4 *rec = (float4 *)(g.rec + w * 8);
-                rec[0] = st;
-                rec[1] = make_float4((float)d1, (float)d2, nd, lam);
-            }
-            dl += d2;
         }
-        if (lane == 0) sh[wv * cols + dv + hd] = -dl;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            o[e] = o1[e] - lam * o2[e];
+            ss += o[e] * o[e];
+            d[e] = dy[e];
+        }
+        if (g.gain) {
+            const float r = 1.0f / sqrtf(group_sum<LPU>(ss) / (float)dv + g.eps);
+            float s = 0.f;
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                o[e] *= r;
+                s += dy[e] * gain[e] * o[e];
+                dg[e] += (double)dy[e] * (double)o[e];
+            }
+            s = group_sum<LPU>(s) / (float)dv;
+#pragma unroll
+            for (int e = 0; e < E; e++) d[e] = r * (dy[e] * gain[e] - o[e] * s);
+        }
+        double d1 = 0.0, d2 = 0.0;
+        float nd = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            d1 += (double)d[e] * (double)o1[e];
+            d2 += (double)d[e] * (double)o2[e];
+            nd += d[e] * d[e];
+        }
+        d1 = group_sum<LPU>(d1);
+        d2 = group_sum<LPU>(d2);
+        nd = sqrtf(group_sum<LPU>(nd));
+        float *pd = g.dout + (long long)u * dv + c0;
+        if constexpr (VEC) {
+            if (in) *(f4 *)pd = f4{d[0], d[1], d[2], d[3]};
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                if (c0 + e < dv) pd[e] = d[e];
+        }
+        if (c0 == 0) {
+            const f4 z = {0.f, 0.f, 0.f, 0.f};
+            f4 *rec = (f4 *)(g.rec + (long long)u * 8);
+            rec[0] = live ? *(const f4 *)(g.statsc + (long long)u * 4) : z;
+            rec[1] = f4{(float)d1, (float)d2, nd, lam};
+        }
+        dl += d2;
     }
 #pragma unroll
-    for (int u = 0; u < 2; u++)
-        if (lane + 64 * u < dv)
-            sh[wv * cols + lane + 64 * u] = dg[u] * (double)(1.0f - g.lam_init);
+    for (int e = 0; e < E; e++)
+        if (c0 + e < dv) sh[grp][c0 + e] = dg[e] * (double)(1.0f - g.lam_init);
+    double *part = g.part + (long long)blockIdx.x * (dv + GPB);
+    if (c0 == 0) part[dv + grp] = -dl;
     __syncthreads();
-    for (int c = threadIdx.x; c < cols; c += 256)
-        g.part[(long long)blockIdx.x * cols + c] =
-            sh[c] + sh[cols + c] + sh[2 * cols + c] + sh[3 * cols + c];
+    for (int c = threadIdx.x; c < dv; c += 256) {
+        double t = 0.0;
+        for (int i = 0; i < GPB; i++) t += sh[i][c];
+        part[c] = t;
+    }
 }
 
-// dgain and dlam from the blocks' partials: the block's 16 groups of rows
-// each in order, then the groups in order.  Block 0 takes lambda's columns,
-// block 1 + i the gain's columns [16 i, 16 i + 16).
+// dgain and dlam from the blocks' partials.  Block i < ceil(dv / 16): the gain's
+// columns [16 i, 16 i + 16), 16 groups of partials each in order, then the groups
+// in order.  The others: one set of lambda vectors each, the partials of its
+// heads (every group of every block for a shared set, else group index % h = head)
+// in 256 strided sums, added in a fixed tree.
 __global__ __launch_bounds__(256) void diff_bwd_params_kernel(const double *__restrict__ part,
-                                                              int nblk, const float *lam,
+                                                              int nblk, int gpb, const float *lam,
                                                               int lam_heads, int dh, int h,
                                                               float *dlam, float *dgain) {
-    __shared__ double red[16][16];
-    __shared__ double tot[16];
-    const int dv = 2 * dh, cols = dv + h, jl = threadIdx.x % 16, q = threadIdx.x / 16;
+    const int dv = 2 * dh, cols = dv + gpb, ngain = dgain ? (dv + 15) / 16 : 0;
     const int lane = threadIdx.x & 63, wv = wave_index();
-    const int per = (nblk + 15) / 16, k0 = min(nblk, q * per), k1 = min(nblk, k0 + per);
-    const bool gain = blockIdx.x > 0;
-    const int first = gain ? 16 * ((int)blockIdx.x - 1) : 0, end = gain ? dv : h;
-    // a shared lambda's gradient: the heads' in order
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    double shared_dl = 0.0;
-    for (int j0 = first; j0 < (gain ? first + 1 : end); j0 += 16) {
-        const int j = j0 + jl;
+    if ((int)blockIdx.x < ngain) {
+        __shared__ double red[16][16];
+        const int jl = threadIdx.x % 16, q = threadIdx.x / 16, j = 16 * (int)blockIdx.x + jl;
+        const int per = (nblk + 15) / 16, k0 = min(nblk, q * per), k1 = min(nblk, k0 + per);
+        const double *src = part + min(j, dv - 1);
         double s = 0.0;
-        if (j < end)
-            for (int k = k0; k < k1; k++) s += part[(long long)k * cols + (gain ? j : dv + j)];
+        for (int k = k0; k < k1; k += 16) {
+            double v[16];
+#pragma unroll
+            for (int u = 0; u < 16; u++) v[u] = src[(long long)min(k + u, k1 - 1) * cols];
+#pragma unroll
+            for (int u = 0; u < 16; u++)
+                if (k + u < k1) s += v[u];
+        }
         red[q][jl] = s;
         __syncthreads();
-        if (q == 0) {
+        if (q == 0 && j < dv) {
             double t = 0.0;
             for (int u = 0; u < 16; u++) t += red[u][jl];
-            tot[jl] = t;
-            if (gain && j < end) dgain[j] += (float)t;
+            dgain[j] += (float)t;
         }
-        __syncthreads();
-        if (!gain) {
-            if (lam_heads == 1) {
-                for (int u = 0; u < 16 && j0 + u < h; u++) shared_dl += tot[u];
-            } else {
-                for (int u = wv; u < 16 && j0 + u < h; u += 4) {
-                    double e1, e2;
-                    lambda_terms(lam, lam_heads, dh, j0 + u, &e1, &e2);
-                    const float *l = lam + (long long)(j0 + u) * 4 * dh;
-                    float *d = dlam + (long long)(j0 + u) * 4 * dh;
-                    if (lane < dh) {
-                        d[lane] += (float)(tot[u] * e1 * l[dh + lane]);
-                        d[dh + lane] += (float)(tot[u] * e1 * l[lane]);
-                        d[2 * dh + lane] -= (float)(tot[u] * e2 * l[3 * dh + lane]);
-                        d[3 * dh + lane] -= (float)(tot[u] * e2 * l[2 * dh + lane]);
-                    }
-                }
-            }
-        }
-        __syncthreads();
+        return;
     }
-    (void)acc;
-    if (!gain && lam_heads == 1 && wv == 0) {
-        double e1, e2;
-        lambda_terms(lam, 1, dh, 0, &e1, &e2);
-        if (lane < dh) {
-            const double t = shared_dl;
-            dlam[lane] += (float)(t * e1 * lam[dh + lane]);
-            dlam[dh + lane] += (float)(t * e1 * lam[lane]);
-            dlam[2 * dh + lane] -= (float)(t * e2 * lam[3 * dh + lane]);
-            dlam[3 * dh + lane] -= (float)(t * e2 * lam[2 * dh + lane]);
+    __shared__ double sums[4];
+    const int set = (int)blockIdx.x - ngain, step = lam_heads > 1 ? h : 1;
+    const int groups = nblk * gpb;
+    double s = 0.0;
+    for (int k0 = set + step * (int)threadIdx.x; k0 < groups; k0 += step * 256 * 8) {
+        double v[8];
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+            const int k = min(k0 + u * step * 256, groups - 1);
+            v[u] = part[(long long)(k / gpb) * cols + dv + k % gpb];
         }
+#pragma unroll
+        for (int u = 0; u < 8; u++)
+            if (k0 + u * step * 256 < groups) s += v[u];
+    }
+    s = rnn_wave_sum_d(s);
+    if (lane == 0) sums[wv] = s;
+    __syncthreads();
+    if (wv) return;
+    const double t = sums[0] + sums[1] + sums[2] + sums[3];
+    double e1, e2;
+    lambda_terms(lam, lam_heads, dh, set, &e1, &e2);
+    const float *l = lam + (long long)set * 4 * dh;
+    float *d = dlam + (long long)set * 4 * dh;
+    if (lane < dh) {
+        d[lane] += (float)(t * e1 * l[dh + lane]);
+        d[dh + lane] += (float)(t * e1 * l[lane]);
+        d[2 * dh + lane] -= (float)(t * e2 * l[3 * dh + lane]);
+        d[3 * dh + lane] -= (float)(t * e2 * l[2 * dh + lane]);
     }
 }
 
@@ -1329,9 +1404,26 @@ diff_dkv_kernel(DiffArgs g) {
         put_channels<VEC>(vd, 2 * g.dh, 32 * c, dv[c], down_of(dup) * sgn, down_of(pup), live, g.acc_kv);
 }
 
-// Token rows of a block of the backward's first pass, and its blocks: at most
-// 1024, four rows or more each.
-int pre_rows(size_t rows) { return (int)std::max<size_t>(4, rnn_div_up(rows, 1024)); }
+// The backward's first pass: lanes of a unit and blocks, so that the groups of
+// lanes are a multiple of the heads and take about four units each.
+struct PrePlan {
+    int lpu;
+    size_t blocks;
+};
+PrePlan plan_pre(const rnn_diff_attn_desc *d, size_t n, bool vec) {
+    PrePlan p;
+    p.lpu = !vec ? 64 : d->dh <= 16 ? 8 : d->dh <= 32 ? 16 : 32;
+    const size_t gpb = 256 / p.lpu;
+    size_t a = gpb, b = d->h;
+    while (b) {
+        const size_t r = a % b;
+        a = b;
+        b = r;
+    }
+    const size_t mult = d->h / a, units = n * d->tq * d->h;
+    p.blocks = std::max<size_t>(1, std::min<size_t>(rnn_div_up(units, 4 * gpb), 1024) / mult) * mult;
+    return p;
+}
 
 // Row groups of 32 a workgroup of the forward, and the splits of the keys: a
 // power of two of groups up to four, keys split where the rows leave CUs idle.
@@ -1345,8 +1437,8 @@ FwdPlan plan_fwd(const rnn_diff_attn_desc *d, size_t n, bool vec) {
     p.qg = !vec ? 4 : R <= 32 ? 1 : R <= 64 ? 2 : 4;
     p.blocks = probs * rnn_div_up(R, (size_t)32 * p.qg);
     const size_t tiles = rnn_div_up(d->tk, (size_t)64);
-    size_t s = p.blocks ? std::min(tiles / 4, 512 / p.blocks) : 1;
-    s = std::max<size_t>(1, std::min<size_t>(s, 256));
+    size_t s = p.blocks && p.blocks < 256 ? std::min(tiles / 4, 512 / p.blocks) : 1;
+    s = std::max<size_t>(1, std::min<size_t>(s, 64));
     const size_t per = rnn_div_up(std::max<size_t>(tiles, 1), s);
     p.split_keys = (int)per * 64;
     p.splits = (int)rnn_div_up(std::max<size_t>(tiles, 1), per);
@@ -1364,8 +1456,12 @@ DiffWs plan_ws(const rnn_diff_attn_desc *d, size_t n, bool backward) {
     if (backward) {
         w.dout = cv.take(heads * 2 * d->dh * sizeof(float));
         w.rec = cv.take(heads * 8 * sizeof(float));
-        const size_t nblk = rows ? rnn_div_up(rows, (size_t)pre_rows(rows)) : 0;
-        w.part = cv.take(nblk * (2 * d->dh + d->h) * sizeof(double));
+        size_t part = 0;  // whichever alignment the operands turn out to have
+        for (int vec = 0; vec < 2; vec++) {
+            const PrePlan p = plan_pre(d, n, vec != 0);
+            part = std::max(part, p.blocks * (2 * d->dh + 256 / p.lpu));
+        }
+        w.part = cv.take(part * sizeof(double));
     } else {
         // whichever alignment the operands turn out to have
         const int splits = std::max(plan_fwd(d, n, true).splits, plan_fwd(d, n, false).splits);
@@ -1563,8 +1659,11 @@ int rnn_diff_attn_forward(rnn_ctx *ctx, const rnn_diff_attn_desc *d, size_t n, c
     }
     RNN_LAUNCHED(ctx);
     if (p.splits > 1) {
-        diff_join_kernel<<<(unsigned)rnn_div_up(n * d->tq * d->h, 4), 256, 0, ctx->stream>>>(
-            g, p.splits);
+        const size_t units = n * d->tq * d->h;
+        if (p.splits > 4)
+            diff_join_kernel<4><<<(unsigned)units, 256, 0, ctx->stream>>>(g, p.splits);
+        else
+            diff_join_kernel<1><<<(unsigned)rnn_div_up(units, 4), 256, 0, ctx->stream>>>(g, p.splits);
         RNN_LAUNCHED(ctx);
     }
     return RNN_OK;
@@ -1603,19 +1702,25 @@ int rnn_diff_attn_backward(rnn_ctx *ctx, const rnn_diff_attn_desc *d, size_t n, 
     g.part = (double *)((char *)ws + w.part);
     g.acc_q = (flags & RNN_ATTN_SET_DQ) ? 0 : 1;
     g.acc_kv = (flags & RNN_ATTN_SET_DKV) ? 0 : 1;
+    const bool vec = rows_vec(g);
     const size_t rows = n * d->tq;
     if (rows) {
-        g.rpb = pre_rows(rows);
-        const unsigned nblk = (unsigned)rnn_div_up(rows, (size_t)g.rpb);
-        const int cols = 2 * g.dh + g.h;
-        diff_bwd_pre_kernel<<<nblk, 256, 4 * cols * sizeof(double), ctx->stream>>>(g);
+        const PrePlan p = plan_pre(d, n, vec);
+        const unsigned nblk = (unsigned)p.blocks;
+        if (p.lpu == 8)
+            diff_bwd_pre_kernel<8><<<nblk, 256, 0, ctx->stream>>>(g);
+        else if (p.lpu == 16)
+            diff_bwd_pre_kernel<16><<<nblk, 256, 0, ctx->stream>>>(g);
+        else if (p.lpu == 32)
+            diff_bwd_pre_kernel<32><<<nblk, 256, 0, ctx->stream>>>(g);
+        else
+            diff_bwd_pre_kernel<64><<<nblk, 256, 0, ctx->stream>>>(g);
         RNN_LAUNCHED(ctx);
-        diff_bwd_params_kernel<<<1 + (gain ? (unsigned)rnn_div_up(2 * g.dh, 16) : 0u), 256, 0,
-                                 ctx->stream>>>(g.part, (int)nblk, lam, g.lam_heads, g.dh, g.h,
-                                                dlam, dgain);
+        const unsigned np = (gain ? (unsigned)rnn_div_up(2 * g.dh, 16) : 0u) + (unsigned)g.lam_heads;
+        diff_bwd_params_kernel<<<np, 256, 0, ctx->stream>>>(g.part, (int)nblk, 256 / p.lpu, lam,
+                                                            g.lam_heads, g.dh, g.h, dlam, dgain);
         RNN_LAUNCHED(ctx);
     }
-    const bool vec = rows_vec(g);
     switch ((g.dh + 15) / 16) {
         case 1: launch_bwd<16>(ctx, g, vec); break;
         case 2: launch_bwd<32>(ctx, g, vec); break;
