@@ -339,6 +339,7 @@ class Context:
     def set_stream(self, stream):
         ptr = stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream or 0)
         self.check(lib().rnn_ctx_set_stream(self.h, _vp(ptr)))
+        self.stream = ptr
 
     def stream_ptr(self) -> int:
         return lib().rnn_ctx_stream(self.h) or 0
@@ -410,20 +411,33 @@ def _new(n, like=None, device=0):
     return torch.empty(n, dtype=torch.float32, device=dev)
 
 
+_dtypes = {}
+
+
 def _arg(ctx, t, need, name, dtype="float32"):
-    """Device pointer of a contiguous tensor of ``dtype`` ("float32", or
+    """Device address of a contiguous tensor of ``dtype`` ("float32", or
     "u32": uint32 / int32) on the context's device with >= need elements."""
     if t is None:
         return None
-    import torch
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+    if not _dtypes:
+        import torch
+        _dtypes.update(tensor=torch.Tensor, float32=(torch.float32,),
+                       u32=(torch.int32, torch.uint32))
+    ok = _dtypes[dtype]
+    if not isinstance(t, _dtypes["tensor"]):
         raise TypeError(f"{name} must be a CUDA tensor")
-    want = (torch.float32,) if dtype == "float32" else (torch.uint32, torch.int32)
-    if t.dtype not in want:
-        raise TypeError(f"{name} must be {'/'.join(str(w)[6:] for w in want)} (got {t.dtype})")
-    if t.device.index != ctx.device:
-        raise ValueError(f"{name} is on cuda:{t.device.index}, the context on cuda:{ctx.device}")
-    return _ptr(t, need, name)
+    if (t.get_device() == ctx.device and t.dtype in ok and t.is_contiguous() and
+            t.numel() >= need):
+        return t.data_ptr() or None
+    if not t.is_cuda:
+        raise TypeError(f"{name} must be a CUDA tensor")
+    if t.dtype not in ok:
+        raise TypeError(f"{name} must be {'/'.join(str(w)[6:] for w in ok)} (got {t.dtype})")
+    if t.get_device() != ctx.device:
+        raise ValueError(f"{name} is on cuda:{t.get_device()}, the context on cuda:{ctx.device}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    raise ValueError(f"{name} has {t.numel()} elements, needs {need}")
 
 
 def _on_ctx_stream(ctx, *ts):
@@ -431,8 +445,8 @@ def _on_ctx_stream(ctx, *ts):
     that is not the current one, so that their memory is not handed out again
     before its work is done."""
     import torch
-    sp = ctx.stream_ptr()
-    if torch.cuda.current_stream(ctx.device).cuda_stream == sp:
+    sp = ctx.stream
+    if torch._C._cuda_getCurrentRawStream(ctx.device) == sp:
         return
     st = torch.cuda.ExternalStream(sp, device=ctx.device) if sp else \
         torch.cuda.default_stream(ctx.device)
@@ -766,17 +780,21 @@ class Rotary:
             raise ValueError("Rotary: a negative size")
         self.interleaved, self.ctx = bool(interleaved), ctx
         self.t = math.prod(self.grid)
+        self._descs = {}  # the C description of each layout
         w = self.heads * self.dh
         rc = lib().rnn_rotary_check(C.byref(self._desc(w, 0, w, 0)), 1, self.t, 0)
         if rc:
             raise ValueError(f"Rotary: {lib().rnn_status_string(rc).decode()} (heads={heads} "
                              f"dh={dh} grid={self.grid} pairs={self.pairs} base={base})")
 
-    def _desc(self, xstride, xoff, ystride, yoff):
-        p = self.pairs + (0,) * (3 - len(self.pairs))
-        g = self.grid + (1,) * (3 - len(self.grid))
-        return RotaryDesc(self.heads, self.dh, xstride, xoff, ystride, yoff, len(self.grid), *p,
-                          *g, int(self.interleaved), self.base)
+    def _desc(self, *layout):
+        d = self._descs.get(layout)
+        if d is None:
+            p = self.pairs + (0,) * (3 - len(self.pairs))
+            g = self.grid + (1,) * (3 - len(self.grid))
+            d = self._descs[layout] = RotaryDesc(self.heads, self.dh, *layout, len(self.grid), *p,
+                                                 *g, int(self.interleaved), self.base)
+        return d
 
     def _turn(self, n, x, xstride, xoff, pos, y, ystride, yoff, t, inverse):
         import torch
@@ -827,33 +845,38 @@ class DiffCore:
         self.scale = 1.0 / math.sqrt(max(self.dh, 1)) if scale is None else float(scale)
         self.lam_init, self.eps, self.ctx = float(lam_init), float(eps), ctx
         self.c = 2 * self.h * self.dh
+        self._plans = {}  # the C description and workspace of each layout and batch
         kw = 2 * self.hkv * self.dh
-        d = self.desc(self.c, 0, 2 * kw, 0, kw)
-        self._bytes(d, 1, 0)
+        self._plan(1, 0, (self.c, 0, 2 * kw, 0, kw))
 
     def desc(self, qstride, qoff, kvstride, koff, voff):
         return DiffAttnDesc(self.h, self.hkv, self.dh, self.tq, self.tk, qstride, qoff, kvstride,
                             koff, voff, self.lam_heads, int(self.mask_diag), int(self.causal),
                             self.scale, self.lam_init, self.eps)
 
-    def _bytes(self, d, n, backward):
-        nb = _sz()
+    def _plan(self, n, backward, layout):
+        """(description, workspace bytes, floats of q and of kv that it spans)."""
+        p = self._plans.get((n, backward, layout))
+        if p is not None:
+            return p
+        d, nb = self.desc(*layout), _sz()
         rc = lib().rnn_diff_attn_workspace(C.byref(d), n, backward, C.byref(nb))
         if rc:
             raise ValueError(f"DiffCore: {lib().rnn_status_string(rc).decode()} (h={self.h} "
                              f"hkv={self.hkv} dh={self.dh} tq={self.tq} tk={self.tk} n={n} "
                              f"lam_heads={self.lam_heads} scale={self.scale} "
-                             f"lam_init={self.lam_init} eps={self.eps})")
-        return nb.value
-
-    def _inputs(self, ctx, d, n, q, kv, lam, gain, qlen, klen):
-        kw = 2 * self.hkv * self.dh
+                             f"lam_init={self.lam_init} eps={self.eps} layout={layout})")
         nq = (n * self.tq - 1) * d.qstride + d.qoff + self.c if n * self.tq else 0
-        nkv = (n * self.tk - 1) * d.kvstride + max(d.koff, d.voff) + kw if n * self.tk else 0
-        return nq, nkv, (_arg(ctx, q, nq, "q"), _arg(ctx, kv, nkv, "kv"),
-                         _arg(ctx, lam, self.lam_heads * 4 * self.dh, "lam"),
-                         _arg(ctx, gain, 2 * self.dh, "gain"), _arg(ctx, qlen, n, "qlen", "u32"),
-                         _arg(ctx, klen, n, "klen", "u32"))
+        nkv = ((n * self.tk - 1) * d.kvstride + max(d.koff, d.voff) + 2 * self.hkv * self.dh
+               if n * self.tk else 0)
+        p = self._plans[n, backward, layout] = d, nb.value, nq, nkv
+        return p
+
+    def _inputs(self, ctx, n, nq, nkv, q, kv, lam, gain, qlen, klen):
+        return (_arg(ctx, q, nq, "q"), _arg(ctx, kv, nkv, "kv"),
+                _arg(ctx, lam, self.lam_heads * 4 * self.dh, "lam"),
+                _arg(ctx, gain, 2 * self.dh, "gain"), _arg(ctx, qlen, n, "qlen", "u32"),
+                _arg(ctx, klen, n, "klen", "u32"))
 
     def forward(self, n, q, qstride, qoff, kv, kvstride, koff, voff, lam, gain=None, qlen=None,
                 klen=None, train=True, y=None):
@@ -861,9 +884,8 @@ class DiffCore:
         klen (int32 / uint32 [n]): the images' lengths where they are padded."""
         import torch
         ctx = self.ctx or default_ctx(q.device.index or 0)
-        d = self.desc(qstride, qoff, kvstride, koff, voff)
-        nb = self._bytes(d, n, 0)
-        _, _, ins = self._inputs(ctx, d, n, q, kv, lam, gain, qlen, klen)
+        d, nb, nq, nkv = self._plan(n, 0, (qstride, qoff, kvstride, koff, voff))
+        ins = self._inputs(ctx, n, nq, nkv, q, kv, lam, gain, qlen, klen)
         rows = n * self.tq
         if y is None:
             y = torch.empty(n, self.tq, self.c, dtype=torch.float32, device=q.device)
@@ -888,9 +910,8 @@ class DiffCore:
         if saved is None:
             raise ValueError("DiffCore.backward: the forward did not keep its maps (train=False)")
         ctx = self.ctx or default_ctx(dy.device.index or 0)
-        d = self.desc(qstride, qoff, kvstride, koff, voff)
-        nb = self._bytes(d, n, 1)
-        nq, nkv, ins = self._inputs(ctx, d, n, q, kv, lam, gain, qlen, klen)
+        d, nb, nq, nkv = self._plan(n, 1, (qstride, qoff, kvstride, koff, voff))
+        ins = self._inputs(ctx, n, nq, nkv, q, kv, lam, gain, qlen, klen)
         rows = n * self.tq
         o12, stats = saved
         ws = torch.empty(nb, dtype=torch.uint8, device=dy.device) if nb else None

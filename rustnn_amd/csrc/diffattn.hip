@@ -39,16 +39,14 @@ __device__ __forceinline__ int len_of(const uint32_t *len, int b, int t) {
     return len ? (int)min(len[b], (uint32_t)t) : t;
 }
 
-// exp(lq1 . lk1) and exp(lq2 . lk2) of a head, on every lane.
-__device__ __forceinline__ void lambda_terms(const float *lam, int lam_heads, int dh, int head,
-                                             double *e1, double *e2) {
-    const int lane = threadIdx.x & 63;
+// lq1 . lk1 and lq2 . lk2 of a head, on every lane, summed in 64 bits.
+__device__ __forceinline__ void lambda_dots(const float *lam, int lam_heads, int dh, int head,
+                                            double *a, double *b) {
+    const int lane = threadIdx.x & 63, c = min(lane, dh - 1);
     const float *l = lam + (lam_heads > 1 ? (long long)head * 4 * dh : 0);
-    const bool in = lane < dh;
-    const double a = in ? (double)l[lane] * (double)l[dh + lane] : 0.0;
-    const double b = in ? (double)l[2 * dh + lane] * (double)l[3 * dh + lane] : 0.0;
-    *e1 = exp(rnn_wave_sum_d(a));
-    *e2 = exp(rnn_wave_sum_d(b));
+    const float x = l[c], y = l[dh + c], z = l[2 * dh + c], w = l[3 * dh + c];
+    *a = rnn_wave_sum_d(lane < dh ? (double)x * (double)y : 0.0);
+    *b = rnn_wave_sum_d(lane < dh ? (double)z * (double)w : 0.0);
 }
 
 // Maxima in one instruction each (fmaxf takes a second one to quiet NaNs).
@@ -300,25 +298,30 @@ __device__ __forceinline__ float absmax8(const float (&x)[8], float m) {
     return m;
 }
 
-// A lane's row of 16 N channels (of `lim` channels, zeros past them) as an operand:
-// times the power of two that its largest magnitude calls for, whose reciprocal
-// and the magnitude are returned.  The lanes l and l + 32 hold a row together.
-template <bool VEC, int N>
-__device__ __forceinline__ float load_row(__amdgpu_buffer_rsrc_t rs, uint32_t off, int lim,
-                                          Half2 (&x)[N], float *mx = nullptr) {
-    const int lh = (threadIdx.x >> 5) & 1;
-    float v[N][8], m = 0.f;
+// A lane's row of 16 N channels (of `lim` channels, zeros past them); the lanes l
+// and l + 32 hold it together.  split() makes it an operand, times the power of two
+// that its largest magnitude (mx) calls for, whose reciprocal is returned.
+template <int N>
+struct RowFrag {
+    float v[N][8], mx;
+    template <bool VEC>
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rs, uint32_t off, int lim) {
+        const int lh = (threadIdx.x >> 5) & 1;
 #pragma unroll
-    for (int s = 0; s < N; s++) load8<VEC>(rs, off + 16 * s + 8 * lh, lim - (16 * s + 8 * lh), v[s]);
+        for (int s = 0; s < N; s++)
+            load8<VEC>(rs, off + 16 * s + 8 * lh, lim - (16 * s + 8 * lh), v[s]);
+    }
+    __device__ __forceinline__ float split(Half2 (&x)[N]) {
+        mx = 0.f;
 #pragma unroll
-    for (int s = 0; s < N; s++) m = absmax8(v[s], m);
-    m = pair32(m, max2);
-    const float up = up_of(m);
+        for (int s = 0; s < N; s++) mx = absmax8(v[s], mx);
+        mx = pair32(mx, max2);
+        const float up = up_of(mx);
 #pragma unroll
-    for (int s = 0; s < N; s++) x[s] = half_split(v[s], up);
-    if (mx) *mx = m;
-    return down_of(up);
-}
+        for (int s = 0; s < N; s++) x[s] = half_split(v[s], up);
+        return down_of(up);
+    }
+};
 // A resource over `rows` rows (at most 64) of `stride` floats from p on, the last
 // of them `width` floats long.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const float *p, int rows, long long stride,
@@ -341,20 +344,17 @@ __device__ __forceinline__ long long xcd_order(long long id, long long total) {
 // Lambda of a lane's own head: the wave's one head together, else each lane its
 // own.
 __device__ __forceinline__ float lane_lambda(const DiffArgs &g, int head) {
-    double e1, e2;
+    double a = 0.0, b = 0.0;
     if (g.lam_heads == 1 || g.group == 1) {
-        lambda_terms(g.lam, g.lam_heads, g.dh, __builtin_amdgcn_readfirstlane(head), &e1, &e2);
+        lambda_dots(g.lam, g.lam_heads, g.dh, __builtin_amdgcn_readfirstlane(head), &a, &b);
     } else {
         const float *l = g.lam + (long long)head * 4 * g.dh;
-        double a = 0.0, b = 0.0;
         for (int c = 0; c < g.dh; c++) {
             a = fma((double)l[c], (double)l[g.dh + c], a);
             b = fma((double)l[2 * g.dh + c], (double)l[3 * g.dh + c], b);
         }
-        e1 = exp(a);
-        e2 = exp(b);
     }
-    return (float)(e1 - e2 + (double)g.lam_init);
+    return expf((float)a) - expf((float)b) + g.lam_init;
 }
 
 // Tiles of TK keys and values on their way to LDS: a thread's share in registers
@@ -495,15 +495,16 @@ diff_fwd_kernel(DiffArgs g) {
     if (ntile) st.load(kbeg);
     // the row's query of this map; the wave's queries
     const int w_first = row0 / g.group, w_last = min(nq - 1, (row0 + 31) / g.group);
-    Half2 q[KS];
     const int q0 = min(w_first, g.tq - 1);
-    float qdown = load_row<VEC>(rows_rsrc(g.q + ((long long)b * g.tq + q0) * g.qstride,
-                                          min(g.tq - q0, 32), g.qstride, 2 * g.h * g.dh),
-                                (uint32_t)(qi - q0) * (uint32_t)g.qstride + (2 * head + map) * g.dh,
-                                live ? g.dh : 0, q);
-    qdown *= g.scale * LOG2E;
+    Half2 q[KS];
+    RowFrag<KS> qf;
+    qf.template load<VEC>(rows_rsrc(g.q + ((long long)b * g.tq + q0) * g.qstride,
+                                    min(g.tq - q0, 32), g.qstride, 2 * g.h * g.dh),
+                          (uint32_t)(qi - q0) * (uint32_t)g.qstride + (2 * head + map) * g.dh,
+                          live ? g.dh : 0);
     float lam = 0.f;
     if (!SPLIT && map == 0) lam = lane_lambda(g, min(head, g.h - 1));
+    const float qdown = qf.split(q) * (g.scale * LOG2E);
     f32x16 o[CT];
 #pragma unroll
     for (int c = 0; c < CT; c++)
@@ -528,8 +529,10 @@ diff_fwd_kernel(DiffArgs g) {
         st.maxima(tmax[0][0], tmax[0][1]);
         __syncthreads();
         stage(0);
-        st.load(kbeg + TK);
-        st.maxima(tmax[1][0], tmax[1][1]);
+        if (ntile > 1) {
+            st.load(kbeg + TK);
+            st.maxima(tmax[1][0], tmax[1][1]);
+        }
     }
     for (int t = 0; t < ntile; t++) {
         const int k0 = kbeg + t * TK;
@@ -537,9 +540,8 @@ diff_fwd_kernel(DiffArgs g) {
         const _Float16 *const kt = lds[t & 1], *const vt = kt + Tile::HALVES;
         const float f = down_of(kup1) * qdown, turn = down_of(vup) * vup1;
         vup = vup1;
-        // (past the last tile: zeros, into a buffer that nothing reads)
-        stage(t + 1);
-        st.load(k0 + 2 * TK);
+        if (t + 1 < ntile) stage(t + 1);
+        if (t + 2 < ntile) st.load(k0 + 2 * TK);
         f32x16 u[S2];
 #pragma unroll
         for (int s2 = 0; s2 < S2; s2++) {
@@ -593,7 +595,7 @@ diff_fwd_kernel(DiffArgs g) {
         l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
 #pragma unroll
         for (int c = 0; c < CT; c++) dot_across<Tile>(vt, 32 * c, p, o[c]);
-        st.maxima(tmax[t & 1][0], tmax[t & 1][1]);
+        if (t + 2 < ntile) st.maxima(tmax[t & 1][0], tmax[t & 1][1]);
     }
     l = pair32(l, add2);
     const bool some = live && l > 0.f;
@@ -654,6 +656,13 @@ diff_fwd_kernel(DiffArgs g) {
     if (g.o12)
         store(g.o12 + (out * 2 + map) * dv, [&](int c, int r, int) { return o[c][r]; });
     if (map == 1) return;
+    // (the gain in registers before the stores, which its loads would wait for)
+    f32x16 gv[CT];
+#pragma unroll
+    for (int c = 0; c < CT; c++)
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+            gv[c][r] = g.gain ? g.gain[min(32 * c + 8 * (r >> 2) + 4 * lh + (r & 3), dv - 1)] : 1.f;
     float ss = 0.f;
 #pragma unroll
     for (int c = 0; c < CT; c++)
@@ -666,7 +675,7 @@ diff_fwd_kernel(DiffArgs g) {
     if (g.gain) {
         ss = pair32(ss, add2);
         rn = (1.0f / sqrtf(ss / (float)dv + g.eps)) * (1.0f - g.lam_init);
-        store(g.y + out * dv, [&](int c, int r, int ch) { return o[c][r] * rn * g.gain[ch]; });
+        store(g.y + out * dv, [&](int c, int r, int) { return o[c][r] * rn * gv[c][r]; });
     } else {
         store(g.y + out * dv, [&](int c, int r, int) { return o[c][r]; });
     }
@@ -792,9 +801,7 @@ __global__ __launch_bounds__(256) void diff_bwd_pre_kernel(DiffArgs g) {
         e1 += (double)lp[c] * (double)lp[g.dh + c];
         e2 += (double)lp[2 * g.dh + c] * (double)lp[3 * g.dh + c];
     }
-    e1 = exp(group_sum<LPU>(e1));
-    e2 = exp(group_sum<LPU>(e2));
-    const float lam = (float)(e1 - e2 + (double)g.lam_init);
+    const float lam = expf((float)group_sum<LPU>(e1)) - expf((float)group_sum<LPU>(e2)) + g.lam_init;
     float gain[E];
     double dg[E], dl = 0.0;
 #pragma unroll
@@ -937,7 +944,9 @@ __global__ __launch_bounds__(256) void diff_bwd_params_kernel(const double *__re
     if (wv) return;
     const double t = sums[0] + sums[1] + sums[2] + sums[3];
     double e1, e2;
-    lambda_terms(lam, lam_heads, dh, set, &e1, &e2);
+    lambda_dots(lam, lam_heads, dh, set, &e1, &e2);
+    e1 = exp(e1);
+    e2 = exp(e2);
     const float *l = lam + (long long)set * 4 * dh;
     float *d = dlam + (long long)set * 4 * dh;
     if (lane < dh) {
@@ -1012,12 +1021,19 @@ diff_dq_kernel(DiffArgs g) {
         dd = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rr, at + 16u, 0, 0));
     }
     Half2 q[2][KS], d[VS];
-    float qdown[2];
+    float qdown[2], ddown;
+    {
+        RowFrag<KS> qf[2];
+        RowFrag<VS> df;
 #pragma unroll
-    for (int m = 0; m < 2; m++)
-        qdown[m] = load_row<VEC>(rq, (uint32_t)qx * (uint32_t)g.qstride + (2 * head + m) * g.dh,
-                                 live ? g.dh : 0, q[m]) * (g.scale * LOG2E);
-    const float ddown = load_row<VEC>(rd, (uint32_t)(qx * g.h + head) * dv, live ? dv : 0, d);
+        for (int m = 0; m < 2; m++)
+            qf[m].template load<VEC>(rq, (uint32_t)qx * (uint32_t)g.qstride + (2 * head + m) * g.dh,
+                                     live ? g.dh : 0);
+        df.template load<VEC>(rd, (uint32_t)(qx * g.h + head) * dv, live ? dv : 0);
+#pragma unroll
+        for (int m = 0; m < 2; m++) qdown[m] = qf[m].split(q[m]) * (g.scale * LOG2E);
+        ddown = df.split(d);
+    }
     const float pup = p_up(fabsf(dd[3]));
     const float nm[2] = {-sm[0], -sm[2]};
     float il[2] = {sm[1] * pup, sm[3] * dd[3] * pup};
@@ -1045,8 +1061,10 @@ diff_dq_kernel(DiffArgs g) {
         st.maxima(tmax[0][0], tmax[0][1]);
         __syncthreads();
         stage(0);
-        st.load(TK);
-        st.maxima(tmax[1][0], tmax[1][1]);
+        if (ntile > 1) {
+            st.load(TK);
+            st.maxima(tmax[1][0], tmax[1][1]);
+        }
     }
     for (int t = 0; t < ntile; t++) {
         const int k0 = t * TK;
@@ -1070,9 +1088,8 @@ diff_dq_kernel(DiffArgs g) {
 #pragma unroll
                     for (int r = 0; r < 16; r++) acc[m][c][r] *= ratio;
         }
-        // (past the last tile: zeros, into a buffer that nothing reads)
-        stage(t + 1);
-        st.load(k0 + 2 * TK);
+        if (t + 1 < ntile) stage(t + 1);
+        if (t + 2 < ntile) st.load(k0 + 2 * TK);
         {
             const _Float16 *const kt = lds[t & 1], *const vt = kt + Tile::HALVES;
             const float kdown = down_of(kup);
@@ -1115,7 +1132,7 @@ diff_dq_kernel(DiffArgs g) {
             }
             read_ahead<4 * CT, 4, 3>();
         }
-        st.maxima(tmax[t & 1][0], tmax[t & 1][1]);
+        if (t + 2 < ntile) st.maxima(tmax[t & 1][0], tmax[t & 1][1]);
     }
     if (row >= R) return;
     float *dst = g.dq + ((long long)b * g.tq + qi) * g.qstride + 2 * head * g.dh;
@@ -1230,12 +1247,15 @@ diff_dkv_kernel(DiffArgs g) {
         const auto rk = rows_rsrc(kvp + g.koff, rows, g.kvstride, dw);
         const auto rv = rows_rsrc(kvp + g.voff, rows, g.kvstride, dw);
         const uint32_t off = (uint32_t)(key - k0) * (uint32_t)g.kvstride;
+        RowFrag<KS> kf[2];
+        RowFrag<VS> vf;
 #pragma unroll
-        for (int m = 0; m < 2; m++)
-            kdown[m] = load_row<VEC>(rk, off + m * g.dh, live ? g.dh : 0, k[m]) * (g.scale * LOG2E);
-        float mx;
-        vdown = load_row<VEC>(rv, off, live ? dw : 0, v, &mx);
-        mx = wave_max(mx);
+        for (int m = 0; m < 2; m++) kf[m].template load<VEC>(rk, off + m * g.dh, live ? g.dh : 0);
+        vf.template load<VEC>(rv, off, live ? dw : 0);
+#pragma unroll
+        for (int m = 0; m < 2; m++) kdown[m] = kf[m].split(k[m]) * (g.scale * LOG2E);
+        vdown = vf.split(v);
+        const float mx = wave_max(vf.mx);
         if (lane == 0) vmaxs[wave] = mx;
     }
     f32x16 dk[2][CT], dv[VT];
@@ -1293,8 +1313,10 @@ diff_dkv_kernel(DiffArgs g) {
 #pragma unroll
         for (int i = 0; i < NW; i++) vmax = max2(vmax, vmaxs[i]);
         stage(0);
-        load(row_beg + TR);
-        maxima(1);
+        if (ntile > 1) {
+            load(row_beg + TR);
+            maxima(1);
+        }
     }
     for (int t = 0; t < ntile; t++) {
         const int row0 = row_beg + t * TR;
@@ -1320,9 +1342,8 @@ diff_dkv_kernel(DiffArgs g) {
                 for (int c = 0; c < VT; c++) dv[c][r] *= rv;
             }
         }
-        // (past the last tile: zeros, into a buffer that nothing reads)
-        stage(t + 1);
-        load(row0 + 2 * TR);
+        if (t + 1 < ntile) stage(t + 1);
+        if (t + 2 < ntile) load(row0 + 2 * TR);
         const int tq0 = row0 / g.group, tq1 = min(nq - 1, (row0 + TR - 1) / g.group);
         {
             const _Float16 *const qt = lds[t & 1], *const dt = qt + Tile::HALVES;
@@ -1387,7 +1408,7 @@ diff_dkv_kernel(DiffArgs g) {
             }
             read_ahead<2 * (VT + 2 * CT), 4, 3>();
         }
-        maxima(t & 1);
+        if (t + 2 < ntile) maxima(t & 1);
     }
     if (key >= g.tk) return;
     float *kd = g.dkv + krow * g.kvstride + g.koff + 2 * kh * g.dh;
