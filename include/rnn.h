@@ -341,11 +341,12 @@ int rnn_linear_backward_ex(rnn_ctx *ctx, size_t rows, size_t fin, size_t fout, c
 
 /* The Linear product with an activation and a residual (no counterpart in the
  * reference, whose MLP is SwiGLU): z = x W^T + b, y = act(z) + res (b, res may
- * be NULL; res [rows x fout], may be y).  z [rows x fout] is kept for the
- * backward (NULL: not kept; not needed for RNN_ACT_NONE).  act: RNN_ACT_NONE
- * z, RNN_ACT_RELU max(z, 0), RNN_ACT_GELU z (1 + erf(z / sqrt 2)) / 2,
- * RNN_ACT_GELU_TANH z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2,
- * RNN_ACT_SILU z / (1 + exp(-z)). */
+ * be NULL; res [rows x fout], may be y).  slope [rows x fout] receives act'(z)
+ * for the backward (NULL: not kept; not needed for RNN_ACT_NONE).  act:
+ * RNN_ACT_NONE z, RNN_ACT_RELU max(z, 0), RNN_ACT_GELU z (1 + erf(z / sqrt 2)) /
+ * 2, RNN_ACT_GELU_TANH z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2,
+ * RNN_ACT_SILU z / (1 + exp(-z)); RELU's slope at 0 is 0.  rows <= 2^30, fin and
+ * fout <= 2^20. */
 #define RNN_ACT_NONE 0u
 #define RNN_ACT_RELU 1u
 #define RNN_ACT_GELU 2u
@@ -353,15 +354,18 @@ int rnn_linear_backward_ex(rnn_ctx *ctx, size_t rows, size_t fin, size_t fout, c
 #define RNN_ACT_SILU 4u
 int rnn_linear_act_forward(rnn_ctx *ctx, size_t rows, size_t fin, size_t fout, const float *x,
                            const float *w, const float *b, uint32_t act, const float *res,
-                           float *z, float *y);
-/* Its backward: dz = dy act'(z) (0 for RELU at z = 0), then as
- * rnn_linear_backward_ex: dw += dz^T x, db += colsum(dz) (db may be NULL), dx =
- * dz W (added with RNN_LINEAR_ACC_DX).  dz [rows x fout] is the caller's
- * scratch, may be z and is not read for RNN_ACT_NONE (z and dz may then be
- * NULL).  The residual's gradient is dy itself. */
+                           float *slope, float *y);
+/* Bytes of device workspace that the backward needs; host only.  The workspace
+ * is the caller's, 256-byte aligned, holds nothing between calls and is not
+ * shared by calls that may run at the same time. */
+int rnn_linear_act_workspace(size_t rows, size_t fin, size_t fout, size_t *bytes);
+/* Its backward, from the forward's slope (NULL: RNN_ACT_NONE): dz = dy slope,
+ * dx = dz W (added with RNN_LINEAR_ACC_DX), dw += dz^T x, db += colsum(dz) (db may
+ * be NULL, and is with fin = 0).  The residual's gradient is dy itself.  Sums run
+ * in a fixed order. */
 int rnn_linear_act_backward(rnn_ctx *ctx, size_t rows, size_t fin, size_t fout, const float *dy,
-                            const float *x, const float *w, const float *z, uint32_t act,
-                            float *dz, float *dw, float *db, float *dx, uint32_t flags);
+                            const float *x, const float *w, const float *slope, void *ws,
+                            size_t ws_bytes, float *dw, float *db, float *dx, uint32_t flags);
 
 /* ------------------------------------------ host-slice forms (Rust shim) */
 /* The same entry points over HOST memory, for the Rust shim, whose callers

@@ -165,7 +165,8 @@ def lib():
                                        [_sz, _vp, _vp, _vp, _vp, _u32]),
             "rnn_linear_act_forward": (_i, [_vp, _sz, _sz, _sz, _vp, _vp, _vp, _u32, _vp, _vp,
                                             _vp]),
-            "rnn_linear_act_backward": (_i, [_vp, _sz, _sz, _sz, _vp, _vp, _vp, _vp, _u32, _vp,
+            "rnn_linear_act_workspace": (_i, [_sz, _sz, _sz, P(_sz)]),
+            "rnn_linear_act_backward": (_i, [_vp, _sz, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _sz,
                                              _vp, _vp, _vp, _u32]),
             "rnn_linear_forward": (_i, [_vp, _sz, _sz, _sz, _vp, _vp, _vp, _vp]),
             "rnn_linear_forward_residual": (_i, [_vp, _sz, _sz, _sz, _vp, _vp, _vp, _vp, _vp,
@@ -970,43 +971,52 @@ def _act_code(act):
 
 def linear_act_forward(rows, fin, fout, x, w, b=None, act="none", res=None, y=None, train=True,
                        ctx=None):
-    """(y, z): z = x W^T + b, y = act(z) + res, act one of ACTS; z is kept for
-    linear_act_backward when train and act is not "none", else None."""
+    """(y, slope): z = x W^T + b, y = act(z) + res, act one of ACTS; the slope
+    act'(z) is kept for linear_act_backward when train and act is not "none",
+    else None."""
     import torch
     code = _act_code(act)
     ctx = ctx or default_ctx(x.device.index or 0)
-    new = lambda: torch.empty(rows, fout, dtype=torch.float32, device=x.device)
-    y = new() if y is None else y
-    z = new() if train and code else None
+    y = torch.empty(rows, fout, dtype=torch.float32, device=x.device) if y is None else y
+    slope = (torch.empty(rows, fout, dtype=torch.float32, device=x.device) if train and code
+             else None)
     ctx.check(lib().rnn_linear_act_forward(
         ctx.h, rows, fin, fout, _arg(ctx, x, rows * fin, "x"), _arg(ctx, w, fout * fin, "w"),
         _arg(ctx, b, fout, "b"), code, _arg(ctx, res, rows * fout, "res"),
-        _arg(ctx, z, rows * fout, "z"), _arg(ctx, y, rows * fout, "y")))
-    _on_ctx_stream(ctx, x, w, b, res, z, y)
-    return y, z
+        _arg(ctx, slope, 0, "slope"), _arg(ctx, y, rows * fout, "y")))
+    _on_ctx_stream(ctx, x, w, b, res, slope, y)
+    return y, slope
 
 
-def linear_act_backward(rows, fin, fout, dy, x, w, z, act, dw, db=None, dx=None, acc_dx=False,
+_linear_act_ws = {}  # workspace bytes by size
+
+
+def linear_act_backward(rows, fin, fout, dy, x, w, slope, act, dw, db=None, dx=None, acc_dx=False,
                         ctx=None):
     """dx (returned; acc_dx: added to the given dx); dw and db accumulate.
-    z, as linear_act_forward kept it, is left unchanged.  The residual's
+    slope, as linear_act_forward kept it, is left unchanged.  The residual's
     gradient is dy."""
     import torch
     code = _act_code(act)
     if acc_dx and dx is None:
         raise ValueError("linear_act_backward: acc_dx needs dx")
-    if code and z is None:
-        raise ValueError("linear_act_backward: the forward did not keep z (train=False)")
+    if code and slope is None:
+        raise ValueError("linear_act_backward: the forward did not keep its slope (train=False)")
     ctx = ctx or default_ctx(dy.device.index or 0)
+    nb = _linear_act_ws.get((rows, fin, fout))
+    if nb is None:
+        out = _sz()
+        ctx.check(lib().rnn_linear_act_workspace(rows, fin, fout, C.byref(out)))
+        nb = _linear_act_ws[rows, fin, fout] = out.value
+    ws = torch.empty(nb, dtype=torch.uint8, device=dy.device) if nb else None
     dx = torch.empty(rows, fin, dtype=torch.float32, device=dy.device) if dx is None else dx
-    dz = torch.empty(rows, fout, dtype=torch.float32, device=dy.device) if code else None
     ctx.check(lib().rnn_linear_act_backward(
         ctx.h, rows, fin, fout, _arg(ctx, dy, rows * fout, "dy"), _arg(ctx, x, rows * fin, "x"),
-        _arg(ctx, w, fout * fin, "w"), _arg(ctx, z, rows * fout, "z"), code,
-        _arg(ctx, dz, rows * fout, "dz"), _arg(ctx, dw, fout * fin, "dw"),
+        _arg(ctx, w, fout * fin, "w"), _arg(ctx, slope, rows * fout, "slope") if code else None,
+        ws.data_ptr() if nb else None, nb, _arg(ctx, dw, fout * fin, "dw"),
         _arg(ctx, db, fout, "db"), _arg(ctx, dx, rows * fin, "dx"),
         RNN_LINEAR_ACC_DX if acc_dx else 0))
-    _on_ctx_stream(ctx, dy, x, w, z, dz, dw, db, dx)
+    _on_ctx_stream(ctx, dy, x, w, slope, ws, dw, db, dx)
     return dx
 
 

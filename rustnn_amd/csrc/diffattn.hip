@@ -9,7 +9,7 @@
 //   dS_1 = P_1 (dA - D_1), dS_2 = -lambda P_2 (dA - D_2),
 //   dQ_m = scale dS_m K_m, dK_m = scale dS_m^T Q_m, dV = (P_1 - lambda P_2)^T dO,
 //   dlambda = -sum D_2.
-#include "rnn_internal.h"
+#include "mfma_half.h"
 
 #include <algorithm>
 #include <cmath>
@@ -48,172 +48,6 @@ __device__ __forceinline__ void lambda_dots(const float *lam, int lam_heads, int
     *a = rnn_wave_sum_d(lane < dh ? (double)x * (double)y : 0.0);
     *b = rnn_wave_sum_d(lane < dh ? (double)z * (double)w : 0.0);
 }
-
-// Maxima in one instruction each (fmaxf takes a second one to quiet NaNs).
-__device__ __forceinline__ float max2(float a, float b) {
-    float d;
-    asm("v_max_f32 %0, %1, %2" : "=v"(d) : "v"(a), "v"(b));
-    return d;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
-    return d;
-}
-__device__ __forceinline__ float max3abs(float a, float b, float c) {
-    float d;
-    asm("v_max3_f32 %0, %1, |%2|, |%3|" : "=v"(d) : "v"(a), "v"(b), "v"(c));
-    return d;
-}
-template <int CTRL>
-__device__ __forceinline__ float dpp_f(float v) {
-    return __uint_as_float(__builtin_amdgcn_mov_dpp((int)__float_as_uint(v), CTRL, 0xf, 0xf, false));
-}
-// Both lanes of each pair (l, l xor 32), or (l, l xor 16): f of the two values.
-template <typename F>
-__device__ __forceinline__ float pair32(float v, F f) {
-    const uint32_t u = __float_as_uint(v);
-    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-    return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-template <typename F>
-__device__ __forceinline__ float pair16(float v, F f) {
-    const uint32_t u = __float_as_uint(v);
-    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float add2(float a, float b) { return a + b; }
-// f over the 64 lanes, every lane receiving it, in a fixed tree.
-template <typename F>
-__device__ __forceinline__ float wave_all(float v, F f) {
-    v = f(v, dpp_f<0xB1>(v));
-    v = f(v, dpp_f<0x4E>(v));
-    v = f(v, dpp_f<0x141>(v));
-    v = f(v, dpp_f<0x140>(v));
-    return pair32(pair16(v, f), f);
-}
-__device__ __forceinline__ float wave_max(float v) { return wave_all(v, max2); }
-__device__ __forceinline__ float wave_sum(float v) { return wave_all(v, add2); }
-
-// ---------------------------------------------------------------------------
-// fp32 products on the fp16 matrix cores.
-//
-// A float times a power of two is hi + lo, hi its nearest fp16 and lo the
-// nearest fp16 of the rest: hi + lo is within half a step of 2^-22, so 2^-23, of
-// it, as long as lo is no subnormal, which ends 2^-25 at 2^15.  With the power
-// chosen so that the largest magnitude of a row or tile comes to
-// [2^14, 2^15), every element down to 2^-16 of the largest keeps 2^-23, and
-// below that all keep 2^-39 of the largest.  a b is then hi hi + hi lo + lo hi:
-// products of 22 bits, exact in the matrix core, summed in its fp32
-// accumulator; lo lo, left out, is below 2^-22 of the product and of no common
-// sign.  Three products an element and four bytes in LDS, where three bf16
-// parts (mfma_split.h) take six and six; their range of exponents is not needed
-// here, since rows and tiles carry their power of two beside them.
-typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef __fp16 g4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef float f2 __attribute__((ext_vector_type(2)));
-typedef float f2u __attribute__((ext_vector_type(2), aligned(4)));
-typedef float f4 __attribute__((ext_vector_type(4)));
-
-struct Half2 {
-    h8 hi, lo;
-};
-
-// x - (the lower / upper half of h): the rest of a rounding, exact.
-__device__ __forceinline__ float rest_lo(uint32_t h, float x) {
-    float d;
-    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(d) : "v"(h), "v"(x));
-    return d;
-}
-__device__ __forceinline__ float rest_hi(uint32_t h, float x) {
-    float d;
-    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(d) : "v"(h), "v"(x));
-    return d;
-}
-// Two floats' parts, each pair in a register.
-__device__ __forceinline__ void half_pair(float a, float b, uint32_t &hi, uint32_t &lo) {
-    const f2 v = {a, b};
-    hi = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, h2));
-    const f2 d = {rest_lo(hi, a), rest_hi(hi, b)};
-    lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(d, h2));
-}
-
-// The two parts of 8 floats times up (a power of two).
-__device__ __forceinline__ Half2 half_split(const float (&x)[8], float up) {
-    u32x4 hi, lo;
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        uint32_t a, b;
-        half_pair(x[2 * j] * up, x[2 * j + 1] * up, a, b);
-        hi[j] = a;
-        lo[j] = b;
-    }
-    return Half2{__builtin_bit_cast(h8, hi), __builtin_bit_cast(h8, lo)};
-}
-// The parts of an accumulator's registers 0..7 and 8..15, as they are.
-__device__ __forceinline__ void split16(const f32x16 &x, Half2 (&d)[2]) {
-#pragma unroll
-    for (int s = 0; s < 2; s++) {
-        u32x4 hi, lo;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            uint32_t a, b;
-            half_pair(x[8 * s + 2 * j], x[8 * s + 2 * j + 1], a, b);
-            hi[j] = a;
-            lo[j] = b;
-        }
-        d[s] = Half2{__builtin_bit_cast(h8, hi), __builtin_bit_cast(h8, lo)};
-    }
-}
-
-// The power of two that takes a largest magnitude m to [2^14, 2^15) (m of 0,
-// an infinity or a NaN: 1), and its reciprocal.  Magnitudes below 2^-112 stay
-// smaller.
-__device__ __forceinline__ float up_of(float m) {
-    const int e = (int)(__float_as_uint(m) >> 23) & 255;
-    const int f = (e == 255 || m == 0.0f) ? 127 : min(268 - e, 253);
-    return __uint_as_float((uint32_t)f << 23);
-}
-__device__ __forceinline__ float down_of(float up) {
-    return __uint_as_float((254u << 23) - __float_as_uint(up));
-}
-
-__device__ __forceinline__ f32x16 mm(h8 a, h8 b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-}
-
-// A tile of ROWS rows of W channels in LDS, both parts: row r's hi at
-// r * STRIDE, its lo PART further on.  The 16 bytes of padding put the b128
-// reads of 8 consecutive rows on distinct banks (an odd number of 16-byte
-// slots a row).
-template <int ROWS, int W>
-struct HalfTile {
-    static constexpr int STRIDE = W + 8;  // in halves
-    static constexpr int PART = ROWS * STRIDE;
-    static constexpr int HALVES = 2 * PART;
-    // 8 consecutive channels of a row: an operand with its k along channels
-    static __device__ __forceinline__ h8 along(const _Float16 *t, int row, int c) {
-        return *(const h8 *)(t + row * STRIDE + c);
-    }
-    // Rows row0 + {0..3, 8..11} (row0 + 4 for the upper half wave) of channel
-    // c0 + lane % 32: an operand with its k along rows, in the order in which
-    // a 32 x 32 accumulator's registers 8 s .. 8 s + 7 hold the rows of the
-    // block of 16 at row0.  Each 16 lanes read 4 rows of 16 channels, which
-    // the LDS hands back transposed.
-    static __device__ __forceinline__ h8 across(const _Float16 *t, int row0, int c0) {
-        const int l = threadIdx.x & 63;
-        const _Float16 *p = t + (row0 + 4 * (l >> 5) + ((l & 15) >> 2)) * STRIDE + c0 +
-                            16 * ((l >> 4) & 1) + 4 * (l & 3);
-        typedef __attribute__((address_space(3))) g4 *lds_g4;
-        const h4 a = __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_g4)p));
-        const h4 b = __builtin_bit_cast(
-            h4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_g4)(p + 8 * STRIDE)));
-        return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-    }
-};
 
 // acc += the rows of a tile times a register operand over channels c0 ..
 // c0 + 16 N - 1: accumulator rows are the tile's, columns the operand's lanes.
@@ -257,47 +91,6 @@ __device__ __forceinline__ void read_ahead() {
     __builtin_amdgcn_sched_group_barrier(0x8, 3 * A, 0);
 }
 
-// 8 consecutive channels, `off` floats into a buffer resource, zero from `lim`
-// channels on and past the resource's end.
-template <bool VEC>
-__device__ __forceinline__ void load8(__amdgpu_buffer_rsrc_t rs, uint32_t off, int lim,
-                                      float (&x)[8]) {
-    if constexpr (VEC) {
-#pragma unroll
-        for (int q = 0; q < 2; q++) {
-            const uint32_t at = 4 * q < lim ? (off + 4 * q) * 4 : DMA_OOB;
-            const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(rs, at, 0, 0);
-#pragma unroll
-            for (int e = 0; e < 4; e++) x[4 * q + e] = __uint_as_float(v[e]);
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-            x[e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
-                rs, e < lim ? (off + e) * 4 : DMA_OOB, 0, 0));
-    }
-}
-
-// How NT threads stage a tile of ROWS rows of W channels: RPP rows a pass, 8
-// channels a thread, so that a thread keeps its channels from pass to pass
-// (W = 96: the last quarter of the threads idle).
-template <int ROWS, int W, int NT>
-struct StagePlan {
-    static constexpr int C8 = W / 8;
-    static constexpr int fit = NT / C8;
-    static constexpr int most = fit >= 64 ? 64 : fit >= 32 ? 32 : fit >= 16 ? 16 : fit >= 8 ? 8 : 4;
-    static constexpr int RPP = most < ROWS ? most : ROWS;
-    static constexpr int PASSES = ROWS / RPP;
-    static constexpr bool ALL = RPP * C8 == NT;
-    static_assert(RPP * C8 <= NT && PASSES * RPP == ROWS, "whole passes");
-};
-
-__device__ __forceinline__ float absmax8(const float (&x)[8], float m) {
-#pragma unroll
-    for (int e = 0; e < 8; e += 2) m = max3abs(m, x[e], x[e + 1]);
-    return m;
-}
-
 // A lane's row of 16 N channels (of `lim` channels, zeros past them); the lanes l
 // and l + 32 hold it together.  split() makes it an operand, times the power of two
 // that its largest magnitude (mx) calls for, whose reciprocal is returned.
@@ -322,24 +115,10 @@ struct RowFrag {
         return down_of(up);
     }
 };
-// A resource over `rows` rows (at most 64) of `stride` floats from p on, the last
-// of them `width` floats long.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const float *p, int rows, long long stride,
-                                                            int width) {
-    return make_rsrc(p, rows > 0 ? ((uint32_t)(rows - 1) * (uint32_t)stride + width) * 4u : 0u);
-}
-
 // Softmax values enter the products times 2^6, relative to a reference that a row's
 // largest score may pass by 2^8 before it moves: at most 2^14.
 constexpr float P_UP = 64.0f, P_EXP = 6.0f, SLACK = 8.0f;
 constexpr float NO_MAX = -1e30f;                 // a running maximum before any score
-
-// The block's number in an order in which each XCD (block id % 8) gets a
-// contiguous run: the blocks that share a problem's keys meet in one L2.
-__device__ __forceinline__ long long xcd_order(long long id, long long total) {
-    const long long per = total >> 3, rem = total & 7, x = id & 7, loc = id >> 3;
-    return x < rem ? x * (per + 1) + loc : rem * (per + 1) + (x - rem) * per + loc;
-}
 
 // Lambda of a lane's own head: the wave's one head together, else each lane its
 // own.
@@ -511,18 +290,17 @@ diff_fwd_kernel(DiffArgs g) {
 #pragma unroll
         for (int r = 0; r < 16; r++) o[c][r] = 0.f;
     float m = NO_MAX, l = 0.f;
-    // powers of two of the tile that is staged, from the largest magnitudes (of
-    // the values: so far, so that the output's unit hardly changes)
-    float kup1 = 1.f, vup1 = 1.f, vup = 1.f, mv = 0.f;
+    // powers of two of the tile that is staged; the output is in the values' unit
+    float kup1 = 1.f, vup1 = FIRST_UP, vup = FIRST_UP;
     auto stage = [&](int t) {
-        float mk = 0.f;
+        float mk = 0.f, mv = 0.f;
 #pragma unroll
         for (int i = 0; i < 2 * QG; i++) {
             mk = max2(mk, tmax[t & 1][0][i]);
             mv = max2(mv, tmax[t & 1][1][i]);
         }
         kup1 = up_of(mk);
-        vup1 = up_of(mv);
+        vup1 = sticky_up(mv, vup1);
         st.store(lds[t & 1], kup1, vup1);
     };
     if (ntile) {
@@ -958,11 +736,13 @@ __global__ __launch_bounds__(256) void diff_bwd_params_kernel(const double *__re
 }
 
 // The power of two that takes 2 |dA| of rows with |dO| <= nd and values of
-// magnitude <= vmax below 2: |dA| <= nd sqrt(W) vmax, and D is a mean of dA.
+// magnitude <= vmax to 2 or below: |dA| <= nd sqrt(W) vmax, and D is a mean of dA.
+// It stays as it was (up) while that holds, as sticky_up.
 template <int W>
-__device__ __forceinline__ float ds_up(float nd, float vmax) {
+__device__ __forceinline__ float ds_up(float nd, float vmax, float up) {
     constexpr float root = W == 32 ? 5.6568543f : W == 64 ? 8.0f : W == 96 ? 9.7979590f : 11.313709f;
-    return up_of(nd * (2.0f * root * vmax)) * 0x1p-14f;
+    const float m = nd * (2.0f * root * vmax);
+    return m * up < 2.0f ? up : up_of(m) * 0x1p-18f;
 }
 // The power of two that softmax values, and lambda times them, enter the
 // backward's products with: at most 2^14, so that P_1 - lambda P_2 and P (dA - D)
@@ -978,8 +758,8 @@ __device__ __forceinline__ int flip_at(int ntile) { return (2 * ntile + 2) / 3; 
 // dQ.  Rows as in the forward, a wave on both maps of its 32 rows, tiles of 32
 // keys in two LDS buffers: S_m^T = K_m Q_m^T and dA^T = V dO^T (lane = row), and
 // P (dA - D) in registers is the operand of dQ_m^T = K_m^T dS_m^T, which is
-// summed over all tiles in the accumulators.  Their unit is a power of two from
-// the largest magnitudes so far; where it changes they are rescaled.
+// summed over all tiles in the accumulators.  Their unit is a power of two that
+// hardly changes (sticky_up); where it does they are rescaled.
 template <int DHP, bool VEC, int NW>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DHP <= 32 ? 2 : 1))) void
 diff_dq_kernel(DiffArgs g) {
@@ -1044,16 +824,19 @@ diff_dq_kernel(DiffArgs g) {
         for (int c = 0; c < CT; c++)
 #pragma unroll
             for (int r = 0; r < 16; r++) acc[m][c][r] = 0.f;
-    // largest magnitudes so far, and the powers of two of the tile in each buffer
-    float mk = 0.f, mv = 0.f, kup1 = 1.f, vup1 = 1.f, kup = 1.f, dsup = 1.f, sgn = 1.f;
+    // the staged tile's largest value, and powers of two: of the tile that is staged
+    // (.1) and of the one that is computed
+    float mv = 0.f, kup1 = FIRST_UP, vup1 = 1.f, kup = FIRST_UP, dsup = FIRST_UP, sgn = 1.f;
     const int flip = flip_at(ntile);
     auto stage = [&](int t) {  // tile t, whose maxima are there, into its buffer
+        float mk = 0.f;
+        mv = 0.f;
 #pragma unroll
         for (int i = 0; i < NW; i++) {
             mk = max2(mk, tmax[t & 1][0][i]);
             mv = max2(mv, tmax[t & 1][1][i]);
         }
-        kup1 = up_of(mk);
+        kup1 = sticky_up(mk, kup1);
         vup1 = up_of(mv);
         st.store(lds[t & 1], kup1, vup1);
     };
@@ -1070,7 +853,7 @@ diff_dq_kernel(DiffArgs g) {
         const int k0 = t * TK;
         __syncthreads();
         // dS's power of two, and the accumulators in the tile's unit
-        const float vup = vup1, dsup1 = ds_up<W>(dd[2], mv);
+        const float vup = vup1, dsup1 = ds_up<W>(dd[2], mv, dsup);
         float ratio = down_of(kup) * kup1 * (down_of(dsup) * dsup1);
         kup = kup1;
         dsup = dsup1;
@@ -1268,23 +1051,23 @@ diff_dkv_kernel(DiffArgs g) {
 #pragma unroll
         for (int c = 0; c < VT; c++) dv[c][r] = 0.f;
     }
-    // largest magnitudes so far, the powers of two of the tile that is staged
-    // (.1) and of the one that is computed
-    float mq = 0.f, md = 0.f, mn = 0.f, ml = 0.f, vmax = 0.f;
-    float qup1 = 1.f, dup1 = 1.f, pup1 = 1.f, sup1 = 1.f, qup = 1.f, dup = 1.f, pup = 1.f, sup = 1.f;
+    // the largest value and lambda so far, the powers of two of the tile that is
+    // staged (.1) and of the one that is computed
+    float vmax = 0.f, ml = 0.f, qup1 = FIRST_UP, dup1 = FIRST_UP, pup1 = 1.f, sup1 = FIRST_UP;
+    float qup = FIRST_UP, dup = FIRST_UP, pup = 1.f, sup = FIRST_UP;
     const int flip = flip_at(ntile);
     auto stage = [&](int t) {
+        float mq = 0.f, md = 0.f;
 #pragma unroll
         for (int i = 0; i < NW; i++) {
             mq = max2(mq, tmax[t & 1][0][i]);
             md = max2(md, tmax[t & 1][1][i]);
         }
-        mn = max2(mn, tmax[t & 1][2][0]);
         ml = max2(ml, tmax[t & 1][3][0]);
-        qup1 = up_of(mq);
-        dup1 = up_of(md);
+        qup1 = sticky_up(mq, qup1);
+        dup1 = sticky_up(md, dup1);
         pup1 = p_up(ml);
-        sup1 = ds_up<W>(mn, vmax);
+        sup1 = ds_up<W>(tmax[t & 1][2][0], vmax, sup1);
         if (stager) {
 #pragma unroll
             for (int i = 0; i < CH; i++) {

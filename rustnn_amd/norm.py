@@ -204,7 +204,7 @@ class Mlp:
         self.up = Linear(c, h, True, w1, b1, device, self.ctx)
         self.down = Linear(h, c, True, w2, b2, device, self.ctx)
         self._params = _linear_param(self.up) + _linear_param(self.down)
-        self.x = self.z = None
+        self.x = self.slope = None
         self.rows = 0
 
     def forward(self, x, train, residual=None):
@@ -214,17 +214,18 @@ class Mlp:
         if c != self.c:
             raise ValueError(f"Mlp: {c} channels, the layer has {self.c}")
         up = self.up
-        u, z = linear_act_forward(rows, c, self.h, x, up.w, up.b, self.act, train=train,
-                                  ctx=self.ctx)
+        u, slope = linear_act_forward(rows, c, self.h, x, up.w, up.b, self.act, train=train,
+                                      ctx=self.ctx)
         if train:
-            self.x, self.z, self.rows = x, z, rows
+            self.x, self.slope, self.rows = x, slope, rows
         return self.down.forward(u.view(-1), rows, train, residual).view(x.shape)
 
     def backward(self, dy):
         up = self.up
         du = self.down.backward(dy.reshape(-1))
-        return linear_act_backward(self.rows, self.c, self.h, du, self.x, up.w, self.z, self.act,
-                                   up.gw, up.gb, ctx=self.ctx).view(dy.shape)
+        return linear_act_backward(self.rows, self.c, self.h, du, self.x, up.w, self.slope,
+                                   self.act, up.gw, up.gb,
+                                   ctx=self.ctx).view(dy.shape)
 
     def for_each_param(self, f):
         for p in self._params:

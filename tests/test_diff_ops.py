@@ -21,8 +21,12 @@ def test_null_context_is_refused():
         R.RNN_E_NULL
     assert L.rnn_linear_act_forward(None, 1, 1, 1, None, None, None, 0, None, None, None) == \
         R.RNN_E_NULL
-    assert L.rnn_linear_act_backward(None, 1, 1, 1, None, None, None, None, 0, None, None, None,
-                                     None, 0) == R.RNN_E_NULL
+    assert L.rnn_linear_act_backward(None, 1, 1, 1, *[None] * 5, 0, None, None, None, 0) == \
+        R.RNN_E_NULL
+    nb = C.c_size_t()
+    assert L.rnn_linear_act_workspace(8, 8, 8, None) == R.RNN_E_NULL
+    assert L.rnn_linear_act_workspace(8, 1 << 21, 8, C.byref(nb)) == R.RNN_E_UNSUPPORTED
+    assert L.rnn_linear_act_workspace(0, 0, 0, C.byref(nb)) == R.RNN_OK and nb.value == 0
 
 
 @pytest.mark.parametrize("kw", [

@@ -12,8 +12,11 @@ from diffref import D, act
 
 pytestmark = pytest.mark.gpu
 
+# small and odd ones, then one for every tile and split of each product
 SIZES = [(1, 1, 1), (1, 256, 1024), (3, 7, 5), (64, 256, 1024), (65, 33, 129), (200, 96, 352),
-         (1813, 387, 251), (513, 64, 64), (8192, 32, 48), (37, 0, 9)]
+         (1813, 387, 251), (513, 64, 64), (8192, 32, 48), (37, 0, 9), (4096, 40, 36),
+         (2048, 256, 160), (130, 1030, 70), (4099, 129, 131), (8192, 33, 511), (4099, 129, 384),
+         (2100, 70, 330), (8200, 513, 40), (4099, 384, 33), (2100, 330, 70)]
 
 
 def inputs(rows, fin, fout, seed=0, whole=False):
@@ -45,9 +48,8 @@ def test_forward_and_gradients(rnn, size, name):
     ev, none = rnn.linear_act_forward(*size, X, W, B, name, res=RES, train=False)
     assert none is None and torch.equal(ev, y)
     inpl = RES.clone()
-    if name != "none":
-        rnn.linear_act_forward(*size, X, W, B, name, res=inpl, y=inpl)
-        assert torch.equal(inpl, y)
+    rnn.linear_act_forward(*size, X, W, B, name, res=inpl, y=inpl)
+    assert torch.equal(inpl, y)
     dw, db = torch.full_like(W, 0.5), torch.full_like(B, 0.25)
     z0 = None if z is None else z.clone()
     if fin == 0:
@@ -136,6 +138,59 @@ def test_refusals(rnn):
         rnn.RNN_E_INVALID
     assert L.rnn_linear_act_forward(ctx.h, *size, p(x), None, None, 1, None, None, p(y)) == \
         rnn.RNN_E_NULL
-    dx = torch.zeros_like(x)
-    assert L.rnn_linear_act_backward(ctx.h, *size, p(dy), p(x), p(w), p(y), 1, p(dx), p(w.clone()),
-                                     None, p(dx), 0) == rnn.RNN_E_INVALID
+    dx, dw, db = torch.zeros_like(x), torch.zeros_like(w), torch.zeros_like(b)
+    bwd = lambda sz, ws, nb, dx, db=None, flags=0: L.rnn_linear_act_backward(
+        ctx.h, *sz, p(dy), p(x), p(w), p(y), ws, nb, p(dw), db, dx, flags)
+    assert bwd(size, None, 0, p(dy)) == rnn.RNN_E_INVALID  # dx over dy
+    assert bwd(size, None, 0, p(dx), None, 2) == rnn.RNN_E_INVALID
+    assert bwd(size, None, 0, None) == rnn.RNN_E_NULL
+    assert bwd((8, 0, 4), None, 0, p(dx), p(db)) == rnn.RNN_E_UNSUPPORTED  # db without inputs
+    assert bwd((1 << 31, 16, 4), None, 0, p(dx)) == rnn.RNN_E_UNSUPPORTED
+    import ctypes as C
+    nb = C.c_size_t()
+    big = (4096, 64, 64)
+    assert L.rnn_linear_act_workspace(*big, C.byref(nb)) == 0 and nb.value > 0
+    ws = torch.zeros(nb.value + 256, dtype=torch.uint8, device="cuda")
+    assert bwd(big, None, nb.value, p(dx)) == rnn.RNN_E_NULL
+    assert bwd(big, p(ws), nb.value - 1, p(dx)) == rnn.RNN_E_INVALID
+    assert bwd(big, p(ws) + 16, nb.value, p(dx)) == rnn.RNN_E_INVALID
+
+
+def test_same_bits_captured_and_replayed(rnn):
+    """Two graphs of forward and backward on one context, replayed in turn with
+    eager calls between, each to its eager result, bit for bit."""
+    size = (700, 130, 190)
+    st = torch.cuda.Stream()
+    ctx = rnn.Context(0, stream=st)
+    runs = []
+    for s in range(2):
+        x, w, b, res, dy = (t.cuda() for t in inputs(*size, seed=10 + s))
+        dw, db = torch.zeros_like(w), torch.zeros_like(b)
+
+        def call(x=x, w=w, b=b, res=res, dy=dy, dw=dw, db=db):
+            dw.zero_()
+            db.zero_()
+            y, sl = rnn.linear_act_forward(*size, x, w, b, "gelu", res=res, ctx=ctx)
+            return y, rnn.linear_act_backward(*size, dy, x, w, sl, "gelu", dw, db, ctx=ctx)
+
+        torch.cuda.synchronize()
+        with torch.cuda.stream(st):
+            y, dx = call()
+        st.synchronize()
+        want = [t.clone() for t in (y, dx, dw, db)]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=st):
+            y, dx = call()
+        runs.append((graph, (y, dx, dw, db), want, call))
+    for _ in range(3):
+        for graph, out, want, call in runs:
+            with torch.cuda.stream(st):
+                for t in out:
+                    t.fill_(0.5)
+                graph.replay()
+            st.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+            with torch.cuda.stream(st):
+                call()
+            st.synchronize()
+    ctx.close()
