@@ -32,6 +32,8 @@ struct DiffArgs {
     long long qstride, kvstride;
     int n, h, hkv, dh, tq, tk, koff, voff, lam_heads, diag, causal, group;
     int acc_q, acc_kv, split_keys;
+    int nblk, gpb;         // blocks of the backward's first pass, their groups of lanes
+    float *dlam, *dgain;
     float scale, lam_init, eps;
 };
 
@@ -178,26 +180,23 @@ struct KvStage {
             load8<VEC>(rv, voff + i * step, vlim, xv[i]);
         }
     }
-    __device__ __forceinline__ void maxima(float *mk, float *mv) const {
+    // Largest magnitudes past what the powers of two are good for, each wave's.
+    __device__ __forceinline__ void maxima(f2 *mx, float kgood, float vgood) const {
         float a = 0.f, b = 0.f;
 #pragma unroll
         for (int i = 0; i < CH; i++) {
             a = absmax8(xk[i], a);
             b = absmax8(xv[i], b);
         }
-        a = wave_max(a);
-        b = wave_max(b);
-        if ((threadIdx.x & 63) == 0) {
-            mk[wave_index()] = a;
-            mv[wave_index()] = b;
-        }
+        const f2 m = {wave_over(a, kgood), wave_over(b, vgood)};
+        if ((threadIdx.x & 63) == 0) mx[wave_index()] = m;
     }
     // K's tile at lds, V's behind it.
     __device__ __forceinline__ void store(_Float16 *lds, float kup, float vup) const {
         if (!stager()) return;
 #pragma unroll
         for (int i = 0; i < CH; i++) {
-            _Float16 *d = lds + (sr + i * Stage::RPP) * Tile::STRIDE + sc;
+            _Float16 *d = lds + row_pos(sr + i * Stage::RPP) * Tile::STRIDE + sc;
             const Half2 hk = half_split(xk[i], kup), hv = half_split(xv[i], vup);
             *(h8 *)d = hk.hi;
             *(h8 *)(d + Tile::PART) = hk.lo;
@@ -251,7 +250,7 @@ diff_fwd_kernel(DiffArgs g) {
     using Tile = HalfTile<TK, W>;
     static_assert((int)sizeof(_Float16) * 4 * Tile::HALVES >= QG * CT * 16 * 64 * 4, "exchange");
     __shared__ __align__(16) _Float16 lds[2][2 * Tile::HALVES];
-    __shared__ float tmax[2][2][2 * QG];
+    __shared__ f2 tmax[2][2 * QG];
     const int lane = threadIdx.x & 63, wave = wave_index(), lr = lane & 31, lh = lane >> 5;
     const int map = wave & 1, qg = wave >> 1;
     const int R = g.tq * g.group, nrb = (R + 32 * QG - 1) / (32 * QG);
@@ -290,26 +289,29 @@ diff_fwd_kernel(DiffArgs g) {
 #pragma unroll
         for (int r = 0; r < 16; r++) o[c][r] = 0.f;
     float m = NO_MAX, l = 0.f;
-    // powers of two of the tile that is staged; the output is in the values' unit
-    float kup1 = 1.f, vup1 = FIRST_UP, vup = FIRST_UP;
+    // the largest key so far, and powers of two of the tile that is staged; the
+    // output is in the values' unit
+    float kmax = 0.f, kup1 = 1.f, vup1 = FIRST_UP, vup = FIRST_UP;
+    auto maxima = [&](int slot) { st.maxima(tmax[slot], kmax, good_for(vup1)); };
     auto stage = [&](int t) {
-        float mk = 0.f, mv = 0.f;
+        float mv = 0.f;
 #pragma unroll
         for (int i = 0; i < 2 * QG; i++) {
-            mk = max2(mk, tmax[t & 1][0][i]);
-            mv = max2(mv, tmax[t & 1][1][i]);
+            const f2 m = tmax[t & 1][i];
+            kmax = max2(kmax, m[0]);
+            mv = max2(mv, m[1]);
         }
-        kup1 = up_of(mk);
+        kup1 = up_of(kmax);
         vup1 = sticky_up(mv, vup1);
         st.store(lds[t & 1], kup1, vup1);
     };
     if (ntile) {
-        st.maxima(tmax[0][0], tmax[0][1]);
+        maxima(0);
         __syncthreads();
         stage(0);
         if (ntile > 1) {
             st.load(kbeg + TK);
-            st.maxima(tmax[1][0], tmax[1][1]);
+            maxima(1);
         }
     }
     for (int t = 0; t < ntile; t++) {
@@ -373,7 +375,7 @@ diff_fwd_kernel(DiffArgs g) {
         l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
 #pragma unroll
         for (int c = 0; c < CT; c++) dot_across<Tile>(vt, 32 * c, p, o[c]);
-        if (t + 2 < ntile) st.maxima(tmax[t & 1][0], tmax[t & 1][1]);
+        if (t + 2 < ntile) maxima(t & 1);
     }
     l = pair32(l, add2);
     const bool some = live && l > 0.f;
@@ -667,22 +669,24 @@ __global__ __launch_bounds__(256) void diff_bwd_pre_kernel(DiffArgs g) {
     }
 }
 
-// dgain and dlam from the blocks' partials.  Block i < ceil(dv / 16): the gain's
-// columns [16 i, 16 i + 16), 16 groups of partials each in order, then the groups
-// in order.  The others: one set of lambda vectors each, the partials of its
-// heads (every group of every block for a shared set, else group index % h = head)
-// in 256 strided sums, added in a fixed tree.
-__global__ __launch_bounds__(256) void diff_bwd_params_kernel(const double *__restrict__ part,
-                                                              int nblk, int gpb, const float *lam,
-                                                              int lam_heads, int dh, int h,
-                                                              float *dlam, float *dgain) {
-    const int dv = 2 * dh, cols = dv + gpb, ngain = dgain ? (dv + 15) / 16 : 0;
+// dgain and dlam from the first pass's partials, in the first blocks of dQ's launch
+// (on their own they took 5 to 6 us), NT threads each.  Block i < ceil(dv / 16): the
+// gain's columns [16 i, 16 i + 16), NT / 16 groups of partials each in order, then
+// the groups in order.  The others: one set of lambda vectors each, the partials of
+// its heads (every group of every block for a shared set, else group index % h =
+// head) in NT strided sums, added in a fixed tree.
+__device__ __forceinline__ int params_blocks(const DiffArgs &g) {
+    return (g.dgain ? (2 * g.dh + 15) / 16 : 0) + g.lam_heads;
+}
+template <int NT>
+__device__ __forceinline__ void bwd_params(const DiffArgs &g, int blk, double *red) {
+    const int dv = 2 * g.dh, cols = dv + g.gpb, ngain = g.dgain ? (dv + 15) / 16 : 0;
     const int lane = threadIdx.x & 63, wv = wave_index();
-    if ((int)blockIdx.x < ngain) {
-        __shared__ double red[16][16];
-        const int jl = threadIdx.x % 16, q = threadIdx.x / 16, j = 16 * (int)blockIdx.x + jl;
-        const int per = (nblk + 15) / 16, k0 = min(nblk, q * per), k1 = min(nblk, k0 + per);
-        const double *src = part + min(j, dv - 1);
+    if (blk < ngain) {
+        constexpr int Q = NT / 16;
+        const int jl = threadIdx.x % 16, q = threadIdx.x / 16, j = 16 * blk + jl;
+        const int per = (g.nblk + Q - 1) / Q, k0 = min(g.nblk, q * per), k1 = min(g.nblk, k0 + per);
+        const double *src = g.part + min(j, dv - 1);
         double s = 0.0;
         for (int k = k0; k < k1; k += 16) {
             double v[16];
@@ -692,41 +696,42 @@ __global__ __launch_bounds__(256) void diff_bwd_params_kernel(const double *__re
             for (int u = 0; u < 16; u++)
                 if (k + u < k1) s += v[u];
         }
-        red[q][jl] = s;
+        red[q * 16 + jl] = s;
         __syncthreads();
         if (q == 0 && j < dv) {
             double t = 0.0;
-            for (int u = 0; u < 16; u++) t += red[u][jl];
-            dgain[j] += (float)t;
+            for (int u = 0; u < Q; u++) t += red[u * 16 + jl];
+            g.dgain[j] += (float)t;
         }
         return;
     }
-    __shared__ double sums[4];
-    const int set = (int)blockIdx.x - ngain, step = lam_heads > 1 ? h : 1;
-    const int groups = nblk * gpb;
+    const int set = blk - ngain, step = g.lam_heads > 1 ? g.h : 1;
+    const int groups = g.nblk * g.gpb;
     double s = 0.0;
-    for (int k0 = set + step * (int)threadIdx.x; k0 < groups; k0 += step * 256 * 8) {
+    for (int k0 = set + step * (int)threadIdx.x; k0 < groups; k0 += step * NT * 8) {
         double v[8];
 #pragma unroll
         for (int u = 0; u < 8; u++) {
-            const int k = min(k0 + u * step * 256, groups - 1);
-            v[u] = part[(long long)(k / gpb) * cols + dv + k % gpb];
+            const int k = min(k0 + u * step * NT, groups - 1);
+            v[u] = g.part[(long long)(k / g.gpb) * cols + dv + k % g.gpb];
         }
 #pragma unroll
         for (int u = 0; u < 8; u++)
-            if (k0 + u * step * 256 < groups) s += v[u];
+            if (k0 + u * step * NT < groups) s += v[u];
     }
     s = rnn_wave_sum_d(s);
-    if (lane == 0) sums[wv] = s;
+    if (lane == 0) red[wv] = s;
     __syncthreads();
     if (wv) return;
-    const double t = sums[0] + sums[1] + sums[2] + sums[3];
+    double t = 0.0;
+    for (int i = 0; i < NT / 64; i++) t += red[i];
     double e1, e2;
-    lambda_dots(lam, lam_heads, dh, set, &e1, &e2);
+    lambda_dots(g.lam, g.lam_heads, g.dh, set, &e1, &e2);
     e1 = exp(e1);
     e2 = exp(e2);
-    const float *l = lam + (long long)set * 4 * dh;
-    float *d = dlam + (long long)set * 4 * dh;
+    const int dh = g.dh;
+    const float *l = g.lam + (long long)set * 4 * dh;
+    float *d = g.dlam + (long long)set * 4 * dh;
     if (lane < dh) {
         d[lane] += (float)(t * e1 * l[dh + lane]);
         d[dh + lane] += (float)(t * e1 * l[lane]);
@@ -735,13 +740,15 @@ __global__ __launch_bounds__(256) void diff_bwd_params_kernel(const double *__re
     }
 }
 
-// The power of two that takes 2 |dA| of rows with |dO| <= nd and values of
-// magnitude <= vmax to 2 or below: |dA| <= nd sqrt(W) vmax, and D is a mean of dA.
-// It stays as it was (up) while that holds, as sticky_up.
+// The power of two of dA for rows with |dO| <= nd and values of magnitude <= vmax,
+// from m = nd ds_root vmax >= 2 |dA| (|dA| <= nd sqrt(W) vmax, and D is a mean of
+// dA): it takes m to 2 or below, and stays as it was (up) while that holds, as
+// sticky_up.
 template <int W>
-__device__ __forceinline__ float ds_up(float nd, float vmax, float up) {
-    constexpr float root = W == 32 ? 5.6568543f : W == 64 ? 8.0f : W == 96 ? 9.7979590f : 11.313709f;
-    const float m = nd * (2.0f * root * vmax);
+__device__ __forceinline__ constexpr float ds_root() {
+    return W == 32 ? 11.313709f : W == 64 ? 16.0f : W == 96 ? 19.595918f : 22.627417f;
+}
+__device__ __forceinline__ float ds_up(float m, float up) {
     return m * up < 2.0f ? up : up_of(m) * 0x1p-18f;
 }
 // The power of two that softmax values, and lambda times them, enter the
@@ -755,39 +762,47 @@ __device__ __forceinline__ float p_up(float lam) { return up_of(fmaxf(1.0f, lam)
 // change sign, and the operand from registers with them.
 __device__ __forceinline__ int flip_at(int ntile) { return (2 * ntile + 2) / 3; }
 
-// dQ.  Rows as in the forward, a wave on both maps of its 32 rows, tiles of 32
-// keys in two LDS buffers: S_m^T = K_m Q_m^T and dA^T = V dO^T (lane = row), and
+// dQ.  Rows as in the forward, RG groups of 32 a workgroup, a wave on both maps of
+// its rows and on one of the KS 32 keys of a tile; tiles in two LDS buffers: S_m^T = K_m Q_m^T and dA^T = V dO^T (lane = row), and
 // P (dA - D) in registers is the operand of dQ_m^T = K_m^T dS_m^T, which is
 // summed over all tiles in the accumulators.  Their unit is a power of two that
-// hardly changes (sticky_up); where it does they are rescaled.
-template <int DHP, bool VEC, int NW>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DHP <= 32 ? 2 : 1))) void
+// hardly changes (sticky_up); where it does they are rescaled.  The waves that share
+// rows add theirs at the end.
+template <int DHP, bool VEC, int RG, int KG>
+__global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(DHP <= 32 ? 2 : 1))) void
 diff_dq_kernel(DiffArgs g) {
-    constexpr int W = 2 * DHP, TK = 32, NT = 64 * NW, KS = DHP / 16, VS = W / 16;
-    constexpr int CT = (DHP + 31) / 32;
+    constexpr int W = 2 * DHP, TK = 32 * KG, NW = RG * KG, NT = 64 * NW, KS = DHP / 16, VS = W / 16;
+    constexpr int CT = (DHP + 31) / 32, BR = 32 * RG;
     using Tile = HalfTile<TK, W>;
     // (a map's last 32-channel tile may run past the row: into the padding)
     __shared__ __align__(16) _Float16 lds[2][2 * Tile::HALVES + 32];
-    __shared__ float tmax[2][2][NW];
+    static_assert(KG == 1 || sizeof(lds) >= (size_t)(KG - 1) * RG * 2 * CT * 16 * 64 * 4, "exchange");
+    __shared__ f2 tmax[2][NW];
     const int lane = threadIdx.x & 63, wave = wave_index(), lr = lane & 31, lh = lane >> 5;
-    const int R = g.tq * g.group, nrb = (R + 32 * NW - 1) / (32 * NW);
-    const long long id = xcd_order(blockIdx.x, gridDim.x);
+    const int rg = wave % RG, kg = wave / RG;
+    const int R = g.tq * g.group, nrb = (R + BR - 1) / BR;
+    const int np = params_blocks(g);
+    if ((int)blockIdx.x < np) {
+        bwd_params<NT>(g, (int)blockIdx.x, (double *)lds);
+        return;
+    }
+    const long long id = xcd_order(blockIdx.x - np, gridDim.x - np);
     const int prob = (int)(id / nrb), rb = nrb - 1 - (int)(id % nrb);
     const int b = prob / g.hkv, kh = prob % g.hkv;
     const int nq = len_of(g.qlen, b, g.tq), nk = len_of(g.klen, b, g.tk), shift = nk - nq;
-    const int row = rb * 32 * NW + wave * 32 + lr;
+    const int row = rb * BR + rg * 32 + lr;
     const int qi = row / g.group, head = kh * g.group + row % g.group;
     const bool live = qi < nq;
-    const int last_q = min(nq - 1, (rb * 32 * NW + 32 * NW - 1) / g.group);
+    const int last_q = min(nq - 1, (rb * BR + BR - 1) / g.group);
     int kend = g.causal ? min(nk, last_q + shift + 1) : nk;
-    if (rb * 32 * NW / g.group >= nq) kend = 0;
+    if (rb * BR / g.group >= nq) kend = 0;
     const int ntile = kend > 0 ? (kend + TK - 1) / TK : 0;
     KvStage<DHP, TK, NT, VEC> st(g, b, kh, kend);
     if (ntile) st.load(0);
 
     // the row's queries, its dO and what the first pass left of it
-    const int w_first = (rb * 32 * NW + wave * 32) / g.group;
-    const int w_last = min(nq - 1, (rb * 32 * NW + wave * 32 + 31) / g.group);
+    const int w_first = (rb * BR + rg * 32) / g.group;
+    const int w_last = min(nq - 1, (rb * BR + rg * 32 + 31) / g.group);
     const int q0 = min(w_first, g.tq - 1), qx = qi - q0, dv = 2 * g.dh;
     const long long img = (long long)b * g.tq + q0;
     const int left = min(g.tq - q0, 32);
@@ -824,36 +839,37 @@ diff_dq_kernel(DiffArgs g) {
         for (int c = 0; c < CT; c++)
 #pragma unroll
             for (int r = 0; r < 16; r++) acc[m][c][r] = 0.f;
-    // the staged tile's largest value, and powers of two: of the tile that is staged
-    // (.1) and of the one that is computed
-    float mv = 0.f, kup1 = FIRST_UP, vup1 = 1.f, kup = FIRST_UP, dsup = FIRST_UP, sgn = 1.f;
+    // the largest value so far, and powers of two: of the tile that is staged (.1)
+    // and of the one that is computed
+    float vmax = 0.f, kup1 = FIRST_UP, vup1 = 1.f, kup = FIRST_UP, dsup = FIRST_UP, sgn = 1.f;
     const int flip = flip_at(ntile);
+    auto maxima = [&](int slot) { st.maxima(tmax[slot], good_for(kup1), vmax); };
     auto stage = [&](int t) {  // tile t, whose maxima are there, into its buffer
         float mk = 0.f;
-        mv = 0.f;
 #pragma unroll
         for (int i = 0; i < NW; i++) {
-            mk = max2(mk, tmax[t & 1][0][i]);
-            mv = max2(mv, tmax[t & 1][1][i]);
+            const f2 m = tmax[t & 1][i];
+            mk = max2(mk, m[0]);
+            vmax = max2(vmax, m[1]);
         }
         kup1 = sticky_up(mk, kup1);
-        vup1 = up_of(mv);
+        vup1 = up_of(vmax);
         st.store(lds[t & 1], kup1, vup1);
     };
     if (ntile) {
-        st.maxima(tmax[0][0], tmax[0][1]);
+        maxima(0);
         __syncthreads();
         stage(0);
         if (ntile > 1) {
             st.load(TK);
-            st.maxima(tmax[1][0], tmax[1][1]);
+            maxima(1);
         }
     }
     for (int t = 0; t < ntile; t++) {
         const int k0 = t * TK;
         __syncthreads();
         // dS's power of two, and the accumulators in the tile's unit
-        const float vup = vup1, dsup1 = ds_up<W>(dd[2], mv, dsup);
+        const float vup = vup1, dsup1 = ds_up(dd[2] * (ds_root<W>() * vmax), dsup);
         float ratio = down_of(kup) * kup1 * (down_of(dsup) * dsup1);
         kup = kup1;
         dsup = dsup1;
@@ -874,7 +890,8 @@ diff_dq_kernel(DiffArgs g) {
         if (t + 1 < ntile) stage(t + 1);
         if (t + 2 < ntile) st.load(k0 + 2 * TK);
         {
-            const _Float16 *const kt = lds[t & 1], *const vt = kt + Tile::HALVES;
+            const _Float16 *const kt = lds[t & 1] + 32 * kg * Tile::STRIDE, *const vt = kt + Tile::HALVES;
+            const int k1 = k0 + 32 * kg;
             const float kdown = down_of(kup);
             f32x16 s1, s2, da;
 #pragma unroll
@@ -889,12 +906,12 @@ diff_dq_kernel(DiffArgs g) {
                 s1[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s1[r], f1, nm[0])) * il[0];
                 s2[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s2[r], f2, nm[1])) * il[1];
             }
-            const bool whole = k0 + TK <= nk && !(g.causal && k0 + TK - 1 > w_first + shift) &&
-                               !(g.diag && k0 <= w_last && w_first < k0 + TK);
+            const bool whole = k1 + 32 <= nk && !(g.causal && k1 + 31 > w_first + shift) &&
+                               !(g.diag && k1 <= w_last && w_first < k1 + 32);
             if (!whole) {
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
-                    const int j = k0 + 8 * (r >> 2) + 4 * lh + (r & 3);
+                    const int j = k1 + 8 * (r >> 2) + 4 * lh + (r & 3);
                     const bool in = j < nk && !(g.causal && j > qi + shift) && !(g.diag && j == qi);
                     s1[r] = in ? s1[r] : 0.f;
                     s2[r] = in ? s2[r] : 0.f;
@@ -915,7 +932,25 @@ diff_dq_kernel(DiffArgs g) {
             }
             read_ahead<4 * CT, 4, 3>();
         }
-        if (t + 2 < ntile) st.maxima(tmax[t & 1][0], tmax[t & 1][1]);
+        if (t + 2 < ntile) maxima(t & 1);
+    }
+    if constexpr (KG > 1) {
+        __syncthreads();
+        float *const ex = (float *)lds + rg * 2 * CT * 16 * 64 + lane;
+        auto each = [&](int i, auto &&f) {
+            float *e = ex + (i - 1) * RG * 2 * CT * 16 * 64;
+#pragma unroll
+            for (int m = 0; m < 2; m++)
+#pragma unroll
+                for (int c = 0; c < CT; c++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) f(e[((m * CT + c) * 16 + r) * 64], acc[m][c], r);
+        };
+        if (kg) each(kg, [](float &e, f32x16 &v, int r) { e = v[r]; });
+        __syncthreads();
+        if (kg) return;
+#pragma unroll
+        for (int i = 1; i < KG; i++) each(i, [](float &e, f32x16 &v, int r) { v[r] += e; });
     }
     if (row >= R) return;
     float *dst = g.dq + ((long long)b * g.tq + qi) * g.qstride + 2 * head * g.dh;
@@ -928,36 +963,42 @@ diff_dq_kernel(DiffArgs g) {
                               g.acc_q);
 }
 
-// dK and dV.  One workgroup of NW waves per (image, key head, 32 NW keys), wave
-// w on 32 of them: its keys' and values' parts stay in registers.  Tiles of 32
-// rows (queries of the head group) and their records in two LDS buffers:
-// S_m = Q_m K_m^T and dA = dO V^T (lane = key), and P and dS in registers are
-// the operands of dV^T = dO^T (P_1 - lambda P_2) and dK_m^T = Q_m^T dS_m, summed
-// over all tiles in the accumulators as in diff_dq_kernel.
-template <int DHP, bool VEC, int NW>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(1))) void
+// dK and dV.  One workgroup of 2 KG waves per (image, key head, 32 KG keys); a pair
+// of waves takes 32 keys, wave 2 i + m map m of them: its half of a row's channels
+// of Q K^T (a map) and of dO V^T stays in registers.  Tiles of 32 rows (queries of
+// the head group) and their records in two LDS buffers: S_m = Q_m K_m^T and the
+// wave's half of dA = dO V^T (lane = key); P_m and that half go to the partner
+// through LDS, and then P and dS in registers are the operands of the wave's half
+// of dV^T = dO^T (P_1 - lambda P_2) and of dK_m^T = Q_m^T dS_m, summed over all tiles
+// in the accumulators as in diff_dq_kernel.
+template <int DHP, bool VEC, int KG>
+__global__ __launch_bounds__(128 * KG) __attribute__((amdgpu_waves_per_eu(2))) void
 diff_dkv_kernel(DiffArgs g) {
-    constexpr int W = 2 * DHP, TR = 32, NT = 64 * NW, KS = DHP / 16, VS = W / 16;
-    constexpr int CT = (DHP + 31) / 32, VT = DHP / 16;
+    constexpr int W = 2 * DHP, TR = 32, NW = 2 * KG, NT = 64 * NW, KS = DHP / 16;
+    constexpr int CT = (DHP + 31) / 32, VT = (DHP / 16 + 1) / 2, BK = 32 * KG;
     using Tile = HalfTile<TR, W>;
     using Stage = StagePlan<TR, W, NT>;
     constexpr int CH = Stage::PASSES;
     __shared__ __align__(16) _Float16 lds[2][2 * Tile::HALVES + 32];
-    // -m1, il1, -m2, lambda il2, -D1, -D2, with their powers of two
+    // -m1, il1, -m2, -lambda il2, -D1, -D2, with their powers of two
     __shared__ __align__(16) float rec[2][6][TR];
-    __shared__ float tmax[2][4][NW];  // largest |q|, |dO|, |dO|_2, |lambda| of a tile
+    // largest |q|, |dO|, |dO|_2, |lambda| of a tile past what is known of them
+    __shared__ f4 tmax[2][NW];
     __shared__ float vmaxs[NW];
+    __shared__ float vkey[NW][32];
+    __shared__ __align__(16) f32x4 ex[NW][8][64];  // P_m and a half of dA, each wave's
     const int lane = threadIdx.x & 63, wave = wave_index(), lr = lane & 31, lh = lane >> 5;
-    const int nkb = (g.tk + 32 * NW - 1) / (32 * NW);
+    const int kg = wave >> 1, map = wave & 1;
+    const int nkb = (g.tk + BK - 1) / BK;
     const long long id = xcd_order(blockIdx.x, gridDim.x);
     const int prob = (int)(id / nkb), kb = (int)(id % nkb);
     const int b = prob / g.hkv, kh = prob % g.hkv;
     const int nq = len_of(g.qlen, b, g.tq), nk = len_of(g.klen, b, g.tk), shift = nk - nq;
-    const int w_first = kb * 32 * NW + wave * 32, key = w_first + lr;
+    const int w_first = kb * BK + kg * 32, key = w_first + lr;
     const bool live = key < nk;
     // rows that see some key of the block
-    const int first_q = g.causal ? max(0, kb * 32 * NW - shift) : 0;
-    const int row_end = kb * 32 * NW < nk ? nq * g.group : 0;
+    const int first_q = g.causal ? max(0, kb * BK - shift) : 0;
+    const int row_end = kb * BK < nk ? nq * g.group : 0;
     const int row_beg = min(first_q, nq) * g.group;
     const int ntile = row_end > row_beg ? (row_end - row_beg + TR - 1) / TR : 0;
     const float ginv = 1.0f / (float)g.group;
@@ -970,33 +1011,57 @@ diff_dkv_kernel(DiffArgs g) {
     const int qlim = stager ? g.dh - (sc - run * DHP) : 0, dlim = stager ? dw - sc : 0;
     const long long img = (long long)b * g.tq;
     const int qc = run * g.dh + sc - run * DHP;
-    auto load = [&](int row0) {
-        // row x of the tile is query q0 + (x0 + x) / group, head (x0 + x) % group of
-        // the group (x0 + x < 32 + group, exact in floats); rows from row_end on
-        // are left out
-        const int q0 = row0 / g.group, x0 = row0 - q0 * g.group, left = row_end - row0;
-        const int rows = left > 0 ? min(nq - q0, 33) : 0;
-        const auto rq = rows_rsrc(g.q + (img + q0) * g.qstride + 2 * kh * g.group * g.dh, rows,
-                                  g.qstride, 2 * g.group * g.dh);
-        const auto rd = rows_rsrc(g.dout + ((img + q0) * g.h + kh * g.group) * dw, rows,
-                                  (long long)g.h * dw, g.group * dw);
-        const auto rr = rows_rsrc(g.rec + ((img + q0) * g.h + kh * g.group) * 8, rows,
-                                  (long long)g.h * 8, g.group * 8);
-#pragma unroll
-        for (int i = 0; i < CH; i++) {
-            const int x = sr + i * Stage::RPP;
-            const int dq = (int)(((float)(x0 + x) + 0.5f) * ginv), hd = x0 + x - dq * g.group;
-            const bool in = x < left;
-            load8<VEC>(rq, (uint32_t)dq * (uint32_t)g.qstride + 2 * hd * g.dh + qc, in ? qlim : 0, xq[i]);
-            load8<VEC>(rd, (uint32_t)(dq * g.h + hd) * dw + sc, in ? dlim : 0, xd[i]);
-        }
-        if (wave == 0) {
-            const int dq = (int)(((float)(x0 + lr) + 0.5f) * ginv), hd = x0 + lr - dq * g.group;
-            const uint32_t at = lr < left ? (uint32_t)(dq * g.h + hd) * 32u : DMA_OOB;
-            r0 = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rr, at, 0, 0));
-            r1 = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rr, at + 16u, 0, 0));
+    // row x of a tile is query q0 + (x0 + x) / group, head (x0 + x) % group of the
+    // group (x0 + x < TR + group, exact in floats).  lq0, lx0: of the tile that is
+    // loaded next, whose offsets are those of every tile where the group divides TR.
+    int lq0 = row_beg / g.group, lx0 = 0, cq0 = lq0, cx0 = 0;
+    const bool steady = TR % g.group == 0;
+    auto next = [&](int &q0, int &x0) {
+        q0 += TR / g.group;
+        x0 += TR % g.group;
+        if (x0 >= g.group) {
+            x0 -= g.group;
+            q0++;
         }
     };
+    uint32_t qo[CH], od[CH], ro;
+    auto offsets = [&] {
+#pragma unroll
+        for (int i = 0; i < CH; i++) {
+            const int x = lx0 + sr + i * Stage::RPP;
+            const int dq = (int)(((float)x + 0.5f) * ginv), hd = x - dq * g.group;
+            qo[i] = (uint32_t)dq * (uint32_t)g.qstride + 2 * hd * g.dh + qc;
+            od[i] = (uint32_t)(dq * g.h + hd) * dw + sc;
+        }
+        const int x = lx0 + lr, dq = (int)(((float)x + 0.5f) * ginv);
+        ro = (uint32_t)(dq * g.h + x - dq * g.group) * 32u;
+    };
+    offsets();
+    auto load = [&] {
+        if (!steady) offsets();
+        // queries from nq on are past the resources' end
+        const int rows = min(nq - lq0, TR + 1);
+        const auto rq = rows_rsrc(g.q + (img + lq0) * g.qstride + 2 * kh * g.group * g.dh, rows,
+                                  g.qstride, 2 * g.group * g.dh);
+        const auto rd = rows_rsrc(g.dout + ((img + lq0) * g.h + kh * g.group) * dw, rows,
+                                  (long long)g.h * dw, g.group * dw);
+#pragma unroll
+        for (int i = 0; i < CH; i++) {
+            load8<VEC>(rq, qo[i], qlim, xq[i]);
+            load8<VEC>(rd, od[i], dlim, xd[i]);
+        }
+        if (wave == 0) {
+            const auto rr = rows_rsrc(g.rec + ((img + lq0) * g.h + kh * g.group) * 8, rows,
+                                      (long long)g.h * 8, g.group * 8);
+            r0 = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rr, ro, 0, 0));
+            r1 = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rr, ro + 16u, 0, 0));
+        }
+        next(lq0, lx0);
+    };
+    // the largest value and lambda so far, the powers of two of the tile that is
+    // staged (.1) and of the one that is computed
+    float vmax = INFINITY, ml = 0.f, qup1 = FIRST_UP, dup1 = FIRST_UP, pup1 = 1.f, sup1 = FIRST_UP;
+    float qup = FIRST_UP, dup = FIRST_UP, pup = 1.f, sup = FIRST_UP;
     auto maxima = [&](int slot) {
         float mq = 0.f, md = 0.f;
 #pragma unroll
@@ -1004,25 +1069,18 @@ diff_dkv_kernel(DiffArgs g) {
             mq = absmax8(xq[i], mq);
             md = absmax8(xd[i], md);
         }
-        mq = wave_max(mq);
-        md = wave_max(md);
-        float mn = 0.f, ml = 0.f;
+        f4 m = {wave_over(mq, good_for(qup1)), wave_over(md, good_for(dup1)), 0.f, 0.f};
         if (wave == 0) {
-            mn = wave_max(r1[2]);
-            ml = wave_max(fabsf(r1[3]));
+            if (__any(!(r1[2] * (ds_root<W>() * vmax) * sup1 < 2.0f))) m[2] = wave_max(r1[2]);
+            m[3] = wave_over(fabsf(r1[3]), ml);
         }
-        if (lane == 0) {
-            tmax[slot][0][wave] = mq;
-            tmax[slot][1][wave] = md;
-            tmax[slot][2][wave] = mn;
-            tmax[slot][3][wave] = ml;
-        }
+        if (lane == 0) tmax[slot][wave] = m;
     };
-    if (ntile) load(row_beg);
+    if (ntile) load();
 
-    // the lane's key and value
-    Half2 k[2][KS], v[VS];
-    float kdown[2], vdown;
+    // the lane's key and value: the map's half of their channels
+    Half2 k[KS], v[KS];
+    float kdown, vdown;
     const long long krow = (long long)b * g.tk + min(key, g.tk - 1);
     {
         const int k0 = min(w_first, g.tk - 1), rows = min(g.tk - k0, 32);
@@ -1030,48 +1088,52 @@ diff_dkv_kernel(DiffArgs g) {
         const auto rk = rows_rsrc(kvp + g.koff, rows, g.kvstride, dw);
         const auto rv = rows_rsrc(kvp + g.voff, rows, g.kvstride, dw);
         const uint32_t off = (uint32_t)(key - k0) * (uint32_t)g.kvstride;
-        RowFrag<KS> kf[2];
-        RowFrag<VS> vf;
+        RowFrag<KS> kf, vf;
+        kf.template load<VEC>(rk, off + map * g.dh, live ? g.dh : 0);
+        vf.template load<VEC>(rv, off + map * DHP, live ? dw - map * DHP : 0);
+        kdown = kf.split(k) * (g.scale * LOG2E);
+        // (a key's two halves share their power of two)
+        float mv = 0.f;
 #pragma unroll
-        for (int m = 0; m < 2; m++) kf[m].template load<VEC>(rk, off + m * g.dh, live ? g.dh : 0);
-        vf.template load<VEC>(rv, off, live ? dw : 0);
-#pragma unroll
-        for (int m = 0; m < 2; m++) kdown[m] = kf[m].split(k[m]) * (g.scale * LOG2E);
-        vdown = vf.split(v);
-        const float mx = wave_max(vf.mx);
+        for (int s = 0; s < KS; s++) mv = absmax8(vf.v[s], mv);
+        mv = pair32(mv, max2);
+        if (lh == 0) vkey[wave][lr] = mv;
+        const float mx = wave_max(mv);
         if (lane == 0) vmaxs[wave] = mx;
+        if (ntile) maxima(0);
+        __syncthreads();
+        const float up = up_of(max2(mv, vkey[wave ^ 1][lr]));
+#pragma unroll
+        for (int s = 0; s < KS; s++) v[s] = half_split(vf.v[s], up);
+        vdown = down_of(up);
     }
-    f32x16 dk[2][CT], dv[VT];
+    f32x16 dk[CT], dv[VT];
 #pragma unroll
     for (int r = 0; r < 16; r++) {
 #pragma unroll
-        for (int m = 0; m < 2; m++)
-#pragma unroll
-            for (int c = 0; c < CT; c++) dk[m][c][r] = 0.f;
+        for (int c = 0; c < CT; c++) dk[c][r] = 0.f;
 #pragma unroll
         for (int c = 0; c < VT; c++) dv[c][r] = 0.f;
     }
-    // the largest value and lambda so far, the powers of two of the tile that is
-    // staged (.1) and of the one that is computed
-    float vmax = 0.f, ml = 0.f, qup1 = FIRST_UP, dup1 = FIRST_UP, pup1 = 1.f, sup1 = FIRST_UP;
-    float qup = FIRST_UP, dup = FIRST_UP, pup = 1.f, sup = FIRST_UP;
     const int flip = flip_at(ntile);
     auto stage = [&](int t) {
         float mq = 0.f, md = 0.f;
 #pragma unroll
         for (int i = 0; i < NW; i++) {
-            mq = max2(mq, tmax[t & 1][0][i]);
-            md = max2(md, tmax[t & 1][1][i]);
+            const f4 m = tmax[t & 1][i];
+            mq = max2(mq, m[0]);
+            md = max2(md, m[1]);
+            if (i) continue;
+            ml = max2(ml, m[3]);
+            sup1 = ds_up(m[2] * (ds_root<W>() * vmax), sup1);
         }
-        ml = max2(ml, tmax[t & 1][3][0]);
         qup1 = sticky_up(mq, qup1);
         dup1 = sticky_up(md, dup1);
         pup1 = p_up(ml);
-        sup1 = ds_up<W>(tmax[t & 1][2][0], vmax, sup1);
         if (stager) {
 #pragma unroll
             for (int i = 0; i < CH; i++) {
-                _Float16 *p = lds[t & 1] + (sr + i * Stage::RPP) * Tile::STRIDE + sc;
+                _Float16 *p = lds[t & 1] + row_pos(sr + i * Stage::RPP) * Tile::STRIDE + sc;
                 const Half2 hq = half_split(xq[i], qup1), hd = half_split(xd[i], dup1);
                 *(h8 *)p = hq.hi;
                 *(h8 *)(p + Tile::PART) = hq.lo;
@@ -1085,24 +1147,22 @@ diff_dkv_kernel(DiffArgs g) {
             rc[0][threadIdx.x] = -r0[0];
             rc[1][threadIdx.x] = r0[1] * u;
             rc[2][threadIdx.x] = -r0[2];
-            rc[3][threadIdx.x] = r0[3] * r1[3] * u;
+            rc[3][threadIdx.x] = -r0[3] * r1[3] * u;
             rc[4][threadIdx.x] = -r1[0] * sup1;
             rc[5][threadIdx.x] = -r1[1] * sup1;
         }
     };
     if (ntile) {
-        maxima(0);
-        __syncthreads();
+        vmax = 0.f;
 #pragma unroll
         for (int i = 0; i < NW; i++) vmax = max2(vmax, vmaxs[i]);
         stage(0);
         if (ntile > 1) {
-            load(row_beg + TR);
+            load();
             maxima(1);
         }
     }
     for (int t = 0; t < ntile; t++) {
-        const int row0 = row_beg + t * TR;
         __syncthreads();
         float rv = down_of(pup) * pup1 * (down_of(dup) * dup1);
         float rk = down_of(pup) * pup1 * (down_of(qup) * qup1) * (down_of(sup) * sup1);
@@ -1118,94 +1178,105 @@ diff_dkv_kernel(DiffArgs g) {
 #pragma unroll
             for (int r = 0; r < 16; r++) {
 #pragma unroll
-                for (int m = 0; m < 2; m++)
-#pragma unroll
-                    for (int c = 0; c < CT; c++) dk[m][c][r] *= rk;
+                for (int c = 0; c < CT; c++) dk[c][r] *= rk;
 #pragma unroll
                 for (int c = 0; c < VT; c++) dv[c][r] *= rv;
             }
         }
         if (t + 1 < ntile) stage(t + 1);
-        if (t + 2 < ntile) load(row0 + 2 * TR);
-        const int tq0 = row0 / g.group, tq1 = min(nq - 1, (row0 + TR - 1) / g.group);
-        {
-            const _Float16 *const qt = lds[t & 1], *const dt = qt + Tile::HALVES;
-            const float(*rc)[TR] = rec[t & 1];
-            f32x16 s1, s2, da;
+        if (t + 2 < ntile) load();
+        const int tq0 = cq0, x0 = cx0;
+        next(cq0, cx0);
+        const _Float16 *const qt = lds[t & 1], *const dt = qt + Tile::HALVES;
+        const float(*rc)[TR] = &rec[t & 1][2 * map];
+        f32x16 s, da;
 #pragma unroll
-            for (int r = 0; r < 16; r++) s1[r] = s2[r] = da[r] = 0.f;
-            dot_along<Tile>(qt, 0, k[0], s1);
-            dot_along<Tile>(qt, DHP, k[1], s2);
-            dot_along<Tile>(dt, 0, v, da);
-            read_ahead<2 * KS + VS, 2, 3>();
-            const float qd = down_of(qup), f1 = qd * kdown[0], f2 = qd * kdown[1];
+        for (int r = 0; r < 16; r++) s[r] = da[r] = 0.f;
+        dot_along<Tile>(qt, map * DHP, k, s);
+        dot_along<Tile>(dt, map * DHP, v, da);
+        read_ahead<2 * KS, 2, 3>();
+        const float f = down_of(qup) * kdown;
 #pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const f32x4 m1 = *(const f32x4 *)&rc[0][2 * r + 4 * lh], l1 = *(const f32x4 *)&rc[1][2 * r + 4 * lh];
-                const f32x4 m2 = *(const f32x4 *)&rc[2][2 * r + 4 * lh], l2 = *(const f32x4 *)&rc[3][2 * r + 4 * lh];
+        for (int r = 0; r < 16; r += 4) {
+            const f32x4 m4 = *(const f32x4 *)&rc[0][2 * r + 4 * lh], l4 = *(const f32x4 *)&rc[1][2 * r + 4 * lh];
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    s1[r + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s1[r + e], f1, m1[e])) * l1[e];
-                    s2[r + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s2[r + e], f2, m2[e])) * l2[e];
-                }
-            }
-            // rows past the last carry il = 0, keys past the last are not stored
-            const bool whole = !(g.causal && w_first + 31 > tq0 + shift) &&
-                               !(g.diag && w_first <= tq1 && tq0 <= w_first + 31);
-            if (!whole) {
-                const int x0 = row0 - tq0 * g.group;
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const int x = x0 + 8 * (r >> 2) + 4 * lh + (r & 3);
-                    const int i = tq0 + (int)(((float)x + 0.5f) * ginv);
-                    const bool in = !(g.causal && key > i + shift) && !(g.diag && key == i);
-                    s1[r] = in ? s1[r] : 0.f;
-                    s2[r] = in ? s2[r] : 0.f;
-                }
-            }
-            {
-                f32x16 a;
-#pragma unroll
-                for (int r = 0; r < 16; r++) a[r] = s1[r] - s2[r];
-                Half2 ah[2];
-                split16(a, ah);
-#pragma unroll
-                for (int c = 0; c < VT; c++) dot_across<Tile>(dt, 32 * c, ah, dv[c]);
-            }
-            const float fd = vdown * down_of(dup) * sup;
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const f32x4 D1 = *(const f32x4 *)&rc[4][2 * r + 4 * lh], D2 = *(const f32x4 *)&rc[5][2 * r + 4 * lh];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    s1[r + e] *= __builtin_fmaf(da[r + e], fd, D1[e]);
-                    s2[r + e] *= __builtin_fmaf(da[r + e], fd, D2[e]);
-                }
-            }
-#pragma unroll
-            for (int m = 0; m < 2; m++) {
-                Half2 ds[2];
-                split16(m ? s2 : s1, ds);
-#pragma unroll
-                for (int c = 0; c < CT; c++) dot_across<Tile>(qt, m * DHP + 32 * c, ds, dk[m][c]);
-            }
-            read_ahead<2 * (VT + 2 * CT), 4, 3>();
+            for (int e = 0; e < 4; e++)
+                s[r + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + e], f, m4[e])) * l4[e];
         }
+        // rows past the last carry il = 0, keys past the last are not stored
+        const bool whole = !(g.causal && w_first + 31 > tq0 + shift) &&
+                           !(g.diag && w_first <= tq0 + (x0 + TR - 1) / g.group && tq0 <= w_first + 31);
+        if (!whole) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const int x = x0 + 8 * (r >> 2) + 4 * lh + (r & 3);
+                const int i = tq0 + (int)(((float)x + 0.5f) * ginv);
+                const bool in = !(g.causal && key > i + shift) && !(g.diag && key == i);
+                s[r] = in ? s[r] : 0.f;
+            }
+        }
+        const float fd = vdown * down_of(dup) * sup;
+        f32x4 *const mine = &ex[wave][0][lane], *const other = &ex[wave ^ 1][0][lane];
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            f32x4 p, d;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                p[e] = s[r + e];
+                d[e] = da[r + e];
+            }
+            mine[16 * r] = p;
+            mine[16 * r + 256] = d;
+        }
+        __syncthreads();
+        {
+            // P_1 - lambda P_2 (P_2's sign is in its rec) and dA, the same in both waves
+            f32x16 a;
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const f32x4 p = other[16 * r], d = other[16 * r + 256];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    a[r + e] = s[r + e] + p[e];
+                    da[r + e] += d[e];
+                }
+            }
+            Half2 ah[2];
+            split16(a, ah);
+#pragma unroll
+            for (int c = 0; c < VT; c++)
+                if (VT * 32 * 2 == W || map * VT + c < W / 32)
+                    dot_across<Tile>(dt, 32 * (map * VT + c), ah, dv[c]);
+        }
+        rc = &rec[t & 1][4 + map];
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const f32x4 D = *(const f32x4 *)&rc[0][2 * r + 4 * lh];
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[r + e] *= __builtin_fmaf(da[r + e], fd, D[e]);
+        }
+        {
+            Half2 ds[2];
+            split16(s, ds);
+#pragma unroll
+            for (int c = 0; c < CT; c++) dot_across<Tile>(qt, map * DHP + 32 * c, ds, dk[c]);
+        }
+        read_ahead<2 * (VT + CT), 4, 3>();
         if (t + 2 < ntile) maxima(t & 1);
     }
     if (key >= g.tk) return;
-    float *kd = g.dkv + krow * g.kvstride + g.koff + 2 * kh * g.dh;
+    float *kd = g.dkv + krow * g.kvstride + g.koff + (2 * kh + map) * g.dh;
     float *vd = g.dkv + krow * g.kvstride + g.voff + 2 * kh * g.dh;
     const float sgn = ntile > flip ? -1.0f : 1.0f;
     const float fk = down_of(qup) * (g.scale * sgn), fk2 = down_of(pup) * down_of(sup);
 #pragma unroll
-    for (int m = 0; m < 2; m++)
-#pragma unroll
-        for (int c = 0; c < CT; c++)
-            put_channels<VEC>(kd + m * g.dh, g.dh, 32 * c, dk[m][c], m ? -fk : fk, fk2, live, g.acc_kv);
+    for (int c = 0; c < CT; c++)
+        put_channels<VEC>(kd, g.dh, 32 * c, dk[c], fk, fk2, live, g.acc_kv);
 #pragma unroll
     for (int c = 0; c < VT; c++)
-        put_channels<VEC>(vd, 2 * g.dh, 32 * c, dv[c], down_of(dup) * sgn, down_of(pup), live, g.acc_kv);
+        if (VT * 32 * 2 == W || map * VT + c < W / 32)
+            put_channels<VEC>(vd, 2 * g.dh, 32 * (map * VT + c), dv[c], down_of(dup) * sgn,
+                              down_of(pup), live, g.acc_kv);
 }
 
 // The backward's first pass: lanes of a unit and blocks, so that the groups of
@@ -1230,7 +1301,9 @@ PrePlan plan_pre(const rnn_diff_attn_desc *d, size_t n, bool vec) {
 }
 
 // Row groups of 32 a workgroup of the forward, and the splits of the keys: a
-// power of two of groups up to four, keys split where the rows leave CUs idle.
+// power of two of groups up to four, keys split where the rows leave half of the
+// CUs idle (2 x 8 causal heads of 1568 rows and keys, dh 64, 208 workgroups: 111 us
+// unsplit, 124 and 24 for the join with two splits).
 struct FwdPlan {
     int qg, splits, split_keys;
     size_t blocks;
@@ -1241,7 +1314,7 @@ FwdPlan plan_fwd(const rnn_diff_attn_desc *d, size_t n, bool vec) {
     p.qg = !vec ? 4 : R <= 32 ? 1 : R <= 64 ? 2 : 4;
     p.blocks = probs * rnn_div_up(R, (size_t)32 * p.qg);
     const size_t tiles = rnn_div_up(d->tk, (size_t)64);
-    size_t s = p.blocks && p.blocks < 256 ? std::min(tiles / 4, 512 / p.blocks) : 1;
+    size_t s = p.blocks && p.blocks < 128 ? std::min(tiles / 4, 512 / p.blocks) : 1;
     s = std::max<size_t>(1, std::min<size_t>(s, 64));
     const size_t per = rnn_div_up(std::max<size_t>(tiles, 1), s);
     p.split_keys = (int)per * 64;
@@ -1363,43 +1436,44 @@ void launch_fwd(rnn_ctx *ctx, const DiffArgs &g, const FwdPlan &p, bool vec) {
         launch_fwd_qg<DHP, true, 4>(ctx, g, p);
 }
 
-// Waves of a workgroup by the rows (or keys) that there are: 32 each, up to four.
-int waves_of(size_t rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : 4; }
-
-template <int DHP, bool VEC, int NW>
+template <int DHP, bool VEC, int RG, int KG>
 void launch_dq(rnn_ctx *ctx, const DiffArgs &g) {
     const size_t R = (size_t)g.tq * g.group;
-    const unsigned grid = (unsigned)((size_t)g.n * g.hkv * rnn_div_up(R, 32 * NW));
-    diff_dq_kernel<DHP, VEC, NW><<<grid, 64 * NW, 0, ctx->stream>>>(g);
+    const size_t params = (g.dgain ? rnn_div_up(2 * (size_t)g.dh, 16) : 0) + (size_t)g.lam_heads;
+    const unsigned grid = (unsigned)((size_t)g.n * g.hkv * rnn_div_up(R, 32 * RG) + params);
+    diff_dq_kernel<DHP, VEC, RG, KG><<<grid, 64 * RG * KG, 0, ctx->stream>>>(g);
 }
-template <int DHP, bool VEC, int NW>
+template <int DHP, bool VEC, int KG>
 void launch_dkv(rnn_ctx *ctx, const DiffArgs &g) {
-    const unsigned grid = (unsigned)((size_t)g.n * g.hkv * rnn_div_up((size_t)g.tk, 32 * NW));
-    diff_dkv_kernel<DHP, VEC, NW><<<grid, 64 * NW, 0, ctx->stream>>>(g);
+    const unsigned grid = (unsigned)((size_t)g.n * g.hkv * rnn_div_up((size_t)g.tk, 32 * KG));
+    diff_dkv_kernel<DHP, VEC, KG><<<grid, 128 * KG, 0, ctx->stream>>>(g);
 }
+// dQ: two waves share 32 rows wherever rows are short of filling 4 groups in every
+// CU twice (128 x 4 heads of 64 rows and keys, dh 32: 16.6 us against 17.4; 64 rows
+// on 256 keys: 26.8 against 32.2; 2 x 8 causal heads of 1568, dh 64: 110 against
+// 146; 8 x 6 of 577, dh 32: 38.9 against 38.0).  dK and dV: two groups of 32 keys, a
+// workgroup of four waves (the same with four groups: 26.8 against 16.7 us, 60.6
+// against 49.4, 188 against 167, 55.1 against 56.5).
 template <int DHP>
 void launch_bwd(rnn_ctx *ctx, const DiffArgs &g, bool vec) {
+    const size_t probs = (size_t)g.n * g.hkv, R = (size_t)g.tq * g.group;
     if (g.tq) {
-        const int nw = waves_of((size_t)g.tq * g.group);
         if (!vec)
-            launch_dq<DHP, false, 4>(ctx, g);
-        else if (nw == 1)
-            launch_dq<DHP, true, 1>(ctx, g);
-        else if (nw == 2)
-            launch_dq<DHP, true, 2>(ctx, g);
+            launch_dq<DHP, false, 4, 1>(ctx, g);
+        else if (R <= 32)
+            launch_dq<DHP, true, 1, 2>(ctx, g);
+        else if (R <= 64 || probs * rnn_div_up(R, 128) < 512)
+            launch_dq<DHP, true, 2, 2>(ctx, g);
         else
-            launch_dq<DHP, true, 4>(ctx, g);
+            launch_dq<DHP, true, 4, 1>(ctx, g);
     }
     if (g.tk) {
-        const int nw = waves_of((size_t)g.tk);
         if (!vec)
-            launch_dkv<DHP, false, 4>(ctx, g);
-        else if (nw == 1)
+            launch_dkv<DHP, false, 2>(ctx, g);
+        else if (g.tk <= 32)
             launch_dkv<DHP, true, 1>(ctx, g);
-        else if (nw == 2)
-            launch_dkv<DHP, true, 2>(ctx, g);
         else
-            launch_dkv<DHP, true, 4>(ctx, g);
+            launch_dkv<DHP, true, 2>(ctx, g);
     }
 }
 
@@ -1506,11 +1580,15 @@ int rnn_diff_attn_backward(rnn_ctx *ctx, const rnn_diff_attn_desc *d, size_t n, 
     g.part = (double *)((char *)ws + w.part);
     g.acc_q = (flags & RNN_ATTN_SET_DQ) ? 0 : 1;
     g.acc_kv = (flags & RNN_ATTN_SET_DKV) ? 0 : 1;
+    g.dlam = dlam;
+    g.dgain = dgain;
     const bool vec = rows_vec(g);
     const size_t rows = n * d->tq;
     if (rows) {
         const PrePlan p = plan_pre(d, n, vec);
         const unsigned nblk = (unsigned)p.blocks;
+        g.nblk = (int)nblk;
+        g.gpb = 256 / p.lpu;
         if (p.lpu == 8)
             diff_bwd_pre_kernel<8><<<nblk, 256, 0, ctx->stream>>>(g);
         else if (p.lpu == 16)
@@ -1519,10 +1597,6 @@ int rnn_diff_attn_backward(rnn_ctx *ctx, const rnn_diff_attn_desc *d, size_t n, 
             diff_bwd_pre_kernel<32><<<nblk, 256, 0, ctx->stream>>>(g);
         else
             diff_bwd_pre_kernel<64><<<nblk, 256, 0, ctx->stream>>>(g);
-        RNN_LAUNCHED(ctx);
-        const unsigned np = (gain ? (unsigned)rnn_div_up(2 * g.dh, 16) : 0u) + (unsigned)g.lam_heads;
-        diff_bwd_params_kernel<<<np, 256, 0, ctx->stream>>>(g.part, (int)nblk, 256 / p.lpu, lam,
-                                                            g.lam_heads, g.dh, g.h, dlam, dgain);
         RNN_LAUNCHED(ctx);
     }
     switch ((g.dh + 15) / 16) {

@@ -181,14 +181,14 @@ struct Operand {
                 for (int e = 0; e < 8; e++) x[SET][i][e] *= x2[SET][i][e];
         }
     }
-    // !KC: the wave's largest magnitude of a set.
+    // !KC: the wave's largest magnitude of a set past what up is good for.
     template <int SET>
     __device__ __forceinline__ float largest() {
         multiply<SET>();
         float m = 0.f;
 #pragma unroll
         for (int i = 0; i < CH; i++) m = absmax8(x[SET][i], m);
-        return wave_max(m);
+        return wave_over(m, good_for(up[0]));
     }
     // A set into the tile at t, the powers of two into ups; whether one changed.
     // largest: !KC, the tile's largest magnitude.
@@ -213,7 +213,7 @@ struct Operand {
                 up[i] = u;
                 if (KC ? sc == 0 : threadIdx.x == 0) ups[KC ? r : 0] = u;
             }
-            _Float16 *d = t + r * STRIDE + (KC ? 8 * slot(r, sc / 8) : sc);
+            _Float16 *d = t + (KC ? r : row_pos(r)) * STRIDE + (KC ? 8 * slot(r, sc / 8) : sc);
             const Half2 h = half_split(x[SET][i], KC ? up[i] : up[0]);
             *(h8 *)d = h.hi;
             *(h8 *)(d + PART) = h.lo;
@@ -228,11 +228,11 @@ struct Operand {
             return *(const h8 *)(t + r * STRIDE + 8 * slot(r, 2 * ks + (l >> 5)));
         } else {
             typedef __attribute__((address_space(3))) g4 *lds_g4;
-            const _Float16 *q = t + (16 * ks + 8 * (l >> 5) + ((l & 15) >> 2)) * STRIDE + r0 +
+            const _Float16 *q = t + (16 * ks + 2 * (l >> 5) + (l & 12)) * STRIDE + r0 +
                                 16 * ((l >> 4) & 1) + 4 * (l & 3);
             const h4 a = __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_g4)q));
             const h4 b = __builtin_bit_cast(
-                h4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_g4)(q + 4 * STRIDE)));
+                h4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_g4)(q + STRIDE)));
             return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
         }
     }

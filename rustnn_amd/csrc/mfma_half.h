@@ -103,10 +103,18 @@ __device__ __forceinline__ f32x16 mm(h8 a, h8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
+// Where row r of a tile is kept: the rows of a block of 16 as the transpose of a
+// 4 x 4.  Rows are an odd number of 16-byte slots long, so that 16 of them at one
+// slot are on distinct banks, and four consecutive ones, 4 positions apart, on
+// distinct quarters of them, of which a transposing read takes 64 bytes a row (in
+// order, conflicts were 58% of the LDS's busy cycles of differential attention's
+// forward).
+__device__ __forceinline__ constexpr int row_pos(int r) {
+    return (r & ~15) | (r & 3) << 2 | (r >> 2 & 3);
+}
+
 // A tile of ROWS rows of W channels in LDS, both parts: row r's hi at
-// r * STRIDE, its lo PART further on.  The 16 bytes of padding put the b128
-// reads of 8 consecutive rows on distinct banks (an odd number of 16-byte
-// slots a row).
+// row_pos(r) * STRIDE, its lo PART further on.
 template <int ROWS, int W>
 struct HalfTile {
     static constexpr int STRIDE = W + 8;  // in halves
@@ -114,7 +122,7 @@ struct HalfTile {
     static constexpr int HALVES = 2 * PART;
     // 8 consecutive channels of a row: an operand with its k along channels
     static __device__ __forceinline__ h8 along(const _Float16 *t, int row, int c) {
-        return *(const h8 *)(t + row * STRIDE + c);
+        return *(const h8 *)(t + row_pos(row) * STRIDE + c);
     }
     // Rows row0 + {0..3, 8..11} (row0 + 4 for the upper half wave) of channel
     // c0 + lane % 32: an operand with its k along rows, in the order in which
@@ -123,12 +131,12 @@ struct HalfTile {
     // the LDS hands back transposed.
     static __device__ __forceinline__ h8 across(const _Float16 *t, int row0, int c0) {
         const int l = threadIdx.x & 63;
-        const _Float16 *p = t + (row0 + 4 * (l >> 5) + ((l & 15) >> 2)) * STRIDE + c0 +
+        const _Float16 *p = t + (row0 + (l >> 5) + (l & 12)) * STRIDE + c0 +
                             16 * ((l >> 4) & 1) + 4 * (l & 3);
         typedef __attribute__((address_space(3))) g4 *lds_g4;
         const h4 a = __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_g4)p));
         const h4 b = __builtin_bit_cast(
-            h4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_g4)(p + 8 * STRIDE)));
+            h4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_g4)(p + 2 * STRIDE)));
         return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     }
 };
@@ -207,6 +215,14 @@ __device__ __forceinline__ float absmax8(const float (&x)[8], float m) {
     for (int e = 0; e < 8; e += 2) m = max3abs(m, x[e], x[e + 1]);
     return m;
 }
+
+// The wave's largest magnitude where it passes what its power of two is good for,
+// else 0: the reduction is rarely taken.
+__device__ __forceinline__ float wave_over(float m, float good) {
+    return __any(m > good) ? wave_max(m) : 0.f;
+}
+// What sticky_up's power is good for.
+__device__ __forceinline__ float good_for(float up) { return 0x1p15f * down_of(up); }
 
 // How NT threads stage a tile of ROWS rows of W channels: RPP rows a pass, 8
 // channels a thread, so that a thread keeps its channels from pass to pass
