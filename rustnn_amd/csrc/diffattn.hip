@@ -191,8 +191,9 @@ struct KvStage {
         const f2 m = {wave_over(a, kgood), wave_over(b, vgood)};
         if ((threadIdx.x & 63) == 0) mx[wave_index()] = m;
     }
-    // K's tile at lds, V's behind it.
-    __device__ __forceinline__ void store(_Float16 *lds, float kup, float vup) const {
+    // K's tile at lds, V's `behind` halves further on.
+    __device__ __forceinline__ void store(_Float16 *lds, float kup, float vup,
+                                          int behind = Tile::HALVES) const {
         if (!stager()) return;
 #pragma unroll
         for (int i = 0; i < CH; i++) {
@@ -200,8 +201,8 @@ struct KvStage {
             const Half2 hk = half_split(xk[i], kup), hv = half_split(xv[i], vup);
             *(h8 *)d = hk.hi;
             *(h8 *)(d + Tile::PART) = hk.lo;
-            *(h8 *)(d + Tile::HALVES) = hv.hi;
-            *(h8 *)(d + Tile::HALVES + Tile::PART) = hv.lo;
+            *(h8 *)(d + behind) = hv.hi;
+            *(h8 *)(d + behind + Tile::PART) = hv.lo;
         }
     }
 };
@@ -243,7 +244,7 @@ __device__ __forceinline__ void put_channels(float *dst, int lim, int c0, const 
 // normalised output, maximum and sum left for diff_join_kernel.
 template <int DHP, bool VEC, int QG, bool SPLIT>
 __global__ __launch_bounds__(128 * QG)
-__attribute__((amdgpu_waves_per_eu(QG == 4 || DHP <= 32 ? 2 : 1))) void
+__attribute__((amdgpu_waves_per_eu(QG == 4 || (QG == 2 && DHP <= 32) ? 2 : 1))) void
 diff_fwd_kernel(DiffArgs g) {
     constexpr int W = 2 * DHP, TK = QG < 4 && DHP > 32 ? 32 : 64, NT = 128 * QG, KS = DHP / 16;
     constexpr int CT = DHP / 16, S2 = TK / 32;
@@ -769,7 +770,7 @@ __device__ __forceinline__ int flip_at(int ntile) { return (2 * ntile + 2) / 3; 
 // hardly changes (sticky_up); where it does they are rescaled.  The waves that share
 // rows add theirs at the end.
 template <int DHP, bool VEC, int RG, int KG>
-__global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(DHP <= 32 ? 2 : 1))) void
+__global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(DHP <= 32 && RG > 1 ? 2 : 1))) void
 diff_dq_kernel(DiffArgs g) {
     constexpr int W = 2 * DHP, TK = 32 * KG, NW = RG * KG, NT = 64 * NW, KS = DHP / 16, VS = W / 16;
     constexpr int CT = (DHP + 31) / 32, BR = 32 * RG;
@@ -972,7 +973,7 @@ diff_dq_kernel(DiffArgs g) {
 // of dV^T = dO^T (P_1 - lambda P_2) and of dK_m^T = Q_m^T dS_m, summed over all tiles
 // in the accumulators as in diff_dq_kernel.
 template <int DHP, bool VEC, int KG>
-__global__ __launch_bounds__(128 * KG) __attribute__((amdgpu_waves_per_eu(2))) void
+__global__ __launch_bounds__(128 * KG) __attribute__((amdgpu_waves_per_eu(DHP <= 32 && KG > 1 ? 2 : 1))) void
 diff_dkv_kernel(DiffArgs g) {
     constexpr int W = 2 * DHP, TR = 32, NW = 2 * KG, NT = 64 * NW, KS = DHP / 16;
     constexpr int CT = (DHP + 31) / 32, VT = (DHP / 16 + 1) / 2, BK = 32 * KG;
@@ -1279,6 +1280,244 @@ diff_dkv_kernel(DiffArgs g) {
                               down_of(pup), live, g.acc_kv);
 }
 
+// acc += over 64 rows: columns ca .. ca + 31 of one tile (accumulator rows) times
+// columns cb .. cb + 31 of another (lanes).
+template <class TA, class TB>
+__device__ __forceinline__ void dot_tiles(const _Float16 *ta, int ca, const _Float16 *tb, int cb,
+                                          f32x16 &acc) {
+#pragma unroll
+    for (int s = 0; s < 4; s++) {
+        const h8 ah = TA::across(ta, 16 * s, ca), al = TA::across(ta + TA::PART, 16 * s, ca);
+        const h8 bh = TB::across(tb, 16 * s, cb), bl = TB::across(tb + TB::PART, 16 * s, cb);
+        acc = mm(al, bh, acc);
+        acc = mm(ah, bl, acc);
+        acc = mm(ah, bh, acc);
+    }
+}
+
+// dQ, dK and dV of problems of at most 64 rows and 64 keys, a workgroup of four
+// waves each, so that Q, K, V and dO are read and split once.  Wave (rg, kg) has
+// the scores of 32 rows with 32 keys, both maps, as diff_dq_kernel; P_1 - lambda P_2
+// and dS_m go through LDS where a tile has been read for the last time, row by
+// row, and come back transposed as operands of dV and dK, whose blocks of 32 keys
+// and 32 channels the waves share out.  Memory bounds it: 128 x 4 heads of 64 rows
+// and keys, dh 32, 20.5 us (60 MB; 12 at a copy's rate) where dQ and dK/dV apart took
+// 18.7 + 18.3.
+template <int DHP>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DHP <= 32 ? 2 : 1))) void
+diff_bwd_small_kernel(DiffArgs g) {
+    constexpr int W = 2 * DHP, KS = DHP / 16, VS = W / 16, CT = (DHP + 31) / 32;
+    using Tile = HalfTile<64, W>;
+    using PTile = HalfTile<64, 64>;
+    using Stage = StagePlan<64, W, 256>;
+    constexpr int CH = Stage::PASSES;
+    // (a map's last 32-channel tile may run past the row: into the padding)
+    constexpr int EX = 2 * 2 * CT * 16 * 64 * 2;  // dQ's halves, in halves
+    constexpr int SLOT = std::max({Tile::HALVES + 32, PTile::HALVES, EX});
+    __shared__ __align__(16) _Float16 lds[4][SLOT];  // K, V, Q, dO
+    __shared__ float rec[6][64];  // as in diff_dkv_kernel
+    __shared__ float tmax[4][6];
+    const int np = params_blocks(g);
+    if ((int)blockIdx.x < np) {
+        bwd_params<256>(g, (int)blockIdx.x, (double *)lds);
+        return;
+    }
+    const int lane = threadIdx.x & 63, wave = wave_index(), lr = lane & 31, lh = lane >> 5;
+    const int prob = (int)xcd_order(blockIdx.x - np, gridDim.x - np);
+    const int b = prob / g.hkv, kh = prob % g.hkv;
+    const int nq = len_of(g.qlen, b, g.tq), nk = len_of(g.klen, b, g.tk), shift = nk - nq;
+    const int dw = 2 * g.dh;
+    _Float16 *const kt = lds[0], *const vt = lds[1], *const qt = lds[2], *const dt = lds[3];
+
+    KvStage<DHP, 64, 256, true> st(g, b, kh, nk);
+    st.load(0);
+    const int sc = (int)threadIdx.x % Stage::C8 * 8, sr = (int)threadIdx.x / Stage::C8;
+    const bool stager = st.stager();
+    float xq[CH][8], xd[CH][8];
+    f32x4 r0, r1;
+    {
+        const int run = sc >= DHP ? 1 : 0;
+        const long long img = (long long)b * g.tq;
+        const auto rq = rows_rsrc(g.q + img * g.qstride + 2 * kh * g.group * g.dh, nq, g.qstride,
+                                  2 * g.group * g.dh);
+        const auto rd = rows_rsrc(g.dout + (img * g.h + kh * g.group) * dw, nq,
+                                  (long long)g.h * dw, g.group * dw);
+        const auto rr = rows_rsrc(g.rec + (img * g.h + kh * g.group) * 8, nq, (long long)g.h * 8,
+                                  g.group * 8);
+#pragma unroll
+        for (int i = 0; i < CH; i++) {
+            const int x = sr + i * Stage::RPP, i0 = x / g.group, hd = x - i0 * g.group;
+            load8<true>(rq, (uint32_t)i0 * (uint32_t)g.qstride + 2 * hd * g.dh + run * g.dh + sc - run * DHP,
+                        stager ? g.dh - (sc - run * DHP) : 0, xq[i]);
+            load8<true>(rd, (uint32_t)(i0 * g.h + hd) * dw + sc, stager ? dw - sc : 0, xd[i]);
+        }
+        const int i0 = lane / g.group;
+        const uint32_t at = (uint32_t)(i0 * g.h + lane - i0 * g.group) * 32u;
+        r0 = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rr, at, 0, 0));
+        r1 = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rr, at + 16u, 0, 0));
+    }
+    {
+        float m[6] = {0.f, 0.f, 0.f, 0.f, r1[2], fabsf(r1[3])};
+#pragma unroll
+        for (int i = 0; i < CH; i++) {
+            m[0] = absmax8(st.xk[i], m[0]);
+            m[1] = absmax8(st.xv[i], m[1]);
+            m[2] = absmax8(xq[i], m[2]);
+            m[3] = absmax8(xd[i], m[3]);
+        }
+#pragma unroll
+        for (int i = 0; i < 6; i++) m[i] = wave_max(m[i]);
+        if (lane == 0)
+#pragma unroll
+            for (int i = 0; i < 6; i++) tmax[wave][i] = m[i];
+    }
+    __syncthreads();
+    float mx[6];
+#pragma unroll
+    for (int i = 0; i < 6; i++)
+        mx[i] = max2(max2(tmax[0][i], tmax[1][i]), max2(tmax[2][i], tmax[3][i]));
+    const float kup = up_of(mx[0]), vup = up_of(mx[1]), qup = up_of(mx[2]), dup = up_of(mx[3]);
+    const float pup = p_up(mx[5]), sup = ds_up(mx[4] * (ds_root<W>() * mx[1]), FIRST_UP);
+    st.store(kt, kup, vup, SLOT);
+    if (stager) {
+#pragma unroll
+        for (int i = 0; i < CH; i++) {
+            _Float16 *p = qt + row_pos(sr + i * Stage::RPP) * Tile::STRIDE + sc;
+            const Half2 hq = half_split(xq[i], qup), hd = half_split(xd[i], dup);
+            *(h8 *)p = hq.hi;
+            *(h8 *)(p + Tile::PART) = hq.lo;
+            *(h8 *)(p + SLOT) = hd.hi;
+            *(h8 *)(p + SLOT + Tile::PART) = hd.lo;
+        }
+    }
+    if (wave == 0) {
+        rec[0][lane] = -r0[0];
+        rec[1][lane] = r0[1] * pup;
+        rec[2][lane] = -r0[2];
+        rec[3][lane] = -r0[3] * r1[3] * pup;
+        rec[4][lane] = -r1[0] * sup;
+        rec[5][lane] = -r1[1] * sup;
+    }
+    __syncthreads();
+
+    const int rg = wave & 1, kg = wave >> 1, row = 32 * rg + lr;
+    const int qi = row / g.group, head = kh * g.group + row % g.group;
+    const _Float16 *const k1 = kt + 32 * kg * Tile::STRIDE;
+    Half2 ah[2], ds[2][2];
+    {
+        f32x16 s[2], da;
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[0][r] = s[1][r] = da[r] = 0.f;
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+            Half2 q[KS];
+#pragma unroll
+            for (int i = 0; i < KS; i++) {
+                q[i].hi = Tile::along(qt, row, m * DHP + 16 * i + 8 * lh);
+                q[i].lo = Tile::along(qt + Tile::PART, row, m * DHP + 16 * i + 8 * lh);
+            }
+            dot_along<Tile>(k1, m * DHP, q, s[m]);
+        }
+        Half2 d[VS];
+#pragma unroll
+        for (int i = 0; i < VS; i++) {
+            d[i].hi = Tile::along(dt, row, 16 * i + 8 * lh);
+            d[i].lo = Tile::along(dt + Tile::PART, row, 16 * i + 8 * lh);
+        }
+        dot_along<Tile>(vt + 32 * kg * Tile::STRIDE, 0, d, da);
+        const float f = down_of(kup) * (down_of(qup) * (g.scale * LOG2E));
+        const float fd = down_of(vup) * down_of(dup) * sup;
+        const float nm1 = rec[0][row], il1 = rec[1][row], nm2 = rec[2][row], il2 = rec[3][row];
+        const float D1 = rec[4][row], D2 = rec[5][row];
+        f32x16 a;
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            const int j = 32 * kg + 8 * (r >> 2) + 4 * lh + (r & 3);
+            const bool in = j < nk && !(g.causal && j > qi + shift) && !(g.diag && j == qi);
+            const float p1 = in ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], f, nm1)) * il1 : 0.f;
+            const float p2 = in ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[1][r], f, nm2)) * il2 : 0.f;
+            a[r] = p1 + p2;
+            s[0][r] = p1 * __builtin_fmaf(da[r], fd, D1);
+            s[1][r] = p2 * __builtin_fmaf(da[r], fd, D2);
+        }
+        split16(a, ah);
+        split16(s[0], ds[0]);
+        split16(s[1], ds[1]);
+    }
+    // 32 keys of a row, in the order of an accumulator's registers
+    auto put = [&](_Float16 *t, const Half2 (&x)[2]) {
+        _Float16 *p = t + row_pos(row) * PTile::STRIDE + 32 * kg + 4 * lh;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            *(h4 *)(p + 16 * i) = __builtin_shufflevector(x[i].hi, x[i].hi, 0, 1, 2, 3);
+            *(h4 *)(p + 16 * i + 8) = __builtin_shufflevector(x[i].hi, x[i].hi, 4, 5, 6, 7);
+            *(h4 *)(p + PTile::PART + 16 * i) = __builtin_shufflevector(x[i].lo, x[i].lo, 0, 1, 2, 3);
+            *(h4 *)(p + PTile::PART + 16 * i + 8) = __builtin_shufflevector(x[i].lo, x[i].lo, 4, 5, 6, 7);
+        }
+    };
+    auto zero = [](f32x16 &x) {
+#pragma unroll
+        for (int r = 0; r < 16; r++) x[r] = 0.f;
+    };
+    __syncthreads();  // V is read
+    put(vt, ah);
+    f32x16 dq[2][CT];
+#pragma unroll
+    for (int m = 0; m < 2; m++)
+#pragma unroll
+        for (int c = 0; c < CT; c++) {
+            zero(dq[m][c]);
+            dot_across<Tile>(k1, m * DHP + 32 * c, ds[m], dq[m][c]);
+        }
+    __syncthreads();  // K is read, P_1 - lambda P_2 there
+    float *const ex = (float *)kt + rg * 2 * CT * 16 * 64 + lane;
+    auto each = [&](auto &&f) {
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+#pragma unroll
+            for (int c = 0; c < CT; c++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) f(ex[((m * CT + c) * 16 + r) * 64], dq[m][c], r);
+    };
+    if (kg) each([](float &e, f32x16 &v, int r) { e = v[r]; });
+    const int key = 32 * rg + lr;  // of the wave's blocks of dK and dV
+    const bool live = key < nk;
+    float *const kv = g.dkv + ((long long)b * g.tk + min(key, g.tk - 1)) * g.kvstride + 2 * kh * g.dh;
+    for (int c = kg; c < W / 32; c += 2) {
+        f32x16 dv;
+        zero(dv);
+        dot_tiles<Tile, PTile>(dt, 32 * c, vt, 32 * rg, dv);
+        if (key < g.tk)
+            put_channels<true>(kv + g.voff, dw, 32 * c, dv, down_of(dup), down_of(pup), live, g.acc_kv);
+    }
+    __syncthreads();  // dO and P_1 - lambda P_2 are read
+    put(vt, ds[0]);
+    put(dt, ds[1]);
+    const float fs = down_of(sup) * down_of(pup);
+    if (!kg) {
+        each([](float &e, f32x16 &v, int r) { v[r] += e; });
+        if (qi < g.tq) {
+            float *dst = g.dq + ((long long)b * g.tq + qi) * g.qstride + 2 * head * g.dh;
+#pragma unroll
+            for (int m = 0; m < 2; m++)
+#pragma unroll
+                for (int c = 0; c < CT; c++)
+                    put_channels<true>(dst + m * g.dh, g.dh, 32 * c, dq[m][c],
+                                       down_of(kup) * g.scale, fs, qi < nq, g.acc_q);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < CT; c++) {
+        f32x16 dk;
+        zero(dk);
+        dot_tiles<Tile, PTile>(qt, kg * DHP + 32 * c, kg ? dt : vt, 32 * rg, dk);
+        if (key < g.tk)
+            put_channels<true>(kv + g.koff + kg * g.dh, g.dh, 32 * c, dk, down_of(qup) * g.scale, fs,
+                               live, g.acc_kv);
+    }
+}
+
 // The backward's first pass: lanes of a unit and blocks, so that the groups of
 // lanes are a multiple of the heads and take about four units each.
 struct PrePlan {
@@ -1436,11 +1675,15 @@ void launch_fwd(rnn_ctx *ctx, const DiffArgs &g, const FwdPlan &p, bool vec) {
         launch_fwd_qg<DHP, true, 4>(ctx, g, p);
 }
 
+// The blocks for the parameters' gradients, params_blocks on the host.
+size_t params_of(const DiffArgs &g) {
+    return (g.dgain ? rnn_div_up(2 * (size_t)g.dh, 16) : 0) + (size_t)g.lam_heads;
+}
+
 template <int DHP, bool VEC, int RG, int KG>
 void launch_dq(rnn_ctx *ctx, const DiffArgs &g) {
     const size_t R = (size_t)g.tq * g.group;
-    const size_t params = (g.dgain ? rnn_div_up(2 * (size_t)g.dh, 16) : 0) + (size_t)g.lam_heads;
-    const unsigned grid = (unsigned)((size_t)g.n * g.hkv * rnn_div_up(R, 32 * RG) + params);
+    const unsigned grid = (unsigned)((size_t)g.n * g.hkv * rnn_div_up(R, 32 * RG) + params_of(g));
     diff_dq_kernel<DHP, VEC, RG, KG><<<grid, 64 * RG * KG, 0, ctx->stream>>>(g);
 }
 template <int DHP, bool VEC, int KG>
@@ -1457,6 +1700,10 @@ void launch_dkv(rnn_ctx *ctx, const DiffArgs &g) {
 template <int DHP>
 void launch_bwd(rnn_ctx *ctx, const DiffArgs &g, bool vec) {
     const size_t probs = (size_t)g.n * g.hkv, R = (size_t)g.tq * g.group;
+    if (vec && g.tq && R <= 64 && g.tk && g.tk <= 64) {
+        diff_bwd_small_kernel<DHP><<<(unsigned)(probs + params_of(g)), 256, 0, ctx->stream>>>(g);
+        return;
+    }
     if (g.tq) {
         if (!vec)
             launch_dq<DHP, false, 4, 1>(ctx, g);

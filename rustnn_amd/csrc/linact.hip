@@ -247,7 +247,7 @@ struct Operand {
 // C[M x N] over k: a tile of BM x BN a workgroup, KB of k a stage, WM x WN x WK
 // waves (WK shares of a stage's depth, added at the end).  PRO: op(A) = a a2.
 template <int BM, int BN, int KB, int WM, int WN, int WK, bool AK, bool BK, bool PRO, int EPI>
-__global__ __launch_bounds__(64 * WM * WN * WK) __attribute__((amdgpu_waves_per_eu(2))) void
+__global__ __launch_bounds__(64 * WM * WN * WK) __attribute__((amdgpu_waves_per_eu(BM == 32 && BN == 128 ? 1 : 2))) void
 linact_kernel(LinArgs g) {
     constexpr int NW = WM * WN * WK, NT = 64 * NW, MT = BM / 32 / WM, NN = BN / 32 / WN;
     constexpr int KS = KB / 16 / WK;

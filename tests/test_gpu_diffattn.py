@@ -96,6 +96,20 @@ CASES = [
     ("few_queries_long", 1, 4, 4, 32, 1, 3001, True, dict(gap=0)),
     ("few_queries_causal", 2, 4, 1, 48, 4, 900, True, dict(causal=True, klen=[900, 2], gap=2)),
     ("peaked", 2, 2, 2, 32, 64, 200, True, dict(amp=8.0, gap=0)),
+    # one for every way that rows and keys are shared out
+    ("small_shared_48", 3, 6, 2, 48, 21, 60, True, dict(gap=0, causal=True, klen=[60, 7, 0])),
+    ("small_shared_16", 2, 4, 1, 16, 16, 64, True, dict(gap=0, per_head=True)),
+    ("small_64_ragged", 4, 2, 2, 64, 64, 64, False,
+     dict(gap=0, causal=True, diag=True, qlen=[64, 33, 0, 1], klen=[64, 33, 0, 1])),
+    ("small_32_shared", 3, 6, 2, 32, 20, 33, True, dict(gap=0, qlen=[20, 3, 11], gain=False)),
+    ("few_keys_32", 2, 4, 1, 32, 150, 20, True, dict(gap=0, diag=True)),
+    ("few_keys_64", 2, 2, 2, 64, 70, 31, True, dict(gap=0, causal=True)),
+    ("few_rows_16", 2, 2, 2, 16, 9, 333, True, dict(gap=0, klen=[333, 70])),
+    ("rows_64_split", 1, 2, 2, 32, 50, 600, True, dict(gap=0)),
+    ("rows_128_split", 1, 2, 1, 64, 65, 700, True, dict(gap=0, causal=True)),
+    ("group_of_three", 2, 6, 2, 32, 47, 140, True, dict(gap=0, causal=True, per_head=True)),
+    ("many_problems_16", 64, 4, 4, 16, 130, 70, True, dict(gap=0)),
+    ("many_problems_64", 64, 8, 8, 64, 66, 65, True, dict(gap=0, causal=True)),
 ]
 IDS = [c[0] for c in CASES]
 
@@ -129,7 +143,7 @@ def test_eval_gives_the_same_output(rnn, c):
 
 
 @pytest.mark.parametrize("name", ["grid_8x8", "memory_256", "ragged_cross", "ragged_self",
-                                  "dh_64_aligned", "one_query"])
+                                  "dh_64_aligned", "one_query", "small_shared_48", "few_keys_32"])
 def test_gradients_accumulate(rnn, name):
     """Unflagged operands receive old + gradient: one rounding of the sum."""
     cs = case(CASES[IDS.index(name)], seed=2)
@@ -211,7 +225,8 @@ def test_other_stream_and_context(rnn):
     del got
 
 
-@pytest.mark.parametrize("name", ["grid_8x8", "ragged_cross", "few_queries_shared"])
+@pytest.mark.parametrize("name", ["grid_8x8", "ragged_cross", "few_queries_shared",
+                                  "few_keys_32"])
 def test_captured_and_replayed(rnn, name):
     """Two graphs of two calls share nothing but their context: replayed in
     turn, with eager calls between, each gives its eager result."""
