@@ -1295,17 +1295,17 @@ __device__ __forceinline__ void dot_tiles(const _Float16 *ta, int ca, const _Flo
     }
 }
 
-// dQ, dK and dV of problems of at most 64 rows and 64 keys, a workgroup of four
-// waves each, so that Q, K, V and dO are read and split once.  Wave (rg, kg) has
-// the scores of 32 rows with 32 keys, both maps, as diff_dq_kernel; P_1 - lambda P_2
-// and dS_m go through LDS where a tile has been read for the last time, row by
-// row, and come back transposed as operands of dV and dK, whose blocks of 32 keys
-// and 32 channels the waves share out.  Memory bounds it: 128 x 4 heads of 64 rows
-// and keys, dh 32, 20.5 us (60 MB; 12 at a copy's rate) where dQ and dK/dV apart took
-// 18.7 + 18.3.
+// dQ, dK and dV of problems of at most 64 rows, a workgroup of four waves each,
+// over tiles of 64 keys: Q and dO are read and split once, K and V once for all
+// three.  Wave (rg, kg) has the scores of 32 rows with 32 keys, both maps, and sums
+// dQ as diff_dq_kernel does; P_1 - lambda P_2 and dS_m go through LDS where the tile
+// has been read for the last time, row by row, and come back transposed as
+// operands of dV and dK, whose blocks of 32 keys and 32 channels the waves share
+// out.  Memory bounds it: 128 x 4 heads of 64 rows and keys, dh 32, 20.5 us (60 MB;
+// 12 at a copy's rate) where dQ and dK/dV apart took 18.7 + 18.3.
 template <int DHP>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DHP <= 32 ? 2 : 1))) void
-diff_bwd_small_kernel(DiffArgs g) {
+diff_bwd_rows_kernel(DiffArgs g) {
     constexpr int W = 2 * DHP, KS = DHP / 16, VS = W / 16, CT = (DHP + 31) / 32;
     using Tile = HalfTile<64, W>;
     using PTile = HalfTile<64, 64>;
@@ -1316,7 +1316,8 @@ diff_bwd_small_kernel(DiffArgs g) {
     constexpr int SLOT = std::max({Tile::HALVES + 32, PTile::HALVES, EX});
     __shared__ __align__(16) _Float16 lds[4][SLOT];  // K, V, Q, dO
     __shared__ float rec[6][64];  // as in diff_dkv_kernel
-    __shared__ float tmax[4][6];
+    __shared__ f4 rmax[4];
+    __shared__ f2 tmax[4];
     const int np = params_blocks(g);
     if ((int)blockIdx.x < np) {
         bwd_params<256>(g, (int)blockIdx.x, (double *)lds);
@@ -1357,28 +1358,23 @@ diff_bwd_small_kernel(DiffArgs g) {
         r1 = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rr, at + 16u, 0, 0));
     }
     {
-        float m[6] = {0.f, 0.f, 0.f, 0.f, r1[2], fabsf(r1[3])};
+        f4 m = {0.f, 0.f, r1[2], fabsf(r1[3])};
 #pragma unroll
         for (int i = 0; i < CH; i++) {
-            m[0] = absmax8(st.xk[i], m[0]);
-            m[1] = absmax8(st.xv[i], m[1]);
-            m[2] = absmax8(xq[i], m[2]);
-            m[3] = absmax8(xd[i], m[3]);
+            m[0] = absmax8(xq[i], m[0]);
+            m[1] = absmax8(xd[i], m[1]);
         }
 #pragma unroll
-        for (int i = 0; i < 6; i++) m[i] = wave_max(m[i]);
-        if (lane == 0)
-#pragma unroll
-            for (int i = 0; i < 6; i++) tmax[wave][i] = m[i];
+        for (int i = 0; i < 4; i++) m[i] = wave_max(m[i]);
+        if (lane == 0) rmax[wave] = m;
     }
     __syncthreads();
-    float mx[6];
+    f4 mx = rmax[0];
 #pragma unroll
-    for (int i = 0; i < 6; i++)
-        mx[i] = max2(max2(tmax[0][i], tmax[1][i]), max2(tmax[2][i], tmax[3][i]));
-    const float kup = up_of(mx[0]), vup = up_of(mx[1]), qup = up_of(mx[2]), dup = up_of(mx[3]);
-    const float pup = p_up(mx[5]), sup = ds_up(mx[4] * (ds_root<W>() * mx[1]), FIRST_UP);
-    st.store(kt, kup, vup, SLOT);
+    for (int i = 1; i < 4; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) mx[e] = max2(mx[e], rmax[i][e]);
+    const float qup = up_of(mx[0]), dup = up_of(mx[1]), pup = p_up(mx[3]);
     if (stager) {
 #pragma unroll
         for (int i = 0; i < CH; i++) {
@@ -1395,56 +1391,12 @@ diff_bwd_small_kernel(DiffArgs g) {
         rec[1][lane] = r0[1] * pup;
         rec[2][lane] = -r0[2];
         rec[3][lane] = -r0[3] * r1[3] * pup;
-        rec[4][lane] = -r1[0] * sup;
-        rec[5][lane] = -r1[1] * sup;
+        rec[4][lane] = -r1[0];
+        rec[5][lane] = -r1[1];
     }
-    __syncthreads();
-
     const int rg = wave & 1, kg = wave >> 1, row = 32 * rg + lr;
     const int qi = row / g.group, head = kh * g.group + row % g.group;
-    const _Float16 *const k1 = kt + 32 * kg * Tile::STRIDE;
-    Half2 ah[2], ds[2][2];
-    {
-        f32x16 s[2], da;
-#pragma unroll
-        for (int r = 0; r < 16; r++) s[0][r] = s[1][r] = da[r] = 0.f;
-#pragma unroll
-        for (int m = 0; m < 2; m++) {
-            Half2 q[KS];
-#pragma unroll
-            for (int i = 0; i < KS; i++) {
-                q[i].hi = Tile::along(qt, row, m * DHP + 16 * i + 8 * lh);
-                q[i].lo = Tile::along(qt + Tile::PART, row, m * DHP + 16 * i + 8 * lh);
-            }
-            dot_along<Tile>(k1, m * DHP, q, s[m]);
-        }
-        Half2 d[VS];
-#pragma unroll
-        for (int i = 0; i < VS; i++) {
-            d[i].hi = Tile::along(dt, row, 16 * i + 8 * lh);
-            d[i].lo = Tile::along(dt + Tile::PART, row, 16 * i + 8 * lh);
-        }
-        dot_along<Tile>(vt + 32 * kg * Tile::STRIDE, 0, d, da);
-        const float f = down_of(kup) * (down_of(qup) * (g.scale * LOG2E));
-        const float fd = down_of(vup) * down_of(dup) * sup;
-        const float nm1 = rec[0][row], il1 = rec[1][row], nm2 = rec[2][row], il2 = rec[3][row];
-        const float D1 = rec[4][row], D2 = rec[5][row];
-        f32x16 a;
-#pragma unroll
-        for (int r = 0; r < 16; r++) {
-            const int j = 32 * kg + 8 * (r >> 2) + 4 * lh + (r & 3);
-            const bool in = j < nk && !(g.causal && j > qi + shift) && !(g.diag && j == qi);
-            const float p1 = in ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], f, nm1)) * il1 : 0.f;
-            const float p2 = in ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[1][r], f, nm2)) * il2 : 0.f;
-            a[r] = p1 + p2;
-            s[0][r] = p1 * __builtin_fmaf(da[r], fd, D1);
-            s[1][r] = p2 * __builtin_fmaf(da[r], fd, D2);
-        }
-        split16(a, ah);
-        split16(s[0], ds[0]);
-        split16(s[1], ds[1]);
-    }
-    // 32 keys of a row, in the order of an accumulator's registers
+    // 32 keys of the wave's row, in the order of an accumulator's registers
     auto put = [&](_Float16 *t, const Half2 (&x)[2]) {
         _Float16 *p = t + row_pos(row) * PTile::STRIDE + 32 * kg + 4 * lh;
 #pragma unroll
@@ -1459,17 +1411,132 @@ diff_bwd_small_kernel(DiffArgs g) {
 #pragma unroll
         for (int r = 0; r < 16; r++) x[r] = 0.f;
     };
-    __syncthreads();  // V is read
-    put(vt, ah);
     f32x16 dq[2][CT];
 #pragma unroll
     for (int m = 0; m < 2; m++)
 #pragma unroll
-        for (int c = 0; c < CT; c++) {
-            zero(dq[m][c]);
-            dot_across<Tile>(k1, m * DHP + 32 * c, ds[m], dq[m][c]);
+        for (int c = 0; c < CT; c++) zero(dq[m][c]);
+    // keys that some row sees; the others' gradients are zeros
+    const int kend = g.causal ? min(nk, nq + shift) : nq ? nk : 0;
+    const int nt = (g.tk + 63) / 64, flip = flip_at((max(kend, 0) + 63) / 64);
+    // the largest value so far and powers of two, sgn: the accumulators' sign
+    float vmax = 0.f, kup = FIRST_UP, sup = FIRST_UP, sgn = 1.f;
+    for (int t = 0; t < nt; t++) {
+        const int k0 = 64 * t, key = k0 + 32 * rg + lr;  // of the wave's blocks of dK and dV
+        const bool live = key < nk;
+        float *const kv = g.dkv + ((long long)b * g.tk + min(key, g.tk - 1)) * g.kvstride + 2 * kh * g.dh;
+        if (k0 >= kend) {  // (the accumulators are left as they are)
+            f32x16 z;
+            zero(z);
+            for (int c = kg; c < W / 32 && key < g.tk; c += 2)
+                put_channels<true>(kv + g.voff, dw, 32 * c, z, 0.f, 0.f, live, g.acc_kv);
+            for (int c = 0; c < CT && key < g.tk; c++)
+                put_channels<true>(kv + g.koff + kg * g.dh, g.dh, 32 * c, z, 0.f, 0.f, live, g.acc_kv);
+            continue;
         }
-    __syncthreads();  // K is read, P_1 - lambda P_2 there
+        st.maxima(tmax, good_for(kup), vmax);
+        __syncthreads();  // dS is read
+        float mk = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            mk = max2(mk, tmax[i][0]);
+            vmax = max2(vmax, tmax[i][1]);
+        }
+        const float kup1 = sticky_up(mk, kup), vup = up_of(vmax);
+        const float sup1 = ds_up(mx[2] * (ds_root<W>() * vmax), sup);
+        float ratio = down_of(kup) * kup1 * (down_of(sup) * sup1);
+        kup = kup1;
+        sup = sup1;
+        if (t == flip) {
+            sgn = -1.f;
+            ratio = -ratio;
+        }
+        if (t && ratio != 1.0f) {
+#pragma unroll
+            for (int m = 0; m < 2; m++)
+#pragma unroll
+                for (int c = 0; c < CT; c++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) dq[m][c][r] *= ratio;
+        }
+        st.store(kt, kup, vup, SLOT);
+        if (k0 + 64 < kend) st.load(k0 + 64);
+        __syncthreads();
+        const _Float16 *const k1 = kt + 32 * kg * Tile::STRIDE;
+        Half2 ah[2], ds[2][2];
+        {
+            f32x16 s[2], da;
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[0][r] = s[1][r] = da[r] = 0.f;
+#pragma unroll
+            for (int m = 0; m < 2; m++) {
+                Half2 q[KS];
+#pragma unroll
+                for (int i = 0; i < KS; i++) {
+                    q[i].hi = Tile::along(qt, row, m * DHP + 16 * i + 8 * lh);
+                    q[i].lo = Tile::along(qt + Tile::PART, row, m * DHP + 16 * i + 8 * lh);
+                }
+                dot_along<Tile>(k1, m * DHP, q, s[m]);
+            }
+            Half2 d[VS];
+#pragma unroll
+            for (int i = 0; i < VS; i++) {
+                d[i].hi = Tile::along(dt, row, 16 * i + 8 * lh);
+                d[i].lo = Tile::along(dt + Tile::PART, row, 16 * i + 8 * lh);
+            }
+            dot_along<Tile>(vt + 32 * kg * Tile::STRIDE, 0, d, da);
+            const float f = down_of(kup) * (down_of(qup) * (g.scale * LOG2E));
+            const float fd = down_of(vup) * down_of(dup) * sup;
+            const float nm1 = rec[0][row], il1 = rec[1][row] * sgn, nm2 = rec[2][row], il2 = rec[3][row] * sgn;
+            const float D1 = rec[4][row] * sup, D2 = rec[5][row] * sup;
+            f32x16 a;
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const int j = k0 + 32 * kg + 8 * (r >> 2) + 4 * lh + (r & 3);
+                const bool in = j < nk && !(g.causal && j > qi + shift) && !(g.diag && j == qi);
+                const float p1 = in ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], f, nm1)) * il1 : 0.f;
+                const float p2 = in ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[1][r], f, nm2)) * il2 : 0.f;
+                a[r] = p1 + p2;
+                s[0][r] = p1 * __builtin_fmaf(da[r], fd, D1);
+                s[1][r] = p2 * __builtin_fmaf(da[r], fd, D2);
+            }
+            split16(a, ah);
+            split16(s[0], ds[0]);
+            split16(s[1], ds[1]);
+        }
+        __syncthreads();  // V is read
+        put(vt, ah);
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+#pragma unroll
+            for (int c = 0; c < CT; c++)
+                dot_across<Tile>(k1, m * DHP + 32 * c, ds[m], dq[m][c]);
+        __syncthreads();  // K is read, P_1 - lambda P_2 there
+        put(kt, ds[1]);
+        for (int c = kg; c < W / 32; c += 2) {
+            f32x16 dv;
+            zero(dv);
+            dot_tiles<Tile, PTile>(dt, 32 * c, vt, 32 * rg, dv);
+            if (key < g.tk)
+                put_channels<true>(kv + g.voff, dw, 32 * c, dv, down_of(dup) * sgn, down_of(pup),
+                                   live, g.acc_kv);
+        }
+        __syncthreads();  // P_1 - lambda P_2 is read
+        put(vt, ds[0]);
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < CT; c++) {
+            f32x16 dk;
+            zero(dk);
+            dot_tiles<Tile, PTile>(qt, kg * DHP + 32 * c, kg ? kt : vt, 32 * rg, dk);
+            if (key < g.tk)
+                put_channels<true>(kv + g.koff + kg * g.dh, g.dh, 32 * c, dk,
+                                   down_of(qup) * (g.scale * sgn), down_of(sup) * down_of(pup), live,
+                                   g.acc_kv);
+        }
+    }
+    // the halves of dQ that waves (rg, 0) and (rg, 1) have
+    __syncthreads();
     float *const ex = (float *)kt + rg * 2 * CT * 16 * 64 + lane;
     auto each = [&](auto &&f) {
 #pragma unroll
@@ -1480,42 +1547,16 @@ diff_bwd_small_kernel(DiffArgs g) {
                 for (int r = 0; r < 16; r++) f(ex[((m * CT + c) * 16 + r) * 64], dq[m][c], r);
     };
     if (kg) each([](float &e, f32x16 &v, int r) { e = v[r]; });
-    const int key = 32 * rg + lr;  // of the wave's blocks of dK and dV
-    const bool live = key < nk;
-    float *const kv = g.dkv + ((long long)b * g.tk + min(key, g.tk - 1)) * g.kvstride + 2 * kh * g.dh;
-    for (int c = kg; c < W / 32; c += 2) {
-        f32x16 dv;
-        zero(dv);
-        dot_tiles<Tile, PTile>(dt, 32 * c, vt, 32 * rg, dv);
-        if (key < g.tk)
-            put_channels<true>(kv + g.voff, dw, 32 * c, dv, down_of(dup), down_of(pup), live, g.acc_kv);
-    }
-    __syncthreads();  // dO and P_1 - lambda P_2 are read
-    put(vt, ds[0]);
-    put(dt, ds[1]);
-    const float fs = down_of(sup) * down_of(pup);
-    if (!kg) {
-        each([](float &e, f32x16 &v, int r) { v[r] += e; });
-        if (qi < g.tq) {
-            float *dst = g.dq + ((long long)b * g.tq + qi) * g.qstride + 2 * head * g.dh;
-#pragma unroll
-            for (int m = 0; m < 2; m++)
-#pragma unroll
-                for (int c = 0; c < CT; c++)
-                    put_channels<true>(dst + m * g.dh, g.dh, 32 * c, dq[m][c],
-                                       down_of(kup) * g.scale, fs, qi < nq, g.acc_q);
-        }
-    }
     __syncthreads();
+    if (kg || qi >= g.tq) return;
+    each([](float &e, f32x16 &v, int r) { v[r] += e; });
+    float *dst = g.dq + ((long long)b * g.tq + qi) * g.qstride + 2 * head * g.dh;
 #pragma unroll
-    for (int c = 0; c < CT; c++) {
-        f32x16 dk;
-        zero(dk);
-        dot_tiles<Tile, PTile>(qt, kg * DHP + 32 * c, kg ? dt : vt, 32 * rg, dk);
-        if (key < g.tk)
-            put_channels<true>(kv + g.koff + kg * g.dh, g.dh, 32 * c, dk, down_of(qup) * g.scale, fs,
-                               live, g.acc_kv);
-    }
+    for (int m = 0; m < 2; m++)
+#pragma unroll
+        for (int c = 0; c < CT; c++)
+            put_channels<true>(dst + m * g.dh, g.dh, 32 * c, dq[m][c], down_of(kup) * (g.scale * sgn),
+                               down_of(sup) * down_of(pup), qi < nq, g.acc_q);
 }
 
 // The backward's first pass: lanes of a unit and blocks, so that the groups of
@@ -1700,8 +1741,8 @@ void launch_dkv(rnn_ctx *ctx, const DiffArgs &g) {
 template <int DHP>
 void launch_bwd(rnn_ctx *ctx, const DiffArgs &g, bool vec) {
     const size_t probs = (size_t)g.n * g.hkv, R = (size_t)g.tq * g.group;
-    if (vec && g.tq && R <= 64 && g.tk && g.tk <= 64) {
-        diff_bwd_small_kernel<DHP><<<(unsigned)(probs + params_of(g)), 256, 0, ctx->stream>>>(g);
+    if (vec && g.tq && R <= 64 && g.tk && (g.tk <= 64 || probs >= 256)) {
+        diff_bwd_rows_kernel<DHP><<<(unsigned)(probs + params_of(g)), 256, 0, ctx->stream>>>(g);
         return;
     }
     if (g.tq) {

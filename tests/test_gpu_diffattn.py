@@ -108,6 +108,10 @@ CASES = [
     ("rows_64_split", 1, 2, 2, 32, 50, 600, True, dict(gap=0)),
     ("rows_128_split", 1, 2, 1, 64, 65, 700, True, dict(gap=0, causal=True)),
     ("group_of_three", 2, 6, 2, 32, 47, 140, True, dict(gap=0, causal=True, per_head=True)),
+    ("many_few_rows_32", 64, 4, 4, 32, 20, 150, True, dict(gap=0, causal=True, diag=True)),
+    ("many_few_rows_64", 128, 4, 2, 64, 9, 201, True,
+     dict(gap=0, klen=[37 * i % 202 for i in range(128)])),
+    ("many_few_rows_48", 128, 4, 2, 48, 32, 66, True, dict(gap=0, per_head=True)),
     ("many_problems_16", 64, 4, 4, 16, 130, 70, True, dict(gap=0)),
     ("many_problems_64", 64, 8, 8, 64, 66, 65, True, dict(gap=0, causal=True)),
 ]
