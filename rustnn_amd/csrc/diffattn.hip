@@ -180,7 +180,8 @@ struct KvStage {
             load8<VEC>(rv, voff + i * step, vlim, xv[i]);
         }
     }
-    // Largest magnitudes past what the powers of two are good for, each wave's.
+    // Each wave's largest magnitudes, where one passes what its power of two is good
+    // for (else 0: the reductions are rarely taken).
     __device__ __forceinline__ void maxima(f2 *mx, float kgood, float vgood) const {
         float a = 0.f, b = 0.f;
 #pragma unroll
@@ -188,7 +189,8 @@ struct KvStage {
             a = absmax8(xk[i], a);
             b = absmax8(xv[i], b);
         }
-        const f2 m = {wave_over(a, kgood), wave_over(b, vgood)};
+        f2 m = {0.f, 0.f};
+        if (__any(a > kgood || b > vgood)) m = f2{wave_max(a), wave_max(b)};
         if ((threadIdx.x & 63) == 0) mx[wave_index()] = m;
     }
     // K's tile at lds, V's `behind` halves further on.
@@ -239,21 +241,22 @@ __device__ __forceinline__ void put_channels(float *dst, int lim, int c0, const 
 // in two lanes, and the exponentials are, register by register, the operand of
 // O^T = V^T P^T.  Tiles of 64 keys and values are split into LDS once for all
 // waves, in two buffers: while one is read the next is written, and the loads of
-// the one after it are in flight.
+// the one after it are in flight.  KH: two waves take half of each tile's keys and
+// join their sums at the end (wave 2 (QG h + i) + m).
 // SPLIT: the keys [z TS, (z + 1) TS) alone (z = blockIdx.y), each map's own
 // normalised output, maximum and sum left for diff_join_kernel.
-template <int DHP, bool VEC, int QG, bool SPLIT>
-__global__ __launch_bounds__(128 * QG)
-__attribute__((amdgpu_waves_per_eu(QG == 4 || (QG == 2 && DHP <= 32) ? 2 : 1))) void
+template <int DHP, bool VEC, int QG, int KH, bool SPLIT>
+__global__ __launch_bounds__(128 * QG * KH)
+__attribute__((amdgpu_waves_per_eu(QG * KH == 4 || (QG == 2 && DHP <= 32) ? 2 : 1))) void
 diff_fwd_kernel(DiffArgs g) {
-    constexpr int W = 2 * DHP, TK = QG < 4 && DHP > 32 ? 32 : 64, NT = 128 * QG, KS = DHP / 16;
-    constexpr int CT = DHP / 16, S2 = TK / 32;
+    constexpr int W = 2 * DHP, TK = QG * KH < 4 && DHP > 32 ? 32 : 64, NT = 128 * QG * KH, KS = DHP / 16;
+    constexpr int CT = DHP / 16, S2 = TK / 32 / KH, HALF = (CT * 16 + 2) * 64;
     using Tile = HalfTile<TK, W>;
-    static_assert((int)sizeof(_Float16) * 4 * Tile::HALVES >= QG * CT * 16 * 64 * 4, "exchange");
+    static_assert(8 * Tile::HALVES >= 4 * ((KH - 1) * 2 * QG * HALF + QG * CT * 16 * 64) && (KH == 1 || !SPLIT), "exchange");
     __shared__ __align__(16) _Float16 lds[2][2 * Tile::HALVES];
-    __shared__ f2 tmax[2][2 * QG];
+    __shared__ f2 tmax[2][2 * QG * KH];
     const int lane = threadIdx.x & 63, wave = wave_index(), lr = lane & 31, lh = lane >> 5;
-    const int map = wave & 1, qg = wave >> 1;
+    const int map = wave & 1, qg = (wave >> 1) % QG, half = (wave >> 1) / QG;
     const int R = g.tq * g.group, nrb = (R + 32 * QG - 1) / (32 * QG);
     const long long id = xcd_order(blockIdx.x, gridDim.x);
     const int prob = (int)(id / nrb), rb = nrb - 1 - (int)(id % nrb);  // causal: longest first
@@ -297,7 +300,7 @@ diff_fwd_kernel(DiffArgs g) {
     auto stage = [&](int t) {
         float mv = 0.f;
 #pragma unroll
-        for (int i = 0; i < 2 * QG; i++) {
+        for (int i = 0; i < 2 * QG * KH; i++) {
             const f2 m = tmax[t & 1][i];
             kmax = max2(kmax, m[0]);
             mv = max2(mv, m[1]);
@@ -316,9 +319,9 @@ diff_fwd_kernel(DiffArgs g) {
         }
     }
     for (int t = 0; t < ntile; t++) {
-        const int k0 = kbeg + t * TK;
+        const int k0 = kbeg + t * TK, k1 = k0 + 32 * S2 * half;
         __syncthreads();
-        const _Float16 *const kt = lds[t & 1], *const vt = kt + Tile::HALVES;
+        const _Float16 *const kt = lds[t & 1] + 32 * S2 * half * Tile::STRIDE, *const vt = kt + Tile::HALVES;
         const float f = down_of(kup1) * qdown, turn = down_of(vup) * vup1;
         vup = vup1;
         if (t + 1 < ntile) stage(t + 1);
@@ -330,14 +333,14 @@ diff_fwd_kernel(DiffArgs g) {
             for (int r = 0; r < 16; r++) u[s2][r] = 0.f;
             dot_along<Tile>(kt + 32 * s2 * Tile::STRIDE, map * DHP, q, u[s2]);
         }
-        const bool whole = k0 + TK <= nk && !(g.causal && k0 + TK - 1 > w_first + shift) &&
-                           !(g.diag && k0 <= w_last && w_first < k0 + TK);
+        const bool whole = k1 + 32 * S2 <= nk && !(g.causal && k1 + 32 * S2 - 1 > w_first + shift) &&
+                           !(g.diag && k1 <= w_last && w_first < k1 + 32 * S2);
         if (!whole) {
 #pragma unroll
             for (int s2 = 0; s2 < S2; s2++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
-                    const int j = k0 + 32 * s2 + 8 * (r >> 2) + 4 * lh + (r & 3);
+                    const int j = k1 + 32 * s2 + 8 * (r >> 2) + 4 * lh + (r & 3);
                     const bool in = j < nk && !(g.causal && j > qi + shift) && !(g.diag && j == qi);
                     u[s2][r] = in ? u[s2][r] : -INFINITY;
                 }
@@ -379,6 +382,31 @@ diff_fwd_kernel(DiffArgs g) {
         if (t + 2 < ntile) maxima(t & 1);
     }
     l = pair32(l, add2);
+    if constexpr (KH > 1) {  // the second half's sums to the first
+        static_assert(KH == 2);
+        __syncthreads();
+        float *const e = (float *)lds[0] + (2 * qg + map) * HALF + lane;
+        if (half) {
+#pragma unroll
+            for (int c = 0; c < CT; c++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) e[(c * 16 + r) * 64] = o[c][r];
+            e[CT * 16 * 64] = m;
+            e[CT * 16 * 64 + 64] = l;
+        }
+        __syncthreads();
+        if (!half) {
+            const float m2 = e[CT * 16 * 64], top = max2(m, m2);
+            const float x = __builtin_amdgcn_exp2f(m - top), y = __builtin_amdgcn_exp2f(m2 - top);
+            l = l * x + e[CT * 16 * 64 + 64] * y;
+            m = top;
+#pragma unroll
+            for (int c = 0; c < CT; c++)
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    o[c][r] = __builtin_fmaf(o[c][r], x, e[(c * 16 + r) * 64] * y);
+        }
+    }
     const bool some = live && l > 0.f;
     const float il = some ? down_of(vup) / l : 0.f;  // both carry 2^6
 #pragma unroll
@@ -404,15 +432,15 @@ diff_fwd_kernel(DiffArgs g) {
         return;
     }
     // map 1's output to its partner wave
-    __syncthreads();
-    float *ex = (float *)lds[0] + qg * CT * 16 * 64;
-    if (map == 1) {
+    if (KH == 1) __syncthreads();
+    float *ex = (float *)lds[0] + (KH - 1) * 2 * QG * HALF + qg * CT * 16 * 64;
+    if (map == 1 && !half) {
 #pragma unroll
         for (int c = 0; c < CT; c++)
 #pragma unroll
             for (int r = 0; r < 16; r++) ex[(c * 16 + r) * 64 + lane] = o[c][r];
     }
-    if (g.stats && row < R && lh == 0)
+    if (g.stats && row < R && lh == 0 && !half)
         *(f2 *)(g.stats + out * 4 + 2 * map) = f2{m, some ? P_UP / l : 0.f};
     __syncthreads();
     const bool vst = VEC;  // whole float4s: dv % 4 == 0, aligned rows
@@ -433,7 +461,7 @@ diff_fwd_kernel(DiffArgs g) {
                 }
             }
     };
-    if (row >= R) return;
+    if (row >= R || half) return;
     if (g.o12)
         store(g.o12 + (out * 2 + map) * dv, [&](int c, int r, int) { return o[c][r]; });
     if (map == 1) return;
@@ -763,16 +791,18 @@ __device__ __forceinline__ float p_up(float lam) { return up_of(fmaxf(1.0f, lam)
 // change sign, and the operand from registers with them.
 __device__ __forceinline__ int flip_at(int ntile) { return (2 * ntile + 2) / 3; }
 
-// dQ.  Rows as in the forward, RG groups of 32 a workgroup, a wave on both maps of
-// its rows and on one of the KS 32 keys of a tile; tiles in two LDS buffers: S_m^T = K_m Q_m^T and dA^T = V dO^T (lane = row), and
-// P (dA - D) in registers is the operand of dQ_m^T = K_m^T dS_m^T, which is
-// summed over all tiles in the accumulators.  Their unit is a power of two that
+// dQ.  Rows as in the forward, RG groups of 32 a workgroup, a wave on NM maps of its
+// rows (both, or a pair of waves one each, dA in both) and on one of the KG 32 keys
+// of a tile; tiles in two LDS buffers: S_m^T = K_m Q_m^T and dA^T = V dO^T (lane =
+// row), and P (dA - D) in registers is the operand of dQ_m^T = K_m^T dS_m^T, which
+// is summed over all tiles in the accumulators.  Their unit is a power of two that
 // hardly changes (sticky_up); where it does they are rescaled.  The waves that share
 // rows add theirs at the end.
-template <int DHP, bool VEC, int RG, int KG>
-__global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(DHP <= 32 && RG > 1 ? 2 : 1))) void
+template <int DHP, bool VEC, int RG, int KG, int NM>
+__global__ __launch_bounds__(128 / NM * RG * KG)
+__attribute__((amdgpu_waves_per_eu((DHP <= 32 && RG > 1) || NM == 1 ? 2 : 1))) void
 diff_dq_kernel(DiffArgs g) {
-    constexpr int W = 2 * DHP, TK = 32 * KG, NW = RG * KG, NT = 64 * NW, KS = DHP / 16, VS = W / 16;
+    constexpr int W = 2 * DHP, TK = 32 * KG, NW = 2 / NM * RG * KG, NT = 64 * NW, KS = DHP / 16, VS = W / 16;
     constexpr int CT = (DHP + 31) / 32, BR = 32 * RG;
     using Tile = HalfTile<TK, W>;
     // (a map's last 32-channel tile may run past the row: into the padding)
@@ -780,7 +810,8 @@ diff_dq_kernel(DiffArgs g) {
     static_assert(KG == 1 || sizeof(lds) >= (size_t)(KG - 1) * RG * 2 * CT * 16 * 64 * 4, "exchange");
     __shared__ f2 tmax[2][NW];
     const int lane = threadIdx.x & 63, wave = wave_index(), lr = lane & 31, lh = lane >> 5;
-    const int rg = wave % RG, kg = wave / RG;
+    const int map = NM == 2 ? 0 : wave & 1;  // the first of the wave's
+    const int rg = wave / (2 / NM) % RG, kg = wave / (2 / NM) / RG;
     const int R = g.tq * g.group, nrb = (R + BR - 1) / BR;
     const int np = params_blocks(g);
     if ((int)blockIdx.x < np) {
@@ -816,26 +847,32 @@ diff_dq_kernel(DiffArgs g) {
         sm = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rr, at, 0, 0));
         dd = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rr, at + 16u, 0, 0));
     }
-    Half2 q[2][KS], d[VS];
-    float qdown[2], ddown;
+    Half2 q[NM][KS], d[VS];
+    float qdown[NM], ddown;
     {
-        RowFrag<KS> qf[2];
+        RowFrag<KS> qf[NM];
         RowFrag<VS> df;
 #pragma unroll
-        for (int m = 0; m < 2; m++)
-            qf[m].template load<VEC>(rq, (uint32_t)qx * (uint32_t)g.qstride + (2 * head + m) * g.dh,
+        for (int m = 0; m < NM; m++)
+            qf[m].template load<VEC>(rq, (uint32_t)qx * (uint32_t)g.qstride + (2 * head + map + m) * g.dh,
                                      live ? g.dh : 0);
         df.template load<VEC>(rd, (uint32_t)(qx * g.h + head) * dv, live ? dv : 0);
 #pragma unroll
-        for (int m = 0; m < 2; m++) qdown[m] = qf[m].split(q[m]) * (g.scale * LOG2E);
+        for (int m = 0; m < NM; m++) qdown[m] = qf[m].split(q[m]) * (g.scale * LOG2E);
         ddown = df.split(d);
     }
     const float pup = p_up(fabsf(dd[3]));
-    const float nm[2] = {-sm[0], -sm[2]};
-    float il[2] = {sm[1] * pup, sm[3] * dd[3] * pup};
-    f32x16 acc[2][CT];
+    float nm[NM], il[NM], D[NM];
 #pragma unroll
-    for (int m = 0; m < 2; m++)
+    for (int m = 0; m < NM; m++) {
+        const bool second = map + m;
+        nm[m] = second ? -sm[2] : -sm[0];
+        il[m] = (second ? sm[3] * dd[3] : sm[1]) * pup;
+        D[m] = second ? -dd[1] : -dd[0];
+    }
+    f32x16 acc[NM][CT];
+#pragma unroll
+    for (int m = 0; m < NM; m++)
 #pragma unroll
         for (int c = 0; c < CT; c++)
 #pragma unroll
@@ -876,13 +913,13 @@ diff_dq_kernel(DiffArgs g) {
         dsup = dsup1;
         if (t == flip) {
             sgn = -1.0f;
-            il[0] = -il[0];
-            il[1] = -il[1];
+#pragma unroll
+            for (int m = 0; m < NM; m++) il[m] = -il[m];
             ratio = -ratio;
         }
         if (t && __any(ratio != 1.0f)) {
 #pragma unroll
-            for (int m = 0; m < 2; m++)
+            for (int m = 0; m < NM; m++)
 #pragma unroll
                 for (int c = 0; c < CT; c++)
 #pragma unroll
@@ -894,18 +931,23 @@ diff_dq_kernel(DiffArgs g) {
             const _Float16 *const kt = lds[t & 1] + 32 * kg * Tile::STRIDE, *const vt = kt + Tile::HALVES;
             const int k1 = k0 + 32 * kg;
             const float kdown = down_of(kup);
-            f32x16 s1, s2, da;
+            f32x16 s[NM], da;
 #pragma unroll
-            for (int r = 0; r < 16; r++) s1[r] = s2[r] = da[r] = 0.f;
-            dot_along<Tile>(kt, 0, q[0], s1);
-            dot_along<Tile>(kt, DHP, q[1], s2);
+            for (int r = 0; r < 16; r++) da[r] = 0.f;
+#pragma unroll
+            for (int m = 0; m < NM; m++) {
+#pragma unroll
+                for (int r = 0; r < 16; r++) s[m][r] = 0.f;
+                dot_along<Tile>(kt, (map + m) * DHP, q[m], s[m]);
+            }
             dot_along<Tile>(vt, 0, d, da);
-            read_ahead<2 * KS + VS, 2, 3>();
-            const float f1 = kdown * qdown[0], f2 = kdown * qdown[1];
+            read_ahead<NM * KS + VS, 2, 3>();
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-                s1[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s1[r], f1, nm[0])) * il[0];
-                s2[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s2[r], f2, nm[1])) * il[1];
+            for (int m = 0; m < NM; m++) {
+                const float f = kdown * qdown[m];
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    s[m][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[m][r], f, nm[m])) * il[m];
             }
             const bool whole = k1 + 32 <= nk && !(g.causal && k1 + 31 > w_first + shift) &&
                                !(g.diag && k1 <= w_last && w_first < k1 + 32);
@@ -914,34 +956,33 @@ diff_dq_kernel(DiffArgs g) {
                 for (int r = 0; r < 16; r++) {
                     const int j = k1 + 8 * (r >> 2) + 4 * lh + (r & 3);
                     const bool in = j < nk && !(g.causal && j > qi + shift) && !(g.diag && j == qi);
-                    s1[r] = in ? s1[r] : 0.f;
-                    s2[r] = in ? s2[r] : 0.f;
+#pragma unroll
+                    for (int m = 0; m < NM; m++) s[m][r] = in ? s[m][r] : 0.f;
                 }
             }
-            const float fd = down_of(vup) * ddown * dsup, D1 = -dd[0] * dsup, D2 = -dd[1] * dsup;
+            const float fd = down_of(vup) * ddown * dsup;
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-                s1[r] *= __builtin_fmaf(da[r], fd, D1);
-                s2[r] *= __builtin_fmaf(da[r], fd, D2);
-            }
+            for (int m = 0; m < NM; m++) {
+                const float dm = D[m] * dsup;
 #pragma unroll
-            for (int m = 0; m < 2; m++) {
+                for (int r = 0; r < 16; r++) s[m][r] *= __builtin_fmaf(da[r], fd, dm);
                 Half2 ds[2];
-                split16(m ? s2 : s1, ds);
+                split16(s[m], ds);
 #pragma unroll
-                for (int c = 0; c < CT; c++) dot_across<Tile>(kt, m * DHP + 32 * c, ds, acc[m][c]);
+                for (int c = 0; c < CT; c++)
+                    dot_across<Tile>(kt, (map + m) * DHP + 32 * c, ds, acc[m][c]);
             }
-            read_ahead<4 * CT, 4, 3>();
+            read_ahead<2 * NM * CT, 4, 3>();
         }
         if (t + 2 < ntile) maxima(t & 1);
     }
     if constexpr (KG > 1) {
         __syncthreads();
-        float *const ex = (float *)lds + rg * 2 * CT * 16 * 64 + lane;
+        float *const ex = (float *)lds + (rg * 2 + map) * CT * 16 * 64 + lane;
         auto each = [&](int i, auto &&f) {
             float *e = ex + (i - 1) * RG * 2 * CT * 16 * 64;
 #pragma unroll
-            for (int m = 0; m < 2; m++)
+            for (int m = 0; m < NM; m++)
 #pragma unroll
                 for (int c = 0; c < CT; c++)
 #pragma unroll
@@ -957,10 +998,10 @@ diff_dq_kernel(DiffArgs g) {
     float *dst = g.dq + ((long long)b * g.tq + qi) * g.qstride + 2 * head * g.dh;
     const float f = down_of(kup) * (g.scale * sgn), f2 = down_of(dsup) * down_of(pup);
 #pragma unroll
-    for (int m = 0; m < 2; m++)
+    for (int m = 0; m < NM; m++)
 #pragma unroll
         for (int c = 0; c < CT; c++)
-            put_channels<VEC>(dst + m * g.dh, g.dh, 32 * c, acc[m][c], m ? -f : f, f2, live,
+            put_channels<VEC>(dst + (map + m) * g.dh, g.dh, 32 * c, acc[m][c], map + m ? -f : f, f2, live,
                               g.acc_q);
 }
 
@@ -1070,7 +1111,11 @@ diff_dkv_kernel(DiffArgs g) {
             mq = absmax8(xq[i], mq);
             md = absmax8(xd[i], md);
         }
-        f4 m = {wave_over(mq, good_for(qup1)), wave_over(md, good_for(dup1)), 0.f, 0.f};
+        f4 m = {0.f, 0.f, 0.f, 0.f};
+        if (__any(mq > good_for(qup1) || md > good_for(dup1))) {
+            m[0] = wave_max(mq);
+            m[1] = wave_max(md);
+        }
         if (wave == 0) {
             if (__any(!(r1[2] * (ds_root<W>() * vmax) * sup1 < 2.0f))) m[2] = wave_max(r1[2]);
             m[3] = wave_over(fabsf(r1[3]), ml);
@@ -1302,7 +1347,8 @@ __device__ __forceinline__ void dot_tiles(const _Float16 *ta, int ca, const _Flo
 // has been read for the last time, row by row, and come back transposed as
 // operands of dV and dK, whose blocks of 32 keys and 32 channels the waves share
 // out.  Memory bounds it: 128 x 4 heads of 64 rows and keys, dh 32, 20.5 us (60 MB;
-// 12 at a copy's rate) where dQ and dK/dV apart took 18.7 + 18.3.
+// 12 at a copy's rate) where dQ and dK/dV apart took 18.7 + 18.3; 64 rows on 256
+// keys 44.3 us (160 MB; 32) instead of 28.7 + 50.8.
 template <int DHP>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DHP <= 32 ? 2 : 1))) void
 diff_bwd_rows_kernel(DiffArgs g) {
@@ -1583,9 +1629,14 @@ PrePlan plan_pre(const rnn_diff_attn_desc *d, size_t n, bool vec) {
 // Row groups of 32 a workgroup of the forward, and the splits of the keys: a
 // power of two of groups up to four, keys split where the rows leave half of the
 // CUs idle (2 x 8 causal heads of 1568 rows and keys, dh 64, 208 workgroups: 111 us
-// unsplit, 124 and 24 for the join with two splits).
+// unsplit, 124 and 24 for the join with two splits).  Above 32 channels, where LDS
+// holds one workgroup a CU, two row groups with two waves on each row where four
+// would not fill the CUs (208 workgroups: 90 us against 122; 8 heads of 2048: 110
+// against 157; 256 workgroups, 8 heads of 4096: 390 against 333; at 32 channels 8 x 6
+// heads of 577: 46.9 against 36.2).
 struct FwdPlan {
     int qg, splits, split_keys;
+    bool halves;  // two waves share a row's keys
     size_t blocks;
 };
 FwdPlan plan_fwd(const rnn_diff_attn_desc *d, size_t n, bool vec) {
@@ -1599,6 +1650,12 @@ FwdPlan plan_fwd(const rnn_diff_attn_desc *d, size_t n, bool vec) {
     const size_t per = rnn_div_up(std::max<size_t>(tiles, 1), s);
     p.split_keys = (int)per * 64;
     p.splits = (int)rnn_div_up(std::max<size_t>(tiles, 1), per);
+    p.halves = false;
+    if (p.qg == 4 && vec && d->dh > 32 && p.splits == 1 && p.blocks < 256) {
+        p.halves = true;
+        p.qg = 2;
+        p.blocks = probs * rnn_div_up(R, (size_t)64);
+    }
     return p;
 }
 
@@ -1696,13 +1753,16 @@ bool rows_vec(const DiffArgs &g) {
            al(g.dy) && al(g.dq) && al(g.dkv);
 }
 
-template <int DHP, bool VEC, int QG>
+template <int DHP, bool VEC, int QG, int KH = 1>
 void launch_fwd_qg(rnn_ctx *ctx, const DiffArgs &g, const FwdPlan &p) {
     const dim3 grid((unsigned)p.blocks, (unsigned)p.splits);
-    if (p.splits > 1)
-        diff_fwd_kernel<DHP, VEC, QG, true><<<grid, 128 * QG, 0, ctx->stream>>>(g);
-    else
-        diff_fwd_kernel<DHP, VEC, QG, false><<<grid, 128 * QG, 0, ctx->stream>>>(g);
+    if constexpr (KH == 1) {
+        if (p.splits > 1) {
+            diff_fwd_kernel<DHP, VEC, QG, 1, true><<<grid, 128 * QG, 0, ctx->stream>>>(g);
+            return;
+        }
+    }
+    diff_fwd_kernel<DHP, VEC, QG, KH, false><<<grid, 128 * QG * KH, 0, ctx->stream>>>(g);
 }
 template <int DHP>
 void launch_fwd(rnn_ctx *ctx, const DiffArgs &g, const FwdPlan &p, bool vec) {
@@ -1710,6 +1770,8 @@ void launch_fwd(rnn_ctx *ctx, const DiffArgs &g, const FwdPlan &p, bool vec) {
         launch_fwd_qg<DHP, false, 4>(ctx, g, p);
     else if (p.qg == 1)
         launch_fwd_qg<DHP, true, 1>(ctx, g, p);
+    else if (DHP > 32 && p.halves)
+        launch_fwd_qg<DHP, true, 2, (DHP > 32 ? 2 : 1)>(ctx, g, p);
     else if (p.qg == 2)
         launch_fwd_qg<DHP, true, 2>(ctx, g, p);
     else
@@ -1721,23 +1783,25 @@ size_t params_of(const DiffArgs &g) {
     return (g.dgain ? rnn_div_up(2 * (size_t)g.dh, 16) : 0) + (size_t)g.lam_heads;
 }
 
-template <int DHP, bool VEC, int RG, int KG>
+template <int DHP, bool VEC, int RG, int KG, int NM = 2>
 void launch_dq(rnn_ctx *ctx, const DiffArgs &g) {
     const size_t R = (size_t)g.tq * g.group;
     const unsigned grid = (unsigned)((size_t)g.n * g.hkv * rnn_div_up(R, 32 * RG) + params_of(g));
-    diff_dq_kernel<DHP, VEC, RG, KG><<<grid, 64 * RG * KG, 0, ctx->stream>>>(g);
+    diff_dq_kernel<DHP, VEC, RG, KG, NM><<<grid, 128 / NM * RG * KG, 0, ctx->stream>>>(g);
 }
 template <int DHP, bool VEC, int KG>
 void launch_dkv(rnn_ctx *ctx, const DiffArgs &g) {
     const unsigned grid = (unsigned)((size_t)g.n * g.hkv * rnn_div_up((size_t)g.tk, 32 * KG));
     diff_dkv_kernel<DHP, VEC, KG><<<grid, 128 * KG, 0, ctx->stream>>>(g);
 }
-// dQ: two waves share 32 rows wherever rows are short of filling 4 groups in every
-// CU twice (128 x 4 heads of 64 rows and keys, dh 32: 16.6 us against 17.4; 64 rows
-// on 256 keys: 26.8 against 32.2; 2 x 8 causal heads of 1568, dh 64: 110 against
-// 146; 8 x 6 of 577, dh 32: 38.9 against 38.0).  dK and dV: two groups of 32 keys, a
-// workgroup of four waves (the same with four groups: 26.8 against 16.7 us, 60.6
-// against 49.4, 188 against 167, 55.1 against 56.5).
+// Joint kernel for up to 64 rows where one tile holds the keys or problems fill the
+// CUs (128 x 4 heads of 64 rows on 256 keys 44 us, apart 29 + 51).
+// dQ: two waves share 32 rows where four groups of 32 would not fill the CUs (2 x 8
+// causal heads of 1568, dh 64: 104 us against 160; 8 x 6 of 577, dh 32: 39.6 against
+// 38.0; 4 x 8 of 2048, dh 64: 515 against 436; 32 x 8 of 256, dh 64: 114 against 81).
+// dK and dV: four waves on two groups of 32 keys; above 32 channels, where a CU
+// holds one workgroup, eight on four where those fill the CUs (the same four: 188
+// against 167 us; 55.1 against 56.5; 578 against 870; 97 against 140).
 template <int DHP>
 void launch_bwd(rnn_ctx *ctx, const DiffArgs &g, bool vec) {
     const size_t probs = (size_t)g.n * g.hkv, R = (size_t)g.tq * g.group;
@@ -1750,8 +1814,8 @@ void launch_bwd(rnn_ctx *ctx, const DiffArgs &g, bool vec) {
             launch_dq<DHP, false, 4, 1>(ctx, g);
         else if (R <= 32)
             launch_dq<DHP, true, 1, 2>(ctx, g);
-        else if (R <= 64 || probs * rnn_div_up(R, 128) < 512)
-            launch_dq<DHP, true, 2, 2>(ctx, g);
+        else if (R <= 64 || probs * rnn_div_up(R, 128) < 256)
+            launch_dq<DHP, true, 2, 2, (DHP <= 32 ? 2 : 1)>(ctx, g);
         else
             launch_dq<DHP, true, 4, 1>(ctx, g);
     }
@@ -1760,6 +1824,8 @@ void launch_bwd(rnn_ctx *ctx, const DiffArgs &g, bool vec) {
             launch_dkv<DHP, false, 2>(ctx, g);
         else if (g.tk <= 32)
             launch_dkv<DHP, true, 1>(ctx, g);
+        else if (DHP > 32 && probs * rnn_div_up((size_t)g.tk, 128) >= 256)
+            launch_dkv<DHP, true, (DHP > 32 ? 4 : 2)>(ctx, g);
         else
             launch_dkv<DHP, true, 2>(ctx, g);
     }

@@ -114,6 +114,8 @@ CASES = [
     ("many_few_rows_48", 128, 4, 2, 48, 32, 66, True, dict(gap=0, per_head=True)),
     ("many_problems_16", 64, 4, 4, 16, 130, 70, True, dict(gap=0)),
     ("many_problems_64", 64, 8, 8, 64, 66, 65, True, dict(gap=0, causal=True)),
+    ("halves_48", 2, 4, 2, 48, 100, 140, True, dict(gap=0, qlen=[100, 7], klen=[140, 65])),
+    ("halves_64", 1, 3, 3, 64, 200, 200, False, dict(gap=0, causal=True, diag=True)),
 ]
 IDS = [c[0] for c in CASES]
 
