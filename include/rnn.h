@@ -279,7 +279,9 @@ int rnn_rotary(rnn_ctx *ctx, const rnn_rotary_desc *d, size_t n, size_t t, const
  * may hold anything.  causal: query i sees keys j <= i + (keys - queries), the
  * two sequences aligned at their ends; mask_diag: not key j = i.  A query that
  * sees no key, and a padding query, give y = 0.  The values that are read are
- * finite. */
+ * finite.  Products are taken in two fp16 parts under a power of two (of a row, of
+ * a tile, or in sums of all tiles so far): elements down to 2^-12 of the largest
+ * keep 2^-23 of themselves, smaller ones 2^-35 of the largest. */
 typedef struct {
     uint32_t h, hkv, dh, tq, tk;
     size_t qstride, qoff, kvstride, koff, voff;
@@ -291,8 +293,8 @@ typedef struct {
  * forward (backward = 0) or the backward needs for n images; host only.  The
  * workspace is the caller's, 256-byte aligned, holds nothing between calls
  * and is not shared by calls that may run at the same time.  dh <= 64
- * and row strides <= 2^22 (RNN_E_UNSUPPORTED above), scale > 0, 0 <= lam_init
- * < 1. */
+ * and row strides <= 2^22, n * max(tq, tk) * h < 2^30 (RNN_E_UNSUPPORTED above),
+ * scale > 0, 0 <= lam_init < 1. */
 int rnn_diff_attn_workspace(const rnn_diff_attn_desc *d, size_t n, int backward, size_t *bytes);
 /* y [n][tq][h][2 dh].  For a backward: o12 [n][tq][h][2][2 dh] receives each
  * map's P_m V and stats [n][tq][h][4] (16-byte aligned) each map's largest score
@@ -307,7 +309,7 @@ int rnn_diff_attn_forward(rnn_ctx *ctx, const rnn_diff_attn_desc *d, size_t n, c
  * (RNN_ATTN_SET_DQ, RNN_ATTN_SET_DKV: the columns of queries, or of keys and
  * values, padding rows included, which receive 0); dlam [lam_heads][4][dh] and
  * dgain [2 dh] (NULL with gain) accumulate.  dq and dkv may be one buffer with
- * disjoint columns.  Sums run in a fixed order. */
+ * disjoint columns, and overlap no other operand.  Sums run in a fixed order. */
 int rnn_diff_attn_backward(rnn_ctx *ctx, const rnn_diff_attn_desc *d, size_t n, const float *q,
                            const float *kv, const float *lam, const float *gain,
                            const uint32_t *qlen, const uint32_t *klen, const float *o12,
@@ -346,7 +348,10 @@ int rnn_linear_backward_ex(rnn_ctx *ctx, size_t rows, size_t fin, size_t fout, c
  * RNN_ACT_NONE z, RNN_ACT_RELU max(z, 0), RNN_ACT_GELU z (1 + erf(z / sqrt 2)) /
  * 2, RNN_ACT_GELU_TANH z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2,
  * RNN_ACT_SILU z / (1 + exp(-z)); RELU's slope at 0 is 0.  rows <= 2^30, fin and
- * fout <= 2^20. */
+ * fout <= 2^20.  Products are taken in two fp16 parts under a power of two (of a
+ * row of x, W and dz where the sum runs along rows, else of the whole tile):
+ * elements down to 2^-12 of the largest so far keep 2^-23 of themselves, smaller
+ * ones 2^-35 of the largest; an infinity in x, W or dy gives NaN. */
 #define RNN_ACT_NONE 0u
 #define RNN_ACT_RELU 1u
 #define RNN_ACT_GELU 2u

@@ -243,6 +243,11 @@ __device__ __forceinline__ void put_channels(float *dst, int lim, int c0, const 
 // waves, in two buffers: while one is read the next is written, and the loads of
 // the one after it are in flight.  KH: two waves take half of each tile's keys and
 // join their sums at the end (wave 2 (QG h + i) + m).
+// A tile's chain bounds it (barrier, S, maximum, exponentials, split, P V) with two
+// waves a SIMD: 8 heads of 4096 rows and keys over 2 key heads, dh 64, 303 us, 227
+// TFLOP/s of fp32 work, the matrix cores busy half of the time (rnn_matmul 168);
+// small problems by memory: 128 x 4 heads of 64, dh 32, 18 us (50 MB), 64 rows on 256
+// keys 27.5 us (101 MB).  One query over 4 x 16384 keys, split, 30 us for 134 MB.
 // SPLIT: the keys [z TS, (z + 1) TS) alone (z = blockIdx.y), each map's own
 // normalised output, maximum and sum left for diff_join_kernel.
 template <int DHP, bool VEC, int QG, int KH, bool SPLIT>
@@ -572,9 +577,9 @@ __global__ __launch_bounds__(256) void diff_join_kernel(DiffArgs g, int splits) 
 // Backward's first pass: dO, D_1 and D_2 of every (row, head), and the block's
 // partials of dgain and dlambda.  LPU lanes a unit, four channels each (VEC), or a
 // wave (LPU 64), two each; a group of lanes keeps one head, the groups in the
-// grid being a multiple of the heads.  The dots are 64-bit sums: dO is
+// grid being a multiple of the heads.  In 64 bits up to dO's own rounding: dO is
 // perpendicular to O, so that D_2, whose sum dlambda is, is small beside its
-// terms.
+// terms.  Memory bounds it: 128 x 4 heads of 64, dh 32, 12 us (35 MB).
 template <int LPU>
 __device__ __forceinline__ float group_sum(float v) {
     v += dpp_f<0xB1>(v);
@@ -622,7 +627,8 @@ __global__ __launch_bounds__(256) void diff_bwd_pre_kernel(DiffArgs g) {
     for (int u = unit0; u < units; u += stride) {
         const int row = u / g.h, b = row / g.tq;
         const bool live = row - b * g.tq < len_of(g.qlen, b, g.tq);
-        float o1[E], o2[E], o[E], dy[E], d[E], ss = 0.f;
+        float o1[E], o2[E], dy[E];
+        double o[E], d[E], ss = 0.0;
         const float *p1 = g.o12c + (long long)u * 2 * dv + c0, *py = g.dy + (long long)u * dv + c0;
         if constexpr (VEC) {
             const f4 z = {0.f, 0.f, 0.f, 0.f};
@@ -641,41 +647,41 @@ __global__ __launch_bounds__(256) void diff_bwd_pre_kernel(DiffArgs g) {
         }
 #pragma unroll
         for (int e = 0; e < E; e++) {
-            o[e] = o1[e] - lam * o2[e];
+            o[e] = (double)o1[e] - (double)lam * (double)o2[e];
             ss += o[e] * o[e];
-            d[e] = dy[e];
+            d[e] = (double)dy[e];
         }
         if (g.gain) {
-            const float r = 1.0f / sqrtf(group_sum<LPU>(ss) / (float)dv + g.eps);
-            float s = 0.f;
+            const double r = 1.0 / sqrt(group_sum<LPU>(ss) / (double)dv + (double)g.eps);
+            double t = 0.0;
 #pragma unroll
             for (int e = 0; e < E; e++) {
                 o[e] *= r;
-                s += dy[e] * gain[e] * o[e];
-                dg[e] += (double)dy[e] * (double)o[e];
+                t += (double)dy[e] * (double)gain[e] * o[e];
+                dg[e] += (double)dy[e] * o[e];
             }
-            s = group_sum<LPU>(s) / (float)dv;
+            t = group_sum<LPU>(t) / (double)dv;
 #pragma unroll
-            for (int e = 0; e < E; e++) d[e] = r * (dy[e] * gain[e] - o[e] * s);
+            for (int e = 0; e < E; e++) d[e] = r * ((double)dy[e] * (double)gain[e] - o[e] * t);
         }
         double d1 = 0.0, d2 = 0.0;
         float nd = 0.f;
 #pragma unroll
         for (int e = 0; e < E; e++) {
-            d1 += (double)d[e] * (double)o1[e];
-            d2 += (double)d[e] * (double)o2[e];
-            nd += d[e] * d[e];
+            d1 += d[e] * (double)o1[e];
+            d2 += d[e] * (double)o2[e];
+            nd += (float)d[e] * (float)d[e];
         }
         d1 = group_sum<LPU>(d1);
         d2 = group_sum<LPU>(d2);
         nd = sqrtf(group_sum<LPU>(nd));
         float *pd = g.dout + (long long)u * dv + c0;
         if constexpr (VEC) {
-            if (in) *(f4 *)pd = f4{d[0], d[1], d[2], d[3]};
+            if (in) *(f4 *)pd = f4{(float)d[0], (float)d[1], (float)d[2], (float)d[3]};
         } else {
 #pragma unroll
             for (int e = 0; e < E; e++)
-                if (c0 + e < dv) pd[e] = d[e];
+                if (c0 + e < dv) pd[e] = (float)d[e];
         }
         if (c0 == 0) {
             const f4 z = {0.f, 0.f, 0.f, 0.f};
@@ -771,14 +777,15 @@ __device__ __forceinline__ void bwd_params(const DiffArgs &g, int blk, double *r
 
 // The power of two of dA for rows with |dO| <= nd and values of magnitude <= vmax,
 // from m = nd ds_root vmax >= 2 |dA| (|dA| <= nd sqrt(W) vmax, and D is a mean of
-// dA): it takes m to 2 or below, and stays as it was (up) while that holds, as
-// sticky_up.
+// dA): it takes m to [1, 2), and stays as it was (up) until m times it passes 2.
+// Without sticky_up's slack: the bound is a hundred times what dA mostly is, and P
+// far below 1, so that another 2^-4 would leave dS 2^-19 of itself.
 template <int W>
 __device__ __forceinline__ constexpr float ds_root() {
     return W == 32 ? 11.313709f : W == 64 ? 16.0f : W == 96 ? 19.595918f : 22.627417f;
 }
 __device__ __forceinline__ float ds_up(float m, float up) {
-    return m * up < 2.0f ? up : up_of(m) * 0x1p-18f;
+    return m * up < 2.0f ? up : up_of(m) * 0x1p-14f;
 }
 // The power of two that softmax values, and lambda times them, enter the
 // backward's products with: at most 2^14, so that P_1 - lambda P_2 and P (dA - D)
@@ -797,7 +804,9 @@ __device__ __forceinline__ int flip_at(int ntile) { return (2 * ntile + 2) / 3; 
 // row), and P (dA - D) in registers is the operand of dQ_m^T = K_m^T dS_m^T, which
 // is summed over all tiles in the accumulators.  Their unit is a power of two that
 // hardly changes (sticky_up); where it does they are rescaled.  The waves that share
-// rows add theirs at the end.
+// rows add theirs at the end.  Bound as the forward: 4 x 8 heads of 2048, dh 64, 436
+// us (236 TFLOP/s of fp32 work); 2 x 8 causal heads of 1568 104 us (145, the longest
+// rows' chain); 8 x 6 ragged of up to 577, dh 32, 40 us.
 template <int DHP, bool VEC, int RG, int KG, int NM>
 __global__ __launch_bounds__(128 / NM * RG * KG)
 __attribute__((amdgpu_waves_per_eu((DHP <= 32 && RG > 1) || NM == 1 ? 2 : 1))) void
@@ -1013,6 +1022,9 @@ diff_dq_kernel(DiffArgs g) {
 // through LDS, and then P and dS in registers are the operands of the wave's half
 // of dV^T = dO^T (P_1 - lambda P_2) and of dK_m^T = Q_m^T dS_m, summed over all tiles
 // in the accumulators as in diff_dq_kernel.
+// A tile's chain bounds it here too: 4 x 8 heads of 2048, dh 64, 578 us (238 TFLOP/s
+// of fp32 work); 2 x 8 causal heads of 1568 167 us (120); 8 x 6 ragged of up to 577,
+// dh 32, 56 us.
 template <int DHP, bool VEC, int KG>
 __global__ __launch_bounds__(128 * KG) __attribute__((amdgpu_waves_per_eu(DHP <= 32 && KG > 1 ? 2 : 1))) void
 diff_dkv_kernel(DiffArgs g) {
@@ -1346,10 +1358,10 @@ __device__ __forceinline__ void dot_tiles(const _Float16 *ta, int ca, const _Flo
 // dQ as diff_dq_kernel does; P_1 - lambda P_2 and dS_m go through LDS where the tile
 // has been read for the last time, row by row, and come back transposed as
 // operands of dV and dK, whose blocks of 32 keys and 32 channels the waves share
-// out.  Memory bounds it: 128 x 4 heads of 64 rows and keys, dh 32, 20.5 us (60 MB;
+// out.  ONE: one tile holds the keys.  Memory bounds it: 128 x 4 heads of 64 rows and keys, dh 32, 20.5 us (60 MB;
 // 12 at a copy's rate) where dQ and dK/dV apart took 18.7 + 18.3; 64 rows on 256
 // keys 44.3 us (160 MB; 32) instead of 28.7 + 50.8.
-template <int DHP>
+template <int DHP, bool ONE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DHP <= 32 ? 2 : 1))) void
 diff_bwd_rows_kernel(DiffArgs g) {
     constexpr int W = 2 * DHP, KS = DHP / 16, VS = W / 16, CT = (DHP + 31) / 32;
@@ -1364,6 +1376,7 @@ diff_bwd_rows_kernel(DiffArgs g) {
     __shared__ float rec[6][64];  // as in diff_dkv_kernel
     __shared__ f4 rmax[4];
     __shared__ f2 tmax[4];
+    __shared__ f4 psum[2][ONE ? 64 : 1];  // sums of P_m and of P_m dA over 32 keys
     const int np = params_blocks(g);
     if ((int)blockIdx.x < np) {
         bwd_params<256>(g, (int)blockIdx.x, (double *)lds);
@@ -1464,7 +1477,7 @@ diff_bwd_rows_kernel(DiffArgs g) {
         for (int c = 0; c < CT; c++) zero(dq[m][c]);
     // keys that some row sees; the others' gradients are zeros
     const int kend = g.causal ? min(nk, nq + shift) : nq ? nk : 0;
-    const int nt = (g.tk + 63) / 64, flip = flip_at((max(kend, 0) + 63) / 64);
+    const int nt = ONE ? 1 : (g.tk + 63) / 64, flip = flip_at((max(kend, 0) + 63) / 64);
     // the largest value so far and powers of two, sgn: the accumulators' sign
     float vmax = 0.f, kup = FIRST_UP, sup = FIRST_UP, sgn = 1.f;
     for (int t = 0; t < nt; t++) {
@@ -1506,7 +1519,7 @@ diff_bwd_rows_kernel(DiffArgs g) {
                     for (int r = 0; r < 16; r++) dq[m][c][r] *= ratio;
         }
         st.store(kt, kup, vup, SLOT);
-        if (k0 + 64 < kend) st.load(k0 + 64);
+        if (!ONE && k0 + 64 < kend) st.load(k0 + 64);
         __syncthreads();
         const _Float16 *const k1 = kt + 32 * kg * Tile::STRIDE;
         Half2 ah[2], ds[2][2];
@@ -1534,17 +1547,50 @@ diff_bwd_rows_kernel(DiffArgs g) {
             const float f = down_of(kup) * (down_of(qup) * (g.scale * LOG2E));
             const float fd = down_of(vup) * down_of(dup) * sup;
             const float nm1 = rec[0][row], il1 = rec[1][row] * sgn, nm2 = rec[2][row], il2 = rec[3][row] * sgn;
-            const float D1 = rec[4][row] * sup, D2 = rec[5][row] * sup;
             f32x16 a;
-#pragma unroll
-            for (int r = 0; r < 16; r++) {
+            auto softmax = [&](int r, float &p1, float &p2) {
                 const int j = k0 + 32 * kg + 8 * (r >> 2) + 4 * lh + (r & 3);
                 const bool in = j < nk && !(g.causal && j > qi + shift) && !(g.diag && j == qi);
-                const float p1 = in ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], f, nm1)) * il1 : 0.f;
-                const float p2 = in ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[1][r], f, nm2)) * il2 : 0.f;
+                p1 = in ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], f, nm1)) * il1 : 0.f;
+                p2 = in ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[1][r], f, nm2)) * il2 : 0.f;
                 a[r] = p1 + p2;
-                s[0][r] = p1 * __builtin_fmaf(da[r], fd, D1);
-                s[1][r] = p2 * __builtin_fmaf(da[r], fd, D2);
+            };
+            if constexpr (ONE) {
+                // D_m as the mean of these dA, whose rounding it shares: a row that sees
+                // one key has dS = 0, and nothing but rounding would be left of it
+                f4 ps = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    float p1, p2;
+                    softmax(r, p1, p2);
+                    s[0][r] = p1;
+                    s[1][r] = p2;
+                    ps[0] += p1;
+                    ps[1] = __builtin_fmaf(p1, da[r], ps[1]);
+                    ps[2] += p2;
+                    ps[3] = __builtin_fmaf(p2, da[r], ps[3]);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) ps[i] = pair32(ps[i], add2);
+                if (lh == 0) psum[kg][row] = ps;
+                __syncthreads();
+                ps = psum[0][row] + psum[1][row];
+                const float D1 = ps[0] != 0.f ? -fd * (ps[1] / ps[0]) : 0.f;
+                const float D2 = ps[2] != 0.f ? -fd * (ps[3] / ps[2]) : 0.f;
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    s[0][r] *= __builtin_fmaf(da[r], fd, D1);
+                    s[1][r] *= __builtin_fmaf(da[r], fd, D2);
+                }
+            } else {
+                const float D1 = rec[4][row] * sup, D2 = rec[5][row] * sup;
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    float p1, p2;
+                    softmax(r, p1, p2);
+                    s[0][r] = p1 * __builtin_fmaf(da[r], fd, D1);
+                    s[1][r] = p2 * __builtin_fmaf(da[r], fd, D2);
+                }
             }
             split16(a, ah);
             split16(s[0], ds[0]);
@@ -1708,7 +1754,7 @@ int diff_check(rnn_ctx *ctx, const rnn_diff_attn_desc *d, size_t n) {
         return rnn_fail(ctx, RNN_E_INVALID, "diff_attn: heads do not fit a row");
     if (d->koff < d->voff + kw && d->voff < d->koff + kw)
         return rnn_fail(ctx, RNN_E_INVALID, "diff_attn: keys and values overlap");
-    const size_t lim = 0x7fffffffu;
+    const size_t lim = 0x3fffffffu;  // (a grid's stride past a row's number stays an int)
     if (n > lim || d->tq > (1u << 26) || d->tk > (1u << 26) || d->kvstride > (1u << 22) || d->qstride > (1u << 22) ||
         (d->tq && n > lim / d->tq) || (d->tk && n > lim / d->tk) ||
         n * std::max(d->tq, d->tk) > lim / d->h)
@@ -1806,7 +1852,11 @@ template <int DHP>
 void launch_bwd(rnn_ctx *ctx, const DiffArgs &g, bool vec) {
     const size_t probs = (size_t)g.n * g.hkv, R = (size_t)g.tq * g.group;
     if (vec && g.tq && R <= 64 && g.tk && (g.tk <= 64 || probs >= 256)) {
-        diff_bwd_rows_kernel<DHP><<<(unsigned)(probs + params_of(g)), 256, 0, ctx->stream>>>(g);
+        const unsigned grid = (unsigned)(probs + params_of(g));
+        if (g.tk <= 64)
+            diff_bwd_rows_kernel<DHP, true><<<grid, 256, 0, ctx->stream>>>(g);
+        else
+            diff_bwd_rows_kernel<DHP, false><<<grid, 256, 0, ctx->stream>>>(g);
         return;
     }
     if (g.tq) {

@@ -85,6 +85,8 @@ def test_diff_description_is_checked():
     assert code(kvstride=1 << 40) == R.RNN_E_UNSUPPORTED
     assert code(n=1 << 40) == R.RNN_E_UNSUPPORTED
     assert code(n=1 << 29) == R.RNN_E_UNSUPPORTED
+    assert code(n=1 << 25) == R.RNN_E_UNSUPPORTED  # n tq h = 2^30
+    assert code(n=(1 << 25) - 1) == R.RNN_OK
     assert R.lib().rnn_diff_attn_workspace(None, 1, 0, C.byref(nb)) == R.RNN_E_NULL
 
 

@@ -97,6 +97,7 @@ CASES = [
     ("few_queries_causal", 2, 4, 1, 48, 4, 900, True, dict(causal=True, klen=[900, 2], gap=2)),
     ("peaked", 2, 2, 2, 32, 64, 200, True, dict(amp=8.0, gap=0)),
     # one for every way that rows and keys are shared out
+    ("one_token_aligned", 3, 4, 2, 64, 1, 1, True, dict(gap=0, causal=True)),
     ("small_shared_48", 3, 6, 2, 48, 21, 60, True, dict(gap=0, causal=True, klen=[60, 7, 0])),
     ("small_shared_16", 2, 4, 1, 16, 16, 64, True, dict(gap=0, per_head=True)),
     ("small_64_ragged", 4, 2, 2, 64, 64, 64, False,
