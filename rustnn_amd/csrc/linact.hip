@@ -61,8 +61,8 @@ __device__ __forceinline__ float act_both(float z, float *slope) {
         // slope is 0 or 1 to the last bit, and z^2 stays finite
         const float c = fminf(fmaxf(z, -30.0f), 30.0f), cc = c * c;
         float d;
-        const float s = logistic(1.59576912160573072f * __builtin_fmaf(0.044715f * cc, c, c), &d);
-        *slope = __builtin_fmaf(c * 1.59576912160573072f * __builtin_fmaf(0.134145f, cc, 1.0f), d, s);
+        const float s = logistic(1.5957691216f * __builtin_fmaf(0.044715f * cc, c, c), &d);
+        *slope = __builtin_fmaf(c * 1.5957691216f * __builtin_fmaf(0.134145f, cc, 1.0f), d, s);
         return z * s;
     } else if constexpr (ACT == RNN_ACT_SILU) {
         float d;
@@ -120,8 +120,8 @@ __device__ __forceinline__ void quad_store(float *p, f4 v, int cnt) {
 // How an operand of R rows (of C) is staged over a depth of KB: KC: k runs along
 // its rows in memory (R rows of KB), 16-byte slots of a row exchanged so that the
 // b128 reads of 8 rows fall on distinct banks; each row has its own power of two
-// (its threads are neighbours).  Else k runs
-// across them (KB rows of R, padded), read transposed, one power for the tile.
+// (its threads are neighbours).  Else k runs across them (KB rows of R, padded, in
+// row_pos' order), read transposed, one power for the tile.
 // Two register sets: stage t's loads go out while stage t - 3 is computed.
 template <int R, int KB, bool KC, bool PRO, int NT>
 struct Operand {
