@@ -517,26 +517,26 @@ __global__ __launch_bounds__(256) void diff_join_kernel(DiffArgs g, int splits) 
     const float t0 = wave_sum(w0), t1 = wave_sum(w1);
     f2 o0 = {0.f, 0.f}, o1 = o0;
     const int c = 2 * lane;
-    if (c < dv) {
-        const float *src = g.part32 + w * splits * 2 * dv + c;
-        for (int s0 = part; s0 < splits; s0 += 8 * WPR) {
-            f2 a[8], b[8];
+    // (every lane goes along, since it hands its split's weights to the others; those
+    // past the row read its last channels)
+    const float *src = g.part32 + w * splits * 2 * dv + min(c, dv - 2);
+    for (int s0 = part; s0 < splits; s0 += 8 * WPR) {
+        f2 a[8], b[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const long long at = (long long)min(s0 + i * WPR, splits - 1) * 2 * dv;
-                a[i] = *(const f2 *)(src + at);
-                b[i] = *(const f2 *)(src + at + dv);
-            }
+        for (int i = 0; i < 8; i++) {
+            const long long at = (long long)min(s0 + i * WPR, splits - 1) * 2 * dv;
+            a[i] = *(const f2 *)(src + at);
+            b[i] = *(const f2 *)(src + at + dv);
+        }
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int s = s0 + i * WPR;
-                if (s >= splits) break;
-                const float x = __shfl(w0, s, 64), y = __shfl(w1, s, 64);
+        for (int i = 0; i < 8; i++) {
+            const int s = s0 + i * WPR;
+            if (s >= splits) break;
+            const float x = __shfl(w0, s, 64), y = __shfl(w1, s, 64);
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    o0[e] = __builtin_fmaf(x, a[i][e], o0[e]);
-                    o1[e] = __builtin_fmaf(y, b[i][e], o1[e]);
-                }
+            for (int e = 0; e < 2; e++) {
+                o0[e] = __builtin_fmaf(x, a[i][e], o0[e]);
+                o1[e] = __builtin_fmaf(y, b[i][e], o1[e]);
             }
         }
     }
@@ -557,7 +557,7 @@ __global__ __launch_bounds__(256) void diff_join_kernel(DiffArgs g, int splits) 
     float rn = 1.0f;
     f2 gn = {1.f, 1.f};
     if (g.gain) {
-        const float ss = wave_sum(out[0] * out[0] + out[1] * out[1]);
+        const float ss = wave_sum(c < dv ? out[0] * out[0] + out[1] * out[1] : 0.f);
         rn = (1.0f / sqrtf(ss / (float)dv + g.eps)) * (1.0f - g.lam_init);
         if (c < dv) gn = f2{g.gain[c], g.gain[c + 1]};
     }
@@ -1675,11 +1675,13 @@ PrePlan plan_pre(const rnn_diff_attn_desc *d, size_t n, bool vec) {
 // Row groups of 32 a workgroup of the forward, and the splits of the keys: a
 // power of two of groups up to four, keys split where the rows leave half of the
 // CUs idle (2 x 8 causal heads of 1568 rows and keys, dh 64, 208 workgroups: 111 us
-// unsplit, 124 and 24 for the join with two splits).  Above 32 channels, where LDS
-// holds one workgroup a CU, two row groups with two waves on each row where four
-// would not fill the CUs (208 workgroups: 90 us against 122; 8 heads of 2048: 110
-// against 157; 256 workgroups, 8 heads of 4096: 390 against 333; at 32 channels 8 x 6
-// heads of 577: 46.9 against 36.2).
+// unsplit, 124 and 24 for the join with two splits), down to a tile a split where
+// the partial sums are small (11 x 1 query over 473 keys, dh 64, 12 + 4 us; with four
+// tiles 24.5 + 4).  Above 32 channels, where LDS holds one workgroup a CU, two row
+// groups with two waves on each row where four would not fill the CUs (208
+// workgroups: 90 us against 122; 8 heads of 2048: 110 against 157; 256 workgroups, 8
+// heads of 4096: 390 against 333; at 32 channels 8 x 6 heads of 577: 46.9 against
+// 36.2).
 struct FwdPlan {
     int qg, splits, split_keys;
     bool halves;  // two waves share a row's keys
@@ -1691,7 +1693,8 @@ FwdPlan plan_fwd(const rnn_diff_attn_desc *d, size_t n, bool vec) {
     p.qg = !vec ? 4 : R <= 32 ? 1 : R <= 64 ? 2 : 4;
     p.blocks = probs * rnn_div_up(R, (size_t)32 * p.qg);
     const size_t tiles = rnn_div_up(d->tk, (size_t)64);
-    size_t s = p.blocks && p.blocks < 128 ? std::min(tiles / 4, 512 / p.blocks) : 1;
+    const size_t least = p.blocks <= 16 ? 1 : p.blocks <= 64 ? 2 : 4;  // tiles of a split
+    size_t s = p.blocks && p.blocks < 128 && tiles >= 4 ? std::min(tiles / least, 512 / p.blocks) : 1;
     s = std::max<size_t>(1, std::min<size_t>(s, 64));
     const size_t per = rnn_div_up(std::max<size_t>(tiles, 1), s);
     p.split_keys = (int)per * 64;

@@ -106,6 +106,8 @@ CASES = [
     ("few_keys_32", 2, 4, 1, 32, 150, 20, True, dict(gap=0, diag=True)),
     ("few_keys_64", 2, 2, 2, 64, 70, 31, True, dict(gap=0, causal=True)),
     ("few_rows_16", 2, 2, 2, 16, 9, 333, True, dict(gap=0, klen=[333, 70])),
+    ("splits_past_32", 1, 2, 2, 16, 1, 8300, True, dict(gap=0, gain=False)),
+    ("splits_past_32_odd", 1, 2, 1, 5, 2, 9001, True, dict(gap=1)),
     ("rows_64_split", 1, 2, 2, 32, 50, 600, True, dict(gap=0)),
     ("rows_128_split", 1, 2, 1, 64, 65, 700, True, dict(gap=0, causal=True)),
     ("group_of_three", 2, 6, 2, 32, 47, 140, True, dict(gap=0, causal=True, per_head=True)),
