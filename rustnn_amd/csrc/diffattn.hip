@@ -775,14 +775,20 @@ __device__ __forceinline__ void bwd_params(const DiffArgs &g, int blk, double *r
     }
 }
 
-// The power of two of dA for rows with |dO| <= nd and values of magnitude <= vmax,
-// from m = nd ds_root vmax >= 2 |dA| (|dA| <= nd sqrt(W) vmax, and D is a mean of
-// dA): it takes m to [1, 2), and stays as it was (up) until m times it passes 2.
+// The power of two of dA - D for rows with |dO| <= nd and values of magnitude <=
+// vmax, from m = ds_bound >= |dA| + |D| (|dA| <= nd sqrt(W) vmax; D, a mean of dA over
+// all of the row's keys, may be far above it where vmax is of some of them alone): it
+// takes m to [1, 2), and stays as it was (up) until m times it passes 2.
 // Without sticky_up's slack: the bound is a hundred times what dA mostly is, and P
 // far below 1, so that another 2^-4 would leave dS 2^-19 of itself.
 template <int W>
 __device__ __forceinline__ constexpr float ds_root() {
     return W == 32 ? 11.313709f : W == 64 ? 16.0f : W == 96 ? 19.595918f : 22.627417f;
+}
+// dmax: the larger |D_m|.
+template <int W>
+__device__ __forceinline__ float ds_bound(float nd, float vmax, float dmax) {
+    return max2(nd * (ds_root<W>() * vmax), 2.0f * dmax);
 }
 __device__ __forceinline__ float ds_up(float m, float up) {
     return m * up < 2.0f ? up : up_of(m) * 0x1p-14f;
@@ -870,7 +876,7 @@ diff_dq_kernel(DiffArgs g) {
         for (int m = 0; m < NM; m++) qdown[m] = qf[m].split(q[m]) * (g.scale * LOG2E);
         ddown = df.split(d);
     }
-    const float pup = p_up(fabsf(dd[3]));
+    const float pup = p_up(fabsf(dd[3])), dmax = max2(fabsf(dd[0]), fabsf(dd[1]));
     float nm[NM], il[NM], D[NM];
 #pragma unroll
     for (int m = 0; m < NM; m++) {
@@ -916,7 +922,7 @@ diff_dq_kernel(DiffArgs g) {
         const int k0 = t * TK;
         __syncthreads();
         // dS's power of two, and the accumulators in the tile's unit
-        const float vup = vup1, dsup1 = ds_up(dd[2] * (ds_root<W>() * vmax), dsup);
+        const float vup = vup1, dsup1 = ds_up(ds_bound<W>(dd[2], vmax, dmax), dsup);
         float ratio = down_of(kup) * kup1 * (down_of(dsup) * dsup1);
         kup = kup1;
         dsup = dsup1;
@@ -1036,8 +1042,10 @@ diff_dkv_kernel(DiffArgs g) {
     __shared__ __align__(16) _Float16 lds[2][2 * Tile::HALVES + 32];
     // -m1, il1, -m2, -lambda il2, -D1, -D2, with their powers of two
     __shared__ __align__(16) float rec[2][6][TR];
-    // largest |q|, |dO|, |dO|_2, |lambda| of a tile past what is known of them
+    // largest |q|, |dO|, |dO|_2, |lambda| of a tile past what is known of them; with
+    // |dO|_2's, the largest |D_m|
     __shared__ f4 tmax[2][NW];
+    __shared__ float tdmax[2];
     __shared__ float vmaxs[NW];
     __shared__ float vkey[NW][32];
     __shared__ __align__(16) f32x4 ex[NW][8][64];  // P_m and a half of dA, each wave's
@@ -1129,8 +1137,14 @@ diff_dkv_kernel(DiffArgs g) {
             m[1] = wave_max(md);
         }
         if (wave == 0) {
-            if (__any(!(r1[2] * (ds_root<W>() * vmax) * sup1 < 2.0f))) m[2] = wave_max(r1[2]);
+            const float dm = max2(fabsf(r1[0]), fabsf(r1[1]));
+            float dall = 0.f;
+            if (__any(!(ds_bound<W>(r1[2], vmax, dm) * sup1 < 2.0f))) {
+                m[2] = wave_max(r1[2]);
+                dall = wave_max(dm);
+            }
             m[3] = wave_over(fabsf(r1[3]), ml);
+            if (lane == 0) tdmax[slot] = dall;
         }
         if (lane == 0) tmax[slot][wave] = m;
     };
@@ -1183,7 +1197,7 @@ diff_dkv_kernel(DiffArgs g) {
             md = max2(md, m[1]);
             if (i) continue;
             ml = max2(ml, m[3]);
-            sup1 = ds_up(m[2] * (ds_root<W>() * vmax), sup1);
+            sup1 = ds_up(ds_bound<W>(m[2], vmax, tdmax[t & 1]), sup1);
         }
         qup1 = sticky_up(mq, qup1);
         dup1 = sticky_up(md, dup1);
@@ -1375,6 +1389,7 @@ diff_bwd_rows_kernel(DiffArgs g) {
     __shared__ __align__(16) _Float16 lds[4][SLOT];  // K, V, Q, dO
     __shared__ float rec[6][64];  // as in diff_dkv_kernel
     __shared__ f4 rmax[4];
+    __shared__ float rdmax[4];
     __shared__ f2 tmax[4];
     __shared__ f4 psum[2][ONE ? 64 : 1];  // sums of P_m and of P_m dA over 32 keys
     const int np = params_blocks(g);
@@ -1426,13 +1441,20 @@ diff_bwd_rows_kernel(DiffArgs g) {
 #pragma unroll
         for (int i = 0; i < 4; i++) m[i] = wave_max(m[i]);
         if (lane == 0) rmax[wave] = m;
+        if (!ONE) {
+            const float dm = wave_max(max2(fabsf(r1[0]), fabsf(r1[1])));
+            if (lane == 0) rdmax[wave] = dm;
+        }
     }
     __syncthreads();
     f4 mx = rmax[0];
+    float dmax = ONE ? 0.f : rdmax[0];  // (ONE: D is a mean of this tile's dA)
 #pragma unroll
-    for (int i = 1; i < 4; i++)
+    for (int i = 1; i < 4; i++) {
 #pragma unroll
         for (int e = 0; e < 4; e++) mx[e] = max2(mx[e], rmax[i][e]);
+        if (!ONE) dmax = max2(dmax, rdmax[i]);
+    }
     const float qup = up_of(mx[0]), dup = up_of(mx[1]), pup = p_up(mx[3]);
     if (stager) {
 #pragma unroll
@@ -1502,7 +1524,7 @@ diff_bwd_rows_kernel(DiffArgs g) {
             vmax = max2(vmax, tmax[i][1]);
         }
         const float kup1 = sticky_up(mk, kup), vup = up_of(vmax);
-        const float sup1 = ds_up(mx[2] * (ds_root<W>() * vmax), sup);
+        const float sup1 = ds_up(ds_bound<W>(mx[2], vmax, dmax), sup);
         float ratio = down_of(kup) * kup1 * (down_of(sup) * sup1);
         kup = kup1;
         sup = sup1;

@@ -1,0 +1,167 @@
+"""GPU: differential attention away from magnitude 1: blocks of values that are
+zero or small, gradients of any size, tiny queries and keys, long keys,
+outliers, and what is not finite, against the operator's formulas in 64 bits.
+
+Tolerances.  A gradient is compared row by row or block by block, each against
+TOL (1e-5) of its own terms' size before they cancel: dS_ij = P_ij (dA_ij - D_i)
+has the terms P_ij |dA_ij| and P_ij |dO_i| |O_i|, and a sum's size is the root of
+the sum of its terms' squares (the terms' errors have no common sign).  A term's
+error is a few times 2^-22 (two operands of two fp16 parts, 2^-23 each; the
+score's error, 2^-22 |q| |k| scale = 2e-6 at a score of 8, in P; O from the forward,
+2^-24 of itself and P's again), so TOL leaves a factor of three at least."""
+import pytest
+import torch
+
+from conftest import TOL
+from diffref import D, DiffCase, seen
+from test_gpu_diffattn import run
+
+pytestmark = pytest.mark.gpu
+
+
+def refill(cs):
+    """The buffers of a case again, after its values were changed."""
+    nan = float("nan")
+    kl = cs.kvv.reshape(cs.n, cs.tk, cs.kw).masked_fill(cs.padk, nan)
+    vl = cs.vv.reshape(cs.n, cs.tk, cs.kw).masked_fill(cs.padk, nan)
+    cs.q[..., cs.qoff:cs.qoff + cs.qw] = cs.qv.reshape(cs.n, cs.tq, cs.qw).masked_fill(cs.padq, nan)
+    cs.kv[..., cs.koff:cs.koff + cs.kw] = kl
+    cs.kv[..., cs.voff:cs.voff + cs.kw] = vl
+    cs.dy = cs.dyv.masked_fill(cs.padq, nan)
+    return cs
+
+
+def formulas(cs):
+    """y, dq, dk, dv and the sizes of their terms, image by image in 64 bits."""
+    h, g, dh = cs.h, cs.h // cs.hkv, cs.dh
+    lam = cs.lam.to(D)
+    e1 = torch.exp((lam[:, 0] * lam[:, 1]).sum(-1))
+    e2 = torch.exp((lam[:, 2] * lam[:, 3]).sum(-1))
+    lam = (e1 - e2 + cs.lam_init).expand(h).view(h, 1, 1)
+    gain = None if cs.gain is None else (1.0 - cs.lam_init) * cs.gain.to(D)
+    see = seen(cs.n, cs.tq, cs.tk, cs.causal, cs.diag, cs.qlen, cs.klen)
+    out = {k: [] for k in ("y", "dq", "dk", "dv", "sq", "sk", "sv")}
+    rep = lambda t: t.repeat_interleave(g, 0)
+    fold = lambda t: t.view(cs.hkv, g, *t.shape[1:]).sum(1)
+    for b in range(cs.n):
+        q = cs.qv[b].to(D).permute(1, 2, 0, 3)                       # [h, 2, tq, dh]
+        k = rep(cs.kvv[b].to(D).permute(1, 2, 0, 3))
+        v = rep(cs.vv[b].to(D).permute(1, 0, 2))                     # [h, tk, 2 dh]
+        dy = cs.dyv[b].to(D).masked_fill(cs.padq[b], 0.0).view(cs.tq, h, 2 * dh).permute(1, 0, 2)
+        p, o = [], []
+        for m in range(2):
+            s = q[:, m] @ k[:, m].transpose(1, 2) * cs.scale
+            s = torch.softmax(s.masked_fill(~see[b], -1e300), -1) * see[b].any(-1, keepdim=True)
+            p.append(s)
+            o.append(s @ v)
+        O = o[0] - lam * o[1]
+        if gain is None:
+            y, do = O, dy
+        else:
+            r = 1.0 / torch.sqrt((O * O).mean(-1, keepdim=True) + cs.eps)
+            y = O * r * gain
+            t = dy * gain
+            do = r * (t - O * r * (t * O * r).mean(-1, keepdim=True))
+        da, a = do @ v.transpose(1, 2), p[0] - lam * p[1]
+        big = do.norm(dim=-1, keepdim=True)
+        out["y"].append(y.permute(1, 0, 2).reshape(cs.tq, -1))
+        out["dv"].append(fold(a.transpose(1, 2) @ do))
+        out["sv"].append(fold(((p[0] + lam * p[1]) ** 2).transpose(1, 2) @ big ** 2).sqrt())
+        grads = {n: [] for n in ("dq", "dk", "sq", "sk")}
+        for m in range(2):
+            c = 1.0 if m == 0 else -lam
+            ds = c * p[m] * (da - (do * o[m]).sum(-1, keepdim=True)) * cs.scale
+            t = (c * p[m] * (da.abs() + big * o[m].norm(dim=-1, keepdim=True)) * cs.scale) ** 2
+            grads["dq"].append(ds @ k[:, m])
+            grads["dk"].append(fold(ds.transpose(1, 2) @ q[:, m]))
+            grads["sq"].append((t @ k[:, m].norm(dim=-1, keepdim=True) ** 2).sqrt())
+            grads["sk"].append(fold(t.transpose(1, 2) @ q[:, m].norm(dim=-1, keepdim=True) ** 2).sqrt())
+        for n, x in grads.items():
+            out[n].append(torch.stack(x, 1))
+    t = {n: torch.stack(x) for n, x in out.items()}
+    t["dq"] = t["dq"].permute(0, 3, 1, 2, 4)                         # [n, tq, h, 2, dh]
+    t["sq"] = t["sq"].permute(0, 3, 1, 2, 4)
+    t["dk"] = t["dk"].permute(0, 3, 1, 2, 4)
+    t["sk"] = t["sk"].permute(0, 3, 1, 2, 4)
+    t["dv"] = t["dv"].permute(0, 2, 1, 3)                            # [n, tk, hkv, 2 dh]
+    t["sv"] = t["sv"].permute(0, 2, 1, 3)
+    return t
+
+
+def shaped(cs, got):
+    return dict(y=got["y"].to(D), dq=got["dq"].to(D).reshape(cs.n, cs.tq, cs.h, 2, cs.dh),
+                dk=got["dk"].to(D).reshape(cs.n, cs.tk, cs.hkv, 2, cs.dh),
+                dv=got["dv"].to(D).reshape(cs.n, cs.tk, cs.hkv, 2 * cs.dh))
+
+
+def check(cs, got, per_row=False, tol=TOL, what=("dq", "dk", "dv")):
+    """Gradients per block of 64 queries or keys of an image, or per query row
+    and per key, each against tol of its terms' size; y by its norm."""
+    want, got = formulas(cs), shaped(cs, got)
+    assert torch.isfinite(got["y"]).all() and (got["y"] - want["y"]).norm() <= TOL * want["y"].norm()
+    for nm in what:
+        assert torch.isfinite(got[nm]).all(), nm
+        err, size = (got[nm] - want[nm]) ** 2, want["s" + nm[1]] ** 2
+        if per_row:  # each head's, each map's own row
+            bad = (err.sum(-1) > tol ** 2 * size[..., 0]).nonzero()
+            assert not len(bad), (nm, bad[:4].tolist(), float((err.sum(-1) / size[..., 0]).max()) ** 0.5)
+            continue
+        err, size = err.flatten(2).sum(-1), size.flatten(2).sum(-1)
+        for r0 in range(0, err.shape[1], 64):
+            e, s = err[:, r0:r0 + 64].sum(1), size[:, r0:r0 + 64].sum(1)
+            assert (e <= tol ** 2 * s).all(), (nm, r0, float((e / s).max()) ** 0.5)
+
+
+# one for each kernel and sharing of rows and keys of the backward
+PATHS = [
+    ("rows_by_key_64", 1, 2, 2, 64, 100, 300, {}),
+    ("rows_by_key_32", 1, 4, 2, 32, 90, 330, {}),
+    ("rows_by_key_shared_48", 2, 4, 1, 48, 70, 200, dict(causal=True)),
+    ("few_rows", 1, 2, 2, 32, 9, 333, {}),
+    ("four_groups_16", 64, 4, 4, 16, 130, 140, {}),
+    ("four_groups_64", 32, 8, 8, 64, 66, 150, {}),
+    ("joint_one_tile", 3, 2, 2, 32, 50, 64, {}),
+    ("joint_tiles_32", 64, 4, 4, 32, 20, 200, {}),
+    ("joint_tiles_64", 128, 4, 2, 64, 9, 201, dict(causal=True)),
+    ("unaligned", 2, 2, 1, 5, 70, 200, dict(gap=1)),
+]
+NAMES = [p[0] for p in PATHS]
+
+
+def path(p, **kw):
+    return DiffCase(*p[1:7], True, **dict(dict(gap=0), **p[7], **kw))
+
+
+# one for each sharing of the forward: one group of rows, two, four, two waves on
+# a row's keys, split keys, unaligned
+FORWARD = [
+    ("one_group", 3, 4, 2, 32, 10, 150, {}),
+    ("two_groups", 3, 4, 2, 32, 50, 150, {}),
+    ("four_groups", 3, 4, 2, 32, 150, 150, {}),
+    ("halves", 1, 2, 2, 64, 200, 190, {}),
+    ("split", 2, 2, 2, 64, 3, 900, {}),
+    ("split_of_many", 1, 2, 2, 32, 2, 5000, {}),
+    ("unaligned", 2, 2, 2, 5, 40, 90, dict(gap=1)),
+]
+
+
+@pytest.mark.parametrize("factor", [0.0, 2.0 ** -20, 2.0 ** -60])
+@pytest.mark.parametrize("p", PATHS, ids=NAMES)
+def test_a_block_of_small_values(rnn, p, factor):
+    """The first, a middle and the last 64 keys' values times factor, in turn:
+    D_i, a mean over all of a row's keys, is then far above that block's dA."""
+    tk = p[6]
+    for k0 in sorted({0, 64 * (tk // 128), (tk - 1) // 64 * 64}):
+        cs = path(p, seed=k0 + 1)
+        cs.vv[:, k0:k0 + 64] *= factor
+        check(cs, run(rnn, refill(cs)))
+
+
+@pytest.mark.parametrize("p", PATHS, ids=NAMES)
+def test_values_all_zero(rnn, p):
+    cs = path(p, seed=5)
+    cs.vv.zero_()
+    got = run(rnn, refill(cs))
+    for nm in ("y", "dq", "dk"):
+        assert (got[nm] == 0).all(), nm
+    assert torch.isfinite(got["dv"]).all()
