@@ -581,16 +581,6 @@ __global__ __launch_bounds__(256) void diff_join_kernel(DiffArgs g, int splits) 
 // perpendicular to O, so that D_2, whose sum dlambda is, is small beside its
 // terms.  Memory bounds it: 128 x 4 heads of 64, dh 32, 12 us (35 MB).
 template <int LPU>
-__device__ __forceinline__ float group_sum(float v) {
-    v += dpp_f<0xB1>(v);
-    v += dpp_f<0x4E>(v);
-    v += dpp_f<0x141>(v);
-    if (LPU > 8) v += dpp_f<0x140>(v);
-    if (LPU > 16) v = pair16(v, add2);
-    if (LPU > 32) v = pair32(v, add2);
-    return v;
-}
-template <int LPU>
 __device__ __forceinline__ double group_sum(double v) {
     v += rnn_dpp_d<0xB1>(v);
     v += rnn_dpp_d<0x4E>(v);
@@ -664,17 +654,16 @@ __global__ __launch_bounds__(256) void diff_bwd_pre_kernel(DiffArgs g) {
 #pragma unroll
             for (int e = 0; e < E; e++) d[e] = r * ((double)dy[e] * (double)gain[e] - o[e] * t);
         }
-        double d1 = 0.0, d2 = 0.0;
-        float nd = 0.f;
+        double d1 = 0.0, d2 = 0.0, nd = 0.0;  // (a float's square underflows below 1e-19)
 #pragma unroll
         for (int e = 0; e < E; e++) {
             d1 += d[e] * (double)o1[e];
             d2 += d[e] * (double)o2[e];
-            nd += (float)d[e] * (float)d[e];
+            nd += d[e] * d[e];
         }
         d1 = group_sum<LPU>(d1);
         d2 = group_sum<LPU>(d2);
-        nd = sqrtf(group_sum<LPU>(nd));
+        nd = sqrt(group_sum<LPU>(nd));
         float *pd = g.dout + (long long)u * dv + c0;
         if constexpr (VEC) {
             if (in) *(f4 *)pd = f4{(float)d[0], (float)d[1], (float)d[2], (float)d[3]};
@@ -687,7 +676,7 @@ __global__ __launch_bounds__(256) void diff_bwd_pre_kernel(DiffArgs g) {
             const f4 z = {0.f, 0.f, 0.f, 0.f};
             f4 *rec = (f4 *)(g.rec + (long long)u * 8);
             rec[0] = live ? *(const f4 *)(g.statsc + (long long)u * 4) : z;
-            rec[1] = f4{(float)d1, (float)d2, nd, lam};
+            rec[1] = f4{(float)d1, (float)d2, (float)nd, lam};
         }
         dl += d2;
     }

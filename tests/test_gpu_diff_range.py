@@ -165,3 +165,12 @@ def test_values_all_zero(rnn, p):
     for nm in ("y", "dq", "dk"):
         assert (got[nm] == 0).all(), nm
     assert torch.isfinite(got["dv"]).all()
+
+
+@pytest.mark.parametrize("two", [-100, -84, -60, 40])
+@pytest.mark.parametrize("p", PATHS, ids=NAMES)
+def test_gradients_of_any_magnitude(rnn, p, two):
+    """All of dy times a power of two: the gradients' too."""
+    cs = path(p, seed=6)
+    cs.dyv *= 2.0 ** two
+    check(cs, run(rnn, refill(cs)))
