@@ -782,6 +782,12 @@ __device__ __forceinline__ float ds_bound(float nd, float vmax, float dmax) {
 __device__ __forceinline__ float ds_up(float m, float up) {
     return m * up < 2.0f ? up : up_of(m) * 0x1p-14f;
 }
+// From a product of V's and dO's operands to dA times its power of two.  dO of zeros
+// alone leaves the powers where they started, whose product may be infinite: cut off,
+// so that it stays 0 times a number.
+__device__ __forceinline__ float da_unit(float vdown, float ddown, float up) {
+    return fminf(vdown * (ddown * up), 0x1.fffffep127f);
+}
 // The power of two that softmax values, and lambda times them, enter the
 // backward's products with: at most 2^14, so that P_1 - lambda P_2 and P (dA - D)
 // stay below 2^15.
@@ -964,7 +970,7 @@ diff_dq_kernel(DiffArgs g) {
                     for (int m = 0; m < NM; m++) s[m][r] = in ? s[m][r] : 0.f;
                 }
             }
-            const float fd = down_of(vup) * ddown * dsup;
+            const float fd = da_unit(down_of(vup), ddown, dsup);
 #pragma unroll
             for (int m = 0; m < NM; m++) {
                 const float dm = D[m] * dsup;
@@ -1276,7 +1282,7 @@ diff_dkv_kernel(DiffArgs g) {
                 s[r] = in ? s[r] : 0.f;
             }
         }
-        const float fd = vdown * down_of(dup) * sup;
+        const float fd = da_unit(vdown, down_of(dup), sup);
         f32x4 *const mine = &ex[wave][0][lane], *const other = &ex[wave ^ 1][0][lane];
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
@@ -1556,7 +1562,7 @@ diff_bwd_rows_kernel(DiffArgs g) {
             }
             dot_along<Tile>(vt + 32 * kg * Tile::STRIDE, 0, d, da);
             const float f = down_of(kup) * (down_of(qup) * (g.scale * LOG2E));
-            const float fd = down_of(vup) * down_of(dup) * sup;
+            const float fd = da_unit(down_of(vup), down_of(dup), sup);
             const float nm1 = rec[0][row], il1 = rec[1][row] * sgn, nm2 = rec[2][row], il2 = rec[3][row] * sgn;
             f32x16 a;
             auto softmax = [&](int r, float &p1, float &p2) {

@@ -174,3 +174,17 @@ def test_gradients_of_any_magnitude(rnn, p, two):
     cs = path(p, seed=6)
     cs.dyv *= 2.0 ** two
     check(cs, run(rnn, refill(cs)))
+
+
+@pytest.mark.parametrize("p", PATHS, ids=NAMES)
+def test_rows_without_gradient(rnn, p):
+    """dy of zeros, in some rows and in all, with values far from 1."""
+    for part in (slice(0, None, 2), slice(None)):
+        cs = path(p, seed=8, gain=False)
+        cs.vv *= 2.0 ** 60
+        cs.dyv[:, part] = 0.0
+        got = run(rnn, refill(cs))
+        assert (got["dq"][:, part] == 0).all()
+        check(cs, got)
+        if part == slice(None):
+            assert (got["dk"] == 0).all() and (got["dv"] == 0).all()
