@@ -327,7 +327,9 @@ diff_fwd_kernel(DiffArgs g) {
         const int k0 = kbeg + t * TK, k1 = k0 + 32 * S2 * half;
         __syncthreads();
         const _Float16 *const kt = lds[t & 1] + 32 * S2 * half * Tile::STRIDE, *const vt = kt + Tile::HALVES;
-        const float f = down_of(kup1) * qdown, turn = down_of(vup) * vup1;
+        // (f stays above 0, so that a hidden score, -infinity, stays hidden: where it
+        // would be smaller, all scores are 0 to the last bit of an exponential)
+        const float f = fmaxf(down_of(kup1) * qdown, 0x1p-120f), turn = down_of(vup) * vup1;
         vup = vup1;
         if (t + 1 < ntile) stage(t + 1);
         if (t + 2 < ntile) st.load(k0 + 2 * TK);

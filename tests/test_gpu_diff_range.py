@@ -188,3 +188,14 @@ def test_rows_without_gradient(rnn, p):
         check(cs, got)
         if part == slice(None):
             assert (got["dk"] == 0).all() and (got["dv"] == 0).all()
+
+
+@pytest.mark.parametrize("p", PATHS, ids=NAMES)
+def test_tiny_queries_and_keys(rnn, p):
+    """Scores below the smallest float: every key that is seen weighs the same,
+    also where a mask or the last tile's end hides some."""
+    for opt in (dict(), dict(causal=True), dict(klen=[max(1, p[6] - 3)] * p[1])):
+        cs = path(p, seed=9, **opt) if not p[7].get("causal") else path(p, seed=9)
+        cs.qv *= 2.0 ** -70
+        cs.kvv *= 2.0 ** -70
+        check(cs, run(rnn, refill(cs)))
