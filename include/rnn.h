@@ -278,8 +278,10 @@ int rnn_rotary(rnn_ctx *ctx, const rnn_rotary_desc *d, size_t n, size_t t, const
  * arrays; NULL: tq, tk): rows behind them are padding, which is never read and
  * may hold anything.  causal: query i sees keys j <= i + (keys - queries), the
  * two sequences aligned at their ends; mask_diag: not key j = i.  A query that
- * sees no key, and a padding query, give y = 0.  The values that are read are
- * finite.  Products are taken in two fp16 parts under a power of two (of a row, of
+ * sees no key, and a padding query, give y = 0.  A NaN or an infinity gives NaN:
+ * in a query to its row, in a key to every row that sees it, in a value to rows
+ * that do not see it as well, in dy to its row of dq and to what sums over rows.
+ * Products are taken in two fp16 parts under a power of two (of a row, of
  * a tile, or in sums of all tiles so far): elements down to 2^-12 of the largest
  * keep 2^-23 of themselves, smaller ones 2^-35 of the largest. */
 typedef struct {

@@ -414,7 +414,7 @@ diff_fwd_kernel(DiffArgs g) {
                     o[c][r] = __builtin_fmaf(o[c][r], x, e[(c * 16 + r) * 64] * y);
         }
     }
-    const bool some = live && l > 0.f;
+    const bool some = live && !(l <= 0.f);  // (a NaN, of a query or a key, stays one)
     const float il = some ? down_of(vup) / l : 0.f;  // both carry 2^6
 #pragma unroll
     for (int c = 0; c < CT; c++)
@@ -512,11 +512,13 @@ __global__ __launch_bounds__(256) void diff_join_kernel(DiffArgs g, int splits) 
     const int hd = (int)(w % g.h), dv = 2 * g.dh;
     const f4 st = lane < splits ? *(const f4 *)(g.pstat + (w * splits + lane) * 4)
                                 : f4{NO_MAX, 0.f, NO_MAX, 0.f};
-    const float M0 = wave_max(st[1] > 0.f ? st[0] : NO_MAX);
-    const float M1 = wave_max(st[3] > 0.f ? st[2] : NO_MAX);
-    const float w0 = st[1] > 0.f ? st[1] * __builtin_amdgcn_exp2f(st[0] - M0) : 0.f;
-    const float w1 = st[3] > 0.f ? st[3] * __builtin_amdgcn_exp2f(st[2] - M1) : 0.f;
+    // (not "above 0": a NaN stays one)
+    const bool has0 = !(st[1] <= 0.f), has1 = !(st[3] <= 0.f);
+    const float M0 = wave_max(has0 ? st[0] : NO_MAX), M1 = wave_max(has1 ? st[2] : NO_MAX);
+    const float w0 = has0 ? st[1] * __builtin_amdgcn_exp2f(st[0] - M0) : 0.f;
+    const float w1 = has1 ? st[3] * __builtin_amdgcn_exp2f(st[2] - M1) : 0.f;
     const float t0 = wave_sum(w0), t1 = wave_sum(w1);
+    const bool some0 = !(t0 <= 0.f), some1 = !(t1 <= 0.f);
     f2 o0 = {0.f, 0.f}, o1 = o0;
     const int c = 2 * lane;
     // (every lane goes along, since it hands its split's weights to the others; those
@@ -552,8 +554,8 @@ __global__ __launch_bounds__(256) void diff_join_kernel(DiffArgs g, int splits) 
             o1 += sums[wave + i][1][lane];
         }
     }
-    o0 *= t0 > 0.f ? 1.0f / t0 : 0.f;
-    o1 *= t1 > 0.f ? 1.0f / t1 : 0.f;
+    o0 *= some0 ? 1.0f / t0 : 0.f;
+    o1 *= some1 ? 1.0f / t1 : 0.f;
     const float lam = lane_lambda(g, hd);
     f2 out = o0 - lam * o1;
     float rn = 1.0f;
@@ -572,8 +574,8 @@ __global__ __launch_bounds__(256) void diff_join_kernel(DiffArgs g, int splits) 
         }
     }
     if (g.stats && lane == 0)
-        *(f4 *)(g.stats + w * 4) = f4{t0 > 0.f ? M0 : 0.f, t0 > 0.f ? P_UP / t0 : 0.f,
-                                      t1 > 0.f ? M1 : 0.f, t1 > 0.f ? P_UP / t1 : 0.f};
+        *(f4 *)(g.stats + w * 4) = f4{some0 ? M0 : 0.f, some0 ? P_UP / t0 : 0.f,
+                                      some1 ? M1 : 0.f, some1 ? P_UP / t1 : 0.f};
 }
 
 // Backward's first pass: dO, D_1 and D_2 of every (row, head), and the block's

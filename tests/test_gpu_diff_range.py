@@ -199,3 +199,50 @@ def test_tiny_queries_and_keys(rnn, p):
         cs.qv *= 2.0 ** -70
         cs.kvv *= 2.0 ** -70
         check(cs, run(rnn, refill(cs)))
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("f", FORWARD, ids=[f[0] for f in FORWARD])
+def test_what_is_not_finite_shows(rnn, f, bad):
+    """A NaN or an infinity in a query, or in a key, of either map: NaN in every
+    row that takes it, of that key head's query heads alone."""
+    g = f[2] // f[3]
+    clean = run(rnn, path(f, seed=12), train=False)["y"]
+    view = lambda y: y.view(f[1], f[5], f[2], 2 * f[4])
+    for m in range(2):
+        cs = path(f, seed=12)
+        cs.qv[0, 1, 1, m, 2] = bad
+        y = view(run(rnn, refill(cs), train=False)["y"])
+        assert torch.isnan(y[0, 1, 1]).all(), ("query", m)
+        y[0, 1, 1] = view(clean)[0, 1, 1]
+        assert torch.equal(y, view(clean)), ("query", m)
+        for key in (0, f[6] // 2, f[6] - 1):
+            cs = path(f, seed=12)
+            cs.kvv[0, key, 1, m, 2] = bad
+            got = run(rnn, refill(cs))
+            y = view(got["y"])
+            assert torch.isnan(y[0, :, g:2 * g]).all(), ("key", m, key)
+            dq = got["dq"].view(f[1], f[5], f[2], -1)
+            assert not torch.isfinite(dq[0, :, g:2 * g]).any(), ("dq", m, key)
+            y[0, :, g:2 * g] = view(clean)[0, :, g:2 * g]
+            assert torch.equal(y, view(clean)), ("key", m, key)
+
+
+@pytest.mark.parametrize("f", FORWARD, ids=[f[0] for f in FORWARD])
+def test_hidden_keys_that_are_not_finite(rnn, f):
+    """Keys (not values) that a mask hides from a row may hold anything finite
+    or not: causal rows before such a key stay as they were, to the rounding of
+    another power of two."""
+    if f[5] < 40:
+        pytest.skip("every row sees the key")
+    for bad in (float("nan"), float("inf")):
+        cs = path(f, seed=13, causal=True)
+        want = formulas(cs)["y"]
+        key = f[6] - 8
+        cs.kvv[0, key] = bad
+        y = run(rnn, refill(cs), train=False)["y"].to(D)
+        # query i sees keys up to i + tk - tq
+        blind = key - (f[6] - f[5])
+        err = (y[0, :blind] - want[0, :blind]).norm()
+        assert err <= TOL * want[0, :blind].norm()
+        assert torch.isnan(y[0, blind:]).all()
