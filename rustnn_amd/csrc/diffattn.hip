@@ -120,7 +120,8 @@ struct RowFrag {
 // Softmax values enter the products times 2^6, relative to a reference that a row's
 // largest score may pass by 2^8 before it moves: at most 2^14.
 constexpr float P_UP = 64.0f, P_EXP = 6.0f, SLACK = 8.0f;
-constexpr float NO_MAX = -1e30f;                 // a running maximum before any score
+constexpr float NO_MAX = -0x1.fffffep127f;       // a running maximum before any score
+constexpr float FAR_SCORE = 0x1p17f;             // a maximum whose own rounding shows in 2^x
 
 // Lambda of a lane's own head: the wave's one head together, else each lane its
 // own.
@@ -255,7 +256,7 @@ __global__ __launch_bounds__(128 * QG * KH)
 __attribute__((amdgpu_waves_per_eu(QG * KH == 4 || (QG == 2 && DHP <= 32) ? 2 : 1))) void
 diff_fwd_kernel(DiffArgs g) {
     constexpr int W = 2 * DHP, TK = QG * KH < 4 && DHP > 32 ? 32 : 64, NT = 128 * QG * KH, KS = DHP / 16;
-    constexpr int CT = DHP / 16, S2 = TK / 32 / KH, HALF = (CT * 16 + 2) * 64;
+    constexpr int CT = DHP / 16, S2 = TK / 32 / KH, HALF = (CT * 16 + 3) * 64;
     using Tile = HalfTile<TK, W>;
     static_assert(8 * Tile::HALVES >= 4 * ((KH - 1) * 2 * QG * HALF + QG * CT * 16 * 64) && (KH == 1 || !SPLIT), "exchange");
     __shared__ __align__(16) _Float16 lds[2][2 * Tile::HALVES];
@@ -297,7 +298,8 @@ diff_fwd_kernel(DiffArgs g) {
     for (int c = 0; c < CT; c++)
 #pragma unroll
         for (int r = 0; r < 16; r++) o[c][r] = 0.f;
-    float m = NO_MAX, l = 0.f;
+    // the softmax reference, the sum, and the largest score itself
+    float m = NO_MAX, l = 0.f, mtop = NO_MAX;
     // the largest key so far, and powers of two of the tile that is staged; the
     // output is in the values' unit
     float kmax = 0.f, kup1 = 1.f, vup1 = FIRST_UP, vup = FIRST_UP;
@@ -359,6 +361,7 @@ diff_fwd_kernel(DiffArgs g) {
             for (int r = 0; r < 16; r += 2) top = max3(top, u[s2][r], u[s2][r + 1]);
         // (a score times f: f > 0 keeps the order)
         top = pair32(top, max2) * f;
+        mtop = max2(mtop, top);
         // the reference moves where a score passes it by the slack, the output's
         // unit where the tile's does; both rarely after the first tile
         const bool moves = top > m + SLACK;
@@ -371,14 +374,25 @@ diff_fwd_kernel(DiffArgs g) {
 #pragma unroll
                 for (int r = 0; r < 16; r++) o[c][r] *= keep;
         }
-        const float base = P_EXP - m;
+        float fe = f, base = P_EXP - m;
+        // far from 0 the reference is taken off the rounded score: off the exact one, as
+        // a fused multiply-add does it, what its rounding left would be an exponent
+        const bool far = fabsf(m) > FAR_SCORE && m != NO_MAX;
+        if (__any(far)) {
+#pragma unroll
+            for (int s = 0; s < S2; s++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) u[s][r] = far ? u[s][r] * f - m : u[s][r];
+            fe = far ? 1.0f : f;
+            base = far ? P_EXP : base;
+        }
         Half2 p[2 * S2];
         float ps[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = 0; s < S2; s++) {
 #pragma unroll
             for (int r = 0; r < 16; r++) {
-                u[s][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(u[s][r], f, base));
+                u[s][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(u[s][r], fe, base));
                 ps[r & 3] += u[s][r];
             }
             split16(u[s], *(Half2(*)[2]) & p[2 * s]);
@@ -400,6 +414,7 @@ diff_fwd_kernel(DiffArgs g) {
                 for (int r = 0; r < 16; r++) e[(c * 16 + r) * 64] = o[c][r];
             e[CT * 16 * 64] = m;
             e[CT * 16 * 64 + 64] = l;
+            e[CT * 16 * 64 + 128] = mtop;
         }
         __syncthreads();
         if (!half) {
@@ -407,6 +422,7 @@ diff_fwd_kernel(DiffArgs g) {
             const float x = __builtin_amdgcn_exp2f(m - top), y = __builtin_amdgcn_exp2f(m2 - top);
             l = l * x + e[CT * 16 * 64 + 64] * y;
             m = top;
+            mtop = max2(mtop, e[CT * 16 * 64 + 128]);
 #pragma unroll
             for (int c = 0; c < CT; c++)
 #pragma unroll
@@ -414,13 +430,19 @@ diff_fwd_kernel(DiffArgs g) {
                     o[c][r] = __builtin_fmaf(o[c][r], x, e[(c * 16 + r) * 64] * y);
         }
     }
-    const bool some = live && !(l <= 0.f);  // (a NaN, of a query or a key, stays one)
+    // whether the row sees a key (of the split): its sum is then above 0, or no number
+    // for want of one
+    const int seen = min(kend, g.causal ? qi + shift + 1 : nk) - kbeg;
+    const bool some = live && seen > (g.diag && qi >= kbeg && qi < kbeg + seen ? 1 : 0);
     const float il = some ? down_of(vup) / l : 0.f;  // both carry 2^6
 #pragma unroll
     for (int c = 0; c < CT; c++)
 #pragma unroll
         for (int r = 0; r < 16; r++) o[c][r] = some ? o[c][r] * il : 0.f;
-    if (!some) m = 0.f;
+    // the statistics kept are relative to the largest score itself, so that the
+    // backward's exponentials are at most 1
+    l *= __builtin_amdgcn_exp2f(m - mtop);
+    m = some ? mtop : 0.f;
     const int dv = 2 * g.dh;
     const long long out = ((long long)b * g.tq + qi) * g.h + head;  // (image, query, head)
     if constexpr (SPLIT) {
@@ -792,6 +814,11 @@ __device__ __forceinline__ float ds_up(float m, float up) {
 __device__ __forceinline__ float da_unit(float vdown, float ddown, float up) {
     return fminf(vdown * (ddown * up), 0x1.fffffep127f);
 }
+// A softmax value before its row's reciprocal sum, from a score less the largest: at
+// most 1, also where a score's error passes an exponent (v_exp_f32 cuts it off itself).
+__device__ __forceinline__ float exp_below(float x) {
+    return __builtin_amdgcn_fmed3f(__builtin_amdgcn_exp2f(x), 0.0f, 1.0f);
+}
 // The power of two that softmax values, and lambda times them, enter the
 // backward's products with: at most 2^14, so that P_1 - lambda P_2 and P (dA - D)
 // stay below 2^15.
@@ -961,7 +988,7 @@ diff_dq_kernel(DiffArgs g) {
                 const float f = kdown * qdown[m];
 #pragma unroll
                 for (int r = 0; r < 16; r++)
-                    s[m][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[m][r], f, nm[m])) * il[m];
+                    s[m][r] = exp_below(__builtin_fmaf(s[m][r], f, nm[m])) * il[m];
             }
             const bool whole = k1 + 32 <= nk && !(g.causal && k1 + 31 > w_first + shift) &&
                                !(g.diag && k1 <= w_last && w_first < k1 + 32);
@@ -1272,7 +1299,7 @@ diff_dkv_kernel(DiffArgs g) {
             const f32x4 m4 = *(const f32x4 *)&rc[0][2 * r + 4 * lh], l4 = *(const f32x4 *)&rc[1][2 * r + 4 * lh];
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                s[r + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + e], f, m4[e])) * l4[e];
+                s[r + e] = exp_below(__builtin_fmaf(s[r + e], f, m4[e])) * l4[e];
         }
         // rows past the last carry il = 0, keys past the last are not stored
         const bool whole = !(g.causal && w_first + 31 > tq0 + shift) &&
@@ -1572,8 +1599,8 @@ diff_bwd_rows_kernel(DiffArgs g) {
             auto softmax = [&](int r, float &p1, float &p2) {
                 const int j = k0 + 32 * kg + 8 * (r >> 2) + 4 * lh + (r & 3);
                 const bool in = j < nk && !(g.causal && j > qi + shift) && !(g.diag && j == qi);
-                p1 = in ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], f, nm1)) * il1 : 0.f;
-                p2 = in ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[1][r], f, nm2)) * il2 : 0.f;
+                p1 = in ? exp_below(__builtin_fmaf(s[0][r], f, nm1)) * il1 : 0.f;
+                p2 = in ? exp_below(__builtin_fmaf(s[1][r], f, nm2)) * il2 : 0.f;
                 a[r] = p1 + p2;
             };
             if constexpr (ONE) {

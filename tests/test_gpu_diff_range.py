@@ -246,3 +246,36 @@ def test_hidden_keys_that_are_not_finite(rnn, f):
         err = (y[0, :blind] - want[0, :blind]).norm()
         assert err <= TOL * want[0, :blind].norm()
         assert torch.isnan(y[0, blind:]).all()
+
+
+@pytest.mark.parametrize("f", FORWARD, ids=[f[0] for f in FORWARD])
+def test_scores_far_below_zero(rnn, f):
+    """Every score about -2^112: the largest still takes all.  Key j's is
+    -(tk - j + 2) 2^100 or so, exact in its leading bits: the last key wins by
+    2^100 over a score's error of 2^-22 2^112."""
+    cs = path(f, seed=14, gain=False)
+    tk = f[6]
+    cs.qv.zero_()
+    cs.kvv.zero_()
+    cs.qv[..., 1] = 2.0 ** 50
+    cs.kvv[..., 1] = -(2.0 ** 50) * (tk + 2.0 - torch.arange(tk).view(1, -1, 1, 1))
+    cs.scale = 1.0
+    y = run(rnn, refill(cs), train=False)["y"].to(D)
+    want = formulas(cs)["y"]
+    assert (y - want).norm() <= TOL * want.norm()
+
+
+@pytest.mark.parametrize("two", [12, 20, 26, 60, 110])
+@pytest.mark.parametrize("f", FORWARD, ids=[f[0] for f in FORWARD])
+def test_large_scores(rnn, f, two):
+    """Scores far apart and of any size: the largest takes all (the two largest of
+    these are some 2^two / 16 apart, a score's error 2^-22 of it), and gradients
+    stay numbers."""
+    cs = path(f, seed=16, gain=False)
+    cs.qv *= 2.0 ** (two // 2)
+    cs.kvv *= 2.0 ** (two - two // 2)
+    got = run(rnn, refill(cs))
+    want = formulas(cs)["y"]
+    assert (got["y"].to(D) - want).norm() <= TOL * want.norm()
+    for nm in ("dq", "dk", "dv", "dlam"):
+        assert torch.isfinite(got[nm]).all(), nm
