@@ -121,6 +121,7 @@ struct RowFrag {
 // largest score may pass by 2^8 before it moves: at most 2^14.
 constexpr float P_UP = 64.0f, P_EXP = 6.0f, SLACK = 8.0f;
 constexpr float NO_MAX = -0x1.fffffep127f;       // a running maximum before any score
+constexpr float SQUARES_MAX = 0x1p120f;          // a norm's sum of squares that has not overflowed
 constexpr float FAR_SCORE = 0x1p17f;             // a maximum whose own rounding shows in 2^x
 
 // Lambda of a lane's own head: the wave's one head together, else each lane its
@@ -512,7 +513,20 @@ diff_fwd_kernel(DiffArgs g) {
     float rn = 1.0f;
     if (g.gain) {
         ss = pair32(ss, add2);
-        rn = (1.0f / sqrtf(ss / (float)dv + g.eps)) * (1.0f - g.lam_init);
+        rn = 1.0f / sqrtf(ss / (float)dv + g.eps);
+        if (__any(ss > SQUARES_MAX)) {  // again from values 2^-64 their size
+            float sm = 0.f;
+#pragma unroll
+            for (int c = 0; c < CT; c++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const float x = o[c][r] * 0x1p-64f;
+                    sm += x * x;
+                }
+            sm = pair32(sm, add2);
+            if (ss > SQUARES_MAX) rn = 0x1p-64f / sqrtf(sm / (float)dv + g.eps * 0x1p-128f);
+        }
+        rn *= 1.0f - g.lam_init;
         store(g.y + out * dv, [&](int c, int r, int) { return o[c][r] * rn * gv[c][r]; });
     } else {
         store(g.y + out * dv, [&](int c, int r, int) { return o[c][r]; });
@@ -584,7 +598,13 @@ __global__ __launch_bounds__(256) void diff_join_kernel(DiffArgs g, int splits) 
     f2 gn = {1.f, 1.f};
     if (g.gain) {
         const float ss = wave_sum(c < dv ? out[0] * out[0] + out[1] * out[1] : 0.f);
-        rn = (1.0f / sqrtf(ss / (float)dv + g.eps)) * (1.0f - g.lam_init);
+        rn = 1.0f / sqrtf(ss / (float)dv + g.eps);
+        if (ss > SQUARES_MAX) {
+            const f2 x = out * 0x1p-64f;
+            const float sm = wave_sum(c < dv ? x[0] * x[0] + x[1] * x[1] : 0.f);
+            rn = 0x1p-64f / sqrtf(sm / (float)dv + g.eps * 0x1p-128f);
+        }
+        rn *= 1.0f - g.lam_init;
         if (c < dv) gn = f2{g.gain[c], g.gain[c + 1]};
     }
     if (c < dv) {

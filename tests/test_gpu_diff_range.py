@@ -265,6 +265,15 @@ def test_scores_far_below_zero(rnn, f):
     assert (y - want).norm() <= TOL * want.norm()
 
 
+@pytest.mark.parametrize("two", [-80, 40, 80])
+@pytest.mark.parametrize("f", FORWARD, ids=[f[0] for f in FORWARD])
+def test_norm_of_any_magnitude(rnn, f, two):
+    """Values far from 1 under the norm: mean O^2 passes a float's range (2^160)."""
+    cs = path(f, seed=15)
+    cs.vv *= 2.0 ** two
+    check(cs, run(rnn, refill(cs)))
+
+
 @pytest.mark.parametrize("two", [12, 20, 26, 60, 110])
 @pytest.mark.parametrize("f", FORWARD, ids=[f[0] for f in FORWARD])
 def test_large_scores(rnn, f, two):
