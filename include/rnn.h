@@ -284,8 +284,11 @@ int rnn_rotary(rnn_ctx *ctx, const rnn_rotary_desc *d, size_t n, size_t t, const
  * So do scores past a float's range.  The backward forms P again from scores that
  * are within 2^-22 of themselves: those above 2^15 leave it few bits.
  * Products are taken in two fp16 parts under a power of two (of a row, of
- * a tile, or in sums of all tiles so far): elements down to 2^-12 of the largest
- * keep 2^-23 of themselves, smaller ones 2^-35 of the largest. */
+ * a tile, or in sums of all tiles so far; dS of its own row in dq, its own key in
+ * dkv): elements down to 2^-12 of the largest keep 2^-23 of themselves, smaller
+ * ones 2^-35 of the largest.  Sums are fp32: dq, a sum over the keys, is within
+ * some 2^-24 sqrt(3 tk / 16) of its terms' size besides (3e-7 at 256 keys, 2e-6
+ * measured at 65536). */
 typedef struct {
     uint32_t h, hkv, dh, tq, tk;
     size_t qstride, qoff, kvstride, koff, voff;

@@ -813,9 +813,8 @@ __device__ __forceinline__ void bwd_params(const DiffArgs &g, int blk, double *r
 // The power of two of dA - D for rows with |dO| <= nd and values of magnitude <=
 // vmax, from m = ds_bound >= |dA| + |D| (|dA| <= nd sqrt(W) vmax; D, a mean of dA over
 // all of the row's keys, may be far above it where vmax is of some of them alone): it
-// takes m to [1, 2), and stays as it was (up) until m times it passes 2.
-// Without sticky_up's slack: the bound is a hundred times what dA mostly is, and P
-// far below 1, so that another 2^-4 would leave dS 2^-19 of itself.
+// takes m to [1, 2), and stays as it was (up) until m times it passes 2.  It keeps dS
+// within a float's range and no more: ds_fit has the bits of its two parts.
 template <int W>
 __device__ __forceinline__ constexpr float ds_root() {
     return W == 32 ? 11.313709f : W == 64 ? 16.0f : W == 96 ? 19.595918f : 22.627417f;
@@ -839,10 +838,45 @@ __device__ __forceinline__ float da_unit(float vdown, float ddown, float up) {
 __device__ __forceinline__ float exp_below(float x) {
     return __builtin_amdgcn_fmed3f(__builtin_amdgcn_exp2f(x), 0.0f, 1.0f);
 }
-// The power of two that softmax values, and lambda times them, enter the
-// backward's products with: at most 2^14, so that P_1 - lambda P_2 and P (dA - D)
-// stay below 2^15.
-__device__ __forceinline__ float p_up(float lam) { return up_of(fmaxf(1.0f, lam)) * 0.5f; }
+// The power of two that softmax values, and lambda times them, enter the backward's
+// products with, from the largest of them in the rows: they come to at most 2^14, so
+// that P_1 - lambda P_2 stays below 2^15.
+__device__ __forceinline__ float p_up(float pmax) { return up_of(pmax) * 0.5f; }
+
+// The power of two of a lane's dS, its row's in dQ or its key's in dK, on top of what
+// bounds say: it follows the largest magnitude so far as sticky_up does, and the
+// lane's accumulators with it.  Bounds alone left dS an error in proportion to the
+// keys (P falls with them, and |dA| is a hundredth of its bound), 9e-6 of dQ and dK
+// at 65536 keys, and with any outlier of V; now dK is 3e-7 off there, and dQ 2e-6, by
+// the length of its sums.  It costs eight instructions a map and tile, sixteen more
+// in dK, and a branch that is rarely taken: 2 x 8 causal heads of 1568, dh 64, dQ 107
+// us and dK, dV 179 against 105 and 171 without; 4 x 8 of 2048 490 and 559 against
+// 453 and 558.
+constexpr float DS_START = 0x1p108f;  // (dS is at most 2^15 before it)
+// The largest magnitude, which ds_fit is called for from 2^15 on.
+__device__ __forceinline__ float absmax16(const f32x16 &s) {
+    float m = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; r += 2) m = max3abs(m, s[r], s[r + 1]);
+    return m;
+}
+// Takes m, the lane's largest |dS|, to [2^10, 2^11) where it is past 2^15; the factor.
+__device__ __forceinline__ float ds_fit(f32x16 &s, float &m, float &up) {
+    m = pair32(m, max2);
+    const float f = m >= 0x1p15f ? up_of(m) * 0x1p-4f : 1.0f;
+#pragma unroll
+    for (int r = 0; r < 16; r++) s[r] *= f;
+    up *= f;
+    m *= f;
+    return f;
+}
+template <int C>
+__device__ __forceinline__ void scale_all(f32x16 (&acc)[C], float f) {
+#pragma unroll
+    for (int c = 0; c < C; c++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) acc[c][r] *= f;
+}
 
 // The matrix core's sum is cut off towards -inf, which leaves every element of
 // a long sum a little low.  Two thirds of the way (where a sum that grows with
@@ -922,13 +956,15 @@ diff_dq_kernel(DiffArgs g) {
         for (int m = 0; m < NM; m++) qdown[m] = qf[m].split(q[m]) * (g.scale * LOG2E);
         ddown = df.split(d);
     }
-    const float pup = p_up(fabsf(dd[3])), dmax = max2(fabsf(dd[0]), fabsf(dd[1]));
-    float nm[NM], il[NM], D[NM];
+    const float pup = p_up(max2(sm[1], fabsf(sm[3] * dd[3])));
+    const float dmax = max2(fabsf(dd[0]), fabsf(dd[1]));
+    float nm[NM], il[NM], D[NM], own[NM];  // own: dS's power of two, on top of P's
 #pragma unroll
     for (int m = 0; m < NM; m++) {
         const bool second = map + m;
         nm[m] = second ? -sm[2] : -sm[0];
-        il[m] = (second ? sm[3] * dd[3] : sm[1]) * pup;
+        own[m] = DS_START;
+        il[m] = (second ? sm[3] * dd[3] : sm[1]) * pup * DS_START;
         D[m] = second ? -dd[1] : -dd[0];
     }
     f32x16 acc[NM][CT];
@@ -978,13 +1014,9 @@ diff_dq_kernel(DiffArgs g) {
             for (int m = 0; m < NM; m++) il[m] = -il[m];
             ratio = -ratio;
         }
-        if (t && __any(ratio != 1.0f)) {
-#pragma unroll
-            for (int m = 0; m < NM; m++)
-#pragma unroll
-                for (int c = 0; c < CT; c++)
-#pragma unroll
-                    for (int r = 0; r < 16; r++) acc[m][c][r] *= ratio;
+        if (NM == 1 && __any(ratio != 1.0f)) {  // (with one map, registers are short below)
+            scale_all(acc[0], ratio);
+            ratio = 1.0f;
         }
         if (t + 1 < ntile) stage(t + 1);
         if (t + 2 < ntile) st.load(k0 + 2 * TK);
@@ -1022,11 +1054,26 @@ diff_dq_kernel(DiffArgs g) {
                 }
             }
             const float fd = da_unit(down_of(vup), ddown, dsup);
+            float mx[NM];
+            bool past = NM > 1 && ratio != 1.0f;
 #pragma unroll
             for (int m = 0; m < NM; m++) {
                 const float dm = D[m] * dsup;
 #pragma unroll
                 for (int r = 0; r < 16; r++) s[m][r] *= __builtin_fmaf(da[r], fd, dm);
+                mx[m] = absmax16(s[m]);
+                past = past || mx[m] >= 0x1p15f;
+            }
+            if (__builtin_expect(__any(past), 0)) {
+#pragma unroll
+                for (int m = 0; m < NM; m++) {
+                    const float f = ds_fit(s[m], mx[m], own[m]);
+                    il[m] *= f;
+                    scale_all(acc[m], NM > 1 ? f * ratio : f);
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < NM; m++) {
                 Half2 ds[2];
                 split16(s[m], ds);
 #pragma unroll
@@ -1037,6 +1084,9 @@ diff_dq_kernel(DiffArgs g) {
         }
         if (t + 2 < ntile) maxima(t & 1);
     }
+    // (dS's own powers of two come off first: waves that share rows have different ones)
+#pragma unroll
+    for (int m = 0; m < NM; m++) scale_all(acc[m], down_of(own[m]));
     if constexpr (KG > 1) {
         __syncthreads();
         float *const ex = (float *)lds + (rg * 2 + map) * CT * 16 * 64 + lane;
@@ -1088,8 +1138,8 @@ diff_dkv_kernel(DiffArgs g) {
     __shared__ __align__(16) _Float16 lds[2][2 * Tile::HALVES + 32];
     // -m1, il1, -m2, -lambda il2, -D1, -D2, with their powers of two
     __shared__ __align__(16) float rec[2][6][TR];
-    // largest |q|, |dO|, |dO|_2, |lambda| of a tile past what is known of them; with
-    // |dO|_2's, the largest |D_m|
+    // largest |q|, |dO|, |dO|_2 and P (or lambda times it) of a tile past what is known
+    // of them; with |dO|_2's, the largest |D_m|
     __shared__ f4 tmax[2][NW];
     __shared__ float tdmax[2];
     __shared__ float vmaxs[NW];
@@ -1166,8 +1216,9 @@ diff_dkv_kernel(DiffArgs g) {
         }
         next(lq0, lx0);
     };
-    // the largest value and lambda so far, the powers of two of the tile that is
-    // staged (.1) and of the one that is computed
+    // the largest value and P so far, the powers of two of the tile that is staged (.1)
+    // and of the one that is computed; the lane's own of dS
+    float sown = DS_START;
     float vmax = INFINITY, ml = 0.f, qup1 = FIRST_UP, dup1 = FIRST_UP, pup1 = 1.f, sup1 = FIRST_UP;
     float qup = FIRST_UP, dup = FIRST_UP, pup = 1.f, sup = FIRST_UP;
     auto maxima = [&](int slot) {
@@ -1189,7 +1240,7 @@ diff_dkv_kernel(DiffArgs g) {
                 m[2] = wave_max(r1[2]);
                 dall = wave_max(dm);
             }
-            m[3] = wave_over(fabsf(r1[3]), ml);
+            m[3] = wave_over(max2(r0[1], fabsf(r0[3] * r1[3])), ml);
             if (lane == 0) tdmax[slot] = dall;
         }
         if (lane == 0) tmax[slot][wave] = m;
@@ -1292,15 +1343,6 @@ diff_dkv_kernel(DiffArgs g) {
             rv = -rv;
             rk = -rk;
         }
-        if (t && (rv != 1.0f || rk != 1.0f)) {
-#pragma unroll
-            for (int r = 0; r < 16; r++) {
-#pragma unroll
-                for (int c = 0; c < CT; c++) dk[c][r] *= rk;
-#pragma unroll
-                for (int c = 0; c < VT; c++) dv[c][r] *= rv;
-            }
-        }
         if (t + 1 < ntile) stage(t + 1);
         if (t + 2 < ntile) load();
         const int tq0 = cq0, x0 = cx0;
@@ -1347,34 +1389,36 @@ diff_dkv_kernel(DiffArgs g) {
             mine[16 * r + 256] = d;
         }
         __syncthreads();
-        {
-            // P_1 - lambda P_2 (P_2's sign is in its rec) and dA, the same in both waves
-            f32x16 a;
+        // P_1 - lambda P_2 (P_2's sign is in its rec) and dA, the same in both waves
+        f32x16 a;
 #pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const f32x4 p = other[16 * r], d = other[16 * r + 256];
+        for (int r = 0; r < 16; r += 4) {
+            const f32x4 p = other[16 * r], d = other[16 * r + 256];
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    a[r + e] = s[r + e] + p[e];
-                    da[r + e] += d[e];
-                }
+            for (int e = 0; e < 4; e++) {
+                a[r + e] = s[r + e] + p[e];
+                da[r + e] += d[e];
             }
-            Half2 ah[2];
-            split16(a, ah);
-#pragma unroll
-            for (int c = 0; c < VT; c++)
-                if (VT * 32 * 2 == W || map * VT + c < W / 32)
-                    dot_across<Tile>(dt, 32 * (map * VT + c), ah, dv[c]);
         }
         rc = &rec[t & 1][4 + map];
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
             const f32x4 D = *(const f32x4 *)&rc[0][2 * r + 4 * lh];
 #pragma unroll
-            for (int e = 0; e < 4; e++) s[r + e] *= __builtin_fmaf(da[r + e], fd, D[e]);
+            for (int e = 0; e < 4; e++) s[r + e] *= __builtin_fmaf(da[r + e], fd, D[e]) * sown;
+        }
+        float mx = absmax16(s);
+        if (__builtin_expect(__any(mx >= 0x1p15f || rk != 1.0f || rv != 1.0f), 0)) {
+            scale_all(dk, ds_fit(s, mx, sown) * rk);
+            scale_all(dv, rv);
         }
         {
-            Half2 ds[2];
+            Half2 ah[2], ds[2];
+            split16(a, ah);
+#pragma unroll
+            for (int c = 0; c < VT; c++)
+                if (VT * 32 * 2 == W || map * VT + c < W / 32)
+                    dot_across<Tile>(dt, 32 * (map * VT + c), ah, dv[c]);
             split16(s, ds);
 #pragma unroll
             for (int c = 0; c < CT; c++) dot_across<Tile>(qt, map * DHP + 32 * c, ds, dk[c]);
@@ -1387,6 +1431,7 @@ diff_dkv_kernel(DiffArgs g) {
     float *vd = g.dkv + krow * g.kvstride + g.voff + 2 * kh * g.dh;
     const float sgn = ntile > flip ? -1.0f : 1.0f;
     const float fk = down_of(qup) * (g.scale * sgn), fk2 = down_of(pup) * down_of(sup);
+    scale_all(dk, down_of(sown));
 #pragma unroll
     for (int c = 0; c < CT; c++)
         put_channels<VEC>(kd, g.dh, 32 * c, dk[c], fk, fk2, live, g.acc_kv);
@@ -1435,9 +1480,10 @@ diff_bwd_rows_kernel(DiffArgs g) {
     __shared__ __align__(16) _Float16 lds[4][SLOT];  // K, V, Q, dO
     __shared__ float rec[6][64];  // as in diff_dkv_kernel
     __shared__ f4 rmax[4];
-    __shared__ float rdmax[4];
+    __shared__ float rdo[64];  // |dO|_2 of the rows
     __shared__ f2 tmax[4];
     __shared__ f4 psum[2][ONE ? 64 : 1];  // sums of P_m and of P_m dA over 32 keys
+    __shared__ f2 smax[4];                // largest |dS_m| of a wave's part of the tile
     const int np = params_blocks(g);
     if ((int)blockIdx.x < np) {
         bwd_params<256>(g, (int)blockIdx.x, (double *)lds);
@@ -1478,35 +1524,29 @@ diff_bwd_rows_kernel(DiffArgs g) {
         r1 = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rr, at + 16u, 0, 0));
     }
     {
-        f4 m = {0.f, 0.f, r1[2], fabsf(r1[3])};
+        f4 m = {0.f, 0.f, r1[2], max2(r0[1], fabsf(r0[3] * r1[3]))};
 #pragma unroll
-        for (int i = 0; i < CH; i++) {
-            m[0] = absmax8(xq[i], m[0]);
-            m[1] = absmax8(xd[i], m[1]);
-        }
+        for (int i = 0; i < CH; i++) m[0] = absmax8(xq[i], m[0]);
 #pragma unroll
-        for (int i = 0; i < 4; i++) m[i] = wave_max(m[i]);
+        for (int i = 0; i < 4; i++)
+            if (i != 1) m[i] = wave_max(m[i]);
         if (lane == 0) rmax[wave] = m;
-        if (!ONE) {
-            const float dm = wave_max(max2(fabsf(r1[0]), fabsf(r1[1])));
-            if (lane == 0) rdmax[wave] = dm;
-        }
+        if (wave == 0) rdo[lane] = r1[2];
     }
     __syncthreads();
     f4 mx = rmax[0];
-    float dmax = ONE ? 0.f : rdmax[0];  // (ONE: D is a mean of this tile's dA)
 #pragma unroll
-    for (int i = 1; i < 4; i++) {
+    for (int i = 1; i < 4; i++)
 #pragma unroll
         for (int e = 0; e < 4; e++) mx[e] = max2(mx[e], rmax[i][e]);
-        if (!ONE) dmax = max2(dmax, rdmax[i]);
-    }
-    const float qup = up_of(mx[0]), dup = up_of(mx[1]), pup = p_up(mx[3]);
+    // dO has a power of two of its row, that of the largest (dup) where it is 0
+    const float qup = up_of(mx[0]), dup = up_of(mx[2]), pup = p_up(mx[3]);
+    auto dup_of = [&](int row) { return rdo[row] > 0.f ? up_of(rdo[row]) : dup; };
     if (stager) {
 #pragma unroll
         for (int i = 0; i < CH; i++) {
             _Float16 *p = qt + row_pos(sr + i * Stage::RPP) * Tile::STRIDE + sc;
-            const Half2 hq = half_split(xq[i], qup), hd = half_split(xd[i], dup);
+            const Half2 hq = half_split(xq[i], qup), hd = half_split(xd[i], dup_of(sr + i * Stage::RPP));
             *(h8 *)p = hq.hi;
             *(h8 *)(p + Tile::PART) = hq.lo;
             *(h8 *)(p + SLOT) = hd.hi;
@@ -1523,6 +1563,9 @@ diff_bwd_rows_kernel(DiffArgs g) {
     }
     const int rg = wave & 1, kg = wave >> 1, row = 32 * rg + lr;
     const int qi = row / g.group, head = kh * g.group + row % g.group;
+    // the row's power of two of dO, what takes it to the rows' common one in dV (P has
+    // it) and back in dS, and what bounds its dS
+    const float ddown = down_of(dup_of(row)), pcommon = dup * ddown, nd = rdo[row];
     // 32 keys of the wave's row, in the order of an accumulator's registers
     auto put = [&](_Float16 *t, const Half2 (&x)[2]) {
         _Float16 *p = t + row_pos(row) * PTile::STRIDE + 32 * kg + 4 * lh;
@@ -1546,8 +1589,9 @@ diff_bwd_rows_kernel(DiffArgs g) {
     // keys that some row sees; the others' gradients are zeros
     const int kend = g.causal ? min(nk, nq + shift) : nq ? nk : 0;
     const int nt = ONE ? 1 : (g.tk + 63) / 64, flip = flip_at((max(kend, 0) + 63) / 64);
-    // the largest value so far and powers of two, sgn: the accumulators' sign
-    float vmax = 0.f, kup = FIRST_UP, sup = FIRST_UP, sgn = 1.f;
+    // the largest value so far and powers of two (sup, own: of the lane's row), sgn: the
+    // accumulators' sign
+    float vmax = 0.f, kup = FIRST_UP, sup = FIRST_UP, sgn = 1.f, own[2] = {DS_START, DS_START};
     for (int t = 0; t < nt; t++) {
         const int k0 = 64 * t, key = k0 + 32 * rg + lr;  // of the wave's blocks of dK and dV
         const bool live = key < nk;
@@ -1570,7 +1614,9 @@ diff_bwd_rows_kernel(DiffArgs g) {
             vmax = max2(vmax, tmax[i][1]);
         }
         const float kup1 = sticky_up(mk, kup), vup = up_of(vmax);
-        const float sup1 = ds_up(ds_bound<W>(mx[2], vmax, dmax), sup);
+        // (ONE: D is a mean of this tile's dA)
+        const float dmax = ONE ? 0.f : max2(fabsf(rec[4][row]), fabsf(rec[5][row]));
+        const float sup1 = ds_up(ds_bound<W>(nd, vmax, dmax), sup);
         float ratio = down_of(kup) * kup1 * (down_of(sup) * sup1);
         kup = kup1;
         sup = sup1;
@@ -1578,21 +1624,16 @@ diff_bwd_rows_kernel(DiffArgs g) {
             sgn = -1.f;
             ratio = -ratio;
         }
-        if (t && ratio != 1.0f) {
-#pragma unroll
-            for (int m = 0; m < 2; m++)
-#pragma unroll
-                for (int c = 0; c < CT; c++)
-#pragma unroll
-                    for (int r = 0; r < 16; r++) dq[m][c][r] *= ratio;
-        }
         st.store(kt, kup, vup, SLOT);
         if (!ONE && k0 + 64 < kend) st.load(k0 + 64);
         __syncthreads();
         const _Float16 *const k1 = kt + 32 * kg * Tile::STRIDE;
         Half2 ah[2], ds[2][2];
+        f32x16 s[2];
+        // from the row's units, own's apart, to the rows' common ones
+        const float units = dup_of(row) * down_of(dup) * down_of(sup);
         {
-            f32x16 s[2], da;
+            f32x16 da;
 #pragma unroll
             for (int r = 0; r < 16; r++) s[0][r] = s[1][r] = da[r] = 0.f;
 #pragma unroll
@@ -1613,8 +1654,10 @@ diff_bwd_rows_kernel(DiffArgs g) {
             }
             dot_along<Tile>(vt + 32 * kg * Tile::STRIDE, 0, d, da);
             const float f = down_of(kup) * (down_of(qup) * (g.scale * LOG2E));
-            const float fd = da_unit(down_of(vup), down_of(dup), sup);
-            const float nm1 = rec[0][row], il1 = rec[1][row] * sgn, nm2 = rec[2][row], il2 = rec[3][row] * sgn;
+            const float fd = da_unit(down_of(vup), ddown, sup);
+            const float fd1 = fminf(fd * own[0], 0x1.fffffep127f), fd2 = fminf(fd * own[1], 0x1.fffffep127f);
+            const float nm1 = rec[0][row], il1 = rec[1][row] * pcommon * sgn;
+            const float nm2 = rec[2][row], il2 = rec[3][row] * pcommon * sgn;
             f32x16 a;
             auto softmax = [&](int r, float &p1, float &p2) {
                 const int j = k0 + 32 * kg + 8 * (r >> 2) + 4 * lh + (r & 3);
@@ -1643,26 +1686,35 @@ diff_bwd_rows_kernel(DiffArgs g) {
                 if (lh == 0) psum[kg][row] = ps;
                 __syncthreads();
                 ps = psum[0][row] + psum[1][row];
-                const float D1 = ps[0] != 0.f ? -fd * (ps[1] / ps[0]) : 0.f;
-                const float D2 = ps[2] != 0.f ? -fd * (ps[3] / ps[2]) : 0.f;
+                const float D1 = ps[0] != 0.f ? -fd1 * (ps[1] / ps[0]) : 0.f;
+                const float D2 = ps[2] != 0.f ? -fd2 * (ps[3] / ps[2]) : 0.f;
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
-                    s[0][r] *= __builtin_fmaf(da[r], fd, D1);
-                    s[1][r] *= __builtin_fmaf(da[r], fd, D2);
+                    s[0][r] *= __builtin_fmaf(da[r], fd1, D1);
+                    s[1][r] *= __builtin_fmaf(da[r], fd2, D2);
                 }
             } else {
-                const float D1 = rec[4][row] * sup, D2 = rec[5][row] * sup;
+                const float D1 = rec[4][row] * sup * own[0], D2 = rec[5][row] * sup * own[1];
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
                     float p1, p2;
                     softmax(r, p1, p2);
-                    s[0][r] = p1 * __builtin_fmaf(da[r], fd, D1);
-                    s[1][r] = p2 * __builtin_fmaf(da[r], fd, D2);
+                    s[0][r] = p1 * __builtin_fmaf(da[r], fd1, D1);
+                    s[1][r] = p2 * __builtin_fmaf(da[r], fd2, D2);
                 }
             }
             split16(a, ah);
-            split16(s[0], ds[0]);
-            split16(s[1], ds[1]);
+            float m[2] = {absmax16(s[0]), absmax16(s[1])};
+            if (__builtin_expect(__any(max2(m[0], m[1]) >= 0x1p15f || ratio != 1.0f), 0)) {
+#pragma unroll
+                for (int i = 0; i < 2; i++) scale_all(dq[i], ds_fit(s[i], m[i], own[i]) * ratio);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                m[i] = wave_max(m[i] * (down_of(own[i]) * units));
+                split16(s[i], ds[i]);
+            }
+            if (lane == 0) smax[wave] = f2{m[0], m[1]};
         }
         __syncthreads();  // V is read
         put(vt, ah);
@@ -1671,6 +1723,16 @@ diff_bwd_rows_kernel(DiffArgs g) {
 #pragma unroll
             for (int c = 0; c < CT; c++)
                 dot_across<Tile>(k1, m * DHP + 32 * c, ds[m], dq[m][c]);
+        // dK's sums run over the rows: dS once more, with one power of two for the tile
+        float tup[2];
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+            tup[m] = p_up(max2(max2(smax[0][m], smax[1][m]), max2(smax[2][m], smax[3][m])));
+            const float f = tup[m] * (down_of(own[m]) * units);
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[m][r] *= f;
+            split16(s[m], ds[m]);
+        }
         __syncthreads();  // K is read, P_1 - lambda P_2 there
         put(kt, ds[1]);
         for (int c = kg; c < W / 32; c += 2) {
@@ -1691,11 +1753,13 @@ diff_bwd_rows_kernel(DiffArgs g) {
             dot_tiles<Tile, PTile>(qt, kg * DHP + 32 * c, kg ? kt : vt, 32 * rg, dk);
             if (key < g.tk)
                 put_channels<true>(kv + g.koff + kg * g.dh, g.dh, 32 * c, dk,
-                                   down_of(qup) * (g.scale * sgn), down_of(sup) * down_of(pup), live,
-                                   g.acc_kv);
+                                   down_of(qup) * (g.scale * sgn),
+                                   down_of(pup) * down_of(kg ? tup[1] : tup[0]), live, g.acc_kv);
         }
     }
-    // the halves of dQ that waves (rg, 0) and (rg, 1) have
+    // the halves of dQ that waves (rg, 0) and (rg, 1) have, dS's own powers of two off
+#pragma unroll
+    for (int m = 0; m < 2; m++) scale_all(dq[m], down_of(own[m]) * (dup_of(row) * down_of(dup)));
     __syncthreads();
     float *const ex = (float *)kt + rg * 2 * CT * 16 * 64 + lane;
     auto each = [&](auto &&f) {
@@ -1715,8 +1779,9 @@ diff_bwd_rows_kernel(DiffArgs g) {
     for (int m = 0; m < 2; m++)
 #pragma unroll
         for (int c = 0; c < CT; c++)
-            put_channels<true>(dst + m * g.dh, g.dh, 32 * c, dq[m][c], down_of(kup) * (g.scale * sgn),
-                               down_of(sup) * down_of(pup), qi < nq, g.acc_q);
+            put_channels<true>(dst + m * g.dh, g.dh, 32 * c, dq[m][c],
+                               down_of(kup) * (g.scale * sgn), down_of(sup) * down_of(pup), qi < nq,
+                               g.acc_q);
 }
 
 // The backward's first pass: lanes of a unit and blocks, so that the groups of

@@ -176,6 +176,19 @@ def test_gradients_of_any_magnitude(rnn, p, two):
     check(cs, run(rnn, refill(cs)))
 
 
+@pytest.mark.parametrize("two", [-110, -84, -40, -12, 12])
+@pytest.mark.parametrize("p", PATHS, ids=NAMES)
+def test_rows_of_another_magnitude(rnn, p, two):
+    """Every third query's dy, and then all but one query's, times a power of
+    two: each row of dQ stays within its own size."""
+    for part in (slice(0, None, 3), slice(1, None)):
+        cs = path(p, seed=7)
+        cs.dyv[:, part] *= 2.0 ** two
+        got = run(rnn, refill(cs))
+        check(cs, got, per_row=True, what=("dq",))
+        check(cs, got)
+
+
 @pytest.mark.parametrize("p", PATHS, ids=NAMES)
 def test_rows_without_gradient(rnn, p):
     """dy of zeros, in some rows and in all, with values far from 1."""
@@ -199,6 +212,43 @@ def test_tiny_queries_and_keys(rnn, p):
         cs.qv *= 2.0 ** -70
         cs.kvv *= 2.0 ** -70
         check(cs, run(rnn, refill(cs)))
+
+
+@pytest.mark.parametrize("tq,tk,dh", [(70, 65536, 64), (33, 262144, 16), (3, 200000, 32)])
+def test_gradients_over_long_keys(rnn, tq, tk, dh):
+    """P falls with the number of keys; dS keeps its bits: 4 times 2^-22 (1e-6) of
+    the terms' size, by row and by block.  dQ is besides a sum of 3 tk / 16 matrix
+    instructions, each cut off by at most 2^-23, 2^-24 in the mean, of a partial sum
+    that is at most as large; half-way signs turn, so that these add like a random
+    walk: 2^-24 sqrt(3 tk / 16), 6.6e-6 at 65536 keys.  So is the O that D in dK
+    comes from; dV has neither."""
+    cs = DiffCase(1, 1, 1, dh, tq, tk, True, gap=0, seed=10)
+    got = run(rnn, cs)
+    tol = 1e-6 + 2.0 ** -24 * (3 * tk / 16) ** 0.5
+    check(cs, got, per_row=True, tol=tol, what=("dq",))
+    check(cs, got, tol=tol, what=("dk",))
+    check(cs, got, tol=1e-6, what=("dv",))
+
+
+@pytest.mark.parametrize("p", PATHS, ids=NAMES)
+def test_an_outlier_among_the_values(rnn, p):
+    """One value 2^14 times larger than the others', at a key that hardly counts
+    (a score 14 below the others'): dS of the other keys keeps its bits.  That key
+    itself has |q| |k| scale up to 12 * 14 = 170, so its scores, and P, are within
+    2^-22 170 = 4e-5."""
+    cs = path(p, seed=11)
+    key = p[6] // 2
+    cs.qv[..., 0] = 1.0
+    cs.kvv[..., 0] = 0.0
+    cs.kvv[:, key, :, :, 0] = -14.0 * p[4] ** 0.5
+    cs.vv[:, key] *= 2.0 ** 14
+    got = run(rnn, refill(cs))
+    check(cs, got, per_row=True, what=("dq",))
+    check(cs, got, per_row=True, tol=TOL + 4e-5, what=("dk",))
+    rest = [j for j in range(p[6]) if j != key]
+    want, have = formulas(cs), shaped(cs, got)
+    err = ((have["dk"] - want["dk"])[:, rest] ** 2).sum(-1)
+    assert (err <= TOL ** 2 * want["sk"][:, rest, ..., 0] ** 2).all()
 
 
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
