@@ -11,8 +11,10 @@
 // and x of the third).  Floats go through registers into LDS as two fp16 parts
 // (mfma_half.h) in the layout they have in memory; an operand whose k runs along
 // columns is handed back transposed by the LDS itself.  Two LDS buffers, the loads
-// of the stage after next in flight, one barrier a stage; the parts' power of two
-// follows the largest magnitude so far, and the accumulators with it.
+// of the stage after next in flight, one barrier a stage.  Each row of op(A) and
+// column of op(B), the elements that one sum takes, has a power of two of its own,
+// which follows the largest magnitude so far, and the accumulators with it: a
+// feature or channel keeps its bits beside one 2^30 times as large.
 #include "mfma_half.h"
 
 #include <algorithm>
@@ -119,19 +121,24 @@ __device__ __forceinline__ void quad_store(float *p, f4 v, int cnt) {
 
 // How an operand of R rows (of C) is staged over a depth of KB: KC: k runs along
 // its rows in memory (R rows of KB), 16-byte slots of a row exchanged so that the
-// b128 reads of 8 rows fall on distinct banks; each row has its own power of two
-// (its threads are neighbours).  Else k runs across them (KB rows of R, padded, in
-// row_pos' order), read transposed, one power for the tile.
+// b128 reads of 8 rows fall on distinct banks; a row's power of two comes from its
+// threads, which are neighbours.  Else k runs across them (KB rows of R, padded, in
+// row_pos' order), read transposed; a row of C is spread over the workgroup then, and
+// threads that meet a value past what its power is good for leave it in LDS (a
+// maximum, so in any order) a barrier before the stage is written.
 // Two register sets: stage t's loads go out while stage t - 3 is computed.
-template <int R, int KB, bool KC, bool PRO, int NT>
+// KEEP (k across rows): the thread's powers of two stay in registers, where the kernel
+// has them to spare; else they are read back from LDS.
+template <int R, int KB, bool KC, bool PRO, bool KEEP, int NT>
 struct Operand {
     using Stage = std::conditional_t<KC, StagePlan<R, KB, NT>, StagePlan<KB, R, NT>>;
     static constexpr int STRIDE = KC ? KB : R + 8;
     static constexpr int PART = (KC ? R : KB) * STRIDE, HALVES = 2 * PART;
-    static constexpr int CH = Stage::PASSES, UPS = KC ? R : 1;
+    static constexpr int CH = Stage::PASSES;
     static_assert(Stage::ALL, "every thread stages");
     float x[2][CH][8], x2[PRO ? 2 : 1][PRO ? CH : 1][8];
-    float up[CH];  // powers of two (KC: of each row)
+    float up[KC ? CH : KEEP ? 8 : 1];  // powers of two of the thread's rows of C
+    float good;                        // !KEEP: what all of them are good for
     const float *p, *p2;
     long long ld;
     int rows, kend, sc, sr;  // rows of C from the block's first on
@@ -146,10 +153,11 @@ struct Operand {
         kend = kend_;
         p = base + (KC ? r0 * ld : r0);
         p2 = PRO ? base2 + (KC ? r0 * ld : r0) : nullptr;
+        good = good_for(FIRST_UP);
         sc = (int)threadIdx.x % Stage::C8 * 8;
         sr = (int)threadIdx.x / Stage::C8;
 #pragma unroll
-        for (int i = 0; i < CH; i++) up[i] = FIRST_UP;
+        for (int i = 0; i < (KC ? CH : KEEP ? 8 : 1); i++) up[i] = FIRST_UP;
     }
     template <bool TAIL>
     __device__ __forceinline__ void load_from(const float *src, int k0, float (&v)[CH][8]) const {
@@ -181,40 +189,111 @@ struct Operand {
                 for (int e = 0; e < 8; e++) x[SET][i][e] *= x2[SET][i][e];
         }
     }
-    // !KC: the wave's largest magnitude of a set past what up is good for.
-    template <int SET>
-    __device__ __forceinline__ float largest() {
-        multiply<SET>();
-        float m = 0.f;
+    // !KEEP: the thread's powers of two in LDS (null: before any).
+    __device__ __forceinline__ void powers(const float *ups, float (&u)[8]) const {
 #pragma unroll
-        for (int i = 0; i < CH; i++) m = absmax8(x[SET][i], m);
-        return wave_over(m, good_for(up[0]));
+        for (int e = 0; e < 8; e += 4) {
+            f4 v = {FIRST_UP, FIRST_UP, FIRST_UP, FIRST_UP};
+            if (ups) v = *(const f4 *)(ups + sc + e);
+#pragma unroll
+            for (int i = 0; i < 4; i++) u[e + i] = v[i];
+        }
+    }
+    template <int SET>
+    __device__ __forceinline__ float largest(int e) const {
+        float m = fabsf(x[SET][0][e]);
+        if constexpr (CH > 1) m = max3abs(0.f, x[SET][0][e], x[SET][1][e]);
+#pragma unroll
+        for (int i = 2; i < CH; i += 2) m = max3abs(m, x[SET][i][e], x[SET][i + 1 < CH ? i + 1 : i][e]);
+        return m;
+    }
+    // !KC: the set's magnitudes past what the powers are good for into the stage's
+    // maxima, and its number t beside them.  ups: powers a stage old (they only fall);
+    // good: what all of the thread's are good for, beyond which each is looked at.
+    template <int SET>
+    __device__ __forceinline__ void maxima(const float *ups, uint32_t *most, int *over, int t) {
+        multiply<SET>();
+        float m[8], y[8];
+        if constexpr (KEEP) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                m[e] = largest<SET>(e);
+                y[e] = m[e] * up[e];
+            }
+            if (!(absmax8(y, 0.f) >= 0x1p15f)) return;
+        } else {
+            float all = 0.f;
+#pragma unroll
+            for (int i = 0; i < CH; i++) all = absmax8(x[SET][i], all);
+            if (!(all >= good)) return;
+            powers(ups, y);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                m[e] = largest<SET>(e);
+                y[e] *= m[e];
+            }
+        }
+        *over = t;
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (y[e] >= 0x1p15f) atomicMax(most + sc + e, __float_as_uint(m[e]));
     }
     // A set into the tile at t, the powers of two into ups; whether one changed.
-    // largest: !KC, the tile's largest magnitude.
+    // !KC: last, the stage before's powers (null: before any); most, the stage's maxima
+    // where some value was past its power, else null.
     template <int SET>
-    __device__ __forceinline__ bool store(_Float16 *t, float *ups, float largest) {
+    __device__ __forceinline__ bool store(_Float16 *t, float *ups, const float *last, const uint32_t *most) {
         if (KC) multiply<SET>();
         bool changed = false;
+        float u8[KC ? 1 : 8];
+        if constexpr (!KC) {
+            if constexpr (KEEP) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) u8[e] = up[e];
+            } else {
+                powers(last, u8);
+            }
+            if (most) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float u = sticky_up(__uint_as_float(most[sc + e]), u8[e]);
+                    changed = changed || u != u8[e];
+                    u8[e] = u;
+                }
+                if constexpr (KEEP) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) up[e] = u8[e];
+                } else {
+                    float top = u8[0];
+#pragma unroll
+                    for (int e = 1; e < 8; e++) top = max2(top, u8[e]);
+                    good = good_for(top);
+                }
+            }
+            if (sr == 0) {
+#pragma unroll
+                for (int e = 0; e < 8; e += 4) *(f4 *)(ups + sc + e) = f4{u8[e], u8[e + 1], u8[e + 2], u8[e + 3]};
+            }
+        }
 #pragma unroll
         for (int i = 0; i < CH; i++) {
             const int r = sr + i * Stage::RPP;
-            if (KC || i == 0) {
-                float m = largest;
-                if constexpr (KC) {
-                    m = absmax8(x[SET][i], 0.f);
-                    m = max2(m, dpp_f<0xB1>(m));
-                    m = max2(m, dpp_f<0x4E>(m));
-                    if (Stage::C8 > 4) m = max2(m, dpp_f<0x141>(m));
-                    if (Stage::C8 > 8) m = max2(m, dpp_f<0x140>(m));
-                }
+            if constexpr (KC) {
+                float m = absmax8(x[SET][i], 0.f);
+                m = max2(m, dpp_f<0xB1>(m));
+                m = max2(m, dpp_f<0x4E>(m));
+                if (Stage::C8 > 4) m = max2(m, dpp_f<0x141>(m));
+                if (Stage::C8 > 8) m = max2(m, dpp_f<0x140>(m));
                 const float u = sticky_up(m, up[i]);
                 changed = changed || u != up[i];
                 up[i] = u;
-                if (KC ? sc == 0 : threadIdx.x == 0) ups[KC ? r : 0] = u;
+                if (sc == 0) ups[r] = u;
             }
             _Float16 *d = t + (KC ? r : row_pos(r)) * STRIDE + (KC ? 8 * slot(r, sc / 8) : sc);
-            const Half2 h = half_split(x[SET][i], KC ? up[i] : up[0]);
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = x[SET][i][e] * (KC ? up[i] : u8[KC ? 0 : e]);
+            const Half2 h = half_split(v);
             *(h8 *)d = h.hi;
             *(h8 *)(d + PART) = h.lo;
         }
@@ -236,12 +315,6 @@ struct Operand {
             return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
         }
     }
-    // Row r's power of two.
-    __device__ __forceinline__ static float up_at(const float *ups, int r) { return ups[KC ? r : 0]; }
-    __device__ __forceinline__ static f4 up_at4(const float *ups, int r) {
-        if constexpr (KC) return *(const f4 *)(ups + r);
-        return f4{ups[0], ups[0], ups[0], ups[0]};
-    }
 };
 
 // C[M x N] over k: a tile of BM x BN a workgroup, KB of k a stage, WM x WN x WK
@@ -251,15 +324,18 @@ __global__ __launch_bounds__(64 * WM * WN * WK) __attribute__((amdgpu_waves_per_
 linact_kernel(LinArgs g) {
     constexpr int NW = WM * WN * WK, NT = 64 * NW, MT = BM / 32 / WM, NN = BN / 32 / WN;
     constexpr int KS = KB / 16 / WK;
-    using OA = Operand<BM, KB, AK, PRO, NT>;
-    using OB = Operand<BN, KB, BK, false, NT>;
+    using OA = Operand<BM, KB, AK, PRO, false, NT>;
+    using OB = Operand<BN, KB, BK, false, AK && !BK, NT>;
     constexpr int STAGE = OA::HALVES + OB::HALVES;
     constexpr size_t LDS = std::max<size_t>(4 * STAGE, (size_t)WK * BM * BN * 4);
     __shared__ __align__(16) char lds_raw[LDS];
-    __shared__ float tmax[2][2][NW];
+    // operands whose k runs across rows: the largest magnitudes of even and odd stages
+    // so far that were past their power, and the last stage that had one
+    __shared__ uint32_t most[2][BM + BN];
+    __shared__ int over[2][2];
     // the powers of two of three stages (one is read, one may be compared with it,
     // one is written), and whether a stage's differ from the one before
-    __shared__ __align__(16) float ups[3][(OA::UPS + OB::UPS + 3) / 4 * 4];
+    __shared__ __align__(16) float ups[3][BM + BN];
     __shared__ int changes[3];
     _Float16 *const lds = (_Float16 *)lds_raw;
     const int wave = wave_index(), lane = threadIdx.x & 63, lr = lane & 31, lh = lane >> 5;
@@ -293,31 +369,30 @@ linact_kernel(LinArgs g) {
     const bool sums = SUMS && n0 == 0 && (g.csum || g.db);
     double cs[8] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0};
     if (threadIdx.x < 3) changes[threadIdx.x] = 0;
+    if (!AK || !BK) {
+        for (int i = (int)threadIdx.x; i < 2 * (BM + BN); i += NT) most[0][i] = 0;
+        if (threadIdx.x < 4) over[0][threadIdx.x] = -1;
+        __syncthreads();
+    }
+    // (stage t's are written between the barriers t - 2 and t - 1 and read before t)
     auto maxima = [&](int t, auto set) {
         constexpr int S = decltype(set)::value;
-        if ((AK && BK) || t >= nst) return;
-        const float a = AK ? 0.f : A.template largest<S>(), b = BK ? 0.f : B.template largest<S>();
-        if (lane == 0) {
-            tmax[t & 1][0][wave] = a;
-            tmax[t & 1][1][wave] = b;
-        }
+        if (t >= nst) return;
+        const float *u = t >= 2 ? ups[(t - 2) % 3] : nullptr;
+        if constexpr (!AK) A.template maxima<S>(u, most[t & 1], &over[t & 1][0], t);
+        if constexpr (!BK) B.template maxima<S>(u ? u + BM : u, most[t & 1] + BM, &over[t & 1][1], t);
     };
     // stage t from its set into its buffer, then the loads of stage t + 2
     auto stage = [&](int t, auto set) {
         constexpr int S = decltype(set)::value;
         if (t >= nst) return;
-        float la = 0.f, lb = 0.f;
-        if (!AK || !BK) {
-#pragma unroll
-            for (int i = 0; i < NW; i++) {
-                la = max2(la, tmax[t & 1][0][i]);
-                lb = max2(lb, tmax[t & 1][1][i]);
-            }
-        }
         _Float16 *d = lds + (t & 1) * STAGE;
         float *u = ups[t % 3];
-        const bool ca = A.template store<S>(d, u, la);
-        const bool cb = B.template store<S>(d + OA::HALVES, u + OA::UPS, lb);
+        const uint32_t *ma = !AK && over[t & 1][0] == t ? most[t & 1] : nullptr;
+        const uint32_t *mb = !BK && over[t & 1][1] == t ? most[t & 1] + BM : nullptr;
+        const float *last = t ? ups[(t + 2) % 3] : nullptr;
+        const bool ca = A.template store<S>(d, u, last, ma);
+        const bool cb = B.template store<S>(d + OA::HALVES, u + BM, last ? last + BM : last, mb);
         if (t && (ca || cb)) changes[t % 3] = 1;
         if (SUMS && sums) {
 #pragma unroll
@@ -335,13 +410,13 @@ linact_kernel(LinArgs g) {
 #pragma unroll
             for (int j = 0; j < NN; j++) {
                 const int c = (wn * NN + j) * 32 + lr;
-                const float rb = OB::up_at(u + OA::UPS, c) * down_of(OB::up_at(v + OA::UPS, c));
+                const float rb = u[BM + c] * down_of(v[BM + c]);
 #pragma unroll
                 for (int i = 0; i < MT; i++)
 #pragma unroll
                     for (int r = 0; r < 16; r++) {
                         const int m = (wm * MT + i) * 32 + 8 * (r >> 2) + 4 * lh + (r & 3);
-                        acc[i][j][r] *= OA::up_at(u, m) * down_of(OA::up_at(v, m)) * rb;
+                        acc[i][j][r] *= u[m] * down_of(v[m]) * rb;
                     }
             }
         }
@@ -388,13 +463,13 @@ linact_kernel(LinArgs g) {
 #pragma unroll
     for (int j = 0; j < NN; j++) {
         const int c = (wn * NN + j) * 32 + lr;
-        const float db = nst ? down_of(OB::up_at(ul + OA::UPS, c)) : 0.f;
+        const float db = nst ? down_of(ul[BM + c]) : 0.f;
 #pragma unroll
         for (int i = 0; i < MT; i++)
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
                 const int m = (wm * MT + i) * 32 + 2 * r + 4 * lh;
-                const f4 ua = OA::up_at4(ul, m);
+                const f4 ua = *(const f4 *)(ul + m);
 #pragma unroll
                 for (int e = 0; e < 4; e++)
                     ct[(wk * BM + m + e) * BN + c] = acc[i][j][r + e] * (nst ? down_of(ua[e]) : 0.f) * db;

@@ -50,17 +50,23 @@ __device__ __forceinline__ void half_pair(float a, float b, uint32_t &hi, uint32
     lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(d, h2));
 }
 
-// The two parts of 8 floats times up (a power of two).
-__device__ __forceinline__ Half2 half_split(const float (&x)[8], float up) {
+// The two parts of 8 floats (times up, a power of two).
+__device__ __forceinline__ Half2 half_split(const float (&x)[8]) {
     u32x4 hi, lo;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         uint32_t a, b;
-        half_pair(x[2 * j] * up, x[2 * j + 1] * up, a, b);
+        half_pair(x[2 * j], x[2 * j + 1], a, b);
         hi[j] = a;
         lo[j] = b;
     }
     return Half2{__builtin_bit_cast(h8, hi), __builtin_bit_cast(h8, lo)};
+}
+__device__ __forceinline__ Half2 half_split(const float (&x)[8], float up) {
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) y[e] = x[e] * up;
+    return half_split(y);
 }
 // The parts of an accumulator's registers 0..7 and 8..15, as they are.
 __device__ __forceinline__ void split16(const f32x16 &x, Half2 (&d)[2]) {
