@@ -441,19 +441,32 @@ def _arg(ctx, t, need, name, dtype="float32"):
     raise ValueError(f"{name} has {t.numel()} elements, needs {need}")
 
 
-def _on_ctx_stream(ctx, *ts):
-    """Tells torch's allocator of tensors that the context's stream uses, where
-    that is not the current one, so that their memory is not handed out again
-    before its work is done."""
-    import torch
-    sp = ctx.stream
-    if torch._C._cuda_getCurrentRawStream(ctx.device) == sp:
-        return
-    st = torch.cuda.ExternalStream(sp, device=ctx.device) if sp else \
-        torch.cuda.default_stream(ctx.device)
-    for t in ts:
-        if t is not None:
-            t.record_stream(st)
+class _OnStream:
+    """A call on the context's stream, ordered with torch's current stream where
+    the two differ: it starts after the work that the current stream holds (its
+    inputs, and whatever last used the memory that torch hands out for its
+    results), and what the current stream is given next starts after it."""
+
+    __slots__ = ("pair",)
+
+    def __init__(self, ctx):
+        import torch
+        self.pair, sp = None, ctx.stream
+        if torch._C._cuda_getCurrentRawStream(ctx.device) != sp:
+            st = (torch.cuda.ExternalStream(sp, device=ctx.device) if sp else
+                  torch.cuda.default_stream(ctx.device))
+            self.pair = torch.cuda.current_stream(ctx.device), st
+            st.wait_stream(self.pair[0])
+
+    def done(self, *ts):
+        """ts: the tensors of the call, which torch's allocator is told of."""
+        if self.pair is None:
+            return
+        cur, st = self.pair
+        cur.wait_stream(st)
+        for t in ts:
+            if t is not None:
+                t.record_stream(st)
 
 
 # ------------------------------------------------------------------ gemm.rs
@@ -809,11 +822,14 @@ class Rotary:
         d = self._desc(xstride, xoff, ystride, yoff)
         rows = n * t
         need = lambda stride, off: (rows - 1) * stride + off + w if rows else 0
-        ctx.check(lib().rnn_rotary(
-            ctx.h, C.byref(d), n, t, _arg(ctx, x, need(xstride, xoff), "x"),
-            _arg(ctx, pos, rows * len(self.grid), "pos"),
-            _arg(ctx, y, need(ystride, yoff), "y"), int(inverse)))
-        _on_ctx_stream(ctx, x, y, pos)
+        args = (_arg(ctx, x, need(xstride, xoff), "x"),
+                _arg(ctx, pos, rows * len(self.grid), "pos"),
+                _arg(ctx, y, need(ystride, yoff), "y"))
+        on = _OnStream(ctx)
+        try:
+            ctx.check(lib().rnn_rotary(ctx.h, C.byref(d), n, t, *args, int(inverse)))
+        finally:
+            on.done(x, y, pos)
         return y
 
     def forward(self, n, x, xstride, xoff=0, pos=None, y=None, ystride=None, yoff=0, t=None):
@@ -896,11 +912,14 @@ class DiffCore:
                      torch.empty(rows * self.h * 4, dtype=torch.float32, device=q.device))
         ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None
         o12, stats = saved or (None, None)
-        ctx.check(lib().rnn_diff_attn_forward(
-            ctx.h, C.byref(d), n, *ins, ws.data_ptr() if nb else None, nb,
-            _arg(ctx, y, rows * self.c, "y"), _arg(ctx, o12, 0, "o12"),
-            _arg(ctx, stats, 0, "stats")))
-        _on_ctx_stream(ctx, q, kv, lam, gain, qlen, klen, ws, y, o12, stats)
+        outs = (_arg(ctx, y, rows * self.c, "y"), _arg(ctx, o12, 0, "o12"),
+                _arg(ctx, stats, 0, "stats"))
+        on = _OnStream(ctx)
+        try:
+            ctx.check(lib().rnn_diff_attn_forward(
+                ctx.h, C.byref(d), n, *ins, ws.data_ptr() if nb else None, nb, *outs))
+        finally:
+            on.done(q, kv, lam, gain, qlen, klen, ws, y, o12, stats)
         return y, saved
 
     def backward(self, n, q, qstride, qoff, kv, kvstride, koff, voff, lam, gain, saved, dy, dq,
@@ -917,13 +936,17 @@ class DiffCore:
         o12, stats = saved
         ws = torch.empty(nb, dtype=torch.uint8, device=dy.device) if nb else None
         flags = (RNN_ATTN_SET_DQ if set_dq else 0) | (RNN_ATTN_SET_DKV if set_dkv else 0)
-        ctx.check(lib().rnn_diff_attn_backward(
-            ctx.h, C.byref(d), n, *ins, _arg(ctx, o12, rows * 2 * self.c, "o12"),
-            _arg(ctx, stats, rows * self.h * 4, "stats"), _arg(ctx, dy, rows * self.c, "dy"),
-            ws.data_ptr() if nb else None, nb, _arg(ctx, dq, nq, "dq"),
-            _arg(ctx, dkv, nkv, "dkv"), _arg(ctx, dlam, self.lam_heads * 4 * self.dh, "dlam"),
-            _arg(ctx, dgain, 2 * self.dh, "dgain"), flags))
-        _on_ctx_stream(ctx, q, kv, lam, gain, qlen, klen, ws, dy, o12, stats, dq, dkv, dlam, dgain)
+        ins += (_arg(ctx, o12, rows * 2 * self.c, "o12"),
+                _arg(ctx, stats, rows * self.h * 4, "stats"), _arg(ctx, dy, rows * self.c, "dy"))
+        outs = (_arg(ctx, dq, nq, "dq"), _arg(ctx, dkv, nkv, "dkv"),
+                _arg(ctx, dlam, self.lam_heads * 4 * self.dh, "dlam"),
+                _arg(ctx, dgain, 2 * self.dh, "dgain"))
+        on = _OnStream(ctx)
+        try:
+            ctx.check(lib().rnn_diff_attn_backward(
+                ctx.h, C.byref(d), n, *ins, ws.data_ptr() if nb else None, nb, *outs, flags))
+        finally:
+            on.done(q, kv, lam, gain, qlen, klen, ws, dy, o12, stats, dq, dkv, dlam, dgain)
 
 
 # ------------------------------------------------------------------ linear.rs
@@ -980,11 +1003,14 @@ def linear_act_forward(rows, fin, fout, x, w, b=None, act="none", res=None, y=No
     y = torch.empty(rows, fout, dtype=torch.float32, device=x.device) if y is None else y
     slope = (torch.empty(rows, fout, dtype=torch.float32, device=x.device) if train and code
              else None)
-    ctx.check(lib().rnn_linear_act_forward(
-        ctx.h, rows, fin, fout, _arg(ctx, x, rows * fin, "x"), _arg(ctx, w, fout * fin, "w"),
-        _arg(ctx, b, fout, "b"), code, _arg(ctx, res, rows * fout, "res"),
-        _arg(ctx, slope, 0, "slope"), _arg(ctx, y, rows * fout, "y")))
-    _on_ctx_stream(ctx, x, w, b, res, slope, y)
+    args = (_arg(ctx, x, rows * fin, "x"), _arg(ctx, w, fout * fin, "w"), _arg(ctx, b, fout, "b"),
+            code, _arg(ctx, res, rows * fout, "res"), _arg(ctx, slope, 0, "slope"),
+            _arg(ctx, y, rows * fout, "y"))
+    on = _OnStream(ctx)
+    try:
+        ctx.check(lib().rnn_linear_act_forward(ctx.h, rows, fin, fout, *args))
+    finally:
+        on.done(x, w, b, res, slope, y)
     return y, slope
 
 
@@ -1010,13 +1036,16 @@ def linear_act_backward(rows, fin, fout, dy, x, w, slope, act, dw, db=None, dx=N
         nb = _linear_act_ws[rows, fin, fout] = out.value
     ws = torch.empty(nb, dtype=torch.uint8, device=dy.device) if nb else None
     dx = torch.empty(rows, fin, dtype=torch.float32, device=dy.device) if dx is None else dx
-    ctx.check(lib().rnn_linear_act_backward(
-        ctx.h, rows, fin, fout, _arg(ctx, dy, rows * fout, "dy"), _arg(ctx, x, rows * fin, "x"),
-        _arg(ctx, w, fout * fin, "w"), _arg(ctx, slope, rows * fout, "slope") if code else None,
-        ws.data_ptr() if nb else None, nb, _arg(ctx, dw, fout * fin, "dw"),
-        _arg(ctx, db, fout, "db"), _arg(ctx, dx, rows * fin, "dx"),
-        RNN_LINEAR_ACC_DX if acc_dx else 0))
-    _on_ctx_stream(ctx, dy, x, w, slope, ws, dw, db, dx)
+    args = (_arg(ctx, dy, rows * fout, "dy"), _arg(ctx, x, rows * fin, "x"),
+            _arg(ctx, w, fout * fin, "w"), _arg(ctx, slope, rows * fout, "slope") if code else None,
+            ws.data_ptr() if nb else None, nb, _arg(ctx, dw, fout * fin, "dw"),
+            _arg(ctx, db, fout, "db"), _arg(ctx, dx, rows * fin, "dx"),
+            RNN_LINEAR_ACC_DX if acc_dx else 0)
+    on = _OnStream(ctx)
+    try:
+        ctx.check(lib().rnn_linear_act_backward(ctx.h, rows, fin, fout, *args))
+    finally:
+        on.done(dy, x, w, slope, ws, dw, db, dx)
     return dx
 
 
