@@ -354,8 +354,8 @@ int rnn_linear_backward_ex(rnn_ctx *ctx, size_t rows, size_t fin, size_t fout, c
  * for the backward (NULL: not kept; not needed for RNN_ACT_NONE).  act:
  * RNN_ACT_NONE z, RNN_ACT_RELU max(z, 0), RNN_ACT_GELU z (1 + erf(z / sqrt 2)) /
  * 2, RNN_ACT_GELU_TANH z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2,
- * RNN_ACT_SILU z / (1 + exp(-z)); RELU's slope at 0 is 0.  rows <= 2^30, fin and
- * fout <= 2^20.  Products are taken in two fp16 parts under a power of two of
+ * RNN_ACT_SILU z / (1 + exp(-z)); RELU's slope at 0 is 0.  rows <= 2^30 - 128, fin
+ * and fout <= 2^20.  Products are taken in two fp16 parts under a power of two of
  * what one sum takes (a row of x, W or dz, a column of W, dz or x): elements down
  * to 2^-12 of its largest so far keep 2^-23 of themselves, smaller ones 2^-35 of the
  * largest.  An infinity or a NaN in x, W or dy gives NaN in the sums that take it. */

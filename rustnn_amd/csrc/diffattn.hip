@@ -32,6 +32,7 @@ struct DiffArgs {
     long long qstride, kvstride;
     int n, h, hkv, dh, tq, tk, koff, voff, lam_heads, diag, causal, group;
     int acc_q, acc_kv, split_keys;
+    long long first;       // the launch's first block of rows, keys or problems
     int nblk, gpb;         // blocks of the backward's first pass, their groups of lanes
     float *dlam, *dgain;
     float scale, lam_init, eps;
@@ -265,7 +266,7 @@ diff_fwd_kernel(DiffArgs g) {
     const int lane = threadIdx.x & 63, wave = wave_index(), lr = lane & 31, lh = lane >> 5;
     const int map = wave & 1, qg = (wave >> 1) % QG, half = (wave >> 1) / QG;
     const int R = g.tq * g.group, nrb = (R + 32 * QG - 1) / (32 * QG);
-    const long long id = xcd_order(blockIdx.x, gridDim.x);
+    const long long id = g.first + xcd_order(blockIdx.x, gridDim.x);
     const int prob = (int)(id / nrb), rb = nrb - 1 - (int)(id % nrb);  // causal: longest first
     const int b = prob / g.hkv, kh = prob % g.hkv;
     const int nq = len_of(g.qlen, b, g.tq), nk = len_of(g.klen, b, g.tk), shift = nk - nq;
@@ -746,7 +747,7 @@ __global__ __launch_bounds__(256) void diff_bwd_pre_kernel(DiffArgs g) {
 // its heads (every group of every block for a shared set, else group index % h =
 // head) in NT strided sums, added in a fixed tree.
 __device__ __forceinline__ int params_blocks(const DiffArgs &g) {
-    return (g.dgain ? (2 * g.dh + 15) / 16 : 0) + g.lam_heads;
+    return g.first ? 0 : (g.dgain ? (2 * g.dh + 15) / 16 : 0) + g.lam_heads;
 }
 template <int NT>
 __device__ __forceinline__ void bwd_params(const DiffArgs &g, int blk, double *red) {
@@ -913,7 +914,7 @@ diff_dq_kernel(DiffArgs g) {
         bwd_params<NT>(g, (int)blockIdx.x, (double *)lds);
         return;
     }
-    const long long id = xcd_order(blockIdx.x - np, gridDim.x - np);
+    const long long id = g.first + xcd_order(blockIdx.x - np, gridDim.x - np);
     const int prob = (int)(id / nrb), rb = nrb - 1 - (int)(id % nrb);
     const int b = prob / g.hkv, kh = prob % g.hkv;
     const int nq = len_of(g.qlen, b, g.tq), nk = len_of(g.klen, b, g.tk), shift = nk - nq;
@@ -1148,7 +1149,7 @@ diff_dkv_kernel(DiffArgs g) {
     const int lane = threadIdx.x & 63, wave = wave_index(), lr = lane & 31, lh = lane >> 5;
     const int kg = wave >> 1, map = wave & 1;
     const int nkb = (g.tk + BK - 1) / BK;
-    const long long id = xcd_order(blockIdx.x, gridDim.x);
+    const long long id = g.first + xcd_order(blockIdx.x, gridDim.x);
     const int prob = (int)(id / nkb), kb = (int)(id % nkb);
     const int b = prob / g.hkv, kh = prob % g.hkv;
     const int nq = len_of(g.qlen, b, g.tq), nk = len_of(g.klen, b, g.tk), shift = nk - nq;
@@ -1490,7 +1491,7 @@ diff_bwd_rows_kernel(DiffArgs g) {
         return;
     }
     const int lane = threadIdx.x & 63, wave = wave_index(), lr = lane & 31, lh = lane >> 5;
-    const int prob = (int)xcd_order(blockIdx.x - np, gridDim.x - np);
+    const int prob = (int)(g.first + xcd_order(blockIdx.x - np, gridDim.x - np));
     const int b = prob / g.hkv, kh = prob % g.hkv;
     const int nq = len_of(g.qlen, b, g.tq), nk = len_of(g.klen, b, g.tk), shift = nk - nq;
     const int dw = 2 * g.dh;
@@ -1935,16 +1936,29 @@ bool rows_vec(const DiffArgs &g) {
            al(g.dy) && al(g.dq) && al(g.dkv);
 }
 
+// Blocks in launches of at most 2^31 threads (a grid holds below 2^32): f(g, blocks)
+// with g.first their first.
+template <typename F>
+void in_launches(DiffArgs g, size_t blocks, size_t threads, F &&f) {
+    const size_t most = ((size_t)1 << 31) / threads;
+    for (size_t b = 0; b < blocks; b += most) {
+        g.first = (long long)b;
+        f(g, (unsigned)std::min(most, blocks - b));
+    }
+}
+
 template <int DHP, bool VEC, int QG, int KH = 1>
 void launch_fwd_qg(rnn_ctx *ctx, const DiffArgs &g, const FwdPlan &p) {
-    const dim3 grid((unsigned)p.blocks, (unsigned)p.splits);
     if constexpr (KH == 1) {
         if (p.splits > 1) {
+            const dim3 grid((unsigned)p.blocks, (unsigned)p.splits);
             diff_fwd_kernel<DHP, VEC, QG, 1, true><<<grid, 128 * QG, 0, ctx->stream>>>(g);
             return;
         }
     }
-    diff_fwd_kernel<DHP, VEC, QG, KH, false><<<grid, 128 * QG * KH, 0, ctx->stream>>>(g);
+    in_launches(g, p.blocks, 128 * QG * KH, [&](const DiffArgs &a, unsigned blocks) {
+        diff_fwd_kernel<DHP, VEC, QG, KH, false><<<blocks, 128 * QG * KH, 0, ctx->stream>>>(a);
+    });
 }
 template <int DHP>
 void launch_fwd(rnn_ctx *ctx, const DiffArgs &g, const FwdPlan &p, bool vec) {
@@ -1961,20 +1975,24 @@ void launch_fwd(rnn_ctx *ctx, const DiffArgs &g, const FwdPlan &p, bool vec) {
 }
 
 // The blocks for the parameters' gradients, params_blocks on the host.
-size_t params_of(const DiffArgs &g) {
-    return (g.dgain ? rnn_div_up(2 * (size_t)g.dh, 16) : 0) + (size_t)g.lam_heads;
+unsigned params_of(const DiffArgs &g) {
+    return g.first ? 0u : (g.dgain ? (2u * g.dh + 15u) / 16u : 0u) + (unsigned)g.lam_heads;
 }
 
 template <int DHP, bool VEC, int RG, int KG, int NM = 2>
 void launch_dq(rnn_ctx *ctx, const DiffArgs &g) {
     const size_t R = (size_t)g.tq * g.group;
-    const unsigned grid = (unsigned)((size_t)g.n * g.hkv * rnn_div_up(R, 32 * RG) + params_of(g));
-    diff_dq_kernel<DHP, VEC, RG, KG, NM><<<grid, 128 / NM * RG * KG, 0, ctx->stream>>>(g);
+    constexpr int threads = 128 / NM * RG * KG;
+    in_launches(g, (size_t)g.n * g.hkv * rnn_div_up(R, 32 * RG), threads, [&](const DiffArgs &a, unsigned blocks) {
+        diff_dq_kernel<DHP, VEC, RG, KG, NM><<<blocks + params_of(a), threads, 0, ctx->stream>>>(a);
+    });
 }
 template <int DHP, bool VEC, int KG>
 void launch_dkv(rnn_ctx *ctx, const DiffArgs &g) {
-    const unsigned grid = (unsigned)((size_t)g.n * g.hkv * rnn_div_up((size_t)g.tk, 32 * KG));
-    diff_dkv_kernel<DHP, VEC, KG><<<grid, 128 * KG, 0, ctx->stream>>>(g);
+    const size_t total = (size_t)g.n * g.hkv * rnn_div_up((size_t)g.tk, 32 * KG);
+    in_launches(g, total, 128 * KG, [&](const DiffArgs &a, unsigned blocks) {
+        diff_dkv_kernel<DHP, VEC, KG><<<blocks, 128 * KG, 0, ctx->stream>>>(a);
+    });
 }
 // Joint kernel for up to 64 rows where one tile holds the keys or problems fill the
 // CUs (128 x 4 heads of 64 rows on 256 keys 44 us, apart 29 + 51).
@@ -1988,11 +2006,12 @@ template <int DHP>
 void launch_bwd(rnn_ctx *ctx, const DiffArgs &g, bool vec) {
     const size_t probs = (size_t)g.n * g.hkv, R = (size_t)g.tq * g.group;
     if (vec && g.tq && R <= 64 && g.tk && (g.tk <= 64 || probs >= 256)) {
-        const unsigned grid = (unsigned)(probs + params_of(g));
-        if (g.tk <= 64)
-            diff_bwd_rows_kernel<DHP, true><<<grid, 256, 0, ctx->stream>>>(g);
-        else
-            diff_bwd_rows_kernel<DHP, false><<<grid, 256, 0, ctx->stream>>>(g);
+        in_launches(g, probs, 256, [&](const DiffArgs &a, unsigned blocks) {
+            if (g.tk <= 64)
+                diff_bwd_rows_kernel<DHP, true><<<blocks + params_of(a), 256, 0, ctx->stream>>>(a);
+            else
+                diff_bwd_rows_kernel<DHP, false><<<blocks + params_of(a), 256, 0, ctx->stream>>>(a);
+        });
         return;
     }
     if (g.tq) {

@@ -631,8 +631,9 @@ LinWs plan_ws(size_t rows, size_t fin, size_t fout) {
     return w;
 }
 
+// (2^30 rows would be a grid of 2^32 threads, which is one too many)
 int size_check(rnn_ctx *ctx, size_t rows, size_t fin, size_t fout) {
-    if (rows > (1u << 30) || fin > (1u << 20) || fout > (1u << 20))
+    if (rows > (1u << 30) - 128 || fin > (1u << 20) || fout > (1u << 20))
         return rnn_fail(ctx, RNN_E_UNSUPPORTED, "linear_act: %zu x %zu -> %zu", rows, fin, fout);
     return RNN_OK;
 }

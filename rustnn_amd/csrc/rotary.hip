@@ -33,6 +33,7 @@ struct RotArgs {
     int p0, p1;  // pairs of the first two axes
     int g1, g2;  // grid sides of the last two axes
     int rpb;     // rows of a block
+    int first;   // the launch's first row
     float sign;  // -1: the inverse
     // quarter turns per unit of position of every pair
     double w[MAX_PAIRS];
@@ -71,7 +72,7 @@ template <int G, bool INTER>
 __global__ __launch_bounds__(256) void rotary_kernel(RotArgs g) {
     const int R = g.npairs, turned = R / G, ng = turned + (g.dh - 2 * R) / G;
     const int units = g.hl * ng;
-    const int row0 = (int)blockIdx.x * g.rpb, nrow = min(g.rpb, g.rows - row0);
+    const int row0 = g.first + (int)blockIdx.x * g.rpb, nrow = min(g.rpb, g.rows - row0);
     for (int e = threadIdx.x; e < nrow * units; e += 256) {
         const int lr = e / units, u = e - lr * units;
         const int hl = u / ng, grp = u - hl * ng;
@@ -240,15 +241,20 @@ int rnn_rotary(rnn_ctx *ctx, const rnn_rotary_desc *d, size_t n, size_t t, const
     const int G = vec ? 4 : 1;
     const int units = g.hl * (g.npairs / G + (g.dh - 2 * g.npairs) / G);
     g.rpb = std::max(1, 256 / units);
-    const unsigned grid = (unsigned)rnn_div_up(rows, (size_t)g.rpb);
-    if (vec && d->interleaved)
-        rotary_kernel<4, true><<<grid, 256, 0, ctx->stream>>>(g);
-    else if (vec)
-        rotary_kernel<4, false><<<grid, 256, 0, ctx->stream>>>(g);
-    else if (d->interleaved)
-        rotary_kernel<1, true><<<grid, 256, 0, ctx->stream>>>(g);
-    else
-        rotary_kernel<1, false><<<grid, 256, 0, ctx->stream>>>(g);
+    // launches of at most 2^23 blocks, 2^31 threads (a grid holds below 2^32)
+    const size_t most = ((size_t)1 << 23) * (size_t)g.rpb;
+    for (size_t r = 0; r < rows; r += most) {
+        g.first = (int)r;
+        const unsigned grid = (unsigned)rnn_div_up(std::min(rows - r, most), (size_t)g.rpb);
+        if (vec && d->interleaved)
+            rotary_kernel<4, true><<<grid, 256, 0, ctx->stream>>>(g);
+        else if (vec)
+            rotary_kernel<4, false><<<grid, 256, 0, ctx->stream>>>(g);
+        else if (d->interleaved)
+            rotary_kernel<1, true><<<grid, 256, 0, ctx->stream>>>(g);
+        else
+            rotary_kernel<1, false><<<grid, 256, 0, ctx->stream>>>(g);
+    }
     RNN_LAUNCHED(ctx);
     return RNN_OK;
 }
