@@ -820,10 +820,11 @@ template <int W>
 __device__ __forceinline__ constexpr float ds_root() {
     return W == 32 ? 11.313709f : W == 64 ? 16.0f : W == 96 ? 19.595918f : 22.627417f;
 }
-// dmax: the larger |D_m|.
+// dmax: the larger |D_m|.  (At most 2^126, whose power is the smallest with a
+// reciprocal: ds_fit makes up for what is past it.)
 template <int W>
 __device__ __forceinline__ float ds_bound(float nd, float vmax, float dmax) {
-    return max2(nd * (ds_root<W>() * vmax), 2.0f * dmax);
+    return fminf(max2(nd * (ds_root<W>() * vmax), 2.0f * dmax), 0x1p126f);
 }
 __device__ __forceinline__ float ds_up(float m, float up) {
     return m * up < 2.0f ? up : up_of(m) * 0x1p-14f;
@@ -1631,8 +1632,8 @@ diff_bwd_rows_kernel(DiffArgs g) {
         const _Float16 *const k1 = kt + 32 * kg * Tile::STRIDE;
         Half2 ah[2], ds[2][2];
         f32x16 s[2];
-        // from the row's units, own's apart, to the rows' common ones
-        const float units = dup_of(row) * down_of(dup) * down_of(sup);
+        // what takes dS from the row's units, own's apart, to itself
+        const float units = dup_of(row) * down_of(dup) * down_of(sup) * down_of(pup);
         {
             f32x16 da;
 #pragma unroll
@@ -1755,7 +1756,7 @@ diff_bwd_rows_kernel(DiffArgs g) {
             if (key < g.tk)
                 put_channels<true>(kv + g.koff + kg * g.dh, g.dh, 32 * c, dk,
                                    down_of(qup) * (g.scale * sgn),
-                                   down_of(pup) * down_of(kg ? tup[1] : tup[0]), live, g.acc_kv);
+                                   down_of(kg ? tup[1] : tup[0]), live, g.acc_kv);
         }
     }
     // the halves of dQ that waves (rg, 0) and (rg, 1) have, dS's own powers of two off

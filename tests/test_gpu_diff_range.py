@@ -338,3 +338,14 @@ def test_large_scores(rnn, f, two):
     assert (got["y"].to(D) - want).norm() <= TOL * want.norm()
     for nm in ("dq", "dk", "dv", "dlam"):
         assert torch.isfinite(got[nm]).all(), nm
+
+
+@pytest.mark.parametrize("p", PATHS, ids=NAMES)
+def test_gradients_near_the_largest_float(rnn, p):
+    """dA of some 2^118: within a float's range, |dO| sqrt(W) max |V| past it."""
+    cs = path(p, seed=17, gain=False)
+    cs.vv *= 2.0 ** 60
+    cs.vv[:, p[6] // 2, :, 1] *= 2.0 ** 6
+    cs.dyv *= 2.0 ** 56
+    cs.qv[..., 0] = 0.0
+    check(cs, run(rnn, refill(cs)))
