@@ -220,7 +220,6 @@ struct Operand {
                 m[e] = largest<SET>(e);
                 y[e] = m[e] * up[e];
             }
-            if (!(absmax8(y, 0.f) >= 0x1p15f)) return;
         } else {
             float all = 0.f;
 #pragma unroll
@@ -233,10 +232,11 @@ struct Operand {
                 y[e] *= m[e];
             }
         }
+        if (!(absmax8(y, 0.f) >= 0x1p15f)) return;
         *over = t;
+        // (all eight, also those that are not past theirs: it changes nothing)
 #pragma unroll
-        for (int e = 0; e < 8; e++)
-            if (y[e] >= 0x1p15f) atomicMax(most + sc + e, __float_as_uint(m[e]));
+        for (int e = 0; e < 8; e++) atomicMax(most + e * Stage::C8 + sc / 8, __float_as_uint(m[e]));
     }
     // A set into the tile at t, the powers of two into ups; whether one changed.
     // !KC: last, the stage before's powers (null: before any); most, the stage's maxima
@@ -256,7 +256,7 @@ struct Operand {
             if (most) {
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    const float u = sticky_up(__uint_as_float(most[sc + e]), u8[e]);
+                    const float u = sticky_up(__uint_as_float(most[e * Stage::C8 + sc / 8]), u8[e]);
                     changed = changed || u != u8[e];
                     u8[e] = u;
                 }
@@ -320,17 +320,18 @@ struct Operand {
 // C[M x N] over k: a tile of BM x BN a workgroup, KB of k a stage, WM x WN x WK
 // waves (WK shares of a stage's depth, added at the end).  PRO: op(A) = a a2.
 template <int BM, int BN, int KB, int WM, int WN, int WK, bool AK, bool BK, bool PRO, int EPI>
-__global__ __launch_bounds__(64 * WM * WN * WK) __attribute__((amdgpu_waves_per_eu(BM == 32 && BN == 128 ? 1 : 2))) void
+__global__ __launch_bounds__(64 * WM * WN * WK) __attribute__((amdgpu_waves_per_eu(BM == 32 && BN == 128 ? 1 : BM == 128 && KB == 32 ? 4 : 2))) void
 linact_kernel(LinArgs g) {
     constexpr int NW = WM * WN * WK, NT = 64 * NW, MT = BM / 32 / WM, NN = BN / 32 / WN;
     constexpr int KS = KB / 16 / WK;
     using OA = Operand<BM, KB, AK, PRO, false, NT>;
-    using OB = Operand<BN, KB, BK, false, AK && !BK, NT>;
+    using OB = Operand<BN, KB, BK, false, AK && !BK && BM < 128, NT>;
     constexpr int STAGE = OA::HALVES + OB::HALVES;
     constexpr size_t LDS = std::max<size_t>(4 * STAGE, (size_t)WK * BM * BN * 4);
     __shared__ __align__(16) char lds_raw[LDS];
     // operands whose k runs across rows: the largest magnitudes of even and odd stages
-    // so far that were past their power, and the last stage that had one
+    // so far, where one was past its power (element e of thread column c at e C8 + c),
+    // and the last stage that had one
     __shared__ uint32_t most[2][BM + BN];
     __shared__ int over[2][2];
     // the powers of two of three stages (one is read, one may be compared with it,
