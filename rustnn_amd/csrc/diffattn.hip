@@ -247,10 +247,12 @@ __device__ __forceinline__ void put_channels(float *dst, int lim, int c0, const 
 // the one after it are in flight.  KH: two waves take half of each tile's keys and
 // join their sums at the end (wave 2 (QG h + i) + m).
 // A tile's chain bounds it (barrier, S, maximum, exponentials, split, P V) with two
-// waves a SIMD: 8 heads of 4096 rows and keys over 2 key heads, dh 64, 303 us, 227
+// waves a SIMD: 8 heads of 4096 rows and keys over 2 key heads, dh 64, 308 us, 223
 // TFLOP/s of fp32 work, the matrix cores busy half of the time (rnn_matmul 168);
-// small problems by memory: 128 x 4 heads of 64, dh 32, 18 us (50 MB), 64 rows on 256
-// keys 27.5 us (101 MB).  One query over 4 x 16384 keys, split, 30 us for 134 MB.
+// small problems by memory: 128 x 4 heads of 64, dh 32, 19 us (50 MB), 64 rows on 256
+// keys 28 us (101 MB).  One query over 4 images of up to 16384 keys, split, 31 us for
+// the 100 MB of three quarters of them: 3.2 TB/s, since splits are cut from tk, and
+// those past an image's length end at once while the others walk their tiles.
 // SPLIT: the keys [z TS, (z + 1) TS) alone (z = blockIdx.y), each map's own
 // normalised output, maximum and sum left for diff_join_kernel.
 template <int DHP, bool VEC, int QG, int KH, bool SPLIT>
@@ -626,7 +628,8 @@ __global__ __launch_bounds__(256) void diff_join_kernel(DiffArgs g, int splits) 
 // wave (LPU 64), two each; a group of lanes keeps one head, the groups in the
 // grid being a multiple of the heads.  In 64 bits up to dO's own rounding: dO is
 // perpendicular to O, so that D_2, whose sum dlambda is, is small beside its
-// terms.  Memory bounds it: 128 x 4 heads of 64, dh 32, 12 us (35 MB).
+// terms.  128 x 4 heads of 64, dh 32, 13 us: 7 for its 35 MB at a copy's rate, the
+// rest first loads, drain and the 64-bit reductions.
 template <int LPU>
 __device__ __forceinline__ double group_sum(double v) {
     v += rnn_dpp_d<0xB1>(v);
@@ -890,11 +893,12 @@ __device__ __forceinline__ int flip_at(int ntile) { return (2 * ntile + 2) / 3; 
 // rows (both, or a pair of waves one each, dA in both) and on one of the KG 32 keys
 // of a tile; tiles in two LDS buffers: S_m^T = K_m Q_m^T and dA^T = V dO^T (lane =
 // row), and P (dA - D) in registers is the operand of dQ_m^T = K_m^T dS_m^T, which
-// is summed over all tiles in the accumulators.  Their unit is a power of two that
-// hardly changes (sticky_up); where it does they are rescaled.  The waves that share
-// rows add theirs at the end.  Bound as the forward: 4 x 8 heads of 2048, dh 64, 436
-// us (236 TFLOP/s of fp32 work); 2 x 8 causal heads of 1568 104 us (145, the longest
-// rows' chain); 8 x 6 ragged of up to 577, dh 32, 40 us.
+// is summed over all tiles in the accumulators.  Their units are powers of two that
+// hardly change (sticky_up, ds_up, ds_fit); where one does they are rescaled.  The
+// waves that share rows add theirs at the end.  Bound as the forward: 4 x 8 heads of
+// 2048, dh 64, 498 us (207 TFLOP/s of fp32 work; the parts' powers by row cost a tenth
+// here); 2 x 8 causal heads of 1568 107 us (141, the longest rows' chain); 8 x 6
+// ragged of up to 577, dh 32, 42 us.
 template <int DHP, bool VEC, int RG, int KG, int NM>
 __global__ __launch_bounds__(128 / NM * RG * KG)
 __attribute__((amdgpu_waves_per_eu((DHP <= 32 && RG > 1) || NM == 1 ? 2 : 1))) void
@@ -1126,9 +1130,9 @@ diff_dq_kernel(DiffArgs g) {
 // through LDS, and then P and dS in registers are the operands of the wave's half
 // of dV^T = dO^T (P_1 - lambda P_2) and of dK_m^T = Q_m^T dS_m, summed over all tiles
 // in the accumulators as in diff_dq_kernel.
-// A tile's chain bounds it here too: 4 x 8 heads of 2048, dh 64, 578 us (238 TFLOP/s
-// of fp32 work); 2 x 8 causal heads of 1568 167 us (120); 8 x 6 ragged of up to 577,
-// dh 32, 56 us.
+// A tile's chain bounds it here too: 4 x 8 heads of 2048, dh 64, 567 us (243 TFLOP/s
+// of fp32 work); 2 x 8 causal heads of 1568 180 us (111); 8 x 6 ragged of up to 577,
+// dh 32, 60 us.
 template <int DHP, bool VEC, int KG>
 __global__ __launch_bounds__(128 * KG) __attribute__((amdgpu_waves_per_eu(DHP <= 32 && KG > 1 ? 2 : 1))) void
 diff_dkv_kernel(DiffArgs g) {
@@ -1465,9 +1469,12 @@ __device__ __forceinline__ void dot_tiles(const _Float16 *ta, int ca, const _Flo
 // dQ as diff_dq_kernel does; P_1 - lambda P_2 and dS_m go through LDS where the tile
 // has been read for the last time, row by row, and come back transposed as
 // operands of dV and dK, whose blocks of 32 keys and 32 channels the waves share
-// out.  ONE: one tile holds the keys.  Memory bounds it: 128 x 4 heads of 64 rows and keys, dh 32, 20.5 us (60 MB;
-// 12 at a copy's rate) where dQ and dK/dV apart took 18.7 + 18.3; 64 rows on 256
-// keys 44.3 us (160 MB; 32) instead of 28.7 + 50.8.
+// out.  dO and dS have powers of two by row where a sum runs along one (dA, dQ), and
+// common ones where it runs over the rows (dV through P's, dK with dS split again).
+// ONE: one tile holds the keys.  A tile's chain of loads, splits, products and six
+// barriers bounds it, with two workgroups a CU up to 32 channels: 128 x 4 heads of 64
+// rows and keys, dh 32, 22 us (60 MB; 12 at a copy's rate) where dQ and dK/dV apart
+// take 19.0 + 18.7; 64 rows on 256 keys 47 us (160 MB; 32) instead of 29.3 + 52.9.
 template <int DHP, bool ONE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DHP <= 32 ? 2 : 1))) void
 diff_bwd_rows_kernel(DiffArgs g) {
@@ -1996,13 +2003,14 @@ void launch_dkv(rnn_ctx *ctx, const DiffArgs &g) {
     });
 }
 // Joint kernel for up to 64 rows where one tile holds the keys or problems fill the
-// CUs (128 x 4 heads of 64 rows on 256 keys 44 us, apart 29 + 51).
+// CUs (128 x 4 heads of 64 rows on 256 keys 47 us, apart 29 + 53).
 // dQ: two waves share 32 rows where four groups of 32 would not fill the CUs (2 x 8
-// causal heads of 1568, dh 64: 104 us against 160; 8 x 6 of 577, dh 32: 39.6 against
-// 38.0; 4 x 8 of 2048, dh 64: 515 against 436; 32 x 8 of 256, dh 64: 114 against 81).
+// causal heads of 1568, dh 64: 108 us against 173; 8 x 6 of 577, dh 32: 42.0 against
+// 42.4; 4 x 8 of 2048, dh 64: 503 against 500; 32 x 8 of 256, dh 64: 123 against 91).
 // dK and dV: four waves on two groups of 32 keys; above 32 channels, where a CU
-// holds one workgroup, eight on four where those fill the CUs (the same four: 188
-// against 167 us; 55.1 against 56.5; 578 against 870; 97 against 140).
+// holds one workgroup, eight on four where those fill the CUs (eight against four in
+// the same cases: 195 against 182 us; 58.3 against 59.0; 569 against 917; 103 against
+// 159).  Operands that are not whole float4s take one plan each, unmeasured.
 template <int DHP>
 void launch_bwd(rnn_ctx *ctx, const DiffArgs &g, bool vec) {
     const size_t probs = (size_t)g.n * g.hkv, R = (size_t)g.tq * g.group;

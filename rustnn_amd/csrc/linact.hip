@@ -319,8 +319,11 @@ struct Operand {
 
 // C[M x N] over k: a tile of BM x BN a workgroup, KB of k a stage, WM x WN x WK
 // waves (WK shares of a stage's depth, added at the end).  PRO: op(A) = a a2.
+// Waves a SIMD: two workgroups a CU for the 128 x 128 tile of y and dX (dX of 8192 x
+// 1152 -> 1152 136 us, 165 with one).
 template <int BM, int BN, int KB, int WM, int WN, int WK, bool AK, bool BK, bool PRO, int EPI>
-__global__ __launch_bounds__(64 * WM * WN * WK) __attribute__((amdgpu_waves_per_eu(BM == 32 && BN == 128 ? 1 : BM == 128 && KB == 32 ? 4 : 2))) void
+__global__ __launch_bounds__(64 * WM * WN * WK)
+__attribute__((amdgpu_waves_per_eu(BM == 32 && BN == 128 ? 1 : BM == 128 && KB == 32 ? 4 : 2))) void
 linact_kernel(LinArgs g) {
     constexpr int NW = WM * WN * WK, NT = 64 * NW, MT = BM / 32 / WM, NN = BN / 32 / WN;
     constexpr int KS = KB / 16 / WK;
@@ -564,8 +567,8 @@ __global__ __launch_bounds__(256) void linact_reduce_kernel(const float *__restr
 // The tile of y and dX by the number of tiles that it leaves: the largest that
 // gives the 256 CUs about one each; in the smaller ones waves share a stage's
 // depth.  Forward 8192 x 256 -> 1024 with 128 x 128 / 64 x 128 / 32 x 128 tiles:
-// 30.2 / 47.9 / 83.8 us; 1813 x 387 -> 1003: 27.3 / 19.8 / 35.1.  dX of these:
-// 48.4 / 33.4 / 58.5 and 56.3 / 33.2 / 30.5 us.
+// 30.2 / 49.0 / 86.9 us; 1813 x 387 -> 1003: 26.8 / 20.1 / 35.5.  dX of these:
+// 50.6 / 33.0 / 57.8 and 57.6 / 32.0 / 30.3 us.
 enum { TILE_128, TILE_64X128, TILE_32X128, TILE_32 };
 int pick_tile(size_t m, size_t n) {
     auto tiles = [&](size_t bm, size_t bn) { return rnn_div_up(m, bm) * rnn_div_up(n, bn); };
@@ -592,8 +595,8 @@ void launch(rnn_ctx *ctx, const LinArgs &g) {
 }
 
 // dW's tile and the splits of its k (the rows), at least 128 rows each: about one
-// workgroup a CU.  8192 x 256 -> 1024 with 128 x 128 / 64 x 128 / 64 x 64 tiles:
-// 34.8 / 39.8 / 39.9 us; twice the splits 36 and more to add up.
+// workgroup a CU.  8192 x 256 -> 1024 with 128 x 128 / 64 x 64 tiles: 36 + 7 / 59 + 5
+// us with the splits' sum; twice the splits 47 + 12.
 struct DwPlan {
     bool wide;  // 128 x 128, else 64 x 64
     size_t nz, kchunk;

@@ -278,13 +278,12 @@ def test_what_is_not_finite_shows(rnn, f, bad):
             assert torch.equal(y, view(clean)), ("key", m, key)
 
 
-@pytest.mark.parametrize("f", FORWARD, ids=[f[0] for f in FORWARD])
+@pytest.mark.parametrize("f", [f for f in FORWARD if f[5] >= 40],
+                         ids=[f[0] for f in FORWARD if f[5] >= 40])
 def test_hidden_keys_that_are_not_finite(rnn, f):
-    """Keys (not values) that a mask hides from a row may hold anything finite
-    or not: causal rows before such a key stay as they were, to the rounding of
-    another power of two."""
-    if f[5] < 40:
-        pytest.skip("every row sees the key")
+    """Keys (not values) that a mask hides from a row may hold anything, finite or
+    not: causal rows before such a key stay as they were, to the rounding of
+    another power of two.  (With fewer rows, every row sees the key.)"""
     for bad in (float("nan"), float("inf")):
         cs = path(f, seed=13, causal=True)
         want = formulas(cs)["y"]
