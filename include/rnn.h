@@ -281,6 +281,8 @@ int rnn_rotary(rnn_ctx *ctx, const rnn_rotary_desc *d, size_t n, size_t t, const
  * sees no key, and a padding query, give y = 0.  A NaN or an infinity gives NaN:
  * in a query to its row, in a key to every row that sees it, in a value to rows
  * that do not see it as well, in dy to its row of dq and to what sums over rows.
+ * (An infinity also leaves its image's other keys steps of 2^-24, and NaN past
+ * 2^15; its other values, in rows that are not NaN already, 2^-20 and 2^19.)
  * So do scores past a float's range.  The backward forms P again from scores that
  * are within 2^-22 of themselves: those above 2^15 leave it few bits.
  * Products are taken in two fp16 parts under a power of two (of a row, of
