@@ -262,6 +262,98 @@ int rnn_rotary_check(const rnn_rotary_desc *d, size_t n, size_t t, int have_pos)
 int rnn_rotary(rnn_ctx *ctx, const rnn_rotary_desc *d, size_t n, size_t t, const float *x,
                const float *pos, float *y, int inverse);
 
+/* Norm and rotary position of each head in one pass (no counterpart in the
+ * reference): of the h heads of a row (h, dh, the positions and the layouts of x
+ * and y as rnn_rotary takes them), the first hq are queries, the rest keys.
+ *   x^ = x / sqrt(mean(x^2) + eps),  y = turn(gain x^)
+ * gain [2][dh]: queries', keys' (NULL: 1).  Channels past the pairs are normed and
+ * not turned.  dh <= 256 (RNN_E_UNSUPPORTED above), eps > 0.  Squares are summed in
+ * 64 bits, so that heads of any size keep their norm.  A NaN gives NaN in its
+ * head, an infinity in its channel's pair and zeros in the others of its head.
+ * y may be x when strides and offsets agree, else the two must not overlap. */
+int rnn_norm_rotary_forward(rnn_ctx *ctx, const rnn_rotary_desc *d, uint32_t hq, float eps, size_t n,
+                            size_t t, const float *x, const float *gain, const float *pos, float *y);
+/* Checks the arguments and gives the bytes of device workspace that a backward
+ * with dgain needs; host only.  The workspace is the caller's, 256-byte aligned,
+ * holds nothing between calls and is not shared by calls that may run at the same
+ * time. */
+int rnn_norm_rotary_workspace(const rnn_rotary_desc *d, uint32_t hq, float eps, size_t n, size_t t,
+                              int have_pos, size_t *bytes);
+/* From the forward's input x and dy (rows of dystride floats, heads from dyoff on):
+ * dx, laid out as y, is overwritten; dgain [2][dh] (NULL: not wanted) accumulates,
+ * in a fixed order.  dx may be dy when their layouts agree and overlaps nothing
+ * else. */
+int rnn_norm_rotary_backward(rnn_ctx *ctx, const rnn_rotary_desc *d, uint32_t hq, float eps, size_t n,
+                             size_t t, const float *x, const float *gain, const float *pos,
+                             const float *dy, size_t dystride, size_t dyoff, void *ws, size_t ws_bytes,
+                             float *dx, float *dgain);
+
+/* Norm of each head times SiLU of a gate (no counterpart in the reference): rows
+ * of h heads of d channels, x and y [rows][h][d], z at z + r*zstride + zoff.
+ *   y = gain x / sqrt(mean(x^2) + eps) z / (1 + exp(-z))
+ * gain [h][d] (NULL: 1); the mean is a head's.  d <= 512, h <= 65536, eps > 0.  y
+ * may be x. */
+int rnn_head_gate_forward(rnn_ctx *ctx, size_t rows, size_t h, size_t d, float eps, const float *x,
+                          const float *z, size_t zstride, size_t zoff, const float *gain, float *y);
+/* Bytes of device workspace that a backward with dgain needs, as
+ * rnn_norm_rotary_workspace; host only. */
+int rnn_head_gate_workspace(size_t rows, size_t h, size_t d, size_t *bytes);
+/* Its backward: dx [rows][h][d] and dz (at dz + r*dzstride + dzoff) are
+ * overwritten, dgain [h][d] (NULL: not wanted) accumulates in a fixed order.  dx
+ * may be dy or x, dz may be z where their layouts agree. */
+int rnn_head_gate_backward(rnn_ctx *ctx, size_t rows, size_t h, size_t d, float eps, const float *x,
+                           const float *z, size_t zstride, size_t zoff, const float *gain,
+                           const float *dy, void *ws, size_t ws_bytes, float *dx, float *dz,
+                           size_t dzstride, size_t dzoff, float *dgain);
+
+/* ----------------------------------------------- linear attention with decay */
+/* Linear attention with a decay for each head (no counterpart in the reference).
+ * Head j reads queries of dk channels at q + r*qstride + qoff + j*dk; key head
+ * g = j / (h / hkv) has keys at kv + r*kvstride + koff + g*dk and values of dv
+ * channels at kv + r*kvstride + voff + g*dv.  With gamma_j = exp(-exp(rate[j])),
+ * over the tokens i of a sequence in order,
+ *   S_i = gamma S_(i-1) + k_i^T v_i,   y_i = scale q_i S_i
+ * which is y_i = scale sum_(l <= i) gamma^(i-l) (q_i . k_l) v_l.  The last
+ * `reverse` heads take the tokens from the last to the first.
+ * Sequence b has min(lens[b], t) tokens (device array; NULL: t): rows behind them
+ * are padding, which is never read and may hold anything; y is 0 there.
+ * state_in [n][h][dk][dv] is S before the first token (NULL: 0), state_out S
+ * after the last (NULL: not wanted; may be state_in): a sequence may be given in
+ * pieces, or token by token.  gamma is within [0, 1] for any rate; -infinity: 1, no
+ * decay.  Products are fp32 and so are states; powers of gamma are formed in 64
+ * bits.  A NaN or an infinity shows in the tokens that see it and in no others. */
+typedef struct {
+    uint32_t h, hkv, dk, dv;
+    size_t qstride, qoff, kvstride, koff, voff;
+    uint32_t reverse;
+    float scale;
+} rnn_decay_attn_desc;
+/* Checks a description and gives the bytes of device workspace that the forward
+ * (backward = 0) or the backward needs for n sequences of t tokens; host only.
+ * The workspace is the caller's, 256-byte aligned, holds nothing between calls
+ * and is not shared by calls that may run at the same time.  dk and dv <= 128, row
+ * strides <= 2^22, n * t * h and n * h * dk * dv < 2^31 (RNN_E_UNSUPPORTED above),
+ * scale finite. */
+int rnn_decay_attn_workspace(const rnn_decay_attn_desc *d, size_t n, size_t t, int backward,
+                             size_t *bytes);
+/* y [n][t][h][dv]. */
+int rnn_decay_attn_forward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n, size_t t,
+                           const float *q, const float *kv, const float *rate, const uint32_t *lens,
+                           const float *state_in, void *ws, size_t ws_bytes, float *y,
+                           float *state_out);
+/* From the forward's inputs, dy [n][t][h][dv] and, where state_out was used, its
+ * gradient dstate_out (NULL: 0): dq and dkv, laid out as q and kv, ACCUMULATE or are
+ * overwritten as flags say (RNN_ATTN_SET_DQ, RNN_ATTN_SET_DKV: the columns of
+ * queries, or of keys and values, padding rows included, which receive 0); drate
+ * [h] (NULL: not wanted) accumulates; dstate_in (NULL: not wanted) is overwritten.
+ * dq and dkv may be one buffer with disjoint columns; neither they nor dstate_in
+ * overlap another operand.  Sums run in a fixed order. */
+int rnn_decay_attn_backward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n, size_t t,
+                            const float *q, const float *kv, const float *rate, const uint32_t *lens,
+                            const float *state_in, const float *dy, const float *dstate_out, void *ws,
+                            size_t ws_bytes, float *dq, float *dkv, float *drate, float *dstate_in,
+                            uint32_t flags);
+
 /* -------------------------------------------------- differential attention */
 /* Differential attention (no counterpart in the reference): the difference of
  * two softmax maps, with a norm over each head's output.  Head j has two query

@@ -11,6 +11,9 @@ reference's host interface for the hot path:
 * ``Rotary``, ``DiffCore``, ``linear_act_forward`` / ``linear_act_backward``:
   rotary positions, differential attention and the Linear product with an
   activation and a residual (no counterpart in the reference)
+* ``NormRotary``, ``DecayCore``, ``HeadGate``: head norms with rotary positions,
+  linear attention with a decay for each head, normed and gated head outputs
+  (no counterpart in the reference)
 * ``rustnn_amd.nn``: BatchNorm2d, the classifier Linear, gap, softmax_ce,
   Param::step                                           -- nn.rs:37-637
 * ``rustnn_amd.model.ResNet``: the device-resident train step -- model.rs
@@ -99,6 +102,13 @@ class RotaryDesc(C.Structure):
                                   ] + [("interleaved", _i), ("base", C.c_float)]
 
 
+class DecayAttnDesc(C.Structure):
+    """rnn_decay_attn_desc."""
+    _fields_ = [(k, _u32) for k in ("h", "hkv", "dk", "dv")] + [
+        (k, _sz) for k in ("qstride", "qoff", "kvstride", "koff", "voff")] + [
+        ("reverse", _u32), ("scale", C.c_float)]
+
+
 class DiffAttnDesc(C.Structure):
     """rnn_diff_attn_desc."""
     _fields_ = [(k, _u32) for k in ("h", "hkv", "dh", "tq", "tk")] + [
@@ -158,6 +168,22 @@ def lib():
                                           _vp, _vp, _vp, _u32]),
             "rnn_rotary_check": (_i, [P(RotaryDesc), _sz, _sz, _i]),
             "rnn_rotary": (_i, [_vp, P(RotaryDesc), _sz, _sz, _vp, _vp, _vp, _i]),
+            "rnn_norm_rotary_forward": (_i, [_vp, P(RotaryDesc), _u32, C.c_float, _sz, _sz] +
+                                        [_vp] * 4),
+            "rnn_norm_rotary_workspace": (_i, [P(RotaryDesc), _u32, C.c_float, _sz, _sz, _i,
+                                               P(_sz)]),
+            "rnn_norm_rotary_backward": (_i, [_vp, P(RotaryDesc), _u32, C.c_float, _sz, _sz] +
+                                         [_vp] * 4 + [_sz, _sz, _vp, _sz, _vp, _vp]),
+            "rnn_head_gate_forward": (_i, [_vp, _sz, _sz, _sz, C.c_float, _vp, _vp, _sz, _sz, _vp,
+                                           _vp]),
+            "rnn_head_gate_workspace": (_i, [_sz, _sz, _sz, P(_sz)]),
+            "rnn_head_gate_backward": (_i, [_vp, _sz, _sz, _sz, C.c_float, _vp, _vp, _sz, _sz, _vp,
+                                            _vp, _vp, _sz, _vp, _vp, _sz, _sz, _vp]),
+            "rnn_decay_attn_workspace": (_i, [P(DecayAttnDesc), _sz, _sz, _i, P(_sz)]),
+            "rnn_decay_attn_forward": (_i, [_vp, P(DecayAttnDesc), _sz, _sz] + [_vp] * 6 +
+                                       [_sz, _vp, _vp]),
+            "rnn_decay_attn_backward": (_i, [_vp, P(DecayAttnDesc), _sz, _sz] + [_vp] * 8 +
+                                        [_sz, _vp, _vp, _vp, _vp, _u32]),
             "rnn_diff_attn_workspace": (_i, [P(DiffAttnDesc), _sz, _i, P(_sz)]),
             "rnn_diff_attn_forward": (_i, [_vp, P(DiffAttnDesc), _sz] + [_vp] * 7 +
                                       [_sz, _vp, _vp, _vp]),
@@ -947,6 +973,261 @@ class DiffCore:
                 ctx.h, C.byref(d), n, *ins, ws.data_ptr() if nb else None, nb, *outs, flags))
         finally:
             on.done(q, kv, lam, gain, qlen, klen, ws, dy, o12, stats, dq, dkv, dlam, dgain)
+
+
+class NormRotary:
+    """The norm of each query and key head and its rotary position in one pass
+    (rnn_norm_rotary_*): heads 0 .. hq - 1 of a row are queries, the hk after
+    them keys, of dh channels each; grid, base, pairs and interleaved as Rotary
+    takes them.  gain [2, dh]: the queries' and the keys' (None: 1)."""
+
+    def __init__(self, hq, hk, dh, grid, base=10000.0, pairs=None, interleaved=False, eps=1e-6,
+                 ctx=None):
+        self.hq, self.hk, self.eps, self.ctx = int(hq), int(hk), float(eps), ctx
+        if min(self.hq, self.hk) < 0:
+            raise ValueError("NormRotary: a negative size")
+        self.rot = Rotary(self.hq + self.hk, dh, grid, base, pairs, interleaved, ctx)
+        self.heads, self.dh, self.t = self.rot.heads, self.rot.dh, self.rot.t
+        self._ws = {}  # workspace bytes by rows and positions
+        self._plan(1, self.t, False, (self.heads * self.dh, 0, self.heads * self.dh, 0))
+
+    def _plan(self, n, t, have_pos, layout):
+        """(the C description, workspace bytes of a backward)."""
+        d = self.rot._desc(*layout)
+        nb = self._ws.get((n, t, have_pos, layout))
+        if nb is None:
+            out = _sz()
+            rc = lib().rnn_norm_rotary_workspace(C.byref(d), self.hq, self.eps, n, t, int(have_pos),
+                                                 C.byref(out))
+            if rc:
+                raise ValueError(f"NormRotary: {lib().rnn_status_string(rc).decode()} (hq={self.hq} "
+                                 f"hk={self.hk} dh={self.dh} grid={self.rot.grid} eps={self.eps} "
+                                 f"n={n} t={t} layout={layout})")
+            nb = self._ws[n, t, have_pos, layout] = out.value
+        return d, nb
+
+    def _out(self, like, n, t, y, ystride, yoff, xstride, xoff):
+        import torch
+        if y is None:
+            w = self.heads * self.dh
+            return torch.empty(n, t, w, dtype=torch.float32, device=like.device), w, 0
+        return (y, xstride, xoff) if ystride is None else (y, ystride, yoff)
+
+    def forward(self, n, x, xstride, xoff=0, gain=None, pos=None, y=None, ystride=None, yoff=0,
+                t=None):
+        """Norms and turns the heads at x[r * xstride + xoff ...] of n images;
+        writes y (x: in place, which a backward cannot follow; None: a new
+        [n, t, (hq + hk) dh]), at the same layout unless ystride is given.
+        pos and t as Rotary's."""
+        ctx, w = self.ctx or default_ctx(x.device.index or 0), self.heads * self.dh
+        t = self.t if t is None else int(t)
+        y, ystride, yoff = self._out(x, n, t, y, ystride, yoff, xstride, xoff)
+        d, _ = self._plan(n, t, pos is not None, (xstride, xoff, ystride, yoff))
+        rows = n * t
+        need = lambda stride, off: (rows - 1) * stride + off + w if rows else 0
+        args = (_arg(ctx, x, need(xstride, xoff), "x"), _arg(ctx, gain, 2 * self.dh, "gain"),
+                _arg(ctx, pos, rows * len(self.rot.grid), "pos"),
+                _arg(ctx, y, need(ystride, yoff), "y"))
+        on = _OnStream(ctx)
+        try:
+            ctx.check(lib().rnn_norm_rotary_forward(ctx.h, C.byref(d), self.hq, self.eps, n, t,
+                                                    *args))
+        finally:
+            on.done(x, gain, pos, y)
+        return y
+
+    def backward(self, n, x, xstride, xoff, gain, dy, dystride, dyoff=0, dgain=None, pos=None,
+                 dx=None, dxstride=None, dxoff=0, t=None):
+        """dx (returned) from the forward's input x and dy; dx given: at dy's
+        layout unless dxstride is (dy: in place).  dgain [2, dh] accumulates."""
+        import torch
+        ctx, w = self.ctx or default_ctx(x.device.index or 0), self.heads * self.dh
+        t = self.t if t is None else int(t)
+        dx, dxstride, dxoff = self._out(x, n, t, dx, dxstride, dxoff, dystride, dyoff)
+        d, nb = self._plan(n, t, pos is not None, (xstride, xoff, dxstride, dxoff))
+        rows = n * t
+        need = lambda stride, off: (rows - 1) * stride + off + w if rows else 0
+        nb = nb if dgain is not None else 0
+        ws = torch.empty(nb, dtype=torch.uint8, device=x.device) if nb else None
+        args = (_arg(ctx, x, need(xstride, xoff), "x"), _arg(ctx, gain, 2 * self.dh, "gain"),
+                _arg(ctx, pos, rows * len(self.rot.grid), "pos"),
+                _arg(ctx, dy, need(dystride, dyoff), "dy"), dystride, dyoff,
+                ws.data_ptr() if nb else None, nb, _arg(ctx, dx, need(dxstride, dxoff), "dx"),
+                _arg(ctx, dgain, 2 * self.dh, "dgain"))
+        on = _OnStream(ctx)
+        try:
+            ctx.check(lib().rnn_norm_rotary_backward(ctx.h, C.byref(d), self.hq, self.eps, n, t,
+                                                     *args))
+        finally:
+            on.done(x, gain, pos, dy, ws, dx, dgain)
+        return dx
+
+
+class DecayCore:
+    """Linear attention with a decay for each head (rnn_decay_attn_*):
+    S_i = gamma S_(i-1) + k_i^T v_i, y_i = scale q_i S_i with gamma_j =
+    exp(-exp(rate[j])), h query heads on hkv key heads of dk and value heads of
+    dv channels; the last ``reverse`` heads take a sequence's tokens from the
+    last to the first.  forward / backward take q and kv as Core's: a buffer
+    with its row stride and the first channel of the queries, and of the keys
+    and values.  scale: default 1 / sqrt(dk)."""
+
+    def __init__(self, h, dk, dv=None, hkv=None, reverse=0, scale=None, ctx=None):
+        self.h, self.dk = int(h), int(dk)
+        self.dv = self.dk if dv is None else int(dv)
+        self.hkv = self.h if hkv is None else int(hkv)
+        self.reverse = int(reverse)
+        if min(self.h, self.dk, self.dv, self.hkv, self.reverse) < 0:
+            raise ValueError("DecayCore: a negative size")
+        self.scale = 1.0 / math.sqrt(max(self.dk, 1)) if scale is None else float(scale)
+        self.ctx = ctx
+        self.c = self.h * self.dv
+        self._plans = {}  # the C description and workspace of each layout and size
+        kw = self.hkv * self.dk
+        self._plan(1, 1, 0, (self.h * self.dk, 0, kw + self.hkv * self.dv, 0, kw))
+
+    def desc(self, qstride, qoff, kvstride, koff, voff):
+        return DecayAttnDesc(self.h, self.hkv, self.dk, self.dv, qstride, qoff, kvstride, koff, voff,
+                             self.reverse, self.scale)
+
+    def _plan(self, n, t, backward, layout):
+        """(description, workspace bytes, floats of q and of kv that it spans)."""
+        p = self._plans.get((n, t, backward, layout))
+        if p is not None:
+            return p
+        d, nb = self.desc(*layout), _sz()
+        rc = lib().rnn_decay_attn_workspace(C.byref(d), n, t, backward, C.byref(nb))
+        if rc:
+            raise ValueError(f"DecayCore: {lib().rnn_status_string(rc).decode()} (h={self.h} "
+                             f"hkv={self.hkv} dk={self.dk} dv={self.dv} reverse={self.reverse} "
+                             f"scale={self.scale} n={n} t={t} layout={layout})")
+        rows = n * t
+        nq = (rows - 1) * d.qstride + d.qoff + self.h * self.dk if rows else 0
+        nkv = ((rows - 1) * d.kvstride + max(d.koff + self.hkv * self.dk,
+                                             d.voff + self.hkv * self.dv) if rows else 0)
+        p = self._plans[n, t, backward, layout] = d, nb.value, nq, nkv
+        return p
+
+    def _inputs(self, ctx, n, nq, nkv, q, kv, rate, lens, state):
+        return (_arg(ctx, q, nq, "q"), _arg(ctx, kv, nkv, "kv"), _arg(ctx, rate, self.h, "rate"),
+                _arg(ctx, lens, n, "lens", "u32"),
+                _arg(ctx, state, n * self.h * self.dk * self.dv, "state"))
+
+    def forward(self, n, t, q, qstride, qoff, kv, kvstride, koff, voff, rate, lens=None, state=None,
+                keep_state=False, state_out=None, y=None):
+        """(y [n, t, h dv], the state after the last token [n, h, dk, dv]: None
+        unless keep_state or state_out, which may be state).  lens (int32 /
+        uint32 [n]): the sequences' lengths where they are padded."""
+        import torch
+        ctx = self.ctx or default_ctx(q.device.index or 0)
+        d, nb, nq, nkv = self._plan(n, t, 0, (qstride, qoff, kvstride, koff, voff))
+        ins = self._inputs(ctx, n, nq, nkv, q, kv, rate, lens, state)
+        if y is None:
+            y = torch.empty(n, t, self.c, dtype=torch.float32, device=q.device)
+        if state_out is None and keep_state:
+            state_out = torch.empty(n, self.h, self.dk, self.dv, dtype=torch.float32,
+                                    device=q.device)
+        ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None
+        outs = (_arg(ctx, y, n * t * self.c, "y"),
+                _arg(ctx, state_out, n * self.h * self.dk * self.dv, "state_out"))
+        on = _OnStream(ctx)
+        try:
+            ctx.check(lib().rnn_decay_attn_forward(
+                ctx.h, C.byref(d), n, t, *ins, ws.data_ptr() if nb else None, nb, *outs))
+        finally:
+            on.done(q, kv, rate, lens, state, ws, y, state_out)
+        return y, state_out
+
+    def backward(self, n, t, q, qstride, qoff, kv, kvstride, koff, voff, rate, dy, dq, dkv,
+                 drate=None, lens=None, state=None, dstate_out=None, dstate=None, set_dq=False,
+                 set_dkv=False):
+        """Accumulates into dq, dkv (laid out as q, kv) and drate; set_dq /
+        set_dkv overwrite dq / dkv instead.  dstate_out: the gradient of the
+        state that forward returned; dstate receives the given state's."""
+        import torch
+        ctx = self.ctx or default_ctx(dy.device.index or 0)
+        d, nb, nq, nkv = self._plan(n, t, 1, (qstride, qoff, kvstride, koff, voff))
+        ins = self._inputs(ctx, n, nq, nkv, q, kv, rate, lens, state)
+        ws = torch.empty(nb, dtype=torch.uint8, device=dy.device) if nb else None
+        flags = (RNN_ATTN_SET_DQ if set_dq else 0) | (RNN_ATTN_SET_DKV if set_dkv else 0)
+        st = n * self.h * self.dk * self.dv
+        ins += (_arg(ctx, dy, n * t * self.c, "dy"), _arg(ctx, dstate_out, st, "dstate_out"))
+        outs = (_arg(ctx, dq, nq, "dq"), _arg(ctx, dkv, nkv, "dkv"),
+                _arg(ctx, drate, self.h, "drate"), _arg(ctx, dstate, st, "dstate"))
+        on = _OnStream(ctx)
+        try:
+            ctx.check(lib().rnn_decay_attn_backward(
+                ctx.h, C.byref(d), n, t, *ins, ws.data_ptr() if nb else None, nb, *outs, flags))
+        finally:
+            on.done(q, kv, rate, lens, state, ws, dy, dstate_out, dq, dkv, drate, dstate)
+
+
+class HeadGate:
+    """The norm of each head times SiLU of a gate (rnn_head_gate_*): y =
+    gain x / sqrt(mean(x^2) + eps) silu(z) over h heads of d channels; x and y
+    [rows, h d], z in rows of zstride floats from zoff on, gain [h d] (None: 1)."""
+
+    def __init__(self, h, d, eps=1e-6, ctx=None):
+        self.h, self.d, self.eps, self.ctx = int(h), int(d), float(eps), ctx
+        self.c = self.h * self.d
+        if min(self.h, self.d) < 0:
+            raise ValueError("HeadGate: a negative size")
+        if not (self.eps > 0.0 and math.isfinite(self.eps)):
+            raise ValueError(f"HeadGate: eps={eps}")
+        self._ws = {}  # workspace bytes by rows
+        self._bytes(1)
+
+    def _bytes(self, rows):
+        nb = self._ws.get(rows)
+        if nb is None:
+            out = _sz()
+            rc = lib().rnn_head_gate_workspace(rows, self.h, self.d, C.byref(out))
+            if rc:
+                raise ValueError(f"HeadGate: {lib().rnn_status_string(rc).decode()} (rows={rows} "
+                                 f"h={self.h} d={self.d})")
+            nb = self._ws[rows] = out.value
+        return nb
+
+    def _need(self, rows, stride, off):
+        return (rows - 1) * stride + off + self.c if rows else 0
+
+    def forward(self, rows, x, z, zstride, zoff=0, gain=None, y=None):
+        """y (returned; x: in place, which a backward cannot follow)."""
+        import torch
+        ctx = self.ctx or default_ctx(x.device.index or 0)
+        self._bytes(rows)
+        if y is None:
+            y = torch.empty(rows, self.c, dtype=torch.float32, device=x.device)
+        args = (_arg(ctx, x, rows * self.c, "x"), _arg(ctx, z, self._need(rows, zstride, zoff), "z"),
+                zstride, zoff, _arg(ctx, gain, self.c, "gain"), _arg(ctx, y, rows * self.c, "y"))
+        on = _OnStream(ctx)
+        try:
+            ctx.check(lib().rnn_head_gate_forward(ctx.h, rows, self.h, self.d, self.eps, *args))
+        finally:
+            on.done(x, z, gain, y)
+        return y
+
+    def backward(self, rows, x, z, zstride, zoff, gain, dy, dz, dzstride, dzoff=0, dgain=None,
+                 dx=None):
+        """dx (returned) and dz, in rows of dzstride floats from dzoff on, are
+        overwritten; dgain [h d] accumulates."""
+        import torch
+        ctx = self.ctx or default_ctx(x.device.index or 0)
+        nb = self._bytes(rows) if dgain is not None else 0
+        if dx is None:
+            dx = torch.empty(rows, self.c, dtype=torch.float32, device=x.device)
+        ws = torch.empty(nb, dtype=torch.uint8, device=x.device) if nb else None
+        args = (_arg(ctx, x, rows * self.c, "x"), _arg(ctx, z, self._need(rows, zstride, zoff), "z"),
+                zstride, zoff, _arg(ctx, gain, self.c, "gain"), _arg(ctx, dy, rows * self.c, "dy"),
+                ws.data_ptr() if nb else None, nb, _arg(ctx, dx, rows * self.c, "dx"),
+                _arg(ctx, dz, self._need(rows, dzstride, dzoff), "dz"), dzstride, dzoff,
+                _arg(ctx, dgain, self.c, "dgain"))
+        on = _OnStream(ctx)
+        try:
+            ctx.check(lib().rnn_head_gate_backward(ctx.h, rows, self.h, self.d, self.eps, *args))
+        finally:
+            on.done(x, z, gain, dy, ws, dx, dz, dgain)
+        return dx
 
 
 # ------------------------------------------------------------------ linear.rs

@@ -1,27 +1,19 @@
 // Rotary positions with up to three axes (time, height, width) on the heads
 // of a token row (rnn_rotary).  No counterpart in the reference.
 //
-// A pair (u, v) of axis a turns by pos_a w, w = base^(-p / p_a).  In 32 bits
-// pos w alone is off by 2^-24 of itself, a fifth of a turn at a position of
-// 2^23, so the angle is formed in 64 bits, in quarter turns: pos (w 2 / pi),
-// its nearest whole number taken off exactly, and what remains, at most pi / 4,
-// goes into the Taylor sums of sine and cosine up to x^13 and x^14 (the first
-// term left out is below 3e-14 there), rounded once to 32 bits.  Each output
-// then carries the rounding of sine and cosine, of one product and of one
-// fused multiply-add.
+// Each output carries the rounding of sine and cosine (rotary_angle.h), of one
+// product and of one fused multiply-add.
 //
 // The work is one read and one write of the heads: HBM-bound.  A thread owns
 // a group of pairs of one token in up to four heads, so that the 64-bit part
 // (about 45 instructions a pair) serves them together; consecutive lanes take
 // the groups of a head, then the next head, so that a wave reads whole lines.
-#include "rnn_internal.h"
+#include "rotary_angle.h"
 
 #include <algorithm>
 #include <cmath>
 
 namespace {
-
-constexpr int MAX_PAIRS = 256;
 
 constexpr int HPT = 4;  // heads of a thread: hl, hl + HL, ... (HL = ceil(h / HPT))
 
@@ -38,33 +30,6 @@ struct RotArgs {
     // quarter turns per unit of position of every pair
     double w[MAX_PAIRS];
 };
-
-// Sine and cosine of `q` quarter turns.
-__device__ __forceinline__ void rot_sincos(double q, float *s, float *c) {
-    const double k = rint(q);
-    const double x = (q - k) * 1.57079632679489661923;
-    const double z = x * x;
-    double a = 1.0 / 6227020800.0;  // 1 / 13!
-    a = fma(a, z, -1.0 / 39916800.0);
-    a = fma(a, z, 1.0 / 362880.0);
-    a = fma(a, z, -1.0 / 5040.0);
-    a = fma(a, z, 1.0 / 120.0);
-    a = fma(a, z, -1.0 / 6.0);
-    const double sn = fma(a * z, x, x);
-    double b = -1.0 / 87178291200.0;  // 1 / 14!
-    b = fma(b, z, 1.0 / 479001600.0);
-    b = fma(b, z, -1.0 / 3628800.0);
-    b = fma(b, z, 1.0 / 40320.0);
-    b = fma(b, z, -1.0 / 720.0);
-    b = fma(b, z, 1.0 / 24.0);
-    b = fma(b, z, -0.5);
-    const double cs = fma(b, z, 1.0);
-    // the quadrant: k mod 4 (k may be beyond an int)
-    const int m = (int)(k - 4.0 * floor(k * 0.25));
-    const double ss = (m & 1) ? cs : sn, cc = (m & 1) ? sn : cs;
-    *s = (float)((m & 2) ? -ss : ss);
-    *c = (float)((m == 1 || m == 2) ? -cc : cc);
-}
 
 // G pairs a thread (4: 16-byte accesses, R, dh and the strides multiples of 4;
 // 1: any layout), channels past 2R copied G at a time.
@@ -111,15 +76,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotArgs g) {
         float sn[G], cs[G];
 #pragma unroll
         for (int k = 0; k < G; k++) {
-            const int j = j0 + k, ax = j < g.p0 ? 0 : j < g.p0 + g.p1 ? 1 : 2;
-            double p;
-            if (g.pos) {
-                p = g.pos[(long long)r * g.axes + ax];
-            } else {
-                const int tt = r % g.t, q = tt / g.g2;
-                p = ax == 0 ? q / g.g1 : ax == 1 ? q % g.g1 : tt % g.g2;
-            }
-            rot_sincos(p * g.w[j], &sn[k], &cs[k]);
+            rot_sincos(rot_position(g, r, j0 + k) * g.w[j0 + k], &sn[k], &cs[k]);
             sn[k] *= g.sign;
         }
 #pragma unroll
@@ -152,7 +109,9 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotArgs g) {
     }
 }
 
-int rot_check(rnn_ctx *ctx, const rnn_rotary_desc *d, size_t n, size_t t, bool have_pos) {
+}  // namespace
+
+int rnn_rotary_checked(rnn_ctx *ctx, const rnn_rotary_desc *d, size_t n, size_t t, bool have_pos) {
     if (!d) return rnn_fail(ctx, RNN_E_NULL, "rotary: desc is null");
     if (!d->h || !d->dh) return rnn_fail(ctx, RNN_E_INVALID, "rotary: zero heads or channels");
     if (d->axes < 1 || d->axes > 3)
@@ -188,19 +147,17 @@ int rot_check(rnn_ctx *ctx, const rnn_rotary_desc *d, size_t n, size_t t, bool h
     return RNN_OK;
 }
 
-}  // namespace
-
 extern "C" {
 
 int rnn_rotary_check(const rnn_rotary_desc *d, size_t n, size_t t, int have_pos) {
-    return rot_check(nullptr, d, n, t, have_pos != 0);
+    return rnn_rotary_checked(nullptr, d, n, t, have_pos != 0);
 }
 
 int rnn_rotary(rnn_ctx *ctx, const rnn_rotary_desc *d, size_t n, size_t t, const float *x,
                const float *pos, float *y, int inverse) {
     if (!ctx) return RNN_E_NULL;
     std::lock_guard<std::recursive_mutex> lk(ctx->mu);
-    const int rc = rot_check(ctx, d, n, t, pos != nullptr);
+    const int rc = rnn_rotary_checked(ctx, d, n, t, pos != nullptr);
     if (rc) return rc;
     const size_t rows = n * t;
     if (!rows) return RNN_OK;
@@ -226,12 +183,7 @@ int rnn_rotary(rnn_ctx *ctx, const rnn_rotary_desc *d, size_t n, size_t t, const
     g.g1 = (int)d->g1;
     g.g2 = (int)d->g2;
     g.sign = inverse ? -1.0f : 1.0f;
-    const uint32_t np[3] = {d->p0, d->p1, d->p2};
-    int j = 0;
-    for (int a = 0; a < 3; a++)
-        for (uint32_t p = 0; p < np[a]; p++)
-            g.w[j++] = std::pow((double)d->base, -(double)p / (double)np[a]) *
-                       0.63661977236758134308;  // 2 / pi
+    rot_frequencies(d, g.w);
     // 16-byte accesses: whole groups of four pairs and of four copied
     // channels, every head's start aligned
     auto al = [](const float *p, long long stride) {
