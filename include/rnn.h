@@ -332,7 +332,7 @@ typedef struct {
  * (backward = 0) or the backward needs for n sequences of t tokens; host only.
  * The workspace is the caller's, 256-byte aligned, holds nothing between calls
  * and is not shared by calls that may run at the same time.  dk and dv <= 128, row
- * strides <= 2^22, n * t * h and n * h * dk * dv < 2^31 (RNN_E_UNSUPPORTED above),
+ * strides <= 2^22 (y's too), n * t * h and n * h * dk * dv < 2^31 (RNN_E_UNSUPPORTED above),
  * scale finite. */
 int rnn_decay_attn_workspace(const rnn_decay_attn_desc *d, size_t n, size_t t, int backward,
                              size_t *bytes);

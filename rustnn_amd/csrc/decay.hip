@@ -13,7 +13,7 @@
 // The rates' gradient is g dL/dg, g = -exp(rate) = log gamma: with Z = dS/dg,
 // Z_i = gamma (Z_(i-1) + S_(i-1)), dL/dg = scale sum q_i . (Z^T-weighted sum of k),
 // that is, dq's form with each term times i - l, dotted with q; and <Z_last, R^>.
-#include "rnn_internal.h"
+#include "mfma_half.h"
 
 #include <algorithm>
 #include <cmath>
@@ -21,6 +21,7 @@
 namespace {
 
 constexpr int MAX_D = 128;
+constexpr int C = 32;  // tokens of a chunk
 
 struct DecayJob {
     const float *a, *b, *c;
@@ -29,6 +30,8 @@ struct DecayJob {
     float *s1;          // states after the last; null: not wanted
     const float *dot;   // the rates' gradient: what the weighted sums are dotted with
     const float *s1g;   // and the gradient of the last state
+    float *seg;         // [nseg][n][h] states before each segment of the walk
+    const float *segg;  // the rates' gradient: those of the walk the other way
     long long as, bs, cs, ys, ds;  // row strides
     int da, dc;         // channels
     int ga, gb, gc, gy; // query heads that share a head of the operand
@@ -41,8 +44,9 @@ struct DecayArgs {
     DecayJob job[3];
     const float *rate;
     const uint32_t *lens;
-    double *part;  // [n][h] parts of dL/dg
+    double *part;  // [n][nseg][slices][h] parts of dL/dg
     int n, t, h, reverse;
+    int nseg, slen;  // segments of a sequence, and their tokens
 };
 
 // log gamma of a head: at most 0, and finite, so that its multiple by 0 is 0.
@@ -56,98 +60,447 @@ __device__ __forceinline__ float decayed(float s, float gam, float rest) {
     return __builtin_fmaf(s, gam, s * rest);
 }
 
-// Token by token: a block holds a head's state, wave w rows 32 w .. 32 w + 31,
-// a lane columns lane and lane + 64.
-template <bool SLOPE>
+// Token by token, forward: a block holds a head's state, wave w rows 32 w .. 32 w
+// + 31, a lane columns lane and lane + 64.
 __global__ __launch_bounds__(256) void decay_tokens_kernel(DecayArgs g) {
-    __shared__ float red[2][4][MAX_D];
-    __shared__ double dred[4];
-    const DecayJob &q = g.job[blockIdx.y];
-    const bool slope = SLOPE && q.dot;
+    __shared__ float red[4][MAX_D];
+    const DecayJob &q = g.job[0];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int heads = g.h / q.gy;
-    const int b = blockIdx.x / heads, ho = blockIdx.x % heads;
+    const int b = blockIdx.x / g.h, hd = blockIdx.x % g.h;
     const int len = g.lens ? (int)min(g.lens[b], (uint32_t)g.t) : g.t;
-    for (int r = 0; r < q.gy; r++) {
-        const int hd = ho * q.gy + r;
-        const bool back = (hd >= g.h - g.reverse) != (q.rev != 0);
-        // gamma in two floats: one rounded alone would be off by its last bit to
-        // the power of the tokens
-        const double g64 = exp(log_gamma(g.rate[hd]));
-        const float gam = (float)g64, rest = (float)(g64 - (double)gam);
-        const long long st = ((long long)b * g.h + hd) * q.da * q.dc;
-        float s[32][2], z[32][2];
+    const bool back = hd >= g.h - g.reverse;
+    // gamma in two floats: one rounded alone would be off by its last bit to
+    // the power of the tokens
+    const double g64 = exp(log_gamma(g.rate[hd]));
+    const float gam = (float)g64, rest = (float)(g64 - (double)gam);
+    const long long st = ((long long)b * g.h + hd) * q.da * q.dc;
+    float s[32][2];
 #pragma unroll
-        for (int i = 0; i < 32; i++)
+    for (int i = 0; i < 32; i++)
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const int ia = 32 * wave + i, jc = lane + 64 * k;
-                s[i][k] = q.s0 && ia < q.da && jc < q.dc ? q.s0[st + ia * q.si + jc * q.sj] : 0.f;
-                z[i][k] = 0.f;
-            }
-        double dg = 0.0;
-        for (int i = 0; i < g.t; i++) {
-            if (i >= len) {
-                if (!q.acc && r == 0 && wave < 2 && threadIdx.x < q.dc)
-                    q.y[((long long)b * g.t + i) * q.ys + (hd / q.gy) * q.dc + threadIdx.x] = 0.f;
-                continue;
-            }
-            const long long row = (long long)b * g.t + (back ? len - 1 - i : i);
-            const float *a = q.a + row * q.as + (hd / q.ga) * q.da;
-            const float *bb = q.b + row * q.bs + (hd / q.gb) * q.da;
-            const float *c = q.c + row * q.cs + (hd / q.gc) * q.dc;
-            float cv[2], o[2] = {0.f, 0.f}, oz[2] = {0.f, 0.f};
+        for (int k = 0; k < 2; k++) {
+            const int ia = 32 * wave + i, jc = lane + 64 * k;
+            s[i][k] = q.s0 && ia < q.da && jc < q.dc ? q.s0[st + ia * q.dc + jc] : 0.f;
+        }
+    for (int i = 0; i < g.t; i++) {
+        if (i >= len) {
+            if (threadIdx.x < q.dc)
+                q.y[((long long)b * g.t + i) * q.ys + hd * q.dc + threadIdx.x] = 0.f;
+            continue;
+        }
+        const long long row = (long long)b * g.t + (back ? len - 1 - i : i);
+        const float *a = q.a + row * q.as + hd * q.da;
+        const float *bb = q.b + row * q.bs + (hd / q.gb) * q.da;
+        const float *c = q.c + row * q.cs + (hd / q.gc) * q.dc;
+        float cv[2], o[2] = {0.f, 0.f};
 #pragma unroll
-            for (int k = 0; k < 2; k++) cv[k] = lane + 64 * k < q.dc ? c[lane + 64 * k] : 0.f;
+        for (int k = 0; k < 2; k++) cv[k] = lane + 64 * k < q.dc ? c[lane + 64 * k] : 0.f;
 #pragma unroll
-            for (int e = 0; e < 32; e++) {
-                const int ia = 32 * wave + e;
-                const float av = ia < q.da ? a[ia] : 0.f, bv = ia < q.da ? q.sb * bb[ia] : 0.f;
-#pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    if (SLOPE) z[e][k] = decayed(z[e][k] + s[e][k], gam, rest);
-                    const float old = q.rev ? s[e][k] : decayed(s[e][k], gam, rest);
-                    s[e][k] = __builtin_fmaf(bv, cv[k], old);
-                    o[k] = __builtin_fmaf(av, s[e][k], o[k]);
-                    if (SLOPE) oz[k] = __builtin_fmaf(av, z[e][k], oz[k]);
-                    if (q.rev) s[e][k] = decayed(s[e][k], gam, rest);
-                }
-            }
-            __syncthreads();
+        for (int e = 0; e < 32; e++) {
+            const int ia = 32 * wave + e;
+            const float av = ia < q.da ? a[ia] : 0.f, bv = ia < q.da ? bb[ia] : 0.f;
 #pragma unroll
             for (int k = 0; k < 2; k++) {
-                red[0][wave][lane + 64 * k] = o[k];
-                if (SLOPE) red[1][wave][lane + 64 * k] = oz[k];
-            }
-            __syncthreads();
-            const int jc = threadIdx.x;
-            if (jc < q.dc) {
-                float v = 0.f, vz = 0.f;
-                for (int w = 0; w < 4; w++) {
-                    v += red[0][w][jc];
-                    if (SLOPE) vz += red[1][w][jc];
-                }
-                float *y = q.y + row * q.ys + (hd / q.gy) * q.dc + jc;
-                *y = (q.acc || r > 0 ? *y : 0.f) + q.sa * v;
-                if (slope) dg += (double)(q.sa * vz) * q.dot[row * q.ds + hd * q.dc + jc];
+                s[e][k] = __builtin_fmaf(bv, cv[k], decayed(s[e][k], gam, rest));
+                o[k] = __builtin_fmaf(av, s[e][k], o[k]);
             }
         }
+        __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 32; i++)
+        for (int k = 0; k < 2; k++) red[wave][lane + 64 * k] = o[k];
+        __syncthreads();
+        const int jc = threadIdx.x;
+        if (jc < q.dc)
+            q.y[row * q.ys + hd * q.dc + jc] = q.sa * (red[0][jc] + red[1][jc] + red[2][jc] + red[3][jc]);
+    }
+    if (!q.s1) return;
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const int ia = 32 * wave + i, jc = lane + 64 * k;
-                if (ia >= q.da || jc >= q.dc) continue;
-                if (q.s1) q.s1[st + ia * q.si + jc * q.sj] = s[i][k];
-                if (slope && q.s1g) dg += (double)z[i][k] * q.s1g[st + ia * q.si + jc * q.sj];
+    for (int i = 0; i < 32; i++)
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const int ia = 32 * wave + i, jc = lane + 64 * k;
+            if (ia < q.da && jc < q.dc) q.s1[st + ia * q.dc + jc] = s[i][k];
+        }
+}
+
+__device__ __forceinline__ f32x16 mm32(float a, float b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
+}
+
+// Register r of a 32 x 32 accumulator holds row tile_row(r) + 4 (lane / 32) of
+// column lane % 32.  Taken as an operand of a product, register r stands for the
+// k's tile_row(r) and tile_row(r) + 4: accumulators are operands as they are.
+__device__ __forceinline__ constexpr int tile_row(int r) { return (r & 3) + 8 * (r >> 2); }
+
+// Rows of a head in the order of a walk: the p-th token from `first` on.
+struct Walk {
+    long long first;
+    int dir;  // +1, -1
+};
+
+// Past the end of every resource here (32 rows of at most 2^24 bytes), whatever
+// rows and channels are added to it or taken from it.
+constexpr uint32_t NOWHERE = 0x50000000u;
+
+// Keeps what depends on v in the loop: hoisted out of it, the comparisons of a
+// chunk's places and channels fill the scalar registers.
+__device__ __forceinline__ int opaque(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
+// A chunk's rows of an operand or a result: L of them, the resource beginning at
+// the lowest; what lies outside reads as 0 and is not written.
+struct ChunkRows {
+    __amdgpu_buffer_rsrc_t rs;
+    uint32_t stride;  // bytes
+    int lim, step, L;
+    __device__ __forceinline__ ChunkRows(const float *p, long long st, int width, const Walk &w, int c0,
+                                         int n)
+        : stride((uint32_t)st * 4u), lim(width), step(w.dir), L(n) {
+        const long long low = w.dir < 0 ? w.first - c0 - (n - 1) : w.first + c0;
+        rs = rows_rsrc(p + low * st, n, st, width);
+    }
+    // Byte offset of channel ch at place p.  Places past the end come out beyond
+    // the resource either way, rows below it as offsets near 2^32.
+    __device__ __forceinline__ uint32_t at(int p, int ch) const {
+        const uint32_t c = ch < lim ? 4u * (uint32_t)ch : NOWHERE;
+        return c + (uint32_t)(step < 0 ? L - 1 - p : p) * stride;
+    }
+    // From the offset of place p, that of place p + k.
+    __device__ __forceinline__ uint32_t go(uint32_t at, int k) const {
+        return at + (uint32_t)(step * k) * stride;
+    }
+    __device__ __forceinline__ float load(uint32_t at) const {
+        return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, at, 0, 0));
+    }
+    __device__ __forceinline__ void store(uint32_t at, float v) const {
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), rs, at, 0, 0);
+    }
+};
+
+// An operand's k's along the channels: register 4 k + e of lane l is channel 8 k +
+// 4 (l / 32) + e of the row at place l % 32, as accumulators order their rows.
+// FULL: all 32 DAT channels are there.
+template <int DAT, bool FULL>
+__device__ __forceinline__ void load_rows(const ChunkRows &x, int ln, int half, f32x4 (&v)[4 * DAT]) {
+    const uint32_t at = ln < x.L ? x.at(ln, 0) + 4u * (uint32_t)half : NOWHERE;
+    const int t = opaque(half - x.lim);
+#pragma unroll
+    for (int k = 0; k < 4 * DAT; k++) {
+        u32x4 w = __builtin_amdgcn_raw_buffer_load_b128(x.rs, at + 32 * k, 0, 0);
+        if (!FULL) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] &= (uint32_t)((t + 8 * k + e) >> 31);
+        }
+        v[k] = __builtin_bit_cast(f32x4, w);
+    }
+}
+
+// A state in memory, as the walk's accumulators hold it: register r of tile d is
+// row 32 d + tile_row(r) + half of column col.
+struct StateRows {
+    __amdgpu_buffer_rsrc_t rs;
+    uint32_t si, base;  // bytes
+    int rows;           // rows from `half` on
+    __device__ __forceinline__ StateRows(const float *p, const DecayJob &q, int half, int col)
+        : rs(make_rsrc(p, (uint32_t)(q.da * q.dc) * 4u)), si((uint32_t)q.si * 4u),
+          base(col < q.dc ? (uint32_t)(col * q.sj + half * q.si) * 4u : NOWHERE), rows(q.da - half) {}
+    __device__ __forceinline__ uint32_t at(int d, int r) const {
+        const int i = 32 * d + tile_row(r);
+        return i < opaque(rows) ? base + (uint32_t)i * si : NOWHERE;
+    }
+    __device__ __forceinline__ float load(int d, int r) const {
+        return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, at(d, r), 0, 0));
+    }
+    __device__ __forceinline__ void store(int d, int r, float v) const {
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), rs, at(d, r), 0, 0);
+    }
+};
+
+// A head's powers of gamma in LDS, of a wave's own.
+struct Powers {
+    float near[C];      // gamma^m
+    float first[C];     // gamma^(p + e) sa
+    float left[C];      // gamma^(L - p - e) sb, of a chunk of L places
+};
+
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Sixteen places' entries of a table, as an accumulator's rows.
+__device__ __forceinline__ void places(const float *tab, int half, float (&v)[16]) {
+    const float *t = tab + opaque(half);
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        const f32x4 w = *(const f32x4 *)(t + 8 * q);
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[4 * q + e] = w[e];
+    }
+}
+
+// o + p c over a chunk, where p (register r: the keys of operand register r) is 0
+// for keys behind the query: a value of c that is no number makes its column's
+// rows from its own on NaN, and none before.
+__device__ __forceinline__ f32x16 tri_product(const f32x16 &p, const float (&c)[16], f32x16 o, int half) {
+    float m = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; r++) m = __builtin_fmaf(c[r], 0.f, m);
+    if (!__any(m != m)) {
+#pragma unroll
+        for (int r = 0; r < 16; r++) o = mm32(p[r], c[r], o);
+        return o;
+    }
+    int bad = C;
+#pragma unroll
+    for (int r = 0; r < 16; r++) {  // the same sums in the same order
+        const bool ok = c[r] * 0.f == 0.f;
+        if (!ok) bad = min(bad, tile_row(r) + half);
+        o = mm32(p[r], ok ? c[r] : 0.f, o);
+    }
+    bad = min(bad, __shfl_xor(bad, 32, 64));
+#pragma unroll
+    for (int r = 0; r < 16; r++)
+        if (tile_row(r) + half >= bad) o[r] = __builtin_nanf("");
+    return o;
+}
+
+enum { WALK = 0, WALK_RATE = 1, STATE = 2 };
+
+// A wave takes 32 of c's channels of a head through a segment, 32 tokens at a
+// time, its part of the state (DAT tiles of 32 x 32) in accumulators:
+//   P^T = b a^T, weighted by gamma^(i-l) and cut; y = gamma^(i + e) a T + P c;
+//   T = gamma^32 T + (gamma^(32 - l - e) b)^T c        (e: 1, rev: 0)
+// Rows come straight from global memory in the operands' layouts; a wave shares
+// nothing with another one and waits for none.  STATE: the segment's own T alone.
+template <int DAT, bool FULL, int MODE>
+__global__ __launch_bounds__(256, DAT <= 2 ? 2 : 1) void decay_walk_kernel(DecayArgs g) {
+    __shared__ __attribute__((aligned(16))) Powers tables[4];
+    const DecayJob &q = g.job[blockIdx.y];
+    const int lane = threadIdx.x & 63, ln = lane & 31, half = 4 * (lane >> 5), wave = wave_index();
+    const int nsl = (q.dc + 31) / 32, heads = g.h / q.gy;
+    long long u = xcd_order(blockIdx.x, gridDim.x) * 4 + wave;
+    const int slice = (int)(u % nsl), col = slice * 32 + ln;
+    u /= nsl;
+    const int seg = (int)(u % g.nseg);
+    u /= g.nseg;
+    const int ho = (int)(u % heads);
+    const long long b = u / heads;
+    if (b >= g.n) return;
+    const int len = __builtin_amdgcn_readfirstlane(g.lens ? (int)min(g.lens[b], (uint32_t)g.t) : g.t);
+    const int t0 = seg * g.slen, t1 = min(t0 + g.slen, len), T = max(t1 - t0, 0);
+    const bool lastseg = len > 0 ? t0 < len && t1 == len : seg == 0;
+    const bool slope = MODE == WALK_RATE && q.dot;
+    const int e0 = q.rev ? 0 : 1;
+    const bool incol = col < q.dc;
+    if (MODE != STATE && !q.acc) {  // padding rows
+        const int z1 = (int)min((long long)t0 + g.slen, (long long)g.t);
+        for (int i = max(t0, len) + (lane >> 5); i < z1; i += 2)
+            if (incol) q.y[(b * g.t + i) * q.ys + ho * q.dc + col] = 0.f;
+    }
+    Powers &pw = tables[wave];
+    for (int r0 = 0; r0 < q.gy; r0++) {
+        const int hd = ho * q.gy + r0;
+        double dg = 0.0;
+        const long long st = (b * g.h + hd) * q.da * q.dc;
+        const long long sg = ((long long)seg * g.n * g.h) * q.da * q.dc + st;
+        const double lg = log_gamma(g.rate[hd]);
+        // segments are rows' whatever the walk's direction, so that the heads that
+        // share a row of y meet in one wave
+        const bool down = (hd >= g.h - g.reverse) != (q.rev != 0);
+        const Walk w = {b * g.t + (down ? t1 - 1 : t0), down ? -1 : 1};
+        const bool ends = down ? seg == 0 : lastseg;    // holds the walk's last token
+        const bool begins = down ? lastseg : seg == 0;  // holds its first
+        if (MODE == STATE && (T == 0 || ends)) return;
+        wave_sync();
+        if (lane < C) {
+            pw.near[lane] = (float)exp(lg * lane);
+            pw.first[lane] = (float)exp(lg * (lane + e0)) * q.sa;
+        }
+        // the state: rows 32 d + tile_row(r) + half, column col
+        const float *s0 = MODE == STATE ? nullptr : g.nseg > 1 ? q.seg + sg : begins && q.s0 ? q.s0 + st : nullptr;
+        f32x16 S[DAT], Z[MODE == WALK_RATE ? DAT : 1];
+#pragma unroll
+        for (int d = 0; d < DAT; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                S[d][r] = 0.f;
+                if (MODE == WALK_RATE) Z[d][r] = 0.f;
             }
+        if (s0) {
+            const StateRows x(s0, q, half, col);
+#pragma unroll
+            for (int d = 0; d < DAT; d++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) S[d][r] = x.load(d, r);
+        }
+        bool any = s0 != nullptr;  // whether the state may be other than 0
+        const float *pa = q.a + (hd / q.ga) * q.da, *pb = q.b + (hd / q.gb) * q.da,
+                    *pc = q.c + (hd / q.gc) * q.dc;
+        float hi = 0.f, lo = 0.f;  // gamma^L, in two parts
+        for (int c0 = 0; c0 < T; c0 += C) {
+            const int L = min(C, T - c0);
+            if (c0 == 0 || L < C) {
+                const double all = exp(lg * L);
+                hi = (float)all;
+                lo = (float)(all - (double)hi);
+                wave_sync();
+                if (lane < C) pw.left[lane] = (float)exp(lg * max(L - lane - e0, 0)) * q.sb;
+                wave_sync();
+            }
+            const ChunkRows rb(pb, q.bs, q.da, w, c0, L), rc(pc, q.cs, q.dc, w, c0, L);
+            float cf[16];
+            const uint32_t c_at = rc.at(half, col);
+#pragma unroll
+            for (int r = 0; r < 16; r++) cf[r] = rc.load(rc.go(c_at, tile_row(r)));
+            if constexpr (MODE != STATE) {
+                const ChunkRows ra(pa, q.as, q.da, w, c0, L);
+                f32x4 af[4 * DAT];
+                f32x16 P, o, oz;
+#pragma unroll
+                for (int r = 0; r < 16; r++) P[r] = o[r] = oz[r] = 0.f;
+                load_rows<DAT, FULL>(ra, ln, half, af);
+                {
+                    f32x4 bf[4 * DAT];
+                    load_rows<DAT, FULL>(rb, ln, half, bf);
+#pragma unroll
+                    for (int k = 0; k < 4 * DAT; k++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) P = mm32(bf[k][e], af[k][e], P);
+                }
+                const int query = opaque(ln - half);
+                const float sab = q.sa * q.sb;
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int far = query - tile_row(r);
+                    P[r] = far >= 0 ? P[r] * (pw.near[max(far, 0)] * sab) : 0.f;
+                }
+                if (any) {
+                    float row[16];
+                    places(pw.first, half, row);
+#pragma unroll
+                    for (int d = 0; d < DAT; d++)
+#pragma unroll
+                        for (int r = 0; r < 16; r++) o = mm32(af[4 * d + (r >> 2)][r & 3], S[d][r], o);
+                    if (slope) {
+#pragma unroll
+                        for (int d = 0; d < DAT; d++)
+#pragma unroll
+                            for (int r = 0; r < 16; r++) oz = mm32(af[4 * d + (r >> 2)][r & 3], Z[d][r], oz);
+                        const float one = (float)(half + 1);
+#pragma unroll
+                        for (int r = 0; r < 16; r++)
+                            oz[r] = row[r] * __builtin_fmaf(one + (float)tile_row(r), o[r], oz[r]);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 16; r++) o[r] *= row[r];
+                }
+                o = tri_product(P, cf, o, half);
+                if (slope) {
+                    const float fq = (float)query;
+#pragma unroll
+                    for (int r = 0; r < 16; r++) P[r] *= fq - (float)tile_row(r);
+                    oz = tri_product(P, cf, oz, half);
+                    const ChunkRows rd(q.dot + hd * q.dc, q.ds, q.dc, w, c0, L);
+                    const uint32_t d_at = rd.at(half, col);
+                    float sum = 0.f;
+#pragma unroll
+                    for (int r = 0; r < 16; r++)
+                        sum = __builtin_fmaf(oz[r], rd.load(rd.go(d_at, tile_row(r))), sum);
+                    dg += (double)sum;
+                }
+                const ChunkRows ry(q.y + ho * q.dc, q.ys, q.dc, w, c0, L);
+                const uint32_t y_at = ry.at(half, col);
+                if (q.acc || r0 > 0) {
+#pragma unroll
+                    for (int r = 0; r < 16; r++) o[r] += ry.load(ry.go(y_at, tile_row(r)));
+                }
+#pragma unroll
+                for (int r = 0; r < 16; r++) ry.store(ry.go(y_at, tile_row(r)), o[r]);
+            }
+            // the state behind the chunk, where a reader follows
+            if (MODE != STATE && c0 + L == T && !slope && !(ends && q.s1)) break;
+            float left[16];
+            places(pw.left, half, left);
+#pragma unroll
+            for (int r = 0; r < 16; r++) cf[r] *= left[r];
+#pragma unroll
+            for (int d = 0; d < DAT; d++) {
+                float bt[16];
+                const uint32_t b_at = rb.at(half, 32 * d + ln);
+#pragma unroll
+                for (int r = 0; r < 16; r++) bt[r] = rb.load(rb.go(b_at, tile_row(r)));
+                if (slope) {
+                    const float fl = (float)(L - 1 - half);
+#pragma unroll
+                    for (int r = 0; r < 16; r++)
+                        Z[d][r] = decayed(__builtin_fmaf((float)L, S[d][r], Z[d][r]), hi, lo);
+#pragma unroll
+                    for (int r = 0; r < 16; r++)
+                        Z[d] = mm32(bt[r], cf[r] * (fl - (float)tile_row(r)), Z[d]);
+                }
+#pragma unroll
+                for (int r = 0; r < 16; r++) S[d][r] = decayed(S[d][r], hi, lo);
+#pragma unroll
+                for (int r = 0; r < 16; r++) S[d] = mm32(bt[r], cf[r], S[d]);
+            }
+            any = true;
+        }
+        const float *sgrad = !slope || !T ? nullptr : g.nseg > 1 ? q.segg + sg : q.s1g ? q.s1g + st : nullptr;
+        float *s1 = MODE == STATE ? q.seg + sg : ends && q.s1 ? q.s1 + st : nullptr;
+        if (s1) {
+            const StateRows x(s1, q, half, col);
+#pragma unroll
+            for (int d = 0; d < DAT; d++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) x.store(d, r, S[d][r]);
+        }
+        if (MODE == WALK_RATE && sgrad) {
+            const StateRows x(sgrad, q, half, col);
+#pragma unroll
+            for (int d = 0; d < DAT; d++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) dg += (double)Z[d][r] * x.load(d, r);
+        }
         if (slope) {
             dg = rnn_wave_sum_d(dg);
-            __syncthreads();
-            if (lane == 0) dred[wave] = dg;
-            __syncthreads();
-            if (threadIdx.x == 0)
-                g.part[(long long)b * g.h + hd] = dred[0] + dred[1] + dred[2] + dred[3];
+            if (lane == 0) g.part[((b * g.nseg + seg) * nsl + slice) * g.h + hd] = dg;
+        }
+    }
+}
+
+// The states before each segment, in the walk's direction, from the segments' own
+// ones: one thread an element, over the segments in order.
+__global__ __launch_bounds__(256) void decay_scan_kernel(DecayArgs g) {
+    const DecayJob &q = g.job[blockIdx.y];
+    const long long per = (long long)q.da * q.dc, all = (long long)g.n * g.h * per;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= all) return;
+    const int hd = (int)(i / per % g.h);
+    const long long b = i / per / g.h;
+    const int len = g.lens ? (int)min(g.lens[b], (uint32_t)g.t) : g.t;
+    const int last = len > 0 ? (len - 1) / g.slen : 0;
+    const double lg = log_gamma(g.rate[hd]);
+    double all64 = exp(lg * g.slen);
+    const float hi = (float)all64, lo = (float)(all64 - (double)hi);
+    float s = q.s0 ? q.s0[i] : 0.f;
+    if ((hd >= g.h - g.reverse) == (q.rev != 0)) {
+        for (int k = 0; k <= last; k++) {
+            const float own = k < last ? q.seg[k * all + i] : 0.f;
+            q.seg[k * all + i] = s;
+            s = decayed(s, hi, lo) + own;
+        }
+    } else {
+        all64 = exp(lg * (len - last * g.slen));
+        float a = (float)all64, z = (float)(all64 - (double)a);
+        for (int k = last; k >= 0; k--) {
+            const float own = k > 0 ? q.seg[k * all + i] : 0.f;
+            q.seg[k * all + i] = s;
+            s = decayed(s, a, z) + own;
+            a = hi, z = lo;
         }
     }
 }
@@ -166,15 +519,33 @@ __global__ __launch_bounds__(256) void decay_rate_kernel(const double *part, int
         drate[j] += (float)(log_gamma(rate[j]) * (red[0] + red[1] + red[2] + red[3]));
 }
 
-struct DecayWs {
-    size_t part = 0, bytes = 0;
+// The form's walks over a sequence, and where a workspace's parts are.
+struct DecayPlan {
+    bool tokens = false;  // token by token
+    int nseg = 1, slen = 1;
+    size_t seg = 0, segr = 0, part = 0, bytes = 0;
 };
-DecayWs plan_ws(const rnn_decay_attn_desc *d, size_t n, size_t t, bool backward) {
-    DecayWs w;
+DecayPlan plan_of(const rnn_decay_attn_desc *d, size_t n, size_t t, bool backward) {
+    DecayPlan p;
     WsCarve c;
-    if (backward) w.part = c.take(n * d->h * sizeof(double));
-    w.bytes = c.off;
-    return w;
+    // few tokens: the state's read and write are all there is to do
+    p.tokens = !backward && t <= 8;
+    const size_t nsl = rnn_div_up(backward ? std::max(d->dk, d->dv) : d->dv, 32);
+    const size_t waves = n * d->h * nsl * (backward ? 3 : 1);
+    p.slen = (int)rnn_round_up(std::max<size_t>(t, 1), C);
+    if (!p.tokens && waves && waves < 1024 && t > 256) {
+        const size_t want = std::min(rnn_div_up(2048, waves), t / 128);
+        p.slen = (int)rnn_round_up(rnn_div_up(t, want), C);
+        p.nseg = (int)rnn_div_up(t, p.slen);
+    }
+    const size_t states = (size_t)p.nseg * n * d->h * d->dk * d->dv * sizeof(float);
+    if (p.nseg > 1) {
+        p.seg = c.take(states);
+        if (backward) p.segr = c.take(states);
+    }
+    if (backward) p.part = c.take(n * p.nseg * rnn_div_up(d->dk, 32) * d->h * sizeof(double));
+    p.bytes = c.off;
+    return p;
 }
 
 int decay_check(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n, size_t t) {
@@ -192,7 +563,7 @@ int decay_check(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n, size_t t) 
                         d->dk, d->dv, MAX_D);
     const uint64_t qw = (uint64_t)d->h * d->dk, kw = (uint64_t)d->hkv * d->dk,
                    vw = (uint64_t)d->hkv * d->dv;
-    if (d->qstride > (1u << 22) || d->kvstride > (1u << 22))
+    if (d->qstride > (1u << 22) || d->kvstride > (1u << 22) || (uint64_t)d->h * d->dv > (1u << 22))
         return rnn_fail(ctx, RNN_E_UNSUPPORTED, "decay_attn: row stride above 2^22");
     if (d->qoff > d->qstride || d->qstride - d->qoff < qw || d->koff > d->kvstride ||
         d->kvstride - d->koff < kw || d->voff > d->kvstride || d->kvstride - d->voff < vw)
@@ -205,7 +576,7 @@ int decay_check(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n, size_t t) 
     return RNN_OK;
 }
 
-int check_ws(rnn_ctx *ctx, const DecayWs &w, const void *ws, size_t bytes) {
+int check_ws(rnn_ctx *ctx, const DecayPlan &w, const void *ws, size_t bytes) {
     if (!w.bytes) return RNN_OK;
     if (!ws) return rnn_fail(ctx, RNN_E_NULL, "decay_attn: workspace is null");
     if (bytes < w.bytes)
@@ -236,8 +607,10 @@ DecayJob make_job(const Operand &a, const Operand &b, int da, const Operand &c, 
     return j;
 }
 
-void fill_args(DecayArgs &g, const rnn_decay_attn_desc *d, size_t n, size_t t, const float *rate,
-               const uint32_t *lens) {
+void fill_args(DecayArgs &g, const rnn_decay_attn_desc *d, const DecayPlan &p, size_t n, size_t t,
+               const float *rate, const uint32_t *lens) {
+    g.nseg = p.nseg;
+    g.slen = p.slen;
     g.rate = rate;
     g.lens = lens;
     g.part = nullptr;
@@ -245,6 +618,37 @@ void fill_args(DecayArgs &g, const rnn_decay_attn_desc *d, size_t n, size_t t, c
     g.t = (int)t;
     g.h = (int)d->h;
     g.reverse = (int)d->reverse;
+}
+
+template <int MODE>
+void launch_walk(rnn_ctx *ctx, const DecayArgs &g, int jobs) {
+    size_t waves = 0;
+    bool full = true;
+    for (int k = 0; k < jobs; k++) {
+        const DecayJob &q = g.job[k];
+        const int nsl = (q.dc + 31) / 32;
+        waves = std::max(waves, (size_t)g.n * (g.h / q.gy) * g.nseg * nsl);
+        full = full && q.da % 32 == 0;
+    }
+    const dim3 grid((unsigned)rnn_div_up(waves, 4), (unsigned)jobs);
+    hipStream_t s = ctx->stream;
+#define WALK_AS(DAT)                                                                \
+    (full ? decay_walk_kernel<DAT, true, MODE><<<grid, 256, 0, s>>>(g)              \
+          : decay_walk_kernel<DAT, false, MODE><<<grid, 256, 0, s>>>(g))
+    switch ((g.job[0].da + 31) / 32) {
+        case 1: WALK_AS(1); break;
+        case 2: WALK_AS(2); break;
+        case 3: WALK_AS(3); break;
+        default: WALK_AS(4); break;
+    }
+#undef WALK_AS
+}
+
+// The states between segments: every segment's own, then over the segments.
+void launch_segments(rnn_ctx *ctx, const DecayArgs &g, int jobs) {
+    launch_walk<STATE>(ctx, g, jobs);
+    const size_t all = (size_t)g.n * g.h * g.job[0].da * g.job[0].dc;
+    decay_scan_kernel<<<dim3((unsigned)rnn_div_up(all, 256), jobs), 256, 0, ctx->stream>>>(g);
 }
 
 }  // namespace
@@ -256,7 +660,7 @@ int rnn_decay_attn_workspace(const rnn_decay_attn_desc *d, size_t n, size_t t, i
     const int rc = decay_check(nullptr, d, n, t);
     if (rc) return rc;
     if (!bytes) return RNN_E_NULL;
-    *bytes = plan_ws(d, n, t, backward != 0).bytes;
+    *bytes = plan_of(d, n, t, backward != 0).bytes;
     return RNN_OK;
 }
 
@@ -270,12 +674,12 @@ int rnn_decay_attn_forward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n,
     if (rc) return rc;
     if (!n || (!t && !state_out)) return RNN_OK;
     if ((t && (!q || !kv || !y)) || !rate) return rnn_fail(ctx, RNN_E_NULL, "decay_attn_forward: null operand");
-    const DecayWs w = plan_ws(d, n, t, false);
+    const DecayPlan w = plan_of(d, n, t, false);
     rc = check_ws(ctx, w, ws, ws_bytes);
     if (rc) return rc;
     RNN_ON_DEVICE(ctx);
     DecayArgs g;
-    fill_args(g, d, n, t, rate, lens);
+    fill_args(g, d, w, n, t, rate, lens);
     const int grp = (int)(d->h / d->hkv);
     const Operand Q = {q + d->qoff, d->qstride, 1}, K = {kv + d->koff, d->kvstride, grp},
                   V = {kv + d->voff, d->kvstride, grp};
@@ -284,7 +688,17 @@ int rnn_decay_attn_forward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n,
     j.s0 = state_in;
     j.s1 = state_out;
     j.sa = d->scale;
-    decay_tokens_kernel<false><<<dim3((unsigned)(n * d->h), 1), 256, 0, ctx->stream>>>(g);
+    if (w.tokens) {
+        decay_tokens_kernel<<<(unsigned)(n * d->h), 256, 0, ctx->stream>>>(g);
+        RNN_LAUNCHED(ctx);
+        return RNN_OK;
+    }
+    if (w.nseg > 1) {
+        j.seg = (float *)((char *)ws + w.seg);
+        launch_segments(ctx, g, 1);
+        RNN_LAUNCHED(ctx);
+    }
+    launch_walk<WALK>(ctx, g, 1);
     RNN_LAUNCHED(ctx);
     return RNN_OK;
 }
@@ -305,12 +719,12 @@ int rnn_decay_attn_backward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n
         return rnn_fail(ctx, RNN_E_NULL, "decay_attn_backward: null operand");
     if (dstate_in && (dstate_in == dstate_out || dstate_in == state_in))
         return rnn_fail(ctx, RNN_E_INVALID, "decay_attn_backward: dstate_in is an operand");
-    const DecayWs w = plan_ws(d, n, t, true);
+    const DecayPlan w = plan_of(d, n, t, true);
     rc = check_ws(ctx, w, ws, ws_bytes);
     if (rc) return rc;
     RNN_ON_DEVICE(ctx);
     DecayArgs g;
-    fill_args(g, d, n, t, rate, lens);
+    fill_args(g, d, w, n, t, rate, lens);
     const int grp = (int)(d->h / d->hkv), dk = (int)d->dk, dv = (int)d->dv;
     const Operand Q = {q + d->qoff, d->qstride, 1}, K = {kv + d->koff, d->kvstride, grp},
                   V = {kv + d->voff, d->kvstride, grp}, O = {dy, (size_t)d->h * d->dv, 1};
@@ -334,19 +748,37 @@ int rnn_decay_attn_backward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n
     jk.rev = jv.rev = 1;
     jk.acc = jv.acc = !(flags & RNN_ATTN_SET_DKV);
     jv.s1 = dstate_in;
-    // one launch a job: of shared heads, dk and dv have fewer blocks
-    for (int k = 0; k < 3; k++) {
+    if (w.nseg > 1) {
+        // S from the keys and values, R from the queries and dy
+        DecayArgs sg = g;
+        sg.job[0] = make_job(Q, K, dk, V, dv, nullptr, 0, 1);
+        sg.job[0].s0 = state_in;
+        sg.job[0].seg = (float *)((char *)ws + w.seg);
+        sg.job[1] = jv;
+        sg.job[1].gy = 1;
+        sg.job[1].seg = (float *)((char *)ws + w.segr);
+        launch_segments(ctx, sg, 2);
+        RNN_LAUNCHED(ctx);
+        jq.seg = sg.job[0].seg;
+        jk.seg = jv.seg = sg.job[1].seg;
+        jq.segg = sg.job[1].seg;
+    }
+    // one launch where the three jobs' states have as many tiles, else dv's apart
+    const bool joint = (dk + 31) / 32 == (dv + 31) / 32;
+    if (drate)
+        launch_walk<WALK_RATE>(ctx, g, joint ? 3 : 2);
+    else
+        launch_walk<WALK>(ctx, g, joint ? 3 : 2);
+    RNN_LAUNCHED(ctx);
+    if (!joint) {
         DecayArgs one = g;
-        one.job[0] = g.job[k];
-        const unsigned blocks = (unsigned)(n * (k ? d->hkv : d->h));
-        if (k == 0 && drate)
-            decay_tokens_kernel<true><<<dim3(blocks, 1), 256, 0, ctx->stream>>>(one);
-        else
-            decay_tokens_kernel<false><<<dim3(blocks, 1), 256, 0, ctx->stream>>>(one);
+        one.job[0] = jv;
+        launch_walk<WALK>(ctx, one, 1);
         RNN_LAUNCHED(ctx);
     }
     if (drate) {
-        decay_rate_kernel<<<(unsigned)d->h, 256, 0, ctx->stream>>>(g.part, (int)n, (int)d->h, rate, drate);
+        decay_rate_kernel<<<(unsigned)d->h, 256, 0, ctx->stream>>>(
+            g.part, (int)(n * w.nseg * rnn_div_up(d->dk, 32)), (int)d->h, rate, drate);
         RNN_LAUNCHED(ctx);
     }
     return RNN_OK;
