@@ -181,20 +181,31 @@ struct ChunkRows {
 
 // An operand's k's along the channels: register 4 k + e of lane l is channel 8 k +
 // 4 (l / 32) + e of the row at place l % 32, as accumulators order their rows.
-// FULL: all 32 DAT channels are there.
-template <int DAT, bool FULL>
+template <int DAT>
 __device__ __forceinline__ void load_rows(const ChunkRows &x, int ln, int half, f32x4 (&v)[4 * DAT]) {
     const uint32_t at = ln < x.L ? x.at(ln, 0) + 4u * (uint32_t)half : NOWHERE;
-    const int t = opaque(half - x.lim);
+#pragma unroll
+    for (int k = 0; k < 4 * DAT; k++)
+        v[k] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(x.rs, at + 32 * k, 0, 0));
+}
+// Channels from `lim` on, which are another head's, as 0 (FULL: there are none).
+template <int DAT, bool FULL>
+__device__ __forceinline__ void cut_rows(int lim, int half, f32x4 (&v)[4 * DAT]) {
+    if (FULL) return;
+    const int t = opaque(half - lim);
 #pragma unroll
     for (int k = 0; k < 4 * DAT; k++) {
-        u32x4 w = __builtin_amdgcn_raw_buffer_load_b128(x.rs, at + 32 * k, 0, 0);
-        if (!FULL) {
+        u32x4 w = __builtin_bit_cast(u32x4, v[k]);
 #pragma unroll
-            for (int e = 0; e < 4; e++) w[e] &= (uint32_t)((t + 8 * k + e) >> 31);
-        }
+        for (int e = 0; e < 4; e++) w[e] &= (uint32_t)((t + 8 * k + e) >> 31);
         v[k] = __builtin_bit_cast(f32x4, w);
     }
+}
+// Sixteen places of channel ch: k's along the tokens.
+__device__ __forceinline__ void load_cols(const ChunkRows &x, int half, int ch, float (&v)[16]) {
+    const uint32_t at = x.at(half, ch);
+#pragma unroll
+    for (int r = 0; r < 16; r++) v[r] = x.load(x.go(at, tile_row(r)));
 }
 
 // A state in memory, as the walk's accumulators hold it: register r of tile d is
@@ -274,26 +285,32 @@ enum { WALK = 0, WALK_RATE = 1, STATE = 2 };
 // time, its part of the state (DAT tiles of 32 x 32) in accumulators:
 //   P^T = b a^T, weighted by gamma^(i-l) and cut; y = gamma^(i + e) a T + P c;
 //   T = gamma^32 T + (gamma^(32 - l - e) b)^T c        (e: 1, rev: 0)
-// Rows come straight from global memory in the operands' layouts; a wave shares
-// nothing with another one and waits for none.  STATE: the segment's own T alone.
+// Rows come straight from global memory in the operands' layouts, the next
+// chunk's into the registers that this one's products have freed; b's channels by
+// tokens through the wave's own LDS.  A wave shares nothing with another one and
+// waits for none.  WALK_RATE: the rates' gradient as well.  STATE: the segment's
+// own T alone.
 template <int DAT, bool FULL, int MODE>
-__global__ __launch_bounds__(256, DAT <= 2 ? 2 : 1) void decay_walk_kernel(DecayArgs g) {
+__global__ __launch_bounds__(256, DAT <= (MODE == WALK_RATE ? 1 : 2) ? 2 : 1) void decay_walk_kernel(DecayArgs g) {
+    // rows of b: 4 rows apart are half of the banks apart
+    constexpr int BS = 32 * DAT + 8;
     __shared__ __attribute__((aligned(16))) Powers tables[4];
+    __shared__ __attribute__((aligned(16))) float btile[MODE == STATE ? 1 : 4][MODE == STATE ? 4 : C * BS];
     const DecayJob &q = g.job[blockIdx.y];
     const int lane = threadIdx.x & 63, ln = lane & 31, half = 4 * (lane >> 5), wave = wave_index();
     const int nsl = (q.dc + 31) / 32, heads = g.h / q.gy;
-    long long u = xcd_order(blockIdx.x, gridDim.x) * 4 + wave;
-    const int slice = (int)(u % nsl), col = slice * 32 + ln;
-    u /= nsl;
-    const int seg = (int)(u % g.nseg);
-    u /= g.nseg;
-    const int ho = (int)(u % heads);
-    const long long b = u / heads;
+    uint32_t u = (uint32_t)xcd_order(blockIdx.x, gridDim.x) * 4 + wave;  // fewer than 2^31 waves
+    const int slice = (int)(u % (uint32_t)nsl), col = slice * 32 + ln;
+    u /= (uint32_t)nsl;
+    const int seg = (int)(u % (uint32_t)g.nseg);
+    u /= (uint32_t)g.nseg;
+    const int ho = (int)(u % (uint32_t)heads);
+    const long long b = u / (uint32_t)heads;
     if (b >= g.n) return;
     const int len = __builtin_amdgcn_readfirstlane(g.lens ? (int)min(g.lens[b], (uint32_t)g.t) : g.t);
     const int t0 = seg * g.slen, t1 = min(t0 + g.slen, len), T = max(t1 - t0, 0);
     const bool lastseg = len > 0 ? t0 < len && t1 == len : seg == 0;
-    const bool slope = MODE == WALK_RATE && q.dot;
+    constexpr bool slope = MODE == WALK_RATE;
     const int e0 = q.rev ? 0 : 1;
     const bool incol = col < q.dc;
     if (MODE != STATE && !q.acc) {  // padding rows
@@ -302,12 +319,12 @@ __global__ __launch_bounds__(256, DAT <= 2 ? 2 : 1) void decay_walk_kernel(Decay
             if (incol) q.y[(b * g.t + i) * q.ys + ho * q.dc + col] = 0.f;
     }
     Powers &pw = tables[wave];
+    float *bt = btile[MODE == STATE ? 0 : wave];
     for (int r0 = 0; r0 < q.gy; r0++) {
         const int hd = ho * q.gy + r0;
         double dg = 0.0;
         const long long st = (b * g.h + hd) * q.da * q.dc;
         const long long sg = ((long long)seg * g.n * g.h) * q.da * q.dc + st;
-        const double lg = log_gamma(g.rate[hd]);
         // segments are rows' whatever the walk's direction, so that the heads that
         // share a row of y meet in one wave
         const bool down = (hd >= g.h - g.reverse) != (q.rev != 0);
@@ -315,10 +332,21 @@ __global__ __launch_bounds__(256, DAT <= 2 ? 2 : 1) void decay_walk_kernel(Decay
         const bool ends = down ? seg == 0 : lastseg;    // holds the walk's last token
         const bool begins = down ? lastseg : seg == 0;  // holds its first
         if (MODE == STATE && (T == 0 || ends)) return;
-        wave_sync();
-        if (lane < C) {
-            pw.near[lane] = (float)exp(lg * lane);
-            pw.first[lane] = (float)exp(lg * (lane + e0)) * q.sa;
+        const float *pa = q.a + (hd / q.ga) * q.da, *pb = q.b + (hd / q.gb) * q.da,
+                    *pc = q.c + (hd / q.gc) * q.dc;
+        f32x4 af[4 * DAT], bf[4 * DAT];
+        float cf[16], bcol[MODE == STATE ? DAT : 1][16];
+        {
+            const int L = min(C, T);
+            const ChunkRows rb(pb, q.bs, q.da, w, 0, L);
+            if constexpr (MODE != STATE) {
+                load_rows<DAT>(rb, ln, half, bf);
+                load_rows<DAT>(ChunkRows(pa, q.as, q.da, w, 0, L), ln, half, af);
+            } else {
+#pragma unroll
+                for (int d = 0; d < DAT; d++) load_cols(rb, half, 32 * d + ln, bcol[d]);
+            }
+            load_cols(ChunkRows(pc, q.cs, q.dc, w, 0, L), half, col, cf);
         }
         // the state: rows 32 d + tile_row(r) + half, column col
         const float *s0 = MODE == STATE ? nullptr : g.nseg > 1 ? q.seg + sg : begins && q.s0 ? q.s0 + st : nullptr;
@@ -338,11 +366,15 @@ __global__ __launch_bounds__(256, DAT <= 2 ? 2 : 1) void decay_walk_kernel(Decay
                 for (int r = 0; r < 16; r++) S[d][r] = x.load(d, r);
         }
         bool any = s0 != nullptr;  // whether the state may be other than 0
-        const float *pa = q.a + (hd / q.ga) * q.da, *pb = q.b + (hd / q.gb) * q.da,
-                    *pc = q.c + (hd / q.gc) * q.dc;
+        const double lg = log_gamma(g.rate[hd]);
+        wave_sync();
+        if (lane < C) {
+            pw.near[lane] = (float)exp(lg * lane);
+            pw.first[lane] = (float)exp(lg * (lane + e0)) * q.sa;
+        }
         float hi = 0.f, lo = 0.f;  // gamma^L, in two parts
         for (int c0 = 0; c0 < T; c0 += C) {
-            const int L = min(C, T - c0);
+            const int L = min(C, T - c0), next = min(C, max(T - c0 - C, 0));
             if (c0 == 0 || L < C) {
                 const double all = exp(lg * L);
                 hi = (float)all;
@@ -351,32 +383,32 @@ __global__ __launch_bounds__(256, DAT <= 2 ? 2 : 1) void decay_walk_kernel(Decay
                 if (lane < C) pw.left[lane] = (float)exp(lg * max(L - lane - e0, 0)) * q.sb;
                 wave_sync();
             }
-            const ChunkRows rb(pb, q.bs, q.da, w, c0, L), rc(pc, q.cs, q.dc, w, c0, L);
-            float cf[16];
-            const uint32_t c_at = rc.at(half, col);
-#pragma unroll
-            for (int r = 0; r < 16; r++) cf[r] = rc.load(rc.go(c_at, tile_row(r)));
+            // whether a reader of the state follows
+            const bool goes = MODE == STATE || c0 + L < T || slope || (ends && q.s1);
             if constexpr (MODE != STATE) {
-                const ChunkRows ra(pa, q.as, q.da, w, c0, L);
-                f32x4 af[4 * DAT];
                 f32x16 P, o, oz;
 #pragma unroll
                 for (int r = 0; r < 16; r++) P[r] = o[r] = oz[r] = 0.f;
-                load_rows<DAT, FULL>(ra, ln, half, af);
-                {
-                    f32x4 bf[4 * DAT];
-                    load_rows<DAT, FULL>(rb, ln, half, bf);
+                cut_rows<DAT, FULL>(q.da, half, af);
+                cut_rows<DAT, FULL>(q.da, half, bf);
+                wave_sync();
 #pragma unroll
-                    for (int k = 0; k < 4 * DAT; k++)
+                for (int k = 0; k < 4 * DAT; k++) *(f32x4 *)(bt + ln * BS + 8 * k + half) = bf[k];
 #pragma unroll
-                        for (int e = 0; e < 4; e++) P = mm32(bf[k][e], af[k][e], P);
-                }
+                for (int k = 0; k < 4 * DAT; k++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) P = mm32(bf[k][e], af[k][e], P);
+                __builtin_amdgcn_sched_barrier(0);
+                load_rows<DAT>(ChunkRows(pb, q.bs, q.da, w, c0 + C, next), ln, half, bf);
+                __builtin_amdgcn_sched_barrier(0);
                 const int query = opaque(ln - half);
                 const float sab = q.sa * q.sb;
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
+                    // keys behind the query: 0, also of what is no number
                     const int far = query - tile_row(r);
-                    P[r] = far >= 0 ? P[r] * (pw.near[max(far, 0)] * sab) : 0.f;
+                    const float v = __uint_as_float(__float_as_uint(P[r]) & ~(uint32_t)(far >> 31));
+                    P[r] = v * (pw.near[max(far, 0)] * sab);
                 }
                 if (any) {
                     float row[16];
@@ -398,20 +430,12 @@ __global__ __launch_bounds__(256, DAT <= 2 ? 2 : 1) void decay_walk_kernel(Decay
 #pragma unroll
                     for (int r = 0; r < 16; r++) o[r] *= row[r];
                 }
+                __builtin_amdgcn_sched_barrier(0);
+                load_rows<DAT>(ChunkRows(pa, q.as, q.da, w, c0 + C, next), ln, half, af);
+                float dot[16];
+                if (slope) load_cols(ChunkRows(q.dot + hd * q.dc, q.ds, q.dc, w, c0, L), half, col, dot);
+                __builtin_amdgcn_sched_barrier(0);
                 o = tri_product(P, cf, o, half);
-                if (slope) {
-                    const float fq = (float)query;
-#pragma unroll
-                    for (int r = 0; r < 16; r++) P[r] *= fq - (float)tile_row(r);
-                    oz = tri_product(P, cf, oz, half);
-                    const ChunkRows rd(q.dot + hd * q.dc, q.ds, q.dc, w, c0, L);
-                    const uint32_t d_at = rd.at(half, col);
-                    float sum = 0.f;
-#pragma unroll
-                    for (int r = 0; r < 16; r++)
-                        sum = __builtin_fmaf(oz[r], rd.load(rd.go(d_at, tile_row(r))), sum);
-                    dg += (double)sum;
-                }
                 const ChunkRows ry(q.y + ho * q.dc, q.ys, q.dc, w, c0, L);
                 const uint32_t y_at = ry.at(half, col);
                 if (q.acc || r0 > 0) {
@@ -420,34 +444,50 @@ __global__ __launch_bounds__(256, DAT <= 2 ? 2 : 1) void decay_walk_kernel(Decay
                 }
 #pragma unroll
                 for (int r = 0; r < 16; r++) ry.store(ry.go(y_at, tile_row(r)), o[r]);
-            }
-            // the state behind the chunk, where a reader follows
-            if (MODE != STATE && c0 + L == T && !slope && !(ends && q.s1)) break;
-            float left[16];
-            places(pw.left, half, left);
-#pragma unroll
-            for (int r = 0; r < 16; r++) cf[r] *= left[r];
-#pragma unroll
-            for (int d = 0; d < DAT; d++) {
-                float bt[16];
-                const uint32_t b_at = rb.at(half, 32 * d + ln);
-#pragma unroll
-                for (int r = 0; r < 16; r++) bt[r] = rb.load(rb.go(b_at, tile_row(r)));
                 if (slope) {
-                    const float fl = (float)(L - 1 - half);
+                    const float fq = (float)query;
 #pragma unroll
-                    for (int r = 0; r < 16; r++)
-                        Z[d][r] = decayed(__builtin_fmaf((float)L, S[d][r], Z[d][r]), hi, lo);
+                    for (int r = 0; r < 16; r++) P[r] *= fq - (float)tile_row(r);
+                    oz = tri_product(P, cf, oz, half);
+                    float sum = 0.f;
 #pragma unroll
-                    for (int r = 0; r < 16; r++)
-                        Z[d] = mm32(bt[r], cf[r] * (fl - (float)tile_row(r)), Z[d]);
+                    for (int r = 0; r < 16; r++) sum = __builtin_fmaf(oz[r], dot[r], sum);
+                    dg += (double)sum;
                 }
-#pragma unroll
-                for (int r = 0; r < 16; r++) S[d][r] = decayed(S[d][r], hi, lo);
-#pragma unroll
-                for (int r = 0; r < 16; r++) S[d] = mm32(bt[r], cf[r], S[d]);
             }
-            any = true;
+            if (goes) {
+                float left[16];
+                places(pw.left, half, left);
+#pragma unroll
+                for (int r = 0; r < 16; r++) cf[r] *= left[r];
+#pragma unroll
+                for (int d = 0; d < DAT; d++) {
+                    float bd[16];
+#pragma unroll
+                    for (int r = 0; r < 16; r++)
+                        bd[r] = MODE == STATE ? bcol[MODE == STATE ? d : 0][r]
+                                              : bt[(tile_row(r) + half) * BS + 32 * d + ln];
+                    if (slope) {
+                        const float fl = (float)(L - 1 - half);
+#pragma unroll
+                        for (int r = 0; r < 16; r++)
+                            Z[d][r] = decayed(__builtin_fmaf((float)L, S[d][r], Z[d][r]), hi, lo);
+#pragma unroll
+                        for (int r = 0; r < 16; r++)
+                            Z[d] = mm32(bd[r], cf[r] * (fl - (float)tile_row(r)), Z[d]);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 16; r++) S[d][r] = decayed(S[d][r], hi, lo);
+#pragma unroll
+                    for (int r = 0; r < 16; r++) S[d] = mm32(bd[r], cf[r], S[d]);
+                    if constexpr (MODE == STATE)
+                        load_cols(ChunkRows(pb, q.bs, q.da, w, c0 + C, next), half, 32 * d + ln, bcol[d]);
+                }
+                any = true;
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            load_cols(ChunkRows(pc, q.cs, q.dc, w, c0 + C, next), half, col, cf);
+            __builtin_amdgcn_sched_barrier(0);
         }
         const float *sgrad = !slope || !T ? nullptr : g.nseg > 1 ? q.segg + sg : q.s1g ? q.s1g + st : nullptr;
         float *s1 = MODE == STATE ? q.seg + sg : ends && q.s1 ? q.s1 + st : nullptr;
@@ -763,15 +803,19 @@ int rnn_decay_attn_backward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n
         jk.seg = jv.seg = sg.job[1].seg;
         jq.segg = sg.job[1].seg;
     }
-    // one launch where the three jobs' states have as many tiles, else dv's apart
+    // dq: with the rates' gradient it takes twice the registers, by itself; dk and
+    // dv together where their states have as many tiles
+    DecayArgs one = g;
+    if (drate) {
+        launch_walk<WALK_RATE>(ctx, one, 1);
+        RNN_LAUNCHED(ctx);
+        one.job[0] = jk;
+        one.job[1] = jv;
+    }
     const bool joint = (dk + 31) / 32 == (dv + 31) / 32;
-    if (drate)
-        launch_walk<WALK_RATE>(ctx, g, joint ? 3 : 2);
-    else
-        launch_walk<WALK>(ctx, g, joint ? 3 : 2);
+    launch_walk<WALK>(ctx, one, (drate ? 1 : 2) + (joint ? 1 : 0));
     RNN_LAUNCHED(ctx);
     if (!joint) {
-        DecayArgs one = g;
         one.job[0] = jv;
         launch_walk<WALK>(ctx, one, 1);
         RNN_LAUNCHED(ctx);

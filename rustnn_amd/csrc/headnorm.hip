@@ -8,9 +8,9 @@
 // One read of each input and one write of each output: HBM-bound.  A head is
 // owned by L lanes (a power of two) of eight channels each, held in registers
 // between the sum and its use; groups of L lanes take consecutive heads, so
-// that a wave reads whole lines.  Squares, dots and what they are multiplied
-// with are in 64 bits: a square passes a float's range from 2^64 on and falls
-// below it from 2^-75, and 64-bit additions run at the rate of 32-bit ones here.
+// that a wave reads whole lines; the next head's loads are in flight while one is
+// worked on.  Squares are summed in 64 bits: a square passes a float's range from
+// 2^64 on and falls below it from 2^-75.  So are the sums over lanes and rows.
 #include "rotary_angle.h"
 
 #include <algorithm>
@@ -19,8 +19,8 @@ namespace {
 
 constexpr int MAX_HEAD = 256;      // channels of a head with rotary positions
 constexpr int MAX_GATE = 512;      // channels of a gated head
-constexpr int MAX_BLOCKS = 8192;   // of a forward: 32 a CU
-constexpr int MAX_PARTS = 1024;    // of a backward, each leaving its part of dgain
+constexpr int MAX_BLOCKS = 1280;   // of a forward: 5 a CU
+constexpr int MAX_PARTS = 768;     // of a backward: 3 a CU, each leaving its part of dgain
 constexpr int TABLE = 512;         // sines and cosines of a block's rows
 
 // The sum over the L lanes of a group, every lane receiving it, in a fixed tree.
@@ -33,6 +33,39 @@ __device__ __forceinline__ double group_sum(double v, int L) {
     if (L > 32) v += __shfl_xor(v, 32, 64);
     return v;
 }
+
+// 1 / sqrt(v): the instruction's approximation, within 2^-23, and a Newton step on
+// it, which leaves 3/8 of its square: below 2^-46.
+__device__ __forceinline__ double inv_sqrt(double v) {
+    const double r = __builtin_amdgcn_rsq(v);
+    return fma(0.5 * r, fma(-v * r, r, 1.0), r);
+}
+
+// 1 / (1 + exp(-z)), within 6.5 U (U = 2^-24).  exp(-z) as a power of two, its exponent
+// in two parts, so that far gates lose nothing: the instruction's 2 U and two
+// products; the sum's U; its reciprocal by the instruction (2 U) and a Newton step
+// on it: 1.5 U.  Below -88 it is 0.
+__device__ __forceinline__ float sigmoid(float z) {
+    z = fminf(fmaxf(z, -104.f), 104.f);
+    const float t = z * -1.44269504f;
+    const float lo = __builtin_fmaf(z, -1.44269504f, -t) + z * -1.92596299e-8f;
+    const float e = __builtin_amdgcn_exp2f(t) * __builtin_fmaf(lo, 0.69314718f, 1.f);
+    const float d = 1.f + e, r = __builtin_amdgcn_rcpf(d);
+    return d < 0x1p126f ? __builtin_fmaf(r, __builtin_fmaf(-d, r, 1.f), r) : 0.f;
+}
+
+// x^ in 32 bits whatever the head's size: 1 / norm as a float of [1, 2) times a
+// power of two, which the channels take first.
+struct Norm32 {
+    float r, up;  // 1 / norm = r up
+    __device__ __forceinline__ explicit Norm32(double rn) {
+        const int e = (int)((uint64_t)__double_as_longlong(rn) >> 52) - 1023;
+        const int k = max(-126, min(e, 126));
+        up = __uint_as_float((uint32_t)(k + 127) << 23);
+        r = (float)(rn * (double)__uint_as_float((uint32_t)(127 - k) << 23));
+    }
+    __device__ __forceinline__ float operator()(float v) const { return v * up * r; }
+};
 
 // Eight sums a lane over the groups of a block (256 threads), to out[e] by the
 // first group's lanes: store(lane of the group, e, sum).
@@ -65,92 +98,89 @@ struct NrArgs {
     int rows, t, h, hq, dh, axes, npairs;
     int p0, p1;  // pairs of the first two axes
     int g1, g2;  // grid sides of the last two axes
-    int lanes, rpb;
+    int lanes, rpb, span;  // a block's rows, of which rpb at a time
     double eps;
     double w[MAX_PAIRS];  // quarter turns per unit of position of every pair
 };
 
-// A lane's channels: element e < 4 is the first channel of its pair e, e >= 4
-// the second one of pair e - 4; lanes past the pairs hold eight channels that
-// do not turn.  -1: no such channel.
-template <bool INTER>
-__device__ __forceinline__ int nr_channel(const NrArgs &g, int u, int e) {
-    const int R = g.npairs, T = (R + 3) / 4;
-    const int p = INTER ? (e < 4 ? 2 * e : 2 * e - 7) : e;
-    if (u < T) {
-        if (4 * u + (e & 3) >= R) return -1;
-        return INTER ? 8 * u + p : e < 4 ? 4 * u + e : R + 4 * u + e - 4;
-    }
-    const int c = 2 * R + 8 * (u - T) + p;
-    return c < g.dh ? c : -1;
-}
-
-// VEC: 16-byte accesses; whole groups of four pairs and of four other
-// channels, rows and heads aligned.
+// A lane's channels: two runs of four, from ca and cb on, neighbouring lanes' runs
+// next to each other, so that a load takes whole lines.  Lanes before T hold four
+// pairs: (j, j + R) of the two runs, or, alternating, two pairs of each run; those
+// past them channels that do not turn.  As elements, e < 4 is the first channel of
+// the lane's pair e and e >= 4 the second one of pair e - 4.
+// VEC: 16-byte accesses; R and dh are multiples of four, rows and heads aligned.
+// Else a run's four pairs end where R ends, and channels are loaded one by one.
 template <bool VEC, bool INTER>
-__device__ __forceinline__ void nr_load(const NrArgs &g, const float *p, int u, float (&v)[8]) {
-    if constexpr (VEC) {
-        const int R = g.npairs, T = R / 4;
-        const int ca = u < T ? (INTER ? 8 * u : 4 * u) : 2 * R + 8 * (u - T);
-        const int cb = u < T && !INTER ? R + 4 * u : ca + 4;
-        const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-        const float4 a = ca < g.dh ? *(const float4 *)(p + ca) : z;
-        const float4 b = cb < g.dh ? *(const float4 *)(p + cb) : z;
-        if constexpr (INTER) {
-            v[0] = a.x, v[4] = a.y, v[1] = a.z, v[5] = a.w;
-            v[2] = b.x, v[6] = b.y, v[3] = b.z, v[7] = b.w;
-        } else {
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-            v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        }
-    } else {
+struct NrLane {
+    int ca, cb, u, R, dh;
+    bool turned;
+    __device__ __forceinline__ NrLane(const NrArgs &g, int lane) : u(lane), R(g.npairs), dh(g.dh) {
+        const int T = (R + 3) / 4, n = (dh - 2 * R + 7) / 8, v = u - T;
+        turned = u < T;
+        ca = turned ? (VEC || !INTER ? 4 * u : 8 * u) : v < n ? 2 * R + 4 * v : dh;
+        cb = turned ? (VEC || !INTER ? R + 4 * u : 8 * u + 4) : v < n ? 2 * R + 4 * (n + v) : dh;
+    }
+    // the pair of elements q and q + 4
+    __device__ __forceinline__ int pair(int q) const {
+        return VEC && INTER ? (q < 2 ? 2 * u + q : R / 2 + 2 * u + q - 2) : 4 * u + q;
+    }
+    // element e's place in the two runs, and its channel; -1: none
+    static __device__ __forceinline__ constexpr int place(int e) {
+        return INTER ? (e < 4 ? 2 * e : 2 * e - 7) : e;
+    }
+    __device__ __forceinline__ int channel(int e) const {
+        const int p = place(e), c = p < 4 ? ca + p : cb + p - 4;
+        if (turned) return VEC || 4 * u + (e & 3) < R ? c : -1;
+        return c < dh ? c : -1;
+    }
+    __device__ __forceinline__ void load(const float *p, float (&v)[8]) const {
+        if constexpr (VEC) {
+            float t[8];
+            const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+            *(float4 *)t = ca < dh ? *(const float4 *)(p + ca) : z;
+            *(float4 *)(t + 4) = cb < dh ? *(const float4 *)(p + cb) : z;
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const int c = nr_channel<INTER>(g, u, e);
-            v[e] = c >= 0 ? p[c] : 0.f;
+            for (int e = 0; e < 8; e++) v[e] = t[place(e)];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int c = channel(e);
+                v[e] = c >= 0 ? p[c] : 0.f;
+            }
         }
     }
-}
-
-template <bool VEC, bool INTER>
-__device__ __forceinline__ void nr_store(const NrArgs &g, float *p, int u, const float (&v)[8]) {
-    if constexpr (VEC) {
-        const int R = g.npairs, T = R / 4;
-        const int ca = u < T ? (INTER ? 8 * u : 4 * u) : 2 * R + 8 * (u - T);
-        const int cb = u < T && !INTER ? R + 4 * u : ca + 4;
-        float4 a, b;
-        if constexpr (INTER) {
-            a = make_float4(v[0], v[4], v[1], v[5]);
-            b = make_float4(v[2], v[6], v[3], v[7]);
-        } else {
-            a = make_float4(v[0], v[1], v[2], v[3]);
-            b = make_float4(v[4], v[5], v[6], v[7]);
-        }
-        if (ca < g.dh) *(float4 *)(p + ca) = a;
-        if (cb < g.dh) *(float4 *)(p + cb) = b;
-    } else {
+    __device__ __forceinline__ void store(float *p, const float (&v)[8]) const {
+        if constexpr (VEC) {
+            float t[8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const int c = nr_channel<INTER>(g, u, e);
-            if (c >= 0) p[c] = v[e];
+            for (int e = 0; e < 8; e++) t[place(e)] = v[e];
+            if (ca < dh) *(float4 *)(p + ca) = *(const float4 *)t;
+            if (cb < dh) *(float4 *)(p + cb) = *(const float4 *)(t + 4);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int c = channel(e);
+                if (c >= 0) p[c] = v[e];
+            }
         }
     }
-}
+};
 
-// A block takes `rpb` rows at a time: their sines and cosines into LDS, formed
+// A block has `span` rows, of which it takes `rpb` at a time: their sines and cosines into LDS, formed
 // once for all heads, then every head.
 template <bool VEC, bool INTER, bool BACK>
-__global__ __launch_bounds__(256) void norm_rotary_kernel(NrArgs g) {
+__global__ __launch_bounds__(256, BACK ? 3 : VEC ? 5 : 4) void norm_rotary_kernel(NrArgs g) {
     __shared__ __attribute__((aligned(16))) float2 tab[TABLE];
-    const int L = g.lanes, R = g.npairs, T = (R + 3) / 4;
-    const int ng = 256 / L, grp = threadIdx.x / L, u = threadIdx.x & (L - 1);
-    const bool turned = u < T;
+    const int L = g.lanes, R = g.npairs;
+    const int ng = 256 / L, grp = threadIdx.x / L;
+    using Lane = NrLane<VEC, INTER>;
+    const Lane own(g, threadIdx.x & (L - 1));
     float gain[2][8];
 #pragma unroll
     for (int k = 0; k < 2; k++)
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            const int c = nr_channel<INTER>(g, u, e);
+            const int c = own.channel(e);
             gain[k][e] = c < 0 ? 0.f : g.gain ? g.gain[k * g.dh + c] : 1.f;
         }
     double acc[2][8];
@@ -161,9 +191,9 @@ __global__ __launch_bounds__(256) void norm_rotary_kernel(NrArgs g) {
             for (int e = 0; e < 8; e++) acc[k][e] = 0.0;
     }
     const double inv = 1.0 / g.dh;
-    for (long long row0 = (long long)blockIdx.x * g.rpb; row0 < g.rows;
-         row0 += (long long)gridDim.x * g.rpb) {
-        const int nrow = (int)min((long long)g.rpb, g.rows - row0);
+    const long long begin = (long long)blockIdx.x * g.span, end = min(begin + g.span, (long long)g.rows);
+    for (long long row0 = begin; row0 < end; row0 += g.rpb) {
+        const int nrow = (int)min((long long)g.rpb, end - row0);
         __syncthreads();
         for (int e = threadIdx.x; e < nrow * R; e += 256) {
             const int lr = e / R, j = e - lr * R;
@@ -175,27 +205,41 @@ __global__ __launch_bounds__(256) void norm_rotary_kernel(NrArgs g) {
 #pragma unroll
         for (int k = 0; k < 2; k++) {
             const int hn = k ? g.h - g.hq : g.hq, items = nrow * hn;
+            if (items == 0) continue;
+            float v[8], d[8], nv[8], nd[8];
+            long long r, nr;
+            int hd, lr, nhd, nlr;
+            auto fetch = [&](int it) {
+                it = min(it, items - 1);
+                nlr = it / hn;
+                nhd = it - nlr * hn + k * g.hq;
+                nr = row0 + nlr;
+                own.load(g.x + nr * g.xstride + nhd * g.dh, nv);
+                if constexpr (BACK) own.load(g.dy + nr * g.dystride + nhd * g.dh, nd);
+            };
+            fetch(grp);
             for (int i0 = 0; i0 < items; i0 += ng) {
                 const bool live = i0 + grp < items;
-                const int it = live ? i0 + grp : items - 1;
-                const int lr = it / hn, hd = it - lr * hn + k * g.hq;
-                const long long r = row0 + lr;
-                float v[8], d[8];
-                nr_load<VEC, INTER>(g, g.x + r * g.xstride + hd * g.dh, u, v);
-                if constexpr (BACK) nr_load<VEC, INTER>(g, g.dy + r * g.dystride + hd * g.dh, u, d);
+                r = nr, hd = nhd, lr = nlr;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    v[e] = nv[e];
+                    if constexpr (BACK) d[e] = nd[e];
+                }
+                if (i0 + ng < items) fetch(i0 + ng + grp);
                 double s = 0.0;
 #pragma unroll
                 for (int e = 0; e < 8; e++) s = fma((double)v[e], (double)v[e], s);
-                const double rn = 1.0 / sqrt(group_sum(s, L) * inv + g.eps);
+                const double rn = inv_sqrt(group_sum(s, L) * inv + g.eps);
                 float o[8];
                 if constexpr (!BACK) {
 #pragma unroll
                     for (int e = 0; e < 8; e++) d[e] = (float)(v[e] * rn) * gain[k][e];
                 }
-                if (turned) {
+                if (own.turned) {
 #pragma unroll
                     for (int q = 0; q < 4; q++) {
-                        const float2 w = tab[lr * R + min(4 * u + q, R - 1)];
+                        const float2 w = tab[lr * R + min(own.pair(q), R - 1)];
                         o[q] = __builtin_fmaf(d[q], w.x, -(d[q + 4] * w.y));
                         o[q + 4] = __builtin_fmaf(d[q + 4], w.x, d[q] * w.y);
                     }
@@ -204,20 +248,21 @@ __global__ __launch_bounds__(256) void norm_rotary_kernel(NrArgs g) {
                     for (int e = 0; e < 8; e++) o[e] = d[e];
                 }
                 if constexpr (BACK) {
-                    double m = 0.0;
-                    double hat[8], t[8];
+                    const Norm32 hat32(rn);
+                    float hat[8], m32 = 0.f;
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
-                        hat[e] = v[e] * rn;
-                        if (live) acc[k][e] = fma((double)o[e], hat[e], acc[k][e]);
-                        t[e] = (double)o[e] * gain[k][e];
-                        m = fma(t[e], hat[e], m);
+                        hat[e] = hat32(v[e]);
+                        if (live) acc[k][e] = fma((double)o[e], (double)hat[e], acc[k][e]);
+                        o[e] *= gain[k][e];
+                        m32 = __builtin_fmaf(o[e], hat[e], m32);
                     }
-                    m = group_sum(m, L) * inv;
+                    m32 = (float)(group_sum((double)m32, L) * inv);
 #pragma unroll
-                    for (int e = 0; e < 8; e++) o[e] = (float)(fma(-hat[e], m, t[e]) * rn);
+                    for (int e = 0; e < 8; e++)
+                        o[e] = hat32(__builtin_fmaf(-hat[e], m32, o[e]));
                 }
-                if (live) nr_store<VEC, INTER>(g, g.y + r * g.ystride + hd * g.dh, u, o);
+                if (live) own.store(g.y + r * g.ystride + hd * g.dh, o);
             }
         }
     }
@@ -226,7 +271,7 @@ __global__ __launch_bounds__(256) void norm_rotary_kernel(NrArgs g) {
 #pragma unroll
         for (int k = 0; k < 2; k++)
             block_sum8(acc[k], L, [&](int lane, int e, double s) {
-                const int c = nr_channel<INTER>(g, lane, e);
+                const int c = Lane(g, lane).channel(e);
                 if (c >= 0) g.part[((long long)blockIdx.x * 2 + k) * g.dh + c] = s;
             });
     }
@@ -243,91 +288,133 @@ struct GateArgs {
     double eps;
 };
 
+// A lane's channels: four from c on, and four from c + 4 L on.
 template <bool VEC>
-__device__ __forceinline__ void gate_load(const float *p, int c, int d, float (&v)[8]) {
+__device__ __forceinline__ void gate_load(const float *p, int c, int c2, int d, float (&v)[8]) {
     if constexpr (VEC) {
         const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
         *(float4 *)v = c < d ? *(const float4 *)(p + c) : z;
-        *(float4 *)(v + 4) = c + 4 < d ? *(const float4 *)(p + c + 4) : z;
+        *(float4 *)(v + 4) = c2 < d ? *(const float4 *)(p + c2) : z;
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = c + e < d ? p[c + e] : 0.f;
+        for (int e = 0; e < 8; e++) {
+            const int at = e < 4 ? c + e : c2 + e - 4;
+            v[e] = at < d ? p[at] : 0.f;
+        }
     }
 }
 template <bool VEC>
-__device__ __forceinline__ void gate_store(float *p, int c, int d, const float (&v)[8]) {
+__device__ __forceinline__ void gate_store(float *p, int c, int c2, int d, const float (&v)[8]) {
     if constexpr (VEC) {
         if (c < d) *(float4 *)(p + c) = *(const float4 *)v;
-        if (c + 4 < d) *(float4 *)(p + c + 4) = *(const float4 *)(v + 4);
+        if (c2 < d) *(float4 *)(p + c2) = *(const float4 *)(v + 4);
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; e++)
-            if (c + e < d) p[c + e] = v[e];
+        for (int e = 0; e < 8; e++) {
+            const int at = e < 4 ? c + e : c2 + e - 4;
+            if (at < d) p[at] = v[e];
+        }
     }
 }
 
 // Block b: head b % h, rows (b / h) * groups + group, and every splits * groups
-// further, so that dgain's sums stay with one head's channels.
+// further, so that dgain's sums stay with one head's channels.  (Neighbouring
+// heads in one block, whole rows at a time, took no less: 2.1 to 2.4 TB/s.)
 template <bool VEC, bool BACK>
 __global__ __launch_bounds__(256) void head_gate_kernel(GateArgs g) {
-    const int L = g.lanes, ng = 256 / L, grp = threadIdx.x / L, u = threadIdx.x & (L - 1);
+    const int L = g.lanes, ng = 256 / L, at = threadIdx.x / L, u = threadIdx.x & (L - 1);
     const int head = blockIdx.x % g.h, split = blockIdx.x / g.h, splits = gridDim.x / g.h;
-    const int c = 8 * u, col = head * g.d;
+    const int c = 4 * u, c2 = 4 * (L + u), col = head * g.d;
     const long long w = (long long)g.h * g.d;
     float gain[8];
 #pragma unroll
-    for (int e = 0; e < 8; e++) gain[e] = c + e >= g.d ? 0.f : g.gain ? g.gain[col + c + e] : 1.f;
+    for (int e = 0; e < 8; e++) {
+        const int at = e < 4 ? c + e : c2 + e - 4;
+        gain[e] = at >= g.d ? 0.f : g.gain ? g.gain[col + at] : 1.f;
+    }
     double acc[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) acc[e] = 0.0;
     const double inv = 1.0 / g.d;
-    for (long long r0 = (long long)split * ng; r0 < g.rows; r0 += (long long)splits * ng) {
-        const bool live = r0 + grp < g.rows;
-        const long long r = live ? r0 + grp : g.rows - 1;
-        float v[8], z[8], d[8];
-        gate_load<VEC>(g.x + r * w + col, c, g.d, v);
-        gate_load<VEC>(g.z + r * g.zstride + col, c, g.d, z);
-        if constexpr (BACK) gate_load<VEC>(g.dy + r * w + col, c, g.d, d);
+    const long long step = (long long)splits * ng;
+    float v[8], z[8], d[8], nv[8], nz[8], nd[8];
+    long long r, nr;
+    auto fetch = [&](long long at) {
+        nr = min(at, g.rows - 1);
+        gate_load<VEC>(g.x + nr * w + col, c, c2, g.d, nv);
+        gate_load<VEC>(g.z + nr * g.zstride + col, c, c2, g.d, nz);
+        if constexpr (BACK) gate_load<VEC>(g.dy + nr * w + col, c, c2, g.d, nd);
+    };
+    fetch((long long)split * ng + at);
+    for (long long r0 = (long long)split * ng; r0 < g.rows; r0 += step) {
+        const bool live = r0 + at < g.rows;
+        r = nr;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            v[e] = nv[e], z[e] = nz[e];
+            if constexpr (BACK) d[e] = nd[e];
+        }
+        if (r0 + step < g.rows) fetch(r0 + step + at);
         double s = 0.0;
 #pragma unroll
         for (int e = 0; e < 8; e++) s = fma((double)v[e], (double)v[e], s);
-        const double rn = 1.0 / sqrt(group_sum(s, L) * inv + g.eps);
+        const double rn = inv_sqrt(group_sum(s, L) * inv + g.eps);
         float o[8];
         if constexpr (!BACK) {
 #pragma unroll
             for (int e = 0; e < 8; e++)
-                o[e] = (float)(v[e] * rn) * gain[e] * (z[e] / (1.f + expf(-z[e])));
+                o[e] = (float)(v[e] * rn) * gain[e] * (z[e] * sigmoid(z[e]));
         } else {
-            float dz[8];
-            double hat[8], t[8], m = 0.0;
+            const Norm32 hat32(rn);
+            float dz[8], hat[8], m32 = 0.f;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float sig = 1.f / (1.f + expf(-z[e]));
-                hat[e] = v[e] * rn;
-                dz[e] = d[e] * ((float)hat[e] * gain[e]) * (sig * (1.f + z[e] * (1.f - sig)));
-                const double du = (double)d[e] * (z[e] * sig);
-                if (live) acc[e] = fma(du, hat[e], acc[e]);
-                t[e] = du * gain[e];
-                m = fma(t[e], hat[e], m);
+                const float sig = sigmoid(z[e]);
+                hat[e] = hat32(v[e]);
+                dz[e] = d[e] * (hat[e] * gain[e]) * (sig * (1.f + z[e] * (1.f - sig)));
+                o[e] = d[e] * (z[e] * sig);
+                if (live) acc[e] = fma((double)o[e], (double)hat[e], acc[e]);
+                o[e] *= gain[e];
+                m32 = __builtin_fmaf(o[e], hat[e], m32);
             }
-            m = group_sum(m, L) * inv;
+            m32 = (float)(group_sum((double)m32, L) * inv);
 #pragma unroll
-            for (int e = 0; e < 8; e++) o[e] = (float)(fma(-hat[e], m, t[e]) * rn);
-            if (live) gate_store<VEC>(g.dz + r * g.dzstride + col, c, g.d, dz);
+            for (int e = 0; e < 8; e++) o[e] = hat32(__builtin_fmaf(-hat[e], m32, o[e]));
+            if (live) gate_store<VEC>(g.dz + r * g.dzstride + col, c, c2, g.d, dz);
         }
-        if (live) gate_store<VEC>(g.y + r * w + col, c, g.d, o);
+        if (live) gate_store<VEC>(g.y + r * w + col, c, c2, g.d, o);
     }
     if constexpr (BACK) {
         if (!g.part) return;
         block_sum8(acc, L, [&](int lane, int e, double s) {
-            if (8 * lane + e < g.d) g.part[split * w + col + 8 * lane + e] = s;
+            const int at = e < 4 ? 4 * lane + e : 4 * (L + lane) + e - 4;
+            if (at < g.d) g.part[split * w + col + at] = s;
         });
     }
 }
 
-__global__ __launch_bounds__(256) void gain_reduce_kernel(int nrow, size_t len, const double *part,
+// out[j] += the sum of part [nrow][len]'s column j, four columns a block: each over
+// 64 groups of rows in order, then over the groups.
+__global__ __launch_bounds__(256) void gain_reduce_kernel(int nrow, int len, const double *part,
                                                           float *out) {
-    rnn_colsum_red_block(nrow, len, len, part, out, out, blockIdx.x);
+    __shared__ double red[64][4];
+    const int q = threadIdx.x >> 2, j = threadIdx.x & 3, col = (int)blockIdx.x * 4 + j;
+    const int G = (nrow + 63) / 64, k0 = min(nrow, q * G), k1 = min(nrow, k0 + G);
+    double s = 0.0;
+    for (int k = k0; k < k1; k += 16) {
+        double v[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+            v[i] = k + i < k1 && col < len ? part[(size_t)(k + i) * len + col] : 0.0;
+#pragma unroll
+        for (int i = 0; i < 16; i++) s += v[i];
+    }
+    red[q][j] = s;
+    __syncthreads();
+    if (threadIdx.x >= 4 || col >= len) return;
+    double t = red[0][j];
+    for (int i = 1; i < 64; i++) t += red[i][j];
+    out[col] += (float)t;
 }
 
 // ---------------------------------------------------------------- plans
@@ -337,20 +424,21 @@ int pow2_lanes(int units) {
     return L;
 }
 
+// Blocks for `all` pieces of work, at most `most`, with as many pieces each.
+size_t even_blocks(size_t all, size_t most) { return rnn_div_up(all, rnn_div_up(all, most)); }
+
 struct NrPlan {
-    int lanes, rpb, blocks, parts;  // blocks of a forward, of a backward
+    int lanes, rpb, span, blocks;
 };
-NrPlan nr_plan(const rnn_rotary_desc *d, size_t rows) {
+NrPlan nr_plan(const rnn_rotary_desc *d, size_t rows, size_t most) {
     NrPlan p;
     const int R = (int)(d->p0 + d->p1 + d->p2);
     p.lanes = pow2_lanes((R + 3) / 4 + ((int)d->dh - 2 * R + 7) / 8);
-    // rows enough for a sine and cosine a thread, fewer where that would leave
-    // CUs idle
-    const int most = R ? std::min(32, (int)rnn_div_up(256, R)) : 8;
-    p.rpb = (int)std::max<size_t>(1, std::min<size_t>(most, rows / 512));
-    const size_t b = rnn_div_up(rows, p.rpb);
-    p.blocks = (int)std::min<size_t>(b, MAX_BLOCKS);
-    p.parts = (int)std::min<size_t>(b, MAX_PARTS);
+    // a row's blocks at most, as many rows each; of those, enough at a time for a
+    // sine and cosine a thread
+    p.span = (int)rnn_div_up(rows, most);
+    p.rpb = std::min(p.span, R ? std::min(32, (int)rnn_div_up(256, R)) : 8);
+    p.blocks = (int)rnn_div_up(rows, p.span);
     return p;
 }
 
@@ -418,8 +506,8 @@ GatePlan gate_plan(size_t rows, size_t h, size_t d) {
     GatePlan p;
     p.lanes = pow2_lanes((int)rnn_div_up(d, 8));
     const size_t all = rnn_div_up(rows, 256 / p.lanes);
-    p.splits = std::min(all, std::max<size_t>(1, MAX_BLOCKS / h));
-    p.parts = std::min(all, std::max<size_t>(1, MAX_PARTS / h));
+    p.splits = even_blocks(all, std::max<size_t>(1, MAX_BLOCKS / h));
+    p.parts = even_blocks(all, std::max<size_t>(1, MAX_PARTS / h));
     return p;
 }
 
@@ -456,7 +544,7 @@ int rnn_norm_rotary_workspace(const rnn_rotary_desc *d, uint32_t hq, float eps, 
     if (rc) return rc;
     if (!bytes) return RNN_E_NULL;
     const size_t rows = n * t;
-    *bytes = rows ? (size_t)nr_plan(d, rows).parts * 2 * d->dh * sizeof(double) : 0;
+    *bytes = rows ? (size_t)nr_plan(d, rows, MAX_PARTS).blocks * 2 * d->dh * sizeof(double) : 0;
     return RNN_OK;
 }
 
@@ -473,9 +561,10 @@ int rnn_norm_rotary_forward(rnn_ctx *ctx, const rnn_rotary_desc *d, uint32_t hq,
     RNN_ON_DEVICE(ctx);
     NrArgs g;
     nr_fill(g, d, hq, eps, n, t, x, gain, pos, y);
-    const NrPlan p = nr_plan(d, n * t);
+    const NrPlan p = nr_plan(d, n * t, MAX_BLOCKS);
     g.lanes = p.lanes;
     g.rpb = p.rpb;
+    g.span = p.span;
     const bool vec = g.npairs % 4 == 0 && g.dh % 4 == 0 && aligned16(g.x, g.xstride) &&
                      aligned16(g.y, g.ystride);
     nr_launch<false>(ctx, g, p.blocks, vec, d->interleaved != 0);
@@ -500,8 +589,8 @@ int rnn_norm_rotary_backward(rnn_ctx *ctx, const rnn_rotary_desc *d, uint32_t hq
     if (dx == x) return rnn_fail(ctx, RNN_E_INVALID, "norm_rotary: dx is x");
     if (dx == dy && (d->ystride != dystride || d->yoff != dyoff))
         return rnn_fail(ctx, RNN_E_INVALID, "norm_rotary: in place with two layouts");
-    const NrPlan p = nr_plan(d, n * t);
-    rc = ws_checked(ctx, "norm_rotary", dgain ? (size_t)p.parts * 2 * d->dh * sizeof(double) : 0, ws,
+    const NrPlan p = nr_plan(d, n * t, MAX_PARTS);
+    rc = ws_checked(ctx, "norm_rotary", dgain ? (size_t)p.blocks * 2 * d->dh * sizeof(double) : 0, ws,
                     ws_bytes);
     if (rc) return rc;
     RNN_ON_DEVICE(ctx);
@@ -512,14 +601,15 @@ int rnn_norm_rotary_backward(rnn_ctx *ctx, const rnn_rotary_desc *d, uint32_t hq
     g.part = dgain ? (double *)ws : nullptr;
     g.lanes = p.lanes;
     g.rpb = p.rpb;
+    g.span = p.span;
     const bool vec = g.npairs % 4 == 0 && g.dh % 4 == 0 && aligned16(g.x, g.xstride) &&
                      aligned16(g.y, g.ystride) && aligned16(g.dy, g.dystride);
-    nr_launch<true>(ctx, g, p.parts, vec, d->interleaved != 0);
+    nr_launch<true>(ctx, g, p.blocks, vec, d->interleaved != 0);
     RNN_LAUNCHED(ctx);
     if (dgain) {
         const size_t len = 2 * (size_t)d->dh;
-        gain_reduce_kernel<<<(unsigned)rnn_div_up(len, 16), 256, 0, ctx->stream>>>(p.parts, len, g.part,
-                                                                                   dgain);
+        gain_reduce_kernel<<<(unsigned)rnn_div_up(len, 4), 256, 0, ctx->stream>>>(p.blocks, (int)len,
+                                                                                  g.part, dgain);
         RNN_LAUNCHED(ctx);
     }
     return RNN_OK;
@@ -585,8 +675,8 @@ int rnn_head_gate_backward(rnn_ctx *ctx, size_t rows, size_t h, size_t d, float 
         head_gate_kernel<false, true><<<grid, 256, 0, ctx->stream>>>(g);
     RNN_LAUNCHED(ctx);
     if (dgain) {
-        gain_reduce_kernel<<<(unsigned)rnn_div_up((size_t)w, 16), 256, 0, ctx->stream>>>(
-            (int)p.parts, (size_t)w, g.part, dgain);
+        gain_reduce_kernel<<<(unsigned)rnn_div_up((size_t)w, 4), 256, 0, ctx->stream>>>((int)p.parts, (int)w,
+                                                                                        g.part, dgain);
         RNN_LAUNCHED(ctx);
     }
     return RNN_OK;

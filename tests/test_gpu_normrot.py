@@ -4,14 +4,18 @@ their plain statement in 64 bits.
 Tolerances, element by element, U = 2^-24.  Forward: x^ and its product with the
 gain are rounded once each (2 U), then the turn: 3 U and 1e-8 for the angle of
 |a| + |b| (as rotary positions alone): (5 U + 1e-8) (|a| + |b|) of the normed
-pair, second orders below 1e-9.  Backward: the gradient turned back is off by
-e = (3 U + 1e-8) (|da| + |db|), all that follows is in 64 bits and rounded once,
-so dx by |gain| e / norm, by the mean of |gain| e |x^| times |x^| / norm, and by
-U |dx|; dgain by the sum of e |x^| and U |dgain|."""
+pair, second orders below 1e-9.  Backward: the gradient turned back, du, is off by
+e = (3 U + 1e-8) (|da| + |db|); x^ by 2 U (1 / norm and the product), t = gain du by
+U besides.  mean(t x^): a product and up to eight additions in 32 bits (the lanes'
+sums are in 64), so 2 + 1 + 1 + 8 = 12 U of mean |t x^| with its operands' errors.  dx =
+(t - x^ mean) / norm: U |t|, x^'s 2 U, the mean's 12 U and its rounding, the
+difference's rounding U (|t| + |x^| mean |t x^|), 2 U |dx| for the last product:
+U (2 |t| + 17 |x^| mean |t x^|) / norm + 2 U |dx|, and e as it goes through.  dgain: the
+sum of (e + 2 U |du|) |x^|, and U |dgain|."""
 import pytest
 import torch
 
-from decayref import D, U, head_norm, norm_rotary, pair_size
+from decayref import D, U, head_norm, norm_rotary, pair_size, turn
 from test_gpu_rotary import grid_pos
 
 pytestmark = pytest.mark.gpu
@@ -55,9 +59,11 @@ def tolerances(x, gain, dy, hq, hk, dh, pairs, inter, eps, want):
     ty = (5 * U + 1.1e-8) * pair_size((hat * gh).reshape(x.shape), heads, dh, pairs, inter)
     e = (3 * U + 1.1e-8) * pair_size(dy, heads, dh, pairs, inter).view(hat.shape)
     rn = 1 / torch.sqrt((x.view(hat.shape) ** 2).mean(-1, keepdim=True) + eps)
+    du = want["du"].abs().view(hat.shape)
     tx = rn * (gh * e + hat.abs() * (gh * e * hat.abs()).mean(-1, keepdim=True))
-    tx = tx.reshape(x.shape) + 1.01 * U * want["dx"].abs()
-    s = (e * hat.abs()).sum(0)
+    tx += U * rn * (2 * gh * du + 17 * hat.abs() * (gh * du * hat.abs()).mean(-1, keepdim=True))
+    tx = 1.01 * (tx.reshape(x.shape) + 2 * U * want["dx"].abs())
+    s = 1.01 * ((e + 2 * U * du) * hat.abs()).sum(0)
     tg = torch.stack([s[:hq].sum(0), s[hq:].sum(0)]) + 1.01 * U * want["dgain"].abs()
     return ty + 1e-37, tx + 1e-37, tg + 1e-37
 
@@ -67,7 +73,8 @@ def statement(x, gain, dy, hq, hk, dh, pos, pairs, base, inter, eps):
     y = norm_rotary(x, gain, hq, hk, dh, pos, pairs, base, inter, eps)
     dx, dgain = torch.autograd.grad(y, (x, gain), dy)
     x.requires_grad_(False), gain.requires_grad_(False)
-    return dict(y=y.detach(), dx=dx, dgain=dgain)
+    du = turn(dy, hq + hk, dh, pos, pairs, base, inter, inverse=True)
+    return dict(y=y.detach(), dx=dx, dgain=dgain, du=du)
 
 
 @pytest.mark.parametrize("c", CASES, ids=[c[0] for c in CASES])
