@@ -22,6 +22,25 @@ namespace {
 
 constexpr int MAX_D = 128;
 constexpr int C = 32;  // tokens of a chunk
+#ifndef SEG_WAVES
+#define SEG_WAVES 2048
+#define SEG_TOKENS 128
+#endif
+
+// Division of numbers below 2^31 by d: (mulhi(x, m) + x) >> s.
+struct Divider {
+    uint32_t d = 1, m = 0, s = 0;
+    Divider() = default;
+    explicit Divider(uint32_t by) : d(by) {
+        while ((1ull << s) < by) s++;
+        m = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << s) - by)) / by + 1);
+    }
+    __device__ __forceinline__ uint32_t operator()(uint32_t x, uint32_t &rest) const {
+        const uint32_t q = (__umulhi(x, m) + x) >> s;
+        rest = x - q * d;
+        return q;
+    }
+};
 
 struct DecayJob {
     const float *a, *b, *c;
@@ -38,6 +57,7 @@ struct DecayJob {
     int si, sj;         // a state's strides along da and dc
     float sa, sb;       // factors of a and of b
     int rev, acc;       // from the last token; y accumulates
+    Divider slices, heads;  // c's, of 32 channels; those of y
 };
 
 struct DecayArgs {
@@ -47,6 +67,7 @@ struct DecayArgs {
     double *part;  // [n][nseg][slices][h] parts of dL/dg
     int n, t, h, reverse;
     int nseg, slen;  // segments of a sequence, and their tokens
+    Divider segs;
 };
 
 // log gamma of a head: at most 0, and finite, so that its multiple by 0 is 0.
@@ -55,72 +76,108 @@ __device__ __forceinline__ double log_gamma(float rate) {
     return g < -1e30 ? -1e30 : g;
 }
 
+// gamma^m in 32 bits, as a power of two whose exponent m log2(gamma) is in two parts:
+// the instruction's ulp and a product's rounding.
+struct Power {
+    float hi, lo;
+    __device__ __forceinline__ explicit Power(double lg) {
+        const double l2 = fmax(lg, -1e30) * 1.4426950408889634;
+        hi = (float)l2;
+        lo = (float)(l2 - (double)hi);
+    }
+    __device__ __forceinline__ float operator()(int m) const {
+        const float f = (float)m, t = f * hi;
+        const float rest = t < -200.f ? 0.f : __builtin_fmaf(f, hi, -t) + f * lo;
+        return __builtin_amdgcn_exp2f(t) * __builtin_fmaf(rest, 0.69314718f, 1.f);
+    }
+};
+
 // s gamma, gamma in two parts.
 __device__ __forceinline__ float decayed(float s, float gam, float rest) {
     return __builtin_fmaf(s, gam, s * rest);
 }
 
-// Token by token, forward: a block holds a head's state, wave w rows 32 w .. 32 w
-// + 31, a lane columns lane and lane + 64.
+// Token by token, forward: a block holds a head's state, four channels of v a
+// thread in every RP-th row, RP = 256 / G, G groups of four channels (a power of
+// two).  Its read and write are the work: 16 bytes an access (VEC: dv a multiple of
+// four, states aligned), all of them in flight at once.
+template <bool VEC, int G>
 __global__ __launch_bounds__(256) void decay_tokens_kernel(DecayArgs g) {
-    __shared__ float red[4][MAX_D];
+    constexpr int RP = 256 / G, K = MAX_D / RP;
+    __shared__ __attribute__((aligned(16))) float red[RP][4 * G], ab[2][MAX_D];
     const DecayJob &q = g.job[0];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int c4 = 4 * (threadIdx.x & (G - 1)), r0 = threadIdx.x / G;
     const int b = blockIdx.x / g.h, hd = blockIdx.x % g.h;
+    const long long st = ((long long)b * g.h + hd) * q.da * q.dc;
+    f32x4 s[K];
+    const auto each = [&](auto f) {
+#pragma unroll
+        for (int k = 0; k < K; k++)
+            if (r0 + k * RP < q.da && c4 < q.dc) f(k, st + (long long)(r0 + k * RP) * q.dc + c4);
+    };
+#pragma unroll
+    for (int k = 0; k < K; k++) s[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (q.s0)
+        each([&](int k, long long at) {
+            if constexpr (VEC) {
+                s[k] = *(const f32x4 *)(q.s0 + at);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) s[k][e] = c4 + e < q.dc ? q.s0[at + e] : 0.f;
+            }
+        });
     const int len = g.lens ? (int)min(g.lens[b], (uint32_t)g.t) : g.t;
     const bool back = hd >= g.h - g.reverse;
     // gamma in two floats: one rounded alone would be off by its last bit to
     // the power of the tokens
     const double g64 = exp(log_gamma(g.rate[hd]));
     const float gam = (float)g64, rest = (float)(g64 - (double)gam);
-    const long long st = ((long long)b * g.h + hd) * q.da * q.dc;
-    float s[32][2];
-#pragma unroll
-    for (int i = 0; i < 32; i++)
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-            const int ia = 32 * wave + i, jc = lane + 64 * k;
-            s[i][k] = q.s0 && ia < q.da && jc < q.dc ? q.s0[st + ia * q.dc + jc] : 0.f;
-        }
+    const int tid = threadIdx.x;
     for (int i = 0; i < g.t; i++) {
         if (i >= len) {
-            if (threadIdx.x < q.dc)
-                q.y[((long long)b * g.t + i) * q.ys + hd * q.dc + threadIdx.x] = 0.f;
+            if (tid < q.dc) q.y[((long long)b * g.t + i) * q.ys + hd * q.dc + tid] = 0.f;
             continue;
         }
         const long long row = (long long)b * g.t + (back ? len - 1 - i : i);
-        const float *a = q.a + row * q.as + hd * q.da;
-        const float *bb = q.b + row * q.bs + (hd / q.gb) * q.da;
         const float *c = q.c + row * q.cs + (hd / q.gc) * q.dc;
-        float cv[2], o[2] = {0.f, 0.f};
+        if (tid < q.da)
+            ab[0][tid] = q.a[row * q.as + hd * q.da + tid];
+        else if (tid >= 128 && tid - 128 < q.da)
+            ab[1][tid - 128] = q.b[row * q.bs + (hd / q.gb) * q.da + tid - 128];
+        f32x4 cv, o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < 2; k++) cv[k] = lane + 64 * k < q.dc ? c[lane + 64 * k] : 0.f;
+        for (int e = 0; e < 4; e++) cv[e] = c4 + e < q.dc ? c[c4 + e] : 0.f;
+        __syncthreads();
 #pragma unroll
-        for (int e = 0; e < 32; e++) {
-            const int ia = 32 * wave + e;
-            const float av = ia < q.da ? a[ia] : 0.f, bv = ia < q.da ? bb[ia] : 0.f;
+        for (int k = 0; k < K; k++) {
+            const int r = r0 + k * RP;
+            if (r >= q.da) continue;
+            const float av = ab[0][r], bv = ab[1][r];
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
-                s[e][k] = __builtin_fmaf(bv, cv[k], decayed(s[e][k], gam, rest));
-                o[k] = __builtin_fmaf(av, s[e][k], o[k]);
+            for (int e = 0; e < 4; e++) {
+                s[k][e] = __builtin_fmaf(bv, cv[e], decayed(s[k][e], gam, rest));
+                o[e] = __builtin_fmaf(av, s[k][e], o[e]);
             }
         }
+        *(f32x4 *)&red[r0][c4] = o;
         __syncthreads();
+        if (tid < q.dc) {
+            float v = 0.f;
 #pragma unroll
-        for (int k = 0; k < 2; k++) red[wave][lane + 64 * k] = o[k];
-        __syncthreads();
-        const int jc = threadIdx.x;
-        if (jc < q.dc)
-            q.y[row * q.ys + hd * q.dc + jc] = q.sa * (red[0][jc] + red[1][jc] + red[2][jc] + red[3][jc]);
-    }
-    if (!q.s1) return;
-#pragma unroll
-    for (int i = 0; i < 32; i++)
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-            const int ia = 32 * wave + i, jc = lane + 64 * k;
-            if (ia < q.da && jc < q.dc) q.s1[st + ia * q.dc + jc] = s[i][k];
+            for (int k = 0; k < RP; k++) v += red[k][tid];
+            q.y[row * q.ys + hd * q.dc + tid] = q.sa * v;
         }
+    }
+    if (q.s1)
+        each([&](int k, long long at) {
+            if constexpr (VEC) {
+                *(f32x4 *)(q.s1 + at) = s[k];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (c4 + e < q.dc) q.s1[at + e] = s[k][e];
+            }
+        });
 }
 
 __device__ __forceinline__ f32x16 mm32(float a, float b, f32x16 c) {
@@ -298,14 +355,17 @@ __global__ __launch_bounds__(256, DAT <= (MODE == WALK_RATE ? 1 : 2) ? 2 : 1) vo
     __shared__ __attribute__((aligned(16))) float btile[MODE == STATE ? 1 : 4][MODE == STATE ? 4 : C * BS];
     const DecayJob &q = g.job[blockIdx.y];
     const int lane = threadIdx.x & 63, ln = lane & 31, half = 4 * (lane >> 5), wave = wave_index();
-    const int nsl = (q.dc + 31) / 32, heads = g.h / q.gy;
-    uint32_t u = (uint32_t)xcd_order(blockIdx.x, gridDim.x) * 4 + wave;  // fewer than 2^31 waves
-    const int slice = (int)(u % (uint32_t)nsl), col = slice * 32 + ln;
-    u /= (uint32_t)nsl;
-    const int seg = (int)(u % (uint32_t)g.nseg);
-    u /= (uint32_t)g.nseg;
-    const int ho = (int)(u % (uint32_t)heads);
-    const long long b = u / (uint32_t)heads;
+    // the arguments at once: loaded one after the other as they are needed, their
+    // misses took 5000 cycles
+    asm volatile("" ::"s"(q.a), "s"(q.b), "s"(q.c), "s"(q.y), "s"(q.s0), "s"(q.as), "s"(q.bs), "s"(q.cs),
+                 "s"(q.ys), "s"(q.da), "s"(q.ga), "s"(q.sa), "s"(q.rev), "s"(g.rate));
+    uint32_t u = (uint32_t)xcd_order(blockIdx.x, gridDim.x) * 4 + wave, rest;  // fewer than 2^31 waves
+    u = q.slices(u, rest);
+    const int slice = (int)rest, col = slice * 32 + ln;
+    u = g.segs(u, rest);
+    const int seg = (int)rest;
+    const long long b = q.heads(u, rest);
+    const int ho = (int)rest;
     if (b >= g.n) return;
     const int len = __builtin_amdgcn_readfirstlane(g.lens ? (int)min(g.lens[b], (uint32_t)g.t) : g.t);
     const int t0 = seg * g.slen, t1 = min(t0 + g.slen, len), T = max(t1 - t0, 0);
@@ -368,9 +428,10 @@ __global__ __launch_bounds__(256, DAT <= (MODE == WALK_RATE ? 1 : 2) ? 2 : 1) vo
         bool any = s0 != nullptr;  // whether the state may be other than 0
         const double lg = log_gamma(g.rate[hd]);
         wave_sync();
+        const Power pow(lg);
         if (lane < C) {
-            pw.near[lane] = (float)exp(lg * lane);
-            pw.first[lane] = (float)exp(lg * (lane + e0)) * q.sa;
+            pw.near[lane] = pow(lane);
+            pw.first[lane] = pow(lane + e0) * q.sa;
         }
         float hi = 0.f, lo = 0.f;  // gamma^L, in two parts
         for (int c0 = 0; c0 < T; c0 += C) {
@@ -380,7 +441,7 @@ __global__ __launch_bounds__(256, DAT <= (MODE == WALK_RATE ? 1 : 2) ? 2 : 1) vo
                 hi = (float)all;
                 lo = (float)(all - (double)hi);
                 wave_sync();
-                if (lane < C) pw.left[lane] = (float)exp(lg * max(L - lane - e0, 0)) * q.sb;
+                if (lane < C) pw.left[lane] = pow(max(L - lane - e0, 0)) * q.sb;
                 wave_sync();
             }
             // whether a reader of the state follows
@@ -507,7 +568,7 @@ __global__ __launch_bounds__(256, DAT <= (MODE == WALK_RATE ? 1 : 2) ? 2 : 1) vo
         }
         if (slope) {
             dg = rnn_wave_sum_d(dg);
-            if (lane == 0) g.part[((b * g.nseg + seg) * nsl + slice) * g.h + hd] = dg;
+            if (lane == 0) g.part[((b * g.nseg + seg) * q.slices.d + slice) * g.h + hd] = dg;
         }
     }
 }
@@ -527,20 +588,25 @@ __global__ __launch_bounds__(256) void decay_scan_kernel(DecayArgs g) {
     double all64 = exp(lg * g.slen);
     const float hi = (float)all64, lo = (float)(all64 - (double)hi);
     float s = q.s0 ? q.s0[i] : 0.f;
-    if ((hd >= g.h - g.reverse) == (q.rev != 0)) {
-        for (int k = 0; k <= last; k++) {
-            const float own = k < last ? q.seg[k * all + i] : 0.f;
-            q.seg[k * all + i] = s;
-            s = decayed(s, hi, lo) + own;
+    const bool down = (hd >= g.h - g.reverse) != (q.rev != 0);
+    // from the far end the first segment may be short
+    all64 = exp(lg * (len - last * g.slen));
+    const float hi1 = (float)all64, lo1 = (float)(all64 - (double)hi1);
+    // the k-th segment of the walk, eight of them loaded ahead of their stores; the
+    // last one's own state has no reader
+    for (int k0 = 0; k0 <= last; k0 += 8) {
+        float own[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int k = k0 + j;
+            own[j] = k < last ? q.seg[(long long)(down ? last - k : k) * all + i] : 0.f;
         }
-    } else {
-        all64 = exp(lg * (len - last * g.slen));
-        float a = (float)all64, z = (float)(all64 - (double)a);
-        for (int k = last; k >= 0; k--) {
-            const float own = k > 0 ? q.seg[k * all + i] : 0.f;
-            q.seg[k * all + i] = s;
-            s = decayed(s, a, z) + own;
-            a = hi, z = lo;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int k = k0 + j;
+            if (k > last) break;
+            q.seg[(long long)(down ? last - k : k) * all + i] = s;
+            s = (down && k == 0 ? decayed(s, hi1, lo1) : decayed(s, hi, lo)) + own[j];
         }
     }
 }
@@ -570,12 +636,13 @@ DecayPlan plan_of(const rnn_decay_attn_desc *d, size_t n, size_t t, bool backwar
     WsCarve c;
     // few tokens: the state's read and write are all there is to do
     p.tokens = !backward && t <= 8;
-    const size_t nsl = rnn_div_up(backward ? std::max(d->dk, d->dv) : d->dv, 32);
-    const size_t waves = n * d->h * nsl * (backward ? 3 : 1);
+    const size_t kt = rnn_div_up(d->dk, 32), vt = rnn_div_up(d->dv, 32);
+    // the waves of the walk with the fewest
+    const size_t waves = backward ? std::min(n * d->h * kt, n * d->hkv * (kt + vt)) : n * d->h * vt;
     p.slen = (int)rnn_round_up(std::max<size_t>(t, 1), C);
-    if (!p.tokens && waves && waves < 1024 && t > 256) {
-        const size_t want = std::min(rnn_div_up(2048, waves), t / 128);
-        p.slen = (int)rnn_round_up(rnn_div_up(t, want), C);
+    if (!p.tokens && waves && waves < 1024 && t > 4 * C) {
+        const size_t want = std::min(rnn_div_up(SEG_WAVES, waves), t / SEG_TOKENS);
+        p.slen = (int)rnn_round_up(rnn_div_up(t, std::max<size_t>(want, 1)), C);
         p.nseg = (int)rnn_div_up(t, p.slen);
     }
     const size_t states = (size_t)p.nseg * n * d->h * d->dk * d->dv * sizeof(float);
@@ -634,9 +701,9 @@ struct Operand {
     int share;
 };
 
-DecayJob make_job(const Operand &a, const Operand &b, int da, const Operand &c, int dc, float *y,
-                  size_t ys, int gy) {
-    DecayJob j = {};
+DecayJob make_job(uint32_t h, const Operand &a, const Operand &b, int da, const Operand &c, int dc,
+                  float *y, size_t ys, int gy) {
+    DecayJob j{};
     j.a = a.p, j.b = b.p, j.c = c.p, j.y = y;
     j.as = (long long)a.stride, j.bs = (long long)b.stride, j.cs = (long long)c.stride;
     j.ys = (long long)ys;
@@ -644,6 +711,8 @@ DecayJob make_job(const Operand &a, const Operand &b, int da, const Operand &c, 
     j.ga = a.share, j.gb = b.share, j.gc = c.share, j.gy = gy;
     j.si = dc, j.sj = 1;
     j.sa = j.sb = 1.f;
+    j.slices = Divider((uint32_t)(dc + 31) / 32);
+    j.heads = Divider((uint32_t)(h / gy));
     return j;
 }
 
@@ -651,6 +720,7 @@ void fill_args(DecayArgs &g, const rnn_decay_attn_desc *d, const DecayPlan &p, s
                const float *rate, const uint32_t *lens) {
     g.nseg = p.nseg;
     g.slen = p.slen;
+    g.segs = Divider((uint32_t)p.nseg);
     g.rate = rate;
     g.lens = lens;
     g.part = nullptr;
@@ -666,8 +736,7 @@ void launch_walk(rnn_ctx *ctx, const DecayArgs &g, int jobs) {
     bool full = true;
     for (int k = 0; k < jobs; k++) {
         const DecayJob &q = g.job[k];
-        const int nsl = (q.dc + 31) / 32;
-        waves = std::max(waves, (size_t)g.n * (g.h / q.gy) * g.nseg * nsl);
+        waves = std::max(waves, (size_t)g.n * q.heads.d * g.nseg * q.slices.d);
         full = full && q.da % 32 == 0;
     }
     const dim3 grid((unsigned)rnn_div_up(waves, 4), (unsigned)jobs);
@@ -724,12 +793,23 @@ int rnn_decay_attn_forward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n,
     const Operand Q = {q + d->qoff, d->qstride, 1}, K = {kv + d->koff, d->kvstride, grp},
                   V = {kv + d->voff, d->kvstride, grp};
     DecayJob &j = g.job[0];
-    j = make_job(Q, K, (int)d->dk, V, (int)d->dv, y, (size_t)d->h * d->dv, 1);
+    j = make_job(d->h, Q, K, (int)d->dk, V, (int)d->dv, y, (size_t)d->h * d->dv, 1);
     j.s0 = state_in;
     j.s1 = state_out;
     j.sa = d->scale;
     if (w.tokens) {
-        decay_tokens_kernel<<<(unsigned)(n * d->h), 256, 0, ctx->stream>>>(g);
+        const unsigned grid = (unsigned)(n * d->h);
+        const bool vec = d->dv % 4 == 0 && (((uintptr_t)state_in | (uintptr_t)state_out) & 15) == 0;
+#define TOKENS_AS(G)                                                              \
+    (vec ? decay_tokens_kernel<true, G><<<grid, 256, 0, ctx->stream>>>(g)         \
+         : decay_tokens_kernel<false, G><<<grid, 256, 0, ctx->stream>>>(g))
+        if (d->dv > 64)
+            TOKENS_AS(32);
+        else if (d->dv > 32)
+            TOKENS_AS(16);
+        else
+            TOKENS_AS(8);
+#undef TOKENS_AS
         RNN_LAUNCHED(ctx);
         return RNN_OK;
     }
@@ -770,7 +850,7 @@ int rnn_decay_attn_backward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n
                   V = {kv + d->voff, d->kvstride, grp}, O = {dy, (size_t)d->h * d->dv, 1};
     g.part = (double *)((char *)ws + w.part);
     DecayJob &jq = g.job[0], &jk = g.job[1], &jv = g.job[2];
-    jq = make_job(O, V, dv, K, dk, dq + d->qoff, d->qstride, 1);
+    jq = make_job(d->h, O, V, dv, K, dk, dq + d->qoff, d->qstride, 1);
     jq.si = 1, jq.sj = dv;
     jq.s0 = state_in;
     jq.sa = d->scale;
@@ -780,9 +860,9 @@ int rnn_decay_attn_backward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n
         jq.ds = (long long)d->qstride;
         jq.s1g = dstate_out;
     }
-    jk = make_job(V, O, dv, Q, dk, dkv + d->koff, d->kvstride, grp);
+    jk = make_job(d->h, V, O, dv, Q, dk, dkv + d->koff, d->kvstride, grp);
     jk.si = 1, jk.sj = dv;
-    jv = make_job(K, Q, dk, O, dv, dkv + d->voff, d->kvstride, grp);
+    jv = make_job(d->h, K, Q, dk, O, dv, dkv + d->voff, d->kvstride, grp);
     jk.s0 = jv.s0 = dstate_out;
     jk.sb = jv.sb = d->scale;
     jk.rev = jv.rev = 1;
@@ -791,11 +871,12 @@ int rnn_decay_attn_backward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n
     if (w.nseg > 1) {
         // S from the keys and values, R from the queries and dy
         DecayArgs sg = g;
-        sg.job[0] = make_job(Q, K, dk, V, dv, nullptr, 0, 1);
+        sg.job[0] = make_job(d->h, Q, K, dk, V, dv, nullptr, 0, 1);
         sg.job[0].s0 = state_in;
         sg.job[0].seg = (float *)((char *)ws + w.seg);
         sg.job[1] = jv;
         sg.job[1].gy = 1;
+        sg.job[1].heads = Divider(d->h);
         sg.job[1].seg = (float *)((char *)ws + w.segr);
         launch_segments(ctx, sg, 2);
         RNN_LAUNCHED(ctx);
