@@ -22,10 +22,6 @@ namespace {
 
 constexpr int MAX_D = 128;
 constexpr int C = 32;  // tokens of a chunk
-#ifndef SEG_WAVES
-#define SEG_WAVES 2048
-#define SEG_TOKENS 128
-#endif
 
 // Division of numbers below 2^31 by d: (mulhi(x, m) + x) >> s.
 struct Divider {
@@ -53,11 +49,11 @@ struct DecayJob {
     const float *segg;  // the rates' gradient: those of the walk the other way
     long long as, bs, cs, ys, ds;  // row strides
     int da, dc;         // channels
-    int ga, gb, gc, gy; // query heads that share a head of the operand
+    int ga, gb, gc;     // query heads that share a head of the operand
     int si, sj;         // a state's strides along da and dc
     float sa, sb;       // factors of a and of b
     int rev, acc;       // from the last token; y accumulates
-    Divider slices, heads;  // c's, of 32 channels; those of y
+    Divider slices;     // c's channels, by 32
 };
 
 struct DecayArgs {
@@ -67,7 +63,7 @@ struct DecayArgs {
     double *part;  // [n][nseg][slices][h] parts of dL/dg
     int n, t, h, reverse;
     int nseg, slen;  // segments of a sequence, and their tokens
-    Divider segs;
+    Divider segs, heads;
 };
 
 // log gamma of a head: at most 0, and finite, so that its multiple by 0 is 0.
@@ -364,8 +360,8 @@ __global__ __launch_bounds__(256, DAT <= (MODE == WALK_RATE ? 1 : 2) ? 2 : 1) vo
     const int slice = (int)rest, col = slice * 32 + ln;
     u = g.segs(u, rest);
     const int seg = (int)rest;
-    const long long b = q.heads(u, rest);
-    const int ho = (int)rest;
+    const long long b = g.heads(u, rest);
+    const int hd = (int)rest;
     if (b >= g.n) return;
     const int len = __builtin_amdgcn_readfirstlane(g.lens ? (int)min(g.lens[b], (uint32_t)g.t) : g.t);
     const int t0 = seg * g.slen, t1 = min(t0 + g.slen, len), T = max(t1 - t0, 0);
@@ -376,200 +372,196 @@ __global__ __launch_bounds__(256, DAT <= (MODE == WALK_RATE ? 1 : 2) ? 2 : 1) vo
     if (MODE != STATE && !q.acc) {  // padding rows
         const int z1 = (int)min((long long)t0 + g.slen, (long long)g.t);
         for (int i = max(t0, len) + (lane >> 5); i < z1; i += 2)
-            if (incol) q.y[(b * g.t + i) * q.ys + ho * q.dc + col] = 0.f;
+            if (incol) q.y[(b * g.t + i) * q.ys + hd * q.dc + col] = 0.f;
     }
     Powers &pw = tables[wave];
     float *bt = btile[MODE == STATE ? 0 : wave];
-    for (int r0 = 0; r0 < q.gy; r0++) {
-        const int hd = ho * q.gy + r0;
-        double dg = 0.0;
-        const long long st = (b * g.h + hd) * q.da * q.dc;
-        const long long sg = ((long long)seg * g.n * g.h) * q.da * q.dc + st;
-        // segments are rows' whatever the walk's direction, so that the heads that
-        // share a row of y meet in one wave
-        const bool down = (hd >= g.h - g.reverse) != (q.rev != 0);
-        const Walk w = {b * g.t + (down ? t1 - 1 : t0), down ? -1 : 1};
-        const bool ends = down ? seg == 0 : lastseg;    // holds the walk's last token
-        const bool begins = down ? lastseg : seg == 0;  // holds its first
-        if (MODE == STATE && (T == 0 || ends)) return;
-        const float *pa = q.a + (hd / q.ga) * q.da, *pb = q.b + (hd / q.gb) * q.da,
-                    *pc = q.c + (hd / q.gc) * q.dc;
-        f32x4 af[4 * DAT], bf[4 * DAT];
-        float cf[16], bcol[MODE == STATE ? DAT : 1][16];
-        {
-            const int L = min(C, T);
-            const ChunkRows rb(pb, q.bs, q.da, w, 0, L);
-            if constexpr (MODE != STATE) {
-                load_rows<DAT>(rb, ln, half, bf);
-                load_rows<DAT>(ChunkRows(pa, q.as, q.da, w, 0, L), ln, half, af);
-            } else {
+    double dg = 0.0;
+    const long long st = (b * g.h + hd) * q.da * q.dc;
+    const long long sg = ((long long)seg * g.n * g.h) * q.da * q.dc + st;
+    // segments are rows' whatever the walk's direction
+    const bool down = (hd >= g.h - g.reverse) != (q.rev != 0);
+    const Walk w = {b * g.t + (down ? t1 - 1 : t0), down ? -1 : 1};
+    const bool ends = down ? seg == 0 : lastseg;    // holds the walk's last token
+    const bool begins = down ? lastseg : seg == 0;  // holds its first
+    if (MODE == STATE && (T == 0 || ends)) return;
+    const float *pa = q.a + (hd / q.ga) * q.da, *pb = q.b + (hd / q.gb) * q.da,
+                *pc = q.c + (hd / q.gc) * q.dc;
+    f32x4 af[4 * DAT], bf[4 * DAT];
+    float cf[16], bcol[MODE == STATE ? DAT : 1][16];
+    {
+        const int L = min(C, T);
+        const ChunkRows rb(pb, q.bs, q.da, w, 0, L);
+        if constexpr (MODE != STATE) {
+            load_rows<DAT>(rb, ln, half, bf);
+            load_rows<DAT>(ChunkRows(pa, q.as, q.da, w, 0, L), ln, half, af);
+        } else {
 #pragma unroll
-                for (int d = 0; d < DAT; d++) load_cols(rb, half, 32 * d + ln, bcol[d]);
-            }
-            load_cols(ChunkRows(pc, q.cs, q.dc, w, 0, L), half, col, cf);
+            for (int d = 0; d < DAT; d++) load_cols(rb, half, 32 * d + ln, bcol[d]);
         }
-        // the state: rows 32 d + tile_row(r) + half, column col
-        const float *s0 = MODE == STATE ? nullptr : g.nseg > 1 ? q.seg + sg : begins && q.s0 ? q.s0 + st : nullptr;
-        f32x16 S[DAT], Z[MODE == WALK_RATE ? DAT : 1];
+        load_cols(ChunkRows(pc, q.cs, q.dc, w, 0, L), half, col, cf);
+    }
+    // the state: rows 32 d + tile_row(r) + half, column col
+    const float *s0 = MODE == STATE ? nullptr : g.nseg > 1 ? q.seg + sg : begins && q.s0 ? q.s0 + st : nullptr;
+    f32x16 S[DAT], Z[MODE == WALK_RATE ? DAT : 1];
+#pragma unroll
+    for (int d = 0; d < DAT; d++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            S[d][r] = 0.f;
+            if (MODE == WALK_RATE) Z[d][r] = 0.f;
+        }
+    if (s0) {
+        const StateRows x(s0, q, half, col);
 #pragma unroll
         for (int d = 0; d < DAT; d++)
 #pragma unroll
+            for (int r = 0; r < 16; r++) S[d][r] = x.load(d, r);
+    }
+    bool any = s0 != nullptr;  // whether the state may be other than 0
+    const double lg = log_gamma(g.rate[hd]);
+    wave_sync();
+    const Power pow(lg);
+    if (lane < C) {
+        pw.near[lane] = pow(lane);
+        pw.first[lane] = pow(lane + e0) * q.sa;
+    }
+    float hi = 0.f, lo = 0.f;  // gamma^L, in two parts
+    for (int c0 = 0; c0 < T; c0 += C) {
+        const int L = min(C, T - c0), next = min(C, max(T - c0 - C, 0));
+        if (c0 == 0 || L < C) {
+            const double all = exp(lg * L);
+            hi = (float)all;
+            lo = (float)(all - (double)hi);
+            wave_sync();
+            if (lane < C) pw.left[lane] = pow(max(L - lane - e0, 0)) * q.sb;
+            wave_sync();
+        }
+        // whether a reader of the state follows
+        const bool goes = MODE == STATE || c0 + L < T || slope || (ends && q.s1);
+        if constexpr (MODE != STATE) {
+            f32x16 P, o, oz;
+#pragma unroll
+            for (int r = 0; r < 16; r++) P[r] = o[r] = oz[r] = 0.f;
+            cut_rows<DAT, FULL>(q.da, half, af);
+            cut_rows<DAT, FULL>(q.da, half, bf);
+            wave_sync();
+#pragma unroll
+            for (int k = 0; k < 4 * DAT; k++) *(f32x4 *)(bt + ln * BS + 8 * k + half) = bf[k];
+#pragma unroll
+            for (int k = 0; k < 4 * DAT; k++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) P = mm32(bf[k][e], af[k][e], P);
+            __builtin_amdgcn_sched_barrier(0);
+            load_rows<DAT>(ChunkRows(pb, q.bs, q.da, w, c0 + C, next), ln, half, bf);
+            __builtin_amdgcn_sched_barrier(0);
+            const int query = opaque(ln - half);
+            const float sab = q.sa * q.sb;
+#pragma unroll
             for (int r = 0; r < 16; r++) {
-                S[d][r] = 0.f;
-                if (MODE == WALK_RATE) Z[d][r] = 0.f;
+                // keys behind the query: 0, also of what is no number
+                const int far = query - tile_row(r);
+                const float v = __uint_as_float(__float_as_uint(P[r]) & ~(uint32_t)(far >> 31));
+                P[r] = v * (pw.near[max(far, 0)] * sab);
             }
-        if (s0) {
-            const StateRows x(s0, q, half, col);
+            if (any) {
+                float row[16];
+                places(pw.first, half, row);
 #pragma unroll
-            for (int d = 0; d < DAT; d++)
+                for (int d = 0; d < DAT; d++)
 #pragma unroll
-                for (int r = 0; r < 16; r++) S[d][r] = x.load(d, r);
-        }
-        bool any = s0 != nullptr;  // whether the state may be other than 0
-        const double lg = log_gamma(g.rate[hd]);
-        wave_sync();
-        const Power pow(lg);
-        if (lane < C) {
-            pw.near[lane] = pow(lane);
-            pw.first[lane] = pow(lane + e0) * q.sa;
-        }
-        float hi = 0.f, lo = 0.f;  // gamma^L, in two parts
-        for (int c0 = 0; c0 < T; c0 += C) {
-            const int L = min(C, T - c0), next = min(C, max(T - c0 - C, 0));
-            if (c0 == 0 || L < C) {
-                const double all = exp(lg * L);
-                hi = (float)all;
-                lo = (float)(all - (double)hi);
-                wave_sync();
-                if (lane < C) pw.left[lane] = pow(max(L - lane - e0, 0)) * q.sb;
-                wave_sync();
-            }
-            // whether a reader of the state follows
-            const bool goes = MODE == STATE || c0 + L < T || slope || (ends && q.s1);
-            if constexpr (MODE != STATE) {
-                f32x16 P, o, oz;
-#pragma unroll
-                for (int r = 0; r < 16; r++) P[r] = o[r] = oz[r] = 0.f;
-                cut_rows<DAT, FULL>(q.da, half, af);
-                cut_rows<DAT, FULL>(q.da, half, bf);
-                wave_sync();
-#pragma unroll
-                for (int k = 0; k < 4 * DAT; k++) *(f32x4 *)(bt + ln * BS + 8 * k + half) = bf[k];
-#pragma unroll
-                for (int k = 0; k < 4 * DAT; k++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) P = mm32(bf[k][e], af[k][e], P);
-                __builtin_amdgcn_sched_barrier(0);
-                load_rows<DAT>(ChunkRows(pb, q.bs, q.da, w, c0 + C, next), ln, half, bf);
-                __builtin_amdgcn_sched_barrier(0);
-                const int query = opaque(ln - half);
-                const float sab = q.sa * q.sb;
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    // keys behind the query: 0, also of what is no number
-                    const int far = query - tile_row(r);
-                    const float v = __uint_as_float(__float_as_uint(P[r]) & ~(uint32_t)(far >> 31));
-                    P[r] = v * (pw.near[max(far, 0)] * sab);
-                }
-                if (any) {
-                    float row[16];
-                    places(pw.first, half, row);
+                    for (int r = 0; r < 16; r++) o = mm32(af[4 * d + (r >> 2)][r & 3], S[d][r], o);
+                if (slope) {
 #pragma unroll
                     for (int d = 0; d < DAT; d++)
 #pragma unroll
-                        for (int r = 0; r < 16; r++) o = mm32(af[4 * d + (r >> 2)][r & 3], S[d][r], o);
-                    if (slope) {
-#pragma unroll
-                        for (int d = 0; d < DAT; d++)
-#pragma unroll
-                            for (int r = 0; r < 16; r++) oz = mm32(af[4 * d + (r >> 2)][r & 3], Z[d][r], oz);
-                        const float one = (float)(half + 1);
-#pragma unroll
-                        for (int r = 0; r < 16; r++)
-                            oz[r] = row[r] * __builtin_fmaf(one + (float)tile_row(r), o[r], oz[r]);
-                    }
-#pragma unroll
-                    for (int r = 0; r < 16; r++) o[r] *= row[r];
-                }
-                __builtin_amdgcn_sched_barrier(0);
-                load_rows<DAT>(ChunkRows(pa, q.as, q.da, w, c0 + C, next), ln, half, af);
-                float dot[16];
-                if (slope) load_cols(ChunkRows(q.dot + hd * q.dc, q.ds, q.dc, w, c0, L), half, col, dot);
-                __builtin_amdgcn_sched_barrier(0);
-                o = tri_product(P, cf, o, half);
-                const ChunkRows ry(q.y + ho * q.dc, q.ys, q.dc, w, c0, L);
-                const uint32_t y_at = ry.at(half, col);
-                if (q.acc || r0 > 0) {
-#pragma unroll
-                    for (int r = 0; r < 16; r++) o[r] += ry.load(ry.go(y_at, tile_row(r)));
-                }
-#pragma unroll
-                for (int r = 0; r < 16; r++) ry.store(ry.go(y_at, tile_row(r)), o[r]);
-                if (slope) {
-                    const float fq = (float)query;
-#pragma unroll
-                    for (int r = 0; r < 16; r++) P[r] *= fq - (float)tile_row(r);
-                    oz = tri_product(P, cf, oz, half);
-                    float sum = 0.f;
-#pragma unroll
-                    for (int r = 0; r < 16; r++) sum = __builtin_fmaf(oz[r], dot[r], sum);
-                    dg += (double)sum;
-                }
-            }
-            if (goes) {
-                float left[16];
-                places(pw.left, half, left);
-#pragma unroll
-                for (int r = 0; r < 16; r++) cf[r] *= left[r];
-#pragma unroll
-                for (int d = 0; d < DAT; d++) {
-                    float bd[16];
+                        for (int r = 0; r < 16; r++) oz = mm32(af[4 * d + (r >> 2)][r & 3], Z[d][r], oz);
+                    const float one = (float)(half + 1);
 #pragma unroll
                     for (int r = 0; r < 16; r++)
-                        bd[r] = MODE == STATE ? bcol[MODE == STATE ? d : 0][r]
-                                              : bt[(tile_row(r) + half) * BS + 32 * d + ln];
-                    if (slope) {
-                        const float fl = (float)(L - 1 - half);
-#pragma unroll
-                        for (int r = 0; r < 16; r++)
-                            Z[d][r] = decayed(__builtin_fmaf((float)L, S[d][r], Z[d][r]), hi, lo);
-#pragma unroll
-                        for (int r = 0; r < 16; r++)
-                            Z[d] = mm32(bd[r], cf[r] * (fl - (float)tile_row(r)), Z[d]);
-                    }
-#pragma unroll
-                    for (int r = 0; r < 16; r++) S[d][r] = decayed(S[d][r], hi, lo);
-#pragma unroll
-                    for (int r = 0; r < 16; r++) S[d] = mm32(bd[r], cf[r], S[d]);
-                    if constexpr (MODE == STATE)
-                        load_cols(ChunkRows(pb, q.bs, q.da, w, c0 + C, next), half, 32 * d + ln, bcol[d]);
+                        oz[r] = row[r] * __builtin_fmaf(one + (float)tile_row(r), o[r], oz[r]);
                 }
-                any = true;
+#pragma unroll
+                for (int r = 0; r < 16; r++) o[r] *= row[r];
             }
             __builtin_amdgcn_sched_barrier(0);
-            load_cols(ChunkRows(pc, q.cs, q.dc, w, c0 + C, next), half, col, cf);
+            load_rows<DAT>(ChunkRows(pa, q.as, q.da, w, c0 + C, next), ln, half, af);
+            float dot[16];
+            if (slope) load_cols(ChunkRows(q.dot + hd * q.dc, q.ds, q.dc, w, c0, L), half, col, dot);
             __builtin_amdgcn_sched_barrier(0);
-        }
-        const float *sgrad = !slope || !T ? nullptr : g.nseg > 1 ? q.segg + sg : q.s1g ? q.s1g + st : nullptr;
-        float *s1 = MODE == STATE ? q.seg + sg : ends && q.s1 ? q.s1 + st : nullptr;
-        if (s1) {
-            const StateRows x(s1, q, half, col);
+            o = tri_product(P, cf, o, half);
+            const ChunkRows ry(q.y + hd * q.dc, q.ys, q.dc, w, c0, L);
+            const uint32_t y_at = ry.at(half, col);
+            if (q.acc) {
 #pragma unroll
-            for (int d = 0; d < DAT; d++)
+                for (int r = 0; r < 16; r++) o[r] += ry.load(ry.go(y_at, tile_row(r)));
+            }
 #pragma unroll
-                for (int r = 0; r < 16; r++) x.store(d, r, S[d][r]);
-        }
-        if (MODE == WALK_RATE && sgrad) {
-            const StateRows x(sgrad, q, half, col);
+            for (int r = 0; r < 16; r++) ry.store(ry.go(y_at, tile_row(r)), o[r]);
+            if (slope) {
+                const float fq = (float)query;
 #pragma unroll
-            for (int d = 0; d < DAT; d++)
+                for (int r = 0; r < 16; r++) P[r] *= fq - (float)tile_row(r);
+                oz = tri_product(P, cf, oz, half);
+                float sum = 0.f;
 #pragma unroll
-                for (int r = 0; r < 16; r++) dg += (double)Z[d][r] * x.load(d, r);
+                for (int r = 0; r < 16; r++) sum = __builtin_fmaf(oz[r], dot[r], sum);
+                dg += (double)sum;
+            }
         }
-        if (slope) {
-            dg = rnn_wave_sum_d(dg);
-            if (lane == 0) g.part[((b * g.nseg + seg) * q.slices.d + slice) * g.h + hd] = dg;
+        if (goes) {
+            float left[16];
+            places(pw.left, half, left);
+#pragma unroll
+            for (int r = 0; r < 16; r++) cf[r] *= left[r];
+#pragma unroll
+            for (int d = 0; d < DAT; d++) {
+                float bd[16];
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    bd[r] = MODE == STATE ? bcol[MODE == STATE ? d : 0][r]
+                                          : bt[(tile_row(r) + half) * BS + 32 * d + ln];
+                if (slope) {
+                    const float fl = (float)(L - 1 - half);
+#pragma unroll
+                    for (int r = 0; r < 16; r++)
+                        Z[d][r] = decayed(__builtin_fmaf((float)L, S[d][r], Z[d][r]), hi, lo);
+#pragma unroll
+                    for (int r = 0; r < 16; r++)
+                        Z[d] = mm32(bd[r], cf[r] * (fl - (float)tile_row(r)), Z[d]);
+                }
+#pragma unroll
+                for (int r = 0; r < 16; r++) S[d][r] = decayed(S[d][r], hi, lo);
+#pragma unroll
+                for (int r = 0; r < 16; r++) S[d] = mm32(bd[r], cf[r], S[d]);
+                if constexpr (MODE == STATE)
+                    load_cols(ChunkRows(pb, q.bs, q.da, w, c0 + C, next), half, 32 * d + ln, bcol[d]);
+            }
+            any = true;
         }
+        __builtin_amdgcn_sched_barrier(0);
+        load_cols(ChunkRows(pc, q.cs, q.dc, w, c0 + C, next), half, col, cf);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    const float *sgrad = !slope || !T ? nullptr : g.nseg > 1 ? q.segg + sg : q.s1g ? q.s1g + st : nullptr;
+    float *s1 = MODE == STATE ? q.seg + sg : ends && q.s1 ? q.s1 + st : nullptr;
+    if (s1) {
+        const StateRows x(s1, q, half, col);
+#pragma unroll
+        for (int d = 0; d < DAT; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) x.store(d, r, S[d][r]);
+    }
+    if (MODE == WALK_RATE && sgrad) {
+        const StateRows x(sgrad, q, half, col);
+#pragma unroll
+        for (int d = 0; d < DAT; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) dg += (double)Z[d][r] * x.load(d, r);
+    }
+    if (slope) {
+        dg = rnn_wave_sum_d(dg);
+        if (lane == 0) g.part[((b * g.nseg + seg) * q.slices.d + slice) * g.h + hd] = dg;
     }
 }
 
@@ -611,6 +603,31 @@ __global__ __launch_bounds__(256) void decay_scan_kernel(DecayArgs g) {
     }
 }
 
+// dk and dv of shared heads: the sum over the query heads' parts, in order.  Rows
+// behind a sequence's end hold zeros, and stay as they are where dkv accumulates.
+struct GroupArgs {
+    const float *part[2];
+    float *out[2];
+    int d[2];
+    const uint32_t *lens;
+    long long stride;
+    int t, hkv, grp, acc;
+};
+__global__ __launch_bounds__(256) void decay_group_kernel(GroupArgs g, long long rows) {
+    const int k = blockIdx.y, d = g.d[k], w = g.hkv * d;
+    const long long all = rows * w;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long long)gridDim.x * 256) {
+        const long long row = i / w;
+        const int at = (int)(i - row * w), hd = at / d;
+        if (g.acc && g.lens && row % g.t >= (long long)g.lens[row / g.t]) continue;
+        const float *p = g.part[k] + row * w * g.grp + (long long)hd * g.grp * d + (at - hd * d);
+        float s = p[0];
+        for (int r = 1; r < g.grp; r++) s += p[(long long)r * d];
+        float *o = g.out[k] + row * g.stride + at;
+        *o = g.acc ? *o + s : s;
+    }
+}
+
 // drate[j] += g sum of the head's parts, in a fixed order.
 __global__ __launch_bounds__(256) void decay_rate_kernel(const double *part, int rows, int h,
                                                          const float *rate, float *drate) {
@@ -629,7 +646,7 @@ __global__ __launch_bounds__(256) void decay_rate_kernel(const double *part, int
 struct DecayPlan {
     bool tokens = false;  // token by token
     int nseg = 1, slen = 1;
-    size_t seg = 0, segr = 0, part = 0, bytes = 0;
+    size_t seg = 0, segr = 0, part = 0, part_k = 0, part_v = 0, bytes = 0;
 };
 DecayPlan plan_of(const rnn_decay_attn_desc *d, size_t n, size_t t, bool backward) {
     DecayPlan p;
@@ -638,10 +655,15 @@ DecayPlan plan_of(const rnn_decay_attn_desc *d, size_t n, size_t t, bool backwar
     p.tokens = !backward && t <= 8;
     const size_t kt = rnn_div_up(d->dk, 32), vt = rnn_div_up(d->dv, 32);
     // the waves of the walk with the fewest
-    const size_t waves = backward ? std::min(n * d->h * kt, n * d->hkv * (kt + vt)) : n * d->h * vt;
+    const size_t waves = backward ? n * d->h * kt : n * d->h * vt;
     p.slen = (int)rnn_round_up(std::max<size_t>(t, 1), C);
-    if (!p.tokens && waves && waves < 1024 && t > 4 * C) {
-        const size_t want = std::min(rnn_div_up(SEG_WAVES, waves), t / SEG_TOKENS);
+    // Segments where that leaves compute units idle, a chunk at the least: up to two
+    // waves a SIMD of a forward, one of a backward, whose walk for dq and the rates
+    // holds half of a SIMD's registers.  (Us a pass, 1024 / 2048 waves: a prompt of
+    // 16384 tokens 137 / 130, training on 8 x 1568 tokens 240 / 290; at least 32 / 64
+    // / 128 tokens a segment: training on 5 x 577 with shared heads 198 / 257 / 378.)
+    if (!p.tokens && waves && waves < 1024 && t >= 2 * C) {
+        const size_t want = std::min(rnn_div_up(backward ? 1024 : 2048, waves), t / C);
         p.slen = (int)rnn_round_up(rnn_div_up(t, std::max<size_t>(want, 1)), C);
         p.nseg = (int)rnn_div_up(t, p.slen);
     }
@@ -651,6 +673,10 @@ DecayPlan plan_of(const rnn_decay_attn_desc *d, size_t n, size_t t, bool backwar
         if (backward) p.segr = c.take(states);
     }
     if (backward) p.part = c.take(n * p.nseg * rnn_div_up(d->dk, 32) * d->h * sizeof(double));
+    if (backward && d->h != d->hkv) {
+        p.part_k = c.take(n * t * d->h * d->dk * sizeof(float));
+        p.part_v = c.take(n * t * d->h * d->dv * sizeof(float));
+    }
     p.bytes = c.off;
     return p;
 }
@@ -670,7 +696,7 @@ int decay_check(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n, size_t t) 
                         d->dk, d->dv, MAX_D);
     const uint64_t qw = (uint64_t)d->h * d->dk, kw = (uint64_t)d->hkv * d->dk,
                    vw = (uint64_t)d->hkv * d->dv;
-    if (d->qstride > (1u << 22) || d->kvstride > (1u << 22) || (uint64_t)d->h * d->dv > (1u << 22))
+    if (d->qstride > (1u << 22) || d->kvstride > (1u << 22) || (uint64_t)d->h * std::max(d->dk, d->dv) > (1u << 22))
         return rnn_fail(ctx, RNN_E_UNSUPPORTED, "decay_attn: row stride above 2^22");
     if (d->qoff > d->qstride || d->qstride - d->qoff < qw || d->koff > d->kvstride ||
         d->kvstride - d->koff < kw || d->voff > d->kvstride || d->kvstride - d->voff < vw)
@@ -701,18 +727,17 @@ struct Operand {
     int share;
 };
 
-DecayJob make_job(uint32_t h, const Operand &a, const Operand &b, int da, const Operand &c, int dc,
-                  float *y, size_t ys, int gy) {
+DecayJob make_job(const Operand &a, const Operand &b, int da, const Operand &c, int dc,
+                  float *y, size_t ys) {
     DecayJob j{};
     j.a = a.p, j.b = b.p, j.c = c.p, j.y = y;
     j.as = (long long)a.stride, j.bs = (long long)b.stride, j.cs = (long long)c.stride;
     j.ys = (long long)ys;
     j.da = da, j.dc = dc;
-    j.ga = a.share, j.gb = b.share, j.gc = c.share, j.gy = gy;
+    j.ga = a.share, j.gb = b.share, j.gc = c.share;
     j.si = dc, j.sj = 1;
     j.sa = j.sb = 1.f;
     j.slices = Divider((uint32_t)(dc + 31) / 32);
-    j.heads = Divider((uint32_t)(h / gy));
     return j;
 }
 
@@ -721,6 +746,7 @@ void fill_args(DecayArgs &g, const rnn_decay_attn_desc *d, const DecayPlan &p, s
     g.nseg = p.nseg;
     g.slen = p.slen;
     g.segs = Divider((uint32_t)p.nseg);
+    g.heads = Divider(d->h);
     g.rate = rate;
     g.lens = lens;
     g.part = nullptr;
@@ -736,7 +762,7 @@ void launch_walk(rnn_ctx *ctx, const DecayArgs &g, int jobs) {
     bool full = true;
     for (int k = 0; k < jobs; k++) {
         const DecayJob &q = g.job[k];
-        waves = std::max(waves, (size_t)g.n * q.heads.d * g.nseg * q.slices.d);
+        waves = std::max(waves, (size_t)g.n * g.h * g.nseg * q.slices.d);
         full = full && q.da % 32 == 0;
     }
     const dim3 grid((unsigned)rnn_div_up(waves, 4), (unsigned)jobs);
@@ -793,7 +819,7 @@ int rnn_decay_attn_forward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n,
     const Operand Q = {q + d->qoff, d->qstride, 1}, K = {kv + d->koff, d->kvstride, grp},
                   V = {kv + d->voff, d->kvstride, grp};
     DecayJob &j = g.job[0];
-    j = make_job(d->h, Q, K, (int)d->dk, V, (int)d->dv, y, (size_t)d->h * d->dv, 1);
+    j = make_job(Q, K, (int)d->dk, V, (int)d->dv, y, (size_t)d->h * d->dv);
     j.s0 = state_in;
     j.s1 = state_out;
     j.sa = d->scale;
@@ -850,7 +876,7 @@ int rnn_decay_attn_backward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n
                   V = {kv + d->voff, d->kvstride, grp}, O = {dy, (size_t)d->h * d->dv, 1};
     g.part = (double *)((char *)ws + w.part);
     DecayJob &jq = g.job[0], &jk = g.job[1], &jv = g.job[2];
-    jq = make_job(d->h, O, V, dv, K, dk, dq + d->qoff, d->qstride, 1);
+    jq = make_job(O, V, dv, K, dk, dq + d->qoff, d->qstride);
     jq.si = 1, jq.sj = dv;
     jq.s0 = state_in;
     jq.sa = d->scale;
@@ -860,23 +886,25 @@ int rnn_decay_attn_backward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n
         jq.ds = (long long)d->qstride;
         jq.s1g = dstate_out;
     }
-    jk = make_job(d->h, V, O, dv, Q, dk, dkv + d->koff, d->kvstride, grp);
+    // keys and values that query heads share: each head's part, then their sum
+    const bool share = grp > 1;
+    float *part_k = (float *)((char *)ws + w.part_k), *part_v = (float *)((char *)ws + w.part_v);
+    jk = make_job(V, O, dv, Q, dk, share ? part_k : dkv + d->koff, share ? (size_t)d->h * dk : d->kvstride);
     jk.si = 1, jk.sj = dv;
-    jv = make_job(d->h, K, Q, dk, O, dv, dkv + d->voff, d->kvstride, grp);
+    jv = make_job(K, Q, dk, O, dv, share ? part_v : dkv + d->voff, share ? (size_t)d->h * dv : d->kvstride);
     jk.s0 = jv.s0 = dstate_out;
     jk.sb = jv.sb = d->scale;
     jk.rev = jv.rev = 1;
-    jk.acc = jv.acc = !(flags & RNN_ATTN_SET_DKV);
+    const int acc = !(flags & RNN_ATTN_SET_DKV);
+    jk.acc = jv.acc = share ? 0 : acc;
     jv.s1 = dstate_in;
     if (w.nseg > 1) {
         // S from the keys and values, R from the queries and dy
         DecayArgs sg = g;
-        sg.job[0] = make_job(d->h, Q, K, dk, V, dv, nullptr, 0, 1);
+        sg.job[0] = make_job(Q, K, dk, V, dv, nullptr, 0);
         sg.job[0].s0 = state_in;
         sg.job[0].seg = (float *)((char *)ws + w.seg);
         sg.job[1] = jv;
-        sg.job[1].gy = 1;
-        sg.job[1].heads = Divider(d->h);
         sg.job[1].seg = (float *)((char *)ws + w.segr);
         launch_segments(ctx, sg, 2);
         RNN_LAUNCHED(ctx);
@@ -899,6 +927,14 @@ int rnn_decay_attn_backward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n
     if (!joint) {
         one.job[0] = jv;
         launch_walk<WALK>(ctx, one, 1);
+        RNN_LAUNCHED(ctx);
+    }
+    if (share && t) {
+        GroupArgs ga = {{part_k, part_v}, {dkv + d->koff, dkv + d->voff}, {dk, dv}, lens,
+                        (long long)d->kvstride, (int)t, (int)d->hkv, grp, acc};
+        const size_t each = n * t * d->hkv * (size_t)std::max(dk, dv);
+        decay_group_kernel<<<dim3((unsigned)std::min<size_t>(rnn_div_up(each, 256), 4096), 2), 256, 0,
+                             ctx->stream>>>(ga, (long long)(n * t));
         RNN_LAUNCHED(ctx);
     }
     if (drate) {
