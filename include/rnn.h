@@ -309,9 +309,9 @@ int rnn_head_gate_backward(rnn_ctx *ctx, size_t rows, size_t h, size_t d, float 
 /* ----------------------------------------------- linear attention with decay */
 /* Linear attention with a decay for each head (no counterpart in the reference).
  * Head j reads queries of dk channels at q + r*qstride + qoff + j*dk; key head
- * g = j / (h / hkv) has keys at kv + r*kvstride + koff + g*dk and values of dv
- * channels at kv + r*kvstride + voff + g*dv.  With gamma_j = exp(-exp(rate[j])),
- * over the tokens i of a sequence in order,
+ * g = j / (h / hkv) has keys at k + r*kstride + koff + g*dk and values of dv
+ * channels at v + r*vstride + voff + g*dv; q, k and v may be one buffer.  With
+ * gamma_j = exp(-exp(rate[j])), over the tokens i of a sequence in order,
  *   S_i = gamma S_(i-1) + k_i^T v_i,   y_i = scale q_i S_i
  * which is y_i = scale sum_(l <= i) gamma^(i-l) (q_i . k_l) v_l.  The last
  * `reverse` heads take the tokens from the last to the first.
@@ -320,11 +320,12 @@ int rnn_head_gate_backward(rnn_ctx *ctx, size_t rows, size_t h, size_t d, float 
  * state_in [n][h][dk][dv] is S before the first token (NULL: 0), state_out S
  * after the last (NULL: not wanted; may be state_in): a sequence may be given in
  * pieces, or token by token.  gamma is within [0, 1] for any rate; -infinity: 1, no
- * decay.  Products are fp32 and so are states; powers of gamma are formed in 64
- * bits.  A NaN or an infinity shows in the tokens that see it and in no others. */
+ * decay.  Products, sums and states are fp32; powers of gamma are formed with their
+ * exponent in 48 bits or more, so that long memories keep theirs.  A NaN or an
+ * infinity shows, as NaN or infinity, in the tokens that see it and in no others. */
 typedef struct {
     uint32_t h, hkv, dk, dv;
-    size_t qstride, qoff, kvstride, koff, voff;
+    size_t qstride, qoff, kstride, koff, vstride, voff;
     uint32_t reverse;
     float scale;
 } rnn_decay_attn_desc;
@@ -332,27 +333,27 @@ typedef struct {
  * (backward = 0) or the backward needs for n sequences of t tokens; host only.
  * The workspace is the caller's, 256-byte aligned, holds nothing between calls
  * and is not shared by calls that may run at the same time.  dk and dv <= 128, row
- * strides <= 2^22 (y's too), n * t * h and n * h * dk * dv < 2^31 (RNN_E_UNSUPPORTED above),
- * scale finite. */
+ * strides, y's among them, <= 2^22, n * t * h and n * h * dk * dv < 2^31
+ * (RNN_E_UNSUPPORTED above), scale finite. */
 int rnn_decay_attn_workspace(const rnn_decay_attn_desc *d, size_t n, size_t t, int backward,
                              size_t *bytes);
 /* y [n][t][h][dv]. */
 int rnn_decay_attn_forward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n, size_t t,
-                           const float *q, const float *kv, const float *rate, const uint32_t *lens,
-                           const float *state_in, void *ws, size_t ws_bytes, float *y,
-                           float *state_out);
+                           const float *q, const float *k, const float *v, const float *rate,
+                           const uint32_t *lens, const float *state_in, void *ws, size_t ws_bytes,
+                           float *y, float *state_out);
 /* From the forward's inputs, dy [n][t][h][dv] and, where state_out was used, its
- * gradient dstate_out (NULL: 0): dq and dkv, laid out as q and kv, ACCUMULATE or are
- * overwritten as flags say (RNN_ATTN_SET_DQ, RNN_ATTN_SET_DKV: the columns of
- * queries, or of keys and values, padding rows included, which receive 0); drate
- * [h] (NULL: not wanted) accumulates; dstate_in (NULL: not wanted) is overwritten.
- * dq and dkv may be one buffer with disjoint columns; neither they nor dstate_in
- * overlap another operand.  Sums run in a fixed order. */
+ * gradient dstate_out (NULL: 0): dq, dk and dv, laid out as q, k and v, ACCUMULATE or
+ * are overwritten as flags say (RNN_ATTN_SET_DQ, RNN_ATTN_SET_DKV: the columns of the
+ * heads, padding rows included, which receive 0); drate [h] (NULL: not wanted)
+ * accumulates; dstate_in (NULL: not wanted) is overwritten.  dq, dk and dv may be one
+ * buffer with disjoint columns; neither they nor dstate_in overlap another operand.
+ * Sums run in a fixed order. */
 int rnn_decay_attn_backward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n, size_t t,
-                            const float *q, const float *kv, const float *rate, const uint32_t *lens,
-                            const float *state_in, const float *dy, const float *dstate_out, void *ws,
-                            size_t ws_bytes, float *dq, float *dkv, float *drate, float *dstate_in,
-                            uint32_t flags);
+                            const float *q, const float *k, const float *v, const float *rate,
+                            const uint32_t *lens, const float *state_in, const float *dy,
+                            const float *dstate_out, void *ws, size_t ws_bytes, float *dq, float *dk,
+                            float *dv, float *drate, float *dstate_in, uint32_t flags);
 
 /* -------------------------------------------------- differential attention */
 /* Differential attention (no counterpart in the reference): the difference of

@@ -80,8 +80,9 @@ pub struct rnn_decay_attn_desc {
     pub dv: u32,
     pub qstride: usize,
     pub qoff: usize,
-    pub kvstride: usize,
+    pub kstride: usize,
     pub koff: usize,
+    pub vstride: usize,
     pub voff: usize,
     pub reverse: u32,
     pub scale: f32,
@@ -194,8 +195,8 @@ extern "C" {
     pub fn rnn_head_gate_workspace(rows: usize, h: usize, d: usize, bytes: *mut usize) -> c_int;
     pub fn rnn_head_gate_backward(ctx: *mut rnn_ctx, rows: usize, h: usize, d: usize, eps: f32, x: *const f32, z: *const f32, zstride: usize, zoff: usize, gain: *const f32, dy: *const f32, ws: *mut c_void, ws_bytes: usize, dx: *mut f32, dz: *mut f32, dzstride: usize, dzoff: usize, dgain: *mut f32) -> c_int;
     pub fn rnn_decay_attn_workspace(d: *const rnn_decay_attn_desc, n: usize, t: usize, backward: c_int, bytes: *mut usize) -> c_int;
-    pub fn rnn_decay_attn_forward(ctx: *mut rnn_ctx, d: *const rnn_decay_attn_desc, n: usize, t: usize, q: *const f32, kv: *const f32, rate: *const f32, lens: *const u32, state_in: *const f32, ws: *mut c_void, ws_bytes: usize, y: *mut f32, state_out: *mut f32) -> c_int;
-    pub fn rnn_decay_attn_backward(ctx: *mut rnn_ctx, d: *const rnn_decay_attn_desc, n: usize, t: usize, q: *const f32, kv: *const f32, rate: *const f32, lens: *const u32, state_in: *const f32, dy: *const f32, dstate_out: *const f32, ws: *mut c_void, ws_bytes: usize, dq: *mut f32, dkv: *mut f32, drate: *mut f32, dstate_in: *mut f32, flags: u32) -> c_int;
+    pub fn rnn_decay_attn_forward(ctx: *mut rnn_ctx, d: *const rnn_decay_attn_desc, n: usize, t: usize, q: *const f32, k: *const f32, v: *const f32, rate: *const f32, lens: *const u32, state_in: *const f32, ws: *mut c_void, ws_bytes: usize, y: *mut f32, state_out: *mut f32) -> c_int;
+    pub fn rnn_decay_attn_backward(ctx: *mut rnn_ctx, d: *const rnn_decay_attn_desc, n: usize, t: usize, q: *const f32, k: *const f32, v: *const f32, rate: *const f32, lens: *const u32, state_in: *const f32, dy: *const f32, dstate_out: *const f32, ws: *mut c_void, ws_bytes: usize, dq: *mut f32, dk: *mut f32, dv: *mut f32, drate: *mut f32, dstate_in: *mut f32, flags: u32) -> c_int;
     pub fn rnn_diff_attn_workspace(d: *const rnn_diff_attn_desc, n: usize, backward: c_int, bytes: *mut usize) -> c_int;
     pub fn rnn_diff_attn_forward(ctx: *mut rnn_ctx, d: *const rnn_diff_attn_desc, n: usize, q: *const f32, kv: *const f32, lam: *const f32, gain: *const f32, qlen: *const u32, klen: *const u32, ws: *mut c_void, ws_bytes: usize, y: *mut f32, o12: *mut f32, stats: *mut f32) -> c_int;
     pub fn rnn_diff_attn_backward(ctx: *mut rnn_ctx, d: *const rnn_diff_attn_desc, n: usize, q: *const f32, kv: *const f32, lam: *const f32, gain: *const f32, qlen: *const u32, klen: *const u32, o12: *const f32, stats: *const f32, dy: *const f32, ws: *mut c_void, ws_bytes: usize, dq: *mut f32, dkv: *mut f32, dlam: *mut f32, dgain: *mut f32, flags: u32) -> c_int;

@@ -105,7 +105,7 @@ class RotaryDesc(C.Structure):
 class DecayAttnDesc(C.Structure):
     """rnn_decay_attn_desc."""
     _fields_ = [(k, _u32) for k in ("h", "hkv", "dk", "dv")] + [
-        (k, _sz) for k in ("qstride", "qoff", "kvstride", "koff", "voff")] + [
+        (k, _sz) for k in ("qstride", "qoff", "kstride", "koff", "vstride", "voff")] + [
         ("reverse", _u32), ("scale", C.c_float)]
 
 
@@ -180,10 +180,10 @@ def lib():
             "rnn_head_gate_backward": (_i, [_vp, _sz, _sz, _sz, C.c_float, _vp, _vp, _sz, _sz, _vp,
                                             _vp, _vp, _sz, _vp, _vp, _sz, _sz, _vp]),
             "rnn_decay_attn_workspace": (_i, [P(DecayAttnDesc), _sz, _sz, _i, P(_sz)]),
-            "rnn_decay_attn_forward": (_i, [_vp, P(DecayAttnDesc), _sz, _sz] + [_vp] * 6 +
+            "rnn_decay_attn_forward": (_i, [_vp, P(DecayAttnDesc), _sz, _sz] + [_vp] * 7 +
                                        [_sz, _vp, _vp]),
-            "rnn_decay_attn_backward": (_i, [_vp, P(DecayAttnDesc), _sz, _sz] + [_vp] * 8 +
-                                        [_sz, _vp, _vp, _vp, _vp, _u32]),
+            "rnn_decay_attn_backward": (_i, [_vp, P(DecayAttnDesc), _sz, _sz] + [_vp] * 9 +
+                                        [_sz] + [_vp] * 5 + [_u32]),
             "rnn_diff_attn_workspace": (_i, [P(DiffAttnDesc), _sz, _i, P(_sz)]),
             "rnn_diff_attn_forward": (_i, [_vp, P(DiffAttnDesc), _sz] + [_vp] * 7 +
                                       [_sz, _vp, _vp, _vp]),
@@ -1070,7 +1070,8 @@ class DecayCore:
     dv channels; the last ``reverse`` heads take a sequence's tokens from the
     last to the first.  forward / backward take q and kv as Core's: a buffer
     with its row stride and the first channel of the queries, and of the keys
-    and values.  scale: default 1 / sqrt(dk)."""
+    and values; v and vstride where the values are in a buffer of their own.
+    scale: default 1 / sqrt(dk)."""
 
     def __init__(self, h, dk, dv=None, hkv=None, reverse=0, scale=None, ctx=None):
         self.h, self.dk = int(h), int(dk)
@@ -1081,85 +1082,98 @@ class DecayCore:
             raise ValueError("DecayCore: a negative size")
         self.scale = 1.0 / math.sqrt(max(self.dk, 1)) if scale is None else float(scale)
         self.ctx = ctx
-        self.c = self.h * self.dv
+        self.c, self.kw, self.vw = self.h * self.dv, self.hkv * self.dk, self.hkv * self.dv
         self._plans = {}  # the C description and workspace of each layout and size
-        kw = self.hkv * self.dk
-        self._plan(1, 1, 0, (self.h * self.dk, 0, kw + self.hkv * self.dv, 0, kw))
+        self._plan(1, 1, 0, (self.h * self.dk, 0, self.kw + self.vw, 0, None, self.kw))
 
-    def desc(self, qstride, qoff, kvstride, koff, voff):
-        return DecayAttnDesc(self.h, self.hkv, self.dk, self.dv, qstride, qoff, kvstride, koff, voff,
-                             self.reverse, self.scale)
+    def desc(self, qstride, qoff, kstride, koff, vstride, voff):
+        return DecayAttnDesc(self.h, self.hkv, self.dk, self.dv, qstride, qoff, kstride, koff,
+                             vstride, voff, self.reverse, self.scale)
 
     def _plan(self, n, t, backward, layout):
-        """(description, workspace bytes, floats of q and of kv that it spans)."""
+        """(description, workspace bytes, floats of q, of kv and of v that it
+        spans).  layout's vstride None: the values are in kv."""
         p = self._plans.get((n, t, backward, layout))
         if p is not None:
             return p
-        d, nb = self.desc(*layout), _sz()
+        qstride, qoff, kstride, koff, vstride, voff = layout
+        joint = vstride is None
+        d, nb = self.desc(qstride, qoff, kstride, koff, kstride if joint else vstride, voff), _sz()
         rc = lib().rnn_decay_attn_workspace(C.byref(d), n, t, backward, C.byref(nb))
+        what = lib().rnn_status_string(rc).decode()
+        if not rc and joint and koff < voff + self.vw and voff < koff + self.kw:
+            rc, what = RNN_E_INVALID, "keys and values overlap"
         if rc:
-            raise ValueError(f"DecayCore: {lib().rnn_status_string(rc).decode()} (h={self.h} "
-                             f"hkv={self.hkv} dk={self.dk} dv={self.dv} reverse={self.reverse} "
-                             f"scale={self.scale} n={n} t={t} layout={layout})")
+            raise ValueError(f"DecayCore: {what} (h={self.h} hkv={self.hkv} dk={self.dk} "
+                             f"dv={self.dv} reverse={self.reverse} scale={self.scale} n={n} t={t} "
+                             f"layout={layout})")
         rows = n * t
-        nq = (rows - 1) * d.qstride + d.qoff + self.h * self.dk if rows else 0
-        nkv = ((rows - 1) * d.kvstride + max(d.koff + self.hkv * self.dk,
-                                             d.voff + self.hkv * self.dv) if rows else 0)
-        p = self._plans[n, t, backward, layout] = d, nb.value, nq, nkv
+        need = lambda stride, end: (rows - 1) * stride + end if rows else 0
+        nq, nk = need(qstride, qoff + self.h * self.dk), need(kstride, koff + self.kw)
+        nv = need(d.vstride, voff + self.vw)
+        if len(self._plans) >= 4096:  # lengths come and go
+            self._plans.clear()
+        p = self._plans[n, t, backward, layout] = (d, nb.value, nq, max(nk, nv) if joint else nk, nv)
         return p
 
-    def _inputs(self, ctx, n, nq, nkv, q, kv, rate, lens, state):
-        return (_arg(ctx, q, nq, "q"), _arg(ctx, kv, nkv, "kv"), _arg(ctx, rate, self.h, "rate"),
-                _arg(ctx, lens, n, "lens", "u32"),
-                _arg(ctx, state, n * self.h * self.dk * self.dv, "state"))
-
     def forward(self, n, t, q, qstride, qoff, kv, kvstride, koff, voff, rate, lens=None, state=None,
-                keep_state=False, state_out=None, y=None):
+                keep_state=False, state_out=None, y=None, v=None, vstride=None):
         """(y [n, t, h dv], the state after the last token [n, h, dk, dv]: None
         unless keep_state or state_out, which may be state).  lens (int32 /
         uint32 [n]): the sequences' lengths where they are padded."""
         import torch
         ctx = self.ctx or default_ctx(q.device.index or 0)
-        d, nb, nq, nkv = self._plan(n, t, 0, (qstride, qoff, kvstride, koff, voff))
-        ins = self._inputs(ctx, n, nq, nkv, q, kv, rate, lens, state)
+        d, nb, nq, nk, nv = self._plan(n, t, 0, (qstride, qoff, kvstride, koff,
+                                                 None if v is None else vstride, voff))
+        st = n * self.h * self.dk * self.dv
+        kp = _arg(ctx, kv, nk, "kv")
+        ins = (_arg(ctx, q, nq, "q"), kp, kp if v is None else _arg(ctx, v, nv, "v"),
+               _arg(ctx, rate, self.h, "rate"), _arg(ctx, lens, n, "lens", "u32"),
+               _arg(ctx, state, st, "state"))
         if y is None:
             y = torch.empty(n, t, self.c, dtype=torch.float32, device=q.device)
         if state_out is None and keep_state:
             state_out = torch.empty(n, self.h, self.dk, self.dv, dtype=torch.float32,
                                     device=q.device)
         ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None
-        outs = (_arg(ctx, y, n * t * self.c, "y"),
-                _arg(ctx, state_out, n * self.h * self.dk * self.dv, "state_out"))
+        outs = _arg(ctx, y, n * t * self.c, "y"), _arg(ctx, state_out, st, "state_out")
         on = _OnStream(ctx)
         try:
             ctx.check(lib().rnn_decay_attn_forward(
                 ctx.h, C.byref(d), n, t, *ins, ws.data_ptr() if nb else None, nb, *outs))
         finally:
-            on.done(q, kv, rate, lens, state, ws, y, state_out)
+            on.done(q, kv, v, rate, lens, state, ws, y, state_out)
         return y, state_out
 
     def backward(self, n, t, q, qstride, qoff, kv, kvstride, koff, voff, rate, dy, dq, dkv,
                  drate=None, lens=None, state=None, dstate_out=None, dstate=None, set_dq=False,
-                 set_dkv=False):
-        """Accumulates into dq, dkv (laid out as q, kv) and drate; set_dq /
-        set_dkv overwrite dq / dkv instead.  dstate_out: the gradient of the
-        state that forward returned; dstate receives the given state's."""
+                 set_dkv=False, v=None, vstride=None, dv=None):
+        """Accumulates into dq, dkv (laid out as q, kv; dv: as v, where that was
+        given) and drate; set_dq / set_dkv overwrite dq / dkv and dv instead.
+        dstate_out: the gradient of the state that forward returned; dstate
+        receives the given state's."""
         import torch
+        if (v is None) != (dv is None):
+            raise ValueError("DecayCore.backward: v and dv go together")
         ctx = self.ctx or default_ctx(dy.device.index or 0)
-        d, nb, nq, nkv = self._plan(n, t, 1, (qstride, qoff, kvstride, koff, voff))
-        ins = self._inputs(ctx, n, nq, nkv, q, kv, rate, lens, state)
+        d, nb, nq, nk, nv = self._plan(n, t, 1, (qstride, qoff, kvstride, koff,
+                                                 None if v is None else vstride, voff))
+        st = n * self.h * self.dk * self.dv
+        kp, dkp = _arg(ctx, kv, nk, "kv"), _arg(ctx, dkv, nk, "dkv")
+        ins = (_arg(ctx, q, nq, "q"), kp, kp if v is None else _arg(ctx, v, nv, "v"),
+               _arg(ctx, rate, self.h, "rate"), _arg(ctx, lens, n, "lens", "u32"),
+               _arg(ctx, state, st, "state"), _arg(ctx, dy, n * t * self.c, "dy"),
+               _arg(ctx, dstate_out, st, "dstate_out"))
         ws = torch.empty(nb, dtype=torch.uint8, device=dy.device) if nb else None
         flags = (RNN_ATTN_SET_DQ if set_dq else 0) | (RNN_ATTN_SET_DKV if set_dkv else 0)
-        st = n * self.h * self.dk * self.dv
-        ins += (_arg(ctx, dy, n * t * self.c, "dy"), _arg(ctx, dstate_out, st, "dstate_out"))
-        outs = (_arg(ctx, dq, nq, "dq"), _arg(ctx, dkv, nkv, "dkv"),
+        outs = (_arg(ctx, dq, nq, "dq"), dkp, dkp if v is None else _arg(ctx, dv, nv, "dv"),
                 _arg(ctx, drate, self.h, "drate"), _arg(ctx, dstate, st, "dstate"))
         on = _OnStream(ctx)
         try:
             ctx.check(lib().rnn_decay_attn_backward(
                 ctx.h, C.byref(d), n, t, *ins, ws.data_ptr() if nb else None, nb, *outs, flags))
         finally:
-            on.done(q, kv, rate, lens, state, ws, dy, dstate_out, dq, dkv, drate, dstate)
+            on.done(q, kv, v, rate, lens, state, ws, dy, dstate_out, dq, dkv, dv, drate, dstate)
 
 
 class HeadGate:

@@ -610,7 +610,7 @@ struct GroupArgs {
     float *out[2];
     int d[2];
     const uint32_t *lens;
-    long long stride;
+    long long stride[2];
     int t, hkv, grp, acc;
 };
 __global__ __launch_bounds__(256) void decay_group_kernel(GroupArgs g, long long rows) {
@@ -623,7 +623,7 @@ __global__ __launch_bounds__(256) void decay_group_kernel(GroupArgs g, long long
         const float *p = g.part[k] + row * w * g.grp + (long long)hd * g.grp * d + (at - hd * d);
         float s = p[0];
         for (int r = 1; r < g.grp; r++) s += p[(long long)r * d];
-        float *o = g.out[k] + row * g.stride + at;
+        float *o = g.out[k] + row * g.stride[k] + at;
         *o = g.acc ? *o + s : s;
     }
 }
@@ -696,13 +696,11 @@ int decay_check(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n, size_t t) 
                         d->dk, d->dv, MAX_D);
     const uint64_t qw = (uint64_t)d->h * d->dk, kw = (uint64_t)d->hkv * d->dk,
                    vw = (uint64_t)d->hkv * d->dv;
-    if (d->qstride > (1u << 22) || d->kvstride > (1u << 22) || (uint64_t)d->h * std::max(d->dk, d->dv) > (1u << 22))
+    if (d->qstride > (1u << 22) || d->kstride > (1u << 22) || d->vstride > (1u << 22) || (uint64_t)d->h * std::max(d->dk, d->dv) > (1u << 22))
         return rnn_fail(ctx, RNN_E_UNSUPPORTED, "decay_attn: row stride above 2^22");
-    if (d->qoff > d->qstride || d->qstride - d->qoff < qw || d->koff > d->kvstride ||
-        d->kvstride - d->koff < kw || d->voff > d->kvstride || d->kvstride - d->voff < vw)
+    if (d->qoff > d->qstride || d->qstride - d->qoff < qw || d->koff > d->kstride ||
+        d->kstride - d->koff < kw || d->voff > d->vstride || d->vstride - d->voff < vw)
         return rnn_fail(ctx, RNN_E_INVALID, "decay_attn: heads do not fit a row");
-    if (d->koff < d->voff + vw && d->voff < d->koff + kw)
-        return rnn_fail(ctx, RNN_E_INVALID, "decay_attn: keys and values overlap");
     const uint64_t lim = 1ull << 31, per = (uint64_t)d->h * std::max<uint64_t>(t, (uint64_t)d->dk * d->dv);
     if (t >= lim || per >= lim || (n && n > (lim - 1) / per))
         return rnn_fail(ctx, RNN_E_UNSUPPORTED, "decay_attn: too many tokens or states");
@@ -800,15 +798,15 @@ int rnn_decay_attn_workspace(const rnn_decay_attn_desc *d, size_t n, size_t t, i
 }
 
 int rnn_decay_attn_forward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n, size_t t,
-                           const float *q, const float *kv, const float *rate, const uint32_t *lens,
-                           const float *state_in, void *ws, size_t ws_bytes, float *y,
-                           float *state_out) {
+                           const float *q, const float *k, const float *v, const float *rate,
+                           const uint32_t *lens, const float *state_in, void *ws, size_t ws_bytes,
+                           float *y, float *state_out) {
     if (!ctx) return RNN_E_NULL;
     std::lock_guard<std::recursive_mutex> lk(ctx->mu);
     int rc = decay_check(ctx, d, n, t);
     if (rc) return rc;
     if (!n || (!t && !state_out)) return RNN_OK;
-    if ((t && (!q || !kv || !y)) || !rate) return rnn_fail(ctx, RNN_E_NULL, "decay_attn_forward: null operand");
+    if ((t && (!q || !k || !v || !y)) || !rate) return rnn_fail(ctx, RNN_E_NULL, "decay_attn_forward: null operand");
     const DecayPlan w = plan_of(d, n, t, false);
     rc = check_ws(ctx, w, ws, ws_bytes);
     if (rc) return rc;
@@ -816,8 +814,8 @@ int rnn_decay_attn_forward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n,
     DecayArgs g;
     fill_args(g, d, w, n, t, rate, lens);
     const int grp = (int)(d->h / d->hkv);
-    const Operand Q = {q + d->qoff, d->qstride, 1}, K = {kv + d->koff, d->kvstride, grp},
-                  V = {kv + d->voff, d->kvstride, grp};
+    const Operand Q = {q + d->qoff, d->qstride, 1}, K = {k + d->koff, d->kstride, grp},
+                  V = {v + d->voff, d->vstride, grp};
     DecayJob &j = g.job[0];
     j = make_job(Q, K, (int)d->dk, V, (int)d->dv, y, (size_t)d->h * d->dv);
     j.s0 = state_in;
@@ -850,10 +848,10 @@ int rnn_decay_attn_forward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n,
 }
 
 int rnn_decay_attn_backward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n, size_t t,
-                            const float *q, const float *kv, const float *rate, const uint32_t *lens,
-                            const float *state_in, const float *dy, const float *dstate_out, void *ws,
-                            size_t ws_bytes, float *dq, float *dkv, float *drate, float *dstate_in,
-                            uint32_t flags) {
+                            const float *q, const float *k, const float *v, const float *rate,
+                            const uint32_t *lens, const float *state_in, const float *dy,
+                            const float *dstate_out, void *ws, size_t ws_bytes, float *dq, float *dk,
+                            float *dv, float *drate, float *dstate_in, uint32_t flags) {
     if (!ctx) return RNN_E_NULL;
     std::lock_guard<std::recursive_mutex> lk(ctx->mu);
     int rc = decay_check(ctx, d, n, t);
@@ -861,7 +859,7 @@ int rnn_decay_attn_backward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n
     if (flags & ~(uint32_t)(RNN_ATTN_SET_DQ | RNN_ATTN_SET_DKV))
         return rnn_fail(ctx, RNN_E_INVALID, "decay_attn_backward: unknown flags 0x%x", flags);
     if (!n || (!t && !dstate_in)) return RNN_OK;
-    if ((t && (!q || !kv || !dy || !dq || !dkv)) || !rate)
+    if ((t && (!q || !k || !v || !dy || !dq || !dk || !dv)) || !rate)
         return rnn_fail(ctx, RNN_E_NULL, "decay_attn_backward: null operand");
     if (dstate_in && (dstate_in == dstate_out || dstate_in == state_in))
         return rnn_fail(ctx, RNN_E_INVALID, "decay_attn_backward: dstate_in is an operand");
@@ -871,13 +869,13 @@ int rnn_decay_attn_backward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n
     RNN_ON_DEVICE(ctx);
     DecayArgs g;
     fill_args(g, d, w, n, t, rate, lens);
-    const int grp = (int)(d->h / d->hkv), dk = (int)d->dk, dv = (int)d->dv;
-    const Operand Q = {q + d->qoff, d->qstride, 1}, K = {kv + d->koff, d->kvstride, grp},
-                  V = {kv + d->voff, d->kvstride, grp}, O = {dy, (size_t)d->h * d->dv, 1};
+    const int grp = (int)(d->h / d->hkv), kd = (int)d->dk, vd = (int)d->dv;
+    const Operand Q = {q + d->qoff, d->qstride, 1}, K = {k + d->koff, d->kstride, grp},
+                  V = {v + d->voff, d->vstride, grp}, O = {dy, (size_t)d->h * d->dv, 1};
     g.part = (double *)((char *)ws + w.part);
     DecayJob &jq = g.job[0], &jk = g.job[1], &jv = g.job[2];
-    jq = make_job(O, V, dv, K, dk, dq + d->qoff, d->qstride);
-    jq.si = 1, jq.sj = dv;
+    jq = make_job(O, V, vd, K, kd, dq + d->qoff, d->qstride);
+    jq.si = 1, jq.sj = vd;
     jq.s0 = state_in;
     jq.sa = d->scale;
     jq.acc = !(flags & RNN_ATTN_SET_DQ);
@@ -889,9 +887,9 @@ int rnn_decay_attn_backward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n
     // keys and values that query heads share: each head's part, then their sum
     const bool share = grp > 1;
     float *part_k = (float *)((char *)ws + w.part_k), *part_v = (float *)((char *)ws + w.part_v);
-    jk = make_job(V, O, dv, Q, dk, share ? part_k : dkv + d->koff, share ? (size_t)d->h * dk : d->kvstride);
-    jk.si = 1, jk.sj = dv;
-    jv = make_job(K, Q, dk, O, dv, share ? part_v : dkv + d->voff, share ? (size_t)d->h * dv : d->kvstride);
+    jk = make_job(V, O, vd, Q, kd, share ? part_k : dk + d->koff, share ? (size_t)d->h * kd : d->kstride);
+    jk.si = 1, jk.sj = vd;
+    jv = make_job(K, Q, kd, O, vd, share ? part_v : dv + d->voff, share ? (size_t)d->h * vd : d->vstride);
     jk.s0 = jv.s0 = dstate_out;
     jk.sb = jv.sb = d->scale;
     jk.rev = jv.rev = 1;
@@ -901,7 +899,7 @@ int rnn_decay_attn_backward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n
     if (w.nseg > 1) {
         // S from the keys and values, R from the queries and dy
         DecayArgs sg = g;
-        sg.job[0] = make_job(Q, K, dk, V, dv, nullptr, 0);
+        sg.job[0] = make_job(Q, K, kd, V, vd, nullptr, 0);
         sg.job[0].s0 = state_in;
         sg.job[0].seg = (float *)((char *)ws + w.seg);
         sg.job[1] = jv;
@@ -921,7 +919,7 @@ int rnn_decay_attn_backward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n
         one.job[0] = jk;
         one.job[1] = jv;
     }
-    const bool joint = (dk + 31) / 32 == (dv + 31) / 32;
+    const bool joint = (kd + 31) / 32 == (vd + 31) / 32;
     launch_walk<WALK>(ctx, one, (drate ? 1 : 2) + (joint ? 1 : 0));
     RNN_LAUNCHED(ctx);
     if (!joint) {
@@ -930,9 +928,9 @@ int rnn_decay_attn_backward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n
         RNN_LAUNCHED(ctx);
     }
     if (share && t) {
-        GroupArgs ga = {{part_k, part_v}, {dkv + d->koff, dkv + d->voff}, {dk, dv}, lens,
-                        (long long)d->kvstride, (int)t, (int)d->hkv, grp, acc};
-        const size_t each = n * t * d->hkv * (size_t)std::max(dk, dv);
+        GroupArgs ga = {{part_k, part_v}, {dk + d->koff, dv + d->voff}, {kd, vd}, lens,
+                        {(long long)d->kstride, (long long)d->vstride}, (int)t, (int)d->hkv, grp, acc};
+        const size_t each = n * t * d->hkv * (size_t)std::max(kd, vd);
         decay_group_kernel<<<dim3((unsigned)std::min<size_t>(rnn_div_up(each, 256), 4096), 2), 256, 0,
                              ctx->stream>>>(ga, (long long)(n * t));
         RNN_LAUNCHED(ctx);

@@ -1,5 +1,6 @@
 """vit.rs / attn.rs call sites on the device: SelfAttn, CrossAttn, DropPath,
-DiffSelfAttn (differential attention with rotary positions), the pre-LN Block, token merge, TaxoHead and Exit.
+DiffSelfAttn (differential attention with rotary positions), DecaySelfAttn (linear attention with a
+decay), the pre-LN Block, token merge, TaxoHead and Exit.
 
 Mirrors the reference's layer interface (attn.rs:346-560, vit.rs:25-353)
 over token tensors [n, t, c] (float32 CUDA, channel fastest):
@@ -17,7 +18,7 @@ from __future__ import annotations
 
 import numpy as np
 
-from . import (Core, DiffCore, Linear, Rotary, _ptr, default_ctx, lib, linear_backward,
+from . import (Core, DecayCore, DiffCore, HeadGate, Linear, NormRotary, Rotary, _ptr, default_ctx, lib, linear_backward,
                linear_forward, rel_index)
 from .data import Rng
 from .norm import DwConv3, LayerNorm, LayerScale, Mlp, SeqPool, SwiGlu, _linear_param
@@ -174,6 +175,80 @@ class DiffSelfAttn:
         f(self.gain)
 
 
+
+class DecaySelfAttn:
+    """Linear attention with a decay for each head in SelfAttn's interface (no
+    counterpart in the reference): fused Linear(c, 4c) into q, k, v and a gate z
+    -> NormRotary on the queries and keys -> DecayCore of h heads, the last
+    ``reverse`` of them (default: half) from the last token to the first ->
+    HeadGate by z -> proj Linear::scaled.  grid as DiffSelfAttn's.  The heads of
+    a direction begin with memories of 2 tokens up to all of them."""
+
+    def __init__(self, c, h, grid, depth, rng=None, device=0, ctx=None, reverse=None, base=100.0):
+        import torch
+        dev = f"cuda:{device}"
+        self.ctx = ctx or default_ctx(device)
+        rng = _rng(rng, 0)
+        if c % (2 * h):
+            raise ValueError(f"DecaySelfAttn: {c} channels are not {h} even heads")
+        self.c, self.h, self.dh = c, h, c // h
+        self.rot = NormRotary(h, h, self.dh, grid, base, ctx=self.ctx)
+        self.t = self.rot.t
+        back = h // 2 if reverse is None else int(reverse)
+        self.core = DecayCore(h, self.dh, reverse=back, ctx=self.ctx)
+        self.gate = HeadGate(h, self.dh, ctx=self.ctx)
+        self.lin = _linear(c, 4 * c, True, 0.02, rng, dev, self.ctx)
+        self.proj = _linear(c, c, True, _scaled_std(depth), rng, dev, self.ctx)
+        spans = [np.geomspace(2, max(2, self.t), m) for m in (h - back, back)]
+        rate = -np.log(np.concatenate(spans)).astype(np.float32)
+        self.rate = Param(torch.from_numpy(rate).to(dev), False)
+        self.gain = Param(torch.ones(2 * self.dh, device=dev), False)
+        self.ogain = Param(torch.ones(c, device=dev), False)
+        self._lin = _linear_param(self.lin) + _linear_param(self.proj)
+        self.saved = None
+        self.n = 0
+
+    def _geo(self, qk):
+        c = self.c
+        return qk, 2 * c, 0, qk, 2 * c, c, 2 * c
+
+    def forward(self, x, train):
+        n, t, c = x.shape
+        ab = self.lin.forward(x.reshape(-1), n * t, train)
+        qk = self.rot.forward(n, ab, 4 * c, 0, self.gain.v)
+        o, _ = self.core.forward(n, t, *self._geo(qk), self.rate.v, v=ab, vstride=4 * c)
+        u = self.gate.forward(n * t, o, ab, 4 * c, 3 * c, self.ogain.v)
+        y = self.proj.forward(u.view(-1), n * t, train)
+        if train:
+            self.saved, self.n = (ab, qk, o), n
+        return y.view(n, t, c)
+
+    def backward(self, dy, acc_dx=None):
+        """dx, or acc_dx += dx (returned) when given."""
+        import torch
+        n, t, c = self.n, self.t, self.c
+        ab, qk, o = self.saved
+        du = self.proj.backward(dy.reshape(-1))
+        # every column of the fused gradient is written: dq and dk by the norm's
+        # backward, dv by the core's, dz by the gate's
+        dab, dqk = torch.empty_like(ab), torch.empty_like(qk)
+        do = self.gate.backward(n * t, o, ab, 4 * c, 3 * c, self.ogain.v, du, dab, 4 * c, 3 * c,
+                                self.ogain.g)
+        self.core.backward(n, t, *self._geo(qk), self.rate.v, do, dqk, dqk, self.rate.g,
+                           set_dq=True, set_dkv=True, v=ab, vstride=4 * c, dv=dab)
+        self.rot.backward(n, ab, 4 * c, 0, self.gain.v, dqk, 2 * c, 0, self.gain.g, dx=dab,
+                          dxstride=4 * c)
+        acc = acc_dx.reshape(-1) if acc_dx is not None else None
+        return self.lin.backward(dab, acc_dx=acc).view(n, t, c)
+
+    def for_each_param(self, f):
+        for p in self._lin:
+            f(p)
+        f(self.rate)
+        f(self.gain)
+        f(self.ogain)
+
+
 class CrossAttn:
     """CrossAttn (attn.rs:450-560): wq Linear(c, c) -> Core over the memory
     [n, mh*mw, 2c] (K at 0, V at c), no mask -> proj Linear::scaled."""
@@ -324,7 +399,7 @@ class Block:
     """Block (vit.rs:76-250), pre-LN with three branches from one norm:
     h = LN(x); x += ls1 * dp1(SelfAttn(h) + gamma * DwConv3(h));
     x += lsm * dp2(CrossAttn(h, mem)) (reader blocks); x += ls2 * dp3(SwiGlu(LN(x))).
-    attn="diff": DiffSelfAttn in SelfAttn's place; mlp: "swiglu", or an
+    attn="diff" / "decay": DiffSelfAttn / DecaySelfAttn in SelfAttn's place; mlp: "swiglu", or an
     activation (one of rustnn_amd.ACTS) for an Mlp of 4c hidden channels."""
 
     def __init__(self, c, h, th, tw, mem, depth, drop, idx, ls_init, rng=None, device=0,
@@ -339,10 +414,12 @@ class Block:
         self.c, self.idx = c, int(idx)
         hidden = -(-(4 * c // 3) // 16) * 16
         self.n1 = LayerNorm(c, device, self.ctx)
-        if attn not in ("lsa", "diff"):
-            raise ValueError(f"Block: attn {attn!r} (lsa or diff)")
+        if attn not in ("lsa", "diff", "decay"):
+            raise ValueError(f"Block: attn {attn!r} (lsa, diff or decay)")
         self.attn = (SelfAttn(c, h, th, tw, depth, rng, device, self.ctx) if attn == "lsa" else
-                     DiffSelfAttn(c, h, (th, tw), depth, idx, rng, device, self.ctx))
+                     DiffSelfAttn(c, h, (th, tw), depth, idx, rng, device, self.ctx)
+                     if attn == "diff" else
+                     DecaySelfAttn(c, h, (th, tw), depth, rng, device, self.ctx))
         self.dw = DwConv3(c, th, tw, _trunc_normal(9 * c, 0.1, rng, dev), None, device, self.ctx)
         self.gamma = Param(torch.full((c,), 0.5, device=dev), False)
         self.ls1 = LayerScale(c, ls_init, device, self.ctx)

@@ -18,9 +18,9 @@ def test_null_context_is_refused():
     assert L.rnn_norm_rotary_forward(None, C.byref(d), 1, 1e-6, 1, 1, *[None] * 4) == R.RNN_E_NULL
     assert L.rnn_norm_rotary_backward(None, C.byref(d), 1, 1e-6, 1, 1, *[None] * 4, 8, 0, None, 0,
                                       None, None) == R.RNN_E_NULL
-    assert L.rnn_decay_attn_forward(None, C.byref(e), 1, 1, *[None] * 6, 0, None, None) == \
+    assert L.rnn_decay_attn_forward(None, C.byref(e), 1, 1, *[None] * 7, 0, None, None) == \
         R.RNN_E_NULL
-    assert L.rnn_decay_attn_backward(None, C.byref(e), 1, 1, *[None] * 8, 0, *[None] * 4, 0) == \
+    assert L.rnn_decay_attn_backward(None, C.byref(e), 1, 1, *[None] * 9, 0, *[None] * 5, 0) == \
         R.RNN_E_NULL
     assert L.rnn_head_gate_forward(None, 1, 1, 1, 1e-6, None, None, 1, 0, None, None) == R.RNN_E_NULL
     assert L.rnn_head_gate_backward(None, 1, 1, 1, 1e-6, None, None, 1, 0, None, None, None, 0, None,
@@ -63,7 +63,7 @@ def test_decay_core_refuses(kw):
 
 def test_decay_description_is_checked():
     core, nb = R.DecayCore(4, 32, 48, 2), C.c_size_t()
-    ok = dict(qstride=288, qoff=0, kvstride=288, koff=128, voff=192)
+    ok = dict(qstride=288, qoff=0, kstride=288, koff=128, vstride=288, voff=192)
 
     def code(n=2, t=8, back=1, out=nb, **kw):
         d = core.desc(**dict(ok, **kw))
@@ -72,10 +72,14 @@ def test_decay_description_is_checked():
 
     assert code() == R.RNN_OK and code(back=0) == R.RNN_OK and code(n=0) == R.RNN_OK
     assert code(out=None) == R.RNN_E_NULL
-    for kw in (dict(qstride=127), dict(qoff=200), dict(voff=193), dict(koff=225), dict(voff=191),
-               dict(koff=230, voff=160), dict(koff=1 << 40)):
+    for kw in (dict(qstride=127), dict(qoff=200), dict(voff=193), dict(koff=225), dict(vstride=287),
+               dict(koff=1 << 40)):
         assert code(**kw) == R.RNN_E_INVALID, kw
-    assert code(kvstride=(1 << 22) + 1) == R.RNN_E_UNSUPPORTED
+    assert code(kstride=(1 << 22) + 1) == R.RNN_E_UNSUPPORTED
+    assert code(vstride=(1 << 22) + 1) == R.RNN_E_UNSUPPORTED
+    for koff, voff in ((128, 191), (230, 160), (160, 100)):  # in one buffer keys and values overlap
+        with pytest.raises(ValueError):
+            core._plan(2, 8, 0, (288, 0, 288, koff, None, voff))
     assert code(n=1 << 40) == R.RNN_E_UNSUPPORTED and code(t=1 << 40) == R.RNN_E_UNSUPPORTED
     assert code(n=1, t=1 << 29) == R.RNN_E_UNSUPPORTED  # t h = 2^31
     assert code(n=1 << 19, t=1) == R.RNN_E_UNSUPPORTED  # n h dk dv > 2^31
