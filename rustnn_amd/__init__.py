@@ -1019,7 +1019,7 @@ class NormRotary:
         writes y (x: in place, which a backward cannot follow; None: a new
         [n, t, (hq + hk) dh]), at the same layout unless ystride is given.
         pos and t as Rotary's."""
-        ctx, w = self.ctx or default_ctx(x.device.index or 0), self.heads * self.dh
+        ctx, w = self.ctx or default_ctx(max(x.get_device(), 0)), self.heads * self.dh
         t = self.t if t is None else int(t)
         y, ystride, yoff = self._out(x, n, t, y, ystride, yoff, xstride, xoff)
         d, _ = self._plan(n, t, pos is not None, (xstride, xoff, ystride, yoff))
@@ -1041,7 +1041,7 @@ class NormRotary:
         """dx (returned) from the forward's input x and dy; dx given: at dy's
         layout unless dxstride is (dy: in place).  dgain [2, dh] accumulates."""
         import torch
-        ctx, w = self.ctx or default_ctx(x.device.index or 0), self.heads * self.dh
+        ctx, w = self.ctx or default_ctx(max(x.get_device(), 0)), self.heads * self.dh
         t = self.t if t is None else int(t)
         dx, dxstride, dxoff = self._out(x, n, t, dx, dxstride, dxoff, dystride, dyoff)
         d, nb = self._plan(n, t, pos is not None, (xstride, xoff, dxstride, dxoff))
@@ -1122,7 +1122,7 @@ class DecayCore:
         unless keep_state or state_out, which may be state).  lens (int32 /
         uint32 [n]): the sequences' lengths where they are padded."""
         import torch
-        ctx = self.ctx or default_ctx(q.device.index or 0)
+        ctx = self.ctx or default_ctx(max(q.get_device(), 0))
         d, nb, nq, nk, nv = self._plan(n, t, 0, (qstride, qoff, kvstride, koff,
                                                  None if v is None else vstride, voff))
         st = n * self.h * self.dk * self.dv
@@ -1155,7 +1155,7 @@ class DecayCore:
         import torch
         if (v is None) != (dv is None):
             raise ValueError("DecayCore.backward: v and dv go together")
-        ctx = self.ctx or default_ctx(dy.device.index or 0)
+        ctx = self.ctx or default_ctx(max(dy.get_device(), 0))
         d, nb, nq, nk, nv = self._plan(n, t, 1, (qstride, qoff, kvstride, koff,
                                                  None if v is None else vstride, voff))
         st = n * self.h * self.dk * self.dv
@@ -1208,7 +1208,7 @@ class HeadGate:
     def forward(self, rows, x, z, zstride, zoff=0, gain=None, y=None):
         """y (returned; x: in place, which a backward cannot follow)."""
         import torch
-        ctx = self.ctx or default_ctx(x.device.index or 0)
+        ctx = self.ctx or default_ctx(max(x.get_device(), 0))
         self._bytes(rows)
         if y is None:
             y = torch.empty(rows, self.c, dtype=torch.float32, device=x.device)
@@ -1226,7 +1226,7 @@ class HeadGate:
         """dx (returned) and dz, in rows of dzstride floats from dzoff on, are
         overwritten; dgain [h d] accumulates."""
         import torch
-        ctx = self.ctx or default_ctx(x.device.index or 0)
+        ctx = self.ctx or default_ctx(max(x.get_device(), 0))
         nb = self._bytes(rows) if dgain is not None else 0
         if dx is None:
             dx = torch.empty(rows, self.c, dtype=torch.float32, device=x.device)

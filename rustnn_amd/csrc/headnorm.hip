@@ -103,77 +103,93 @@ struct NrArgs {
     double w[MAX_PAIRS];  // quarter turns per unit of position of every pair
 };
 
-// A lane's channels: two runs of four, from ca and cb on, neighbouring lanes' runs
-// next to each other, so that a load takes whole lines.  Lanes before T hold four
-// pairs: (j, j + R) of the two runs, or, alternating, two pairs of each run; those
-// past them channels that do not turn.  As elements, e < 4 is the first channel of
-// the lane's pair e and e >= 4 the second one of pair e - 4.
-// VEC: 16-byte accesses; R and dh are multiples of four, rows and heads aligned.
-// Else a run's four pairs end where R ends, and channels are loaded one by one.
-template <bool VEC, bool INTER>
+// Four channels at p, of which the first n are there.  16-byte accesses need 4-byte
+// alignment alone.
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+__device__ __forceinline__ void load4(const float *p, int n, float *v) {
+    if (n == 4) {
+        const f4u t = *(const f4u *)p;
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = t[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = e < n ? p[e] : 0.f;
+    }
+}
+__device__ __forceinline__ void store4(float *p, int n, const float *v) {
+    if (n == 4) {
+        *(f4u *)p = f4u{v[0], v[1], v[2], v[3]};
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (e < n) p[e] = v[e];
+    }
+}
+
+// A lane's channels: two runs of four, from ca and cb on (na and nb of them are
+// there), neighbouring lanes' runs next to each other, so that an access takes whole
+// lines (eight channels a lane in one piece: a gate's forward 60 us against 32).
+// Lanes before T hold four pairs: (j, j + R) of the two runs, or, alternating, two
+// pairs of each run, which then are two halves of the pairs where those are a
+// multiple of four; lanes past them channels that do not turn.  As elements, e < 4
+// is the first channel of the lane's pair e and e >= 4 the second one of pair e - 4.
+template <bool INTER>
 struct NrLane {
-    int ca, cb, u, R, dh;
-    bool turned;
-    __device__ __forceinline__ NrLane(const NrArgs &g, int lane) : u(lane), R(g.npairs), dh(g.dh) {
-        const int T = (R + 3) / 4, n = (dh - 2 * R + 7) / 8, v = u - T;
+    int ca, cb, na, nb, u, R;
+    bool turned, halves;
+    __device__ __forceinline__ NrLane(const NrArgs &g, int lane) : u(lane), R(g.npairs) {
+        const int T = (R + 3) / 4, n = (g.dh - 2 * R + 7) / 8, v = u - T;
         turned = u < T;
-        ca = turned ? (VEC || !INTER ? 4 * u : 8 * u) : v < n ? 2 * R + 4 * v : dh;
-        cb = turned ? (VEC || !INTER ? R + 4 * u : 8 * u + 4) : v < n ? 2 * R + 4 * (n + v) : dh;
+        halves = R % 4 == 0;
+        if (turned) {
+            const int pairs = min(R - 4 * u, 4);
+            ca = INTER && !halves ? 8 * u : 4 * u;
+            cb = INTER && !halves ? 8 * u + 4 : R + 4 * u;
+            na = INTER ? min(2 * pairs, 4) : pairs;
+            nb = INTER ? 2 * pairs - na : pairs;
+        } else {
+            ca = 2 * R + 4 * v;
+            cb = 2 * R + 4 * (n + v);
+            na = v < n ? min(max(g.dh - ca, 0), 4) : 0;
+            nb = v < n ? min(max(g.dh - cb, 0), 4) : 0;
+        }
     }
     // the pair of elements q and q + 4
     __device__ __forceinline__ int pair(int q) const {
-        return VEC && INTER ? (q < 2 ? 2 * u + q : R / 2 + 2 * u + q - 2) : 4 * u + q;
+        return INTER && halves ? (q < 2 ? 2 * u + q : R / 2 + 2 * u + q - 2) : 4 * u + q;
     }
     // element e's place in the two runs, and its channel; -1: none
     static __device__ __forceinline__ constexpr int place(int e) {
         return INTER ? (e < 4 ? 2 * e : 2 * e - 7) : e;
     }
     __device__ __forceinline__ int channel(int e) const {
-        const int p = place(e), c = p < 4 ? ca + p : cb + p - 4;
-        if (turned) return VEC || 4 * u + (e & 3) < R ? c : -1;
-        return c < dh ? c : -1;
+        const int p = place(e);
+        return p < 4 ? (p < na ? ca + p : -1) : p - 4 < nb ? cb + p - 4 : -1;
     }
     __device__ __forceinline__ void load(const float *p, float (&v)[8]) const {
-        if constexpr (VEC) {
-            float t[8];
-            const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-            *(float4 *)t = ca < dh ? *(const float4 *)(p + ca) : z;
-            *(float4 *)(t + 4) = cb < dh ? *(const float4 *)(p + cb) : z;
+        float t[8];
+        load4(p + ca, na, t);
+        load4(p + cb, nb, t + 4);
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = t[place(e)];
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int c = channel(e);
-                v[e] = c >= 0 ? p[c] : 0.f;
-            }
-        }
+        for (int e = 0; e < 8; e++) v[e] = t[place(e)];
     }
     __device__ __forceinline__ void store(float *p, const float (&v)[8]) const {
-        if constexpr (VEC) {
-            float t[8];
+        float t[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) t[place(e)] = v[e];
-            if (ca < dh) *(float4 *)(p + ca) = *(const float4 *)t;
-            if (cb < dh) *(float4 *)(p + cb) = *(const float4 *)(t + 4);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int c = channel(e);
-                if (c >= 0) p[c] = v[e];
-            }
-        }
+        for (int e = 0; e < 8; e++) t[place(e)] = v[e];
+        store4(p + ca, na, t);
+        store4(p + cb, nb, t + 4);
     }
 };
 
 // A block has `span` rows, of which it takes `rpb` at a time: their sines and cosines into LDS, formed
 // once for all heads, then every head.
-template <bool VEC, bool INTER, bool BACK>
-__global__ __launch_bounds__(256, BACK ? 3 : VEC ? 5 : 4) void norm_rotary_kernel(NrArgs g) {
+template <bool INTER, bool BACK>
+__global__ __launch_bounds__(256, BACK ? 3 : 5) void norm_rotary_kernel(NrArgs g) {
     __shared__ __attribute__((aligned(16))) float2 tab[TABLE];
     const int L = g.lanes, R = g.npairs;
     const int ng = 256 / L, grp = threadIdx.x / L;
-    using Lane = NrLane<VEC, INTER>;
+    using Lane = NrLane<INTER>;
     const Lane own(g, threadIdx.x & (L - 1));
     float gain[2][8];
 #pragma unroll
@@ -288,43 +304,24 @@ struct GateArgs {
     double eps;
 };
 
-// A lane's channels: four from c on, and four from c + 4 L on.
-template <bool VEC>
-__device__ __forceinline__ void gate_load(const float *p, int c, int c2, int d, float (&v)[8]) {
-    if constexpr (VEC) {
-        const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-        *(float4 *)v = c < d ? *(const float4 *)(p + c) : z;
-        *(float4 *)(v + 4) = c2 < d ? *(const float4 *)(p + c2) : z;
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const int at = e < 4 ? c + e : c2 + e - 4;
-            v[e] = at < d ? p[at] : 0.f;
-        }
-    }
-}
-template <bool VEC>
-__device__ __forceinline__ void gate_store(float *p, int c, int c2, int d, const float (&v)[8]) {
-    if constexpr (VEC) {
-        if (c < d) *(float4 *)(p + c) = *(const float4 *)v;
-        if (c2 < d) *(float4 *)(p + c2) = *(const float4 *)(v + 4);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const int at = e < 4 ? c + e : c2 + e - 4;
-            if (at < d) p[at] = v[e];
-        }
-    }
-}
-
 // Block b: head b % h, rows (b / h) * groups + group, and every splits * groups
 // further, so that dgain's sums stay with one head's channels.  (Neighbouring
 // heads in one block, whole rows at a time, took no less: 2.1 to 2.4 TB/s.)
-template <bool VEC, bool BACK>
+template <bool BACK>
 __global__ __launch_bounds__(256) void head_gate_kernel(GateArgs g) {
     const int L = g.lanes, ng = 256 / L, at = threadIdx.x / L, u = threadIdx.x & (L - 1);
     const int head = blockIdx.x % g.h, split = blockIdx.x / g.h, splits = gridDim.x / g.h;
+    // four channels from c on, and four from c2 on
     const int c = 4 * u, c2 = 4 * (L + u), col = head * g.d;
+    const int n1 = min(max(g.d - c, 0), 4), n2 = min(max(g.d - c2, 0), 4);
+    const auto load = [&](const float *p, float (&v)[8]) {
+        load4(p + col + c, n1, v);
+        load4(p + col + c2, n2, v + 4);
+    };
+    const auto store = [&](float *p, const float (&v)[8]) {
+        store4(p + col + c, n1, v);
+        store4(p + col + c2, n2, v + 4);
+    };
     const long long w = (long long)g.h * g.d;
     float gain[8];
 #pragma unroll
@@ -341,9 +338,9 @@ __global__ __launch_bounds__(256) void head_gate_kernel(GateArgs g) {
     long long r, nr;
     auto fetch = [&](long long at) {
         nr = min(at, g.rows - 1);
-        gate_load<VEC>(g.x + nr * w + col, c, c2, g.d, nv);
-        gate_load<VEC>(g.z + nr * g.zstride + col, c, c2, g.d, nz);
-        if constexpr (BACK) gate_load<VEC>(g.dy + nr * w + col, c, c2, g.d, nd);
+        load(g.x + nr * w, nv);
+        load(g.z + nr * g.zstride, nz);
+        if constexpr (BACK) load(g.dy + nr * w, nd);
     };
     fetch((long long)split * ng + at);
     for (long long r0 = (long long)split * ng; r0 < g.rows; r0 += step) {
@@ -380,9 +377,9 @@ __global__ __launch_bounds__(256) void head_gate_kernel(GateArgs g) {
             m32 = (float)(group_sum((double)m32, L) * inv);
 #pragma unroll
             for (int e = 0; e < 8; e++) o[e] = hat32(__builtin_fmaf(-hat[e], m32, o[e]));
-            if (live) gate_store<VEC>(g.dz + r * g.dzstride + col, c, c2, g.d, dz);
+            if (live) store(g.dz + r * g.dzstride, dz);
         }
-        if (live) gate_store<VEC>(g.y + r * w + col, c, c2, g.d, o);
+        if (live) store(g.y + r * w, o);
     }
     if constexpr (BACK) {
         if (!g.part) return;
@@ -456,10 +453,6 @@ int nr_check(rnn_ctx *ctx, const rnn_rotary_desc *d, uint32_t hq, float eps, siz
     return RNN_OK;
 }
 
-bool aligned16(const float *p, long long stride) {
-    return ((uintptr_t)p & 15) == 0 && stride % 4 == 0;
-}
-
 void nr_fill(NrArgs &g, const rnn_rotary_desc *d, uint32_t hq, float eps, size_t n, size_t t,
              const float *x, const float *gain, const float *pos, float *y) {
     g.x = x + d->xoff;
@@ -487,15 +480,11 @@ void nr_fill(NrArgs &g, const rnn_rotary_desc *d, uint32_t hq, float eps, size_t
 }
 
 template <bool BACK>
-void nr_launch(rnn_ctx *ctx, const NrArgs &g, int blocks, bool vec, bool inter) {
-    if (vec && inter)
-        norm_rotary_kernel<true, true, BACK><<<blocks, 256, 0, ctx->stream>>>(g);
-    else if (vec)
-        norm_rotary_kernel<true, false, BACK><<<blocks, 256, 0, ctx->stream>>>(g);
-    else if (inter)
-        norm_rotary_kernel<false, true, BACK><<<blocks, 256, 0, ctx->stream>>>(g);
+void nr_launch(rnn_ctx *ctx, const NrArgs &g, int blocks, bool inter) {
+    if (inter)
+        norm_rotary_kernel<true, BACK><<<blocks, 256, 0, ctx->stream>>>(g);
     else
-        norm_rotary_kernel<false, false, BACK><<<blocks, 256, 0, ctx->stream>>>(g);
+        norm_rotary_kernel<false, BACK><<<blocks, 256, 0, ctx->stream>>>(g);
 }
 
 struct GatePlan {
@@ -565,9 +554,7 @@ int rnn_norm_rotary_forward(rnn_ctx *ctx, const rnn_rotary_desc *d, uint32_t hq,
     g.lanes = p.lanes;
     g.rpb = p.rpb;
     g.span = p.span;
-    const bool vec = g.npairs % 4 == 0 && g.dh % 4 == 0 && aligned16(g.x, g.xstride) &&
-                     aligned16(g.y, g.ystride);
-    nr_launch<false>(ctx, g, p.blocks, vec, d->interleaved != 0);
+    nr_launch<false>(ctx, g, p.blocks, d->interleaved != 0);
     RNN_LAUNCHED(ctx);
     return RNN_OK;
 }
@@ -602,9 +589,7 @@ int rnn_norm_rotary_backward(rnn_ctx *ctx, const rnn_rotary_desc *d, uint32_t hq
     g.lanes = p.lanes;
     g.rpb = p.rpb;
     g.span = p.span;
-    const bool vec = g.npairs % 4 == 0 && g.dh % 4 == 0 && aligned16(g.x, g.xstride) &&
-                     aligned16(g.y, g.ystride) && aligned16(g.dy, g.dystride);
-    nr_launch<true>(ctx, g, p.blocks, vec, d->interleaved != 0);
+    nr_launch<true>(ctx, g, p.blocks, d->interleaved != 0);
     RNN_LAUNCHED(ctx);
     if (dgain) {
         const size_t len = 2 * (size_t)d->dh;
@@ -633,15 +618,10 @@ int rnn_head_gate_forward(rnn_ctx *ctx, size_t rows, size_t h, size_t d, float e
     if (!x || !z || !y) return rnn_fail(ctx, RNN_E_NULL, "head_gate: null operand");
     RNN_ON_DEVICE(ctx);
     const GatePlan p = gate_plan(rows, h, d);
-    const long long w = (long long)(h * d);
     GateArgs g = {x, z + zoff, gain, nullptr, y, nullptr, nullptr, (long long)zstride, 0, (long long)rows,
                   (int)h, (int)d, p.lanes, (double)eps};
-    const bool vec = d % 4 == 0 && aligned16(x, w) && aligned16(g.z, g.zstride) && aligned16(y, w);
     const unsigned grid = (unsigned)(p.splits * h);
-    if (vec)
-        head_gate_kernel<true, false><<<grid, 256, 0, ctx->stream>>>(g);
-    else
-        head_gate_kernel<false, false><<<grid, 256, 0, ctx->stream>>>(g);
+    head_gate_kernel<false><<<grid, 256, 0, ctx->stream>>>(g);
     RNN_LAUNCHED(ctx);
     return RNN_OK;
 }
@@ -666,13 +646,8 @@ int rnn_head_gate_backward(rnn_ctx *ctx, size_t rows, size_t h, size_t d, float 
     GateArgs g = {x, z + zoff, gain, dy, dx, dz + dzoff, dgain ? (double *)ws : nullptr,
                   (long long)zstride, (long long)dzstride, (long long)rows, (int)h, (int)d, p.lanes,
                   (double)eps};
-    const bool vec = d % 4 == 0 && aligned16(x, w) && aligned16(g.z, g.zstride) && aligned16(dy, w) &&
-                     aligned16(dx, w) && aligned16(g.dz, g.dzstride);
     const unsigned grid = (unsigned)(p.parts * h);
-    if (vec)
-        head_gate_kernel<true, true><<<grid, 256, 0, ctx->stream>>>(g);
-    else
-        head_gate_kernel<false, true><<<grid, 256, 0, ctx->stream>>>(g);
+    head_gate_kernel<true><<<grid, 256, 0, ctx->stream>>>(g);
     RNN_LAUNCHED(ctx);
     if (dgain) {
         gain_reduce_kernel<<<(unsigned)rnn_div_up((size_t)w, 4), 256, 0, ctx->stream>>>((int)p.parts, (int)w,

@@ -11,20 +11,34 @@
 #include "rnn_internal.h"
 
 #include <cmath>
+#include <cstring>
 
 constexpr int MAX_PAIRS = 256;
 
 // RNN_OK, or the code with which a description is refused (ctx may be null).
 int rnn_rotary_checked(rnn_ctx *ctx, const rnn_rotary_desc *d, size_t n, size_t t, bool have_pos);
 
-// Quarter turns per unit of position of every pair.
+// Quarter turns per unit of position of every pair.  The powers (50 ns each) are kept
+// for the next call of the same shares and base.
 inline void rot_frequencies(const rnn_rotary_desc *d, double (&w)[MAX_PAIRS]) {
+    struct Kept {
+        uint32_t np[3] = {0, 0, 0};
+        float base = 0.f;
+        double w[MAX_PAIRS];
+    };
+    static thread_local Kept kept;
     const uint32_t np[3] = {d->p0, d->p1, d->p2};
-    int j = 0;
-    for (int a = 0; a < 3; a++)
-        for (uint32_t p = 0; p < np[a]; p++)
-            w[j++] = std::pow((double)d->base, -(double)p / (double)np[a]) *
-                     0.63661977236758134308;  // 2 / pi
+    const size_t all = (size_t)np[0] + np[1] + np[2];
+    if (kept.base != d->base || std::memcmp(kept.np, np, sizeof(np))) {
+        int j = 0;
+        for (int a = 0; a < 3; a++)
+            for (uint32_t p = 0; p < np[a]; p++)
+                kept.w[j++] = std::pow((double)d->base, -(double)p / (double)np[a]) *
+                              0.63661977236758134308;  // 2 / pi
+        std::memcpy(kept.np, np, sizeof(np));
+        kept.base = d->base;
+    }
+    std::memcpy(w, kept.w, all * sizeof(double));
 }
 
 // The position of row r on pair j's axis (g: a kernel's arguments).
