@@ -333,8 +333,8 @@ typedef struct {
  * (backward = 0) or the backward needs for n sequences of t tokens; host only.
  * The workspace is the caller's, 256-byte aligned, holds nothing between calls
  * and is not shared by calls that may run at the same time.  dk and dv <= 128, row
- * strides, y's among them, <= 2^22, n * t * h and n * h * dk * dv < 2^31
- * (RNN_E_UNSUPPORTED above), scale finite. */
+ * strides, y's among them, <= 2^22, t < 2^29, n * h < 2^22, n * h * t and
+ * n * h * dk * dv < 2^31 (RNN_E_UNSUPPORTED above), scale finite. */
 int rnn_decay_attn_workspace(const rnn_decay_attn_desc *d, size_t n, size_t t, int backward,
                              size_t *bytes);
 /* y [n][t][h][dv]. */

@@ -418,6 +418,7 @@ __global__ __launch_bounds__(256, DAT <= (MODE == WALK_RATE ? 1 : 2) ? 2 : 1) vo
 #pragma unroll
             for (int r = 0; r < 16; r++) S[d][r] = x.load(d, r);
     }
+    const float *sgrad = !slope || !T ? nullptr : g.nseg > 1 ? q.segg + sg : q.s1g ? q.s1g + st : nullptr;
     bool any = s0 != nullptr;  // whether the state may be other than 0
     const double lg = log_gamma(g.rate[hd]);
     wave_sync();
@@ -438,7 +439,7 @@ __global__ __launch_bounds__(256, DAT <= (MODE == WALK_RATE ? 1 : 2) ? 2 : 1) vo
             wave_sync();
         }
         // whether a reader of the state follows
-        const bool goes = MODE == STATE || c0 + L < T || slope || (ends && q.s1);
+        const bool goes = MODE == STATE || c0 + L < T || sgrad || (ends && q.s1);
         if constexpr (MODE != STATE) {
             f32x16 P, o, oz;
 #pragma unroll
@@ -543,7 +544,6 @@ __global__ __launch_bounds__(256, DAT <= (MODE == WALK_RATE ? 1 : 2) ? 2 : 1) vo
         load_cols(ChunkRows(pc, q.cs, q.dc, w, c0 + C, next), half, col, cf);
         __builtin_amdgcn_sched_barrier(0);
     }
-    const float *sgrad = !slope || !T ? nullptr : g.nseg > 1 ? q.segg + sg : q.s1g ? q.s1g + st : nullptr;
     float *s1 = MODE == STATE ? q.seg + sg : ends && q.s1 ? q.s1 + st : nullptr;
     if (s1) {
         const StateRows x(s1, q, half, col);
@@ -701,9 +701,11 @@ int decay_check(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n, size_t t) 
     if (d->qoff > d->qstride || d->qstride - d->qoff < qw || d->koff > d->kstride ||
         d->kstride - d->koff < kw || d->voff > d->vstride || d->vstride - d->voff < vw)
         return rnn_fail(ctx, RNN_E_INVALID, "decay_attn: heads do not fit a row");
-    const uint64_t lim = 1ull << 31, per = (uint64_t)d->h * std::max<uint64_t>(t, (uint64_t)d->dk * d->dv);
-    if (t >= lim || per >= lim || (n && n > (lim - 1) / per))
-        return rnn_fail(ctx, RNN_E_UNSUPPORTED, "decay_attn: too many tokens or states");
+    // places and segments in 32 bits, a grid's threads below 2^32
+    const uint64_t heads = (uint64_t)n * d->h;
+    if (t >= (1u << 29) || n >= (1u << 22) || heads >= (1u << 22) || heads * t >= (1ull << 31) ||
+        heads * d->dk * d->dv >= (1ull << 31))
+        return rnn_fail(ctx, RNN_E_UNSUPPORTED, "decay_attn: too many tokens, heads or states");
     return RNN_OK;
 }
 

@@ -81,8 +81,13 @@ def test_decay_description_is_checked():
         with pytest.raises(ValueError):
             core._plan(2, 8, 0, (288, 0, 288, koff, None, voff))
     assert code(n=1 << 40) == R.RNN_E_UNSUPPORTED and code(t=1 << 40) == R.RNN_E_UNSUPPORTED
-    assert code(n=1, t=1 << 29) == R.RNN_E_UNSUPPORTED  # t h = 2^31
+    assert code(n=1, t=1 << 29) == R.RNN_E_UNSUPPORTED
+    assert code(n=2, t=1 << 28) == R.RNN_E_UNSUPPORTED  # n h t = 2^31
+    assert code(n=2, t=(1 << 28) - 1) == R.RNN_OK
     assert code(n=1 << 19, t=1) == R.RNN_E_UNSUPPORTED  # n h dk dv > 2^31
+    one = R.DecayCore(1, 1).desc(1, 0, 2, 0, 2, 1)
+    ws = lambda n: R.lib().rnn_decay_attn_workspace(C.byref(one), n, 1, 1, C.byref(nb))
+    assert ws((1 << 22) - 1) == R.RNN_OK and ws(1 << 22) == R.RNN_E_UNSUPPORTED
     assert R.lib().rnn_decay_attn_workspace(None, 1, 1, 0, C.byref(nb)) == R.RNN_E_NULL
 
 
