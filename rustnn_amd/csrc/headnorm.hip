@@ -11,6 +11,11 @@
 // that a wave reads whole lines; the next head's loads are in flight while one is
 // worked on.  Squares are summed in 64 bits: a square passes a float's range from
 // 2^64 on and falls below it from 2^-75.  So are the sums over lanes and rows.
+//
+// 25088 rows, where a copy of that size runs at 5.0 TB/s: norm and turn of 24 heads
+// of 64 channels 58 us forward (5.3 TB/s) and 104 us backward (4.5), 8 gated heads
+// of 64 channels 26 us (6.0: they stay in the last cache) and 48 (5.3), each
+// backward 5 us more for the gains' gradient.  64 rows take 6 us, a launch's least.
 #include "rotary_angle.h"
 
 #include <algorithm>
@@ -19,7 +24,7 @@ namespace {
 
 constexpr int MAX_HEAD = 256;      // channels of a head with rotary positions
 constexpr int MAX_GATE = 512;      // channels of a gated head
-constexpr int MAX_BLOCKS = 1280;   // of a forward: 5 a CU
+constexpr int MAX_BLOCKS = 1024;   // of a forward: 4 a CU
 constexpr int MAX_PARTS = 768;     // of a backward: 3 a CU, each leaving its part of dgain
 constexpr int TABLE = 512;         // sines and cosines of a block's rows
 
@@ -182,10 +187,12 @@ struct NrLane {
     }
 };
 
-// A block has `span` rows, of which it takes `rpb` at a time: their sines and cosines into LDS, formed
-// once for all heads, then every head.
+// A block has `span` rows, of which it takes `rpb` at a time: their sines and cosines
+// into LDS, formed once for all heads while the first heads' loads are in flight, then
+// every head.  Four blocks of a forward a CU: for five the loads ahead do not fit the
+// registers (25088 rows 64 us against 58, 8177 rows of 52 channels 18 against 12).
 template <bool INTER, bool BACK>
-__global__ __launch_bounds__(256, BACK ? 3 : 5) void norm_rotary_kernel(NrArgs g) {
+__global__ __launch_bounds__(256, BACK ? 3 : 4) void norm_rotary_kernel(NrArgs g) {
     __shared__ __attribute__((aligned(16))) float2 tab[TABLE];
     const int L = g.lanes, R = g.npairs;
     const int ng = 256 / L, grp = threadIdx.x / L;
@@ -208,8 +215,22 @@ __global__ __launch_bounds__(256, BACK ? 3 : 5) void norm_rotary_kernel(NrArgs g
     }
     const double inv = 1.0 / g.dh;
     const long long begin = (long long)blockIdx.x * g.span, end = min(begin + g.span, (long long)g.rows);
+    float v[8], d[8], nv[8], nd[8];
+    long long r, nr;
+    int hd, lr, nhd, nlr;
     for (long long row0 = begin; row0 < end; row0 += g.rpb) {
         const int nrow = (int)min((long long)g.rpb, end - row0);
+        // item `it` of the queries' (k = 0) or the keys' heads, into the next registers
+        const auto fetch = [&](int k, int it) {
+            const int hn = k ? g.h - g.hq : g.hq;
+            it = min(it, nrow * hn - 1);
+            nlr = it / hn;
+            nhd = it - nlr * hn + k * g.hq;
+            nr = row0 + nlr;
+            own.load(g.x + nr * g.xstride + nhd * g.dh, nv);
+            if constexpr (BACK) own.load(g.dy + nr * g.dystride + nhd * g.dh, nd);
+        };
+        fetch(g.hq ? 0 : 1, grp);
         __syncthreads();
         for (int e = threadIdx.x; e < nrow * R; e += 256) {
             const int lr = e / R, j = e - lr * R;
@@ -220,20 +241,7 @@ __global__ __launch_bounds__(256, BACK ? 3 : 5) void norm_rotary_kernel(NrArgs g
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < 2; k++) {
-            const int hn = k ? g.h - g.hq : g.hq, items = nrow * hn;
-            if (items == 0) continue;
-            float v[8], d[8], nv[8], nd[8];
-            long long r, nr;
-            int hd, lr, nhd, nlr;
-            auto fetch = [&](int it) {
-                it = min(it, items - 1);
-                nlr = it / hn;
-                nhd = it - nlr * hn + k * g.hq;
-                nr = row0 + nlr;
-                own.load(g.x + nr * g.xstride + nhd * g.dh, nv);
-                if constexpr (BACK) own.load(g.dy + nr * g.dystride + nhd * g.dh, nd);
-            };
-            fetch(grp);
+            const int items = nrow * (k ? g.h - g.hq : g.hq);
             for (int i0 = 0; i0 < items; i0 += ng) {
                 const bool live = i0 + grp < items;
                 r = nr, hd = nhd, lr = nlr;
@@ -242,7 +250,10 @@ __global__ __launch_bounds__(256, BACK ? 3 : 5) void norm_rotary_kernel(NrArgs g
                     v[e] = nv[e];
                     if constexpr (BACK) d[e] = nd[e];
                 }
-                if (i0 + ng < items) fetch(i0 + ng + grp);
+                if (i0 + ng < items)
+                    fetch(k, i0 + ng + grp);
+                else if (k == 0 && g.hq < g.h)
+                    fetch(1, grp);
                 double s = 0.0;
 #pragma unroll
                 for (int e = 0; e < 8; e++) s = fma((double)v[e], (double)v[e], s);
@@ -305,8 +316,7 @@ struct GateArgs {
 };
 
 // Block b: head b % h, rows (b / h) * groups + group, and every splits * groups
-// further, so that dgain's sums stay with one head's channels.  (Neighbouring
-// heads in one block, whole rows at a time, took no less: 2.1 to 2.4 TB/s.)
+// further, so that dgain's sums stay with one head's channels.
 template <bool BACK>
 __global__ __launch_bounds__(256) void head_gate_kernel(GateArgs g) {
     const int L = g.lanes, ng = 256 / L, at = threadIdx.x / L, u = threadIdx.x & (L - 1);
