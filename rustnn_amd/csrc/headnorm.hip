@@ -40,10 +40,10 @@ __device__ __forceinline__ double group_sum(double v, int L) {
 }
 
 // 1 / sqrt(v): the instruction's approximation, within 2^-23, and a Newton step on
-// it, which leaves 3/8 of its square: below 2^-46.
+// it, which leaves 3/8 of its square: below 2^-46.  0 of infinity.
 __device__ __forceinline__ double inv_sqrt(double v) {
-    const double r = __builtin_amdgcn_rsq(v);
-    return fma(0.5 * r, fma(-v * r, r, 1.0), r);
+    const double r = __builtin_amdgcn_rsq(v), s = fma(0.5 * r, fma(-v * r, r, 1.0), r);
+    return r == 0.0 ? r : s;
 }
 
 // 1 / (1 + exp(-z)), within 6.5 U (U = 2^-24).  exp(-z) as a power of two, its exponent
@@ -626,6 +626,7 @@ int rnn_head_gate_forward(rnn_ctx *ctx, size_t rows, size_t h, size_t d, float e
     if (rc) return rc;
     if (!rows) return RNN_OK;
     if (!x || !z || !y) return rnn_fail(ctx, RNN_E_NULL, "head_gate: null operand");
+    if (y == z + zoff) return rnn_fail(ctx, RNN_E_INVALID, "head_gate: y is the gate");
     RNN_ON_DEVICE(ctx);
     const GatePlan p = gate_plan(rows, h, d);
     GateArgs g = {x, z + zoff, gain, nullptr, y, nullptr, nullptr, (long long)zstride, 0, (long long)rows,
@@ -648,6 +649,10 @@ int rnn_head_gate_backward(rnn_ctx *ctx, size_t rows, size_t h, size_t d, float 
     if (!rows) return RNN_OK;
     if (!x || !z || !dy || !dx || !dz) return rnn_fail(ctx, RNN_E_NULL, "head_gate: null operand");
     if (!gain && dgain) return rnn_fail(ctx, RNN_E_NULL, "head_gate: dgain without gain");
+    if (dz == z && (dzstride != zstride || dzoff != zoff))
+        return rnn_fail(ctx, RNN_E_INVALID, "head_gate: in place with two layouts");
+    if (dx == z + zoff || dx == dz + dzoff || dz + dzoff == x || dz + dzoff == dy)
+        return rnn_fail(ctx, RNN_E_INVALID, "head_gate: a gradient is another operand");
     const GatePlan p = gate_plan(rows, h, d);
     rc = ws_checked(ctx, "head_gate", dgain ? p.parts * h * d * sizeof(double) : 0, ws, ws_bytes);
     if (rc) return rc;

@@ -94,6 +94,39 @@ def test_far_gates_and_large_heads(rnn):
     assert (dz.cpu()[0, :3].abs() <= 1e-36).all() and (dz.cpu()[0, 4:7] == 1).all()
 
 
+def test_numbers_that_are_none(rnn):
+    op, g = rnn.HeadGate(2, 12), torch.Generator().manual_seed(7)
+    x, z = (torch.randn(3, 24, generator=g).cuda() for _ in range(2))
+    clean = op.forward(3, x, z, 24).view(3, 2, 12)
+    nan, inf = float("nan"), float("inf")
+    for v in (nan, inf):
+        bad = x.clone()
+        bad[1, 15] = v
+        y = op.forward(3, bad, z, 24).view(3, 2, 12)
+        assert torch.equal(y[::2], clean[::2]) and torch.equal(y[1, 0], clean[1, 0])
+        rest = torch.cat([y[1, 1, :3], y[1, 1, 4:]])
+        assert torch.isnan(y[1, 1, 3]) and (torch.isnan(rest).all() if v != v else (rest == 0).all())
+        bad = z.clone()
+        bad[1, 15] = v
+        y = op.forward(3, x, bad, 24).view(3, 2, 12)
+        assert not torch.isfinite(y[1, 1, 3])
+        y[1, 1, 3] = clean[1, 1, 3]
+        assert torch.equal(y, clean)
+
+
+def test_offsets_past_32_bits(rnn):
+    """Gates in 2200 rows of 2^21 floats."""
+    op, wide, g = rnn.HeadGate(2, 12), 1 << 21, torch.Generator().manual_seed(8)
+    x, z, dy = (torch.randn(2200, 24, generator=g).cuda() for _ in range(3))
+    Z = torch.empty(2200, wide, device="cuda")
+    Z[:, -24:] = z
+    dz = torch.empty_like(z)
+    dx = op.backward(2200, x, z, 24, 0, None, dy, dz, 24)
+    assert torch.equal(op.forward(2200, x, Z, wide, wide - 24), op.forward(2200, x, z, 24))
+    assert torch.equal(op.backward(2200, x, Z, wide, wide - 24, None, dy, Z, wide, wide - 24), dx)
+    assert torch.equal(Z[:, -24:], dz)
+
+
 def test_gradient_against_differences(rnn):
     """As for head norms with rotary positions: within 1e-3 of the change."""
     op = rnn.HeadGate(3, 40)
@@ -130,4 +163,11 @@ def test_refusals(rnn):
         op.backward(10, x, z, 128, 0, None, x, z.clone(), 128, 0, torch.zeros(64, device="cuda"))
     with pytest.raises(rnn.RnnError):
         op.backward(10, x, z, 128, 0, None, x, z.clone(), 60)
+    with pytest.raises(rnn.RnnError):
+        op.forward(10, x, z, 128, y=z)
+    with pytest.raises(rnn.RnnError):  # in place with two layouts
+        op.backward(10, x, z, 128, 0, None, x.clone(), z, 128, 64)
+    for dx in (z, x):
+        with pytest.raises(rnn.RnnError):
+            op.backward(10, x, z, 128, 0, None, x.clone(), x if dx is x else dx, 64, dx=dx)
     assert op.forward(0, x, z, 128).shape == (0, 64)

@@ -185,6 +185,36 @@ def test_not_a_number_stays_in_its_head(rnn):
     assert torch.equal(y[keep.cuda()], clean.view(8, 6, 32)[keep.cuda()])
 
 
+def test_an_infinity_leaves_zeros_in_its_head(rnn):
+    """As the formula has it: NaN in its own pair, x / infinity in the others."""
+    op = rnn.NormRotary(1, 1, 32, (8,), 100.0, (12,))
+    x = torch.randn(1, 8, 64).cuda()
+    for ch, pair in ((5, (5, 17)), (17, (5, 17)), (30, (30,))):
+        bad = x.clone()
+        bad[0, 3, 32 + ch] = -float("inf")
+        y = op.forward(1, bad, 64).view(8, 2, 32)[3, 1].cpu()
+        shows = torch.zeros(32, dtype=torch.bool)
+        shows[list(pair)] = True
+        assert torch.isnan(y[shows]).all() and (y[~shows] == 0).all()
+
+
+def test_offsets_past_32_bits(rnn):
+    """2200 rows of 2^21 floats."""
+    op, wide = rnn.NormRotary(2, 1, 16, (2200,), 100.0), 1 << 21
+    x, dy, gain = torch.randn(2200, 48).cuda(), torch.randn(2200, 48).cuda(), torch.randn(2, 16).cuda()
+    X = torch.empty(2200, wide, device="cuda")
+    X[:, -48:] = x
+    y = op.forward(1, x, 48, 0, gain)
+    dg = [torch.zeros_like(gain) for _ in range(2)]
+    dx = op.backward(1, x, 48, 0, gain, dy, 48, 0, dg[0])
+    DX = torch.empty_like(X)
+    op.backward(1, X, wide, wide - 48, gain, dy, 48, 0, dg[1], dx=DX, dxstride=wide,
+                dxoff=wide - 48)
+    assert torch.equal(DX[:, -48:], dx[0]) and torch.equal(dg[0], dg[1])
+    op.forward(1, X, wide, wide - 48, gain, y=X)
+    assert torch.equal(X[:, -48:], y[0])
+
+
 def test_gradient_against_differences(rnn):
     """A step along the gradient, central: the outputs' rounding over the step
     (8 U sqrt of the elements over 2^-9) and the third order, 2^-18 of it, stay
