@@ -292,7 +292,9 @@ int rnn_norm_rotary_backward(rnn_ctx *ctx, const rnn_rotary_desc *d, uint32_t hq
  * of h heads of d channels, x and y [rows][h][d], z at z + r*zstride + zoff.
  *   y = gain x / sqrt(mean(x^2) + eps) z / (1 + exp(-z))
  * gain [h][d] (NULL: 1); the mean is a head's.  d <= 512, h <= 65536, eps > 0.  y
- * may be x. */
+ * may be x and overlaps nothing else.  A NaN in x gives NaN in its head, an infinity
+ * NaN in its channel and zeros in the others of its head; either in z stays in its
+ * channel. */
 int rnn_head_gate_forward(rnn_ctx *ctx, size_t rows, size_t h, size_t d, float eps, const float *x,
                           const float *z, size_t zstride, size_t zoff, const float *gain, float *y);
 /* Bytes of device workspace that a backward with dgain needs, as
@@ -300,7 +302,7 @@ int rnn_head_gate_forward(rnn_ctx *ctx, size_t rows, size_t h, size_t d, float e
 int rnn_head_gate_workspace(size_t rows, size_t h, size_t d, size_t *bytes);
 /* Its backward: dx [rows][h][d] and dz (at dz + r*dzstride + dzoff) are
  * overwritten, dgain [h][d] (NULL: not wanted) accumulates in a fixed order.  dx
- * may be dy or x, dz may be z where their layouts agree. */
+ * may be dy or x, dz may be z where their layouts agree; they overlap nothing else. */
 int rnn_head_gate_backward(rnn_ctx *ctx, size_t rows, size_t h, size_t d, float eps, const float *x,
                            const float *z, size_t zstride, size_t zoff, const float *gain,
                            const float *dy, void *ws, size_t ws_bytes, float *dx, float *dz,
@@ -337,7 +339,7 @@ typedef struct {
  * n * h * dk * dv < 2^31 (RNN_E_UNSUPPORTED above), scale finite. */
 int rnn_decay_attn_workspace(const rnn_decay_attn_desc *d, size_t n, size_t t, int backward,
                              size_t *bytes);
-/* y [n][t][h][dv]. */
+/* y [n][t][h][dv], which overlaps no operand. */
 int rnn_decay_attn_forward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n, size_t t,
                            const float *q, const float *k, const float *v, const float *rate,
                            const uint32_t *lens, const float *state_in, void *ws, size_t ws_bytes,

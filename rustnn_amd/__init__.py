@@ -1003,6 +1003,8 @@ class NormRotary:
                 raise ValueError(f"NormRotary: {lib().rnn_status_string(rc).decode()} (hq={self.hq} "
                                  f"hk={self.hk} dh={self.dh} grid={self.rot.grid} eps={self.eps} "
                                  f"n={n} t={t} layout={layout})")
+            if len(self._ws) >= 4096:  # sizes come and go
+                self._ws.clear()
             nb = self._ws[n, t, have_pos, layout] = out.value
         return d, nb
 
@@ -1199,6 +1201,8 @@ class HeadGate:
             if rc:
                 raise ValueError(f"HeadGate: {lib().rnn_status_string(rc).decode()} (rows={rows} "
                                  f"h={self.h} d={self.d})")
+            if len(self._ws) >= 4096:  # sizes come and go
+                self._ws.clear()
             nb = self._ws[rows] = out.value
         return nb
 

@@ -66,7 +66,8 @@ struct DecayArgs {
     Divider segs, heads;
 };
 
-// log gamma of a head: at most 0, and finite, so that its multiple by 0 is 0.
+// log gamma of a head: at most 0, and finite, so that its multiple by 0 is 0 (of a
+// rate that is no number NaN).
 __device__ __forceinline__ double log_gamma(float rate) {
     const double g = -exp((double)rate);
     return g < -1e30 ? -1e30 : g;
@@ -77,7 +78,7 @@ __device__ __forceinline__ double log_gamma(float rate) {
 struct Power {
     float hi, lo;
     __device__ __forceinline__ explicit Power(double lg) {
-        const double l2 = fmax(lg, -1e30) * 1.4426950408889634;
+        const double l2 = lg * 1.4426950408889634;
         hi = (float)l2;
         lo = (float)(l2 - (double)hi);
     }
@@ -809,6 +810,8 @@ int rnn_decay_attn_forward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n,
     if (rc) return rc;
     if (!n || (!t && !state_out)) return RNN_OK;
     if ((t && (!q || !k || !v || !y)) || !rate) return rnn_fail(ctx, RNN_E_NULL, "decay_attn_forward: null operand");
+    if (t && (y == q + d->qoff || y == k + d->koff || y == v + d->voff))
+        return rnn_fail(ctx, RNN_E_INVALID, "decay_attn_forward: y is an operand");
     const DecayPlan w = plan_of(d, n, t, false);
     rc = check_ws(ctx, w, ws, ws_bytes);
     if (rc) return rc;
@@ -865,6 +868,9 @@ int rnn_decay_attn_backward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n
         return rnn_fail(ctx, RNN_E_NULL, "decay_attn_backward: null operand");
     if (dstate_in && (dstate_in == dstate_out || dstate_in == state_in))
         return rnn_fail(ctx, RNN_E_INVALID, "decay_attn_backward: dstate_in is an operand");
+    if (t && (dq == q || dk == k || dv == v || dq + d->qoff == dy || dk + d->koff == dy ||
+              dv + d->voff == dy))
+        return rnn_fail(ctx, RNN_E_INVALID, "decay_attn_backward: a gradient is an operand");
     const DecayPlan w = plan_of(d, n, t, true);
     rc = check_ws(ctx, w, ws, ws_bytes);
     if (rc) return rc;

@@ -18,8 +18,8 @@ from __future__ import annotations
 
 import numpy as np
 
-from . import (Core, DecayCore, DiffCore, HeadGate, Linear, NormRotary, Rotary, _ptr, default_ctx, lib, linear_backward,
-               linear_forward, rel_index)
+from . import (Core, DecayCore, DiffCore, HeadGate, Linear, NormRotary, Rotary, _ptr, default_ctx,
+               lib, linear_backward, linear_forward, rel_index)
 from .data import Rng
 from .norm import DwConv3, LayerNorm, LayerScale, Mlp, SeqPool, SwiGlu, _linear_param
 from .optim import Param
@@ -173,7 +173,6 @@ class DiffSelfAttn:
             f(p)
         f(self.lam)
         f(self.gain)
-
 
 
 class DecaySelfAttn:

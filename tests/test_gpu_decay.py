@@ -16,6 +16,8 @@ CASES = [
     ("one_token_heads", dict(n=3, t=1, h=4, hkv=2, dk=64, dv=64, reverse=1)),
     ("two", dict(n=2, t=2, h=2, hkv=2, dk=8, dv=8)),
     ("few", dict(n=2, t=7, h=4, hkv=4, dk=32, dv=64, reverse=2)),
+    ("few_ragged", dict(n=4, t=5, h=4, hkv=2, dk=24, dv=40, reverse=2, lens=[5, 0, 1, 3])),
+    ("eight", dict(n=2, t=8, h=4, hkv=2, dk=40, dv=36, reverse=2)),
     ("nine", dict(n=2, t=9, h=2, hkv=1, dk=33, dv=31, state=False)),
     ("a_tile", dict(n=2, t=32, h=2, hkv=2, dk=32, dv=32, reverse=1)),
     ("past_a_tile", dict(n=1, t=33, h=2, hkv=2, dk=64, dv=32, reverse=1)),
@@ -168,6 +170,60 @@ def test_extreme_rates(rnn, t):
     assert (got["drate"] == 0).all()
 
 
+@pytest.mark.parametrize("t", [1, 5, 40, 300])
+def test_a_rate_that_is_no_number_shows_in_its_head(rnn, t):
+    cs = DecayCase(2, t, 3, 3, 16, 16, seed=7)
+    clean = run(rnn, cs)
+    cs.rate[1] = float("nan")
+    got = run(rnn, cs)
+    for nm in ("y", "dq", "dk", "dv"):
+        a, b = (v[nm].view(2, t, 3, 16) for v in (got, clean))
+        assert torch.isnan(a[:, :, 1]).all(), nm
+        assert torch.equal(a[:, :, ::2], b[:, :, ::2]), nm
+    for nm in ("state", "dstate"):
+        assert torch.isnan(got[nm][:, 1]).all() and torch.equal(got[nm][:, ::2], clean[nm][:, ::2])
+    assert torch.isnan(got["drate"][1]) and torch.equal(got["drate"][::2], clean["drate"][::2])
+
+
+@pytest.mark.parametrize("t", [3, 70])
+def test_values_in_a_buffer_of_their_own(rnn, t):
+    """The same bits as from one buffer, and gradients in two."""
+    cs = DecayCase(2, t, 4, 2, 24, 40, reverse=1, seed=11, lens=[t, t // 2])
+    full, kv, rate, st = run(rnn, cs), cs.kv.cuda(), cs.rate.cuda(), cs.state.cuda()
+    core, lens = rnn.DecayCore(4, 24, 40, 2, reverse=1), cs.lens.cuda()
+    v = torch.full((2, t, 100), 7.0).cuda()
+    v[..., 3:83] = kv[..., cs.voff:cs.voff + 80]
+    qk = kv[..., :cs.voff].contiguous()
+    geo = (qk, cs.voff, 0, qk, cs.voff, cs.koff, 3)
+    y, out = core.forward(2, t, *geo, rate, lens=lens, state=st, keep_state=True, v=v, vstride=100)
+    assert torch.equal(y, full["y"]) and torch.equal(out, full["state"])
+    dqk, dv, drate = torch.empty_like(qk), torch.full_like(v, 7.0), torch.zeros_like(rate)
+    core.backward(2, t, *geo, rate, cs.dy.cuda(), dqk, dqk, drate, lens=lens, state=st,
+                  dstate_out=cs.dstate.cuda(), set_dq=True, set_dkv=True, v=v, vstride=100, dv=dv)
+    assert torch.equal(dqk[..., :cs.qw], full["dq"])
+    assert torch.equal(dqk[..., cs.koff:cs.koff + cs.kw], full["dk"])
+    assert torch.equal(dv[..., 3:83], full["dv"]) and torch.equal(drate, full["drate"])
+    assert (dv[..., :3] == 7).all() and (dv[..., 83:] == 7).all()
+
+
+@pytest.mark.parametrize("n,t", [(1, 300), (75, 4)])
+def test_offsets_past_32_bits(rnn, n, t):
+    """Rows of 2^22 floats, the most that there may be: 300 of them take 5 GB."""
+    cs = DecayCase(n, t, 2, 1, 24, 40, reverse=1, seed=12, rates=(-5.0, -3.0))
+    full, wide = run(rnn, cs), 1 << 22
+    x = torch.empty(n, t, wide, device="cuda")
+    off = wide - cs.kvstride
+    x[..., off:] = cs.kv.cuda()
+    geo = (x, wide, off, x, wide, off + cs.koff, off + cs.voff)
+    core, rate, st = rnn.DecayCore(2, 24, 40, 1, reverse=1), cs.rate.cuda(), cs.state.cuda()
+    y, out = core.forward(n, t, *geo, rate, state=st, keep_state=True)
+    assert torch.equal(y, full["y"]) and torch.equal(out, full["state"])
+    dx, drate = torch.empty_like(x), torch.zeros_like(rate)
+    core.backward(n, t, *geo, rate, cs.dy.cuda(), dx, dx, drate, state=st,
+                  dstate_out=cs.dstate.cuda(), set_dq=True, set_dkv=True)
+    assert torch.equal(dx[..., off:], full["rest"][0]) and torch.equal(drate, full["drate"])
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 @pytest.mark.parametrize("reverse", [0, 1])
 @pytest.mark.parametrize("t,at", [(6, 3), (100, 37), (100, 64), (700, 600)])
@@ -261,6 +317,11 @@ def test_refusals(rnn):
     with pytest.raises(rnn.RnnError):
         core.backward(2, 10, *geo, rate, y, torch.empty_like(x), torch.empty_like(x), state=st,
                       dstate_out=st, dstate=st)
+    with pytest.raises(rnn.RnnError):  # y over the queries, a gradient over its operand
+        core.forward(2, 10, *geo, rate, y=x)
+    for dq, dkv, dy in ((x, x.clone(), y), (x.clone(), x, y), (x.clone(), x.clone(), None)):
+        with pytest.raises(rnn.RnnError):
+            core.backward(2, 10, *geo, rate, dq if dy is None else dy, dq, dkv)
     assert core.forward(0, 10, *geo, rate)[0].shape == (0, 10, 96)
     # no tokens: the state passes through
     st = torch.randn(2, 4, 16, 24, device="cuda")
