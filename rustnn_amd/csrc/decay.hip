@@ -22,6 +22,7 @@ namespace {
 
 constexpr int MAX_D = 128;
 constexpr int C = 32;  // tokens of a chunk
+constexpr size_t SIMDS = 1024;  // four of each of 256 compute units
 
 // Division of numbers below 2^31 by d: (mulhi(x, m) + x) >> s.
 struct Divider {
@@ -62,8 +63,28 @@ struct DecayArgs {
     const uint32_t *lens;
     double *part;  // [n][nseg][slices][h] parts of dL/dg
     int n, t, h, reverse;
-    int nseg, slen;  // segments of a sequence, and their tokens
+    int nseg;  // segments of a sequence
     Divider segs, heads;
+};
+
+__device__ __forceinline__ int length(const DecayArgs &g, long long b) {
+    return g.lens ? (int)min(g.lens[b], (uint32_t)g.t) : g.t;
+}
+
+// A sequence's segments: its chunks in as many runs, the first ones a chunk longer
+// where they do not divide; a run is of rows, whatever a head's direction.
+struct Segments {
+    int len, longer, each;  // tokens, runs of each + 1 chunks, chunks
+    __device__ __forceinline__ Segments(const DecayArgs &g, int tokens) : len(tokens) {
+        uint32_t rest;
+        each = (int)g.segs((uint32_t)(len + C - 1) / C, rest);
+        longer = (int)rest;
+    }
+    __device__ __forceinline__ int first(int k) const {
+        return min(C * (k * each + min(k, longer)), len);
+    }
+    // the last one that holds tokens; 0 if none does
+    __device__ __forceinline__ int last(int nseg) const { return max(each ? nseg : longer, 1) - 1; }
 };
 
 // log gamma of a head: at most 0, and finite, so that its multiple by 0 is 0 (of a
@@ -123,7 +144,7 @@ __global__ __launch_bounds__(256) void decay_tokens_kernel(DecayArgs g) {
                 for (int e = 0; e < 4; e++) s[k][e] = c4 + e < q.dc ? q.s0[at + e] : 0.f;
             }
         });
-    const int len = g.lens ? (int)min(g.lens[b], (uint32_t)g.t) : g.t;
+    const int len = length(g, b);
     const bool back = hd >= g.h - g.reverse;
     // gamma in two floats: one rounded alone would be off by its last bit to
     // the power of the tokens
@@ -344,6 +365,14 @@ enum { WALK = 0, WALK_RATE = 1, STATE = 2 };
 // tokens through the wave's own LDS.  A wave shares nothing with another one and
 // waits for none.  WALK_RATE: the rates' gradient as well.  STATE: the segment's
 // own T alone.
+//
+// Bound by the fp32 products, 16 + 48 DAT of 64 cycles a chunk (32 + 80 DAT with the
+// rates): one wave a SIMD takes 4.5 us a chunk of 64 x 64 heads, 65 % of their rate at
+// 2.4 GHz, two as much for each.  (Measured and not better: rows shared by a block's
+// waves through LDS with barriers, products and other instructions interleaved by
+// hand.)  8 clips of 1568 tokens, 8 heads of 64: forward 36
+// us and 23 for the states between segments, dq and the rates 67, dk and dv 64, their
+// states 34; 128 images of 64 tokens, 4 heads: 15, 21 and 22.
 template <int DAT, bool FULL, int MODE>
 __global__ __launch_bounds__(256, DAT <= (MODE == WALK_RATE ? 1 : 2) ? 2 : 1) void decay_walk_kernel(DecayArgs g) {
     // rows of b: 4 rows apart are half of the banks apart
@@ -352,8 +381,8 @@ __global__ __launch_bounds__(256, DAT <= (MODE == WALK_RATE ? 1 : 2) ? 2 : 1) vo
     __shared__ __attribute__((aligned(16))) float btile[MODE == STATE ? 1 : 4][MODE == STATE ? 4 : C * BS];
     const DecayJob &q = g.job[blockIdx.y];
     const int lane = threadIdx.x & 63, ln = lane & 31, half = 4 * (lane >> 5), wave = wave_index();
-    // the arguments at once: loaded one after the other as they are needed, their
-    // misses took 5000 cycles
+    // the arguments at once, not one after the other as they are needed (128 x 64
+    // tokens 15.4 us against 14.9)
     asm volatile("" ::"s"(q.a), "s"(q.b), "s"(q.c), "s"(q.y), "s"(q.s0), "s"(q.as), "s"(q.bs), "s"(q.cs),
                  "s"(q.ys), "s"(q.da), "s"(q.ga), "s"(q.sa), "s"(q.rev), "s"(g.rate));
     uint32_t u = (uint32_t)xcd_order(blockIdx.x, gridDim.x) * 4 + wave, rest;  // fewer than 2^31 waves
@@ -364,15 +393,16 @@ __global__ __launch_bounds__(256, DAT <= (MODE == WALK_RATE ? 1 : 2) ? 2 : 1) vo
     const long long b = g.heads(u, rest);
     const int hd = (int)rest;
     if (b >= g.n) return;
-    const int len = __builtin_amdgcn_readfirstlane(g.lens ? (int)min(g.lens[b], (uint32_t)g.t) : g.t);
-    const int t0 = seg * g.slen, t1 = min(t0 + g.slen, len), T = max(t1 - t0, 0);
-    const bool lastseg = len > 0 ? t0 < len && t1 == len : seg == 0;
+    const Segments runs(g, __builtin_amdgcn_readfirstlane(length(g, b)));
+    const int t0 = runs.first(seg), t1 = runs.first(seg + 1), T = t1 - t0;
+    const bool lastseg = seg == runs.last(g.nseg);
     constexpr bool slope = MODE == WALK_RATE;
     const int e0 = q.rev ? 0 : 1;
     const bool incol = col < q.dc;
-    if (MODE != STATE && !q.acc) {  // padding rows
-        const int z1 = (int)min((long long)t0 + g.slen, (long long)g.t);
-        for (int i = max(t0, len) + (lane >> 5); i < z1; i += 2)
+    if (MODE != STATE && !q.acc && runs.len < g.t) {  // padding rows, shared among the runs
+        const int pad = g.t - runs.len, each = (pad + g.nseg - 1) / g.nseg;
+        const int z0 = min(seg * each, pad), z1 = min(z0 + each, pad);
+        for (int i = runs.len + z0 + (lane >> 5); i < runs.len + z1; i += 2)
             if (incol) q.y[(b * g.t + i) * q.ys + hd * q.dc + col] = 0.f;
     }
     Powers &pw = tables[wave];
@@ -380,7 +410,6 @@ __global__ __launch_bounds__(256, DAT <= (MODE == WALK_RATE ? 1 : 2) ? 2 : 1) vo
     double dg = 0.0;
     const long long st = (b * g.h + hd) * q.da * q.dc;
     const long long sg = ((long long)seg * g.n * g.h) * q.da * q.dc + st;
-    // segments are rows' whatever the walk's direction
     const bool down = (hd >= g.h - g.reverse) != (q.rev != 0);
     const Walk w = {b * g.t + (down ? t1 - 1 : t0), down ? -1 : 1};
     const bool ends = down ? seg == 0 : lastseg;    // holds the walk's last token
@@ -575,16 +604,19 @@ __global__ __launch_bounds__(256) void decay_scan_kernel(DecayArgs g) {
     if (i >= all) return;
     const int hd = (int)(i / per % g.h);
     const long long b = i / per / g.h;
-    const int len = g.lens ? (int)min(g.lens[b], (uint32_t)g.t) : g.t;
-    const int last = len > 0 ? (len - 1) / g.slen : 0;
+    const Segments runs(g, length(g, b));
+    const int last = runs.last(g.nseg);
     const double lg = log_gamma(g.rate[hd]);
-    double all64 = exp(lg * g.slen);
-    const float hi = (float)all64, lo = (float)(all64 - (double)hi);
     float s = q.s0 ? q.s0[i] : 0.f;
     const bool down = (hd >= g.h - g.reverse) != (q.rev != 0);
-    // from the far end the first segment may be short
-    all64 = exp(lg * (len - last * g.slen));
-    const float hi1 = (float)all64, lo1 = (float)(all64 - (double)hi1);
+    // gamma to the tokens of a run: the last one's, a longer and another one's
+    float hi[3], lo[3];
+#pragma unroll
+    for (int j = 0; j < 3; j++) {
+        const double all64 = exp(lg * (j ? C * (runs.each + (j == 1)) : runs.len - runs.first(last)));
+        hi[j] = (float)all64;
+        lo[j] = (float)(all64 - (double)hi[j]);
+    }
     // the k-th segment of the walk, eight of them loaded ahead of their stores; the
     // last one's own state has no reader
     for (int k0 = 0; k0 <= last; k0 += 8) {
@@ -598,8 +630,12 @@ __global__ __launch_bounds__(256) void decay_scan_kernel(DecayArgs g) {
         for (int j = 0; j < 8; j++) {
             const int k = k0 + j;
             if (k > last) break;
-            q.seg[(long long)(down ? last - k : k) * all + i] = s;
-            s = (down && k == 0 ? decayed(s, hi1, lo1) : decayed(s, hi, lo)) + own[j];
+            const int run = down ? last - k : k;
+            q.seg[(long long)run * all + i] = s;
+            s = (run == last          ? decayed(s, hi[0], lo[0])
+                 : run < runs.longer ? decayed(s, hi[1], lo[1])
+                                     : decayed(s, hi[2], lo[2])) +
+                own[j];
         }
     }
 }
@@ -646,28 +682,37 @@ __global__ __launch_bounds__(256) void decay_rate_kernel(const double *part, int
 // The form's walks over a sequence, and where a workspace's parts are.
 struct DecayPlan {
     bool tokens = false;  // token by token
-    int nseg = 1, slen = 1;
+    int nseg = 1;
     size_t seg = 0, segr = 0, part = 0, part_k = 0, part_v = 0, bytes = 0;
 };
+// Segments of a walk of so many chunks by so many waves: a wave a SIMD, two of a
+// forward whose registers leave room (two) and that keep four chunks each.  They cost
+// a pass for the states, which are written, scanned and read, and pay where the
+// chunks that a walk is spared come to more; in sixths of a chunk's time.  Four heads of
+// 64 channels, us without / with them: one image of 64 tokens 12 / 16 forward and 31 /
+// 41 backward, of 128 tokens 21 / 17 and 56 / 42; 64 sequences of 256 tokens 42 / 47 and
+// 112 / 125, of 2048 tokens 320 / 230 and 821 / 661; 8 of 1024 tokens 149 / 31 and 407 /
+// 81 (half and twice as many segments: 40, 36 and 94, 104).
+size_t segments(size_t waves, size_t chunks, bool two, bool backward) {
+    size_t k = SIMDS / waves;
+    if (k < 2 || chunks < 2) return 1;  // 800 waves, 32 chunks: 106 us, in two 128
+    if (two && chunks >= 4 * (2 * SIMDS / waves)) k = 2 * SIMDS / waves;
+    // the scan takes them one after the other: beyond 64, two chunks each
+    k = std::min(k, std::min(chunks, std::max<size_t>(64, chunks / 2)));
+    const size_t each = rnn_div_up(chunks, k);
+    return 6 * (chunks - each) > 10 + 2 * each + (backward ? 11 : 9) * (waves * k) / SIMDS ? k : 1;
+}
 DecayPlan plan_of(const rnn_decay_attn_desc *d, size_t n, size_t t, bool backward) {
     DecayPlan p;
     WsCarve c;
-    // few tokens: the state's read and write are all there is to do
+    // Few tokens: the state's read and write are all there is to do.  (Us with 1, 4, 8
+    // and 12 tokens, by the walk: 64 streams of 8 heads of 64 x 128 17, 17, 18, 18, one of
+    // 4 heads of 64 x 64 9 throughout; token by token 9, 12, 17, 22 and 4, 7, 10, 13.)
     p.tokens = !backward && t <= 8;
     const size_t kt = rnn_div_up(d->dk, 32), vt = rnn_div_up(d->dv, 32);
     // the waves of the walk with the fewest
-    const size_t waves = backward ? n * d->h * kt : n * d->h * vt;
-    p.slen = (int)rnn_round_up(std::max<size_t>(t, 1), C);
-    // Segments where that leaves compute units idle, a chunk at the least: up to two
-    // waves a SIMD of a forward, one of a backward, whose walk for dq and the rates
-    // holds half of a SIMD's registers.  (Us a pass, 1024 / 2048 waves: a prompt of
-    // 16384 tokens 137 / 130, training on 8 x 1568 tokens 240 / 290; at least 32 / 64
-    // / 128 tokens a segment: training on 5 x 577 with shared heads 198 / 257 / 378.)
-    if (!p.tokens && waves && waves < 1024 && t >= 2 * C) {
-        const size_t want = std::min(rnn_div_up(backward ? 1024 : 2048, waves), t / C);
-        p.slen = (int)rnn_round_up(rnn_div_up(t, std::max<size_t>(want, 1)), C);
-        p.nseg = (int)rnn_div_up(t, p.slen);
-    }
+    const size_t waves = n * d->h * (backward ? std::min(kt, vt) : vt);
+    if (!p.tokens && waves) p.nseg = (int)segments(waves, rnn_div_up(t, C), !backward && kt <= 2, backward);
     const size_t states = (size_t)p.nseg * n * d->h * d->dk * d->dv * sizeof(float);
     if (p.nseg > 1) {
         p.seg = c.take(states);
@@ -745,7 +790,6 @@ DecayJob make_job(const Operand &a, const Operand &b, int da, const Operand &c, 
 void fill_args(DecayArgs &g, const rnn_decay_attn_desc *d, const DecayPlan &p, size_t n, size_t t,
                const float *rate, const uint32_t *lens) {
     g.nseg = p.nseg;
-    g.slen = p.slen;
     g.segs = Divider((uint32_t)p.nseg);
     g.heads = Divider(d->h);
     g.rate = rate;
