@@ -118,7 +118,9 @@ __device__ __forceinline__ float decayed(float s, float gam, float rest) {
 // Token by token, forward: a block holds a head's state, four channels of v a
 // thread in every RP-th row, RP = 256 / G, G groups of four channels (a power of
 // two).  Its read and write are the work: 16 bytes an access (VEC: dv a multiple of
-// four, states aligned), all of them in flight at once.
+// four, states aligned), all of them in flight at once: 64 streams of 8 heads of 64 x
+// 128 8.6 us, 3.9 TB/s; one of 4 heads of 64 x 64 4.0, a launch's least.  (Four bytes an
+// access: 16.3.)
 template <bool VEC, int G>
 __global__ __launch_bounds__(256) void decay_tokens_kernel(DecayArgs g) {
     constexpr int RP = 256 / G, K = MAX_D / RP;
@@ -596,19 +598,34 @@ __global__ __launch_bounds__(256, DAT <= (MODE == WALK_RATE ? 1 : 2) ? 2 : 1) vo
 }
 
 // The states before each segment, in the walk's direction, from the segments' own
-// ones: one thread an element, over the segments in order.
-__global__ __launch_bounds__(256) void decay_scan_kernel(DecayArgs g) {
+// ones: one thread an element, over the segments in order.  A block's
+// elements are one head's, so that lengths and factors are the same for all of them.
+// Bound by the chain of loads: 64 segments of 8 heads of 64 x 128 11 us (3.0 TB/s; 16
+// ahead 12.5, without the eight ahead 14), 8 of 64 of 64 x 64 6.3 (2.7).
+__global__ __launch_bounds__(256) void decay_scan_kernel(DecayArgs g, int blocks) {
     const DecayJob &q = g.job[blockIdx.y];
-    const long long per = (long long)q.da * q.dc, all = (long long)g.n * g.h * per;
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= all) return;
-    const int hd = (int)(i / per % g.h);
-    const long long b = i / per / g.h;
+    // `blocks` of them a head of a sequence
+    const int per = q.da * q.dc, head = blockIdx.x / blocks;
+    const int at = (int)(blockIdx.x - head * blocks) * 256 + threadIdx.x;
+    const int b = head / g.h, hd = head - b * g.h;
     const Segments runs(g, length(g, b));
     const int last = runs.last(g.nseg);
-    const double lg = log_gamma(g.rate[hd]);
-    float s = q.s0 ? q.s0[i] : 0.f;
     const bool down = (hd >= g.h - g.reverse) != (q.rev != 0);
+    if (at >= per) return;
+    const long long all = (long long)g.n * g.h * per, i = (long long)head * per + at;
+    float s = q.s0 ? q.s0[i] : 0.f;
+    // the k-th segment of the walk, eight of them loaded while the eight before are
+    // worked on; the last one's own state has no reader
+    float own[8], next[8];
+    const auto fetch = [&](int k0) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int k = min(k0 + j, last);
+            next[j] = q.seg[(long long)(down ? last - k : k) * all + i];
+        }
+    };
+    fetch(0);
+    const double lg = log_gamma(g.rate[hd]);
     // gamma to the tokens of a run: the last one's, a longer and another one's
     float hi[3], lo[3];
 #pragma unroll
@@ -617,31 +634,27 @@ __global__ __launch_bounds__(256) void decay_scan_kernel(DecayArgs g) {
         hi[j] = (float)all64;
         lo[j] = (float)(all64 - (double)hi[j]);
     }
-    // the k-th segment of the walk, eight of them loaded ahead of their stores; the
-    // last one's own state has no reader
     for (int k0 = 0; k0 <= last; k0 += 8) {
-        float own[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const int k = k0 + j;
-            own[j] = k < last ? q.seg[(long long)(down ? last - k : k) * all + i] : 0.f;
-        }
+        for (int j = 0; j < 8; j++) own[j] = next[j];
+        if (k0 + 8 <= last) fetch(k0 + 8);
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const int k = k0 + j;
             if (k > last) break;
             const int run = down ? last - k : k;
             q.seg[(long long)run * all + i] = s;
-            s = (run == last          ? decayed(s, hi[0], lo[0])
-                 : run < runs.longer ? decayed(s, hi[1], lo[1])
-                                     : decayed(s, hi[2], lo[2])) +
-                own[j];
+            const int len = run == last ? 0 : run < runs.longer ? 1 : 2;
+            s = decayed(s, hi[len], lo[len]) + own[j];
         }
     }
 }
 
 // dk and dv of shared heads: the sum over the query heads' parts, in order.  Rows
 // behind a sequence's end hold zeros, and stay as they are where dkv accumulates.
+// (5 x 577 tokens, two key heads of 44 + 72 channels for three query heads each: 5 us,
+// for which the query heads' walks run side by side; one after the other in a wave, all
+// of this training pass took 378 us against 150.)
 struct GroupArgs {
     const float *part[2];
     float *out[2];
@@ -665,7 +678,7 @@ __global__ __launch_bounds__(256) void decay_group_kernel(GroupArgs g, long long
     }
 }
 
-// drate[j] += g sum of the head's parts, in a fixed order.
+// drate[j] += g sum of the head's parts, in a fixed order (4 us, a launch's least).
 __global__ __launch_bounds__(256) void decay_rate_kernel(const double *part, int rows, int h,
                                                          const float *rate, float *drate) {
     __shared__ double red[4];
@@ -827,8 +840,8 @@ void launch_walk(rnn_ctx *ctx, const DecayArgs &g, int jobs) {
 // The states between segments: every segment's own, then over the segments.
 void launch_segments(rnn_ctx *ctx, const DecayArgs &g, int jobs) {
     launch_walk<STATE>(ctx, g, jobs);
-    const size_t all = (size_t)g.n * g.h * g.job[0].da * g.job[0].dc;
-    decay_scan_kernel<<<dim3((unsigned)rnn_div_up(all, 256), jobs), 256, 0, ctx->stream>>>(g);
+    const int blocks = (int)rnn_div_up(g.job[0].da * g.job[0].dc, 256);
+    decay_scan_kernel<<<dim3((unsigned)(g.n * g.h * blocks), jobs), 256, 0, ctx->stream>>>(g, blocks);
 }
 
 }  // namespace
