@@ -372,9 +372,9 @@ enum { WALK = 0, WALK_RATE = 1, STATE = 2 };
 // rates): one wave a SIMD takes 4.5 us a chunk of 64 x 64 heads, 65 % of their rate at
 // 2.4 GHz, two as much for each.  (Measured and not better: rows shared by a block's
 // waves through LDS with barriers, products and other instructions interleaved by
-// hand.)  8 clips of 1568 tokens, 8 heads of 64: forward 36
-// us and 23 for the states between segments, dq and the rates 67, dk and dv 64, their
-// states 34; 128 images of 64 tokens, 4 heads: 15, 21 and 22.
+// hand.)  8 clips of 1568 tokens, 8 heads of 64: forward 37 us and 23 for the states
+// between segments, dq and the rates 67, dk and dv 65, their states 35; 128 images of
+// 64 tokens, 4 heads: 15, 21 and 22.
 template <int DAT, bool FULL, int MODE>
 __global__ __launch_bounds__(256, DAT <= (MODE == WALK_RATE ? 1 : 2) ? 2 : 1) void decay_walk_kernel(DecayArgs g) {
     // rows of b: 4 rows apart are half of the banks apart
@@ -598,8 +598,8 @@ __global__ __launch_bounds__(256, DAT <= (MODE == WALK_RATE ? 1 : 2) ? 2 : 1) vo
 }
 
 // The states before each segment, in the walk's direction, from the segments' own
-// ones: one thread an element, over the segments in order.  A block's
-// elements are one head's, so that lengths and factors are the same for all of them.
+// ones: one thread an element, over the segments in order.  A block's elements are
+// one head's, so that lengths and factors are the same for all of them.
 // Bound by the chain of loads: 64 segments of 8 heads of 64 x 128 11 us (3.0 TB/s; 16
 // ahead 12.5, without the eight ahead 14), 8 of 64 of 64 x 64 6.3 (2.7).
 __global__ __launch_bounds__(256) void decay_scan_kernel(DecayArgs g, int blocks) {
