@@ -62,6 +62,8 @@ struct DecayArgs {
     const float *rate;
     const uint32_t *lens;
     double *part;  // [n][nseg][slices][h] parts of dL/dg
+    float *drate;  // their sums' place, added by `h` blocks past a launch's `walk` ones
+    int parts, walk;
     int n, t, h, reverse;
     int nseg;  // segments of a sequence
     Divider segs, heads;
@@ -356,6 +358,19 @@ __device__ __forceinline__ f32x16 tri_product(const f32x16 &p, const float (&c)[
     return o;
 }
 
+// drate[j] += g sum of the head's parts, in a fixed order, by a block among those of the
+// next walk (a launch for it took 4 us more).
+__device__ void sum_rate(const DecayArgs &g, int j) {
+    __shared__ double red[4];
+    double s = 0.0;
+    for (int i = threadIdx.x; i < g.parts; i += 256) s += g.part[(long long)i * g.h + j];
+    s = rnn_wave_sum_d(s);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0)
+        g.drate[j] += (float)(log_gamma(g.rate[j]) * (red[0] + red[1] + red[2] + red[3]));
+}
+
 enum { WALK = 0, WALK_RATE = 1, STATE = 2 };
 
 // A wave takes 32 of c's channels of a head through a segment, 32 tokens at a
@@ -387,7 +402,11 @@ __global__ __launch_bounds__(256, DAT <= (MODE == WALK_RATE ? 1 : 2) ? 2 : 1) vo
     // tokens 15.4 us against 14.9)
     asm volatile("" ::"s"(q.a), "s"(q.b), "s"(q.c), "s"(q.y), "s"(q.s0), "s"(q.as), "s"(q.bs), "s"(q.cs),
                  "s"(q.ys), "s"(q.da), "s"(q.ga), "s"(q.sa), "s"(q.rev), "s"(g.rate));
-    uint32_t u = (uint32_t)xcd_order(blockIdx.x, gridDim.x) * 4 + wave, rest;  // fewer than 2^31 waves
+    if (MODE == WALK && (int)blockIdx.x >= g.walk) {  // of the launch after the one that left the parts
+        if (blockIdx.y == 0) sum_rate(g, (int)blockIdx.x - g.walk);
+        return;
+    }
+    uint32_t u = (uint32_t)xcd_order(blockIdx.x, g.walk) * 4 + wave, rest;  // fewer than 2^31 waves
     u = q.slices(u, rest);
     const int slice = (int)rest, col = slice * 32 + ln;
     u = g.segs(u, rest);
@@ -678,20 +697,6 @@ __global__ __launch_bounds__(256) void decay_group_kernel(GroupArgs g, long long
     }
 }
 
-// drate[j] += g sum of the head's parts, in a fixed order (4 us, a launch's least).
-__global__ __launch_bounds__(256) void decay_rate_kernel(const double *part, int rows, int h,
-                                                         const float *rate, float *drate) {
-    __shared__ double red[4];
-    const int j = blockIdx.x;
-    double s = 0.0;
-    for (int i = threadIdx.x; i < rows; i += 256) s += part[(long long)i * h + j];
-    s = rnn_wave_sum_d(s);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
-    __syncthreads();
-    if (threadIdx.x == 0)
-        drate[j] += (float)(log_gamma(rate[j]) * (red[0] + red[1] + red[2] + red[3]));
-}
-
 // The form's walks over a sequence, and where a workspace's parts are.
 struct DecayPlan {
     bool tokens = false;  // token by token
@@ -808,6 +813,8 @@ void fill_args(DecayArgs &g, const rnn_decay_attn_desc *d, const DecayPlan &p, s
     g.rate = rate;
     g.lens = lens;
     g.part = nullptr;
+    g.drate = nullptr;
+    g.parts = 0;
     g.n = (int)n;
     g.t = (int)t;
     g.h = (int)d->h;
@@ -815,7 +822,7 @@ void fill_args(DecayArgs &g, const rnn_decay_attn_desc *d, const DecayPlan &p, s
 }
 
 template <int MODE>
-void launch_walk(rnn_ctx *ctx, const DecayArgs &g, int jobs) {
+void launch_walk(rnn_ctx *ctx, DecayArgs &g, int jobs) {
     size_t waves = 0;
     bool full = true;
     for (int k = 0; k < jobs; k++) {
@@ -823,7 +830,8 @@ void launch_walk(rnn_ctx *ctx, const DecayArgs &g, int jobs) {
         waves = std::max(waves, (size_t)g.n * g.h * g.nseg * q.slices.d);
         full = full && q.da % 32 == 0;
     }
-    const dim3 grid((unsigned)rnn_div_up(waves, 4), (unsigned)jobs);
+    g.walk = (int)rnn_div_up(waves, 4);
+    const dim3 grid((unsigned)(g.walk + (g.drate ? g.h : 0)), (unsigned)jobs);
     hipStream_t s = ctx->stream;
 #define WALK_AS(DAT)                                                                \
     (full ? decay_walk_kernel<DAT, true, MODE><<<grid, 256, 0, s>>>(g)              \
@@ -838,7 +846,7 @@ void launch_walk(rnn_ctx *ctx, const DecayArgs &g, int jobs) {
 }
 
 // The states between segments: every segment's own, then over the segments.
-void launch_segments(rnn_ctx *ctx, const DecayArgs &g, int jobs) {
+void launch_segments(rnn_ctx *ctx, DecayArgs &g, int jobs) {
     launch_walk<STATE>(ctx, g, jobs);
     const int blocks = (int)rnn_div_up(g.job[0].da * g.job[0].dc, 256);
     decay_scan_kernel<<<dim3((unsigned)(g.n * g.h * blocks), jobs), 256, 0, ctx->stream>>>(g, blocks);
@@ -983,12 +991,15 @@ int rnn_decay_attn_backward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n
         RNN_LAUNCHED(ctx);
         one.job[0] = jk;
         one.job[1] = jv;
+        one.drate = drate;  // dk's and dv's launch adds it
+        one.parts = (int)(n * w.nseg * rnn_div_up(d->dk, 32));
     }
     const bool joint = (kd + 31) / 32 == (vd + 31) / 32;
     launch_walk<WALK>(ctx, one, (drate ? 1 : 2) + (joint ? 1 : 0));
     RNN_LAUNCHED(ctx);
     if (!joint) {
         one.job[0] = jv;
+        one.drate = nullptr;
         launch_walk<WALK>(ctx, one, 1);
         RNN_LAUNCHED(ctx);
     }
@@ -998,11 +1009,6 @@ int rnn_decay_attn_backward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n
         const size_t each = n * t * d->hkv * (size_t)std::max(kd, vd);
         decay_group_kernel<<<dim3((unsigned)std::min<size_t>(rnn_div_up(each, 256), 4096), 2), 256, 0,
                              ctx->stream>>>(ga, (long long)(n * t));
-        RNN_LAUNCHED(ctx);
-    }
-    if (drate) {
-        decay_rate_kernel<<<(unsigned)d->h, 256, 0, ctx->stream>>>(
-            g.part, (int)(n * w.nseg * rnn_div_up(d->dk, 32)), (int)d->h, rate, drate);
         RNN_LAUNCHED(ctx);
     }
     return RNN_OK;
