@@ -35,6 +35,11 @@ CASES = [
                            state=False)),
     ("long", dict(n=1, t=1100, h=2, hkv=2, dk=32, dv=32, reverse=1)),
     ("long_ragged", dict(n=2, t=1500, h=2, hkv=1, dk=20, dv=64, reverse=1, lens=[1500, 700])),
+    ("segments_of_many_lengths", dict(n=9, t=1000, h=4, hkv=2, dk=40, dv=24, reverse=2,
+                                      lens=[1000, 999, 33, 500, 0, 31, 64, 97, 1200])),
+    ("uneven_segments", dict(n=1, t=2245, h=2, hkv=2, dk=8, dv=12, reverse=1)),
+    ("few_wide_segments", dict(n=16, t=420, h=8, hkv=4, dk=36, dv=128, reverse=4,
+                               lens=[420, 7, 300, 1] * 4)),
     ("slow_decay", dict(n=1, t=700, h=2, hkv=2, dk=32, dv=32, rates=(-30.0, -12.0))),
     ("fast_decay", dict(n=1, t=200, h=2, hkv=2, dk=32, dv=32, rates=(1.0, 6.0), reverse=1)),
 ]
