@@ -1124,6 +1124,8 @@ class DecayCore:
         unless keep_state or state_out, which may be state).  lens (int32 /
         uint32 [n]): the sequences' lengths where they are padded."""
         import torch
+        if (v is None) != (vstride is None):
+            raise ValueError("DecayCore.forward: v and vstride go together")
         ctx = self.ctx or default_ctx(max(q.get_device(), 0))
         d, nb, nq, nk, nv = self._plan(n, t, 0, (qstride, qoff, kvstride, koff,
                                                  None if v is None else vstride, voff))
@@ -1155,8 +1157,8 @@ class DecayCore:
         dstate_out: the gradient of the state that forward returned; dstate
         receives the given state's."""
         import torch
-        if (v is None) != (dv is None):
-            raise ValueError("DecayCore.backward: v and dv go together")
+        if not (v is None) == (vstride is None) == (dv is None):
+            raise ValueError("DecayCore.backward: v, vstride and dv go together")
         ctx = self.ctx or default_ctx(max(dy.get_device(), 0))
         d, nb, nq, nk, nv = self._plan(n, t, 1, (qstride, qoff, kvstride, koff,
                                                  None if v is None else vstride, voff))

@@ -91,6 +91,17 @@ def test_decay_description_is_checked():
     assert R.lib().rnn_decay_attn_workspace(None, 1, 1, 0, C.byref(nb)) == R.RNN_E_NULL
 
 
+def test_decay_values_apart_need_their_stride():
+    core, x = R.DecayCore(1, 4), torch.zeros(1, 1, 12)
+    geo = (x, 12, 0, x, 12, 4, 8)
+    for kw in (dict(v=x), dict(vstride=12)):
+        with pytest.raises(ValueError):
+            core.forward(1, 1, *geo, x, **kw)
+    for kw in (dict(v=x), dict(vstride=12), dict(dv=x), dict(v=x, dv=x), dict(v=x, vstride=12)):
+        with pytest.raises(ValueError):
+            core.backward(1, 1, *geo, x, x, x, x, **kw)
+
+
 @pytest.mark.parametrize("kw", [dict(h=0), dict(d=0), dict(h=-1), dict(d=513), dict(h=65537),
                                 dict(eps=0.0), dict(eps=math.nan), dict(eps=math.inf)])
 def test_head_gate_refuses(kw):
