@@ -1009,10 +1009,9 @@ class NormRotary:
         return d, nb
 
     def _out(self, like, n, t, y, ystride, yoff, xstride, xoff):
-        import torch
         if y is None:
             w = self.heads * self.dh
-            return torch.empty(n, t, w, dtype=torch.float32, device=like.device), w, 0
+            return like.new_empty(n, t, w), w, 0
         return (y, xstride, xoff) if ystride is None else (y, ystride, yoff)
 
     def forward(self, n, x, xstride, xoff=0, gain=None, pos=None, y=None, ystride=None, yoff=0,
@@ -1042,7 +1041,6 @@ class NormRotary:
                  dx=None, dxstride=None, dxoff=0, t=None):
         """dx (returned) from the forward's input x and dy; dx given: at dy's
         layout unless dxstride is (dy: in place).  dgain [2, dh] accumulates."""
-        import torch
         ctx, w = self.ctx or default_ctx(max(x.get_device(), 0)), self.heads * self.dh
         t = self.t if t is None else int(t)
         dx, dxstride, dxoff = self._out(x, n, t, dx, dxstride, dxoff, dystride, dyoff)
@@ -1050,7 +1048,7 @@ class NormRotary:
         rows = n * t
         need = lambda stride, off: (rows - 1) * stride + off + w if rows else 0
         nb = nb if dgain is not None else 0
-        ws = torch.empty(nb, dtype=torch.uint8, device=x.device) if nb else None
+        ws = x.new_empty(-(-nb // 4)) if nb else None
         args = (_arg(ctx, x, need(xstride, xoff), "x"), _arg(ctx, gain, 2 * self.dh, "gain"),
                 _arg(ctx, pos, rows * len(self.rot.grid), "pos"),
                 _arg(ctx, dy, need(dystride, dyoff), "dy"), dystride, dyoff,
@@ -1123,7 +1121,6 @@ class DecayCore:
         """(y [n, t, h dv], the state after the last token [n, h, dk, dv]: None
         unless keep_state or state_out, which may be state).  lens (int32 /
         uint32 [n]): the sequences' lengths where they are padded."""
-        import torch
         if (v is None) != (vstride is None):
             raise ValueError("DecayCore.forward: v and vstride go together")
         ctx = self.ctx or default_ctx(max(q.get_device(), 0))
@@ -1135,11 +1132,10 @@ class DecayCore:
                _arg(ctx, rate, self.h, "rate"), _arg(ctx, lens, n, "lens", "u32"),
                _arg(ctx, state, st, "state"))
         if y is None:
-            y = torch.empty(n, t, self.c, dtype=torch.float32, device=q.device)
+            y = q.new_empty(n, t, self.c)
         if state_out is None and keep_state:
-            state_out = torch.empty(n, self.h, self.dk, self.dv, dtype=torch.float32,
-                                    device=q.device)
-        ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None
+            state_out = q.new_empty(n, self.h, self.dk, self.dv)
+        ws = q.new_empty(-(-nb // 4)) if nb else None
         outs = _arg(ctx, y, n * t * self.c, "y"), _arg(ctx, state_out, st, "state_out")
         on = _OnStream(ctx)
         try:
@@ -1156,7 +1152,6 @@ class DecayCore:
         given) and drate; set_dq / set_dkv overwrite dq / dkv and dv instead.
         dstate_out: the gradient of the state that forward returned; dstate
         receives the given state's."""
-        import torch
         if not (v is None) == (vstride is None) == (dv is None):
             raise ValueError("DecayCore.backward: v, vstride and dv go together")
         ctx = self.ctx or default_ctx(max(dy.get_device(), 0))
@@ -1168,7 +1163,7 @@ class DecayCore:
                _arg(ctx, rate, self.h, "rate"), _arg(ctx, lens, n, "lens", "u32"),
                _arg(ctx, state, st, "state"), _arg(ctx, dy, n * t * self.c, "dy"),
                _arg(ctx, dstate_out, st, "dstate_out"))
-        ws = torch.empty(nb, dtype=torch.uint8, device=dy.device) if nb else None
+        ws = dy.new_empty(-(-nb // 4)) if nb else None
         flags = (RNN_ATTN_SET_DQ if set_dq else 0) | (RNN_ATTN_SET_DKV if set_dkv else 0)
         outs = (_arg(ctx, dq, nq, "dq"), dkp, dkp if v is None else _arg(ctx, dv, nv, "dv"),
                 _arg(ctx, drate, self.h, "drate"), _arg(ctx, dstate, st, "dstate"))
@@ -1213,11 +1208,10 @@ class HeadGate:
 
     def forward(self, rows, x, z, zstride, zoff=0, gain=None, y=None):
         """y (returned; x: in place, which a backward cannot follow)."""
-        import torch
         ctx = self.ctx or default_ctx(max(x.get_device(), 0))
         self._bytes(rows)
         if y is None:
-            y = torch.empty(rows, self.c, dtype=torch.float32, device=x.device)
+            y = x.new_empty(rows, self.c)
         args = (_arg(ctx, x, rows * self.c, "x"), _arg(ctx, z, self._need(rows, zstride, zoff), "z"),
                 zstride, zoff, _arg(ctx, gain, self.c, "gain"), _arg(ctx, y, rows * self.c, "y"))
         on = _OnStream(ctx)
@@ -1231,12 +1225,11 @@ class HeadGate:
                  dx=None):
         """dx (returned) and dz, in rows of dzstride floats from dzoff on, are
         overwritten; dgain [h d] accumulates."""
-        import torch
         ctx = self.ctx or default_ctx(max(x.get_device(), 0))
         nb = self._bytes(rows) if dgain is not None else 0
         if dx is None:
-            dx = torch.empty(rows, self.c, dtype=torch.float32, device=x.device)
-        ws = torch.empty(nb, dtype=torch.uint8, device=x.device) if nb else None
+            dx = x.new_empty(rows, self.c)
+        ws = x.new_empty(-(-nb // 4)) if nb else None
         args = (_arg(ctx, x, rows * self.c, "x"), _arg(ctx, z, self._need(rows, zstride, zoff), "z"),
                 zstride, zoff, _arg(ctx, gain, self.c, "gain"), _arg(ctx, dy, rows * self.c, "dy"),
                 ws.data_ptr() if nb else None, nb, _arg(ctx, dx, rows * self.c, "dx"),
