@@ -562,6 +562,8 @@ __global__ __launch_bounds__(256, DAT <= (MODE == WALK_RATE ? 1 : 2) ? 2 : 1) vo
             }
         }
         if (goes) {
+            // b's rows in LDS, which other lanes have written
+            if (MODE != STATE) wave_sync();
             float left[16];
             places(pw.left, half, left);
 #pragma unroll
