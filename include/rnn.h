@@ -339,7 +339,8 @@ typedef struct {
  * n * h * dk * dv < 2^31 (RNN_E_UNSUPPORTED above), scale finite. */
 int rnn_decay_attn_workspace(const rnn_decay_attn_desc *d, size_t n, size_t t, int backward,
                              size_t *bytes);
-/* y [n][t][h][dv], which overlaps no operand. */
+/* y [n][t][h][dv] and state_out, which overlap no other operand (but state_out may
+ * be state_in), else RNN_E_INVALID. */
 int rnn_decay_attn_forward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n, size_t t,
                            const float *q, const float *k, const float *v, const float *rate,
                            const uint32_t *lens, const float *state_in, void *ws, size_t ws_bytes,
@@ -349,8 +350,8 @@ int rnn_decay_attn_forward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n,
  * are overwritten as flags say (RNN_ATTN_SET_DQ, RNN_ATTN_SET_DKV: the columns of the
  * heads, padding rows included, which receive 0); drate [h] (NULL: not wanted)
  * accumulates; dstate_in (NULL: not wanted) is overwritten.  dq, dk and dv may be one
- * buffer with disjoint columns; neither they nor dstate_in overlap another operand.
- * Sums run in a fixed order. */
+ * buffer with disjoint columns; but for that, no gradient overlaps another one or
+ * another operand, else RNN_E_INVALID.  Sums run in a fixed order. */
 int rnn_decay_attn_backward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n, size_t t,
                             const float *q, const float *k, const float *v, const float *rate,
                             const uint32_t *lens, const float *state_in, const float *dy,

@@ -14,6 +14,7 @@
 // Z_i = gamma (Z_(i-1) + S_(i-1)), dL/dg = scale sum q_i . (Z^T-weighted sum of k),
 // that is, dq's form with each term times i - l, dotted with q; and <Z_last, R^>.
 #include "mfma_half.h"
+#include "rnn_overlap.h"
 
 #include <algorithm>
 #include <cmath>
@@ -785,6 +786,25 @@ int check_ws(rnn_ctx *ctx, const DecayPlan &w, const void *ws, size_t bytes) {
     return RNN_OK;
 }
 
+// A call's operands as they lie in memory.
+struct Layout {
+    const rnn_decay_attn_desc *d;
+    size_t n, rows;
+    RnnRows q(const float *p) const {
+        return {p ? p + d->qoff : p, rows, d->qstride, (size_t)d->h * d->dk};
+    }
+    RnnRows k(const float *p) const {
+        return {p ? p + d->koff : p, rows, d->kstride, (size_t)d->hkv * d->dk};
+    }
+    RnnRows v(const float *p) const {
+        return {p ? p + d->voff : p, rows, d->vstride, (size_t)d->hkv * d->dv};
+    }
+    RnnRows y(const float *p) const { return rnn_block(p, rows * d->h * d->dv); }
+    RnnRows rates(const float *p) const { return rnn_block(p, d->h); }
+    RnnRows lens(const uint32_t *p) const { return rnn_block(p, n); }
+    RnnRows states(const float *p) const { return rnn_block(p, n * d->h * d->dk * d->dv); }
+};
+
 // One of the form's operands: where its rows are, and how many query heads share
 // one of its heads.
 struct Operand {
@@ -880,8 +900,13 @@ int rnn_decay_attn_forward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n,
     if (rc) return rc;
     if (!n || (!t && !state_out)) return RNN_OK;
     if ((t && (!q || !k || !v || !y)) || !rate) return rnn_fail(ctx, RNN_E_NULL, "decay_attn_forward: null operand");
-    if (t && (y == q + d->qoff || y == k + d->koff || y == v + d->voff))
-        return rnn_fail(ctx, RNN_E_INVALID, "decay_attn_forward: y is an operand");
+    const Layout at = {d, n, n * t};
+    // the states may be handed on in place
+    const RnnRows ins[] = {at.q(q), at.k(k), at.v(v), at.rates(rate), at.lens(lens),
+                           at.states(state_in == state_out ? nullptr : state_in)};
+    const RnnRows outs[] = {at.y(y), at.states(state_out)};
+    if (rnn_any_overlap(outs, ins))
+        return rnn_fail(ctx, RNN_E_INVALID, "decay_attn_forward: a result over another operand");
     const DecayPlan w = plan_of(d, n, t, false);
     rc = check_ws(ctx, w, ws, ws_bytes);
     if (rc) return rc;
@@ -936,11 +961,12 @@ int rnn_decay_attn_backward(rnn_ctx *ctx, const rnn_decay_attn_desc *d, size_t n
     if (!n || (!t && !dstate_in)) return RNN_OK;
     if ((t && (!q || !k || !v || !dy || !dq || !dk || !dv)) || !rate)
         return rnn_fail(ctx, RNN_E_NULL, "decay_attn_backward: null operand");
-    if (dstate_in && (dstate_in == dstate_out || dstate_in == state_in))
-        return rnn_fail(ctx, RNN_E_INVALID, "decay_attn_backward: dstate_in is an operand");
-    if (t && (dq == q || dk == k || dv == v || dq + d->qoff == dy || dk + d->koff == dy ||
-              dv + d->voff == dy))
-        return rnn_fail(ctx, RNN_E_INVALID, "decay_attn_backward: a gradient is an operand");
+    const Layout at = {d, n, n * t};
+    const RnnRows ins[] = {at.q(q), at.k(k), at.v(v), at.rates(rate), at.lens(lens),
+                           at.states(state_in), at.y(dy), at.states(dstate_out)};
+    const RnnRows outs[] = {at.q(dq), at.k(dk), at.v(dv), at.rates(drate), at.states(dstate_in)};
+    if (rnn_any_overlap(outs, ins))
+        return rnn_fail(ctx, RNN_E_INVALID, "decay_attn_backward: a gradient over another operand");
     const DecayPlan w = plan_of(d, n, t, true);
     rc = check_ws(ctx, w, ws, ws_bytes);
     if (rc) return rc;
