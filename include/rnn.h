@@ -270,7 +270,8 @@ int rnn_rotary(rnn_ctx *ctx, const rnn_rotary_desc *d, size_t n, size_t t, const
  * not turned.  dh <= 256 (RNN_E_UNSUPPORTED above), eps > 0.  Squares are summed in
  * 64 bits, so that heads of any size keep their norm.  A NaN gives NaN in its
  * head, an infinity in its channel's pair and zeros in the others of its head.
- * y may be x when strides and offsets agree, else the two must not overlap. */
+ * y may be x when strides and offsets agree; else it overlaps no operand, though the
+ * two may be columns of one buffer (RNN_E_INVALID otherwise). */
 int rnn_norm_rotary_forward(rnn_ctx *ctx, const rnn_rotary_desc *d, uint32_t hq, float eps, size_t n,
                             size_t t, const float *x, const float *gain, const float *pos, float *y);
 /* Checks the arguments and gives the bytes of device workspace that a backward
@@ -282,7 +283,7 @@ int rnn_norm_rotary_workspace(const rnn_rotary_desc *d, uint32_t hq, float eps, 
 /* From the forward's input x and dy (rows of dystride floats, heads from dyoff on):
  * dx, laid out as y, is overwritten; dgain [2][dh] (NULL: not wanted) accumulates,
  * in a fixed order.  dx may be dy when their layouts agree and overlaps nothing
- * else. */
+ * else (RNN_E_INVALID). */
 int rnn_norm_rotary_backward(rnn_ctx *ctx, const rnn_rotary_desc *d, uint32_t hq, float eps, size_t n,
                              size_t t, const float *x, const float *gain, const float *pos,
                              const float *dy, size_t dystride, size_t dyoff, void *ws, size_t ws_bytes,
@@ -292,9 +293,9 @@ int rnn_norm_rotary_backward(rnn_ctx *ctx, const rnn_rotary_desc *d, uint32_t hq
  * of h heads of d channels, x and y [rows][h][d], z at z + r*zstride + zoff.
  *   y = gain x / sqrt(mean(x^2) + eps) z / (1 + exp(-z))
  * gain [h][d] (NULL: 1); the mean is a head's.  d <= 512, h <= 65536, eps > 0.  y
- * may be x and overlaps nothing else.  A NaN in x gives NaN in its head, an infinity
- * NaN in its channel and zeros in the others of its head; either in z stays in its
- * channel. */
+ * may be x and overlaps nothing else (RNN_E_INVALID).  A NaN in x gives NaN in its
+ * head, an infinity NaN in its channel and zeros in the others of its head; either
+ * in z stays in its channel. */
 int rnn_head_gate_forward(rnn_ctx *ctx, size_t rows, size_t h, size_t d, float eps, const float *x,
                           const float *z, size_t zstride, size_t zoff, const float *gain, float *y);
 /* Bytes of device workspace that a backward with dgain needs, as
@@ -302,7 +303,8 @@ int rnn_head_gate_forward(rnn_ctx *ctx, size_t rows, size_t h, size_t d, float e
 int rnn_head_gate_workspace(size_t rows, size_t h, size_t d, size_t *bytes);
 /* Its backward: dx [rows][h][d] and dz (at dz + r*dzstride + dzoff) are
  * overwritten, dgain [h][d] (NULL: not wanted) accumulates in a fixed order.  dx
- * may be dy or x, dz may be z where their layouts agree; they overlap nothing else. */
+ * may be dy or x, dz may be z where their layouts agree; they overlap nothing else
+ * (RNN_E_INVALID, as for dz and z given as one buffer of two layouts). */
 int rnn_head_gate_backward(rnn_ctx *ctx, size_t rows, size_t h, size_t d, float eps, const float *x,
                            const float *z, size_t zstride, size_t zoff, const float *gain,
                            const float *dy, void *ws, size_t ws_bytes, float *dx, float *dz,

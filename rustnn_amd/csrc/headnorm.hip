@@ -16,6 +16,7 @@
 // of 64 channels 58 us forward (5.3 TB/s) and 104 us backward (4.5), 8 gated heads
 // of 64 channels 26 us (6.0: they stay in the last cache) and 48 (5.3), each
 // backward 5 us more for the gains' gradient.  64 rows take 6 us, a launch's least.
+#include "rnn_overlap.h"
 #include "rotary_angle.h"
 
 #include <algorithm>
@@ -555,8 +556,13 @@ int rnn_norm_rotary_forward(rnn_ctx *ctx, const rnn_rotary_desc *d, uint32_t hq,
     if (rc) return rc;
     if (!(n * t)) return RNN_OK;
     if (!x || !y) return rnn_fail(ctx, RNN_E_NULL, "norm_rotary: null operand");
-    if (x == y && (d->xstride != d->ystride || d->xoff != d->yoff))
-        return rnn_fail(ctx, RNN_E_INVALID, "norm_rotary: in place with two layouts");
+    const size_t width = (size_t)d->h * d->dh;
+    const bool in_place = x + d->xoff == y + d->yoff && d->xstride == d->ystride;
+    const RnnRows ins[] = {{in_place ? nullptr : x + d->xoff, n * t, d->xstride, width},
+                           rnn_block(gain, 2 * (size_t)d->dh),
+                           rnn_block(pos, n * t * d->axes)};
+    const RnnRows outs[] = {{y + d->yoff, n * t, d->ystride, width}};
+    if (rnn_any_overlap(outs, ins)) return rnn_fail(ctx, RNN_E_INVALID, "norm_rotary: y over an operand");
     RNN_ON_DEVICE(ctx);
     NrArgs g;
     nr_fill(g, d, hq, eps, n, t, x, gain, pos, y);
@@ -583,9 +589,15 @@ int rnn_norm_rotary_backward(rnn_ctx *ctx, const rnn_rotary_desc *d, uint32_t hq
     if (!(n * t)) return RNN_OK;
     if (!x || !dy || !dx) return rnn_fail(ctx, RNN_E_NULL, "norm_rotary: null operand");
     if (!gain && dgain) return rnn_fail(ctx, RNN_E_NULL, "norm_rotary: dgain without gain");
-    if (dx == x) return rnn_fail(ctx, RNN_E_INVALID, "norm_rotary: dx is x");
-    if (dx == dy && (d->ystride != dystride || d->yoff != dyoff))
-        return rnn_fail(ctx, RNN_E_INVALID, "norm_rotary: in place with two layouts");
+    const bool in_place = dx + d->yoff == dy + dyoff && d->ystride == dystride;
+    const RnnRows ins[] = {{x + d->xoff, n * t, d->xstride, width},
+                           {in_place ? nullptr : dy + dyoff, n * t, dystride, width},
+                           rnn_block(gain, 2 * (size_t)d->dh),
+                           rnn_block(pos, n * t * d->axes),
+                           rnn_block(dgain, 2 * (size_t)d->dh)};
+    const RnnRows outs[] = {{dx + d->yoff, n * t, d->ystride, width}};
+    if (rnn_any_overlap(outs, ins))
+        return rnn_fail(ctx, RNN_E_INVALID, "norm_rotary: dx over another operand");
     const NrPlan p = nr_plan(d, n * t, MAX_PARTS);
     rc = ws_checked(ctx, "norm_rotary", dgain ? (size_t)p.blocks * 2 * d->dh * sizeof(double) : 0, ws,
                     ws_bytes);
@@ -626,7 +638,12 @@ int rnn_head_gate_forward(rnn_ctx *ctx, size_t rows, size_t h, size_t d, float e
     if (rc) return rc;
     if (!rows) return RNN_OK;
     if (!x || !z || !y) return rnn_fail(ctx, RNN_E_NULL, "head_gate: null operand");
-    if (y == z + zoff) return rnn_fail(ctx, RNN_E_INVALID, "head_gate: y is the gate");
+    const RnnRows ins[] = {rnn_block(y == x ? nullptr : x, rows * h * d),
+                           {z + zoff, rows, zstride, h * d},
+                           rnn_block(gain, h * d)};
+    const RnnRows outs[] = {rnn_block(y, rows * h * d)};
+    if (rnn_any_overlap(outs, ins))
+        return rnn_fail(ctx, RNN_E_INVALID, "head_gate: y over another operand");
     RNN_ON_DEVICE(ctx);
     const GatePlan p = gate_plan(rows, h, d);
     GateArgs g = {x, z + zoff, gain, nullptr, y, nullptr, nullptr, (long long)zstride, 0, (long long)rows,
@@ -651,8 +668,16 @@ int rnn_head_gate_backward(rnn_ctx *ctx, size_t rows, size_t h, size_t d, float 
     if (!gain && dgain) return rnn_fail(ctx, RNN_E_NULL, "head_gate: dgain without gain");
     if (dz == z && (dzstride != zstride || dzoff != zoff))
         return rnn_fail(ctx, RNN_E_INVALID, "head_gate: in place with two layouts");
-    if (dx == z + zoff || dx == dz + dzoff || dz + dzoff == x || dz + dzoff == dy)
-        return rnn_fail(ctx, RNN_E_INVALID, "head_gate: a gradient is another operand");
+    const bool over_z = dz + dzoff == z + zoff && dzstride == zstride;
+    // what dx or dz may take the place of is met by the other one as dx or dz
+    const RnnRows ins[] = {rnn_block(dx == x ? nullptr : x, rows * h * d),
+                           rnn_block(dx == dy ? nullptr : dy, rows * h * d),
+                           {over_z ? nullptr : z + zoff, rows, zstride, h * d},
+                           rnn_block(gain, h * d),
+                           rnn_block(dgain, h * d)};
+    const RnnRows outs[] = {rnn_block(dx, rows * h * d), {dz + dzoff, rows, dzstride, h * d}};
+    if (rnn_any_overlap(outs, ins))
+        return rnn_fail(ctx, RNN_E_INVALID, "head_gate: a gradient over another operand");
     const GatePlan p = gate_plan(rows, h, d);
     rc = ws_checked(ctx, "head_gate", dgain ? p.parts * h * d * sizeof(double) : 0, ws, ws_bytes);
     if (rc) return rc;
