@@ -47,18 +47,27 @@ __device__ __forceinline__ double inv_sqrt(double v) {
     return r == 0.0 ? r : s;
 }
 
-// 1 / (1 + exp(-z)), within 6.5 U (U = 2^-24).  exp(-z) as a power of two, its exponent
-// in two parts, so that far gates lose nothing: the instruction's 2 U and two
-// products; the sum's U; its reciprocal by the instruction (2 U) and a Newton step
-// on it: 1.5 U.  Below -88 it is 0.
-__device__ __forceinline__ float sigmoid(float z) {
-    z = fminf(fmaxf(z, -104.f), 104.f);
-    const float t = z * -1.44269504f;
-    const float lo = __builtin_fmaf(z, -1.44269504f, -t) + z * -1.92596299e-8f;
-    const float e = __builtin_amdgcn_exp2f(t) * __builtin_fmaf(lo, 0.69314718f, 1.f);
-    const float d = 1.f + e, r = __builtin_amdgcn_rcpf(d);
-    return d < 0x1p126f ? __builtin_fmaf(r, __builtin_fmaf(-d, r, 1.f), r) : 0.f;
-}
+// sigma(z) = 1 / (1 + exp(-z)) = s down, s within 6.5 U (U = 2^-24).  exp(-z) as a power
+// of two, its exponent in two parts, so that far gates lose nothing: the
+// instruction's 2 U and two products; the sum's U; its reciprocal by the instruction
+// (2 U) and a Newton step on it: 1.5 U.  From exp(-z) = 2^100 on (z = -69) all of it is
+// taken 2^64 smaller, down = 2^-64, so that the reciprocal, which gives 0 for what is
+// below the normal range, stays in it: z sigma, a normal number down to z = -91, is right
+// to its last bit below that.  `down` is multiplied last; s z and s alone are below
+// 1 where it is not 1.  From -120 on z sigma is below half of the least number: s = 0.
+struct Sigma {
+    float s, down;
+    __device__ __forceinline__ explicit Sigma(float z) {
+        const float c = __builtin_amdgcn_fmed3f(z, -120.f, 104.f);
+        const float t = c * -1.44269504f;
+        const float lo = __builtin_fmaf(c, -1.44269504f, -t) + c * -1.92596299e-8f;
+        const bool far = t > 100.f;
+        down = far ? 0x1p-64f : 1.f;
+        const float e = __builtin_amdgcn_exp2f(far ? t - 64.f : t) * __builtin_fmaf(lo, 0.69314718f, 1.f);
+        const float d = down + e, r = __builtin_amdgcn_rcpf(d);
+        s = z < -120.f ? 0.f : __builtin_fmaf(r, __builtin_fmaf(-d, r, 1.f), r);
+    }
+};
 
 // x^ in 32 bits whatever the head's size: 1 / norm as a float of [1, 2) times a
 // power of two, which the channels take first.
@@ -370,17 +379,20 @@ __global__ __launch_bounds__(256) void head_gate_kernel(GateArgs g) {
         float o[8];
         if constexpr (!BACK) {
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-                o[e] = (float)(v[e] * rn) * gain[e] * (z[e] * sigmoid(z[e]));
+            for (int e = 0; e < 8; e++) {
+                const Sigma sg(z[e]);
+                o[e] = (float)(v[e] * rn) * gain[e] * (z[e] * sg.s) * sg.down;
+            }
         } else {
             const Norm32 hat32(rn);
             float dz[8], hat[8], m32 = 0.f;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float sig = sigmoid(z[e]);
+                const Sigma sg(z[e]);
+                const float f = 1.f + z[e] * __builtin_fmaf(-sg.s, sg.down, 1.f);
                 hat[e] = hat32(v[e]);
-                dz[e] = d[e] * (hat[e] * gain[e]) * (sig * (1.f + z[e] * (1.f - sig)));
-                o[e] = d[e] * (z[e] * sig);
+                dz[e] = d[e] * (hat[e] * gain[e]) * (sg.s * f) * sg.down;
+                o[e] = d[e] * (z[e] * sg.s) * sg.down;
                 if (live) acc[e] = fma((double)o[e], (double)hat[e], acc[e]);
                 o[e] *= gain[e];
                 m32 = __builtin_fmaf(o[e], hat[e], m32);
