@@ -295,7 +295,7 @@ int rnn_norm_rotary_backward(rnn_ctx *ctx, const rnn_rotary_desc *d, uint32_t hq
  * gain [h][d] (NULL: 1); the mean is a head's.  d <= 512, h <= 65536, eps > 0.  y
  * may be x and overlaps nothing else (RNN_E_INVALID).  A NaN in x gives NaN in its
  * head, an infinity NaN in its channel and zeros in the others of its head; either
- * in z stays in its channel. */
+ * in z stays in its channel.  z / (1 + exp(-z)) is 0 below z = -120. */
 int rnn_head_gate_forward(rnn_ctx *ctx, size_t rows, size_t h, size_t d, float eps, const float *x,
                           const float *z, size_t zstride, size_t zoff, const float *gain, float *y);
 /* Bytes of device workspace that a backward with dgain needs, as

@@ -389,8 +389,11 @@ enum { WALK = 0, WALK_RATE = 1, STATE = 2 };
 // 2.4 GHz, two as much for each.  (Measured and not better: rows shared by a block's
 // waves through LDS with barriers, products and other instructions interleaved by
 // hand.)  8 clips of 1568 tokens, 8 heads of 64: forward 37 us and 23 for the states
-// between segments, dq and the rates 67, dk and dv 65, their states 35; 128 images of
-// 64 tokens, 4 heads: 15, 21 and 22.
+// between segments, dq and the rates 67, dk and dv 64, their states 34; 128 images of
+// 64 tokens, 4 heads: 15, 21 and 23.  Four tiles with the rates do not fit the
+// registers, 66 or 68 of which go through scratch: 8 x 1568 tokens unpadded, 4 heads of
+// 128 x 128 173 us, where the products come to 135 by those of 8 heads of 64 x 64 (74);
+// three tiles fit but for one register at most (4 heads of 96 x 96: 78).
 template <int DAT, bool FULL, int MODE>
 __global__ __launch_bounds__(256, DAT <= (MODE == WALK_RATE ? 1 : 2) ? 2 : 1) void decay_walk_kernel(DecayArgs g) {
     // rows of b: 4 rows apart are half of the banks apart
@@ -713,7 +716,8 @@ struct DecayPlan {
 // 64 channels, us without / with them: one image of 64 tokens 12 / 16 forward and 31 /
 // 41 backward, of 128 tokens 21 / 17 and 56 / 42; 64 sequences of 256 tokens 42 / 47 and
 // 112 / 125, of 2048 tokens 320 / 230 and 821 / 661; 8 of 1024 tokens 149 / 31 and 407 /
-// 81 (half and twice as many segments: 40, 36 and 94, 104).
+// 81 (half and twice as many segments: 40, 36 and 94, 104).  Other heads' sizes have not
+// been timed with and without; they do not enter.
 size_t segments(size_t waves, size_t chunks, bool two, bool backward) {
     size_t k = SIMDS / waves;
     if (k < 2 || chunks < 2) return 1;  // 800 waves, 32 chunks: 106 us, in two 128
@@ -728,7 +732,8 @@ DecayPlan plan_of(const rnn_decay_attn_desc *d, size_t n, size_t t, bool backwar
     WsCarve c;
     // Few tokens: the state's read and write are all there is to do.  (Us with 1, 4, 8
     // and 12 tokens, by the walk: 64 streams of 8 heads of 64 x 128 17, 17, 18, 18, one of
-    // 4 heads of 64 x 64 9 throughout; token by token 9, 12, 17, 22 and 4, 7, 10, 13.)
+    // 4 heads of 64 x 64 9 throughout; token by token 9, 12, 17, 22 and 4, 7, 10, 13: the
+    // one stream's limit lies at 7, the many streams' at 9.)
     p.tokens = !backward && t <= 8;
     const size_t kt = rnn_div_up(d->dk, 32), vt = rnn_div_up(d->dv, 32);
     // the waves of the walk with the fewest

@@ -14,7 +14,7 @@
 //
 // 25088 rows, where a copy of that size runs at 5.0 TB/s: norm and turn of 24 heads
 // of 64 channels 58 us forward (5.3 TB/s) and 104 us backward (4.5), 8 gated heads
-// of 64 channels 26 us (6.0: they stay in the last cache) and 48 (5.3), each
+// of 64 channels 26 us (5.8: they stay in the last cache) and 48 (5.3), each
 // backward 5 us more for the gains' gradient.  64 rows take 6 us, a launch's least.
 #include "rnn_overlap.h"
 #include "rotary_angle.h"
@@ -41,7 +41,7 @@ __device__ __forceinline__ double group_sum(double v, int L) {
 }
 
 // 1 / sqrt(v): the instruction's approximation, within 2^-23, and a Newton step on
-// it, which leaves 3/8 of its square: below 2^-46.  0 of infinity.
+// it, which leaves 3/2 of its square: 1.5 2^-46.  0 of infinity.
 __device__ __forceinline__ double inv_sqrt(double v) {
     const double r = __builtin_amdgcn_rsq(v), s = fma(0.5 * r, fma(-v * r, r, 1.0), r);
     return r == 0.0 ? r : s;
@@ -201,6 +201,8 @@ struct NrLane {
 // into LDS, formed once for all heads while the first heads' loads are in flight, then
 // every head.  Four blocks of a forward a CU: for five the loads ahead do not fit the
 // registers (25088 rows 64 us against 58, 8177 rows of 52 channels 18 against 12).
+// Queries and then keys go over the lane groups in rounds, whose last ones may be
+// partly empty: 8 rows of 6 + 2 heads on 32 groups take three for the work of two.
 template <bool INTER, bool BACK>
 __global__ __launch_bounds__(256, BACK ? 3 : 4) void norm_rotary_kernel(NrArgs g) {
     __shared__ __attribute__((aligned(16))) float2 tab[TABLE];

@@ -181,7 +181,9 @@ class DecaySelfAttn:
     -> NormRotary on the queries and keys -> DecayCore of h heads, the last
     ``reverse`` of them (default: half) from the last token to the first ->
     HeadGate by z -> proj Linear::scaled.  grid as DiffSelfAttn's.  The heads of
-    a direction begin with memories of 2 tokens up to all of them."""
+    a direction begin with memories of 2 tokens up to all of them.  It takes whole
+    grids, without lengths or states: a sequence served in pieces calls the three
+    operators itself, with positions and states of its own."""
 
     def __init__(self, c, h, grid, depth, rng=None, device=0, ctx=None, reverse=None, base=100.0):
         import torch
